@@ -1,0 +1,389 @@
+// Attention over packed sequences (dg_attention_packed) and over a few tokens per cached
+// row (dg_attention_tree): the entry points, the host-side plan of packed tiles, the join
+// of split rows, and the kernel that takes any shape and type.  head_dim 16, 32, 64 and
+// 128 in 16-bit types and fp32 run on the matrix cores (dg_attn_seq_mfma.hip).
+//
+// The kernel here: a wavefront takes one (query, head) row at a time.  Its 64 lanes are
+// 64 / LPK groups of LPK lanes; a group takes every (64 / LPK)-th key of the range, lane d
+// of it the elements d, d + LPK, ... of the key and of the value (consecutive lanes read
+// consecutive elements at any alignment).  Every group keeps a running maximum, sum and
+// output of its own, in fp32 (fp64 for fp64 data); the groups meet once, at the end.  A
+// hidden key is skipped outright, so nothing it holds can reach a row.  Bound by the
+// vector ALU's cross-lane sums: log2(LPK) exchanges for every key and row.
+#include "dg_seq.h"
+
+#include <algorithm>
+#include <cmath>
+#include <numeric>
+#include <vector>
+
+namespace dg {
+
+// arithmetic of a row: fp32 in log2 units, fp64 in natural ones (no fp64 exp2 needed)
+template <typename T>
+struct SeqAcc {
+  using type = float;
+  static __device__ __forceinline__ float load(T x) { return to_f32(x); }
+  static __device__ __forceinline__ float unit_scale(const SeqArgs& a) { return a.scale_log2; }
+  static __device__ __forceinline__ float exp(float x) { return __builtin_amdgcn_exp2f(x); }
+  static __device__ __forceinline__ T store(float x) { return from_f32<T>(x); }
+};
+template <>
+struct SeqAcc<double> {
+  using type = double;
+  static __device__ __forceinline__ double load(double x) { return x; }
+  static __device__ __forceinline__ double unit_scale(const SeqArgs& a) {
+    // an fp32 rounding of 1/sqrt(D) stands for 1/sqrt(D) itself, as in dg_attention
+    const double root = 1.0 / sqrt((double)a.D);
+    return a.scale == (float)root ? root : (double)a.scale;
+  }
+  static __device__ __forceinline__ double exp(double x) { return ::exp(x); }
+  static __device__ __forceinline__ double store(double x) { return x; }
+};
+
+template <typename A>
+__device__ __forceinline__ A neg_inf() {
+  return -(A)__builtin_huge_valf();
+}
+
+// The state of a softmax row, joined with another's: (m, l) <- both, and the factors of
+// the two outputs.  -inf stands for "no key yet", whose factor is 0.
+template <typename S, typename A>
+__device__ __forceinline__ void join_softmax(A& m, A& l, A m2, A l2, A& f1, A& f2) {
+  const A mn = m > m2 ? m : m2;
+  f1 = m == neg_inf<A>() ? (A)0 : S::exp(m - mn);
+  f2 = m2 == neg_inf<A>() ? (A)0 : S::exp(m2 - mn);
+  l = l * f1 + l2 * f2;
+  m = mn;
+}
+
+template <typename T, int LPK, int CPL, bool TREE>
+__global__ __launch_bounds__(256) void seq_vec_kernel(const SeqArgs a) {
+  using S = SeqAcc<T>;
+  using A = typename S::type;
+  constexpr int KPW = 64 / LPK;
+  SeqPiece p;
+  if (!seq_piece<TREE>(a, p)) return;
+  const int lane = threadIdx.x & 63, kl = lane / LPK, dl = lane % LPK;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T* kp = static_cast<const T*>(a.k) + p.b * a.kb + p.k0 * a.kt + (int64_t)p.kvh * a.kh;
+  const T* vp = static_cast<const T*>(a.v) + p.b * a.vb + p.k0 * a.vt + (int64_t)p.kvh * a.vh;
+  const A us = S::unit_scale(a);
+  for (int r = p.row0 + wv; r < p.row0 + p.rows; r += 4) {
+    const int i = r / a.G, h = p.kvh * a.G + r % a.G;
+    const T* qp = static_cast<const T*>(a.q) + p.b * a.qb + (p.q0 + i) * a.qt + (int64_t)h * a.qh;
+    A q[CPL], o[CPL];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      q[c] = dl + LPK * c < a.D ? S::load(qp[dl + LPK * c]) : (A)0;
+      o[c] = (A)0;
+    }
+    uint64_t mask = 0;
+    int end = p.kend;
+    if constexpr (TREE) mask = tree_mask(a, p.b, i);
+    else end = i + p.off + 1;
+    A m = neg_inf<A>(), l = (A)0;
+    for (int t0 = p.kbeg; t0 < end; t0 += KPW) {
+      const int t = t0 + kl;
+      bool seen = t < end;
+      if (TREE && t >= p.own) seen = seen && ((mask >> ((t - p.own) & 63)) & 1);
+      const int64_t tt = min(t, end - 1);  // lanes past the end re-read the last key
+      A d = (A)0;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c)
+        if (dl + LPK * c < a.D) d += q[c] * S::load(kp[tt * a.kt + dl + LPK * c]);
+#pragma unroll
+      for (int x = 1; x < LPK; x <<= 1) d += __shfl_xor(d, x, 64);
+      d = d * us;
+      if (!seen) continue;
+      const A mn = d > m || d != d ? d : m;  // a NaN score makes the row NaN
+      const A f = m == neg_inf<A>() ? (A)0 : S::exp(m - mn);
+      const A w = mn == neg_inf<A>() ? (A)0 : S::exp(d - mn);
+      m = mn;
+      l = l * f + w;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) {
+        if (dl + LPK * c < a.D) o[c] = o[c] * f + w * S::load(vp[tt * a.vt + dl + LPK * c]);
+      }
+    }
+#pragma unroll
+    for (int x = LPK; x < 64; x <<= 1) {
+      const A m2 = __shfl_xor(m, x, 64), l2 = __shfl_xor(l, x, 64);
+      A f1, f2;
+      join_softmax<S, A>(m, l, m2, l2, f1, f2);
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) {
+        const A o2 = __shfl_xor(o[c], x, 64);
+        // a group without a key has no output: 0 * NaN stays out
+        o[c] = (f1 == (A)0 ? (A)0 : o[c] * f1) + (f2 == (A)0 ? (A)0 : o2 * f2);
+      }
+    }
+    if (kl != 0) continue;
+    if (TREE && a.nsplit > 1) {
+      const int64_t part = ((p.b * a.Hkv + p.kvh) * (int64_t)(a.N * a.G) + r) * a.nsplit + p.split;
+      A* wo = static_cast<A*>(a.ws_o) + part * a.D;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c)
+        if (dl + LPK * c < a.D) wo[dl + LPK * c] = o[c];
+      if (dl == 0) {
+        A* ml = static_cast<A*>(a.ws_ml) + 2 * part;
+        ml[0] = m;
+        ml[1] = l;
+      }
+    } else {
+      // no key at all: zeros; keys whose scores are all -inf: 0 / 0, as a softmax gives
+      const bool none = TREE ? p.own == 0 && mask == 0 : end <= 0;
+      T* yp = static_cast<T*>(a.y) + p.b * a.yb + (p.q0 + i) * a.yt + (int64_t)h * a.yh;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c)
+        if (dl + LPK * c < a.D) yp[dl + LPK * c] = S::store(none ? (A)0 : o[c] / l);
+    }
+  }
+}
+
+// The splits of a row joined: a wavefront per row, lanes along the head.  A row's used
+// splits follow from its length, so what the workspace held before does not matter.
+template <typename T>
+__global__ __launch_bounds__(256) void seq_join_kernel(const SeqArgs a, const int64_t nrows) {
+  using S = SeqAcc<T>;
+  using A = typename S::type;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= nrows) return;
+  const int R = a.N * a.G;
+  const int r = (int)(row % R);
+  const int64_t bh = row / R;
+  const int kvh = (int)(bh % a.Hkv);
+  const int64_t b = bh / a.Hkv;
+  const int i = r / a.G, h = kvh * a.G + r % a.G;
+  const int own = min(max(a.lens != nullptr ? a.lens[b] : a.len, 0), a.Tcap - a.N);
+  const int used = min(a.nsplit, (own + a.N + a.chunk - 1) / a.chunk);
+  const A* ml = static_cast<const A*>(a.ws_ml) + 2 * row * a.nsplit;
+  const A* wo = static_cast<const A*>(a.ws_o) + row * a.nsplit * a.D;
+  A m = neg_inf<A>();
+  bool bad = false;
+  for (int s = lane; s < used; s += 64) {
+    const A ms = ml[2 * s];
+    bad = bad || ms != ms;
+    m = ms > m ? ms : m;
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const A m2 = __shfl_xor(m, x, 64);
+    m = m2 > m ? m2 : m;
+  }
+  bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+  A l = (A)0;
+  for (int s = 0; s < used; ++s) {
+    const A ms = ml[2 * s];
+    if (ms != neg_inf<A>()) l += ml[2 * s + 1] * S::exp(ms - m);
+  }
+  const bool none = own == 0 && tree_mask(a, b, i) == 0;
+  T* yp = static_cast<T*>(a.y) + b * a.yb + i * a.yt + (int64_t)h * a.yh;
+  for (int d = lane; d < a.D; d += 64) {
+    A o = (A)0;
+    for (int s = 0; s < used; ++s) {
+      const A ms = ml[2 * s];
+      if (ms != neg_inf<A>()) o += wo[(int64_t)s * a.D + d] * S::exp(ms - m);
+    }
+    yp[d] = S::store(none ? (A)0 : bad ? (A)__builtin_nanf("") : o / l);
+  }
+}
+
+namespace {
+
+template <typename T, bool TREE>
+int launch_vec(const SeqArgs& a, dim3 grid, hipStream_t s) {
+#define DG_SEQ_VEC(LPK, CPL) hipLaunchKernelGGL((seq_vec_kernel<T, LPK, CPL, TREE>), grid, dim3(256), 0, s, a)
+  if (a.D <= 8) DG_SEQ_VEC(8, 1);
+  else if (a.D <= 16) DG_SEQ_VEC(16, 1);
+  else if (a.D <= 32) DG_SEQ_VEC(32, 1);
+  else if (a.D <= 64) DG_SEQ_VEC(64, 1);
+  else if (a.D <= 128) DG_SEQ_VEC(64, 2);
+  else if (a.D <= 256) DG_SEQ_VEC(64, 4);
+  else if (a.D <= 512) DG_SEQ_VEC(64, 8);
+  else DG_SEQ_VEC(64, 16);
+#undef DG_SEQ_VEC
+  return check_launch("seq_vec_kernel");
+}
+
+template <bool TREE>
+int launch_vec_any(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
+  if (dtype == DG_F64) return launch_vec<double, TREE>(a, grid, s);
+  if (dtype == DG_F32) return launch_vec<float, TREE>(a, grid, s);
+  if (dtype == DG_BF16) return launch_vec<bf16_t, TREE>(a, grid, s);
+  return launch_vec<f16_t, TREE>(a, grid, s);
+}
+
+constexpr int kWideRows = 128;  // rows of a wide tile
+constexpr int kVecRows = 32;    // rows of a workgroup of the vector kernel over a tree
+
+// Workgroups that a split aims at: two for each of the 256 CUs.  A split's length is a
+// multiple of 128 keys, at least 256, so that joining it costs little beside reading it.
+constexpr int64_t kSplitWorkgroups = 512;
+constexpr int kMaxSplits = 512;
+
+int tree_chunk(int64_t B, int Hkv, int nrb, int keys) {
+  const int64_t wg = B * Hkv * nrb;
+  const int64_t want = (kSplitWorkgroups + wg - 1) / wg;  // splits of a row
+  int64_t chunk = (keys + want - 1) / want;
+  chunk = std::max<int64_t>(chunk, (keys + kMaxSplits - 1) / kMaxSplits);
+  chunk = std::max<int64_t>((chunk + 127) / 128 * 128, 256);
+  return (int)std::min<int64_t>(chunk, 0x7fffff80);
+}
+
+// Row blocks, splits and workspace of a call.
+struct TreeShape {
+  int rows_per_wg, nrb, nsplit, chunk;
+  size_t o_bytes, ws_bytes;
+};
+
+TreeShape tree_shape(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype, int rows_per_wg) {
+  TreeShape t{};
+  const int R = N * (H / Hkv);
+  t.rows_per_wg = rows_per_wg;
+  t.nrb = (R + rows_per_wg - 1) / rows_per_wg;
+  t.chunk = tree_chunk(B, Hkv, t.nrb, Tcap);
+  t.nsplit = (int)(((int64_t)Tcap + t.chunk - 1) / t.chunk);
+  const size_t acc = dtype == DG_F64 ? 8 : 4;
+  const size_t parts = (size_t)B * Hkv * R * t.nsplit;
+  if (t.nsplit > 1) {
+    t.o_bytes = (parts * D * acc + 15) & ~(size_t)15;
+    t.ws_bytes = t.o_bytes + parts * 2 * acc;
+  }
+  return t;
+}
+
+bool known_dtype(int dtype) { return dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64; }
+
+// A bound on the workspace whichever kernel a call takes (the row blocks of each give
+// other splits).
+size_t tree_workspace(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
+  size_t most = 0;
+  for (int rows : {32, 64, 128})
+    most = std::max(most, tree_shape(B, N, H, Hkv, Tcap, D, dtype, rows).ws_bytes);
+  return most;
+}
+
+}  // namespace
+}  // namespace dg
+
+using namespace dg;
+
+extern "C" int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, int group, dg_packed_tile* tiles,
+                              int64_t cap, int64_t* counts) {
+  DG_REQUIRE(S >= 0 && group >= 1 && cap >= 0, DG_EINVAL, "packed_plan: negative size or group");
+  DG_REQUIRE(counts != nullptr && (S == 0 || (lq != nullptr && lk != nullptr)) && (cap == 0 || tiles != nullptr),
+             DG_EINVAL, "packed_plan: NULL argument");
+  int64_t nq = 0, nk = 0;
+  for (int64_t s = 0; s < S; ++s) {
+    DG_REQUIRE(lq[s] >= 0 && lk[s] >= 0, DG_EINVAL, "packed_plan: sequence %lld has a negative length", (long long)s);
+    DG_REQUIRE(lq[s] <= 0x7fffffff / group, DG_EINVAL, "packed_plan: sequence %lld has too many rows", (long long)s);
+    nq += lq[s];
+    nk += lk[s];
+    DG_REQUIRE(nq <= 0x7fffffff && nk <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 rows");
+  }
+  int64_t n = 0;
+  for (int64_t s = 0; s < S; ++s) n += (lq[s] * group + kWideRows - 1) / kWideRows;
+  DG_REQUIRE(n <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 tiles");
+  counts[0] = n;
+  counts[1] = 0;
+  if (tiles == nullptr) return DG_OK;
+  DG_REQUIRE(cap >= n, DG_EINVAL, "packed_plan: room for %lld tiles, %lld needed", (long long)cap, (long long)n);
+  int64_t at = 0, q0 = 0, k0 = 0;
+  for (int64_t s = 0; s < S; ++s) {
+    const int64_t rows = lq[s] * group;
+    for (int64_t r = 0; r < rows; r += kWideRows)
+      tiles[at++] = dg_packed_tile{(int32_t)q0, (int32_t)lq[s], (int32_t)k0, (int32_t)lk[s], (int32_t)r,
+                                   (int32_t)std::min<int64_t>(kWideRows, rows - r), {0, 0}};
+    q0 += lq[s];
+    k0 += lk[s];
+  }
+  return DG_OK;
+}
+
+extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D, int dtype, const void* q, int64_t q_t,
+                                   int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t,
+                                   int64_t v_h, void* y, int64_t y_t, int64_t y_h, float scale,
+                                   const dg_packed_tile* tiles, int64_t n_wide, int64_t n_narrow, void* stream) {
+  DG_REQUIRE(Nq >= 0 && Nk >= 0 && H >= 0 && n_wide >= 0 && n_narrow >= 0, DG_EINVAL, "attention_packed: negative size");
+  DG_REQUIRE(known_dtype(dtype), DG_EUNSUPPORTED, "attention_packed: dtype %d unsupported", dtype);
+  DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "attention_packed: head_dim %d outside [1, %d]", D, kMaxHeadDim);
+  DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "attention_packed: %d query heads on %d key heads", H, Hkv);
+  DG_REQUIRE(Hkv <= 65535, DG_EINVAL, "attention_packed: %d key heads, at most 65535", Hkv);
+  DG_REQUIRE(scale > 0.f && std::isfinite(scale), DG_EINVAL, "attention_packed: the scale must be positive");
+  DG_REQUIRE(n_wide + n_narrow <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 tiles");
+  if (Nq == 0 || H == 0 || n_wide + n_narrow == 0) return DG_OK;
+  DG_REQUIRE(q && y && tiles && (Nk == 0 || (k && v)), DG_EINVAL, "attention_packed: NULL argument");
+  SeqArgs a{};
+  a.q = q; a.k = k; a.v = v; a.y = y;
+  a.qt = q_t; a.qh = q_h; a.kt = k_t; a.kh = k_h;
+  a.vt = v_t; a.vh = v_h; a.yt = y_t; a.yh = y_h;
+  a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
+  a.scale = scale;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.tiles = tiles;
+  a.nq = Nq; a.nk = Nk;
+  a.nsplit = 1;
+  a.rows_per_wg = kWideRows;
+  return launch_vec_any<false>(a, dtype, dim3((unsigned)(n_wide + n_narrow), (unsigned)Hkv),
+                               static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t dg_attention_tree_workspace_size(int B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
+  if (B <= 0 || N <= 0 || N > 64 || H <= 0 || Hkv <= 0 || H % Hkv || Tcap < N || D <= 0) return 0;
+  return tree_workspace(B, N, H, Hkv, Tcap, D, dtype);
+}
+
+extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, int dtype, const void* q,
+                                 const dg_stride3* q_st, const void* k_cache, const dg_stride3* kc_st,
+                                 const void* v_cache, const dg_stride3* vc_st, void* y, const dg_stride3* y_st,
+                                 float scale, int len, const int32_t* lens, const int64_t* masks, int64_t mask_b,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  DG_REQUIRE(B >= 0 && H >= 0, DG_EINVAL, "attention_tree: negative size");
+  DG_REQUIRE(known_dtype(dtype), DG_EUNSUPPORTED, "attention_tree: dtype %d unsupported", dtype);
+  DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "attention_tree: head_dim %d outside [1, %d]", D, kMaxHeadDim);
+  DG_REQUIRE(N >= 1 && N <= 64, DG_EINVAL, "attention_tree: %d tokens a row, 1 to 64", N);
+  DG_REQUIRE(Tcap >= N, DG_EINVAL, "attention_tree: the cache holds %d positions, %d tokens", Tcap, N);
+  DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "attention_tree: %d query heads on %d key heads", H, Hkv);
+  DG_REQUIRE(H / Hkv <= 0x7fffff, DG_EINVAL, "attention_tree: %d heads a group", H / Hkv);
+  DG_REQUIRE(scale > 0.f && std::isfinite(scale), DG_EINVAL, "attention_tree: the scale must be positive");
+  DG_REQUIRE(lens != nullptr || (len >= 0 && len <= Tcap - N), DG_EINVAL,
+             "attention_tree: %d cached positions and %d tokens in a cache of %d", len, N, Tcap);
+  if (B == 0 || H == 0) return DG_OK;
+  DG_REQUIRE(q && k_cache && v_cache && y && q_st && kc_st && vc_st && y_st, DG_EINVAL, "attention_tree: NULL argument");
+  SeqArgs a{};
+  a.q = q; a.k = k_cache; a.v = v_cache; a.y = y;
+  a.qb = q_st->b; a.qt = q_st->t; a.qh = q_st->h;
+  a.kb = kc_st->b; a.kt = kc_st->t; a.kh = kc_st->h;
+  a.vb = vc_st->b; a.vt = vc_st->t; a.vh = vc_st->h;
+  a.yb = y_st->b; a.yt = y_st->t; a.yh = y_st->h;
+  a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
+  a.scale = scale;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.B = B; a.N = N; a.Tcap = Tcap;
+  a.len = len; a.lens = lens;
+  a.masks = masks; a.mask_b = mask_b;
+  const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, kVecRows);
+  a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
+  if (t.nsplit > 1) {
+    DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,
+               "attention_tree: a workspace of %zu bytes, %zu needed", workspace_bytes, t.ws_bytes);
+    DG_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, DG_EINVAL, "attention_tree: workspace not 16-byte aligned");
+    a.ws_o = workspace;
+    a.ws_ml = static_cast<char*>(workspace) + t.o_bytes;
+  }
+  const int64_t blocks = (int64_t)B * Hkv * t.nrb * t.nsplit;
+  DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int rc = launch_vec_any<true>(a, dtype, dim3((unsigned)blocks), s);
+  if (rc != DG_OK || t.nsplit == 1) return rc;
+  const int64_t rows = (int64_t)B * H * N;
+  DG_REQUIRE((rows + 3) / 4 <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
+  const dim3 grid((unsigned)((rows + 3) / 4));
+  if (dtype == DG_F64) hipLaunchKernelGGL(seq_join_kernel<double>, grid, dim3(256), 0, s, a, rows);
+  else if (dtype == DG_F32) hipLaunchKernelGGL(seq_join_kernel<float>, grid, dim3(256), 0, s, a, rows);
+  else if (dtype == DG_BF16) hipLaunchKernelGGL(seq_join_kernel<bf16_t>, grid, dim3(256), 0, s, a, rows);
+  else hipLaunchKernelGGL(seq_join_kernel<f16_t>, grid, dim3(256), 0, s, a, rows);
+  return check_launch("seq_join_kernel");
+}

@@ -1,0 +1,117 @@
+// Launch arguments shared by the kernels of packed attention and of token trees
+// over a cache (dg_attn_seq.hip: any shape; dg_attn_seq_mfma.hip: 16-bit and fp32 data
+// at head_dim 16, 32, 64 and 128).
+//
+// Both operators reduce to one piece of work: the rows of one key head, where the
+// rows are the (query, head of the group) pairs r = i * G + g of a sequence, over a
+// range of that sequence's keys.  Heads of a group so share every key they read, and
+// a few queries still fill a tile of rows.
+#pragma once
+
+#include "dg_common.h"
+
+namespace dg {
+
+struct SeqArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* y;
+  int64_t qb, qt, qh;
+  int64_t kb, kt, kh;
+  int64_t vb, vt, vh;
+  int64_t yb, yt, yh;
+  int H, Hkv, G, D;
+  float scale;       // the softmax scale
+  float scale_log2;  // ... * log2(e)
+  // packed: tiles of rows, and the rows q and k hold in all
+  const dg_packed_tile* tiles;
+  int64_t nq, nk;
+  // tree: rows of the batch, tokens a row, positions a cache page holds
+  int B, N, Tcap;
+  int len;              // cached positions, where lens is null
+  const int32_t* lens;  // (B)
+  const int64_t* masks; // bit m of masks[b * mask_b + n]: token n sees token m; null: the earlier ones and itself
+  int64_t mask_b;
+  int rows_per_wg;  // rows of a workgroup
+  int nrb;          // row blocks of a (b, key head)
+  int nsplit;       // key splits of a row (1: y is written)
+  int chunk;        // keys of a split
+  // nsplit > 1: unnormalised outputs (nsplit, D) and (maximum, sum) pairs (nsplit, 2) of row
+  // (b * Hkv + key head) * N * G + r
+  void* ws_o;
+  void* ws_ml;
+};
+
+// A workgroup's piece: the rows row0 .. row0 + rows - 1 of a sequence of `nrows` rows,
+// over keys [kbeg, kend).  Query i sees key t iff t < own, or t < own + 64 and bit
+// t - own of its mask; packed: iff t <= i + off.
+struct SeqPiece {
+  int row0, rows;  // of the sequence's (query, head) rows
+  int kbeg, kend;
+  int off;         // packed: Lk - Lq
+  int own;         // tree: the cached positions
+  int64_t b;       // tree: the row of the batch; packed: 0
+  int64_t q0, k0;  // packed: the sequence's first rows in q and k
+  int kvh, split;
+};
+
+// The piece of this workgroup; false where there is nothing to do.  Nothing a table or
+// a length in device memory says takes an access outside q, k, v and y: tiles that do
+// not lie inside them are left out, lengths beyond the cache are taken as its end.
+template <bool TREE>
+__device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
+  if constexpr (TREE) {
+    int64_t u = (int64_t)blockIdx.x;
+    p.split = (int)(u % a.nsplit);
+    u /= a.nsplit;
+    const int rb = (int)(u % a.nrb);
+    u /= a.nrb;
+    p.kvh = (int)(u % a.Hkv);
+    p.b = u / a.Hkv;
+    const int len = a.lens != nullptr ? a.lens[p.b] : a.len;
+    p.own = min(max(len, 0), a.Tcap - a.N);
+    p.row0 = rb * a.rows_per_wg;
+    p.rows = min(a.rows_per_wg, a.N * a.G - p.row0);
+    p.kbeg = p.split * a.chunk;
+    p.kend = min(p.own + a.N, p.kbeg + a.chunk);
+    p.off = 0;
+    p.q0 = p.k0 = 0;
+    return p.kbeg < p.kend;
+  } else {
+    const dg_packed_tile t = a.tiles[blockIdx.x];
+    p.kvh = blockIdx.y;
+    p.split = 0;
+    p.b = 0;
+    p.own = 0;
+    if (t.lq <= 0 || t.lk < 0 || t.q0 < 0 || t.k0 < 0 || (int64_t)t.q0 + t.lq > a.nq || (int64_t)t.k0 + t.lk > a.nk)
+      return false;
+    if (t.row0 < 0 || t.rows <= 0 || t.rows > a.rows_per_wg || (int64_t)t.row0 + t.rows > (int64_t)t.lq * a.G)
+      return false;
+    p.row0 = t.row0;
+    p.rows = t.rows;
+    p.off = t.lk - t.lq;
+    p.q0 = t.q0;
+    p.k0 = t.k0;
+    p.kbeg = 0;
+    // the keys that the tile's last query sees
+    p.kend = max(0, (t.row0 + t.rows - 1) / a.G + p.off + 1);
+    return true;
+  }
+}
+
+// The tokens of the tree that token n of row b sees.
+__device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n) {
+  const uint64_t all = a.N >= 64 ? ~0ull : (1ull << a.N) - 1;
+  if (a.masks == nullptr) return n >= 63 ? ~0ull : (2ull << n) - 1;
+  return (uint64_t)a.masks[b * a.mask_b + n] & all;
+}
+
+// dg_attn_seq_mfma.hip: whether it takes the shape, the rows of its wide and narrow
+// workgroups, and its launches
+bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree);
+int seq_mfma_tree_rows(const SeqArgs& a, int dtype);
+int launch_seq_mfma_packed(SeqArgs a, int dtype, int64_t n_wide, int64_t n_narrow, hipStream_t s);
+int launch_seq_mfma_tree(const SeqArgs& a, int dtype, hipStream_t s);
+
+}  // namespace dg

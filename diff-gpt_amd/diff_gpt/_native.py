@@ -13,6 +13,7 @@ and returns immediately.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -247,13 +248,40 @@ _SIGNATURES = {
          ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_void_p,
          ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
     ),
+    "dg_packed_plan": (
+        ctypes.c_int,
+        [ctypes.c_int64, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64), ctypes.c_int,
+         ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)],
+    ),
+    "dg_attention_packed": (
+        ctypes.c_int,
+        [ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int] * 4
+        + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64] * 4  # q, k, v, y
+        + [ctypes.c_float, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "dg_attention_tree_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 7),
+    "dg_attention_tree": (
+        ctypes.c_int,
+        [ctypes.c_int] * 7
+        + [ctypes.c_void_p, ctypes.POINTER(Stride3)] * 4  # q, k_cache, v_cache, y
+        + [ctypes.c_float, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "dg_token_logprobs": (
+        ctypes.c_int,
+        [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
+    ),
 }
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 # head_dim the kernels take: every even size up to 1024 (a row padded to the
 # next power of two spreads over at most 64 lanes of 16 elements)
 MAX_HEAD_DIM = 1024
+
+# most alternatives a row of dg_token_logprobs gives
+MAX_TOP = 64
 
 
 def head_dim_supported(D: int) -> bool:
@@ -722,6 +750,166 @@ def draw_argmax_(probs: torch.Tensor, q: torch.Tensor, ids: torch.Tensor) -> boo
                               _ptr(ids), _stream(p2))
     _check(rc, "draw_argmax")
     return True
+
+
+def _check_tensors(what: str, *tensors: torch.Tensor) -> None:
+    """On one ROCm device, of one supported type, tracked by nobody."""
+    require_device(what, *tensors)
+    require_inference(what, *tensors)
+    first = tensors[0]
+    for t in tensors:
+        if t.dtype != first.dtype:
+            raise TypeError(f"{what}: the tensors must share one dtype, got {first.dtype} and {t.dtype}")
+        if t.device != first.device:
+            raise ValueError(f"{what}: the tensors must share one device, got {first.device} and {t.device}")
+    _dtype_code(first)
+
+
+def _on_device_of(t: torch.Tensor):
+    """A context in which t's device is the current one, which a launch on its stream needs."""
+    if t.get_device() == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _check_scale(what: str, scale: float) -> float:
+    scale = float(scale)
+    if not (math.isfinite(scale) and scale > 0 and float(ctypes.c_float(scale).value) > 0):
+        raise ValueError(f"{what}: the scale must be positive and finite, got {scale}")
+    return scale
+
+
+# rows of a dg_packed_tile: eight 32-bit integers
+_TILE_WORDS = 8
+
+
+def packed_plan(q_lengths: list[int], k_lengths: list[int], group: int) -> tuple[torch.Tensor, int, int]:
+    """dg_packed_plan: the (tiles, 8) int32 table of a batch, on the host, and how many of
+    its tiles are wide (they come first) and narrow."""
+    n = len(q_lengths)
+    lq, lk = (ctypes.c_int64 * n)(*q_lengths), (ctypes.c_int64 * n)(*k_lengths)
+    counts = (ctypes.c_int64 * 2)()
+    L = lib()
+    _check(L.dg_packed_plan(n, lq, lk, group, None, 0, counts), "packed_plan")
+    tiles = torch.empty((counts[0] + counts[1], _TILE_WORDS), dtype=torch.int32)
+    if len(tiles):
+        _check(L.dg_packed_plan(n, lq, lk, group, tiles.data_ptr(), len(tiles), counts), "packed_plan")
+    return tiles, counts[0], counts[1]
+
+
+def attention_packed_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, y: torch.Tensor, layout, scale: float) -> None:
+    """dg_attention_packed: q, y (Nq,H,D) and k, v (Nk,Hkv,D) hold the sequences of
+    ``layout`` (a PackedLayout for groups of H / Hkv heads) one after the other.  Rows of y
+    behind the last sequence are left as they are."""
+    _check_tensors("attention_packed", q, k, v, y)
+    if q.dim() != 3 or k.dim() != 3 or y.shape != q.shape or v.shape != k.shape or k.size(2) != q.size(2):
+        raise ValueError("attention_packed: q, y must be (Nq, H, D) and k, v (Nk, Hkv, D)")
+    Nq, H, D = q.shape
+    Nk, Hkv, _ = k.shape
+    if not 1 <= D <= MAX_HEAD_DIM:
+        raise ValueError(f"attention_packed: head_dim {D} outside 1 .. {MAX_HEAD_DIM}")
+    if Hkv < 1 or H % Hkv or H // Hkv != layout.group:
+        raise ValueError(f"attention_packed: {H} query heads on {Hkv} key heads, a layout for groups of {layout.group}")
+    if layout.total_q > Nq or layout.total_k > Nk:
+        raise ValueError(f"attention_packed: the layout covers {layout.total_q} and {layout.total_k} rows, "
+                         f"q and k hold {Nq} and {Nk}")
+    if layout.tiles.device != q.device:
+        raise ValueError(f"attention_packed: the layout is on {layout.tiles.device}, q on {q.device}")
+    for t in (q, k, v, y):
+        if t.stride(2) != 1 and D > 1:
+            raise ValueError("attention_packed: the last (head_dim) dimension must be contiguous")
+    scale = _check_scale("attention_packed", scale)
+    st = lambda t: (_ptr(t), t.stride(0), t.stride(1))  # noqa: E731
+    with _on_device_of(q):
+        rc = lib().dg_attention_packed(
+            Nq, Nk, H, Hkv, D, _dtype_code(q), *st(q), *st(k), *st(v), *st(y), scale, _ptr(layout.tiles),
+            layout.n_wide, layout.n_narrow, _stream(q),
+        )
+    _check(rc, "attention_packed")
+
+
+def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, y: torch.Tensor, scale: float,
+                    lengths: int | torch.Tensor, masks: torch.Tensor | None = None) -> None:
+    """dg_attention_tree: q, y (B,N,H,D); the caches (B,Tcap,Hkv,D) views hold each row's
+    cached positions and, behind them, the N tokens' own.  lengths: the cached positions,
+    one int or a (B,) int32 tensor; masks: (N,) or (B,N) int64, bit m of a token's mask set
+    where it sees token m (None: the tokens before it and itself)."""
+    _check_tensors("attention_tree", q, k_cache, v_cache, y)
+    if q.dim() != 4 or k_cache.dim() != 4 or y.shape != q.shape or v_cache.shape != k_cache.shape:
+        raise ValueError("attention_tree: q, y must be (B, N, H, D) and the caches (B, Tcap, Hkv, D)")
+    B, N, H, D = q.shape
+    _, Tcap, Hkv, _ = k_cache.shape
+    if k_cache.size(0) != B or k_cache.size(3) != D:
+        raise ValueError("attention_tree: the caches must have q's rows and head_dim")
+    if not 1 <= D <= MAX_HEAD_DIM:
+        raise ValueError(f"attention_tree: head_dim {D} outside 1 .. {MAX_HEAD_DIM}")
+    if not 1 <= N <= 64:
+        raise ValueError(f"attention_tree: {N} tokens a row, 1 to 64")
+    if Hkv < 1 or H % Hkv:
+        raise ValueError(f"attention_tree: {H} query heads on {Hkv} key heads")
+    if Tcap < N:
+        raise ValueError(f"attention_tree: a cache of {Tcap} positions does not hold {N} tokens")
+    lens, host_len = None, 0
+    if isinstance(lengths, torch.Tensor):
+        if lengths.shape != (B,) or lengths.dtype != torch.int32 or lengths.device != q.device or (
+                B > 1 and lengths.stride(0) != 1):
+            raise ValueError("attention_tree: lengths must be a contiguous (B,) int32 tensor on q's device")
+        lens = lengths
+    else:
+        host_len = int(lengths)
+        if not 0 <= host_len <= Tcap - N:
+            raise ValueError(f"attention_tree: {host_len} cached positions and {N} tokens in a cache of {Tcap}")
+    mask_b = 0
+    if masks is not None:
+        if masks.shape not in ((N,), (B, N)) or masks.dtype != torch.int64 or masks.device != q.device:
+            raise ValueError("attention_tree: masks must be an (N,) or (B, N) int64 tensor on q's device")
+        if N > 1 and masks.stride(-1) != 1:
+            masks = masks.contiguous()
+        mask_b = masks.stride(0) if masks.dim() == 2 else 0
+    scale = _check_scale("attention_tree", scale)
+    code = _dtype_code(q)
+    L = lib()
+    st = lambda t: ctypes.pointer(_bthd_strides(t))  # noqa: E731
+    with _on_device_of(q):
+        ws_bytes = L.dg_attention_tree_workspace_size(B, N, H, Hkv, Tcap, D, code)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        rc = L.dg_attention_tree(
+            B, N, H, Hkv, Tcap, D, code, _ptr(q), st(q), _ptr(k_cache), st(k_cache), _ptr(v_cache), st(v_cache),
+            _ptr(y), st(y), scale, host_len, _ptr(lens), _ptr(masks), mask_b, _ptr(ws), ws_bytes, _stream(q),
+        )
+    _check(rc, "attention_tree")
+
+
+def token_logprobs_(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, entropy: torch.Tensor | None,
+                    top_logprobs: torch.Tensor | None = None, top_ids: torch.Tensor | None = None) -> None:
+    """dg_token_logprobs: per row of logits (M,V) the log probability of ids (M,) int64 and
+    the entropy into (M,) tensors, and with top_logprobs, top_ids (M,top) the most likely
+    alternatives.  The results are fp32, fp64 for fp64 logits."""
+    _check_tensors("token_logprobs", logits)
+    if logits.dim() != 2:
+        raise ValueError(f"token_logprobs: logits must be (M, V), got {tuple(logits.shape)}")
+    M, V = logits.shape
+    if V < 1:
+        raise ValueError("token_logprobs: an empty vocabulary")
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("token_logprobs: the last (vocabulary) dimension must be contiguous")
+    out = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    if (top_logprobs is None) != (top_ids is None):
+        raise ValueError("token_logprobs: top_logprobs and top_ids come together")
+    top = 0 if top_ids is None else top_ids.size(-1)
+    if not 0 <= top <= min(V, MAX_TOP):
+        raise ValueError(f"token_logprobs: top {top} outside 0 .. min(V, {MAX_TOP})")
+    for name, t, shape, dtype in (("ids", ids, (M,), torch.int64), ("logprobs", logprobs, (M,), out),
+                                  ("entropy", entropy, (M,), out), ("top_logprobs", top_logprobs, (M, top), out),
+                                  ("top_ids", top_ids, (M, top), torch.int64)):
+        if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != logits.device):
+            raise ValueError(f"token_logprobs: {name} must be a contiguous {shape} {dtype} tensor on the logits' device")
+    with _on_device_of(logits):
+        rc = lib().dg_token_logprobs(
+            M, V, _dtype_code(logits), _ptr(logits), logits.stride(0), _ptr(ids), _ptr(logprobs), _ptr(entropy), top,
+            _ptr(top_logprobs), _ptr(top_ids), _stream(logits),
+        )
+    _check(rc, "token_logprobs")
 
 
 def copy4d_(src: torch.Tensor, dst: torch.Tensor) -> None:

@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define DG_ABI_VERSION 3
+#define DG_ABI_VERSION 4
 
 #if defined(__GNUC__)
 #define DG_API __attribute__((visibility("default")))
@@ -53,7 +53,9 @@ extern "C" {
  * DG_EUNSUPPORTED for it.  The attention scale is an fp32 argument: with
  * fp64 data its rounding of 1/sqrt(D) (SDPA's default) stands for 1/sqrt(D)
  * in fp64, any other scale acts as its fp32 value.  ABI version 3 added
- * DG_F64 and made dg_swiglu's alpha / limit and dg_softcap's cap double. */
+ * DG_F64 and made dg_swiglu's alpha / limit and dg_softcap's cap double;
+ * version 4 added dg_packed_plan, dg_attention_packed, dg_attention_tree and
+ * dg_token_logprobs, which take fp64 as well. */
 enum dg_dtype { DG_F32 = 0, DG_BF16 = 1, DG_F16 = 2, DG_F64 = 3 };
 
 enum dg_status {
@@ -571,6 +573,83 @@ DG_API int dg_linear_rows(int64_t M, int N, int K, int dtype, const void* x, int
  */
 DG_API int dg_draw_argmax(int64_t M, int V, int dtype, const void* probs, int64_t p_ld, const void* q,
                    int64_t q_ld, int64_t* ids, void* stream);
+
+/*
+ * Attention over packed sequences of different lengths, with grouped heads: no
+ * counterpart in the reference, which scores one series at a time
+ * (diff_gpt.py:295-363).  q and y hold Nq rows of H heads, k and v Nk rows of Hkv heads
+ * (H a multiple of Hkv; query head h reads key head h / (H / Hkv)), each addressed as
+ * base + row * *_t + head * *_h + d.  Sequence s owns lq[s] consecutive rows of q and
+ * lk[s] of k, one sequence after the other; its query i sees its keys
+ * 0 .. i + lk[s] - lq[s], so that with lk > lq the first keys are cached ones.  A query
+ * that sees no key gets zeros.  Rows of y behind the last sequence are left as they are.
+ *
+ * dg_packed_plan lays the work out once per batch, on the host and without the device: it
+ * writes the tiles of the sequences for heads in groups of `group` into `tiles` (room for
+ * `cap`; NULL with cap 0 only counts) and counts[0] wide ones, which come first, and
+ * counts[1] narrow ones.  The caller copies the table to the device and hands it to every
+ * dg_attention_packed over such a batch.  A tile that does not lie inside Nq and Nk rows
+ * is skipped, never followed.
+ * fp32 / bf16 / fp16 / fp64, every head_dim up to 1024, rows with unit stride over d; the
+ * scale is positive.
+ */
+typedef struct dg_packed_tile {
+  int32_t q0, lq, k0, lk; /* the sequence's rows of q and of k */
+  int32_t row0, rows;     /* the tile's (query, head of the group) rows, query * group + head */
+  int32_t pad[2];
+} dg_packed_tile;
+
+DG_API int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, int group, dg_packed_tile* tiles,
+                          int64_t cap, int64_t* counts);
+
+DG_API int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D, int dtype,
+                               const void* q, int64_t q_t, int64_t q_h,
+                               const void* k, int64_t k_t, int64_t k_h,
+                               const void* v, int64_t v_t, int64_t v_h,
+                               void* y, int64_t y_t, int64_t y_h, float scale,
+                               const dg_packed_tile* tiles, int64_t n_wide, int64_t n_narrow, void* stream);
+
+/*
+ * Attention of a few tokens a row -- a tree of candidates, or a decode step's one --
+ * over the row's cache, with grouped heads and rows of different lengths: no counterpart
+ * in the reference.  q and y are (B,N,H,D) views, the caches (B,Tcap,Hkv,D) views from
+ * position 0.  Row b holds len[b] cached positions (`lens`, an int32 array on the device,
+ * or `len` for every row where it is NULL; taken as 0 .. Tcap - N) and after them the N
+ * tokens' own keys and values.  Token n sees all cached positions and token m where bit m
+ * of masks[b * mask_b + n] (int64 on the device; mask_b 0: one tree for all rows) is set;
+ * masks NULL: token n sees tokens 0 .. n.  A token that sees nothing gets zeros.  What
+ * positions hidden from a token hold, NaN and infinities included, does not reach it.
+ * 1 <= N <= 64, Tcap >= N.  Long rows are split over workgroups whose partial results meet
+ * in the caller's workspace (dg_attention_tree_workspace_size bytes, 16-byte aligned; its
+ * contents need no initialisation, and calls that may overlap need one each).
+ * Types, head_dim and scale as dg_attention_packed.
+ */
+DG_API size_t dg_attention_tree_workspace_size(int B, int N, int H, int Hkv, int Tcap, int D, int dtype);
+
+DG_API int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, int dtype,
+                             const void* q, const dg_stride3* q_st,
+                             const void* k_cache, const dg_stride3* kc_st,
+                             const void* v_cache, const dg_stride3* vc_st,
+                             void* y, const dg_stride3* y_st, float scale,
+                             int len, const int32_t* lens, const int64_t* masks, int64_t mask_b,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probability of a given token per row of logits, the row's entropy and its most
+ * likely alternatives, in one pass over the logits (diff_gpt.py:348-352 takes the first
+ * of them through a whole log_softmax).  For each of the M rows x of V logits (row stride
+ * x_ld, unit column stride), with p = softmax(x):
+ *   logprob[m] = log p[ids[m]]       (NaN for an id outside [0, V))
+ *   entropy[m] = -sum_v p_v log p_v  (NULL: not wanted)
+ *   top_logprob[m][j], top_ids[m][j], j < top: the `top` largest logits in descending
+ *     order, equal ones by ascending id (contiguous rows of `top`)
+ * computed and stored in fp32 (fp64 for fp64 logits).  A row that holds a NaN or +inf, or
+ * -inf alone, gives NaN log probabilities and entropy, as log_softmax does; its ids are
+ * those of its largest logits, NaN ones last.  0 <= top <= min(V, 64).
+ */
+DG_API int dg_token_logprobs(int64_t M, int64_t V, int dtype, const void* x, int64_t x_ld, const int64_t* ids,
+                             void* logprob, void* entropy, int top, void* top_logprob, int64_t* top_ids,
+                             void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,355 @@
+"""Packed attention and token trees over a cache (dg_attn_seq.hip, dg_attn_seq_mfma.hip)
+against float64 at the lengths, masks and layouts where they can go wrong."""
+
+import pytest
+import torch
+
+from diff_gpt import _native
+from diff_gpt.model.packed import PackedLayout, attention_packed
+from diff_gpt.model.tree import attention_tree, tree_masks
+from seq_cases import TDT, attend64, close, some_tree, tree_seen
+
+pytestmark = pytest.mark.gpu
+INF, NAN = float("inf"), float("nan")
+
+
+def _causal(n, t, dev):
+    return torch.arange(t, device=dev)[None] <= torch.arange(n, device=dev)[:, None] + (t - n)
+
+
+def _packed_case(dev, q_lens, k_lens, H, Hkv, D, dt, seed=0, slack=0, scale=1.0):
+    """q, k, v as column slices of wider rows (an odd number of columns apart when slack)."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    new = lambda n, h: (torch.randn(n, h * D + slack, generator=g, device=dev) * scale).to(dt)  # noqa: E731
+    n, t = sum(q_lens), sum(k_lens)
+    return (new(n, H)[:, : H * D].view(n, H, D), new(t, Hkv)[:, : Hkv * D].view(t, Hkv, D),
+            new(t, Hkv)[:, : Hkv * D].view(t, Hkv, D))
+
+
+def _check_packed(q, k, v, y, q_lens, k_lens, dtype):
+    a = b = 0
+    for n, t in zip(q_lens, k_lens):
+        if n:
+            ref, mag = attend64(q[a : a + n], k[b : b + t], v[b : b + t], _causal(n, t, q.device))
+            close(y[a : a + n], ref, mag, dtype, t, float(v.abs().max()) if v.numel() else 0.0)
+        a, b = a + n, b + t
+
+
+LENGTHS = [
+    ([1], [1]),
+    ([1, 1, 1], [1, 64, 1000]),  # single tokens behind caches of their own length
+    ([0, 5, 0], [0, 5, 7]),
+    ([31, 32, 33, 64, 65], [31, 32, 33, 64, 65]),
+    ([127, 128, 129, 130, 2], [127, 128, 129, 130, 2]),
+    ([10, 200, 3], [300, 200, 150]),  # chunks behind cached keys
+    ([5, 40], [3, 0]),  # queries that see nothing
+    ([700], [701]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("H,Hkv,D", [(4, 4, 16), (2, 1, 32), (6, 2, 64), (8, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("q_lens,k_lens", LENGTHS)
+def test_packed_matches_float64(dev, dtype, H, Hkv, D, q_lens, k_lens):
+    q, k, v = _packed_case(dev, q_lens, k_lens, H, Hkv, D, TDT[dtype], seed=D + H)
+    y = attention_packed(q, k, v, PackedLayout(q_lens, k_lens, group=H // Hkv))
+    _check_packed(q, k, v, y, q_lens, k_lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
+@pytest.mark.parametrize("H,Hkv,D", [(2, 2, 1), (3, 1, 7), (2, 1, 24), (4, 2, 80), (2, 2, 96), (2, 1, 256), (1, 1, 1000)])
+def test_packed_takes_every_head_dim(dev, dtype, H, Hkv, D):
+    q_lens, k_lens = [1, 37, 70], [50, 37, 71]
+    q, k, v = _packed_case(dev, q_lens, k_lens, H, Hkv, D, TDT[dtype], seed=D)
+    y = attention_packed(q, k, v, PackedLayout(q_lens, k_lens, group=H // Hkv))
+    _check_packed(q, k, v, y, q_lens, k_lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_packed_takes_unaligned_rows(dev, dtype, D):
+    """Rows an odd number of elements apart: no 16-byte loads."""
+    q_lens = [40, 133]
+    q, k, v = _packed_case(dev, q_lens, q_lens, 4, 2, D, TDT[dtype], slack=3)
+    y = attention_packed(q, k, v, PackedLayout(q_lens, group=2))
+    _check_packed(q, k, v, y, q_lens, q_lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_packed_hidden_values_stay_hidden(dev, dtype, D):
+    """NaN and infinities in the keys and values of later positions, and in rows behind
+    the last sequence, reach no query that does not see them; those that do see an infinite
+    value get it."""
+    q_lens, k_lens = [50, 70, 5], [50, 90, 40]
+    q, k, v = (x.clone() for x in _packed_case(dev, q_lens, k_lens, 2, 2, D, TDT[dtype], seed=3))
+    extra = torch.full((9, 2, D), NAN, dtype=k.dtype, device=dev)
+    k, v = torch.cat([k, extra]), torch.cat([v, extra])
+    clean = attention_packed(q, k, v, PackedLayout(q_lens, k_lens))
+    kk, vv = k.clone(), v.clone()
+    bad = 50 + 20 + 33  # key 53 of the second sequence: queries 33 .. 69 see it
+    kk[bad] = NAN
+    vv[bad] = INF
+    y = attention_packed(q, kk, vv, PackedLayout(q_lens, k_lens))
+    hidden = torch.ones(125, dtype=torch.bool, device=dev)
+    hidden[50 + 33 : 120] = False
+    assert torch.equal(y[hidden], clean[hidden])
+    assert bool(y[~hidden].isnan().all())
+    vv[bad] = -INF
+    y = attention_packed(q, k, vv, PackedLayout(q_lens, k_lens))
+    assert torch.equal(y[hidden], clean[hidden])
+    assert bool((y[~hidden] == -INF).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_packed_large_scores_rescale(dev, dtype):
+    """Scores that grow to about 200 along the keys: the running maximum is raised block
+    after block.  One key takes nearly the whole weight of each row, and the scores' fp32
+    rounding, some 16 ulps of 200 (2^-24 * 16 * 200 = 2e-4), moves a probability by as much."""
+    D, n = 64, 300
+    q, k, v = _packed_case(dev, [n], [n], 2, 2, D, torch.float32, seed=5)
+    k = k * torch.linspace(0.1, 10.0, n, device=dev)[:, None, None]
+    q, k, v = (x.mul(3.0 if x is q else 1.0).to(TDT[dtype]) for x in (q, k, v))
+    y = attention_packed(q, k, v, PackedLayout([n]))
+    ref, mag = attend64(q, k, v, _causal(n, n, dev))
+    half = {"f32": 0.0, "bf16": 2.0**-8, "f16": 2.0**-11}[dtype]
+    tol = 2 * half * mag + 2e-4 * mag.amax(-1, keepdim=True) + (2e-4 if dtype == "f16" else 0)
+    assert bool(((y.double() - ref).abs() <= tol).all())
+
+
+def test_packed_rows_behind_the_last_sequence(dev):
+    q, k, v = _packed_case(dev, [100], [100], 2, 2, 64, torch.bfloat16)
+    y = torch.full_like(q, 7.0)
+    lay = PackedLayout([30, 41])
+    _native.attention_packed_(q, k, v, y, lay, 0.125)
+    assert bool((y[71:] == 7.0).all())
+    z = attention_packed(q, k, v, lay, 0.125)
+    assert bool((z[71:] == 0).all()) and torch.equal(z[:71], y[:71])
+
+
+def test_packed_all_minus_inf_scores(dev):
+    """Every visible score -inf: 0 / 0, as a softmax gives; no visible key: zeros."""
+    for D in (16, 64, 24):
+        q = torch.ones(4, 1, D, device=dev)
+        k = torch.full((2, 1, D), -INF, device=dev)
+        v = torch.ones(2, 1, D, device=dev)
+        y = attention_packed(q, k, v, PackedLayout([4], [2]))
+        assert bool((y[:2] == 0).all()) and bool(y[2:].isnan().all())
+
+
+def test_packed_agrees_with_the_framework_attention(dev):
+    """One length, every head its own key head: the operator beside ops.attention."""
+    B, T, H, D = 3, 150, 4, 64
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, k, v = (torch.randn(B, T, H, D, generator=g, device=dev) for _ in range(3))
+    y = attention_packed(q.view(-1, H, D), k.view(-1, H, D), v.view(-1, H, D), PackedLayout([T] * B))
+    ref = _native.ops().attention(q, k, v, D**-0.5)
+    assert float((y.view_as(ref) - ref).abs().max()) <= 2e-5 * float(ref.abs().max())
+
+
+def test_packed_refusals(dev):
+    q, k, v = _packed_case(dev, [8], [8], 4, 2, 64, torch.bfloat16)
+    lay = PackedLayout([8], group=2)
+    with pytest.raises(ValueError, match="groups of 1"):
+        attention_packed(q, k, v, PackedLayout([8]))
+    with pytest.raises(ValueError, match="covers"):
+        attention_packed(q, k, v, PackedLayout([9], group=2))
+    with pytest.raises(ValueError, match="covers"):
+        attention_packed(q, k, v, PackedLayout([8], [9], group=2))
+    with pytest.raises(TypeError):
+        attention_packed(q, k.float(), v, lay)
+    with pytest.raises(TypeError):
+        attention_packed(q.int(), k.int(), v.int(), lay)
+    with pytest.raises(ValueError, match="scale"):
+        attention_packed(q, k, v, lay, scale=0.0)
+    with pytest.raises(ValueError, match="contiguous"):
+        attention_packed(q.transpose(1, 2).contiguous().transpose(1, 2), k, v, lay)
+    with pytest.raises(ValueError):
+        attention_packed(q[None], k[None], v[None], lay)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        attention_packed(q.float().requires_grad_(), k.float(), v.float(), lay)
+
+
+def _tree_case(dev, B, N, H, Hkv, Tcap, D, dt, seed=0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    q = torch.randn(B, N, H, D, generator=g, device=dev).to(dt)
+    pages = torch.randn(2, B, Hkv, Tcap, D, generator=g, device=dev).to(dt)
+    return q, pages[0].transpose(1, 2), pages[1].transpose(1, 2)
+
+
+def _check_tree(q, k, v, y, lens, parents, dtype):
+    N = q.size(1)
+    for b, n in enumerate(lens):
+        among = tree_seen(parents if not isinstance(parents[0], list) else parents[b])
+        seen = torch.cat([torch.ones(N, n, dtype=torch.bool), among], dim=1).to(q.device)
+        ref, mag = attend64(q[b], k[b, : n + N], v[b, : n + N], seen)
+        close(y[b], ref, mag, dtype, n + N, float(v[b].float().nan_to_num(0, 0, 0).abs().max()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("H,Hkv,D", [(4, 4, 16), (2, 1, 32), (6, 2, 64), (8, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("N,lens,Tcap", [(1, [0, 1, 31, 32, 33], 64), (1, [100, 900, 2000], 2001), (5, [0, 3, 27, 59], 64),
+                                         (31, [0, 64, 130], 200), (33, [1, 1000], 1100), (64, [0, 37, 700], 764),
+                                         (17, [5000], 6000)])
+def test_tree_matches_float64(dev, dtype, H, Hkv, D, N, lens, Tcap):
+    q, k, v = _tree_case(dev, len(lens), N, H, Hkv, Tcap, D, TDT[dtype], seed=N + D)
+    parents = some_tree(N, seed=N)
+    y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+    _check_tree(q, k, v, y, lens, parents, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
+@pytest.mark.parametrize("H,Hkv,D", [(2, 2, 1), (3, 1, 7), (2, 1, 24), (4, 2, 80), (2, 1, 256), (1, 1, 1000)])
+def test_tree_takes_every_head_dim(dev, dtype, H, Hkv, D):
+    lens, N = [0, 40, 600], 9
+    q, k, v = _tree_case(dev, 3, N, H, Hkv, 700, D, TDT[dtype], seed=D)
+    parents = some_tree(N)
+    y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+    _check_tree(q, k, v, y, lens, parents, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_tree_masks_of_each_row_and_chains(dev, dtype):
+    lens, N = [3, 200, 64], 20
+    q, k, v = _tree_case(dev, 3, N, 4, 2, 300, 64, TDT[dtype], seed=2)
+    trees = [some_tree(N, seed=s) for s in range(3)]
+    ln = torch.tensor(lens, dtype=torch.int32, device=dev)
+    y = attention_tree(q, k, v, ln, torch.stack([tree_masks(t) for t in trees]))
+    _check_tree(q, k, v, y, lens, trees, dtype)
+    y = attention_tree(q, k, v, ln)
+    _check_tree(q, k, v, y, lens, list(range(-1, N - 1)), dtype)
+    # a cache whose tokens' rows lie head by head (b, t, h, d) and one host length
+    kc, vc = k.contiguous(), v.contiguous()
+    y = attention_tree(q, kc, vc, 100)
+    _check_tree(q, k, v, y, [100] * 3, list(range(-1, N - 1)), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
+@pytest.mark.parametrize("D", [16, 64, 128, 40])
+@pytest.mark.parametrize("Tcap", [128, 3000])
+def test_tree_hidden_positions_stay_hidden(dev, dtype, D, Tcap):
+    """NaN and infinities behind a row's tokens and in tokens that others do not see;
+    empty masks and lengths beyond the cache."""
+    B, N, H = 4, 8, 2
+    lens = [0, 30, 57, Tcap - N]
+    q, k, v = (x.clone() for x in _tree_case(dev, B, N, H, H, Tcap, D, TDT[dtype], seed=4))
+    parents = [-1, 0, 0, 1, 1, 2, -1, 6]
+    masks = tree_masks(parents)
+    ln = torch.tensor(lens, dtype=torch.int32, device=dev)
+    clean = attention_tree(q, k, v, ln, masks)
+    _check_tree(q, k, v, clean, lens, parents, dtype)
+    for b, n in enumerate(lens):
+        k[b, n + N :] = NAN
+        v[b, n + N :] = INF
+        k[b, n + 2], v[b, n + 2] = NAN, NAN  # token 2: seen by itself and token 5
+        v[b, n + 6] = INF  # token 6: seen by itself and token 7
+    y = attention_tree(q, k, v, ln, masks)
+    same = [0, 1, 3, 4]
+    assert torch.equal(y[:, same], clean[:, same])
+    assert bool(y[:, [2, 5]].isnan().all()) and bool((y[:, [6, 7]] == INF).all())
+    # lengths outside the cache are taken as its ends
+    wild = torch.tensor([-5, 30, 57, 2**31 - 1], dtype=torch.int32, device=dev)
+    assert torch.equal(attention_tree(q, k, v, wild, masks)[:, same], clean[:, same])
+    # tokens that see nothing
+    empty = masks.clone()
+    empty[4] = 0
+    y = attention_tree(q, k, v, ln, empty)
+    assert bool((y[0, 4] == 0).all()) and torch.equal(y[:, [0, 1, 3]], clean[:, [0, 1, 3]])
+    # bits beyond the tokens mean nothing
+    y = attention_tree(q, k, v, ln, masks | (-1 << N))
+    assert torch.equal(y[:, same], clean[:, same])
+
+
+@pytest.mark.parametrize("D", [64, 24])
+def test_tree_replayed_with_other_lengths(dev, D):
+    """A captured call reads the lengths as they are at each replay, with eager work on the
+    same shapes between the replays."""
+    B, N, Tcap = 3, 4, 2000
+    q, k, v = _tree_case(dev, B, N, 4, 2, Tcap, D, torch.bfloat16, seed=6)
+    ln = torch.tensor([10, 20, 30], dtype=torch.int32, device=dev)
+    masks = tree_masks([-1, 0, 0, 2])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attention_tree(q, k, v, ln, masks)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = attention_tree(q, k, v, ln, masks)
+    for lens in ([0, 1500, 7], [1990, 1, 600], [10, 20, 30]):
+        ln.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        assert torch.equal(got, attention_tree(q, k, v, ln, masks))
+        _check_tree(q, k, v, got, lens, [-1, 0, 0, 2], "bf16")
+
+
+def test_packed_replayed(dev):
+    q, k, v = _packed_case(dev, [70, 200], [70, 200], 4, 4, 64, torch.bfloat16)
+    lay = PackedLayout([70, 200])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attention_packed(q, k, v, lay)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = attention_packed(q, k, v, lay)
+    for s in range(3):
+        q.copy_(torch.randn(q.shape, device=dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, attention_packed(q, k, v, lay))
+
+
+def test_tree_past_32_bit_offsets(dev):
+    """A cache page of more than 2^31 elements: the last row's keys lie beyond it."""
+    B, Tcap, D = 2, 150000, 128
+    big = torch.zeros(B, Tcap, 60, D, dtype=torch.bfloat16, device=dev)  # 2.3e9 elements, 1.15e9 a row
+    k = big[:, :, 7:8]
+    v = big[:, :, 33:34]
+    g = torch.Generator(device=dev).manual_seed(0)
+    k.copy_(torch.randn(k.shape, generator=g, device=dev))
+    v.copy_(torch.randn(v.shape, generator=g, device=dev))
+    q = torch.randn(B, 2, 4, D, generator=g, device=dev).bfloat16()
+    lens = [149000, 149998]
+    y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev))
+    _check_tree(q, k, v, y, lens, [-1, 0], "bf16")
+    y = attention_packed(q.view(4, 4, D), k.reshape(-1, 1, D), v.reshape(-1, 1, D),
+                         PackedLayout([2, 2], [150000, 150000], group=4))
+    _check_packed(q.view(4, 4, D), k.reshape(-1, 1, D), v.reshape(-1, 1, D), y, [2, 2], [150000, 150000], "bf16")
+    # the packed rows themselves 60 heads apart
+    flat = big.view(B * Tcap, 60, D)
+    y2 = attention_packed(q.view(4, 4, D), flat[:, 7:8], flat[:, 33:34],
+                          PackedLayout([2, 2], [150000, 150000], group=4))
+    assert torch.equal(y, y2)
+
+
+def test_tree_refusals(dev):
+    q, k, v = _tree_case(dev, 2, 3, 4, 2, 40, 64, torch.bfloat16)
+    ln = torch.tensor([1, 2], dtype=torch.int32, device=dev)
+    ok = attention_tree(q, k, v, ln)
+    assert ok.shape == q.shape
+    with pytest.raises(ValueError, match="lengths"):
+        attention_tree(q, k, v, ln.long())
+    with pytest.raises(ValueError, match="lengths"):
+        attention_tree(q, k, v, ln[:1])
+    with pytest.raises(ValueError, match="lengths"):
+        attention_tree(q, k, v, ln.cpu())
+    with pytest.raises(ValueError, match="cached positions"):
+        attention_tree(q, k, v, 38)
+    with pytest.raises(ValueError, match="masks"):
+        attention_tree(q, k, v, ln, torch.zeros(4, dtype=torch.int64, device=dev))
+    with pytest.raises(ValueError, match="masks"):
+        attention_tree(q, k, v, ln, torch.zeros(3, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError, match="heads"):
+        attention_tree(q[:, :, :3], k, v, ln)
+    with pytest.raises(ValueError):
+        attention_tree(q, k[:1], v[:1], ln)
+    with pytest.raises(ValueError, match="does not hold"):
+        attention_tree(q, k[:, :2], v[:, :2], 0)
+    with pytest.raises(TypeError):
+        attention_tree(q, k.float(), v.float(), ln)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        attention_tree(q.requires_grad_(), k, v, ln)
