@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void seq_vec_kernel(const SeqArgs a) {
   using A = typename S::type;
   constexpr int KPW = 64 / LPK;
   SeqPiece p;
-  if (!seq_piece<TREE>(a, p)) return;
+  if (!seq_piece<TREE>(a, 0, p)) return;
   const int lane = threadIdx.x & 63, kl = lane / LPK, dl = lane % LPK;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* kp = static_cast<const T*>(a.k) + p.b * a.kb + p.k0 * a.kt + (int64_t)p.kvh * a.kh;
@@ -164,7 +164,8 @@ __global__ __launch_bounds__(256) void seq_join_kernel(const SeqArgs a, const in
   bool bad = false;
   for (int s = lane; s < used; s += 64) {
     const A ms = ml[2 * s];
-    bad = bad || ms != ms;
+    const A ls = ml[2 * s + 1];
+    bad = bad || ms != ms || ls != ls;  // a NaN score
     m = ms > m ? ms : m;
   }
 #pragma unroll
@@ -215,7 +216,8 @@ int launch_vec_any(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
   return launch_vec<f16_t, TREE>(a, grid, s);
 }
 
-constexpr int kWideRows = 128;  // rows of a wide tile
+constexpr int kWideRows = 128;   // rows of a wide tile
+constexpr int kNarrowRows = 32;  // most rows of a narrow one
 constexpr int kVecRows = 32;    // rows of a workgroup of the vector kernel over a tree
 
 // Workgroups that a split aims at: two for each of the 256 CUs.  A split's length is a
@@ -283,19 +285,26 @@ extern "C" int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, i
     nk += lk[s];
     DG_REQUIRE(nq <= 0x7fffffff && nk <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 rows");
   }
-  int64_t n = 0;
-  for (int64_t s = 0; s < S; ++s) n += (lq[s] * group + kWideRows - 1) / kWideRows;
+  int64_t wide = 0, narrow = 0;
+  for (int64_t s = 0; s < S; ++s) {
+    const int64_t rows = lq[s] * group, rest = rows % kWideRows;
+    wide += rows / kWideRows + (rest > kNarrowRows);
+    narrow += rest > 0 && rest <= kNarrowRows;
+  }
+  const int64_t n = wide + narrow;
   DG_REQUIRE(n <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 tiles");
-  counts[0] = n;
-  counts[1] = 0;
+  counts[0] = wide;
+  counts[1] = narrow;
   if (tiles == nullptr) return DG_OK;
   DG_REQUIRE(cap >= n, DG_EINVAL, "packed_plan: room for %lld tiles, %lld needed", (long long)cap, (long long)n);
-  int64_t at = 0, q0 = 0, k0 = 0;
+  int64_t at = 0, at_narrow = wide, q0 = 0, k0 = 0;
   for (int64_t s = 0; s < S; ++s) {
     const int64_t rows = lq[s] * group;
-    for (int64_t r = 0; r < rows; r += kWideRows)
-      tiles[at++] = dg_packed_tile{(int32_t)q0, (int32_t)lq[s], (int32_t)k0, (int32_t)lk[s], (int32_t)r,
-                                   (int32_t)std::min<int64_t>(kWideRows, rows - r), {0, 0}};
+    for (int64_t r = 0; r < rows; r += kWideRows) {
+      const int64_t some = std::min<int64_t>(kWideRows, rows - r);
+      tiles[some <= kNarrowRows ? at_narrow++ : at++] = dg_packed_tile{
+          (int32_t)q0, (int32_t)lq[s], (int32_t)k0, (int32_t)lk[s], (int32_t)r, (int32_t)some, {0, 0}};
+    }
     q0 += lq[s];
     k0 += lk[s];
   }
@@ -326,6 +335,8 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   a.nq = Nq; a.nk = Nk;
   a.nsplit = 1;
   a.rows_per_wg = kWideRows;
+  if (seq_mfma_applicable(a, dtype, false))
+    return launch_seq_mfma_packed(a, dtype, n_wide, n_narrow, static_cast<hipStream_t>(stream));
   return launch_vec_any<false>(a, dtype, dim3((unsigned)(n_wide + n_narrow), (unsigned)Hkv),
                                static_cast<hipStream_t>(stream));
 }
@@ -364,7 +375,8 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   a.B = B; a.N = N; a.Tcap = Tcap;
   a.len = len; a.lens = lens;
   a.masks = masks; a.mask_b = mask_b;
-  const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, kVecRows);
+  const bool mfma = seq_mfma_applicable(a, dtype, true);
+  const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, mfma ? seq_mfma_tree_rows(N * a.G) : kVecRows);
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
   if (t.nsplit > 1) {
     DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,
@@ -376,7 +388,8 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   const int64_t blocks = (int64_t)B * Hkv * t.nrb * t.nsplit;
   DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int rc = launch_vec_any<true>(a, dtype, dim3((unsigned)blocks), s);
+  const int rc = mfma ? launch_seq_mfma_tree(a, dtype, (unsigned)blocks, s)
+                      : launch_vec_any<true>(a, dtype, dim3((unsigned)blocks), s);
   if (rc != DG_OK || t.nsplit == 1) return rc;
   const int64_t rows = (int64_t)B * H * N;
   DG_REQUIRE((rows + 3) / 4 <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");

@@ -1,0 +1,595 @@
+// Packed attention and token trees over a cache on the matrix cores: head_dim 16, 32, 64
+// and 128 in bf16, fp16 and fp32 (dg_attn_seq.hip has the entry points and the kernel for
+// every other shape).
+//
+// A workgroup is WAVES wavefronts over one key head of one sequence: RT tiles of 32
+// (query, head of the group) rows by KS = WAVES / RT groups of keys.  With few rows (RT 1:
+// a decode step, a small tree) the waves split the keys and join their softmax states at
+// the end; with many (RT 4: a prompt) they share each key tile.  Keys stream through two
+// LDS stages per group, copied there straight from global memory (buffer_load_dwordx4 ...
+// lds) while the stage before is computed: K and V rows with their 16-byte pieces
+// XOR-swizzled.  Both products are transposed so that a lane's statistics belong to one row:
+//
+//   S^T (32 keys x 32 rows) = K Q^T     K from LDS, Q^T in registers for the whole loop
+//   O^T (D x 32 rows)      += V^T P^T   P^T is S^T's accumulator registers as they are
+//
+// 16-bit data: v_mfma_f32_32x32x16_{bf16,f16}, V^T through the transposing LDS read;
+// probabilities are rounded to the data's type once, for the second product alone (the
+// row sums add them in fp32).  fp32: v_mfma_f32_32x32x2_f32 throughout.  Lane l (half hh =
+// l / 32) holds, in register r of a 32x32 block, row 8 (r / 4) + 4 hh + r % 4 of column
+// l % 32, its row of the batch.
+//
+// The exponent's offset is a whole number of log2 units, raised only where a row's maximum
+// outgrows it by more than kLazyLog2: rescaling by a power of two is exact, so a row's bits
+// do not depend on when its neighbours in the tile made it rescale.  Scores are masked
+// only in key blocks that some row of the wave sees part of; there a value that is not
+// finite leaves the product (0 * inf is NaN) and is added to the rows that see it.
+#include "dg_seq.h"
+#include "dg_prefill.h"
+
+namespace dg {
+
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 sbf16x8_t;
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 sf16x8_t;
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct SeqMma;
+template <>
+struct SeqMma<bf16_t> {
+  using vec8 = sbf16x8_t;
+  static constexpr uint32_t kExp = 0x7f80u;
+  __device__ static floatx16_t mma(vec8 a, vec8 b, floatx16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct SeqMma<f16_t> {
+  using vec8 = sf16x8_t;
+  static constexpr uint32_t kExp = 0x7c00u;
+  __device__ static floatx16_t mma(vec8 a, vec8 b, floatx16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct SeqMma<float> {
+  using vec8 = float;  // unused
+  static constexpr uint32_t kExp = 0x7f800000u;
+};
+
+// Workgroup shapes.  Two stages of K and V for every key group: up to 128 KB of LDS (one
+// workgroup a CU, 64 KB of keys in flight) where the waves split the keys.
+template <typename T, int D, int RT>
+struct SeqCfg {
+  static constexpr int ES = (int)sizeof(T);
+  static constexpr int WAVES = (ES == 4 && D == 128 && RT == 1) ? 2 : 4;
+  static constexpr int KS = WAVES / RT;
+  // 32-key blocks of a stage
+  static constexpr int MB = D * ES <= 64 ? 2 : (ES == 2 && D == 64 && RT == 4) ? 2 : 1;
+  static constexpr int BN = 32 * MB;
+  static constexpr int PPR = D * ES / 16;        // 16-byte pieces of a row
+  static constexpr int RPD = 64 / PPR;           // rows a wave-wide copy covers
+  static constexpr int NDMA = BN / RPD;          // copies of a K (or V) tile
+  static constexpr int TILE = BN * D;            // elements
+  static constexpr int NC = D / 16;              // 16-bit: contraction steps of S^T
+  static constexpr int QC = D / 2;               // fp32: ... of two dims
+  static constexpr int NB = D < 32 ? 1 : D / 32; // 32-row blocks of O^T (D = 16 fills half of one)
+  static constexpr int JOIN = (NB * 16 + 2) * 64;  // floats of a wave's state
+  static_assert(NDMA >= 1 && KS >= 1, "tile split");
+  // the joined states and the outputs reuse the stages: writers alternate between the two
+  static_assert((((KS - 1) * RT + 1) / 2) * JOIN * 4 <= KS * 2 * TILE * ES, "joined states fit a stage");
+  static_assert(ES == 4 || ((RT + 1) / 2) * 32 * D <= KS * 2 * TILE, "outputs fit a stage");
+  // workgroups a CU that the registers must allow
+  static constexpr int WGS = RT == 4 ? (ES == 4 ? (D <= 64 ? 4 : 2) : D <= 64 ? 4 : 3) : (D * ES <= 128 ? 2 : 1);
+};
+
+template <int PPR, int ES>
+__device__ __forceinline__ int seq_swz(int r) {
+  if constexpr (ES == 4) return r & (PPR >= 16 ? 15 : PPR - 1);
+  else if constexpr (PPR == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+  else if constexpr (PPR == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (PPR == 4) return (r >> 2) & 3;
+  else return 0;
+}
+
+template <typename T, int D, int RT>
+constexpr int seq_threads() {
+  return 64 * SeqCfg<T, D, RT>::WAVES;
+}
+template <typename T, int D, int RT>
+constexpr int seq_wgs_per_cu() {
+  return SeqCfg<T, D, RT>::WGS;
+}
+
+template <typename T, int D, int RT, bool TREE>
+__global__ __launch_bounds__((seq_threads<T, D, RT>()), (seq_wgs_per_cu<T, D, RT>()))
+void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
+  using C = SeqCfg<T, D, RT>;
+  using M = SeqMma<T>;
+  using vec8 = typename M::vec8;
+  constexpr int ES = C::ES, KS = C::KS, MB = C::MB, BN = C::BN, PPR = C::PPR, NB = C::NB, TILE = C::TILE;
+  constexpr bool F32 = ES == 4;
+  constexpr float kNone = kNegInf;
+
+  __shared__ __attribute__((aligned(16))) T kv0[KS * 2 * TILE];
+  __shared__ __attribute__((aligned(16))) T kv1[KS * 2 * TILE];
+
+  SeqPiece pc;
+  if (!seq_piece<TREE>(a, tile0, pc)) return;  // whole workgroups, before any barrier
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rt = wv % RT, kg = wv / RT;
+  const int hh = lane >> 5, r32 = lane & 31;
+
+  // the lane's row: rows past the piece's repeat its last one and are never stored
+  const int wrow = pc.row0 + 32 * rt, rend = pc.row0 + pc.rows;
+  const bool live = wrow < rend;
+  const int row = min(wrow + r32, rend - 1);
+  const int qi = row / a.G, qg = row - qi * a.G;
+  const int head = pc.kvh * a.G + qg;
+  // keys below `open` every row of the wave sees, from `wend` on none does
+  int open, wend;
+  uint64_t mask = 0;
+  if constexpr (TREE) {
+    open = pc.own;
+    wend = pc.kend;
+    mask = tree_mask(a, pc.b, qi);
+  } else {
+    open = min(wrow, rend - 1) / a.G + pc.off + 1;
+    wend = min(wrow + 31, rend - 1) / a.G + pc.off + 1;
+  }
+  if (!live) wend = 0;
+
+  const T* kp = static_cast<const T*>(a.k) + pc.b * a.kb + pc.k0 * a.kt + (int64_t)pc.kvh * a.kh;
+  const T* vp = static_cast<const T*>(a.v) + pc.b * a.vb + pc.k0 * a.vt + (int64_t)pc.kvh * a.vh;
+
+  // ---- global -> LDS copy of a stage's keys -----------------------------------------
+  // The RT waves of a key group share its copies: lane l of copy i fills slot l % PPR of
+  // row l / PPR of rows i * RPD ..  The buffer resource starts at the stage's first key,
+  // with 64-bit arithmetic, and ends behind the piece's last: rows past it read as zeros.
+  int ko[(C::NDMA + RT - 1) / RT], vo[(C::NDMA + RT - 1) / RT];
+#pragma unroll
+  for (int n = 0; n < (C::NDMA + RT - 1) / RT; ++n) {
+    const int r = (n * RT + rt) * C::RPD + lane / PPR;
+    const int piece = (lane % PPR) ^ seq_swz<PPR, ES>(r);
+    ko[n] = r * (int)a.kt * ES + 16 * piece;
+    vo[n] = r * (int)a.vt * ES + 16 * piece;
+  }
+  auto copy_stage = [&](T* st, int k0) __attribute__((always_inline)) {
+    T* const ks = st + kg * 2 * TILE;
+    const int left = min(BN, pc.kend - k0);
+    const int kn = left <= 0 ? 0 : (int)((left - 1) * a.kt + D) * ES;
+    const int vn = left <= 0 ? 0 : (int)((left - 1) * a.vt + D) * ES;
+    const __amdgpu_buffer_rsrc_t krs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + (int64_t)k0 * a.kt), 0, kn, kBufferWord3);
+    const __amdgpu_buffer_rsrc_t vrs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp + (int64_t)k0 * a.vt), 0, vn, kBufferWord3);
+#pragma unroll
+    for (int n = 0; n < (C::NDMA + RT - 1) / RT; ++n) {
+      const int i = n * RT + rt;
+      if (C::NDMA % RT != 0 && i >= C::NDMA) break;  // wave-uniform
+      lds_copy16_buf(krs, ko[n], 0, ks + i * C::RPD * D);
+      lds_copy16_buf(vrs, vo[n], 0, ks + TILE + i * C::RPD * D);
+    }
+  };
+  // this wave's copies have landed; the waves of a group also wait for each other
+  auto stage_ready = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0);
+    if constexpr (RT > 1) __builtin_amdgcn_s_barrier();
+  };
+
+  // ---- the rows ----------------------------------------------------------------------
+  const T* qp = static_cast<const T*>(a.q) + pc.b * a.qb + (pc.q0 + qi) * a.qt + (int64_t)head * a.qh;
+  vec8 qf[F32 ? C::QC : C::NC];
+  if constexpr (F32) {
+#pragma unroll
+    for (int m = 0; m < C::QC / 4; ++m) {
+      const f32x4_t x = reinterpret_cast<const f32x4_t*>(qp + C::QC * hh)[m];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[4 * m + e] = x[e];
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < C::NC; ++c)
+      qf[c] = __builtin_bit_cast(vec8, *reinterpret_cast<const u32x4_t*>(qp + 16 * c + 8 * hh));
+  }
+
+  const int kstep = KS * BN;
+  const int kfirst = pc.kbeg + kg * BN;  // this group's first stage
+  const int nstage = (pc.kend - pc.kbeg + kstep - 1) / kstep;
+  if (nstage > 0) copy_stage(kv0, kfirst);
+
+  floatx16_t o[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[nb][r] = 0.f;
+  float mo = kNone, l = 0.f;  // the exponent's offset (log2 units, whole) and this lane's sum
+
+  // per-lane parts of the transposing reads of V (16-bit)
+  const int g16 = lane >> 4, t16 = lane & 15;
+  int voff[2][NB];
+  if constexpr (!F32) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = 8 * u + 4 * (g16 >> 1) + (t16 >> 2);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int col = (32 * nb + 16 * (g16 & 1) + 4 * (t16 & 3)) & (D - 1);  // D = 16: both halves read its dims
+        voff[u][nb] = r * D + 8 * ((col >> 3) ^ seq_swz<PPR, ES>(r)) + (col & 7);
+      }
+    }
+  }
+  const int kswz = seq_swz<PPR, ES>(r32);
+
+  // which of the 32 keys from kb on this lane's row sees
+  auto visible = [&](int kb) __attribute__((always_inline)) -> uint32_t {
+    if constexpr (TREE) {
+      const int d = pc.own - kb;
+      if (d >= 32) return ~0u;
+      if (d >= 0) return (uint32_t)(((uint64_t)mask << d) | ((1ull << d) - 1));
+      return -d >= 64 ? 0u : (uint32_t)(mask >> -d);
+    } else {
+      const int lim = qi + pc.off - kb;
+      return lim < 0 ? 0u : lim >= 31 ? ~0u : (2u << lim) - 1;
+    }
+  };
+  // whether the V rows of a 32-key block hold only finite values
+  auto block_finite = [&](const T* vs) __attribute__((always_inline)) -> bool {
+    const u32x4_t* p = reinterpret_cast<const u32x4_t*>(vs);
+    bool fine = true;
+    if constexpr (F32) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 32 * D * ES / 1024; ++i) {
+        const u32x4_t w = p[64 * i + lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, w[e] & 0x7fffffffu);
+      }
+      fine = top < M::kExp;
+    } else {
+      u16x2_t top = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 32 * D * ES / 1024; ++i) {
+        const u32x4_t w = p[64 * i + lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w[e] & 0x7fff7fffu));
+      }
+      fine = top[0] < M::kExp && top[1] < M::kExp;
+    }
+    return __builtin_amdgcn_ballot_w64(!fine) == 0;
+  };
+  auto not_finite = [](uint32_t bits) __attribute__((always_inline)) { return (bits & M::kExp) == M::kExp; };
+
+  auto compute = [&](const T* st, int k0) __attribute__((always_inline)) {
+    const T* Ks = st + kg * 2 * TILE;
+    const T* Vs = Ks + TILE;
+    floatx16_t s[MB];
+    bool partial[MB];
+    // a block past the wave's last key has zeros for K: no product, no weight
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
+      if constexpr (F32) {
+        const float* krow = reinterpret_cast<const float*>(Ks) + (32 * mb + r32) * D;
+#pragma unroll
+        for (int p = 0; p < C::QC / 4; ++p) {
+          const f32x4_t kf = *reinterpret_cast<const f32x4_t*>(krow + 4 * (((PPR / 2) * hh + p) ^ kswz));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[4 * p + e], s[mb], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < C::NC; ++c) {
+          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(Ks + (32 * mb + r32) * D + 8 * ((2 * c + hh) ^ kswz));
+          s[mb] = M::mma(__builtin_bit_cast(vec8, kf), qf[c], s[mb]);
+        }
+      }
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const int kb = k0 + 32 * mb;
+      partial[mb] = kb + 32 > open;
+      if (partial[mb]) {
+        const uint32_t vis = visible(kb) >> (4 * hh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((vis >> (8 * (r >> 2) + (r & 3))) & 1u)) s[mb][r] = kNone;
+      }
+    }
+    float mt = s[0][0];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int r = mb == 0 ? 1 : 0; r < 16; ++r) mt = fmaxf(mt, s[mb][r]);
+    mt = half_pair_max(mt) * a.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(mt > mo + kLazyLog2) != 0) {
+      const float mn = mt > mo ? fmaxf(__builtin_floorf(mt), mo) : mo;
+      const float f = mo == kNone ? 0.f : __builtin_amdgcn_exp2f(mo - mn);
+      mo = mn;
+      l *= f;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nb][r] *= f;
+    }
+    const float moff = mo == kNone ? 0.f : mo;  // no key yet: every score here is -inf
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const T* vb = Vs + 32 * mb * D;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[mb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][r], a.scale_log2, -moff));
+        l += s[mb][r];
+      }
+      const bool dirty = partial[mb] && !block_finite(vb);
+      if constexpr (F32) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const int key = 8 * (c >> 2) + 4 * hh + (c & 3);
+          const float* vrow = reinterpret_cast<const float*>(vb) + key * D;
+          const int ksw = seq_swz<PPR, ES>(key);
+          float vf[NB];
+          if constexpr (D == 16) {
+            vf[0] = vrow[4 * (((r32 & 15) >> 2) ^ ksw) + (r32 & 3)];
+          } else if constexpr (D == 32) {
+            vf[0] = vrow[4 * ((r32 >> 2) ^ ksw) + (r32 & 3)];
+          } else if constexpr (D == 64) {
+            const u32x2_t x = *reinterpret_cast<const u32x2_t*>(vrow + 4 * ((r32 >> 1) ^ ksw) + 2 * (r32 & 1));
+            vf[0] = __uint_as_float(x[0]);
+            vf[1] = __uint_as_float(x[1]);
+          } else {
+            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(vrow + 4 * (r32 ^ ksw));
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) vf[nb] = x[nb];
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            if (dirty && not_finite(__float_as_uint(vf[nb]))) vf[nb] = 0.f;
+            o[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[nb], s[mb][c], o[nb], 0, 0, 0);
+          }
+        }
+      } else {
+        vec8 pf[2];
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = pack_pair<T>(s[mb][8 * c2 + 2 * i], s[mb][8 * c2 + 2 * i + 1]);
+          pf[c2] = __builtin_bit_cast(vec8, u32x4_t{w[0], w[1], w[2], w[3]});
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int c2 = 0; c2 < 2; ++c2) {
+            const uint2 lo = lds_read_tr16(vb + 16 * c2 * D + voff[0][nb]);
+            const uint2 hi = lds_read_tr16(vb + 16 * c2 * D + voff[1][nb]);
+            u32x4_t w = {lo.x, lo.y, hi.x, hi.y};
+            if (dirty) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (not_finite(w[e])) w[e] &= 0xffff0000u;
+                if (not_finite(w[e] >> 16)) w[e] &= 0x0000ffffu;
+              }
+            }
+            o[nb] = M::mma(__builtin_bit_cast(vec8, w), pf[c2], o[nb]);
+          }
+      }
+      if (dirty) {
+        // the values that left the product, added to the rows that see them
+        const uint32_t vis = visible(k0 + 32 * mb);
+        for (int j = 0; j < 32; ++j) {
+          const T* vrow = vb + j * D;
+          const int ksw = seq_swz<PPR, ES>(32 * mb + j);
+          const bool sees = (vis >> j) & 1u;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int r = 0; r < (D == 16 ? 8 : 16); ++r) {
+              const int i = 8 * (r >> 2) + 4 * hh + (r & 3);
+              const int d = F32 ? NB * i + nb : 32 * nb + i;
+              constexpr int EPP = 16 / ES;
+              const T x = vrow[EPP * ((d / EPP) ^ ksw) + d % EPP];
+              const float xv = to_f32(x);
+              if (sees && !(__builtin_fabsf(xv) < __builtin_huge_valf())) o[nb][r] += xv;
+            }
+        }
+      }
+    }
+  };
+
+  stage_ready();
+  for (int t = 0; t < nstage; t += 2) {
+    const int k0 = kfirst + t * kstep;
+    if (t + 1 < nstage) copy_stage(kv1, k0 + kstep);
+    if (k0 < wend) compute(kv0, k0);
+    stage_ready();  // stage 1 filled; every wave is done with stage 0
+    if (t + 1 >= nstage) break;
+    if (t + 2 < nstage) copy_stage(kv0, k0 + 2 * kstep);
+    if (k0 + kstep < wend) compute(kv1, k0 + kstep);
+    stage_ready();
+  }
+  l = half_pair_sum(l);
+
+  // ---- the key groups' states joined ---------------------------------------------------
+  if constexpr (KS > 1) {
+    __syncthreads();
+    auto slot = [&](int w) __attribute__((always_inline)) {
+      return reinterpret_cast<float*>((w & 1) ? kv1 : kv0) + (w >> 1) * C::JOIN;
+    };
+    if (kg > 0) {
+      float* f = slot((kg - 1) * RT + rt);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) f[(16 * nb + r) * 64 + lane] = o[nb][r];
+      f[NB * 16 * 64 + lane] = mo;
+      f[(NB * 16 + 1) * 64 + lane] = l;
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int g = 1; g < KS; ++g) {
+      const float* f = slot((g - 1) * RT + rt);
+      const float m2 = f[NB * 16 * 64 + lane], l2 = f[(NB * 16 + 1) * 64 + lane];
+      const float mn = fmaxf(mo, m2);
+      const float f1 = mo == kNone ? 0.f : __builtin_amdgcn_exp2f(mo - mn);
+      const float f2 = m2 == kNone ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
+      mo = mn;
+      // a state without a key has zeros; l takes a NaN along
+      l = l * f1 + l2 * f2;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nb][r] = o[nb][r] * f1 + f[(16 * nb + r) * 64 + lane] * f2;
+    }
+    // the outputs go through the same LDS: reads above come first
+    if constexpr (!F32) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  if (!live) return;
+
+  // ---- the result ----------------------------------------------------------------------
+  const bool stored = wrow + r32 < rend;
+  if (TREE && a.nsplit > 1) {
+    const int64_t part = ((pc.b * a.Hkv + pc.kvh) * (int64_t)(a.N * a.G) + row) * a.nsplit + pc.split;
+    if (stored) {
+      float* wo = static_cast<float*>(a.ws_o) + part * D;
+      if constexpr (F32 && NB > 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = NB * (8 * (r >> 2) + 4 * hh + (r & 3));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) wo[d + nb] = o[nb][r];
+        }
+      } else {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int g = 0; g < (D == 16 ? 2 : 4); ++g)
+            *reinterpret_cast<f32x4_t*>(wo + 32 * nb + 8 * g + 4 * hh) =
+                f32x4_t{o[nb][4 * g], o[nb][4 * g + 1], o[nb][4 * g + 2], o[nb][4 * g + 3]};
+      }
+      if (hh == 0) {
+        float* ml = static_cast<float*>(a.ws_ml) + 2 * part;
+        ml[0] = mo;
+        ml[1] = l;
+      }
+    }
+    return;
+  }
+  // no key at all: zeros; keys whose scores are all -inf: 0 / 0, as a softmax gives
+  const bool none = TREE ? pc.own == 0 && mask == 0 : qi + pc.off < 0;
+  const float inv = none ? 0.f : 1.0f / l;
+  if constexpr (F32) {
+    if (!stored) return;
+    float* yp = static_cast<float*>(a.y) + pc.b * a.yb + (pc.q0 + qi) * a.yt + (int64_t)head * a.yh;
+    // register 4g + e of block nb is dim NB (8 g + 4 hh + e) + nb
+#pragma unroll
+    for (int g = 0; g < (D == 16 ? 2 : 4); ++g) {
+      float w[4 * NB];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) w[NB * e + nb] = none ? 0.f : o[nb][4 * g + e] * inv;
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+        *reinterpret_cast<f32x4_t*>(yp + NB * (8 * g + 4 * hh) + 4 * x) =
+            f32x4_t{w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]};
+    }
+  } else {
+    // through LDS, so that a store writes whole rows; the wave's own rows, no barrier
+    constexpr int RPS = 64 / PPR;  // rows a wave-wide store covers
+    T* stg = ((rt & 1) ? kv1 : kv0) + (rt >> 1) * 32 * D;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int g = 0; g < (D == 16 ? 2 : 4); ++g) {
+        const uint32_t w0 = none ? 0u : pack_pair<T>(o[nb][4 * g] * inv, o[nb][4 * g + 1] * inv);
+        const uint32_t w1 = none ? 0u : pack_pair<T>(o[nb][4 * g + 2] * inv, o[nb][4 * g + 3] * inv);
+        const int sl = (4 * nb + g) ^ (r32 & (PPR - 1));
+        *reinterpret_cast<u32x2_t*>(stg + r32 * D + 8 * sl + 4 * hh) = u32x2_t{w0, w1};
+      }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int piece = lane % PPR;
+#pragma unroll
+    for (int p = 0; p < 32 / RPS; ++p) {
+      const int r = p * RPS + lane / PPR;
+      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(stg + r * D + 8 * (piece ^ (r & (PPR - 1))));
+      const int rr = wrow + r;
+      if (rr < rend) {
+        const int i = rr / a.G, h = pc.kvh * a.G + (rr - i * a.G);
+        T* yp = static_cast<T*>(a.y) + pc.b * a.yb + (pc.q0 + i) * a.yt + (int64_t)h * a.yh;
+        *reinterpret_cast<u32x4_t*>(yp + 8 * piece) = w;
+      }
+    }
+  }
+}
+
+namespace {
+
+template <typename T, int D, int RT, bool TREE>
+int launch_seq(const SeqArgs& a, int64_t tile0, dim3 grid, hipStream_t s) {
+  hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, TREE>), grid, dim3(64 * SeqCfg<T, D, RT>::WAVES), 0, s, a, tile0);
+  return check_launch(TREE ? "seq_mfma_tree_kernel" : "seq_mfma_packed_kernel");
+}
+
+template <typename T, int RT, bool TREE>
+int launch_seq_d(const SeqArgs& a, int64_t tile0, dim3 grid, hipStream_t s) {
+  if (a.D == 16) return launch_seq<T, 16, RT, TREE>(a, tile0, grid, s);
+  if (a.D == 32) return launch_seq<T, 32, RT, TREE>(a, tile0, grid, s);
+  if (a.D == 64) return launch_seq<T, 64, RT, TREE>(a, tile0, grid, s);
+  return launch_seq<T, 128, RT, TREE>(a, tile0, grid, s);
+}
+
+template <int RT, bool TREE>
+int launch_seq_t(const SeqArgs& a, int dtype, int64_t tile0, dim3 grid, hipStream_t s) {
+  if (dtype == DG_F32) return launch_seq_d<float, RT, TREE>(a, tile0, grid, s);
+  if (dtype == DG_BF16) return launch_seq_d<bf16_t, RT, TREE>(a, tile0, grid, s);
+  return launch_seq_d<f16_t, RT, TREE>(a, tile0, grid, s);
+}
+
+}  // namespace
+
+// head_dim 16, 32, 64 and 128 in 16-bit types and fp32, rows aligned to the 16-byte loads
+// and stores, and a stage's rows (up to 64) within 2^31 bytes of each other.
+bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree) {
+  if (dtype == DG_F64 || (a.D != 16 && a.D != 32 && a.D != 64 && a.D != 128)) return false;
+  const int64_t es = dtype_bytes(dtype);
+  auto rows = [&](const void* p, int64_t b, int64_t t, int64_t h) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (!tree || b * es % 16 == 0) && t * es % 16 == 0 && h * es % 16 == 0;
+  };
+  const int64_t most = ((int64_t)1 << 31) / (64 * es) - a.D;
+  if (a.kt < 0 || a.vt < 0 || a.kt > most || a.vt > most) return false;
+  return rows(a.q, a.qb, a.qt, a.qh) && rows(a.k, a.kb, a.kt, a.kh) && rows(a.v, a.vb, a.vt, a.vh) &&
+         rows(a.y, a.yb, a.yt, a.yh);
+}
+
+// Rows of a workgroup: 32, 64 or 128, the smallest that holds a row's (token, head) rows.
+int seq_mfma_tree_rows(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s) {
+  const dim3 grid(blocks);
+  if (a.rows_per_wg == 32) return launch_seq_t<1, true>(a, dtype, 0, grid, s);
+  if (a.rows_per_wg == 64) return launch_seq_t<2, true>(a, dtype, 0, grid, s);
+  return launch_seq_t<4, true>(a, dtype, 0, grid, s);
+}
+
+int launch_seq_mfma_packed(SeqArgs a, int dtype, int64_t n_wide, int64_t n_narrow, hipStream_t s) {
+  if (n_wide > 0) {
+    a.rows_per_wg = 128;
+    const int rc = launch_seq_t<4, false>(a, dtype, 0, dim3((unsigned)n_wide, (unsigned)a.Hkv), s);
+    if (rc != DG_OK) return rc;
+  }
+  if (n_narrow > 0) {
+    a.rows_per_wg = 32;
+    return launch_seq_t<1, false>(a, dtype, n_wide, dim3((unsigned)n_narrow, (unsigned)a.Hkv), s);
+  }
+  return DG_OK;
+}
+
+}  // namespace dg

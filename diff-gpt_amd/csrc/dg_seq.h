@@ -56,11 +56,11 @@ struct SeqPiece {
   int kvh, split;
 };
 
-// The piece of this workgroup; false where there is nothing to do.  Nothing a table or
+// The piece of this workgroup (packed: tile tile0 + blockIdx.x); false where there is nothing to do.  Nothing a table or
 // a length in device memory says takes an access outside q, k, v and y: tiles that do
 // not lie inside them are left out, lengths beyond the cache are taken as its end.
 template <bool TREE>
-__device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
+__device__ __forceinline__ bool seq_piece(const SeqArgs& a, int64_t tile0, SeqPiece& p) {
   if constexpr (TREE) {
     int64_t u = (int64_t)blockIdx.x;
     p.split = (int)(u % a.nsplit);
@@ -79,7 +79,7 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
     p.q0 = p.k0 = 0;
     return p.kbeg < p.kend;
   } else {
-    const dg_packed_tile t = a.tiles[blockIdx.x];
+    const dg_packed_tile t = a.tiles[tile0 + blockIdx.x];
     p.kvh = blockIdx.y;
     p.split = 0;
     p.b = 0;
@@ -107,11 +107,11 @@ __device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n
   return (uint64_t)a.masks[b * a.mask_b + n] & all;
 }
 
-// dg_attn_seq_mfma.hip: whether it takes the shape, the rows of its wide and narrow
-// workgroups, and its launches
+// dg_attn_seq_mfma.hip: whether it takes the shape, the rows of a workgroup over so many
+// (token, head) rows, and its launches
 bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree);
-int seq_mfma_tree_rows(const SeqArgs& a, int dtype);
+int seq_mfma_tree_rows(int rows);
 int launch_seq_mfma_packed(SeqArgs a, int dtype, int64_t n_wide, int64_t n_narrow, hipStream_t s);
-int launch_seq_mfma_tree(const SeqArgs& a, int dtype, hipStream_t s);
+int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s);
 
 }  // namespace dg
