@@ -1,9 +1,23 @@
 // Log probabilities of given tokens, entropy and the most likely alternatives
-// (dg_token_logprobs): one pass over the logits.
+// (dg_token_logprobs), reading the logits once.
 //
-// A wavefront takes a row.  The softmax keeps, per lane, a running maximum m, the sum s of
-// e^(x - m) and the sum t of (x - m) e^(x - m); raising m by d turns t into
-// e^-d (t - d s).  Then log p(id) = x[id] - m - log s and the entropy is log s - t / s.
+// With m the row's maximum, s the sum of e^(x - m) and t that of (x - m) e^(x - m):
+// log p(id) = x[id] - m - log s, and the entropy is log s - t / s.
+//
+//   V <= 256, up to 16 alternatives (lp_small_kernel): 16 lanes a row, its logits in
+//     registers.  Each lane sorts its 16 as (value, inverted id) integers and the lanes'
+//     lists meet in four bitonic merges over DPP: no round per alternative.
+//   V <= 64 x threads (lp_row_kernel): 64, 256 or 1024 threads a row, its logits in
+//     registers.  The row's k-th largest logit is at least the k-th largest of 64 maxima
+//     over disjoint parts of it, which bit-by-bit selection finds in one wave; the few
+//     logits from that bound on (about k + k^2 / 128 of them for small k) go to LDS and
+//     are ranked there by counting.  Ties in number beyond the buffer are taken in id
+//     order from the row; what neither takes (NaN among the first k, thousands of logits
+//     above the bound) goes one alternative after the other.
+//   longer rows: the same over two reads of the row, the second from the caches.
+//   fp64: a wavefront a row, one pass per alternative.
+//
+// MEASURED
 #include "dg_common.h"
 
 namespace dg {
@@ -19,93 +33,553 @@ struct LogprobArgs {
   int64_t* top_ids;
 };
 
+// 16 bytes at any element's address: rows of an odd vocabulary start anywhere, and which
+// thread holds a logit must not depend on where (the sums' order, so a row's bits, would)
+typedef unsigned int u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ u32x4_t load16(const void* p) { return *reinterpret_cast<const u32x4_any_t*>(p); }
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// (value descending, id ascending, NaN last) order of two logits
+template <typename A>
+__device__ __forceinline__ bool comes_before(A v1, int64_t i1, A v2, int64_t i2) {
+  if (v1 != v1) return v2 != v2 && i1 < i2;
+  return v2 != v2 || v1 > v2 || (v1 == v2 && i1 < i2);
+}
+
+// One logit's part of s and t.  A logit of -inf (or one so far below m that the
+// difference overflows) adds 0 to both; NaN, and m = +-inf, make s NaN.
+__device__ __forceinline__ void add_logit(float x, float m, float& s, float& t) {
+  const float z = x - m;
+  const float e = __builtin_amdgcn_exp2f(z * kLog2e);
+  s += e;
+  t = __builtin_fmaf(fmaxf(z, -1e30f), e, t);
+}
+
+// log p(id) and the entropy of a row, by one lane
 template <typename T>
-struct LpAcc {
-  using type = float;
-  static __device__ __forceinline__ float load(T x) { return to_f32(x); }
-  static __device__ __forceinline__ float exp(float x) { return __expf(x); }
-  static __device__ __forceinline__ float log(float x) { return logf(x); }
+__device__ __forceinline__ void store_row_stats(const LogprobArgs& a, int64_t row, const T* x, float m, float logs, float s,
+                                                float t) {
+  const int64_t id = a.ids[row];
+  static_cast<float*>(a.logprob)[row] = id < 0 || id >= a.V ? __builtin_nanf("") : to_f32(x[id]) - m - logs;
+  if (a.entropy != nullptr) static_cast<float*>(a.entropy)[row] = logs - t / s;
+}
+
+// ---------------------------------------------------------------------------
+// V <= 256: 16 lanes a row
+// ---------------------------------------------------------------------------
+
+// (value, id) as an integer that sorts by value, then by descending id: larger comes first.
+// 0 is no logit at all; NaN ranks below -inf.
+template <typename T>
+struct LpKey {
+  using type = uint32_t;  // 16 bits of value, 16 of id
+  static __device__ __forceinline__ uint32_t make(T v, int id) {
+    const uint32_t b = from_f32<T>(to_f32(v) + 0.f).bits;  // -0 ranks as 0
+    const uint32_t u = (b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u;
+    return ((to_f32(v) != to_f32(v) ? 0u : u) << 16) | (0xffffu - (uint32_t)id);
+  }
+  static __device__ __forceinline__ int id(uint32_t k) { return 0xffff - (int)(k & 0xffffu); }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    const uint32_t u = k >> 16;
+    T v;
+    v.bits = (uint16_t)((u & 0x8000u) ? u & 0x7fffu : ~u);
+    return to_f32(v);
+  }
 };
 template <>
-struct LpAcc<double> {
-  using type = double;
-  static __device__ __forceinline__ double load(double x) { return x; }
-  static __device__ __forceinline__ double exp(double x) { return ::exp(x); }
-  static __device__ __forceinline__ double log(double x) { return ::log(x); }
+struct LpKey<float> {
+  using type = uint64_t;
+  static __device__ __forceinline__ uint64_t make(float v, int id) {
+    const uint32_t b = __float_as_uint(v + 0.f);
+    const uint32_t u = (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return ((uint64_t)(v != v ? 0u : u) << 32) | (0xffffffffu - (uint32_t)id);
+  }
+  static __device__ __forceinline__ int id(uint64_t k) { return (int)(0xffffffffu - (uint32_t)k); }
+  static __device__ __forceinline__ float value(uint64_t k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+  }
 };
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_key(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_key(uint64_t v) {
+  return (uint64_t)dpp_key<CTRL>((uint32_t)v) | ((uint64_t)dpp_key<CTRL>((uint32_t)(v >> 32)) << 32);
+}
+
+template <typename K>
+__device__ __forceinline__ void order_keys(K& hi, K& lo) {
+  const bool swap = lo > hi;
+  const K h = swap ? lo : hi, l = swap ? hi : lo;
+  hi = h;
+  lo = l;
+}
+
+// Batcher's odd-even merge sort, descending
+template <int N, typename K>
+__device__ __forceinline__ void sort_keys(K* v) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order_keys(v[i + j], v[i + j + k]);
+}
+// a bitonic sequence, descending
+template <int N, typename K>
+__device__ __forceinline__ void sort_bitonic(K* v) {
+#pragma unroll
+  for (int w = N / 2; w >= 1; w /= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & w) == 0) order_keys(v[i], v[i + w]);
+}
+// the N first of two sorted lists of N, the other one the partner lane's
+template <int N, int CTRL, typename K>
+__device__ __forceinline__ void merge_lists(K* v) {
+  K m[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const K other = dpp_key<CTRL>(v[N - 1 - i]);
+    m[i] = v[i] > other ? v[i] : other;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = m[i];
+  sort_bitonic<N>(v);
+}
+
+// maximum over 16 consecutive lanes
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp<kDppQuadXor1>(v));
+  v = fmaxf(v, dpp<kDppQuadXor2>(v));
+  v = fmaxf(v, dpp<kDppHalfMirror>(v));
+  return fmaxf(v, dpp<kDppMirror>(v));
+}
+
+// KP: the length of the lists, 0 where no alternatives are asked for.  VEC: rows of whole
+// 16-byte vectors.
+template <typename T, int KP, bool VEC>
+__global__ __launch_bounds__(256) void lp_small_kernel(const LogprobArgs a) {
+  using Key = LpKey<T>;
+  using K = typename Key::type;
+  constexpr int VE = VEC ? 16 / (int)sizeof(T) : 1;  // logits of a load
+  constexpr int NV = 16 / VE;
+  const int lane = threadIdx.x & 15;
+  const int64_t r0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int64_t row = r0 < a.M ? r0 : a.M - 1;  // rows past the last repeat it, unstored
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  const int V = (int)a.V;
+  T v[16];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    const int i0 = (16 * c + lane) * VE;
+    if constexpr (VEC) {
+      u32x4_t w = {0u, 0u, 0u, 0u};
+      if (i0 < V) w = load16(x + i0);
+      __builtin_memcpy(&v[c * VE], &w, 16);
+    } else {
+      v[c] = i0 < V ? x[i0] : T{};
+    }
+  }
+  float m = kNegInf;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if ((16 * (i / VE) + lane) * VE < V) m = fmaxf(m, to_f32(v[i]));
+  m = max16(m);
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if ((16 * (i / VE) + lane) * VE < V) add_logit(to_f32(v[i]), m, s, t);
+  s = group_sum_dpp<16>(s);
+  t = group_sum_dpp<16>(t);
+  const float logs = logf(s);
+  if (lane == 0 && r0 < a.M) store_row_stats(a, row, x, m, logs, s, t);
+  if constexpr (KP > 0) {
+    K k[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int id = (16 * (i / VE) + lane) * VE + i % VE;
+      k[i] = id < V ? Key::make(v[i], id) : (K)0;
+    }
+    if constexpr (KP == 8) {
+      sort_keys<8>(k);
+      sort_keys<8>(k + 8);
+      K f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = k[i] > k[15 - i] ? k[i] : k[15 - i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[i] = f[i];
+      sort_bitonic<8>(k);
+    } else {
+      sort_keys<16>(k);
+    }
+    merge_lists<KP, kDppQuadXor1>(k);
+    merge_lists<KP, kDppQuadXor2>(k);
+    merge_lists<KP, kDppHalfMirror>(k);
+    merge_lists<KP, kDppMirror>(k);
+    K mine = k[0];
+#pragma unroll
+    for (int i = 1; i < KP; ++i) mine = lane == i ? k[i] : mine;
+    if (lane < a.top && r0 < a.M) {
+      a.top_ids[row * a.top + lane] = Key::id(mine);
+      static_cast<float*>(a.top_logprob)[row * a.top + lane] = Key::value(mine) - m - logs;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 64, 256 or 1024 threads a row
+// ---------------------------------------------------------------------------
+
+// The k-th largest (k from 1) of the wave's 64 values, NaN-free: bit by bit on integers
+// that sort as the values do.
+template <typename T>
+__device__ __forceinline__ float kth_largest(float v, int k) {
+  constexpr int BITS = 8 * (int)sizeof(T);
+  uint32_t u;
+  if constexpr (BITS == 32) u = __float_as_uint(v);
+  else u = (uint32_t)from_f32<T>(v).bits << 16;  // v is a value of T
+  u = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  uint64_t alive = ~0ull;
+  uint32_t kth = 0;
+#pragma unroll
+  for (int b = 31; b >= 32 - BITS; --b) {
+    const uint64_t ones = __builtin_amdgcn_ballot_w64((u >> b) & 1u) & alive;
+    const int n = __builtin_popcountll(ones);
+    if (n >= k) {
+      alive = ones;
+      kth |= 1u << b;
+    } else {
+      k -= n;
+      alive &= ~ones;
+    }
+  }
+  const uint32_t bits = (kth & 0x80000000u) ? kth & 0x7fffffffu : ~kth;
+  if constexpr (BITS == 32) {
+    return __uint_as_float(bits);
+  } else {
+    T r;
+    r.bits = (uint16_t)(bits >> 16);
+    return to_f32(r);
+  }
+}
+
+// A row's logits as its threads hold them: its 16-byte vectors, the thread's j-th one
+// vector j * NT + tid, and at most one of the logits behind them.
+template <typename T, int NT, int NV, bool HELD>
+struct LpRow {
+  static constexpr int VE = 16 / (int)sizeof(T);
+  const T* x;
+  int V, nvec, tid;
+  int extra;      // id of the single logit, -1: none
+  T single;
+  u32x4_t raw[HELD ? NV : 1];
+
+  __device__ __forceinline__ void load(const T* row, int v, int t) {
+    x = row;
+    V = v;
+    tid = t;
+    nvec = V / VE;
+    extra = tid < V - nvec * VE ? nvec * VE + tid : -1;
+    single = extra >= 0 ? x[extra] : T{};
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        raw[j] = u32x4_t{0u, 0u, 0u, 0u};
+        if (j * NT + tid < nvec) raw[j] = load16(x + (int64_t)(j * NT + tid) * VE);
+      }
+    }
+  }
+  // f(logit, id) over the thread's logits; every lane of a wave takes part in every call
+  // of f, with `there` false where it has none
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    f(to_f32(single), extra, extra >= 0);
+    auto vec = [&](const u32x4_t& w, int i) __attribute__((always_inline)) {
+      T e[VE];
+      __builtin_memcpy(e, &w, 16);
+      const bool there = i < nvec;
+#pragma unroll
+      for (int c = 0; c < VE; ++c) f(to_f32(e[c]), i * VE + c, there);
+    };
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (j * NT + (tid & ~63) >= nvec) break;  // wave-uniform
+        vec(raw[j], j * NT + tid);
+      }
+    } else {
+      for (int i = tid; (i & ~63) < nvec; i += NT) {
+        u32x4_t w = {0u, 0u, 0u, 0u};
+        if (i < nvec) w = load16(x + (int64_t)i * VE);
+        vec(w, i);
+      }
+    }
+  }
+};
+
+// LDS of a row's threads
+template <int NW, int CAP>
+struct LpShared {
+  float part[NW][64];   // the lanes' maxima
+  float sum[NW], tsum[NW];
+  float bound;          // the k-th of the maxima
+  int count;            // candidates
+  float best_v[NW];     // a round's first logit of each wave
+  int best_i[NW];
+  float cand_v[CAP];
+  int cand_i[CAP];
+};
+
+// Threads of a row meet here: one wave needs no barrier.
+template <int NT>
+__device__ __forceinline__ void lp_sync() {
+  if constexpr (NT > 64) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// NT threads a row; workgroups of 256 threads at least (several rows where NT is 64).
+template <typename T, int NT, int NV, bool HELD>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const LogprobArgs a) {
+  constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
+  __shared__ LpShared<NW, CAP> sh_all[RPB];
+  LpShared<NW, CAP>& sh = sh_all[RPB == 1 ? 0 : threadIdx.x / NT];
+  const int tid = threadIdx.x % NT, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = (int64_t)blockIdx.x * RPB + (RPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT));
+  if (row >= a.M) return;  // RPB > 1: whole waves, which share no barrier
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  const int top = a.top;
+  LpRow<T, NT, NV, HELD> r;
+  r.load(x, (int)a.V, tid);
+
+  float m = kNegInf, s = 0.f, t = 0.f;
+  r.each([&](float v, int, bool there) __attribute__((always_inline)) { m = fmaxf(m, there ? v : kNegInf); });
+  const float mine = m;
+  if constexpr (NW > 1) {
+    sh.part[wv][lane] = m;
+    lp_sync<NT>();
+    m = sh.part[0][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, sh.part[w][lane]);
+  }
+  const float part = NW > 1 ? m : mine;  // a 64th of the row
+  m = wave_max(part);
+  if (top > 0 && wv == 0) {
+    const float bound = kth_largest<T>(part, top);
+    if (lane == 0) {
+      sh.bound = bound;
+      sh.count = 0;
+    }
+  }
+  r.each([&](float v, int, bool there) __attribute__((always_inline)) {
+    float s2 = s, t2 = t;
+    add_logit(v, m, s2, t2);
+    s = there ? s2 : s;
+    t = there ? t2 : t;
+  });
+  s = group_sum_dpp<64>(s);
+  t = group_sum_dpp<64>(t);
+  if constexpr (NW > 1) {
+    if (lane == 0) {
+      sh.sum[wv] = s;
+      sh.tsum[wv] = t;
+    }
+  }
+  lp_sync<NT>();
+  if constexpr (NW > 1) {
+    s = sh.sum[0];
+    t = sh.tsum[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      s += sh.sum[w];
+      t += sh.tsum[w];
+    }
+  }
+  const float logs = logf(s);
+  if (tid == 0) store_row_stats(a, row, x, m, logs, s, t);
+  if (top == 0) return;
+
+  int64_t* ids = a.top_ids + row * top;
+  float* lps = static_cast<float*>(a.top_logprob) + row * top;
+  const float bound = sh.bound;
+  // the logits that pass, into LDS as far as they fit; how many there are
+  auto collect = [&](bool equal_too) __attribute__((always_inline)) -> int {
+    r.each([&](float v, int id, bool there) __attribute__((always_inline)) {
+      const bool in = there && (v > bound || (equal_too && v == bound));
+      const uint64_t b = __builtin_amdgcn_ballot_w64(in);
+      if (b != 0) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&sh.count, __builtin_popcountll(b));
+        at = __builtin_amdgcn_readfirstlane(at);
+        at += __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+        if (in && at < CAP) {
+          sh.cand_v[at] = v;
+          sh.cand_i[at] = id;
+        }
+      }
+    });
+    lp_sync<NT>();
+    return sh.count;
+  };
+  auto rank = [&](int n) __attribute__((always_inline)) {
+    for (int c = tid; c < n; c += NT) {
+      const float v = sh.cand_v[c];
+      const int id = sh.cand_i[c];
+      int before = 0;
+      for (int o = 0; o < n; ++o) before += comes_before(sh.cand_v[o], sh.cand_i[o], v, id) ? 1 : 0;
+      if (before < top) {
+        ids[before] = id;
+        lps[before] = v - m - logs;
+      }
+    }
+  };
+  const int n = collect(true);
+  if (n >= top && n <= CAP) {
+    rank(n);
+    return;
+  }
+  lp_sync<NT>();  // everyone has read the count
+  if (tid == 0) sh.count = 0;
+  lp_sync<NT>();
+  const int above = collect(false);
+  if (n >= top && above <= CAP) {
+    rank(above);
+    // the rest are the first of those equal to the bound, in id order
+    if (wv == 0) {
+      int at = above;
+      for (int v0 = 0; v0 < r.V && at < top; v0 += 64) {
+        const bool in = v0 + lane < r.V && to_f32(x[min(v0 + lane, r.V - 1)]) == bound;
+        const uint64_t b = __builtin_amdgcn_ballot_w64(in);
+        const int mine_at = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+        if (in && mine_at < top) {
+          ids[mine_at] = v0 + lane;
+          lps[mine_at] = bound - m - logs;
+        }
+        at += __builtin_popcountll(b);
+      }
+    }
+    return;
+  }
+  // one alternative after the other
+  float pv = 0.f;
+  int pi = -1;
+  for (int j = 0; j < top; ++j) {
+    float bv = 0.f;
+    int bi = r.V;
+    r.each([&](float v, int id, bool there) __attribute__((always_inline)) {
+      const bool in = there && (pi < 0 || comes_before(pv, pi, v, id)) && (bi == r.V || comes_before(v, id, bv, bi));
+      bv = in ? v : bv;
+      bi = in ? id : bi;
+    });
+    auto take = [&](float v2, int i2) __attribute__((always_inline)) {
+      const bool in = i2 < r.V && (bi == r.V || comes_before(v2, i2, bv, bi));
+      bv = in ? v2 : bv;
+      bi = in ? i2 : bi;
+    };
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const float v2 = __shfl_xor(bv, o, 64);
+      const int i2 = __shfl_xor(bi, o, 64);
+      take(v2, i2);
+    }
+    if constexpr (NW > 1) {
+      lp_sync<NT>();
+      if (lane == 0) {
+        sh.best_v[wv] = bv;
+        sh.best_i[wv] = bi;
+      }
+      lp_sync<NT>();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) take(sh.best_v[w], sh.best_i[w]);
+    }
+    pv = bv;
+    pi = bi;
+    if (tid == 0) {
+      ids[j] = bi;
+      lps[j] = bv - m - logs;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// fp64: a wavefront a row
+// ---------------------------------------------------------------------------
+
 // m, s, t of a part of the row, joined with another part's
-template <typename S, typename A>
-__device__ __forceinline__ void join_part(A& m, A& s, A& t, A m2, A s2, A t2) {
-  const A ninf = -(A)__builtin_huge_valf();
-  const A mn = m > m2 ? m : m2;
+__device__ __forceinline__ void join_part(double& m, double& s, double& t, double m2, double s2, double t2) {
+  const double ninf = -__builtin_huge_val();
+  const double mn = m > m2 ? m : m2;
   if (mn == ninf) {  // neither holds a probability; a NaN stays in s
     s += s2;
     return;
   }
   // a part at -inf has s = 0 (or NaN) and no t; one whose factor vanishes, the difference
   // of two finite logits may overflow, adds nothing
-  const A d1 = m - mn, d2 = m2 - mn;
-  const A f1 = S::exp(d1), f2 = S::exp(d2);
-  t = (f1 == (A)0 ? (A)0 : f1 * (t + d1 * s)) + (f2 == (A)0 ? (A)0 : f2 * (t2 + d2 * s2));
+  const double d1 = m - mn, d2 = m2 - mn;
+  const double f1 = exp(d1), f2 = exp(d2);
+  t = (f1 == 0 ? 0 : f1 * (t + d1 * s)) + (f2 == 0 ? 0 : f2 * (t2 + d2 * s2));
   s = (m == ninf ? s : f1 * s) + (m2 == ninf ? s2 : f2 * s2);
   m = mn;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a) {
-  using S = LpAcc<T>;
-  using A = typename S::type;
-  const A ninf = -(A)__builtin_huge_valf();
+__global__ __launch_bounds__(256) void lp_f64_kernel(const LogprobArgs a) {
+  const double ninf = -__builtin_huge_val();
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= a.M) return;
-  const T* x = static_cast<const T*>(a.x) + row * a.ld;
-  A m = ninf, s = (A)0, t = (A)0;
+  const double* x = static_cast<const double*>(a.x) + row * a.ld;
+  double m = ninf, s = 0, t = 0;
   for (int64_t v = lane; v < a.V; v += 64) {
-    const A z = S::load(x[v]);
+    const double z = x[v];
     if (z == ninf) continue;
     if (z != z) {
       s = z;
       continue;
     }
-    join_part<S, A>(m, s, t, z, (A)1, (A)0);
+    join_part(m, s, t, z, 1, 0);
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const A m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), t2 = __shfl_xor(t, o, 64);
-    join_part<S, A>(m, s, t, m2, s2, t2);
+    const double m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), t2 = __shfl_xor(t, o, 64);
+    join_part(m, s, t, m2, s2, t2);
   }
-  const A logs = m == ninf ? (A)__builtin_nanf("") : S::log(s);
+  const double logs = m == ninf ? __builtin_nan("") : log(s);
   if (lane == 0) {
     const int64_t id = a.ids[row];
-    static_cast<A*>(a.logprob)[row] = id < 0 || id >= a.V ? (A)__builtin_nanf("") : S::load(x[id]) - m - logs;
-    if (a.entropy != nullptr) static_cast<A*>(a.entropy)[row] = logs - t / s;
+    static_cast<double*>(a.logprob)[row] = id < 0 || id >= a.V ? __builtin_nan("") : x[id] - m - logs;
+    if (a.entropy != nullptr) static_cast<double*>(a.entropy)[row] = logs - t / s;
   }
-  // one alternative after the other: the first in (value descending, id ascending, NaN
-  // last) order behind the one before it
-  A pv = (A)0;
+  double pv = 0;
   int64_t pi = -1;
   for (int j = 0; j < a.top; ++j) {
-    A bv = (A)0;
+    double bv = 0;
     int64_t bi = a.V;
-    auto before = [](A v1, int64_t i1, A v2, int64_t i2) {
-      if (v1 != v1) return v2 != v2 && i1 < i2;
-      return v2 != v2 || v1 > v2 || (v1 == v2 && i1 < i2);
-    };
     for (int64_t v = lane; v < a.V; v += 64) {
-      const A z = S::load(x[v]);
-      if (pi >= 0 && !before(pv, pi, z, v)) continue;
-      if (bi == a.V || before(z, v, bv, bi)) {
+      const double z = x[v];
+      if (pi >= 0 && !comes_before(pv, pi, z, v)) continue;
+      if (bi == a.V || comes_before(z, v, bv, bi)) {
         bv = z;
         bi = v;
       }
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const A v2 = __shfl_xor(bv, o, 64);
+      const double v2 = __shfl_xor(bv, o, 64);
       const int64_t i2 = __shfl_xor((long long)bi, o, 64);
-      if (i2 < a.V && (bi == a.V || before(v2, i2, bv, bi))) {
+      if (i2 < a.V && (bi == a.V || comes_before(v2, i2, bv, bi))) {
         bv = v2;
         bi = i2;
       }
@@ -114,11 +588,49 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
     pi = bi;
     if (lane == 0) {
       a.top_ids[row * a.top + j] = bi;
-      static_cast<A*>(a.top_logprob)[row * a.top + j] = bv - m - logs;
+      static_cast<double*>(a.top_logprob)[row * a.top + j] = bv - m - logs;
     }
   }
 }
 
+namespace {
+
+template <typename T>
+int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  const bool vec = a.V % VE == 0;
+  if (a.V <= 256 && a.top <= 16) {
+    const dim3 grid((unsigned)((a.M + 15) / 16));
+#define DG_LP(KP)                                                                                    \
+  do {                                                                                               \
+    if (vec) hipLaunchKernelGGL((lp_small_kernel<T, KP, true>), grid, dim3(256), 0, s, a);           \
+    else hipLaunchKernelGGL((lp_small_kernel<T, KP, false>), grid, dim3(256), 0, s, a);              \
+  } while (0)
+    if (a.top == 0) DG_LP(0);
+    else if (a.top <= 8) DG_LP(8);
+    else DG_LP(16);
+#undef DG_LP
+    return check_launch("lp_small_kernel");
+  }
+  // a thread holds up to 64 logits
+  constexpr int NV = 64 / VE;
+  if (a.V <= 64 * 64) {
+    hipLaunchKernelGGL((lp_row_kernel<T, 64, NV, true>), dim3((unsigned)((a.M + 3) / 4)), dim3(256), 0, s, a);
+    return check_launch("lp_row_kernel_64");
+  }
+  if (a.V <= 64 * 256) {
+    hipLaunchKernelGGL((lp_row_kernel<T, 256, NV, true>), dim3((unsigned)a.M), dim3(256), 0, s, a);
+    return check_launch("lp_row_kernel_256");
+  }
+  if (a.V <= 64 * 1024) {
+    hipLaunchKernelGGL((lp_row_kernel<T, 1024, NV, true>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+    return check_launch("lp_row_kernel_1024");
+  }
+  hipLaunchKernelGGL((lp_row_kernel<T, 1024, 1, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+  return check_launch("lp_long_kernel");
+}
+
+}  // namespace
 }  // namespace dg
 
 using namespace dg;
@@ -130,15 +642,16 @@ extern "C" int dg_token_logprobs(int64_t M, int64_t V, int dtype, const void* x,
   DG_REQUIRE(dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64, DG_EUNSUPPORTED,
              "token_logprobs: dtype %d unsupported", dtype);
   DG_REQUIRE(top >= 0 && top <= 64 && top <= V, DG_EINVAL, "token_logprobs: top %d outside [0, min(V, 64)]", top);
-  DG_REQUIRE(V <= 0x7fffffff && (M + 3) / 4 <= 0x7fffffff, DG_EINVAL, "token_logprobs: too many logits or rows");
+  DG_REQUIRE(V <= 0x3fffffff && M <= 0x7fffffff, DG_EINVAL, "token_logprobs: too many logits or rows");
   if (M == 0) return DG_OK;
   DG_REQUIRE(x && ids && logprob && (top == 0 || (top_logprob && top_ids)), DG_EINVAL, "token_logprobs: NULL argument");
-  LogprobArgs a{x, x_ld, M, V, ids, logprob, entropy, top, top_logprob, top_ids};
+  const LogprobArgs a{x, x_ld, M, V, ids, logprob, entropy, top, top_logprob, top_ids};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)((M + 3) / 4));
-  if (dtype == DG_F64) hipLaunchKernelGGL(token_logprobs_kernel<double>, grid, dim3(256), 0, s, a);
-  else if (dtype == DG_F32) hipLaunchKernelGGL(token_logprobs_kernel<float>, grid, dim3(256), 0, s, a);
-  else if (dtype == DG_BF16) hipLaunchKernelGGL(token_logprobs_kernel<bf16_t>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(token_logprobs_kernel<f16_t>, grid, dim3(256), 0, s, a);
-  return check_launch("token_logprobs_kernel");
+  if (dtype == DG_F64) {
+    hipLaunchKernelGGL(lp_f64_kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, a);
+    return check_launch("lp_f64_kernel");
+  }
+  if (dtype == DG_F32) return launch_logprobs<float>(a, s);
+  if (dtype == DG_BF16) return launch_logprobs<bf16_t>(a, s);
+  return launch_logprobs<f16_t>(a, s);
 }
