@@ -272,55 +272,62 @@ __device__ __forceinline__ float kth_largest(float v, int k) {
 }
 
 // A row's logits as its threads hold them: its 16-byte vectors, the thread's j-th one
-// vector j * NT + tid, and at most one of the logits behind them.
+// vector j * NT + tid, and at most one of the logits behind them.  Where a thread has
+// none it holds -inf and an id of V or more.
 template <typename T, int NT, int NV, bool HELD>
 struct LpRow {
   static constexpr int VE = 16 / (int)sizeof(T);
+  static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : __is_same(T, bf16_t) ? 0xff80ff80u : 0xfc00fc00u;
   const T* x;
   int V, nvec, tid;
-  int extra;      // id of the single logit, -1: none
-  T single;
+  int extra;  // id of the single logit
+  float single;
   u32x4_t raw[HELD ? NV : 1];
 
+  __device__ __forceinline__ u32x4_t vector(int i) const {
+    u32x4_t w = {kNone, kNone, kNone, kNone};
+    if (i < nvec) w = load16(x + (int64_t)i * VE);
+    return w;
+  }
   __device__ __forceinline__ void load(const T* row, int v, int t) {
     x = row;
     V = v;
     tid = t;
     nvec = V / VE;
-    extra = tid < V - nvec * VE ? nvec * VE + tid : -1;
-    single = extra >= 0 ? x[extra] : T{};
+    extra = tid < V - nvec * VE ? nvec * VE + tid : V;
+    single = extra < V ? to_f32(x[extra]) : kNegInf;
     if constexpr (HELD) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        raw[j] = u32x4_t{0u, 0u, 0u, 0u};
-        if (j * NT + tid < nvec) raw[j] = load16(x + (int64_t)(j * NT + tid) * VE);
-      }
+      for (int j = 0; j < NV; ++j) raw[j] = vector(j * NT + tid);
     }
   }
-  // f(logit, id) over the thread's logits; every lane of a wave takes part in every call
-  // of f, with `there` false where it has none
+  // The words as they are, unpacked anew by each pass: kept unpacked they would take
+  // twice the registers.
+  __device__ __forceinline__ void forget_unpacked() {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(raw[j]));
+    }
+  }
+  // f(the logits of a vector, the first one's id, its number) over the thread's vectors,
+  // the wave's lanes together
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    f(to_f32(single), extra, extra >= 0);
-    auto vec = [&](const u32x4_t& w, int i) __attribute__((always_inline)) {
+  __device__ __forceinline__ void vectors(F f) const {
+    auto vec = [&](const u32x4_t& w, int i, int j) __attribute__((always_inline)) {
       T e[VE];
       __builtin_memcpy(e, &w, 16);
-      const bool there = i < nvec;
+      float v[VE];
 #pragma unroll
-      for (int c = 0; c < VE; ++c) f(to_f32(e[c]), i * VE + c, there);
+      for (int c = 0; c < VE; ++c) v[c] = to_f32(e[c]);
+      int id = i * VE;
+      asm volatile("" : "+v"(id));  // comparisons with ids are made where they are used, not kept
+      f(v, id, j);
     };
     if constexpr (HELD) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (j * NT + (tid & ~63) >= nvec) break;  // wave-uniform
-        vec(raw[j], j * NT + tid);
-      }
+      for (int j = 0; j < NV; ++j) vec(raw[j], j * NT + tid, j);
     } else {
-      for (int i = tid; (i & ~63) < nvec; i += NT) {
-        u32x4_t w = {0u, 0u, 0u, 0u};
-        if (i < nvec) w = load16(x + (int64_t)i * VE);
-        vec(w, i);
-      }
+      for (int i = tid; (i & ~63) < nvec; i += NT) vec(vector(i), i, 0);
     }
   }
 };
@@ -350,10 +357,18 @@ __device__ __forceinline__ void lp_sync() {
   }
 }
 
+// waves a SIMD that the registers must allow: two rows of 1024 threads on a CU in 16-bit
+// types, whose loads and arithmetic then overlap
+template <typename T, int NT>
+constexpr int lp_row_waves() {
+  return NT == 1024 ? (sizeof(T) == 2 ? 8 : 4) : 4;
+}
+
 // NT threads a row; workgroups of 256 threads at least (several rows where NT is 64).
 template <typename T, int NT, int NV, bool HELD>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void lp_row_kernel(const LogprobArgs a) {
   constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
+  constexpr int VE = 16 / (int)sizeof(T);
   __shared__ LpShared<NW, CAP> sh_all[RPB];
   LpShared<NW, CAP>& sh = sh_all[RPB == 1 ? 0 : threadIdx.x / NT];
   const int tid = threadIdx.x % NT, lane = tid & 63;
@@ -365,9 +380,21 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const Logpr
   LpRow<T, NT, NV, HELD> r;
   r.load(x, (int)a.V, tid);
 
-  float m = kNegInf, s = 0.f, t = 0.f;
-  r.each([&](float v, int, bool there) __attribute__((always_inline)) { m = fmaxf(m, there ? v : kNegInf); });
-  const float mine = m;
+  auto vec_max = [](const float(&v)[VE]) __attribute__((always_inline)) {
+    float x0 = v[0];
+#pragma unroll
+    for (int c = 1; c < VE; ++c) x0 = fmaxf(x0, v[c]);
+    return x0;
+  };
+  float vmax[HELD ? NV : 1];  // each vector's maximum
+  float m = r.single, s = 0.f, t = 0.f;
+  m = fmaxf(m, kNegInf);  // a NaN is no maximum
+  r.vectors([&](const float(&v)[VE], int, int j) __attribute__((always_inline)) {
+    const float x0 = vec_max(v);
+    if constexpr (HELD) vmax[j] = x0;
+    m = fmaxf(m, x0);
+  });
+  r.forget_unpacked();
   if constexpr (NW > 1) {
     sh.part[wv][lane] = m;
     lp_sync<NT>();
@@ -375,7 +402,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const Logpr
 #pragma unroll
     for (int w = 1; w < NW; ++w) m = fmaxf(m, sh.part[w][lane]);
   }
-  const float part = NW > 1 ? m : mine;  // a 64th of the row
+  const float part = m;  // of a 64th of the row
   m = wave_max(part);
   if (top > 0 && wv == 0) {
     const float bound = kth_largest<T>(part, top);
@@ -384,12 +411,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const Logpr
       sh.count = 0;
     }
   }
-  r.each([&](float v, int, bool there) __attribute__((always_inline)) {
-    float s2 = s, t2 = t;
-    add_logit(v, m, s2, t2);
-    s = there ? s2 : s;
-    t = there ? t2 : t;
+  if (r.extra < r.V) add_logit(r.single, m, s, t);
+  r.vectors([&](const float(&v)[VE], int, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < VE; ++c) add_logit(v[c], m, s, t);
   });
+  r.forget_unpacked();
   s = group_sum_dpp<64>(s);
   t = group_sum_dpp<64>(t);
   if constexpr (NW > 1) {
@@ -415,24 +442,19 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const Logpr
   int64_t* ids = a.top_ids + row * top;
   float* lps = static_cast<float*>(a.top_logprob) + row * top;
   const float bound = sh.bound;
-  // the logits that pass, into LDS as far as they fit; how many there are
-  auto collect = [&](bool equal_too) __attribute__((always_inline)) -> int {
-    r.each([&](float v, int id, bool there) __attribute__((always_inline)) {
-      const bool in = there && (v > bound || (equal_too && v == bound));
-      const uint64_t b = __builtin_amdgcn_ballot_w64(in);
-      if (b != 0) {
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&sh.count, __builtin_popcountll(b));
-        at = __builtin_amdgcn_readfirstlane(at);
-        at += __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-        if (in && at < CAP) {
-          sh.cand_v[at] = v;
-          sh.cand_i[at] = id;
-        }
+  // a logit that passes, into LDS as far as there is room; the wave's lanes together
+  auto offer = [&](bool in, float v, int id) __attribute__((always_inline)) {
+    const uint64_t b = __builtin_amdgcn_ballot_w64(in);
+    if (b != 0) {
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sh.count, __builtin_popcountll(b));
+      at = __builtin_amdgcn_readfirstlane(at);
+      at += __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+      if (in && at < CAP) {
+        sh.cand_v[at] = v;
+        sh.cand_i[at] = id;
       }
-    });
-    lp_sync<NT>();
-    return sh.count;
+    }
   };
   auto rank = [&](int n) __attribute__((always_inline)) {
     for (int c = tid; c < n; c += NT) {
@@ -446,27 +468,43 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const Logpr
       }
     }
   };
-  const int n = collect(true);
+  offer(r.single >= bound && r.extra < r.V, r.single, r.extra);
+  r.vectors([&](const float(&v)[VE], int id, int j) __attribute__((always_inline)) {
+    float most;
+    if constexpr (HELD) most = vmax[j];
+    else most = vec_max(v);
+    if (__builtin_amdgcn_ballot_w64(most >= bound) == 0) return;  // the lanes' vectors hold none
+#pragma unroll
+    for (int c = 0; c < VE; ++c) offer(v[c] >= bound && id < r.V, v[c], id + c);
+  });
+  lp_sync<NT>();
+  const int n = sh.count;
   if (n >= top && n <= CAP) {
     rank(n);
     return;
   }
+  // Rare from here on, and read from memory again.  Too many: those above the bound, and
+  // of those equal to it the first in id order.
   lp_sync<NT>();  // everyone has read the count
   if (tid == 0) sh.count = 0;
   lp_sync<NT>();
-  const int above = collect(false);
+  for (int v0 = tid - lane; v0 < r.V; v0 += NT) {
+    const float v = to_f32(x[min(v0 + lane, r.V - 1)]);
+    offer(v > bound && v0 + lane < r.V, v, v0 + lane);
+  }
+  lp_sync<NT>();
+  const int above = sh.count;
   if (n >= top && above <= CAP) {
     rank(above);
-    // the rest are the first of those equal to the bound, in id order
     if (wv == 0) {
       int at = above;
       for (int v0 = 0; v0 < r.V && at < top; v0 += 64) {
         const bool in = v0 + lane < r.V && to_f32(x[min(v0 + lane, r.V - 1)]) == bound;
         const uint64_t b = __builtin_amdgcn_ballot_w64(in);
-        const int mine_at = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-        if (in && mine_at < top) {
-          ids[mine_at] = v0 + lane;
-          lps[mine_at] = bound - m - logs;
+        const int mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+        if (in && mine < top) {
+          ids[mine] = v0 + lane;
+          lps[mine] = bound - m - logs;
         }
         at += __builtin_popcountll(b);
       }
@@ -479,21 +517,20 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const Logpr
   for (int j = 0; j < top; ++j) {
     float bv = 0.f;
     int bi = r.V;
-    r.each([&](float v, int id, bool there) __attribute__((always_inline)) {
-      const bool in = there && (pi < 0 || comes_before(pv, pi, v, id)) && (bi == r.V || comes_before(v, id, bv, bi));
-      bv = in ? v : bv;
-      bi = in ? id : bi;
-    });
-    auto take = [&](float v2, int i2) __attribute__((always_inline)) {
-      const bool in = i2 < r.V && (bi == r.V || comes_before(v2, i2, bv, bi));
+    auto take = [&](float v2, int i2, bool in) __attribute__((always_inline)) {
+      in = in && i2 < r.V && (bi == r.V || comes_before(v2, i2, bv, bi));
       bv = in ? v2 : bv;
       bi = in ? i2 : bi;
     };
+    for (int id = tid; id < r.V; id += NT) {
+      const float v = to_f32(x[id]);
+      take(v, id, pi < 0 || comes_before(pv, pi, v, id));
+    }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const float v2 = __shfl_xor(bv, o, 64);
       const int i2 = __shfl_xor(bi, o, 64);
-      take(v2, i2);
+      take(v2, i2, true);
     }
     if constexpr (NW > 1) {
       lp_sync<NT>();
@@ -503,7 +540,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void lp_row_kernel(const Logpr
       }
       lp_sync<NT>();
 #pragma unroll
-      for (int w = 0; w < NW; ++w) take(sh.best_v[w], sh.best_i[w]);
+      for (int w = 0; w < NW; ++w) take(sh.best_v[w], sh.best_i[w], true);
     }
     pv = bv;
     pi = bi;

@@ -13,7 +13,6 @@ and returns immediately.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import os
@@ -752,24 +751,32 @@ def draw_argmax_(probs: torch.Tensor, q: torch.Tensor, ids: torch.Tensor) -> boo
     return True
 
 
-def _check_tensors(what: str, *tensors: torch.Tensor) -> None:
-    """On one ROCm device, of one supported type, tracked by nobody."""
-    require_device(what, *tensors)
-    require_inference(what, *tensors)
+def _check_tensors(what: str, *tensors: torch.Tensor) -> int:
+    """The device of tensors that lie on one ROCm device, share one supported type and are
+    tracked by nobody."""
     first = tensors[0]
+    dtype, device = first.dtype, first.get_device()
     for t in tensors:
-        if t.dtype != first.dtype:
-            raise TypeError(f"{what}: the tensors must share one dtype, got {first.dtype} and {t.dtype}")
-        if t.device != first.device:
+        if t.get_device() != device or device < 0:
+            require_device(what, *tensors)
             raise ValueError(f"{what}: the tensors must share one device, got {first.device} and {t.device}")
-    _dtype_code(first)
+        if t.dtype != dtype:
+            raise TypeError(f"{what}: the tensors must share one dtype, got {dtype} and {t.dtype}")
+    require_inference(what, *tensors)
+    if dtype not in _DTYPE_CODE:
+        _dtype_code(first)
+    return device
 
 
-def _on_device_of(t: torch.Tensor):
-    """A context in which t's device is the current one, which a launch on its stream needs."""
-    if t.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(what: str, device: int, fn, *args) -> None:
+    """fn(*args, the device's current stream) with that device the current one."""
+    if device == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != 0:
+        _check(rc, what)
 
 
 def _check_scale(what: str, scale: float) -> float:
@@ -801,11 +808,13 @@ def attention_packed_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, y: torc
     """dg_attention_packed: q, y (Nq,H,D) and k, v (Nk,Hkv,D) hold the sequences of
     ``layout`` (a PackedLayout for groups of H / Hkv heads) one after the other.  Rows of y
     behind the last sequence are left as they are."""
-    _check_tensors("attention_packed", q, k, v, y)
-    if q.dim() != 3 or k.dim() != 3 or y.shape != q.shape or v.shape != k.shape or k.size(2) != q.size(2):
+    device = _check_tensors("attention_packed", q, k, v, y)
+    if q.dim() != 3 or k.dim() != 3 or y.shape != q.shape or v.shape != k.shape:
         raise ValueError("attention_packed: q, y must be (Nq, H, D) and k, v (Nk, Hkv, D)")
     Nq, H, D = q.shape
-    Nk, Hkv, _ = k.shape
+    Nk, Hkv, Dk = k.shape
+    if Dk != D:
+        raise ValueError("attention_packed: q, y must be (Nq, H, D) and k, v (Nk, Hkv, D)")
     if not 1 <= D <= MAX_HEAD_DIM:
         raise ValueError(f"attention_packed: head_dim {D} outside 1 .. {MAX_HEAD_DIM}")
     if Hkv < 1 or H % Hkv or H // Hkv != layout.group:
@@ -813,19 +822,17 @@ def attention_packed_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, y: torc
     if layout.total_q > Nq or layout.total_k > Nk:
         raise ValueError(f"attention_packed: the layout covers {layout.total_q} and {layout.total_k} rows, "
                          f"q and k hold {Nq} and {Nk}")
-    if layout.tiles.device != q.device:
+    if layout.tiles.get_device() != device:
         raise ValueError(f"attention_packed: the layout is on {layout.tiles.device}, q on {q.device}")
-    for t in (q, k, v, y):
-        if t.stride(2) != 1 and D > 1:
-            raise ValueError("attention_packed: the last (head_dim) dimension must be contiguous")
-    scale = _check_scale("attention_packed", scale)
-    st = lambda t: (_ptr(t), t.stride(0), t.stride(1))  # noqa: E731
-    with _on_device_of(q):
-        rc = lib().dg_attention_packed(
-            Nq, Nk, H, Hkv, D, _dtype_code(q), *st(q), *st(k), *st(v), *st(y), scale, _ptr(layout.tiles),
-            layout.n_wide, layout.n_narrow, _stream(q),
-        )
-    _check(rc, "attention_packed")
+    qt, qh, qd = q.stride()
+    kt, kh, kd = k.stride()
+    vt, vh, vd = v.stride()
+    yt, yh, yd = y.stride()
+    if not (qd == kd == vd == yd == 1) and D > 1:
+        raise ValueError("attention_packed: the last (head_dim) dimension must be contiguous")
+    _launch("attention_packed", device, lib().dg_attention_packed, Nq, Nk, H, Hkv, D, _DTYPE_CODE[q.dtype],
+            q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, y.data_ptr(), yt, yh,
+            _check_scale("attention_packed", scale), layout.tiles.data_ptr(), layout.n_wide, layout.n_narrow)
 
 
 def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, y: torch.Tensor, scale: float,
@@ -834,7 +841,7 @@ def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     cached positions and, behind them, the N tokens' own.  lengths: the cached positions,
     one int or a (B,) int32 tensor; masks: (N,) or (B,N) int64, bit m of a token's mask set
     where it sees token m (None: the tokens before it and itself)."""
-    _check_tensors("attention_tree", q, k_cache, v_cache, y)
+    device = _check_tensors("attention_tree", q, k_cache, v_cache, y)
     if q.dim() != 4 or k_cache.dim() != 4 or y.shape != q.shape or v_cache.shape != k_cache.shape:
         raise ValueError("attention_tree: q, y must be (B, N, H, D) and the caches (B, Tcap, Hkv, D)")
     B, N, H, D = q.shape
@@ -851,7 +858,7 @@ def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"attention_tree: a cache of {Tcap} positions does not hold {N} tokens")
     lens, host_len = None, 0
     if isinstance(lengths, torch.Tensor):
-        if lengths.shape != (B,) or lengths.dtype != torch.int32 or lengths.device != q.device or (
+        if lengths.shape != (B,) or lengths.dtype != torch.int32 or lengths.get_device() != device or (
                 B > 1 and lengths.stride(0) != 1):
             raise ValueError("attention_tree: lengths must be a contiguous (B,) int32 tensor on q's device")
         lens = lengths
@@ -861,23 +868,21 @@ def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             raise ValueError(f"attention_tree: {host_len} cached positions and {N} tokens in a cache of {Tcap}")
     mask_b = 0
     if masks is not None:
-        if masks.shape not in ((N,), (B, N)) or masks.dtype != torch.int64 or masks.device != q.device:
+        if masks.shape not in ((N,), (B, N)) or masks.dtype != torch.int64 or masks.get_device() != device:
             raise ValueError("attention_tree: masks must be an (N,) or (B, N) int64 tensor on q's device")
         if N > 1 and masks.stride(-1) != 1:
             masks = masks.contiguous()
         mask_b = masks.stride(0) if masks.dim() == 2 else 0
     scale = _check_scale("attention_tree", scale)
-    code = _dtype_code(q)
+    code = _DTYPE_CODE[q.dtype]
     L = lib()
-    st = lambda t: ctypes.pointer(_bthd_strides(t))  # noqa: E731
-    with _on_device_of(q):
-        ws_bytes = L.dg_attention_tree_workspace_size(B, N, H, Hkv, Tcap, D, code)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        rc = L.dg_attention_tree(
-            B, N, H, Hkv, Tcap, D, code, _ptr(q), st(q), _ptr(k_cache), st(k_cache), _ptr(v_cache), st(v_cache),
-            _ptr(y), st(y), scale, host_len, _ptr(lens), _ptr(masks), mask_b, _ptr(ws), ws_bytes, _stream(q),
-        )
-    _check(rc, "attention_tree")
+    ws_bytes = L.dg_attention_tree_workspace_size(B, N, H, Hkv, Tcap, D, code)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    st = [ctypes.byref(_bthd_strides(x)) for x in (q, k_cache, v_cache, y)]
+    _launch("attention_tree", device, L.dg_attention_tree, B, N, H, Hkv, Tcap, D, code, q.data_ptr(), st[0],
+            k_cache.data_ptr(), st[1], v_cache.data_ptr(), st[2], y.data_ptr(), st[3], scale, host_len,
+            None if lens is None else lens.data_ptr(), None if masks is None else masks.data_ptr(), mask_b,
+            None if ws is None else ws.data_ptr(), ws_bytes)
 
 
 def token_logprobs_(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, entropy: torch.Tensor | None,
@@ -885,7 +890,7 @@ def token_logprobs_(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Ten
     """dg_token_logprobs: per row of logits (M,V) the log probability of ids (M,) int64 and
     the entropy into (M,) tensors, and with top_logprobs, top_ids (M,top) the most likely
     alternatives.  The results are fp32, fp64 for fp64 logits."""
-    _check_tensors("token_logprobs", logits)
+    device = _check_tensors("token_logprobs", logits)
     if logits.dim() != 2:
         raise ValueError(f"token_logprobs: logits must be (M, V), got {tuple(logits.shape)}")
     M, V = logits.shape
@@ -902,14 +907,11 @@ def token_logprobs_(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Ten
     for name, t, shape, dtype in (("ids", ids, (M,), torch.int64), ("logprobs", logprobs, (M,), out),
                                   ("entropy", entropy, (M,), out), ("top_logprobs", top_logprobs, (M, top), out),
                                   ("top_ids", top_ids, (M, top), torch.int64)):
-        if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != logits.device):
+        if t is not None and (t.dtype != dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous()):
             raise ValueError(f"token_logprobs: {name} must be a contiguous {shape} {dtype} tensor on the logits' device")
-    with _on_device_of(logits):
-        rc = lib().dg_token_logprobs(
-            M, V, _dtype_code(logits), _ptr(logits), logits.stride(0), _ptr(ids), _ptr(logprobs), _ptr(entropy), top,
-            _ptr(top_logprobs), _ptr(top_ids), _stream(logits),
-        )
-    _check(rc, "token_logprobs")
+    _launch("token_logprobs", device, lib().dg_token_logprobs, M, V, _DTYPE_CODE[logits.dtype], logits.data_ptr(),
+            logits.stride(0), ids.data_ptr(), logprobs.data_ptr(), None if entropy is None else entropy.data_ptr(), top,
+            None if top_ids is None else top_logprobs.data_ptr(), None if top_ids is None else top_ids.data_ptr())
 
 
 def copy4d_(src: torch.Tensor, dst: torch.Tensor) -> None:

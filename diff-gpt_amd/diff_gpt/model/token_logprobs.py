@@ -31,13 +31,19 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tok
     if not 0 <= top <= min(V, _native.MAX_TOP):
         raise ValueError(f"token_logprobs: top {top} outside 0 .. min(V, {_native.MAX_TOP})")
     _native.require_device("token_logprobs", logits, ids)
-    x = logits.reshape(-1, V)
+    flat = logits.dim() == 2
+    x = logits if flat else logits.reshape(-1, V)
     if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
     M = x.size(0)
     out = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    new = lambda *s, dtype=out: torch.empty(s, dtype=dtype, device=logits.device)  # noqa: E731
-    r = TokenLogprobs(new(M), new(M), new(M, top), new(M, top, dtype=torch.int64))
-    _native.token_logprobs_(x, ids.reshape(-1).contiguous(), r.logprobs, r.entropy, r.top_logprobs, r.top_ids)
+    device = logits.device
+    r = TokenLogprobs(
+        torch.empty(M, dtype=out, device=device), torch.empty(M, dtype=out, device=device),
+        torch.empty((M, top), dtype=out, device=device), torch.empty((M, top), dtype=torch.int64, device=device),
+    )
+    _native.token_logprobs_(x, ids.reshape(M).contiguous(), *r)
+    if flat:
+        return r
     return TokenLogprobs(r.logprobs.view(lead), r.entropy.view(lead), r.top_logprobs.view(*lead, top),
                          r.top_ids.view(*lead, top))
