@@ -22,8 +22,8 @@
 // The exponent's offset is a whole number of log2 units, raised only where a row's maximum
 // outgrows it by more than kLazyLog2: rescaling by a power of two is exact, so a row's bits
 // do not depend on when its neighbours in the tile made it rescale.  Scores are masked
-// only in key blocks that some row of the wave sees part of; there a value that is not
-// finite leaves the product (0 * inf is NaN) and is added to the rows that see it.
+// only in key blocks that some row of the wave sees part of; values there that are not
+// finite are kept out of the product (clean_stage).
 #include "dg_seq.h"
 #include "dg_prefill.h"
 
@@ -127,14 +127,16 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
   const int row = min(wrow + r32, rend - 1);
   const int qi = row / a.G, qg = row - qi * a.G;
   const int head = pc.kvh * a.G + qg;
-  // keys below `open` every row of the wave sees, from `wend` on none does
-  int open, wend;
+  // keys below `open` every row of the wave sees, from `wend` on none does; below
+  // `first_open` every row of the workgroup
+  int open, wend, first_open;
   uint64_t mask = 0;
   if constexpr (TREE) {
-    open = pc.own;
+    open = first_open = pc.own;
     wend = pc.kend;
     mask = tree_mask(a, pc.b, qi);
   } else {
+    first_open = pc.row0 / a.G + pc.off + 1;
     open = min(wrow, rend - 1) / a.G + pc.off + 1;
     wend = min(wrow + 31, rend - 1) / a.G + pc.off + 1;
   }
@@ -234,14 +236,18 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
       return lim < 0 ? 0u : lim >= 31 ? ~0u : (2u << lim) - 1;
     }
   };
-  // whether the V rows of a 32-key block hold only finite values
-  auto block_finite = [&](const T* vs) __attribute__((always_inline)) -> bool {
+  // A value that is not finite, in a key block that some row sees only part of, would reach
+  // the others as 0 * inf.  Where a stage that crosses `first_open` holds one, it is added
+  // to the outputs of the rows that see its key, and leaves the tile.  Rare, and out of the
+  // products' way; the waves that share tiles take the same path.
+  auto not_finite = [](uint32_t bits) __attribute__((always_inline)) { return (bits & M::kExp) == M::kExp; };
+  auto finite_tile = [&](const T* vs) __attribute__((always_inline)) -> bool {
     const u32x4_t* p = reinterpret_cast<const u32x4_t*>(vs);
     bool fine = true;
     if constexpr (F32) {
       uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 32 * D * ES / 1024; ++i) {
+#pragma unroll 4
+      for (int i = 0; i < TILE * ES / 1024; ++i) {
         const u32x4_t w = p[64 * i + lane];
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = max(top, w[e] & 0x7fffffffu);
@@ -249,8 +255,8 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
       fine = top < M::kExp;
     } else {
       u16x2_t top = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 32 * D * ES / 1024; ++i) {
+#pragma unroll 4
+      for (int i = 0; i < TILE * ES / 1024; ++i) {
         const u32x4_t w = p[64 * i + lane];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -260,13 +266,62 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
     }
     return __builtin_amdgcn_ballot_w64(!fine) == 0;
   };
-  auto not_finite = [](uint32_t bits) __attribute__((always_inline)) { return (bits & M::kExp) == M::kExp; };
+  auto clean_stage = [&](T* st, int t) __attribute__((always_inline)) {
+    const int s0 = pc.kbeg + t * kstep;
+    if (s0 + kstep <= first_open) return;
+    bool fine = true;
+    if constexpr (RT == 1) {
+      fine = finite_tile(st + kg * 2 * TILE + TILE);
+    } else {
+#pragma unroll
+      for (int g = 0; g < KS; ++g) fine = finite_tile(st + g * 2 * TILE + TILE) && fine;
+    }
+    if (fine) return;
+    T* const vs = st + kg * 2 * TILE + TILE;
+#pragma unroll 1
+    for (int j = 0; j < BN; ++j) {
+      const bool sees = (visible(s0 + kg * BN + (j & ~31)) >> (j & 31)) & 1u;
+      const int ksw = seq_swz<PPR, ES>(j);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < (D == 16 ? 8 : 16); ++r) {
+          constexpr int EPP = 16 / ES;
+          const int i = 8 * (r >> 2) + 4 * hh + (r & 3);
+          const int d = F32 ? NB * i + nb : 32 * nb + i;
+          const float x = to_f32(vs[j * D + EPP * ((d / EPP) ^ ksw) + d % EPP]);
+          if (sees && !(__builtin_fabsf(x) < __builtin_huge_valf())) o[nb][r] += x;
+        }
+    }
+    if constexpr (RT > 1) __syncthreads();  // everyone has added
+    u32x4_t* const p = reinterpret_cast<u32x4_t*>(vs);
+#pragma unroll 1
+    for (int i = 0; i < TILE * ES / 1024; ++i) {
+      u32x4_t w = p[64 * i + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (F32) {
+          if (not_finite(w[e])) w[e] = 0u;
+        } else {
+          if (not_finite(w[e])) w[e] &= 0xffff0000u;
+          if (not_finite(w[e] >> 16)) w[e] &= 0x0000ffffu;
+        }
+      }
+      p[64 * i + lane] = w;
+    }
+    if constexpr (RT > 1) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  };
 
   auto compute = [&](const T* st, int k0) __attribute__((always_inline)) {
     const T* Ks = st + kg * 2 * TILE;
     const T* Vs = Ks + TILE;
     floatx16_t s[MB];
-    bool partial[MB];
     // a block past the wave's last key has zeros for K: no product, no weight
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
@@ -292,8 +347,7 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const int kb = k0 + 32 * mb;
-      partial[mb] = kb + 32 > open;
-      if (partial[mb]) {
+      if (kb + 32 > open) {
         const uint32_t vis = visible(kb) >> (4 * hh);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -308,7 +362,8 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
     mt = half_pair_max(mt) * a.scale_log2;
     if (__builtin_amdgcn_ballot_w64(mt > mo + kLazyLog2) != 0) {
       const float mn = mt > mo ? fmaxf(__builtin_floorf(mt), mo) : mo;
-      const float f = mo == kNone ? 0.f : __builtin_amdgcn_exp2f(mo - mn);
+      // no key before: l is 0, and o what clean_stage added
+      const float f = mo == kNone ? 1.f : __builtin_amdgcn_exp2f(mo - mn);
       mo = mn;
       l *= f;
 #pragma unroll
@@ -325,7 +380,6 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
         s[mb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][r], a.scale_log2, -moff));
         l += s[mb][r];
       }
-      const bool dirty = partial[mb] && !block_finite(vb);
       if constexpr (F32) {
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -347,10 +401,7 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
             for (int nb = 0; nb < NB; ++nb) vf[nb] = x[nb];
           }
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (dirty && not_finite(__float_as_uint(vf[nb]))) vf[nb] = 0.f;
-            o[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[nb], s[mb][c], o[nb], 0, 0, 0);
-          }
+          for (int nb = 0; nb < NB; ++nb) o[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[nb], s[mb][c], o[nb], 0, 0, 0);
         }
       } else {
         vec8 pf[2];
@@ -367,36 +418,8 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
           for (int c2 = 0; c2 < 2; ++c2) {
             const uint2 lo = lds_read_tr16(vb + 16 * c2 * D + voff[0][nb]);
             const uint2 hi = lds_read_tr16(vb + 16 * c2 * D + voff[1][nb]);
-            u32x4_t w = {lo.x, lo.y, hi.x, hi.y};
-            if (dirty) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (not_finite(w[e])) w[e] &= 0xffff0000u;
-                if (not_finite(w[e] >> 16)) w[e] &= 0x0000ffffu;
-              }
-            }
-            o[nb] = M::mma(__builtin_bit_cast(vec8, w), pf[c2], o[nb]);
+            o[nb] = M::mma(__builtin_bit_cast(vec8, u32x4_t{lo.x, lo.y, hi.x, hi.y}), pf[c2], o[nb]);
           }
-      }
-      if (dirty) {
-        // the values that left the product, added to the rows that see them
-        const uint32_t vis = visible(k0 + 32 * mb);
-        for (int j = 0; j < 32; ++j) {
-          const T* vrow = vb + j * D;
-          const int ksw = seq_swz<PPR, ES>(32 * mb + j);
-          const bool sees = (vis >> j) & 1u;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int r = 0; r < (D == 16 ? 8 : 16); ++r) {
-              const int i = 8 * (r >> 2) + 4 * hh + (r & 3);
-              const int d = F32 ? NB * i + nb : 32 * nb + i;
-              constexpr int EPP = 16 / ES;
-              const T x = vrow[EPP * ((d / EPP) ^ ksw) + d % EPP];
-              const float xv = to_f32(x);
-              if (sees && !(__builtin_fabsf(xv) < __builtin_huge_valf())) o[nb][r] += xv;
-            }
-        }
       }
     }
   };
@@ -405,10 +428,12 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
   for (int t = 0; t < nstage; t += 2) {
     const int k0 = kfirst + t * kstep;
     if (t + 1 < nstage) copy_stage(kv1, k0 + kstep);
+    clean_stage(kv0, t);
     if (k0 < wend) compute(kv0, k0);
     stage_ready();  // stage 1 filled; every wave is done with stage 0
     if (t + 1 >= nstage) break;
     if (t + 2 < nstage) copy_stage(kv0, k0 + 2 * kstep);
+    clean_stage(kv1, t + 1);
     if (k0 + kstep < wend) compute(kv1, k0 + kstep);
     stage_ready();
   }

@@ -69,7 +69,7 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, int64_t tile0, SeqPi
     u /= a.nrb;
     p.kvh = (int)(u % a.Hkv);
     p.b = u / a.Hkv;
-    const int len = a.lens != nullptr ? a.lens[p.b] : a.len;
+    const int len = a.lens != nullptr ? __builtin_amdgcn_readfirstlane(a.lens[p.b]) : a.len;
     p.own = min(max(len, 0), a.Tcap - a.N);
     p.row0 = rb * a.rows_per_wg;
     p.rows = min(a.rows_per_wg, a.N * a.G - p.row0);
@@ -79,7 +79,13 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, int64_t tile0, SeqPi
     p.q0 = p.k0 = 0;
     return p.kbeg < p.kend;
   } else {
-    const dg_packed_tile t = a.tiles[tile0 + blockIdx.x];
+    dg_packed_tile t = a.tiles[tile0 + blockIdx.x];
+    t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
+    t.lq = __builtin_amdgcn_readfirstlane(t.lq);
+    t.k0 = __builtin_amdgcn_readfirstlane(t.k0);
+    t.lk = __builtin_amdgcn_readfirstlane(t.lk);
+    t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
+    t.rows = __builtin_amdgcn_readfirstlane(t.rows);
     p.kvh = blockIdx.y;
     p.split = 0;
     p.b = 0;
