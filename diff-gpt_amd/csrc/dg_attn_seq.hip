@@ -14,7 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
-#include <numeric>
+#include <exception>
 #include <vector>
 
 namespace dg {
@@ -141,30 +141,34 @@ __global__ __launch_bounds__(256) void seq_vec_kernel(const SeqArgs a) {
   }
 }
 
-// The splits of a row joined: a wavefront per row, lanes along the head.  A row's used
-// splits follow from its length, so what the workspace held before does not matter.
-template <typename T>
+// The splits of a row joined: WPR wavefronts a row, each over every WPR-th split, lanes
+// along the head.  A row's used splits follow from its length, so what the workspace held
+// before does not matter.  A split's weight is computed once, by the lane of its number.
+template <typename T, int WPR>
 __global__ __launch_bounds__(256) void seq_join_kernel(const SeqArgs a, const int64_t nrows) {
   using S = SeqAcc<T>;
   using A = typename S::type;
+  __shared__ A part[WPR > 1 ? 3 * kMaxHeadDim : 1];
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= nrows) return;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = WPR > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wv;
+  if (row >= nrows) return;  // WPR > 1: whole workgroups
+  const int sub = WPR > 1 ? wv : 0;
   const int R = a.N * a.G;
   const int r = (int)(row % R);
   const int64_t bh = row / R;
   const int kvh = (int)(bh % a.Hkv);
   const int64_t b = bh / a.Hkv;
   const int i = r / a.G, h = kvh * a.G + r % a.G;
-  const int own = min(max(a.lens != nullptr ? a.lens[b] : a.len, 0), a.Tcap - a.N);
+  const int len = a.lens != nullptr ? __builtin_amdgcn_readfirstlane(a.lens[b]) : a.len;
+  const int own = min(max(len, 0), a.Tcap - a.N);
   const int used = min(a.nsplit, (own + a.N + a.chunk - 1) / a.chunk);
   const A* ml = static_cast<const A*>(a.ws_ml) + 2 * row * a.nsplit;
   const A* wo = static_cast<const A*>(a.ws_o) + row * a.nsplit * a.D;
   A m = neg_inf<A>();
   bool bad = false;
   for (int s = lane; s < used; s += 64) {
-    const A ms = ml[2 * s];
-    const A ls = ml[2 * s + 1];
+    const A ms = ml[2 * s], ls = ml[2 * s + 1];
     bad = bad || ms != ms || ls != ls;  // a NaN score
     m = ms > m ? ms : m;
   }
@@ -174,21 +178,47 @@ __global__ __launch_bounds__(256) void seq_join_kernel(const SeqArgs a, const in
     m = m2 > m ? m2 : m;
   }
   bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-  A l = (A)0;
-  for (int s = 0; s < used; ++s) {
-    const A ms = ml[2 * s];
-    if (ms != neg_inf<A>()) l += ml[2 * s + 1] * S::exp(ms - m);
+  constexpr int ND = kMaxHeadDim / 64;
+  A o[ND], l = (A)0;
+#pragma unroll
+  for (int c = 0; c < ND; ++c) o[c] = (A)0;
+  for (int s0 = 0; s0 < used; s0 += 64) {
+    const int s = s0 + lane;
+    const A ms = s < used ? ml[2 * s] : neg_inf<A>();
+    const A w = ms == neg_inf<A>() ? (A)0 : S::exp(ms - m);
+    if (ms != neg_inf<A>()) l += ml[2 * s + 1] * w;
+    const int n = min(64, used - s0);
+#pragma unroll 4
+    for (int t = sub; t < n; t += WPR) {
+      const A wt = __shfl(w, t, 64);
+#pragma unroll
+      for (int c = 0; c < ND; ++c)
+        if (64 * c < a.D && lane + 64 * c < a.D) {
+          const A x = wo[(int64_t)(s0 + t) * a.D + lane + 64 * c];
+          o[c] += wt == (A)0 ? (A)0 : wt * x;  // a split without a key, or of no weight
+        }
+    }
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x, 64);
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int c = 0; c < ND; ++c)
+      if (sub > 0 && lane + 64 * c < a.D) part[(sub - 1) * kMaxHeadDim + lane + 64 * c] = o[c];
+    __syncthreads();
+    if (sub > 0) return;
+#pragma unroll
+    for (int c = 0; c < ND; ++c)
+#pragma unroll
+      for (int w = 0; w < WPR - 1; ++w)
+        if (lane + 64 * c < a.D) o[c] += part[w * kMaxHeadDim + lane + 64 * c];
   }
   const bool none = own == 0 && tree_mask(a, b, i) == 0;
   T* yp = static_cast<T*>(a.y) + b * a.yb + i * a.yt + (int64_t)h * a.yh;
-  for (int d = lane; d < a.D; d += 64) {
-    A o = (A)0;
-    for (int s = 0; s < used; ++s) {
-      const A ms = ml[2 * s];
-      if (ms != neg_inf<A>()) o += wo[(int64_t)s * a.D + d] * S::exp(ms - m);
-    }
-    yp[d] = S::store(none ? (A)0 : bad ? (A)__builtin_nanf("") : o / l);
-  }
+#pragma unroll
+  for (int c = 0; c < ND; ++c)
+    if (lane + 64 * c < a.D)
+      yp[lane + 64 * c] = S::store(none ? (A)0 : bad ? (A)__builtin_nanf("") : o[c] / l);
 }
 
 namespace {
@@ -217,21 +247,22 @@ int launch_vec_any(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
 }
 
 constexpr int kWideRows = 128;   // rows of a wide tile
-constexpr int kNarrowRows = 32;  // most rows of a narrow one
+constexpr int kNarrowRows = 32;  // rows of a narrow one
 constexpr int kVecRows = 32;    // rows of a workgroup of the vector kernel over a tree
 
-// Workgroups that a split aims at: two for each of the 256 CUs.  A split's length is a
-// multiple of 128 keys, at least 256, so that joining it costs little beside reading it.
+// Workgroups that a split aims at: two for each of the 256 CUs.  A split is whole stages
+// of the kernel, kMinStages of them at least, which joining it (a launch of its own, some
+// 5 us) costs about as much as.
 constexpr int64_t kSplitWorkgroups = 512;
+constexpr int kMinStages = 8;
 constexpr int kMaxSplits = 512;
 
-int tree_chunk(int64_t B, int Hkv, int nrb, int keys) {
+int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int stage) {
   const int64_t wg = B * Hkv * nrb;
   const int64_t want = (kSplitWorkgroups + wg - 1) / wg;  // splits of a row
-  int64_t chunk = (keys + want - 1) / want;
-  chunk = std::max<int64_t>(chunk, (keys + kMaxSplits - 1) / kMaxSplits);
-  chunk = std::max<int64_t>((chunk + 127) / 128 * 128, 256);
-  return (int)std::min<int64_t>(chunk, 0x7fffff80);
+  int64_t chunk = std::max<int64_t>((keys + want - 1) / want, (keys + kMaxSplits - 1) / kMaxSplits);
+  chunk = std::max<int64_t>((chunk + stage - 1) / stage, kMinStages) * stage;
+  return (int)std::min<int64_t>(chunk, 0x7fffff00);
 }
 
 // Row blocks, splits and workspace of a call.
@@ -240,12 +271,16 @@ struct TreeShape {
   size_t o_bytes, ws_bytes;
 };
 
+// A stage's keys where a workgroup holds so many rows: 128 and fewer (the vector kernel's
+// waves, which take 32 rows one after the other, have no stages).
+constexpr int stage_keys(int rows_per_wg) { return rows_per_wg == 32 ? 128 : 64; }
+
 TreeShape tree_shape(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype, int rows_per_wg) {
   TreeShape t{};
   const int R = N * (H / Hkv);
   t.rows_per_wg = rows_per_wg;
   t.nrb = (R + rows_per_wg - 1) / rows_per_wg;
-  t.chunk = tree_chunk(B, Hkv, t.nrb, Tcap);
+  t.chunk = tree_chunk(B, Hkv, t.nrb, Tcap, stage_keys(rows_per_wg));
   t.nsplit = (int)(((int64_t)Tcap + t.chunk - 1) / t.chunk);
   const size_t acc = dtype == DG_F64 ? 8 : 4;
   const size_t parts = (size_t)B * Hkv * R * t.nsplit;
@@ -272,43 +307,93 @@ size_t tree_workspace(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dty
 
 using namespace dg;
 
+namespace dg {
+namespace {
+
+// The tiles of a batch in launch order.  Workgroup x of key head h takes entry
+// 8 (x / 8) + (x - h) mod 8 (seq_piece), and workgroup x runs on XCD x mod 8: entry e is of
+// list e mod 8, and each key head of a list's sequences has an XCD, and its L2, to itself.
+// Sequences go whole to the list with the least work so far, longest first; a long one,
+// which would leave lists unequal, tile by tile.  Lists are filled up with empty tiles.
+std::vector<dg_packed_tile> plan_tiles(int64_t S, const int64_t* lq, const int64_t* lk, int group, bool* narrow) {
+  int64_t longest = 0, q0 = 0, k0 = 0;
+  for (int64_t s = 0; s < S; ++s) longest = std::max(longest, lq[s] * group);
+  // Workgroups that split the keys (32 rows) only where no sequence has more rows: beside
+  // wide ones they would be a launch of their own, and a wide one takes as long over as
+  // many keys with fewer rows.
+  *narrow = longest <= kNarrowRows;
+  struct Seq {
+    int64_t q0, k0, lq, lk, work;
+  };
+  std::vector<Seq> seqs;
+  int64_t total = 0;
+  for (int64_t s = 0; s < S; ++s) {
+    if (lq[s] > 0) {
+      const int64_t work = lq[s] * (std::max<int64_t>(0, lk[s] - lq[s] / 2) + 32);
+      seqs.push_back(Seq{q0, k0, lq[s], lk[s], work});
+      total += work;
+    }
+    q0 += lq[s];
+    k0 += lk[s];
+  }
+  std::stable_sort(seqs.begin(), seqs.end(), [](const Seq& a, const Seq& b) { return a.work > b.work; });
+  std::vector<dg_packed_tile> lists[8];
+  int64_t load[8] = {};
+  auto least = [&]() { return (int)(std::min_element(load, load + 8) - load); };
+  for (const Seq& s : seqs) {
+    const int64_t rows = s.lq * group, tiles = (rows + kWideRows - 1) / kWideRows;
+    const bool apart = s.work > total / 32;
+    int at = least();
+    for (int64_t t = tiles - 1; t >= 0; --t) {  // a sequence's last queries see the most keys
+      const int64_t r = t * kWideRows, n = std::min<int64_t>(kWideRows, rows - r);
+      if (apart) at = least();
+      lists[at].push_back(dg_packed_tile{(int32_t)s.q0, (int32_t)s.lq, (int32_t)s.k0, (int32_t)s.lk, (int32_t)r,
+                                         (int32_t)n, {0, 0}});
+      load[at] += std::max<int64_t>(0, (r + n - 1) / group + s.lk - s.lq + 1) + 32;
+    }
+  }
+  size_t most = 0;
+  for (const auto& l : lists) most = std::max(most, l.size());
+  std::vector<dg_packed_tile> out(8 * most, dg_packed_tile{});
+  for (size_t i = 0; i < most; ++i)
+    for (int c = 0; c < 8; ++c)
+      if (i < lists[c].size()) out[8 * i + c] = lists[c][i];
+  return out;
+}
+
+}  // namespace
+}  // namespace dg
+
 extern "C" int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, int group, dg_packed_tile* tiles,
                               int64_t cap, int64_t* counts) {
   DG_REQUIRE(S >= 0 && group >= 1 && cap >= 0, DG_EINVAL, "packed_plan: negative size or group");
   DG_REQUIRE(counts != nullptr && (S == 0 || (lq != nullptr && lk != nullptr)) && (cap == 0 || tiles != nullptr),
              DG_EINVAL, "packed_plan: NULL argument");
-  int64_t nq = 0, nk = 0;
+  int64_t nq = 0, nk = 0, n = 0;
   for (int64_t s = 0; s < S; ++s) {
     DG_REQUIRE(lq[s] >= 0 && lk[s] >= 0, DG_EINVAL, "packed_plan: sequence %lld has a negative length", (long long)s);
     DG_REQUIRE(lq[s] <= 0x7fffffff / group, DG_EINVAL, "packed_plan: sequence %lld has too many rows", (long long)s);
+    DG_REQUIRE(lk[s] <= 0x7fffffff, DG_EINVAL, "packed_plan: sequence %lld has too many keys", (long long)s);
     nq += lq[s];
     nk += lk[s];
     DG_REQUIRE(nq <= 0x7fffffff && nk <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 rows");
+    n += (lq[s] * group + kWideRows - 1) / kWideRows;
+    DG_REQUIRE(n <= 0x7fffffff / 8, DG_EINVAL, "packed_plan: more than 2^28 tiles");
   }
-  int64_t wide = 0, narrow = 0;
-  for (int64_t s = 0; s < S; ++s) {
-    const int64_t rows = lq[s] * group, rest = rows % kWideRows;
-    wide += rows / kWideRows + (rest > kNarrowRows);
-    narrow += rest > 0 && rest <= kNarrowRows;
+  try {
+    bool narrow = false;
+    const std::vector<dg_packed_tile> plan = plan_tiles(S, lq, lk, group, &narrow);
+    counts[0] = narrow ? 0 : (int64_t)plan.size();
+    counts[1] = narrow ? (int64_t)plan.size() : 0;
+    if (tiles == nullptr) return DG_OK;
+    DG_REQUIRE(cap >= (int64_t)plan.size(), DG_EINVAL, "packed_plan: room for %lld tiles, %lld needed", (long long)cap,
+               (long long)plan.size());
+    std::copy(plan.begin(), plan.end(), tiles);
+    return DG_OK;
+  } catch (const std::exception& e) {
+    set_error("packed_plan: %s", e.what());
+    return DG_EWORKSPACE;
   }
-  const int64_t n = wide + narrow;
-  DG_REQUIRE(n <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 tiles");
-  counts[0] = wide;
-  counts[1] = narrow;
-  if (tiles == nullptr) return DG_OK;
-  DG_REQUIRE(cap >= n, DG_EINVAL, "packed_plan: room for %lld tiles, %lld needed", (long long)cap, (long long)n);
-  int64_t at = 0, at_narrow = wide, q0 = 0, k0 = 0;
-  for (int64_t s = 0; s < S; ++s) {
-    const int64_t rows = lq[s] * group;
-    for (int64_t r = 0; r < rows; r += kWideRows) {
-      const int64_t some = std::min<int64_t>(kWideRows, rows - r);
-      tiles[some <= kNarrowRows ? at_narrow++ : at++] = dg_packed_tile{
-          (int32_t)q0, (int32_t)lq[s], (int32_t)k0, (int32_t)lk[s], (int32_t)r, (int32_t)some, {0, 0}};
-    }
-    q0 += lq[s];
-    k0 += lk[s];
-  }
-  return DG_OK;
 }
 
 extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D, int dtype, const void* q, int64_t q_t,
@@ -321,6 +406,9 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "attention_packed: %d query heads on %d key heads", H, Hkv);
   DG_REQUIRE(Hkv <= 65535, DG_EINVAL, "attention_packed: %d key heads, at most 65535", Hkv);
   DG_REQUIRE(scale > 0.f && std::isfinite(scale), DG_EINVAL, "attention_packed: the scale must be positive");
+  DG_REQUIRE(n_wide <= 0x7fffffff && n_narrow <= 0x7fffffff && n_wide % 8 == 0 && n_narrow % 8 == 0, DG_EINVAL,
+             "attention_packed: %lld and %lld tiles, multiples of 8 up to 2^31 - 1 from dg_packed_plan", (long long)n_wide,
+             (long long)n_narrow);
   DG_REQUIRE(n_wide + n_narrow <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 tiles");
   if (Nq == 0 || H == 0 || n_wide + n_narrow == 0) return DG_OK;
   DG_REQUIRE(q && y && tiles && (Nk == 0 || (k && v)), DG_EINVAL, "attention_packed: NULL argument");
@@ -392,11 +480,20 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
                       : launch_vec_any<true>(a, dtype, dim3((unsigned)blocks), s);
   if (rc != DG_OK || t.nsplit == 1) return rc;
   const int64_t rows = (int64_t)B * H * N;
-  DG_REQUIRE((rows + 3) / 4 <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
-  const dim3 grid((unsigned)((rows + 3) / 4));
-  if (dtype == DG_F64) hipLaunchKernelGGL(seq_join_kernel<double>, grid, dim3(256), 0, s, a, rows);
-  else if (dtype == DG_F32) hipLaunchKernelGGL(seq_join_kernel<float>, grid, dim3(256), 0, s, a, rows);
-  else if (dtype == DG_BF16) hipLaunchKernelGGL(seq_join_kernel<bf16_t>, grid, dim3(256), 0, s, a, rows);
-  else hipLaunchKernelGGL(seq_join_kernel<f16_t>, grid, dim3(256), 0, s, a, rows);
+  // a row's waves read its splits in turn: four of them where there are many
+  const bool many = t.nsplit >= 8;
+  const int64_t groups = many ? rows : (rows + 3) / 4;
+  DG_REQUIRE(groups <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
+  const dim3 grid((unsigned)groups);
+#define DG_JOIN(T)                                                                                      \
+  do {                                                                                                  \
+    if (many) hipLaunchKernelGGL((seq_join_kernel<T, 4>), grid, dim3(256), 0, s, a, rows);              \
+    else hipLaunchKernelGGL((seq_join_kernel<T, 1>), grid, dim3(256), 0, s, a, rows);                   \
+  } while (0)
+  if (dtype == DG_F64) DG_JOIN(double);
+  else if (dtype == DG_F32) DG_JOIN(float);
+  else if (dtype == DG_BF16) DG_JOIN(bf16_t);
+  else DG_JOIN(f16_t);
+#undef DG_JOIN
   return check_launch("seq_join_kernel");
 }

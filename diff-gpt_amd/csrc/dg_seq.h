@@ -56,7 +56,7 @@ struct SeqPiece {
   int kvh, split;
 };
 
-// The piece of this workgroup (packed: tile tile0 + blockIdx.x); false where there is nothing to do.  Nothing a table or
+// The piece of this workgroup (packed: a tile from tile0 on); false where there is nothing to do.  Nothing a table or
 // a length in device memory says takes an access outside q, k, v and y: tiles that do
 // not lie inside them are left out, lengths beyond the cache are taken as its end.
 template <bool TREE>
@@ -79,7 +79,8 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, int64_t tile0, SeqPi
     p.q0 = p.k0 = 0;
     return p.kbeg < p.kend;
   } else {
-    dg_packed_tile t = a.tiles[tile0 + blockIdx.x];
+    // which entry: dg_packed_plan's lists, an XCD further for each key head
+    dg_packed_tile t = a.tiles[tile0 + (blockIdx.x & ~7u) + ((blockIdx.x - blockIdx.y) & 7u)];
     t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
     t.lq = __builtin_amdgcn_readfirstlane(t.lq);
     t.k0 = __builtin_amdgcn_readfirstlane(t.k0);

@@ -586,10 +586,10 @@ DG_API int dg_draw_argmax(int64_t M, int V, int dtype, const void* probs, int64_
  *
  * dg_packed_plan lays the work out once per batch, on the host and without the device: it
  * writes the tiles of the sequences for heads in groups of `group` into `tiles` (room for
- * `cap`; NULL with cap 0 only counts) and counts[0] wide ones, which come first, and
- * counts[1] narrow ones.  The caller copies the table to the device and hands it to every
- * dg_attention_packed over such a batch.  A tile that does not lie inside Nq and Nk rows
- * is skipped, never followed.
+ * `cap`; NULL with cap 0 only counts): counts[0] wide ones, which come first, and counts[1]
+ * narrow ones, each a multiple of 8 (some are empty).  The caller copies the table to the
+ * device and hands it with its counts to every dg_attention_packed over such a batch.  A
+ * tile that does not lie inside Nq and Nk rows is skipped, never followed.
  * fp32 / bf16 / fp16 / fp64, every head_dim up to 1024, rows with unit stride over d; the
  * scale is positive.
  */

@@ -102,7 +102,7 @@ def _st(b=16, t=16, h=16):
     return ctypes.pointer(_native.Stride3(b, t, h))
 
 
-def _packed(Nq=4, Nk=4, H=1, Hkv=1, D=16, dtype=0, p=FAKE, scale=1.0, tiles=FAKE, wide=1, narrow=0):
+def _packed(Nq=4, Nk=4, H=1, Hkv=1, D=16, dtype=0, p=FAKE, scale=1.0, tiles=FAKE, wide=8, narrow=0):
     return _native.lib().dg_attention_packed(Nq, Nk, H, Hkv, D, dtype, p, 16, 16, p, 16, 16, p, 16, 16, p, 16, 16, scale,
                                              tiles, wide, narrow, NUL)
 
@@ -115,7 +115,7 @@ def _tree(B=1, N=2, H=1, Hkv=1, Tcap=8, D=16, dtype=0, p=FAKE, scale=1.0, length
 @pytest.mark.parametrize("kw,rc", [(dict(Nq=-1), -1), (dict(dtype=9), -2), (dict(D=0), -2), (dict(D=1025), -2),
                                    (dict(H=3, Hkv=2), -1), (dict(Hkv=0), -1), (dict(scale=0.0), -1),
                                    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(p=NUL), -1),
-                                   (dict(tiles=NUL), -1), (dict(wide=-1), -1), (dict(Nq=0), 0), (dict(wide=0), 0),
+                                   (dict(tiles=NUL), -1), (dict(wide=-1), -1), (dict(wide=1), -1), (dict(Nq=0), 0), (dict(wide=0), 0),
                                    (dict(H=0), 0)])
 def test_packed_refusals(kw, rc):
     assert _packed(**kw) == rc
