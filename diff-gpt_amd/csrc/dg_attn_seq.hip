@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void seq_vec_kernel(const SeqArgs a) {
   using A = typename S::type;
   constexpr int KPW = 64 / LPK;
   SeqPiece p;
-  if (!seq_piece<TREE>(a, 0, p)) return;
+  if (!seq_piece<TREE>(a, p)) return;
   const int lane = threadIdx.x & 63, kl = lane / LPK, dl = lane % LPK;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* kp = static_cast<const T*>(a.k) + p.b * a.kb + p.k0 * a.kt + (int64_t)p.kvh * a.kh;
@@ -221,7 +221,98 @@ __global__ __launch_bounds__(256) void seq_join_kernel(const SeqArgs a, const in
       yp[lane + 64 * c] = S::store(none ? (A)0 : bad ? (A)__builtin_nanf("") : o[c] / l);
 }
 
+// The same for the head dims of the matrix-core kernel: a lane reads four elements of a
+// split at a time, so that a wave reads 64 / (D / 4) splits at once, and lengths and states
+// are in flight together (those of unused splits are read and not looked at).  WPR waves a
+// row as above.
+template <typename T, int D, int WPR>
+__global__ __launch_bounds__(256) void seq_join4_kernel(const SeqArgs a, const int64_t nrows) {
+  constexpr int LPS = D / 4, SPW = 64 / LPS;  // lanes a split, splits a wave
+  __shared__ float part[WPR > 1 ? (WPR - 1) * D : 1];
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = WPR > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wv;
+  if (row >= nrows) return;  // WPR > 1: whole workgroups
+  const int sub = WPR > 1 ? wv : 0;
+  const int R = a.N * a.G;
+  const int64_t bh = row / R;
+  const int r = (int)(row - bh * R);
+  const int64_t b = bh / a.Hkv;
+  const int kvh = (int)(bh - b * a.Hkv);
+  const int i = r / a.G, h = kvh * a.G + (r - i * a.G);
+  const u32x2_t* ml = static_cast<const u32x2_t*>(a.ws_ml) + row * a.nsplit;
+  const float* wo = static_cast<const float*>(a.ws_o) + row * a.nsplit * D;
+  u32x2_t first = {0u, 0u};
+  if (lane < a.nsplit) first = ml[lane];
+  const int len = a.lens != nullptr ? a.lens[b] : a.len;
+  const int own = min(max(__builtin_amdgcn_readfirstlane(len), 0), a.Tcap - a.N);
+  const int used = min(a.nsplit, (own + a.N + a.chunk - 1) / a.chunk);
+  auto state = [&](int s0, float& ms, float& ls) __attribute__((always_inline)) {
+    const int s = s0 + lane;
+    u32x2_t x = first;
+    if (s0 > 0 && s < used) x = ml[s];
+    ms = s < used ? __uint_as_float(x[0]) : kNegInf;
+    ls = s < used ? __uint_as_float(x[1]) : 0.f;
+  };
+  float m = kNegInf;
+  bool bad = false;
+  for (int s0 = 0; s0 < used; s0 += 64) {
+    float ms, ls;
+    state(s0, ms, ls);
+    bad = bad || ms != ms || ls != ls;  // a NaN score
+    m = fmaxf(m, ms);
+  }
+  m = wave_max(m);
+  bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  const int ls4 = lane / LPS, d4 = 4 * (lane % LPS);
+  for (int s0 = 0; s0 < used; s0 += 64) {
+    float ms, ls;
+    state(s0, ms, ls);
+    const float w = ms == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+    l += ms == kNegInf ? 0.f : ls * w;
+    const int n = min(64, used - s0);
+#pragma unroll 4
+    for (int t0 = sub * SPW; t0 < n; t0 += WPR * SPW) {
+      const int t = t0 + ls4;
+      const float wt = __shfl(w, t & 63, 64);
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(wo + (int64_t)(s0 + min(t, n - 1)) * D + d4);
+      const bool in = t < n && wt != 0.f;  // a split without a key, or of no weight, adds nothing
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += in ? wt * x[e] : 0.f;
+    }
+  }
+  l = group_sum_dpp<64>(l);
+#pragma unroll
+  for (int x = LPS; x < 64; x <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x, 64);
+  if constexpr (WPR > 1) {
+    if (sub > 0 && ls4 == 0) *reinterpret_cast<f32x4_t*>(part + (sub - 1) * D + d4) = o;
+    __syncthreads();
+    if (sub > 0) return;
+#pragma unroll
+    for (int w = 0; w < WPR - 1; ++w) o += *reinterpret_cast<const f32x4_t*>(part + w * D + d4);
+  }
+  if (ls4 != 0) return;
+  const bool none = own == 0 && tree_mask(a, b, i) == 0;
+  T* yp = static_cast<T*>(a.y) + b * a.yb + i * a.yt + (int64_t)h * a.yh;
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = none ? 0.f : bad ? __builtin_nanf("") : o[e] / l;
+  store_vec<T, 4>(yp + d4, y);
+}
+
 namespace {
+
+template <typename T, int WPR>
+void launch_join4(const SeqArgs& a, dim3 grid, int64_t rows, hipStream_t s) {
+  if (a.D == 16) hipLaunchKernelGGL((seq_join4_kernel<T, 16, WPR>), grid, dim3(256), 0, s, a, rows);
+  else if (a.D == 32) hipLaunchKernelGGL((seq_join4_kernel<T, 32, WPR>), grid, dim3(256), 0, s, a, rows);
+  else if (a.D == 64) hipLaunchKernelGGL((seq_join4_kernel<T, 64, WPR>), grid, dim3(256), 0, s, a, rows);
+  else hipLaunchKernelGGL((seq_join4_kernel<T, 128, WPR>), grid, dim3(256), 0, s, a, rows);
+}
 
 template <typename T, bool TREE>
 int launch_vec(const SeqArgs& a, dim3 grid, hipStream_t s) {
@@ -246,22 +337,29 @@ int launch_vec_any(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
   return launch_vec<f16_t, TREE>(a, grid, s);
 }
 
-constexpr int kWideRows = 128;   // rows of a wide tile
-constexpr int kNarrowRows = 32;  // rows of a narrow one
 constexpr int kVecRows = 32;    // rows of a workgroup of the vector kernel over a tree
 
-// Workgroups that a split aims at: two for each of the 256 CUs.  A split is whole stages
-// of the kernel, kMinStages of them at least, which joining it (a launch of its own, some
-// 5 us) costs about as much as.
-constexpr int64_t kSplitWorkgroups = 512;
-constexpr int kMinStages = 8;
+// Splits of a row: enough workgroups to fill the CUs as far as their LDS and registers let
+// them share one (256 of 128 KB, as many more as smaller ones fit), and at least so many
+// stages each that joining the splits, a launch of its own of some 6 us, costs no more than
+// it saves: 8, fewer where fp32 products make a stage long.  us at 256 / 512 / 1024
+// workgroups, bf16:
+//   rows of 32, head_dim 128 (64 rows, 4 key heads, lengths to 4096)    52.1 / 58.6 / 68.3
+//               head_dim  64 (64 rows, 8 key heads, lengths to 1024)    17.2 / 17.0 / 25.3
+//           64, head_dim  64 (16 rows, 8 key heads, lengths to 4096)    31.7 / 26.2 / 28.1
+//          128, head_dim 128 (16 rows, 4 key heads, lengths to 7168)    57.3 / 45.2 / 41.1
+//               head_dim  64 (2 rows, 2 key heads, lengths to 131000)   77.1 / 62.3 / 61.2
 constexpr int kMaxSplits = 512;
 
-int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int stage) {
+int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int rows_per_wg, int D, int dtype) {
+  const int stage = rows_per_wg == 32 ? 128 : 64;  // keys; the vector kernel has no stages
+  const int64_t row_bytes = D * dtype_bytes(dtype);
+  const int64_t fill = rows_per_wg == 32 ? (row_bytes >= 256 ? 256 : 512) : rows_per_wg == 64 ? 512 : D == 128 ? 768 : 1024;
+  const int64_t least = dtype == DG_F32 ? std::max(2, std::min(8, 256 / D)) : 8;
   const int64_t wg = B * Hkv * nrb;
-  const int64_t want = (kSplitWorkgroups + wg - 1) / wg;  // splits of a row
+  const int64_t want = (fill + wg - 1) / wg;
   int64_t chunk = std::max<int64_t>((keys + want - 1) / want, (keys + kMaxSplits - 1) / kMaxSplits);
-  chunk = std::max<int64_t>((chunk + stage - 1) / stage, kMinStages) * stage;
+  chunk = std::max<int64_t>((chunk + stage - 1) / stage, least) * stage;
   return (int)std::min<int64_t>(chunk, 0x7fffff00);
 }
 
@@ -271,16 +369,12 @@ struct TreeShape {
   size_t o_bytes, ws_bytes;
 };
 
-// A stage's keys where a workgroup holds so many rows: 128 and fewer (the vector kernel's
-// waves, which take 32 rows one after the other, have no stages).
-constexpr int stage_keys(int rows_per_wg) { return rows_per_wg == 32 ? 128 : 64; }
-
 TreeShape tree_shape(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype, int rows_per_wg) {
   TreeShape t{};
   const int R = N * (H / Hkv);
   t.rows_per_wg = rows_per_wg;
   t.nrb = (R + rows_per_wg - 1) / rows_per_wg;
-  t.chunk = tree_chunk(B, Hkv, t.nrb, Tcap, stage_keys(rows_per_wg));
+  t.chunk = tree_chunk(B, Hkv, t.nrb, Tcap, rows_per_wg, D, dtype);
   t.nsplit = (int)(((int64_t)Tcap + t.chunk - 1) / t.chunk);
   const size_t acc = dtype == DG_F64 ? 8 : 4;
   const size_t parts = (size_t)B * Hkv * R * t.nsplit;
@@ -315,13 +409,8 @@ namespace {
 // list e mod 8, and each key head of a list's sequences has an XCD, and its L2, to itself.
 // Sequences go whole to the list with the least work so far, longest first; a long one,
 // which would leave lists unequal, tile by tile.  Lists are filled up with empty tiles.
-std::vector<dg_packed_tile> plan_tiles(int64_t S, const int64_t* lq, const int64_t* lk, int group, bool* narrow) {
-  int64_t longest = 0, q0 = 0, k0 = 0;
-  for (int64_t s = 0; s < S; ++s) longest = std::max(longest, lq[s] * group);
-  // Workgroups that split the keys (32 rows) only where no sequence has more rows: beside
-  // wide ones they would be a launch of their own, and a wide one takes as long over as
-  // many keys with fewer rows.
-  *narrow = longest <= kNarrowRows;
+std::vector<dg_packed_tile> plan_tiles(int64_t S, const int64_t* lq, const int64_t* lk, int group) {
+  int64_t q0 = 0, k0 = 0;
   struct Seq {
     int64_t q0, k0, lq, lk, work;
   };
@@ -341,11 +430,11 @@ std::vector<dg_packed_tile> plan_tiles(int64_t S, const int64_t* lq, const int64
   int64_t load[8] = {};
   auto least = [&]() { return (int)(std::min_element(load, load + 8) - load); };
   for (const Seq& s : seqs) {
-    const int64_t rows = s.lq * group, tiles = (rows + kWideRows - 1) / kWideRows;
+    const int64_t rows = s.lq * group, tiles = (rows + kTileRows - 1) / kTileRows;
     const bool apart = s.work > total / 32;
     int at = least();
     for (int64_t t = tiles - 1; t >= 0; --t) {  // a sequence's last queries see the most keys
-      const int64_t r = t * kWideRows, n = std::min<int64_t>(kWideRows, rows - r);
+      const int64_t r = t * kTileRows, n = std::min<int64_t>(kTileRows, rows - r);
       if (apart) at = least();
       lists[at].push_back(dg_packed_tile{(int32_t)s.q0, (int32_t)s.lq, (int32_t)s.k0, (int32_t)s.lk, (int32_t)r,
                                          (int32_t)n, {0, 0}});
@@ -377,14 +466,15 @@ extern "C" int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, i
     nq += lq[s];
     nk += lk[s];
     DG_REQUIRE(nq <= 0x7fffffff && nk <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 rows");
-    n += (lq[s] * group + kWideRows - 1) / kWideRows;
+    n += (lq[s] * group + kTileRows - 1) / kTileRows;
     DG_REQUIRE(n <= 0x7fffffff / 8, DG_EINVAL, "packed_plan: more than 2^28 tiles");
   }
   try {
-    bool narrow = false;
-    const std::vector<dg_packed_tile> plan = plan_tiles(S, lq, lk, group, &narrow);
-    counts[0] = narrow ? 0 : (int64_t)plan.size();
-    counts[1] = narrow ? (int64_t)plan.size() : 0;
+    const std::vector<dg_packed_tile> plan = plan_tiles(S, lq, lk, group);
+    counts[0] = (int64_t)plan.size();
+    counts[1] = n;
+    counts[2] = 0;
+    for (const dg_packed_tile& t : plan) counts[2] = std::max<int64_t>(counts[2], t.rows);
     if (tiles == nullptr) return DG_OK;
     DG_REQUIRE(cap >= (int64_t)plan.size(), DG_EINVAL, "packed_plan: room for %lld tiles, %lld needed", (long long)cap,
                (long long)plan.size());
@@ -399,18 +489,19 @@ extern "C" int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, i
 extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D, int dtype, const void* q, int64_t q_t,
                                    int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t,
                                    int64_t v_h, void* y, int64_t y_t, int64_t y_h, float scale,
-                                   const dg_packed_tile* tiles, int64_t n_wide, int64_t n_narrow, void* stream) {
-  DG_REQUIRE(Nq >= 0 && Nk >= 0 && H >= 0 && n_wide >= 0 && n_narrow >= 0, DG_EINVAL, "attention_packed: negative size");
+                                   const dg_packed_tile* tiles, const int64_t counts[3], void* stream) {
+  DG_REQUIRE(Nq >= 0 && Nk >= 0 && H >= 0, DG_EINVAL, "attention_packed: negative size");
   DG_REQUIRE(known_dtype(dtype), DG_EUNSUPPORTED, "attention_packed: dtype %d unsupported", dtype);
   DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "attention_packed: head_dim %d outside [1, %d]", D, kMaxHeadDim);
   DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "attention_packed: %d query heads on %d key heads", H, Hkv);
   DG_REQUIRE(Hkv <= 65535, DG_EINVAL, "attention_packed: %d key heads, at most 65535", Hkv);
   DG_REQUIRE(scale > 0.f && std::isfinite(scale), DG_EINVAL, "attention_packed: the scale must be positive");
-  DG_REQUIRE(n_wide <= 0x7fffffff && n_narrow <= 0x7fffffff && n_wide % 8 == 0 && n_narrow % 8 == 0, DG_EINVAL,
-             "attention_packed: %lld and %lld tiles, multiples of 8 up to 2^31 - 1 from dg_packed_plan", (long long)n_wide,
-             (long long)n_narrow);
-  DG_REQUIRE(n_wide + n_narrow <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 tiles");
-  if (Nq == 0 || H == 0 || n_wide + n_narrow == 0) return DG_OK;
+  DG_REQUIRE(counts != nullptr, DG_EINVAL, "attention_packed: NULL argument");
+  DG_REQUIRE(counts[0] >= 0 && counts[0] <= 0x7fffffff && counts[0] % 8 == 0 && counts[1] >= 0 && counts[1] <= counts[0] &&
+                 counts[2] >= 0 && counts[2] <= kTileRows,
+             DG_EINVAL, "attention_packed: counts (%lld, %lld, %lld) are not dg_packed_plan's", (long long)counts[0],
+             (long long)counts[1], (long long)counts[2]);
+  if (Nq == 0 || H == 0 || counts[0] == 0) return DG_OK;
   DG_REQUIRE(q && y && tiles && (Nk == 0 || (k && v)), DG_EINVAL, "attention_packed: NULL argument");
   SeqArgs a{};
   a.q = q; a.k = k; a.v = v; a.y = y;
@@ -422,11 +513,10 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   a.tiles = tiles;
   a.nq = Nq; a.nk = Nk;
   a.nsplit = 1;
-  a.rows_per_wg = kWideRows;
-  if (seq_mfma_applicable(a, dtype, false))
-    return launch_seq_mfma_packed(a, dtype, n_wide, n_narrow, static_cast<hipStream_t>(stream));
-  return launch_vec_any<false>(a, dtype, dim3((unsigned)(n_wide + n_narrow), (unsigned)Hkv),
-                               static_cast<hipStream_t>(stream));
+  a.rows_per_wg = kTileRows;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (seq_mfma_applicable(a, dtype, false)) return launch_seq_mfma_packed(a, dtype, counts, s);
+  return launch_vec_any<false>(a, dtype, dim3((unsigned)counts[0], (unsigned)Hkv), s);
 }
 
 extern "C" size_t dg_attention_tree_workspace_size(int B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
@@ -473,27 +563,39 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
     a.ws_o = workspace;
     a.ws_ml = static_cast<char*>(workspace) + t.o_bytes;
   }
-  const int64_t blocks = (int64_t)B * Hkv * t.nrb * t.nsplit;
+  const int64_t blocks = ((int64_t)B * Hkv * t.nsplit + 7) / 8 * 8 * t.nrb;
   DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rc = mfma ? launch_seq_mfma_tree(a, dtype, (unsigned)blocks, s)
                       : launch_vec_any<true>(a, dtype, dim3((unsigned)blocks), s);
   if (rc != DG_OK || t.nsplit == 1) return rc;
   const int64_t rows = (int64_t)B * H * N;
-  // a row's waves read its splits in turn: four of them where there are many
-  const bool many = t.nsplit >= 8;
+  // a row's waves read its splits in turn: four of them where there are many and rows few
+  const bool many = t.nsplit >= 16 && rows <= 4096;
   const int64_t groups = many ? rows : (rows + 3) / 4;
   DG_REQUIRE(groups <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
   const dim3 grid((unsigned)groups);
-#define DG_JOIN(T)                                                                                      \
-  do {                                                                                                  \
-    if (many) hipLaunchKernelGGL((seq_join_kernel<T, 4>), grid, dim3(256), 0, s, a, rows);              \
-    else hipLaunchKernelGGL((seq_join_kernel<T, 1>), grid, dim3(256), 0, s, a, rows);                   \
+#define DG_JOIN(T)                                                                         \
+  do {                                                                                     \
+    if (many) hipLaunchKernelGGL((seq_join_kernel<T, 4>), grid, dim3(256), 0, s, a, rows); \
+    else hipLaunchKernelGGL((seq_join_kernel<T, 1>), grid, dim3(256), 0, s, a, rows);      \
   } while (0)
-  if (dtype == DG_F64) DG_JOIN(double);
-  else if (dtype == DG_F32) DG_JOIN(float);
-  else if (dtype == DG_BF16) DG_JOIN(bf16_t);
-  else DG_JOIN(f16_t);
+#define DG_JOIN4(T)                                          \
+  do {                                                       \
+    if (many) launch_join4<T, 4>(a, grid, rows, s);          \
+    else launch_join4<T, 1>(a, grid, rows, s);               \
+  } while (0)
+  if (mfma) {
+    if (dtype == DG_F32) DG_JOIN4(float);
+    else if (dtype == DG_BF16) DG_JOIN4(bf16_t);
+    else DG_JOIN4(f16_t);
+  } else {
+    if (dtype == DG_F64) DG_JOIN(double);
+    else if (dtype == DG_F32) DG_JOIN(float);
+    else if (dtype == DG_BF16) DG_JOIN(bf16_t);
+    else DG_JOIN(f16_t);
+  }
 #undef DG_JOIN
+#undef DG_JOIN4
   return check_launch("seq_join_kernel");
 }

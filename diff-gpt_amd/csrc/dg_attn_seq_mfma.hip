@@ -103,7 +103,7 @@ constexpr int seq_wgs_per_cu() {
 
 template <typename T, int D, int RT, bool TREE>
 __global__ __launch_bounds__((seq_threads<T, D, RT>()), (seq_wgs_per_cu<T, D, RT>()))
-void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
+void seq_mfma_kernel(const SeqArgs a) {
   using C = SeqCfg<T, D, RT>;
   using M = SeqMma<T>;
   using vec8 = typename M::vec8;
@@ -115,7 +115,7 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
   __shared__ __attribute__((aligned(16))) T kv1[KS * 2 * TILE];
 
   SeqPiece pc;
-  if (!seq_piece<TREE>(a, tile0, pc)) return;  // whole workgroups, before any barrier
+  if (!seq_piece<TREE>(a, pc)) return;  // whole workgroups, before any barrier
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rt = wv % RT, kg = wv / RT;
@@ -558,24 +558,24 @@ void seq_mfma_kernel(const SeqArgs a, const int64_t tile0) {
 namespace {
 
 template <typename T, int D, int RT, bool TREE>
-int launch_seq(const SeqArgs& a, int64_t tile0, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, TREE>), grid, dim3(64 * SeqCfg<T, D, RT>::WAVES), 0, s, a, tile0);
+int launch_seq(const SeqArgs& a, dim3 grid, hipStream_t s) {
+  hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, TREE>), grid, dim3(64 * SeqCfg<T, D, RT>::WAVES), 0, s, a);
   return check_launch(TREE ? "seq_mfma_tree_kernel" : "seq_mfma_packed_kernel");
 }
 
 template <typename T, int RT, bool TREE>
-int launch_seq_d(const SeqArgs& a, int64_t tile0, dim3 grid, hipStream_t s) {
-  if (a.D == 16) return launch_seq<T, 16, RT, TREE>(a, tile0, grid, s);
-  if (a.D == 32) return launch_seq<T, 32, RT, TREE>(a, tile0, grid, s);
-  if (a.D == 64) return launch_seq<T, 64, RT, TREE>(a, tile0, grid, s);
-  return launch_seq<T, 128, RT, TREE>(a, tile0, grid, s);
+int launch_seq_d(const SeqArgs& a, dim3 grid, hipStream_t s) {
+  if (a.D == 16) return launch_seq<T, 16, RT, TREE>(a, grid, s);
+  if (a.D == 32) return launch_seq<T, 32, RT, TREE>(a, grid, s);
+  if (a.D == 64) return launch_seq<T, 64, RT, TREE>(a, grid, s);
+  return launch_seq<T, 128, RT, TREE>(a, grid, s);
 }
 
 template <int RT, bool TREE>
-int launch_seq_t(const SeqArgs& a, int dtype, int64_t tile0, dim3 grid, hipStream_t s) {
-  if (dtype == DG_F32) return launch_seq_d<float, RT, TREE>(a, tile0, grid, s);
-  if (dtype == DG_BF16) return launch_seq_d<bf16_t, RT, TREE>(a, tile0, grid, s);
-  return launch_seq_d<f16_t, RT, TREE>(a, tile0, grid, s);
+int launch_seq_t(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
+  if (dtype == DG_F32) return launch_seq_d<float, RT, TREE>(a, grid, s);
+  if (dtype == DG_BF16) return launch_seq_d<bf16_t, RT, TREE>(a, grid, s);
+  return launch_seq_d<f16_t, RT, TREE>(a, grid, s);
 }
 
 }  // namespace
@@ -599,22 +599,27 @@ int seq_mfma_tree_rows(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 12
 
 int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s) {
   const dim3 grid(blocks);
-  if (a.rows_per_wg == 32) return launch_seq_t<1, true>(a, dtype, 0, grid, s);
-  if (a.rows_per_wg == 64) return launch_seq_t<2, true>(a, dtype, 0, grid, s);
-  return launch_seq_t<4, true>(a, dtype, 0, grid, s);
+  if (a.rows_per_wg == 32) return launch_seq_t<1, true>(a, dtype, grid, s);
+  if (a.rows_per_wg == 64) return launch_seq_t<2, true>(a, dtype, grid, s);
+  return launch_seq_t<4, true>(a, dtype, grid, s);
 }
 
-int launch_seq_mfma_packed(SeqArgs a, int dtype, int64_t n_wide, int64_t n_narrow, hipStream_t s) {
-  if (n_wide > 0) {
-    a.rows_per_wg = 128;
-    const int rc = launch_seq_t<4, false>(a, dtype, 0, dim3((unsigned)n_wide, (unsigned)a.Hkv), s);
-    if (rc != DG_OK) return rc;
-  }
-  if (n_narrow > 0) {
-    a.rows_per_wg = 32;
-    return launch_seq_t<1, false>(a, dtype, n_wide, dim3((unsigned)n_narrow, (unsigned)a.Hkv), s);
-  }
-  return DG_OK;
+// A tile goes to one workgroup of 128 rows, to two of 64 that split the keys in two, or to
+// four of 32 that split them in four: the more where tiles are few, since a workgroup
+// walks its keys one stage after the other, and never fewer than fill the rows.  us with
+// 32 / 64 / 128 rows, tiles times key heads in brackets, bf16:
+//   head_dim  64: 8 x 512 tokens [256] 20.5 / 15.2 / 16.6, 16 [512] 32.5 / 21.1 / 22.3,
+//     32 [1024] 56.7 / 32.1 / 28.1; 6 x 2048 [768] 98.0 / 65.0 / 54.8; 48 chunks of up to
+//     300 behind up to 3000 keys, groups of 4 [550] 63.4 / 58.9 / 68.8
+//   head_dim 128: 1 x 3584 [224] 107 / 66.4 / 84.3, 4 x 2048 [512] 143 / 79.5 / 65.4
+int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s) {
+  const int64_t tiles = counts[1] * a.Hkv;
+  const int rt = counts[2] <= 32 || tiles <= 64 ? 1 : counts[2] <= 64 || tiles <= (a.D == 128 ? 384 : 640) ? 2 : 4;
+  a.rows_per_wg = 32 * rt;
+  const dim3 grid((unsigned)counts[0], (unsigned)a.Hkv, (unsigned)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg));
+  if (rt == 1) return launch_seq_t<1, false>(a, dtype, grid, s);
+  if (rt == 2) return launch_seq_t<2, false>(a, dtype, grid, s);
+  return launch_seq_t<4, false>(a, dtype, grid, s);
 }
 
 }  // namespace dg

@@ -43,6 +43,8 @@ struct SeqArgs {
   void* ws_ml;
 };
 
+constexpr int kTileRows = 128;  // most rows of a packed tile
+
 // A workgroup's piece: the rows row0 .. row0 + rows - 1 of a sequence of `nrows` rows,
 // over keys [kbeg, kend).  Query i sees key t iff t < own, or t < own + 64 and bit
 // t - own of its mask; packed: iff t <= i + off.
@@ -56,19 +58,22 @@ struct SeqPiece {
   int kvh, split;
 };
 
-// The piece of this workgroup (packed: a tile from tile0 on); false where there is nothing to do.  Nothing a table or
+// The piece of this workgroup; false where there is nothing to do.  Nothing a table or
 // a length in device memory says takes an access outside q, k, v and y: tiles that do
 // not lie inside them are left out, lengths beyond the cache are taken as its end.
 template <bool TREE>
-__device__ __forceinline__ bool seq_piece(const SeqArgs& a, int64_t tile0, SeqPiece& p) {
+__device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
   if constexpr (TREE) {
-    int64_t u = (int64_t)blockIdx.x;
+    // workgroup x runs on XCD x mod 8: the row blocks of a split, which read the same
+    // keys, follow each other there
+    const unsigned t = blockIdx.x >> 3;
+    const int rb = (int)(t % (unsigned)a.nrb);
+    int64_t u = (int64_t)(t / (unsigned)a.nrb) * 8 + (blockIdx.x & 7u);
     p.split = (int)(u % a.nsplit);
     u /= a.nsplit;
-    const int rb = (int)(u % a.nrb);
-    u /= a.nrb;
     p.kvh = (int)(u % a.Hkv);
     p.b = u / a.Hkv;
+    if (p.b >= a.B) return false;  // the grid is rounded up
     const int len = a.lens != nullptr ? __builtin_amdgcn_readfirstlane(a.lens[p.b]) : a.len;
     p.own = min(max(len, 0), a.Tcap - a.N);
     p.row0 = rb * a.rows_per_wg;
@@ -80,7 +85,7 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, int64_t tile0, SeqPi
     return p.kbeg < p.kend;
   } else {
     // which entry: dg_packed_plan's lists, an XCD further for each key head
-    dg_packed_tile t = a.tiles[tile0 + (blockIdx.x & ~7u) + ((blockIdx.x - blockIdx.y) & 7u)];
+    dg_packed_tile t = a.tiles[(blockIdx.x & ~7u) + ((blockIdx.x - blockIdx.y) & 7u)];
     t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
     t.lq = __builtin_amdgcn_readfirstlane(t.lq);
     t.k0 = __builtin_amdgcn_readfirstlane(t.k0);
@@ -93,8 +98,11 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, int64_t tile0, SeqPi
     p.own = 0;
     if (t.lq <= 0 || t.lk < 0 || t.q0 < 0 || t.k0 < 0 || (int64_t)t.q0 + t.lq > a.nq || (int64_t)t.k0 + t.lk > a.nk)
       return false;
-    if (t.row0 < 0 || t.rows <= 0 || t.rows > a.rows_per_wg || (int64_t)t.row0 + t.rows > (int64_t)t.lq * a.G)
-      return false;
+    if (t.row0 < 0 || t.rows <= 0 || t.rows > kTileRows || (int64_t)t.row0 + t.rows > (int64_t)t.lq * a.G) return false;
+    // the workgroup's part of the tile
+    t.row0 += blockIdx.z * a.rows_per_wg;
+    t.rows = min(a.rows_per_wg, t.rows - (int)blockIdx.z * a.rows_per_wg);
+    if (t.rows <= 0) return false;
     p.row0 = t.row0;
     p.rows = t.rows;
     p.off = t.lk - t.lq;
@@ -118,7 +126,7 @@ __device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n
 // (token, head) rows, and its launches
 bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree);
 int seq_mfma_tree_rows(int rows);
-int launch_seq_mfma_packed(SeqArgs a, int dtype, int64_t n_wide, int64_t n_narrow, hipStream_t s);
+int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s);
 int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s);
 
 }  // namespace dg

@@ -256,7 +256,7 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int] * 4
         + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64] * 4  # q, k, v, y
-        + [ctypes.c_float, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p],
+        + [ctypes.c_float, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p],
     ),
     "dg_attention_tree_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 7),
     "dg_attention_tree": (
@@ -790,18 +790,17 @@ def _check_scale(what: str, scale: float) -> float:
 _TILE_WORDS = 8
 
 
-def packed_plan(q_lengths: list[int], k_lengths: list[int], group: int) -> tuple[torch.Tensor, int, int]:
-    """dg_packed_plan: the (tiles, 8) int32 table of a batch, on the host, and how many of
-    its tiles are wide (they come first) and narrow."""
+def packed_plan(q_lengths: list[int], k_lengths: list[int], group: int) -> tuple[torch.Tensor, ctypes.Array]:
+    """dg_packed_plan: the (entries, 8) int32 table of a batch, on the host, and its counts."""
     n = len(q_lengths)
     lq, lk = (ctypes.c_int64 * n)(*q_lengths), (ctypes.c_int64 * n)(*k_lengths)
-    counts = (ctypes.c_int64 * 2)()
+    counts = (ctypes.c_int64 * 3)()
     L = lib()
     _check(L.dg_packed_plan(n, lq, lk, group, None, 0, counts), "packed_plan")
-    tiles = torch.empty((counts[0] + counts[1], _TILE_WORDS), dtype=torch.int32)
+    tiles = torch.empty((counts[0], _TILE_WORDS), dtype=torch.int32)
     if len(tiles):
         _check(L.dg_packed_plan(n, lq, lk, group, tiles.data_ptr(), len(tiles), counts), "packed_plan")
-    return tiles, counts[0], counts[1]
+    return tiles, counts
 
 
 def attention_packed_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, y: torch.Tensor, layout, scale: float) -> None:
@@ -832,7 +831,7 @@ def attention_packed_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, y: torc
         raise ValueError("attention_packed: the last (head_dim) dimension must be contiguous")
     _launch("attention_packed", device, lib().dg_attention_packed, Nq, Nk, H, Hkv, D, _DTYPE_CODE[q.dtype],
             q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, y.data_ptr(), yt, yh,
-            _check_scale("attention_packed", scale), layout.tiles.data_ptr(), layout.n_wide, layout.n_narrow)
+            _check_scale("attention_packed", scale), layout.tiles.data_ptr(), layout.counts)
 
 
 def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, y: torch.Tensor, scale: float,

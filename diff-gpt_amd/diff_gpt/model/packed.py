@@ -21,7 +21,7 @@ class PackedLayout:
     queries the first keys are cached ones, with fewer the first queries see nothing.
     group: query heads per key head of the tensors the layout is for."""
 
-    __slots__ = ("q_lengths", "k_lengths", "group", "total_q", "total_k", "tiles", "n_wide", "n_narrow")
+    __slots__ = ("q_lengths", "k_lengths", "group", "total_q", "total_k", "tiles", "counts")
 
     def __init__(self, q_lengths: Sequence[int], k_lengths: Sequence[int] | None = None, group: int = 1,
                  device: torch.device | str = "cuda") -> None:
@@ -36,7 +36,7 @@ class PackedLayout:
             raise ValueError(f"group must be at least 1, got {group}")
         self.group = int(group)
         self.total_q, self.total_k = sum(self.q_lengths), sum(self.k_lengths)
-        tiles, self.n_wide, self.n_narrow = _native.packed_plan(self.q_lengths, self.k_lengths, self.group)
+        tiles, self.counts = _native.packed_plan(self.q_lengths, self.k_lengths, self.group)
         self.tiles = tiles.to(device)
 
 

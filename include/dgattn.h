@@ -585,11 +585,12 @@ DG_API int dg_draw_argmax(int64_t M, int V, int dtype, const void* probs, int64_
  * that sees no key gets zeros.  Rows of y behind the last sequence are left as they are.
  *
  * dg_packed_plan lays the work out once per batch, on the host and without the device: it
- * writes the tiles of the sequences for heads in groups of `group` into `tiles` (room for
- * `cap`; NULL with cap 0 only counts): counts[0] wide ones, which come first, and counts[1]
- * narrow ones, each a multiple of 8 (some are empty).  The caller copies the table to the
- * device and hands it with its counts to every dg_attention_packed over such a batch.  A
- * tile that does not lie inside Nq and Nk rows is skipped, never followed.
+ * writes the tiles of the sequences, for heads in groups of `group`, into `tiles` (room for
+ * `cap`; NULL with cap 0 only counts).  counts: [0] the entries of the table, a multiple of
+ * 8, some of them empty; [1] those that are not; [2] the most rows of one.  The caller
+ * copies the table to the device and hands it with its counts to every dg_attention_packed
+ * over such a batch.  A tile that does not lie inside Nq and Nk rows is skipped, never
+ * followed.
  * fp32 / bf16 / fp16 / fp64, every head_dim up to 1024, rows with unit stride over d; the
  * scale is positive.
  */
@@ -600,14 +601,14 @@ typedef struct dg_packed_tile {
 } dg_packed_tile;
 
 DG_API int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, int group, dg_packed_tile* tiles,
-                          int64_t cap, int64_t* counts);
+                          int64_t cap, int64_t counts[3]);
 
 DG_API int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D, int dtype,
                                const void* q, int64_t q_t, int64_t q_h,
                                const void* k, int64_t k_t, int64_t k_h,
                                const void* v, int64_t v_t, int64_t v_h,
                                void* y, int64_t y_t, int64_t y_h, float scale,
-                               const dg_packed_tile* tiles, int64_t n_wide, int64_t n_narrow, void* stream);
+                               const dg_packed_tile* tiles, const int64_t counts[3], void* stream);
 
 /*
  * Attention of a few tokens a row -- a tree of candidates, or a decode step's one --

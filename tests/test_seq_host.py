@@ -17,8 +17,9 @@ FAKE = ctypes.c_void_p(0x1000)
 
 def _covered(q_lens, k_lens, group):
     """Every (query, head) row of every sequence, from the plan's tiles."""
-    tiles, wide, narrow = _native.packed_plan(q_lens, k_lens, group)
-    assert tiles.shape == (wide + narrow, 8)
+    tiles, counts = _native.packed_plan(q_lens, k_lens, group)
+    assert tiles.shape == (counts[0], 8) and counts[0] % 8 == 0
+    assert counts[1] == int((tiles[:, 5] > 0).sum()) and counts[2] == max(tiles[:, 5].tolist(), default=0)
     rows = []
     for q0, lq, k0, lk, row0, n, *_ in tiles.tolist():
         if n == 0:
@@ -43,7 +44,7 @@ def test_plan_covers_every_row_once(q_lens, k_lens, group):
 def test_plan_refusals():
     def plan(lq, lk, group=1, cap=0, tiles=None):
         n = len(lq)
-        counts = (ctypes.c_int64 * 2)()
+        counts = (ctypes.c_int64 * 3)()
         return _native.lib().dg_packed_plan(n, (ctypes.c_int64 * n)(*lq), (ctypes.c_int64 * n)(*lk), group, tiles, cap,
                                             counts)
 
@@ -87,7 +88,7 @@ def test_tree_refusals(parents):
 
 def test_host_tensors_are_refused():
     class Layout:
-        group, total_q, total_k, tiles, n_wide, n_narrow = 1, 2, 2, torch.zeros(1, 8, dtype=torch.int32), 1, 0
+        group, total_q, total_k, tiles, counts = 1, 2, 2, torch.zeros(8, 8, dtype=torch.int32), None
 
     x = torch.zeros(2, 1, 16)
     with pytest.raises(RuntimeError, match="ROCm"):
@@ -102,9 +103,10 @@ def _st(b=16, t=16, h=16):
     return ctypes.pointer(_native.Stride3(b, t, h))
 
 
-def _packed(Nq=4, Nk=4, H=1, Hkv=1, D=16, dtype=0, p=FAKE, scale=1.0, tiles=FAKE, wide=8, narrow=0):
+def _packed(Nq=4, Nk=4, H=1, Hkv=1, D=16, dtype=0, p=FAKE, scale=1.0, tiles=FAKE, counts=(8, 1, 4)):
+    counts = None if counts is None else (ctypes.c_int64 * 3)(*counts)
     return _native.lib().dg_attention_packed(Nq, Nk, H, Hkv, D, dtype, p, 16, 16, p, 16, 16, p, 16, 16, p, 16, 16, scale,
-                                             tiles, wide, narrow, NUL)
+                                             tiles, counts, NUL)
 
 
 def _tree(B=1, N=2, H=1, Hkv=1, Tcap=8, D=16, dtype=0, p=FAKE, scale=1.0, length=3, lens=NUL, ws=NUL, ws_bytes=0):
@@ -115,7 +117,9 @@ def _tree(B=1, N=2, H=1, Hkv=1, Tcap=8, D=16, dtype=0, p=FAKE, scale=1.0, length
 @pytest.mark.parametrize("kw,rc", [(dict(Nq=-1), -1), (dict(dtype=9), -2), (dict(D=0), -2), (dict(D=1025), -2),
                                    (dict(H=3, Hkv=2), -1), (dict(Hkv=0), -1), (dict(scale=0.0), -1),
                                    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(p=NUL), -1),
-                                   (dict(tiles=NUL), -1), (dict(wide=-1), -1), (dict(wide=1), -1), (dict(Nq=0), 0), (dict(wide=0), 0),
+                                   (dict(tiles=NUL), -1), (dict(counts=None), -1), (dict(counts=(-8, 0, 0)), -1),
+                                   (dict(counts=(1, 1, 1)), -1), (dict(counts=(8, 9, 1)), -1),
+                                   (dict(counts=(8, 1, 129)), -1), (dict(Nq=0), 0), (dict(counts=(0, 0, 0)), 0),
                                    (dict(H=0), 0)])
 def test_packed_refusals(kw, rc):
     assert _packed(**kw) == rc
