@@ -65,7 +65,7 @@ struct SeqCfg {
   static constexpr int WAVES = (ES == 4 && D == 128 && RT == 1) ? 2 : 4;
   static constexpr int KS = WAVES / RT;
   // 32-key blocks of a stage
-  static constexpr int MB = D * ES <= 64 ? 2 : (ES == 2 && D == 64 && RT == 4) ? 2 : 1;
+  static constexpr int MB = RT == 4 ? (ES == 2 && D == 64 ? 2 : 1) : D * ES <= 64 ? 2 : 1;
   static constexpr int BN = 32 * MB;
   static constexpr int PPR = D * ES / 16;        // 16-byte pieces of a row
   static constexpr int RPD = 64 / PPR;           // rows a wave-wide copy covers
@@ -147,8 +147,8 @@ void seq_mfma_kernel(const SeqArgs a) {
 
   // ---- global -> LDS copy of a stage's keys -----------------------------------------
   // The RT waves of a key group share its copies: lane l of copy i fills slot l % PPR of
-  // row l / PPR of rows i * RPD ..  The buffer resource starts at the stage's first key,
-  // with 64-bit arithmetic, and ends behind the piece's last: rows past it read as zeros.
+  // row l / PPR of rows i * RPD ..  The buffer resource ends behind the piece's last key:
+  // rows past it read as zeros.
   int ko[(C::NDMA + RT - 1) / RT], vo[(C::NDMA + RT - 1) / RT];
 #pragma unroll
   for (int n = 0; n < (C::NDMA + RT - 1) / RT; ++n) {
@@ -157,21 +157,38 @@ void seq_mfma_kernel(const SeqArgs a) {
     ko[n] = r * (int)a.kt * ES + 16 * piece;
     vo[n] = r * (int)a.vt * ES + 16 * piece;
   }
-  auto copy_stage = [&](T* st, int k0) __attribute__((always_inline)) {
+  // Where the piece's keys span less than 2^31 bytes, one resource serves all stages, the
+  // stage's start in the scalar offset.
+  const int64_t kstep_b = a.kt * ES, vstep_b = a.vt * ES;  // bytes from key to key
+  const int nkeys = max(0, pc.kend - pc.kbeg);
+  const bool near = nkeys * max(kstep_b, vstep_b) + D * ES < ((int64_t)1 << 31);
+  const T* const kp0 = kp + (int64_t)pc.kbeg * a.kt;
+  const T* const vp0 = vp + (int64_t)pc.kbeg * a.vt;
+  const __amdgpu_buffer_rsrc_t krs0 = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<T*>(kp0), 0, near && nkeys > 0 ? (int)((nkeys - 1) * kstep_b + D * ES) : 0, kBufferWord3);
+  const __amdgpu_buffer_rsrc_t vrs0 = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<T*>(vp0), 0, near && nkeys > 0 ? (int)((nkeys - 1) * vstep_b + D * ES) : 0, kBufferWord3);
+  auto copy_from = [&](T* st, __amdgpu_buffer_rsrc_t krs, __amdgpu_buffer_rsrc_t vrs, int ks0, int vs0)
+      __attribute__((always_inline)) {
     T* const ks = st + kg * 2 * TILE;
-    const int left = min(BN, pc.kend - k0);
-    const int kn = left <= 0 ? 0 : (int)((left - 1) * a.kt + D) * ES;
-    const int vn = left <= 0 ? 0 : (int)((left - 1) * a.vt + D) * ES;
-    const __amdgpu_buffer_rsrc_t krs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + (int64_t)k0 * a.kt), 0, kn, kBufferWord3);
-    const __amdgpu_buffer_rsrc_t vrs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp + (int64_t)k0 * a.vt), 0, vn, kBufferWord3);
 #pragma unroll
     for (int n = 0; n < (C::NDMA + RT - 1) / RT; ++n) {
       const int i = n * RT + rt;
       if (C::NDMA % RT != 0 && i >= C::NDMA) break;  // wave-uniform
-      lds_copy16_buf(krs, ko[n], 0, ks + i * C::RPD * D);
-      lds_copy16_buf(vrs, vo[n], 0, ks + TILE + i * C::RPD * D);
+      lds_copy16_buf(krs, ko[n], ks0, ks + i * C::RPD * D);
+      lds_copy16_buf(vrs, vo[n], vs0, ks + TILE + i * C::RPD * D);
+    }
+  };
+  auto copy_stage = [&](T* st, int k0) __attribute__((always_inline)) {
+    const int rel = k0 - pc.kbeg;
+    if (near && rel < nkeys) {
+      copy_from(st, krs0, vrs0, rel * (int)kstep_b, rel * (int)vstep_b);
+    } else {  // far, or a group's stage behind the last key: zeros
+      const int left = min(BN, nkeys - rel);
+      const int kn = left <= 0 ? 0 : (int)((left - 1) * kstep_b) + D * ES;
+      const int vn = left <= 0 ? 0 : (int)((left - 1) * vstep_b) + D * ES;
+      copy_from(st, __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp0 + rel * a.kt), 0, kn, kBufferWord3),
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp0 + rel * a.vt), 0, vn, kBufferWord3), 0, 0);
     }
   };
   // this wave's copies have landed; the waves of a group also wait for each other
@@ -348,10 +365,17 @@ void seq_mfma_kernel(const SeqArgs a) {
     for (int mb = 0; mb < MB; ++mb) {
       const int kb = k0 + 32 * mb;
       if (kb + 32 > open) {
-        const uint32_t vis = visible(kb) >> (4 * hh);
+        if constexpr (TREE) {
+          const uint32_t vis = visible(kb) >> (4 * hh);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((vis >> (8 * (r >> 2) + (r & 3))) & 1u)) s[mb][r] = kNone;
+          for (int r = 0; r < 16; ++r)
+            if (!((vis >> (8 * (r >> 2) + (r & 3))) & 1u)) s[mb][r] = kNone;
+        } else {
+          const int lim = qi + pc.off - kb - 4 * hh;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) > lim) s[mb][r] = kNone;
+        }
       }
     }
     float mt = s[0][0];
@@ -616,7 +640,7 @@ int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStr
   const int64_t tiles = counts[1] * a.Hkv;
   const int rt = counts[2] <= 32 || tiles <= 64 ? 1 : counts[2] <= 64 || tiles <= (a.D == 128 ? 384 : 640) ? 2 : 4;
   a.rows_per_wg = 32 * rt;
-  const dim3 grid((unsigned)counts[0], (unsigned)a.Hkv, (unsigned)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg));
+  const dim3 grid((unsigned)(counts[0] * a.Hkv), (unsigned)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg));
   if (rt == 1) return launch_seq_t<1, false>(a, dtype, grid, s);
   if (rt == 2) return launch_seq_t<2, false>(a, dtype, grid, s);
   return launch_seq_t<4, false>(a, dtype, grid, s);

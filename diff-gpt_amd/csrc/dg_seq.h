@@ -85,14 +85,15 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
     return p.kbeg < p.kend;
   } else {
     // which entry: dg_packed_plan's lists, an XCD further for each key head
-    dg_packed_tile t = a.tiles[(blockIdx.x & ~7u) + ((blockIdx.x - blockIdx.y) & 7u)];
+    const unsigned u = blockIdx.x >> 3, slot = u / (unsigned)a.Hkv;
+    p.kvh = (int)(u - slot * (unsigned)a.Hkv);
+    dg_packed_tile t = a.tiles[8 * (int64_t)slot + ((blockIdx.x - (unsigned)p.kvh) & 7u)];
     t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
     t.lq = __builtin_amdgcn_readfirstlane(t.lq);
     t.k0 = __builtin_amdgcn_readfirstlane(t.k0);
     t.lk = __builtin_amdgcn_readfirstlane(t.lk);
     t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
     t.rows = __builtin_amdgcn_readfirstlane(t.rows);
-    p.kvh = blockIdx.y;
     p.split = 0;
     p.b = 0;
     p.own = 0;
@@ -100,8 +101,8 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
       return false;
     if (t.row0 < 0 || t.rows <= 0 || t.rows > kTileRows || (int64_t)t.row0 + t.rows > (int64_t)t.lq * a.G) return false;
     // the workgroup's part of the tile
-    t.row0 += blockIdx.z * a.rows_per_wg;
-    t.rows = min(a.rows_per_wg, t.rows - (int)blockIdx.z * a.rows_per_wg);
+    t.row0 += blockIdx.y * a.rows_per_wg;
+    t.rows = min(a.rows_per_wg, t.rows - (int)blockIdx.y * a.rows_per_wg);
     if (t.rows <= 0) return false;
     p.row0 = t.row0;
     p.rows = t.rows;

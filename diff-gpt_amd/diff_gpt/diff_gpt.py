@@ -323,6 +323,42 @@ class DiffGPT:
         out[max_order:] = flat.reshape(encoded.shape[0], columns)
         return pd.DataFrame(out, columns=df.columns, index=df.index)
 
+    @torch.inference_mode()
+    def anomaly_scores_batch(self, dfs: "list[pd.DataFrame]") -> "list[pd.DataFrame]":
+        """anomaly_scores for several frames at once, of any lengths: their series are scored
+        as packed sequences in one forward per 65536 tokens (GPT.score)."""
+        assert len(dfs) > 0, "dfs must be a non-empty list of frames"
+        encoded, orders = [], []
+        for df in dfs:
+            order = _max_order(self.order_of_derivative, df.shape[1], "columns")
+            assert order <= df.shape[0], f"max order {order} > signal length {df.shape[0]}"
+            tokens = self._encode_frame(df)[2]
+            assert tokens.size <= self.model.block_size, (
+                f"signal has {tokens.size} tokens but block_size is {self.model.block_size}; "
+                f"chunk the input manually for longer sequences"
+            )
+            encoded.append(tokens)
+            orders.append(order)
+        was_training = self.model.training
+        self.model.eval()
+        some = [i for i, e in enumerate(encoded) if e.size > 0]
+        scored = self.model.score([encoded[i].reshape(-1).astype(np.int64).tolist() for i in some])
+        if was_training:
+            self.model.train()
+        out = []
+        for df, e, order in zip(dfs, encoded, orders):
+            out.append(np.full(df.shape, np.nan, dtype=np.float64))
+        # one copy to the host for all series
+        nll = -torch.cat([r.logprobs for r in scored]).cpu().numpy().astype(np.float64) if scored else np.empty(0)
+        at = 0
+        for i in some:
+            e = encoded[i]
+            flat = np.full(e.size, np.nan, dtype=np.float64)
+            flat[1:] = nll[at : at + e.size - 1]
+            at += e.size - 1
+            out[i][orders[i] :] = flat.reshape(e.shape[0], dfs[i].shape[1])
+        return [pd.DataFrame(o, columns=df.columns, index=df.index) for o, df in zip(out, dfs)]
+
     def _forced_plan(
         self,
         context_df: pd.DataFrame,

@@ -150,6 +150,7 @@ class Block(nn.Module):
         _xn_out: torch.Tensor | None = None,
         _qkvg: torch.Tensor | None = None,
         _tail: _native.Tail | None = None,
+        _rows=None,
     ) -> tuple[tuple[torch.Tensor, ...], torch.Tensor]:
         """block.py:87-107.  With _last_only the attention still runs over
         every position (its keys and values go to the cache), and the rest of
@@ -162,7 +163,9 @@ class Block(nn.Module):
         head's input after the last layer, from the same launch when
         dg_block_out takes the layer.  _qkvg, when given, is this layer's
         q/k/v/g projections, computed by an earlier launch; _tail what follows
-        this layer (its ``done`` says whether the launch took it)."""
+        this layer (its ``done`` says whether the launch took it).  _rows, when
+        given, is the attention of rows that are no (B, T) batch (PackedRows,
+        TreeRows)."""
         _native.require_device("Block", partial_block)
         sa = self.sa
         qkvg = self._project(blocks, partial_block, _xn) if _qkvg is None else _qkvg
@@ -172,8 +175,12 @@ class Block(nn.Module):
             blocks = (*blocks, partial_block)
         # a large prefill's gate goes with the attention's stores, unless
         # dg_block_out takes the ungated output below or only one row goes on
-        gated = not _last_only and sa.n_embd not in LAYER_WIDTHS and sa._gates_in_prefill(qkvg)
-        y = sa._attend(qkvg, freqs_cis, kv_cache, gated=True) if gated else sa._attend(qkvg, freqs_cis, kv_cache)
+        gated = (_rows is None and not _last_only and sa.n_embd not in LAYER_WIDTHS
+                 and sa._gates_in_prefill(qkvg))
+        if _rows is not None:
+            y = sa._attend(qkvg, freqs_cis, kv_cache, rows=_rows)
+        else:
+            y = sa._attend(qkvg, freqs_cis, kv_cache, gated=True) if gated else sa._attend(qkvg, freqs_cis, kv_cache)
         g = sa._gate_logits(qkvg)
         if _last_only:
             y, g, partial_in = y[:, -1:], g[:, -1:], partial_in[:, -1:]

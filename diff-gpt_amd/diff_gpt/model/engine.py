@@ -12,6 +12,8 @@ Beyond the reference: ``generate_multi`` / ``generate_multi_batch`` decode
 several prompts of one length at once -- one batched prefill, each prompt's
 cache shared by its ``num_samples`` rows, one captured decode step for all
 rows -- with a schedule that may differ per prompt or per row.
+``score_continuations`` gives the log probabilities of candidate continuations
+of a prompt, run as trees of tokens behind its cache.
 """
 
 import gc
@@ -23,6 +25,8 @@ import torch
 
 from diff_gpt.model.gpt import GPT, BaseGPT, plain_gpt
 from diff_gpt.model.kv_cache import KVCache
+from diff_gpt.model.token_logprobs import token_logprobs
+from diff_gpt.model.tree import MAX_TREE
 from diff_gpt.sampler.sampler import Sampler
 from diff_gpt.sampler.temperature import draw_one
 
@@ -240,6 +244,48 @@ class Engine:
         self._check_prompts(prompts)
         return self._collect(prompts, num_samples, kwargs, per_prompt=True)
 
+    @torch.inference_mode()
+    def score_continuations(self, tokens: list[int], continuations: list[list[int]]) -> list[list[float]]:
+        """Log probability of every token of each candidate continuation of one prompt
+        (row c: one float per token of continuations[c], given the prompt and the tokens
+        before it).  The prompt is prefilled once; the continuations, whose common beginnings
+        are run once, go behind its cache as trees of up to 64 tokens."""
+        self._check_tokens(tokens)
+        assert isinstance(continuations, list) and len(continuations) > 0, (
+            "continuations must be a non-empty list of token lists"
+        )
+        for c in continuations:
+            self._check_tokens(c)
+            assert len(c) <= MAX_TREE + 1, f"a continuation has at most {MAX_TREE + 1} tokens, got {len(c)}"
+        longest = max(len(c) for c in continuations)
+        model = self.model
+        assert all(0 <= t < model.vocab_size for c in [tokens, *continuations] for t in c), (
+            "a token lies outside the vocabulary"
+        )
+        assert len(tokens) + longest - 1 <= model.block_size * 2, (
+            f"prompt ({len(tokens)}) and continuation ({longest}) exceed 2 * block_size ({model.block_size * 2})"
+        )
+        device = model.device_type
+        cache = KVCache(batch_size=1, num_heads=model.n_head, seq_len=len(tokens) + MAX_TREE,
+                        head_dim=model.n_embd // model.n_head, num_layers=model.n_layer)
+        kw = {"_last_only": True} if isinstance(model, GPT) else {}
+        prompt = torch.tensor([tokens], dtype=torch.long, device=device)
+        last = model.forward(prompt, kv_cache=cache, **kw)[0][0, -1:]
+        scores: list[list[float]] = [[] for _ in continuations]
+        for group, nodes, parents, places in _tries(continuations):
+            logits = last
+            if nodes:
+                ids = torch.tensor([nodes], dtype=torch.long, device=device)
+                logits = torch.cat([last, model.forward_tree(ids, parents, cache)[0]])
+            # row 0 of the logits is the prompt's, row n + 1 token n's
+            rows = torch.tensor([0 if p < 0 else p + 1 for c in group for p in places[c]], dtype=torch.long)
+            wanted = torch.tensor([t for c in group for t in continuations[c]], dtype=torch.long)
+            lp = token_logprobs(logits[rows.to(device)], wanted.to(device)).logprobs.tolist()
+            for c in group:
+                scores[c] = lp[: len(continuations[c])]
+                lp = lp[len(continuations[c]) :]
+        return scores
+
     # -- shared machinery -------------------------------------------------------
 
     @staticmethod
@@ -454,6 +500,44 @@ class Engine:
                     self._kept = (key, cache, decode)
                 else:
                     decode.close()
+
+
+def _tries(continuations: list[list[int]]):
+    """The continuations in groups whose tries have at most MAX_TREE inner tokens (a last
+    token is scored, never run): yields a group's numbers, its trie's tokens and parents,
+    and for each number the token before each of its own (-1: the prompt)."""
+    at = 0
+    while at < len(continuations):
+        group: list[int] = []
+        nodes: list[int] = []
+        parents: list[int] = []
+        child: dict[tuple[int, int], int] = {}
+        places: dict[int, list[int]] = {}
+        while at < len(continuations):
+            c = continuations[at]
+            new_nodes, place, above = 0, [], -1
+            added: list[tuple[int, int]] = []
+            for t in c:
+                place.append(above)
+                if len(place) == len(c):
+                    break
+                key = (above, t)
+                if key in child:
+                    above = child[key]
+                else:
+                    above = len(nodes) + new_nodes
+                    child[key] = above
+                    added.append(key)
+                    new_nodes += 1
+            if len(nodes) + new_nodes > MAX_TREE:
+                break  # the next group's
+            for key in added:
+                parents.append(key[0])
+                nodes.append(key[1])
+            places[at] = place
+            group.append(at)
+            at += 1
+        yield group, nodes, parents, places
 
 
 def _mask_list(mask, rows: int) -> list[int]:

@@ -7,6 +7,7 @@ kernels have no backward, so a forward that would need autograd raises.
 """
 
 from abc import ABC, abstractmethod
+from typing import Sequence
 
 import torch
 import torch.nn as nn
@@ -15,8 +16,11 @@ from torch.nn import functional as F
 from diff_gpt import _native
 from diff_gpt.model.block import Block, plain_block
 from diff_gpt.model.kv_cache import KVCache
+from diff_gpt.model.packed import PackedRows
 from diff_gpt.model.rms_norm import rms_norm
 from diff_gpt.model.rope import precompute_freqs_cis
+from diff_gpt.model.token_logprobs import TokenLogprobs, token_logprobs
+from diff_gpt.model.tree import TreeRows
 from diff_gpt.sampler.sampler import Sampler
 from diff_gpt.sampler.temperature import TemperatureSampler, draw_one
 
@@ -237,6 +241,7 @@ class GPT(BaseGPT):
         _argmax_out: torch.Tensor | None = None,
         _last_only: bool = False,
         _advance: bool = False,
+        _rows: PackedRows | TreeRows | None = None,
     ) -> tuple[torch.Tensor, torch.Tensor | None]:
         """gpt.py:140-200.  _argmax_out (B, T) int64, when given, receives the
         first maximum of every logits row (greedy sampling without a separate
@@ -244,13 +249,16 @@ class GPT(BaseGPT):
         position only (a prefill whose caller reads no others; _argmax_out is
         then (B, 1)): every layer still attends and caches every position, but
         the last layer's work after its attention and the head run for that
-        position alone."""
+        position alone.  _rows: the rows are packed sequences or a tree's tokens,
+        which know their positions and attention themselves."""
         B, T = idx.shape
         assert not (_last_only and targets is not None), "_last_only returns the last position's logits alone"
         start = 0 if kv_cache is None else kv_cache.get_pos()
         end = start + T
-        assert end <= self.freqs_cis.shape[0]
-        if kv_cache is not None and kv_cache.pos_dev is not None:
+        assert _rows is not None or end <= self.freqs_cis.shape[0]
+        if _rows is not None:
+            freqs_cis = _rows.freqs(self.freqs_cis)
+        elif kv_cache is not None and kv_cache.pos_dev is not None:
             # captured decode step: the kernels index the whole table with the
             # position they read on the device
             freqs_cis = self.freqs_cis
@@ -278,6 +286,8 @@ class GPT(BaseGPT):
             tail = self._tail(i, _argmax_out, advance) if (joins_last if one else joins) else None
             # a Block with a forward of its own is not handed what joined launches pass on
             joined = {} if qkvg is None and tail is None else {"_qkvg": qkvg, "_tail": tail}
+            if _rows is not None:
+                joined["_rows"] = _rows
             blocks, partial = block(blocks, partial, freqs_cis=freqs_cis, kv_cache=kv_cache,
                                     _last_only=_last_only and i == last, _xn=xn0 if i == 0 else None,
                                     _xn_out=xn_head if i == last else None, **joined)
@@ -303,6 +313,66 @@ class GPT(BaseGPT):
             else:
                 loss = F.cross_entropy(flat_logits, flat_targets)
         return logits, loss
+
+    @torch.inference_mode()
+    def score(
+        self,
+        sequences: Sequence[Sequence[int]],
+        top: int = 0,
+        max_tokens: int = 65536,
+    ) -> list[TokenLogprobs]:
+        """Log probabilities of token sequences of different lengths, in packed batches of at
+        most max_tokens tokens (a longer sequence goes alone): for each sequence of n tokens
+        the TokenLogprobs of tokens 1 .. n - 1 given those before, (n - 1,) tensors, with the
+        ``top`` most likely ids at each place.  A sequence has 1 to 2 * block_size tokens."""
+        assert max_tokens >= 1, "max_tokens must be positive"
+        seqs = [[int(t) for t in s] for s in sequences]
+        for s in seqs:
+            assert len(s) > 0, "a sequence must have at least one token"
+            assert len(s) <= self.freqs_cis.shape[0], (
+                f"a sequence of {len(s)} tokens is longer than 2 * block_size ({self.freqs_cis.shape[0]})"
+            )
+            assert all(0 <= t < self.vocab_size for t in s), "a token lies outside the vocabulary"
+        assert 0 <= top <= min(self.vocab_size, _native.MAX_TOP), (
+            f"top must be 0 .. min(vocab_size, {_native.MAX_TOP}), got {top}"
+        )
+        device = self.freqs_cis.device
+        out: list[TokenLogprobs] = []
+        at = 0
+        while at < len(seqs):
+            n, total = 1, len(seqs[at])
+            while at + n < len(seqs) and total + len(seqs[at + n]) <= max_tokens:
+                total += len(seqs[at + n])
+                n += 1
+            batch = seqs[at : at + n]
+            at += n
+            ids = torch.tensor([t for s in batch for t in s], dtype=torch.int64)
+            # the token after each; a sequence's last has none
+            after = torch.cat([ids[1:], ids[:1]])
+            ends = torch.tensor([len(s) for s in batch]).cumsum(0)
+            after[ends - 1] = -1
+            rows = PackedRows([len(s) for s in batch], device)
+            logits, _ = self.forward(ids.to(device).unsqueeze(0), _rows=rows)
+            r = token_logprobs(logits[0], after.to(device), top)
+            del logits
+            for end, s in zip(ends.tolist(), batch):
+                out.append(TokenLogprobs(*(t[end - len(s) : end - 1] for t in r)))
+        return out
+
+    @torch.inference_mode()
+    def forward_tree(self, idx: torch.Tensor, parents: Sequence[int], kv_cache: KVCache) -> torch.Tensor:
+        """Logits (B, N, V) of a tree of N <= 64 tokens idx (B, N) behind every row of the
+        cache: token n follows token parents[n], an earlier one, or for -1 the cached row.
+        The tokens' keys and values lie behind the cached positions until the next append;
+        kv_cache.pos stays, and KVCache.keep goes on with one path of the tree."""
+        B, N = idx.shape
+        assert kv_cache.pos_dev is None, "a captured decode step takes one token per row"
+        assert N == len(parents), f"{N} tokens, {len(parents)} parents"
+        assert B == kv_cache.kv_shape[2], f"{B} rows, a cache of {kv_cache.kv_shape[2]}"
+        rows = TreeRows(parents, kv_cache, idx.device)
+        logits, _ = self.forward(idx, kv_cache=kv_cache, _rows=rows)
+        kv_cache.tree = list(parents)
+        return logits
 
     @torch.inference_mode()
     def generate(

@@ -55,6 +55,7 @@ class KVCache:
         "pos_dev",
         "_normed",
         "_exposed",
+        "tree",
     )
 
     def __init__(
@@ -87,6 +88,9 @@ class KVCache:
         self._normed = True
         # True once the cache tensor was handed to or taken from a caller
         self._exposed = False
+        # the parents of the tree whose tokens lie behind pos (GPT.forward_tree), until
+        # the next append
+        self.tree: list[int] | None = None
 
     @property
     def keys_normed(self) -> bool:
@@ -162,6 +166,7 @@ class KVCache:
         self.pos = 0
         self.shared_prefix = None
         self.keys_normed = True
+        self.tree = None
 
     def get_pos(self) -> int:
         return self.pos
@@ -244,12 +249,14 @@ class KVCache:
             self.shared_prefix = None
         self.pos = n
         self.keys_normed = other.keys_normed
+        self.tree = None
 
     # -- capacity management shared by insert_kv and the fused MHA path --
     def ensure_window(
         self, T_add: int, dtype: torch.dtype, device: torch.device
     ) -> tuple[int, int]:
         """Make room for T_add more positions at ``pos``; returns (t0, t1)."""
+        self.tree = None  # about to be overwritten
         if self._kv.size(0) == 0:
             _native.require_device_type("KVCache", device)
             self._kv = torch.empty(self.kv_shape, dtype=dtype, device=device)
@@ -304,6 +311,36 @@ class KVCache:
         """pos moves once the last layer has written its window (kv_cache.py:113-115)."""
         if layer_idx == self.kv_shape[0] - 1:
             self.pos = t1
+
+    def keep(self, path: "list[int] | list[list[int]]") -> None:
+        """Go on with one path of the tree that GPT.forward_tree ran last: the tokens of
+        ``path``, from a child of the cached row downwards (one list for all rows, or one
+        of the same length for each row), become the next cached positions."""
+        assert self.tree is not None, "no tree lies behind the cached positions"
+        rows = self.kv_shape[2]
+        per_row = len(path) > 0 and isinstance(path[0], (list, tuple))
+        paths = [list(p) for p in path] if per_row else [list(path)]
+        assert not per_row or len(paths) == rows, f"{len(paths)} paths, {rows} rows"
+        n = len(paths[0])
+        for p in paths:
+            assert len(p) == n, "the rows' paths must have one length"
+            above = -1
+            for t in p:
+                assert 0 <= t < len(self.tree) and self.tree[t] == above, f"{p} is no path from the cached row"
+                above = t
+        if n == 0:
+            return
+        t0 = self.pos
+        if any(p != list(range(n)) for p in paths):
+            pages = self._tensor()
+            L, two, B, H, cap, D = pages.shape
+            index = torch.tensor(paths, dtype=torch.int64).to(pages.device) + t0
+            index = index.view(1, 1, len(paths), 1, n, 1).expand(L, two, B, H, n, D)
+            # through a copy of their own: the places overlap
+            kept = torch.gather(pages, 4, index)
+            _native.ops().copy4d(_pages(kept, n), _pages(pages, n, t0))
+        self.tree = None
+        self.pos = t0 + n
 
     # -- reference entry point: copy ready-made k/v (B,H,T,D) into the cache --
     def insert_kv(

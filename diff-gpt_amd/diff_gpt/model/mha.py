@@ -29,7 +29,10 @@ too (dg_block_out, fused with the MLP after them); it then calls _attend, the
 part between, directly.
 """
 
+from __future__ import annotations
+
 import math
+from typing import TYPE_CHECKING
 
 import torch
 import torch.nn.functional as F
@@ -37,6 +40,10 @@ from torch import nn
 
 from diff_gpt import _native
 from diff_gpt.model.kv_cache import KVCache
+
+if TYPE_CHECKING:
+    from diff_gpt.model.packed import PackedRows
+    from diff_gpt.model.tree import TreeRows
 
 # A prefill whose attention output y has at least this many bytes applies the
 # sigmoid gate as the attention kernel stores it (dg_prefill_rope_gate), with the
@@ -166,11 +173,13 @@ class MultiHeadAttention(nn.Module):
         return qkvg[..., 3 * self.n_head * self.head_dim :]
 
     def _attend(self, qkvg: torch.Tensor, freqs_cis: torch.Tensor, kv_cache: KVCache | None,
-                gated: bool = False) -> torch.Tensor:
+                gated: bool = False, rows: PackedRows | TreeRows | None = None) -> torch.Tensor:
         """mha.py:44-83 on the projections qkvg (B, T, 3*inner + C), whose
         column slices are q, k, v and the gate logits: RoPE, QK-norm, the
         cache append and the attention; returns y (B, T, inner) before the
-        gate, or with gated (a prefill: _gates_in_prefill) after it (mha.py:84)."""
+        gate, or with gated (a prefill: _gates_in_prefill) after it (mha.py:84).
+        rows, when given, says which rows attend to which (packed sequences, a
+        tree over the cache) and takes the part between; ungated."""
         B, T, _ = qkvg.size()
         H, D = self.n_head, self.head_dim
         ops = _native.ops()
@@ -179,6 +188,8 @@ class MultiHeadAttention(nn.Module):
         k = qkvg[..., inner : 2 * inner].view(B, T, H, D)
         v = qkvg[..., 2 * inner : 3 * inner].view(B, T, H, D)
 
+        if rows is not None:
+            return rows.attend(self.layer_idx, q, k, v, freqs_cis).reshape(B, T, inner)
         if kv_cache is not None and T == 1:
             return self._decode_step(q, k, v, freqs_cis, kv_cache)
         assert kv_cache is None or kv_cache.pos_dev is None, "a captured decode step takes one token per row"

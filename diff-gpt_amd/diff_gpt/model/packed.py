@@ -2,7 +2,7 @@
 
 Beyond the reference, which takes one length per batch: the sequences' rows follow each
 other in one tensor without padding, and a host-side layout of the batch says whose they
-are.  GPT.score runs series of different lengths through the layers this way.
+are.  GPT.score runs series of different lengths through the layers this way (PackedRows).
 """
 
 import math
@@ -52,3 +52,26 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     if layout.total_q < q.size(0):
         y[layout.total_q :].zero_()
     return y
+
+
+class PackedRows:
+    """A packed batch of whole sequences on its way through the layers: rows (1, total, C),
+    each sequence at positions 0 .. length - 1."""
+
+    __slots__ = ("layout", "positions")
+
+    def __init__(self, lengths: Sequence[int], device: torch.device | str) -> None:
+        self.layout = PackedLayout(lengths, device=device)
+        self.positions = torch.cat([torch.arange(n) for n in self.layout.q_lengths]).to(device)
+
+    def freqs(self, table: torch.Tensor) -> torch.Tensor:
+        """The rows' (1, total, 1, D/2, 2) slice of the RoPE table."""
+        assert max(self.layout.q_lengths) <= table.shape[0], "a sequence is longer than the RoPE table"
+        return table[self.positions].view(1, -1, 1, *table.shape[1:])
+
+    def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               freqs: torch.Tensor) -> torch.Tensor:
+        """RoPE, QK-norm and the attention of one layer's (1, total, H, D) projections."""
+        q_rot, k_rot = (torch.empty(q.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+        _native.ops().rope_qknorm_append(q, k, None, freqs, q_rot, k_rot, None, True)
+        return attention_packed(q_rot[0], k_rot[0], v[0], self.layout).unsqueeze(0)

@@ -3,7 +3,7 @@ a decode step's one, with grouped heads and rows of different lengths.
 
 Beyond the reference.  The tokens' keys and values lie in the cache behind the row's
 cached positions; each token sees all of those, itself and its ancestors in the tree.
-GPT.forward_tree runs candidate continuations through the layers this way.
+GPT.forward_tree runs candidate continuations through the layers this way (TreeRows).
 """
 
 import math
@@ -12,6 +12,7 @@ from typing import Sequence
 import torch
 
 from diff_gpt import _native
+from diff_gpt.model.kv_cache import KVCache
 
 # tokens of a tree: one bit each of a 64-bit mask
 MAX_TREE = 64
@@ -56,3 +57,38 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         scale = 1.0 / math.sqrt(max(1, q.size(-1)))
     _native.attention_tree_(q, k_cache, v_cache, y, scale, lengths, masks)
     return y
+
+
+class TreeRows:
+    """A tree of tokens behind every row of a cache on its way through the layers: rows
+    (B, N, C), token n at the position of its depth, its keys and values in the cache's
+    n-th place behind the cached positions."""
+
+    __slots__ = ("cache", "depths", "masks", "start")
+
+    def __init__(self, parents: Sequence[int], cache: KVCache, device: torch.device | str) -> None:
+        self.cache = cache
+        self.depths = tree_depths(parents)
+        self.masks = tree_masks(parents, device)
+        self.start = cache.get_pos()
+
+    def freqs(self, table: torch.Tensor) -> torch.Tensor:
+        """The tokens' (1, N, 1, D/2, 2) slice of the RoPE table."""
+        positions = [self.start + d for d in self.depths]
+        assert max(positions) < table.shape[0], "the tree is deeper than the RoPE table reaches"
+        index = torch.tensor(positions, dtype=torch.int64).to(table.device)
+        return table[index].view(1, -1, 1, *table.shape[1:])
+
+    def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               freqs: torch.Tensor) -> torch.Tensor:
+        """RoPE, QK-norm, the cache append and the attention of one layer's (B, N, H, D)
+        projections."""
+        cache = self.cache
+        t0, t1 = cache.ensure_window(q.size(1), k.dtype, k.device)
+        pages = cache._tensor()
+        if pages.dtype != k.dtype:
+            raise TypeError(f"KV cache holds {pages.dtype} but the layer computes in {k.dtype}")
+        k_pages, v_pages = (pages[layer_idx, i].transpose(1, 2) for i in range(2))
+        q_rot = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _native.ops().rope_qknorm_append(q, k, v, freqs, q_rot, k_pages[:, t0:t1], v_pages[:, t0:t1], True)
+        return attention_tree(q_rot, k_pages, v_pages, t0, self.masks)
