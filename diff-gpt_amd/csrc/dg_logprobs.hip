@@ -56,12 +56,16 @@ __device__ __forceinline__ void add_logit(float x, float m, float& s, float& t) 
   t = __builtin_fmaf(fmaxf(z, -1e30f), e, t);
 }
 
-// log p(id) and the entropy of a row, by one lane
+// The given token's logit; NaN for an id outside the row.
 template <typename T>
-__device__ __forceinline__ void store_row_stats(const LogprobArgs& a, int64_t row, const T* x, float m, float logs, float s,
+__device__ __forceinline__ float given_logit(const LogprobArgs& a, const T* x, int64_t id) {
+  return id < 0 || id >= a.V ? __builtin_nanf("") : to_f32(x[id]);
+}
+
+// log p(id) and the entropy of a row, by one lane
+__device__ __forceinline__ void store_row_stats(const LogprobArgs& a, int64_t row, float given, float m, float logs, float s,
                                                 float t) {
-  const int64_t id = a.ids[row];
-  static_cast<float*>(a.logprob)[row] = id < 0 || id >= a.V ? __builtin_nanf("") : to_f32(x[id]) - m - logs;
+  static_cast<float*>(a.logprob)[row] = given - m - logs;
   if (a.entropy != nullptr) static_cast<float*>(a.entropy)[row] = logs - t / s;
 }
 
@@ -111,10 +115,14 @@ __device__ __forceinline__ uint64_t dpp_key(uint64_t v) {
   return (uint64_t)dpp_key<CTRL>((uint32_t)v) | ((uint64_t)dpp_key<CTRL>((uint32_t)(v >> 32)) << 32);
 }
 
-template <typename K>
-__device__ __forceinline__ void order_keys(K& hi, K& lo) {
+__device__ __forceinline__ void order_keys(uint32_t& hi, uint32_t& lo) {
+  const uint32_t h = max(hi, lo), l = min(hi, lo);
+  hi = h;
+  lo = l;
+}
+__device__ __forceinline__ void order_keys(uint64_t& hi, uint64_t& lo) {
   const bool swap = lo > hi;
-  const K h = swap ? lo : hi, l = swap ? hi : lo;
+  const uint64_t h = swap ? lo : hi, l = swap ? hi : lo;
   hi = h;
   lo = l;
 }
@@ -200,7 +208,7 @@ __global__ __launch_bounds__(256) void lp_small_kernel(const LogprobArgs a) {
   s = group_sum_dpp<16>(s);
   t = group_sum_dpp<16>(t);
   const float logs = logf(s);
-  if (lane == 0 && r0 < a.M) store_row_stats(a, row, x, m, logs, s, t);
+  if (lane == 0 && r0 < a.M) store_row_stats(a, row, given_logit(a, x, a.ids[row]), m, logs, s, t);
   if constexpr (KP > 0) {
     K k[16];
 #pragma unroll
@@ -284,21 +292,40 @@ struct LpRow {
   float single;
   u32x4_t raw[HELD ? NV : 1];
 
+  T single_raw;
+
   __device__ __forceinline__ u32x4_t vector(int i) const {
     u32x4_t w = {kNone, kNone, kNone, kNone};
     if (i < nvec) w = load16(x + (int64_t)i * VE);
     return w;
   }
-  __device__ __forceinline__ void load(const T* row, int v, int t) {
+  // The loads, without a branch around any but where the row has no vector at all: those
+  // of vectors behind the last re-read it.  `row` is the same for the wave.
+  __device__ __forceinline__ void start(const T* row, int v, int t) {
     x = row;
     V = v;
     tid = t;
     nvec = V / VE;
     extra = tid < V - nvec * VE ? nvec * VE + tid : V;
-    single = extra < V ? to_f32(x[extra]) : kNegInf;
+    single_raw = x[min(extra, V - 1)];
+    if constexpr (HELD) {
+      int at = tid;
+      asm volatile("" : "+v"(at));  // the offsets are worked out for each row, not kept
+      if (NT > 64 || nvec > 0) {  // the larger workgroups' rows always have one
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          raw[j] = load16(reinterpret_cast<const char*>(x) + 16u * (uint32_t)min(j * NT + at, nvec - 1));
+      }
+    }
+  }
+  // they have arrived
+  __device__ __forceinline__ void arrive() {
+    single = extra < V ? to_f32(single_raw) : kNegInf;
     if constexpr (HELD) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) raw[j] = vector(j * NT + tid);
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[j][e] = j * NT + tid < nvec ? raw[j][e] : kNone;
     }
   }
   // The words as they are, unpacked anew by each pass: kept unpacked they would take
@@ -345,11 +372,14 @@ struct LpShared {
   int cand_i[CAP];
 };
 
-// Threads of a row meet here: one wave needs no barrier.
+// Threads of a row meet here, as far as LDS goes: loads of the next row stay in flight.
+// One wave needs no barrier.
 template <int NT>
 __device__ __forceinline__ void lp_sync() {
   if constexpr (NT > 64) {
-    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   } else {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -357,28 +387,17 @@ __device__ __forceinline__ void lp_sync() {
   }
 }
 
-// waves a SIMD that the registers must allow: two rows of 1024 threads on a CU in 16-bit
-// types, whose loads and arithmetic then overlap
-template <typename T, int NT>
-constexpr int lp_row_waves() {
-  return NT == 1024 ? (sizeof(T) == 2 ? 8 : 4) : 4;
-}
-
-// NT threads a row; workgroups of 256 threads at least (several rows where NT is 64).
-template <typename T, int NT, int NV, bool HELD>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void lp_row_kernel(const LogprobArgs a) {
-  constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
-  constexpr int VE = 16 / (int)sizeof(T);
-  __shared__ LpShared<NW, CAP> sh_all[RPB];
-  LpShared<NW, CAP>& sh = sh_all[RPB == 1 ? 0 : threadIdx.x / NT];
-  const int tid = threadIdx.x % NT, lane = tid & 63;
+// One row by its NT threads.  Rows that follow each other need no barrier between them:
+// each shared value is written behind a barrier that its readers of the row before have
+// passed.
+template <typename T, int NT, int NV, bool HELD, int CAP>
+__device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, float given, LpRow<T, NT, NV, HELD>& r,
+                                       LpShared<NT / 64, CAP>& sh) {
+  constexpr int NW = NT / 64, VE = 16 / (int)sizeof(T);
+  const T* x = r.x;
+  const int tid = r.tid, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t row = (int64_t)blockIdx.x * RPB + (RPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT));
-  if (row >= a.M) return;  // RPB > 1: whole waves, which share no barrier
-  const T* x = static_cast<const T*>(a.x) + row * a.ld;
   const int top = a.top;
-  LpRow<T, NT, NV, HELD> r;
-  r.load(x, (int)a.V, tid);
 
   auto vec_max = [](const float(&v)[VE]) __attribute__((always_inline)) {
     float x0 = v[0];
@@ -436,7 +455,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void 
     }
   }
   const float logs = logf(s);
-  if (tid == 0) store_row_stats(a, row, x, m, logs, s, t);
+  if (tid == 0) store_row_stats(a, row, given, m, logs, s, t);
   if (top == 0) return;
 
   int64_t* ids = a.top_ids + row * top;
@@ -551,6 +570,45 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void 
   }
 }
 
+// Waves a SIMD that the registers must allow.
+template <typename T, int NT>
+constexpr int lp_row_waves() {
+  return 4;
+}
+
+// NT threads a row; workgroups of 256 threads at least (several rows where NT is 64).  AHEAD:
+// a workgroup walks rows gridDim.x apart and has the next one's loads in flight while it
+// works on one, since at 1024 threads a row a CU holds no second workgroup to overlap with.
+template <typename T, int NT, int NV, bool HELD, bool AHEAD>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void lp_row_kernel(const LogprobArgs a) {
+  constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
+  __shared__ LpShared<NW, CAP> sh_all[RPB];
+  LpShared<NW, CAP>& sh = sh_all[RPB == 1 ? 0 : threadIdx.x / NT];
+  const int tid = threadIdx.x % NT;
+  const int64_t row = (int64_t)blockIdx.x * RPB + (RPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT));
+  if (row >= a.M) return;  // RPB > 1: whole waves, which share no barrier
+  const T* x = static_cast<const T*>(a.x);
+  LpRow<T, NT, NV, HELD> r;
+  int64_t id = a.ids[row];
+  r.start(x + row * a.ld, (int)a.V, tid);
+  if constexpr (!AHEAD) {
+    r.arrive();
+    lp_row<T, NT, NV, HELD, CAP>(a, row, given_logit(a, r.x, id), r, sh);
+  } else {
+    for (int64_t i = row; i < a.M; i += gridDim.x) {
+      r.arrive();
+      // loads return in order: the given logit's before the next row's
+      const float given = given_logit(a, r.x, id);
+      LpRow<T, NT, NV, HELD> next;
+      const int64_t after = i + gridDim.x < a.M ? i + gridDim.x : i;
+      id = a.ids[after];
+      next.start(x + after * a.ld, (int)a.V, tid);
+      lp_row<T, NT, NV, HELD, CAP>(a, i, given, r, sh);
+      r = next;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // fp64: a wavefront a row
 // ---------------------------------------------------------------------------
@@ -649,21 +707,30 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
 #undef DG_LP
     return check_launch("lp_small_kernel");
   }
-  // a thread holds up to 64 logits
+  // a thread holds up to 64 logits (and as many of the next row)
+  constexpr int64_t kLpRows = 256;  // workgroups of 1024 threads at once
   constexpr int NV = 64 / VE;
   if (a.V <= 64 * 64) {
-    hipLaunchKernelGGL((lp_row_kernel<T, 64, NV, true>), dim3((unsigned)((a.M + 3) / 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((lp_row_kernel<T, 64, NV, true, false>), dim3((unsigned)((a.M + 3) / 4)), dim3(256), 0, s, a);
     return check_launch("lp_row_kernel_64");
   }
   if (a.V <= 64 * 256) {
-    hipLaunchKernelGGL((lp_row_kernel<T, 256, NV, true>), dim3((unsigned)a.M), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((lp_row_kernel<T, 256, NV, true, false>), dim3((unsigned)a.M), dim3(256), 0, s, a);
     return check_launch("lp_row_kernel_256");
   }
   if (a.V <= 64 * 1024) {
-    hipLaunchKernelGGL((lp_row_kernel<T, 1024, NV, true>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+    if constexpr (sizeof(T) == 2)
+      hipLaunchKernelGGL((lp_row_kernel<T, 1024, NV, true, true>), dim3((unsigned)(a.M < kLpRows ? a.M : kLpRows)),
+                         dim3(1024), 0, s, a);
+    else
+      hipLaunchKernelGGL((lp_row_kernel<T, 1024, NV, true, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
     return check_launch("lp_row_kernel_1024");
   }
-  hipLaunchKernelGGL((lp_row_kernel<T, 1024, 1, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+  if constexpr (sizeof(T) == 2) if (a.V <= 128 * 1024) {
+    hipLaunchKernelGGL((lp_row_kernel<T, 1024, 2 * NV, true, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+    return check_launch("lp_row_kernel_1024");
+  }
+  hipLaunchKernelGGL((lp_row_kernel<T, 1024, 1, false, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
   return check_launch("lp_long_kernel");
 }
 

@@ -889,27 +889,44 @@ def token_logprobs_(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Ten
     """dg_token_logprobs: per row of logits (M,V) the log probability of ids (M,) int64 and
     the entropy into (M,) tensors, and with top_logprobs, top_ids (M,top) the most likely
     alternatives.  The results are fp32, fp64 for fp64 logits."""
+    out = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    if (top_logprobs is None) != (top_ids is None):
+        raise ValueError("token_logprobs: top_logprobs and top_ids come together")
+    M, top = logits.size(0), 0 if top_ids is None else top_ids.size(-1)
+    for name, t, shape, dtype in (("logprobs", logprobs, (M,), out), ("entropy", entropy, (M,), out),
+                                  ("top_logprobs", top_logprobs, (M, top), out), ("top_ids", top_ids, (M, top), torch.int64)):
+        if t is not None and (t.dtype != dtype or t.shape != shape or t.device != logits.device or not t.is_contiguous()):
+            raise ValueError(f"token_logprobs: {name} must be a contiguous {shape} {dtype} tensor on the logits' device")
+    _token_logprobs(logits, ids, top, logprobs, entropy, top_logprobs, top_ids)
+
+
+def new_token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int) -> tuple[torch.Tensor, ...]:
+    """token_logprobs_ into tensors of its own: (logprobs, entropy, top_logprobs, top_ids)."""
+    out = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    M, device = logits.size(0), logits.device
+    r = (torch.empty(M, dtype=out, device=device), torch.empty(M, dtype=out, device=device),
+         torch.empty((M, top), dtype=out, device=device), torch.empty((M, top), dtype=torch.int64, device=device))
+    _token_logprobs(logits, ids, top, *r)
+    return r
+
+
+def _token_logprobs(logits, ids, top, logprobs, entropy, top_logprobs, top_ids) -> None:
+    """The launch into outputs that fit, once logits and ids have been looked over."""
     device = _check_tensors("token_logprobs", logits)
     if logits.dim() != 2:
         raise ValueError(f"token_logprobs: logits must be (M, V), got {tuple(logits.shape)}")
     M, V = logits.shape
     if V < 1:
         raise ValueError("token_logprobs: an empty vocabulary")
-    if V > 1 and logits.stride(1) != 1:
+    ld, unit = logits.stride()
+    if V > 1 and unit != 1:
         raise ValueError("token_logprobs: the last (vocabulary) dimension must be contiguous")
-    out = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    if (top_logprobs is None) != (top_ids is None):
-        raise ValueError("token_logprobs: top_logprobs and top_ids come together")
-    top = 0 if top_ids is None else top_ids.size(-1)
     if not 0 <= top <= min(V, MAX_TOP):
         raise ValueError(f"token_logprobs: top {top} outside 0 .. min(V, {MAX_TOP})")
-    for name, t, shape, dtype in (("ids", ids, (M,), torch.int64), ("logprobs", logprobs, (M,), out),
-                                  ("entropy", entropy, (M,), out), ("top_logprobs", top_logprobs, (M, top), out),
-                                  ("top_ids", top_ids, (M, top), torch.int64)):
-        if t is not None and (t.dtype != dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous()):
-            raise ValueError(f"token_logprobs: {name} must be a contiguous {shape} {dtype} tensor on the logits' device")
+    if ids.dtype != torch.int64 or ids.shape != (M,) or ids.get_device() != device or not ids.is_contiguous():
+        raise ValueError(f"token_logprobs: ids must be a contiguous ({M},) int64 tensor on the logits' device")
     _launch("token_logprobs", device, lib().dg_token_logprobs, M, V, _DTYPE_CODE[logits.dtype], logits.data_ptr(),
-            logits.stride(0), ids.data_ptr(), logprobs.data_ptr(), None if entropy is None else entropy.data_ptr(), top,
+            ld, ids.data_ptr(), logprobs.data_ptr(), None if entropy is None else entropy.data_ptr(), top,
             None if top_ids is None else top_logprobs.data_ptr(), None if top_ids is None else top_ids.data_ptr())
 
 

@@ -30,20 +30,10 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tok
         raise ValueError(f"token_logprobs: ids {tuple(ids.shape)} for logits {tuple(logits.shape)}")
     if not 0 <= top <= min(V, _native.MAX_TOP):
         raise ValueError(f"token_logprobs: top {top} outside 0 .. min(V, {_native.MAX_TOP})")
-    _native.require_device("token_logprobs", logits, ids)
-    flat = logits.dim() == 2
-    x = logits if flat else logits.reshape(-1, V)
+    if len(lead) == 1 and logits.stride(1) == 1 and ids.is_contiguous():
+        return TokenLogprobs(*_native.new_token_logprobs(logits, ids, top))
+    x = logits.reshape(-1, V)
     if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    M = x.size(0)
-    out = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    device = logits.device
-    r = TokenLogprobs(
-        torch.empty(M, dtype=out, device=device), torch.empty(M, dtype=out, device=device),
-        torch.empty((M, top), dtype=out, device=device), torch.empty((M, top), dtype=torch.int64, device=device),
-    )
-    _native.token_logprobs_(x, ids.reshape(M).contiguous(), *r)
-    if flat:
-        return r
-    return TokenLogprobs(r.logprobs.view(lead), r.entropy.view(lead), r.top_logprobs.view(*lead, top),
-                         r.top_ids.view(*lead, top))
+    lp, entropy, top_lp, top_ids = _native.new_token_logprobs(x, ids.reshape(x.size(0)).contiguous(), top)
+    return TokenLogprobs(lp.view(lead), entropy.view(lead), top_lp.view(*lead, top), top_ids.view(*lead, top))
