@@ -362,11 +362,10 @@ struct LpRow {
 // LDS of a row's threads
 template <int NW, int CAP>
 struct LpShared {
-  float part[NW][64];   // the lanes' maxima
-  float sum[NW], tsum[NW];
-  float bound;          // the k-th of the maxima
-  int count;            // candidates
-  float best_v[NW];     // a round's first logit of each wave
+  float part[NW][64];                 // the lanes' maxima
+  float wmax[NW], sum[NW], tsum[NW];  // m, s and t of the waves' parts
+  int count[2];                       // candidates of this row; of the next, cleared ahead
+  float best_v[NW];                   // a round's first logit of each wave
   int best_i[NW];
   float cand_v[CAP];
   int cand_i[CAP];
@@ -387,11 +386,12 @@ __device__ __forceinline__ void lp_sync() {
   }
 }
 
-// One row by its NT threads.  Rows that follow each other need no barrier between them:
-// each shared value is written behind a barrier that its readers of the row before have
-// passed.
+// One row by its NT threads, which meet twice: when every wave's part of the softmax is
+// known, and when the candidates are collected.  Rows that follow each other need no
+// barrier between them: what one writes in LDS lies behind a barrier that the readers of
+// the row before have passed.  odd: the row's parity.
 template <typename T, int NT, int NV, bool HELD, int CAP>
-__device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, float given, LpRow<T, NT, NV, HELD>& r,
+__device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, int odd, float given, LpRow<T, NT, NV, HELD>& r,
                                        LpShared<NT / 64, CAP>& sh) {
   constexpr int NW = NT / 64, VE = 16 / (int)sizeof(T);
   const T* x = r.x;
@@ -406,67 +406,75 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, float 
     return x0;
   };
   float vmax[HELD ? NV : 1];  // each vector's maximum
-  float m = r.single, s = 0.f, t = 0.f;
-  m = fmaxf(m, kNegInf);  // a NaN is no maximum
+  const float single_max = fmaxf(r.single, kNegInf);  // a NaN is no maximum
+  float mine = single_max;
   r.vectors([&](const float(&v)[VE], int, int j) __attribute__((always_inline)) {
     const float x0 = vec_max(v);
     if constexpr (HELD) vmax[j] = x0;
-    m = fmaxf(m, x0);
+    mine = fmaxf(mine, x0);
   });
   r.forget_unpacked();
-  if constexpr (NW > 1) {
-    sh.part[wv][lane] = m;
-    lp_sync<NT>();
-    m = sh.part[0][lane];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) m = fmaxf(m, sh.part[w][lane]);
-  }
-  const float part = m;  // of a 64th of the row
-  m = wave_max(part);
-  if (top > 0 && wv == 0) {
-    const float bound = kth_largest<T>(part, top);
-    if (lane == 0) {
-      sh.bound = bound;
-      sh.count = 0;
-    }
-  }
-  if (r.extra < r.V) add_logit(r.single, m, s, t);
+  // s and t of the thread's logits about its own maximum, then of the wave's about the wave's
+  // (-inf alone: about the lowest number, which leaves s at 0)
+  const float own = fmaxf(mine, -3.402823466e38f);
+  float s = 0.f, t = 0.f;
+  if (r.extra < r.V) add_logit(r.single, own, s, t);
   r.vectors([&](const float(&v)[VE], int, int) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < VE; ++c) add_logit(v[c], m, s, t);
+    for (int c = 0; c < VE; ++c) add_logit(v[c], own, s, t);
   });
   r.forget_unpacked();
+  auto about = [](float& s1, float& t1, float m1, float m2) __attribute__((always_inline)) {
+    const float d = m1 - m2;  // <= 0; where it overflows, or the factor vanishes, nothing is left
+    const float f = __builtin_amdgcn_exp2f(d * kLog2e);
+    t1 = f == 0.f ? 0.f : f * __builtin_fmaf(d, s1, t1);
+    s1 = f * s1;
+  };
+  float m = wave_max(own);
+  about(s, t, own, m);
   s = group_sum_dpp<64>(s);
   t = group_sum_dpp<64>(t);
+  float part = mine;
   if constexpr (NW > 1) {
+    sh.part[wv][lane] = mine;
     if (lane == 0) {
+      sh.wmax[wv] = m;
       sh.sum[wv] = s;
       sh.tsum[wv] = t;
     }
-  }
-  lp_sync<NT>();
-  if constexpr (NW > 1) {
-    s = sh.sum[0];
-    t = sh.tsum[0];
+    lp_sync<NT>();
+    // every wave joins the waves' parts, a lane each
+    const int w = lane & (NW - 1);
+    const float mw = sh.wmax[w];
+    s = sh.sum[w];
+    t = sh.tsum[w];
+    m = wave_max(mw);
+    about(s, t, mw, m);
+    s = group_sum_dpp<NW>(s);
+    t = group_sum_dpp<NW>(t);
+    part = sh.part[0][lane];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      s += sh.sum[w];
-      t += sh.tsum[w];
-    }
+    for (int v = 1; v < NW; ++v) part = fmaxf(part, sh.part[v][lane]);
   }
-  const float logs = logf(s);
-  if (tid == 0) store_row_stats(a, row, given, m, logs, s, t);
+  const float logs = wave_max(part) == kNegInf ? __builtin_nanf("") : logf(s);
+  if (tid == 0) {
+    sh.count[odd ^ 1] = 0;
+    if (NW == 1) sh.count[odd] = 0;
+    store_row_stats(a, row, given, m, logs, s, t);
+  }
   if (top == 0) return;
+  if constexpr (NW == 1) lp_sync<NT>();
 
   int64_t* ids = a.top_ids + row * top;
   float* lps = static_cast<float*>(a.top_logprob) + row * top;
-  const float bound = sh.bound;
+  const float bound = kth_largest<T>(part, top);
+  int& count = sh.count[odd];
   // a logit that passes, into LDS as far as there is room; the wave's lanes together
   auto offer = [&](bool in, float v, int id) __attribute__((always_inline)) {
     const uint64_t b = __builtin_amdgcn_ballot_w64(in);
     if (b != 0) {
       int at = 0;
-      if (lane == 0) at = atomicAdd(&sh.count, __builtin_popcountll(b));
+      if (lane == 0) at = atomicAdd(&count, __builtin_popcountll(b));
       at = __builtin_amdgcn_readfirstlane(at);
       at += __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
       if (in && at < CAP) {
@@ -487,7 +495,7 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, float 
       }
     }
   };
-  offer(r.single >= bound && r.extra < r.V, r.single, r.extra);
+  if (__builtin_amdgcn_ballot_w64(single_max >= bound) != 0) offer(r.single >= bound && r.extra < r.V, r.single, r.extra);
   r.vectors([&](const float(&v)[VE], int id, int j) __attribute__((always_inline)) {
     float most;
     if constexpr (HELD) most = vmax[j];
@@ -497,7 +505,7 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, float 
     for (int c = 0; c < VE; ++c) offer(v[c] >= bound && id < r.V, v[c], id + c);
   });
   lp_sync<NT>();
-  const int n = sh.count;
+  const int n = count;
   if (n >= top && n <= CAP) {
     rank(n);
     return;
@@ -505,14 +513,14 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, float 
   // Rare from here on, and read from memory again.  Too many: those above the bound, and
   // of those equal to it the first in id order.
   lp_sync<NT>();  // everyone has read the count
-  if (tid == 0) sh.count = 0;
+  if (tid == 0) count = 0;
   lp_sync<NT>();
   for (int v0 = tid - lane; v0 < r.V; v0 += NT) {
     const float v = to_f32(x[min(v0 + lane, r.V - 1)]);
     offer(v > bound && v0 + lane < r.V, v, v0 + lane);
   }
   lp_sync<NT>();
-  const int above = sh.count;
+  const int above = count;
   if (n >= top && above <= CAP) {
     rank(above);
     if (wv == 0) {
@@ -588,13 +596,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void 
   const int64_t row = (int64_t)blockIdx.x * RPB + (RPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT));
   if (row >= a.M) return;  // RPB > 1: whole waves, which share no barrier
   const T* x = static_cast<const T*>(a.x);
+  // the first row's candidates, counted behind its first barrier
+  if (NT > 64 && threadIdx.x == 0) sh.count[0] = 0;
   LpRow<T, NT, NV, HELD> r;
   int64_t id = a.ids[row];
   r.start(x + row * a.ld, (int)a.V, tid);
   if constexpr (!AHEAD) {
     r.arrive();
-    lp_row<T, NT, NV, HELD, CAP>(a, row, given_logit(a, r.x, id), r, sh);
+    lp_row<T, NT, NV, HELD, CAP>(a, row, 0, given_logit(a, r.x, id), r, sh);
   } else {
+    int odd = 0;
     for (int64_t i = row; i < a.M; i += gridDim.x) {
       r.arrive();
       // loads return in order: the given logit's before the next row's
@@ -603,8 +614,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void 
       const int64_t after = i + gridDim.x < a.M ? i + gridDim.x : i;
       id = a.ids[after];
       next.start(x + after * a.ld, (int)a.V, tid);
-      lp_row<T, NT, NV, HELD, CAP>(a, i, given, r, sh);
+      lp_row<T, NT, NV, HELD, CAP>(a, i, odd, given, r, sh);
       r = next;
+      odd ^= 1;
     }
   }
 }
