@@ -584,7 +584,8 @@ namespace {
 template <typename T, int D, int RT, bool TREE>
 int launch_seq(const SeqArgs& a, dim3 grid, hipStream_t s) {
   hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, TREE>), grid, dim3(64 * SeqCfg<T, D, RT>::WAVES), 0, s, a);
-  return check_launch(TREE ? "seq_mfma_tree_kernel" : "seq_mfma_packed_kernel");
+  return check_launch(TREE ? (RT == 1 ? "seq_mfma_tree_32" : RT == 2 ? "seq_mfma_tree_64" : "seq_mfma_tree_128")
+                           : (RT == 1 ? "seq_mfma_packed_32" : RT == 2 ? "seq_mfma_packed_64" : "seq_mfma_packed_128"));
 }
 
 template <typename T, int RT, bool TREE>

@@ -79,9 +79,13 @@ template <typename T>
 struct LpKey {
   using type = uint32_t;  // 16 bits of value, 16 of id
   static __device__ __forceinline__ uint32_t make(T v, int id) {
-    const uint32_t b = from_f32<T>(to_f32(v) + 0.f).bits;  // -0 ranks as 0
-    const uint32_t u = (b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u;
-    return ((to_f32(v) != to_f32(v) ? 0u : u) << 16) | (0xffffu - (uint32_t)id);
+    const float f = to_f32(v) + 0.f;  // -0 ranks as 0
+    uint32_t u;                       // the value's bits in the upper half
+    if constexpr (__is_same(T, bf16_t)) u = __float_as_uint(f);
+    else u = (uint32_t)from_f32<T>(f).bits << 16;
+    u ^= (uint32_t)((int)u >> 31) | 0x80000000u;
+    u = f != f ? 0u : u;
+    return (u & 0xffff0000u) | (0xffffu - (uint32_t)id);
   }
   static __device__ __forceinline__ int id(uint32_t k) { return 0xffff - (int)(k & 0xffffu); }
   static __device__ __forceinline__ float value(uint32_t k) {
@@ -108,7 +112,7 @@ struct LpKey<float> {
 
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_key(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);  // every lane has a partner
 }
 template <int CTRL>
 __device__ __forceinline__ uint64_t dpp_key(uint64_t v) {
@@ -364,7 +368,7 @@ template <int NW, int CAP>
 struct LpShared {
   float part[NW][64];                 // the lanes' maxima
   float wmax[NW], sum[NW], tsum[NW];  // m, s and t of the waves' parts
-  int count[2];                       // candidates of this row; of the next, cleared ahead
+  int count;                          // candidates
   float best_v[NW];                   // a round's first logit of each wave
   int best_i[NW];
   float cand_v[CAP];
@@ -386,18 +390,35 @@ __device__ __forceinline__ void lp_sync() {
   }
 }
 
-// One row by its NT threads, which meet twice: when every wave's part of the softmax is
-// known, and when the candidates are collected.  Rows that follow each other need no
-// barrier between them: what one writes in LDS lies behind a barrier that the readers of
-// the row before have passed.  odd: the row's parity.
-template <typename T, int NT, int NV, bool HELD, int CAP>
-__device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, int odd, float given, LpRow<T, NT, NV, HELD>& r,
-                                       LpShared<NT / 64, CAP>& sh) {
-  constexpr int NW = NT / 64, VE = 16 / (int)sizeof(T);
-  const T* x = r.x;
-  const int tid = r.tid, lane = tid & 63;
+// Waves a SIMD that the registers must allow: two rows of 1024 threads on a CU, whose loads
+// and arithmetic then overlap, as long as a thread's logits leave room (2048 x 49999 bf16:
+// one row on a CU 95 us, one with the next one's loads in flight 87, two 68).
+template <typename T, int NT, int NV>
+constexpr int lp_row_waves() {
+  return NT >= 512 && NV <= 8 ? 8 : 4;
+}
+
+// NT threads a row, which meet twice: when every wave's part of the softmax is known, and
+// when the candidates are collected.  Workgroups of 256 threads at least (several rows
+// where NT is 64).
+template <typename T, int NT, int NV, bool HELD>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV>())) void lp_row_kernel(const LogprobArgs a) {
+  constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
+  constexpr int VE = 16 / (int)sizeof(T);
+  __shared__ LpShared<NW, CAP> sh_all[RPB];
+  LpShared<NW, CAP>& sh = sh_all[RPB == 1 ? 0 : threadIdx.x / NT];
+  const int tid = threadIdx.x % NT, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = (int64_t)blockIdx.x * RPB + (RPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT));
+  if (row >= a.M) return;  // RPB > 1: whole waves, which share no barrier
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
   const int top = a.top;
+  const int64_t given_id = a.ids[row];
+  LpRow<T, NT, NV, HELD> r;
+  r.start(x, (int)a.V, tid);
+  const float given = given_logit(a, x, given_id);
+  if (tid == 0) sh.count = 0;
+  r.arrive();
 
   auto vec_max = [](const float(&v)[VE]) __attribute__((always_inline)) {
     float x0 = v[0];
@@ -457,24 +478,19 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, int od
     for (int v = 1; v < NW; ++v) part = fmaxf(part, sh.part[v][lane]);
   }
   const float logs = wave_max(part) == kNegInf ? __builtin_nanf("") : logf(s);
-  if (tid == 0) {
-    sh.count[odd ^ 1] = 0;
-    if (NW == 1) sh.count[odd] = 0;
-    store_row_stats(a, row, given, m, logs, s, t);
-  }
+  if (tid == 0) store_row_stats(a, row, given, m, logs, s, t);
   if (top == 0) return;
   if constexpr (NW == 1) lp_sync<NT>();
 
   int64_t* ids = a.top_ids + row * top;
   float* lps = static_cast<float*>(a.top_logprob) + row * top;
   const float bound = kth_largest<T>(part, top);
-  int& count = sh.count[odd];
   // a logit that passes, into LDS as far as there is room; the wave's lanes together
   auto offer = [&](bool in, float v, int id) __attribute__((always_inline)) {
     const uint64_t b = __builtin_amdgcn_ballot_w64(in);
     if (b != 0) {
       int at = 0;
-      if (lane == 0) at = atomicAdd(&count, __builtin_popcountll(b));
+      if (lane == 0) at = atomicAdd(&sh.count, __builtin_popcountll(b));
       at = __builtin_amdgcn_readfirstlane(at);
       at += __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
       if (in && at < CAP) {
@@ -505,7 +521,7 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, int od
     for (int c = 0; c < VE; ++c) offer(v[c] >= bound && id < r.V, v[c], id + c);
   });
   lp_sync<NT>();
-  const int n = count;
+  const int n = sh.count;
   if (n >= top && n <= CAP) {
     rank(n);
     return;
@@ -513,14 +529,14 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, int od
   // Rare from here on, and read from memory again.  Too many: those above the bound, and
   // of those equal to it the first in id order.
   lp_sync<NT>();  // everyone has read the count
-  if (tid == 0) count = 0;
+  if (tid == 0) sh.count = 0;
   lp_sync<NT>();
   for (int v0 = tid - lane; v0 < r.V; v0 += NT) {
     const float v = to_f32(x[min(v0 + lane, r.V - 1)]);
     offer(v > bound && v0 + lane < r.V, v, v0 + lane);
   }
   lp_sync<NT>();
-  const int above = count;
+  const int above = sh.count;
   if (n >= top && above <= CAP) {
     rank(above);
     if (wv == 0) {
@@ -574,49 +590,6 @@ __device__ __forceinline__ void lp_row(const LogprobArgs& a, int64_t row, int od
     if (tid == 0) {
       ids[j] = bi;
       lps[j] = bv - m - logs;
-    }
-  }
-}
-
-// Waves a SIMD that the registers must allow.
-template <typename T, int NT>
-constexpr int lp_row_waves() {
-  return 4;
-}
-
-// NT threads a row; workgroups of 256 threads at least (several rows where NT is 64).  AHEAD:
-// a workgroup walks rows gridDim.x apart and has the next one's loads in flight while it
-// works on one, since at 1024 threads a row a CU holds no second workgroup to overlap with.
-template <typename T, int NT, int NV, bool HELD, bool AHEAD>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT>())) void lp_row_kernel(const LogprobArgs a) {
-  constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
-  __shared__ LpShared<NW, CAP> sh_all[RPB];
-  LpShared<NW, CAP>& sh = sh_all[RPB == 1 ? 0 : threadIdx.x / NT];
-  const int tid = threadIdx.x % NT;
-  const int64_t row = (int64_t)blockIdx.x * RPB + (RPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT));
-  if (row >= a.M) return;  // RPB > 1: whole waves, which share no barrier
-  const T* x = static_cast<const T*>(a.x);
-  // the first row's candidates, counted behind its first barrier
-  if (NT > 64 && threadIdx.x == 0) sh.count[0] = 0;
-  LpRow<T, NT, NV, HELD> r;
-  int64_t id = a.ids[row];
-  r.start(x + row * a.ld, (int)a.V, tid);
-  if constexpr (!AHEAD) {
-    r.arrive();
-    lp_row<T, NT, NV, HELD, CAP>(a, row, 0, given_logit(a, r.x, id), r, sh);
-  } else {
-    int odd = 0;
-    for (int64_t i = row; i < a.M; i += gridDim.x) {
-      r.arrive();
-      // loads return in order: the given logit's before the next row's
-      const float given = given_logit(a, r.x, id);
-      LpRow<T, NT, NV, HELD> next;
-      const int64_t after = i + gridDim.x < a.M ? i + gridDim.x : i;
-      id = a.ids[after];
-      next.start(x + after * a.ld, (int)a.V, tid);
-      lp_row<T, NT, NV, HELD, CAP>(a, i, odd, given, r, sh);
-      r = next;
-      odd ^= 1;
     }
   }
 }
@@ -719,30 +692,27 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
 #undef DG_LP
     return check_launch("lp_small_kernel");
   }
-  // a thread holds up to 64 logits (and as many of the next row)
-  constexpr int64_t kLpRows = 256;  // workgroups of 1024 threads at once
-  constexpr int NV = 64 / VE;
-  if (a.V <= 64 * 64) {
-    hipLaunchKernelGGL((lp_row_kernel<T, 64, NV, true, false>), dim3((unsigned)((a.M + 3) / 4)), dim3(256), 0, s, a);
-    return check_launch("lp_row_kernel_64");
-  }
-  if (a.V <= 64 * 256) {
-    hipLaunchKernelGGL((lp_row_kernel<T, 256, NV, true, false>), dim3((unsigned)a.M), dim3(256), 0, s, a);
-    return check_launch("lp_row_kernel_256");
-  }
-  if (a.V <= 64 * 1024) {
-    if constexpr (sizeof(T) == 2)
-      hipLaunchKernelGGL((lp_row_kernel<T, 1024, NV, true, true>), dim3((unsigned)(a.M < kLpRows ? a.M : kLpRows)),
-                         dim3(1024), 0, s, a);
-    else
-      hipLaunchKernelGGL((lp_row_kernel<T, 1024, NV, true, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
-    return check_launch("lp_row_kernel_1024");
-  }
-  if constexpr (sizeof(T) == 2) if (a.V <= 128 * 1024) {
-    hipLaunchKernelGGL((lp_row_kernel<T, 1024, 2 * NV, true, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
-    return check_launch("lp_row_kernel_1024");
-  }
-  hipLaunchKernelGGL((lp_row_kernel<T, 1024, 1, false, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+  // The least threads that hold the row, 16 to 64 logits each (128 in 16-bit types from
+  // 65537 on).  More threads a row gain little where rows are few (256 x 4000, 64 -> 1024
+  // threads: 9.7 -> 8.2 us) and lose elsewhere (512 x 2000: 8.6 -> 11.0).
+#define DG_LP_ROW(NT, PER)                                                                                           \
+  do {                                                                                                               \
+    constexpr int kRows = (NT) < 256 ? 256 / (NT) : 1;                                                               \
+    hipLaunchKernelGGL((lp_row_kernel<T, (NT), (PER) / VE, true>), dim3((unsigned)((a.M + kRows - 1) / kRows)),      \
+                       dim3((NT) < 256 ? 256 : (NT)), 0, s, a);                                                      \
+    return check_launch("lp_row_kernel_" #NT);                                                                       \
+  } while (0)
+  if (a.V <= 16 * 64) DG_LP_ROW(64, 16);
+  if (a.V <= 32 * 64) DG_LP_ROW(64, 32);
+  if (a.V <= 64 * 64) DG_LP_ROW(64, 64);
+  if (a.V <= 32 * 256) DG_LP_ROW(256, 32);
+  if (a.V <= 64 * 256) DG_LP_ROW(256, 64);
+  if (a.V <= 64 * 512) DG_LP_ROW(512, 64);
+  if (a.V <= 64 * 1024) DG_LP_ROW(1024, 64);
+  if constexpr (sizeof(T) == 2)
+    if (a.V <= 128 * 1024) DG_LP_ROW(1024, 128);
+#undef DG_LP_ROW
+  hipLaunchKernelGGL((lp_row_kernel<T, 1024, 1, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
   return check_launch("lp_long_kernel");
 }
 

@@ -903,9 +903,8 @@ def token_logprobs_(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Ten
 def new_token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int) -> tuple[torch.Tensor, ...]:
     """token_logprobs_ into tensors of its own: (logprobs, entropy, top_logprobs, top_ids)."""
     out = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    M, device = logits.size(0), logits.device
-    r = (torch.empty(M, dtype=out, device=device), torch.empty(M, dtype=out, device=device),
-         torch.empty((M, top), dtype=out, device=device), torch.empty((M, top), dtype=torch.int64, device=device))
+    M, new = logits.size(0), logits.new_empty
+    r = new(M, dtype=out), new(M, dtype=out), new((M, top), dtype=out), new((M, top), dtype=torch.int64)
     _token_logprobs(logits, ids, top, *r)
     return r
 

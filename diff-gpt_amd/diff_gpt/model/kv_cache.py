@@ -120,6 +120,7 @@ class KVCache:
         self._kv = value
         self._prefix_kv = None
         self._exposed = True  # contents from the caller
+        self.tree = None
 
     def _tensor(self) -> torch.Tensor:
         """The (L, 2, B, H, Tcap, D) cache tensor for the library's own reads

@@ -208,6 +208,22 @@ def test_tree_and_keep_over_a_shared_prefix(dev):
         assert bool(((got - want).abs() <= TOL[torch.float32]).all())
 
 
+def test_a_tree_behind_an_empty_cache(dev):
+    """No cached position: the roots see themselves alone, as a first token does."""
+    model = _gpt(dev)
+    nodes = torch.tensor([[5, 9, 7, 200]], device=dev)
+    with torch.inference_mode():
+        cache = KVCache(1, 4, 16, 16, 2)
+        logits = model.forward_tree(nodes, [-1, 0, -1, 2], cache)
+        for path in ([0, 1], [2, 3]):
+            want = model(nodes[:, path])[0]
+            assert bool(((logits[:, path] - want).abs() <= TOL[torch.float32]).all())
+        cache.keep([2, 3])
+        got = model(nodes[:, :1], kv_cache=cache)[0][:, -1]
+        want = model(nodes[:, [2, 3, 0]])[0][:, -1]
+        assert bool(((got - want).abs() <= TOL[torch.float32]).all())
+
+
 def test_tree_refusals(dev):
     model = _gpt(dev)
     ids = torch.tensor([_series([20], 256)[0]], device=dev)

@@ -56,6 +56,54 @@ def test_packed_matches_float64(dev, dtype, H, Hkv, D, q_lens, k_lens):
     _check_packed(q, k, v, y, q_lens, k_lens, dtype)
 
 
+# lengths that leave a tile's waves unequal work, 14 tiles in all without groups
+MIXED = ([130, 5, 64, 200, 1, 128, 33, 300], [130, 40, 64, 333, 1, 100, 33, 300])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("Hkv,G,copies,rows", [(1, 1, 1, 32), (8, 1, 2, 64), (4, 3, 2, 64), (8, 1, 7, 128), (6, 2, 7, 128)])
+def test_packed_in_every_workgroup_shape(dev, dtype, D, Hkv, G, copies, rows):
+    """One, two and four 32-row waves a tile, by how many tiles there are."""
+    q_lens, k_lens = MIXED[0] * copies, MIXED[1] * copies
+    q, k, v = _packed_case(dev, q_lens, k_lens, Hkv * G, Hkv, D, TDT[dtype], seed=copies)
+    y = attention_packed(q, k, v, PackedLayout(q_lens, k_lens, group=G))
+    assert _native.last_kernel() == f"seq_mfma_packed_{rows}"
+    _check_packed(q, k, v, y, q_lens, k_lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("Hkv,copies,rows", [(1, 1, 32), (8, 2, 64), (8, 7, 128)])
+def test_packed_hidden_values_in_every_workgroup_shape(dev, dtype, D, Hkv, copies, rows):
+    """NaN keys and infinite and NaN values that some rows of a tile see and others do not:
+    bits of the rows that do not are those without them."""
+    q_lens, k_lens = MIXED[0] * copies, MIXED[1] * copies
+    q, k, v = (x.clone() for x in _packed_case(dev, q_lens, k_lens, Hkv, Hkv, D, TDT[dtype], seed=8))
+    lay = PackedLayout(q_lens, k_lens)
+    clean = attention_packed(q, k, v, lay)
+    kk, vv = k.clone(), v.clone()
+    hidden = torch.ones(q.size(0), dtype=torch.bool, device=dev)
+    what = torch.zeros(q.size(0), device=dev)
+    a = b = 0
+    for i, (n, t) in enumerate(zip(q_lens, k_lens)):
+        at = (37 * (i + 1)) % t  # the key that is not finite
+        first = max(0, at - (t - n))
+        vv[b + at] = (INF, -INF, NAN)[i % 3]
+        what[a + first : a + n] = (INF, -INF, NAN)[i % 3]
+        if i % 4 == 3:
+            kk[b + at] = NAN
+            what[a + first : a + n] = NAN
+        hidden[a + first : a + n] = False
+        a, b = a + n, b + t
+    y = attention_packed(q, kk, vv, lay)
+    assert _native.last_kernel() == f"seq_mfma_packed_{rows}"
+    assert torch.equal(y[hidden], clean[hidden])
+    want = what[~hidden][:, None, None].expand_as(y[~hidden])
+    got = y[~hidden].float()
+    assert bool(((got == want) | (got.isnan() & want.isnan())).all())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
 @pytest.mark.parametrize("H,Hkv,D", [(2, 2, 1), (3, 1, 7), (2, 1, 24), (4, 2, 80), (2, 2, 96), (2, 1, 256), (1, 1, 1000)])
 def test_packed_takes_every_head_dim(dev, dtype, H, Hkv, D):
@@ -195,6 +243,22 @@ def test_tree_matches_float64(dev, dtype, H, Hkv, D, N, lens, Tcap):
     q, k, v = _tree_case(dev, len(lens), N, H, Hkv, Tcap, D, TDT[dtype], seed=N + D)
     parents = some_tree(N, seed=N)
     y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+    rows = N * (H // Hkv)
+    assert _native.last_kernel() in (f"seq_mfma_tree_{32 if rows <= 32 else 64 if rows <= 64 else 128}", "seq_join_kernel")
+    _check_tree(q, k, v, y, lens, parents, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("N,G", [(3, 1), (13, 4), (40, 3)])
+@pytest.mark.parametrize("B,Tcap", [(1, 60000), (2, 9000)])
+def test_tree_splits_meet(dev, dtype, D, N, G, B, Tcap):
+    """Rows split over many and over few workgroups, of very different lengths."""
+    lens = [Tcap - N, 700][:B]
+    q, k, v = _tree_case(dev, B, N, 2 * G, 2, Tcap, D, TDT[dtype], seed=G)
+    parents = some_tree(N, seed=2)
+    y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+    assert _native.last_kernel() == "seq_join_kernel"
     _check_tree(q, k, v, y, lens, parents, dtype)
 
 
