@@ -355,8 +355,10 @@ struct LpRow {
       f(v, id, j);
     };
     if constexpr (HELD) {
+      const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) vec(raw[j], j * NT + tid, j);
+      for (int j = 0; j < NV; ++j)
+        if (j * NT + wave0 < nvec) vec(raw[j], j * NT + tid, j);
     } else {
       for (int i = tid; (i & ~63) < nvec; i += NT) vec(vector(i), i, 0);
     }
@@ -427,6 +429,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV>())) v
     return x0;
   };
   float vmax[HELD ? NV : 1];  // each vector's maximum
+#pragma unroll
+  for (float& x0 : vmax) x0 = kNegInf;
   const float single_max = fmaxf(r.single, kNegInf);  // a NaN is no maximum
   float mine = single_max;
   r.vectors([&](const float(&v)[VE], int, int j) __attribute__((always_inline)) {
