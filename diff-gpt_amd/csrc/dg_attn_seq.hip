@@ -539,6 +539,7 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   a.nq = Nq; a.nk = Nk;
   a.nsplit = 1;
   a.rows_per_wg = kTileRows;
+  a.nrb = 1;
   const int64_t blocks = counts[0] * Hkv;
   DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);

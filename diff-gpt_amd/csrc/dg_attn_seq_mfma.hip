@@ -24,6 +24,16 @@
 // do not depend on when its neighbours in the tile made it rescale.  Scores are masked
 // only in key blocks that some row of the wave sees part of; values there that are not
 // finite are kept out of the product (clean_stage).
+//
+// Bound by the softmax's vector instructions beside the matrix cores' for prompts (28 cycles
+// of a SIMD for 64 scores: fused product, exp2 at a quarter of the rate, sum, pack,
+// maximum), by HBM for few rows.  bf16: 6 sequences of up to 7168 tokens, 16 heads on 4 of
+// 128, 501 us (956 TFLOP/s); 64 of 100 - 2048, 8 heads of 64, 175 us (627 TFLOP/s); one
+// token for each of 64 caches of up to 4096, 16 heads on 4 of 128, 52 us (270 MB, 5.1 TB/s).
+// Not kept: the K fragments of a block in flight together, two chains for the row sums, 168
+// registers at head_dim 64, raised wave priority around the products (each within 2 %);
+// outputs checked for values that are not finite at the end and the piece done again (5 %
+// slower), the look at V shared between the waves (even).
 #include "dg_seq.h"
 #include "dg_prefill.h"
 
@@ -79,8 +89,9 @@ struct SeqCfg {
   // the joined states and the outputs reuse the stages: writers alternate between the two
   static_assert((((KS - 1) * RT + 1) / 2) * JOIN * 4 <= KS * 2 * TILE * ES, "joined states fit a stage");
   static_assert(ES == 4 || ((RT + 1) / 2) * 32 * D <= KS * 2 * TILE, "outputs fit a stage");
-  // workgroups a CU that the registers must allow
-  static constexpr int WGS = RT == 4 ? (ES == 4 ? (D <= 64 ? 4 : 2) : D <= 64 ? 4 : 3) : (D * ES <= 128 ? 2 : 1);
+  // workgroups a CU that the registers must allow (fp32 at head_dim 64, 64 x 512 tokens: four
+  // spill, 215 us; three 177)
+  static constexpr int WGS = RT == 4 ? (ES == 4 ? (D <= 32 ? 4 : D == 64 ? 3 : 2) : D <= 64 ? 4 : 3) : (D * ES <= 128 ? 2 : 1);
 };
 
 template <int PPR, int ES>
@@ -633,15 +644,16 @@ int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream
 // four of 32 that split them in four: the more where tiles are few, since a workgroup
 // walks its keys one stage after the other, and never fewer than fill the rows.  us with
 // 32 / 64 / 128 rows, tiles times key heads in brackets, bf16:
-//   head_dim  64: 8 x 512 tokens [256] 20.5 / 15.2 / 16.6, 16 [512] 32.5 / 21.1 / 22.3,
-//     32 [1024] 56.7 / 32.1 / 28.1; 6 x 2048 [768] 98.0 / 65.0 / 54.8; 48 chunks of up to
-//     300 behind up to 3000 keys, groups of 4 [550] 63.4 / 58.9 / 68.8
-//   head_dim 128: 1 x 3584 [224] 107 / 66.4 / 84.3, 4 x 2048 [512] 143 / 79.5 / 65.4
+//   head_dim  64: 8 x 512 tokens [256] 18.7 / 14.0 / 15.2, 16 [512] 31.6 / 19.5 / 18.2,
+//     32 [1024] 52.3 / 28.7 / 23.3; 6 x 2048 [768] 69.6 / 51.5 / 50; 48 chunks of up to
+//     300 behind up to 3000 keys, groups of 4 [436] 61 / 46.5 / 61.5, 64 [550] 72 / 61 / 59
+//   head_dim 128: 1 x 3584 in groups of 2 [448] 129 / 82 / 92, 2 x 2048 [512] 110 / 63 / 57
 int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s) {
   const int64_t tiles = counts[1] * a.Hkv;
   const int rt = counts[2] <= 32 || tiles <= 64 ? 1 : counts[2] <= 64 || tiles <= (a.D == 128 ? 384 : 640) ? 2 : 4;
   a.rows_per_wg = 32 * rt;
-  const dim3 grid((unsigned)(counts[0] * a.Hkv), (unsigned)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg));
+  a.nrb = (int)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg);
+  const dim3 grid((unsigned)(counts[0] * a.Hkv * a.nrb));
   if (rt == 1) return launch_seq_t<1, false>(a, dtype, grid, s);
   if (rt == 2) return launch_seq_t<2, false>(a, dtype, grid, s);
   return launch_seq_t<4, false>(a, dtype, grid, s);

@@ -34,7 +34,7 @@ struct SeqArgs {
   const int64_t* masks; // bit m of masks[b * mask_b + n]: token n sees token m; null: the earlier ones and itself
   int64_t mask_b;
   int rows_per_wg;  // rows of a workgroup
-  int nrb;          // row blocks of a (b, key head)
+  int nrb;          // row blocks of a (b, key head); packed: workgroups of a tile
   int nsplit;       // key splits of a row (1: y is written)
   int chunk;        // keys of a split
   // nsplit > 1: unnormalised outputs (nsplit, D) and (maximum, sum) pairs (nsplit, 2) of row
@@ -44,6 +44,7 @@ struct SeqArgs {
 };
 
 constexpr int kTileRows = 128;  // most rows of a packed tile
+constexpr unsigned kAtOnce = 1536;  // workgroups that start with the launch, about
 
 // A workgroup's piece: the rows row0 .. row0 + rows - 1 of a sequence of `nrows` rows,
 // over keys [kbeg, kend).  Query i sees key t iff t < own, or t < own + 64 and bit
@@ -84,8 +85,18 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
     p.q0 = p.k0 = 0;
     return p.kbeg < p.kend;
   } else {
+    // Position u of the XCD's workgroups: a tile's parts follow each other, they share its
+    // keys.  Where all run at once every other 32 of them, one for each CU, are taken in
+    // reverse, so that no CU gets each time the most of 32 falling numbers of keys.
+    // 48 chunks of up to 300 queries behind up to 3000 keys, fp16, head_dim 64 in groups
+    // of 4: parts apart 56 us, together 44, and reversed 43; 71 shorter ones at head_dim 128
+    // 25 / 27 / 22.  (Reversed with four times as many workgroups: 481 -> 496.)
+    unsigned u = blockIdx.x >> 3;
+    if (gridDim.x <= kAtOnce && (u & 32u) != 0 && (u | 31u) < gridDim.x >> 3) u ^= 31u;
+    const unsigned part = u % (unsigned)a.nrb;
+    u /= (unsigned)a.nrb;
     // which entry: dg_packed_plan's lists, an XCD further for each key head
-    const unsigned u = blockIdx.x >> 3, slot = u / (unsigned)a.Hkv;
+    const unsigned slot = u / (unsigned)a.Hkv;
     p.kvh = (int)(u - slot * (unsigned)a.Hkv);
     dg_packed_tile t = a.tiles[8 * (int64_t)slot + ((blockIdx.x - (unsigned)p.kvh) & 7u)];
     t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
@@ -101,8 +112,8 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
       return false;
     if (t.row0 < 0 || t.rows <= 0 || t.rows > kTileRows || (int64_t)t.row0 + t.rows > (int64_t)t.lq * a.G) return false;
     // the workgroup's part of the tile
-    t.row0 += blockIdx.y * a.rows_per_wg;
-    t.rows = min(a.rows_per_wg, t.rows - (int)blockIdx.y * a.rows_per_wg);
+    t.row0 += (int)part * a.rows_per_wg;
+    t.rows = min(a.rows_per_wg, t.rows - (int)part * a.rows_per_wg);
     if (t.rows <= 0) return false;
     p.row0 = t.row0;
     p.rows = t.rows;
