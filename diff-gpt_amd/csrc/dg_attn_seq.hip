@@ -342,7 +342,8 @@ constexpr int kVecRows = 32;    // rows of a workgroup of the vector kernel over
 // Splits of a row: enough workgroups to fill the CUs as far as their LDS and registers let
 // them share one (256 of 128 KB, as many more as smaller ones fit), and at least so many
 // stages each that joining the splits, a launch of its own of some 6 us, costs no more than
-// it saves: 8, fewer where fp32 products make a stage long.  us at 256 / 512 / 1024
+// it saves: 8, one where fp32 products make a stage long (16 rows of the batch, 31 tokens
+// behind up to 600 keys, 4 heads of 64: 20 us with 4, 15 with 1).  us at 256 / 512 / 1024
 // workgroups, bf16:
 //   rows of 32, head_dim 128 (64 rows, 4 key heads, lengths to 4096)    52.1 / 58.6 / 68.3
 //               head_dim  64 (64 rows, 8 key heads, lengths to 1024)    17.2 / 17.0 / 25.3
@@ -355,7 +356,7 @@ int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int rows_per_wg, int D, in
   const int stage = rows_per_wg == 32 ? 128 : 64;  // keys; the vector kernel has no stages
   const int64_t row_bytes = D * dtype_bytes(dtype);
   const int64_t fill = rows_per_wg == 32 ? (row_bytes >= 256 ? 256 : 512) : rows_per_wg == 64 ? 512 : D == 128 ? 768 : 1024;
-  const int64_t least = dtype == DG_F32 ? std::max(2, std::min(8, 256 / D)) : 8;
+  const int64_t least = dtype == DG_F32 && D >= 64 ? 1 : 8;
   const int64_t wg = B * Hkv * nrb;
   const int64_t want = (fill + wg - 1) / wg;
   int64_t chunk = std::max<int64_t>((keys + want - 1) / want, (keys + kMaxSplits - 1) / kMaxSplits);
@@ -582,7 +583,7 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   a.len = len; a.lens = lens;
   a.masks = masks; a.mask_b = mask_b;
   const bool mfma = seq_mfma_applicable(a, dtype, true);
-  const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, mfma ? seq_mfma_tree_rows(N * a.G) : kVecRows);
+  const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, mfma ? seq_mfma_tree_rows(B, N * a.G, Hkv, Tcap, D, dtype) : kVecRows);
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
   if (t.nsplit > 1) {
     DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,

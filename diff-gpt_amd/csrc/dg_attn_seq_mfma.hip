@@ -592,6 +592,9 @@ void seq_mfma_kernel(const SeqArgs a) {
 
 namespace {
 
+// Rows of a tree's workgroup, 32 RT, that seq_mfma_tree_rows chooses from.
+constexpr bool tree_has_shape(int D, int RT, bool f32) { return RT == 1 || (f32 ? RT == 2 && D == 128 : D >= 64); }
+
 template <typename T, int D, int RT, bool TREE>
 int launch_seq(const SeqArgs& a, dim3 grid, hipStream_t s) {
   hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, TREE>), grid, dim3(64 * SeqCfg<T, D, RT>::WAVES), 0, s, a);
@@ -601,10 +604,16 @@ int launch_seq(const SeqArgs& a, dim3 grid, hipStream_t s) {
 
 template <typename T, int RT, bool TREE>
 int launch_seq_d(const SeqArgs& a, dim3 grid, hipStream_t s) {
-  if (a.D == 16) return launch_seq<T, 16, RT, TREE>(a, grid, s);
-  if (a.D == 32) return launch_seq<T, 32, RT, TREE>(a, grid, s);
-  if (a.D == 64) return launch_seq<T, 64, RT, TREE>(a, grid, s);
-  return launch_seq<T, 128, RT, TREE>(a, grid, s);
+  constexpr bool kF32 = sizeof(T) == 4;
+#define DG_SEQ_D(DIM)                                  \
+  if constexpr (!TREE || tree_has_shape(DIM, RT, kF32)) \
+    if (a.D == DIM) return launch_seq<T, DIM, RT, TREE>(a, grid, s)
+  DG_SEQ_D(16);
+  DG_SEQ_D(32);
+  DG_SEQ_D(64);
+  DG_SEQ_D(128);
+#undef DG_SEQ_D
+  return DG_EUNSUPPORTED;
 }
 
 template <int RT, bool TREE>
@@ -630,8 +639,25 @@ bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree) {
          rows(a.y, a.yb, a.yt, a.yh);
 }
 
-// Rows of a workgroup: 32, 64 or 128, the smallest that holds a row's (token, head) rows.
-int seq_mfma_tree_rows(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Rows of a tree's workgroup.  32 (the waves split the keys) spread a row's keys over the
+// most waves; 64 and 128 read them fewer times.  us with 32 / 64 / 128 rows, "rows of the
+// batch x (token, head) rows", lengths up to, key heads:
+//   head_dim <= 32, every one tried:  bf16 16 x 60, 600, 4: 11 / 18 / 18; fp32 32 x 60,
+//     2000, 4: 29.9 / 30.6 / 30.8; 64 x 64, 4000, 8: 113 / 147 / 147
+//   fp32 head_dim 64: 3 x 152, 140, 1: 11.8 / 14.2 / 18; 64 x 256, 3000, 4: 288 / 294 / 417
+//     head_dim 128: 32 x 48, 2000, 4: 148 / 105 / 105; 2 x 256, 20000, 2: 188 / 118 / 137
+//   16-bit, few keys in all: head_dim 64 16 x 60, 600, 4: 9.5 / 15.3 / 15.5, head_dim 128
+//     4 x 152, 1500, 4: 18 / 19 / 24, 32 x 96, 2000, 4: 35 / 38 / 40; many: head_dim 64
+//     4 x 128, 70000, 8: 177 / 155 / 131, head_dim 128 16 x 96, 7168, 4: 57 / 46 / 43
+//   64 rows fill the chip, no splits: 64 x 256, 4000, 4: head_dim 64 86 / 74 / 102,
+//     head_dim 128 180 / 136 / 163
+int seq_mfma_tree_rows(int64_t B, int rows, int Hkv, int keys, int D, int dtype) {
+  if (rows <= 32 || D <= 32) return 32;
+  if (dtype == DG_F32) return D == 64 ? 32 : 64;
+  const int64_t tiles = B * Hkv * ((rows + 127) / 128);
+  if (tiles * keys <= 300000) return 32;
+  return rows <= 64 || tiles >= 256 ? 64 : 128;
+}
 
 int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s) {
   const dim3 grid(blocks);

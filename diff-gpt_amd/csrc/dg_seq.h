@@ -137,7 +137,7 @@ __device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n
 // dg_attn_seq_mfma.hip: whether it takes the shape, the rows of a workgroup over so many
 // (token, head) rows, and its launches
 bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree);
-int seq_mfma_tree_rows(int rows);
+int seq_mfma_tree_rows(int64_t B, int rows, int Hkv, int keys, int D, int dtype);
 int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s);
 int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s);
 

@@ -243,8 +243,22 @@ def test_tree_matches_float64(dev, dtype, H, Hkv, D, N, lens, Tcap):
     q, k, v = _tree_case(dev, len(lens), N, H, Hkv, Tcap, D, TDT[dtype], seed=N + D)
     parents = some_tree(N, seed=N)
     y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
-    rows = N * (H // Hkv)
-    assert _native.last_kernel() in (f"seq_mfma_tree_{32 if rows <= 32 else 64 if rows <= 64 else 128}", "seq_join_kernel")
+    assert _native.last_kernel() in ("seq_mfma_tree_32", "seq_mfma_tree_64", "seq_join_kernel")
+    _check_tree(q, k, v, y, lens, parents, dtype)
+
+
+@pytest.mark.parametrize("dtype,D,B,N,Hkv,G,Tcap,rows", [
+    ("f32", 16, 2, 60, 1, 3, 70, 32), ("bf16", 32, 3, 40, 2, 2, 300, 32), ("f32", 64, 2, 50, 1, 3, 90, 32),
+    ("f32", 128, 2, 50, 2, 3, 100, 64), ("f32", 128, 60, 64, 4, 1, 100, 64), ("bf16", 64, 3, 41, 2, 4, 1000, 32),
+    ("f16", 128, 3, 64, 2, 1, 900, 32), ("bf16", 64, 65, 33, 4, 1, 1300, 64), ("f16", 64, 40, 64, 4, 3, 700, 32), ("f16", 64, 40, 64, 4, 3, 1000, 64),
+    ("bf16", 128, 64, 50, 4, 3, 700, 64), ("f16", 128, 128, 45, 1, 2, 2500, 128), ("bf16", 64, 250, 37, 1, 3, 1300, 128)])
+def test_tree_in_every_workgroup_shape(dev, dtype, D, B, N, Hkv, G, Tcap, rows):
+    """32, 64 and 128 rows a workgroup, where one takes all of a row's keys."""
+    lens = [(131 * (b + 1)) % (Tcap - N + 1) for b in range(B)]
+    q, k, v = _tree_case(dev, B, N, Hkv * G, Hkv, Tcap, D, TDT[dtype], seed=B)
+    parents = some_tree(N, seed=B)
+    y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+    assert _native.last_kernel() in (f"seq_mfma_tree_{rows}", "seq_join_kernel")
     _check_tree(q, k, v, y, lens, parents, dtype)
 
 
