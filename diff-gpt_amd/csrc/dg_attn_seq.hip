@@ -488,8 +488,8 @@ extern "C" int dg_packed_plan(int64_t S, const int64_t* lq, const int64_t* lk, i
   int64_t nq = 0, nk = 0, n = 0;
   for (int64_t s = 0; s < S; ++s) {
     DG_REQUIRE(lq[s] >= 0 && lk[s] >= 0, DG_EINVAL, "packed_plan: sequence %lld has a negative length", (long long)s);
-    DG_REQUIRE(lq[s] <= 0x7fffffff / group, DG_EINVAL, "packed_plan: sequence %lld has too many rows", (long long)s);
-    DG_REQUIRE(lk[s] <= 0x7fffffff, DG_EINVAL, "packed_plan: sequence %lld has too many keys", (long long)s);
+    DG_REQUIRE(lq[s] <= kMostPositions / group, DG_EINVAL, "packed_plan: sequence %lld has more than 2^30 rows", (long long)s);
+    DG_REQUIRE(lk[s] <= kMostPositions, DG_EINVAL, "packed_plan: sequence %lld has more than 2^30 keys", (long long)s);
     nq += lq[s];
     nk += lk[s];
     DG_REQUIRE(nq <= 0x7fffffff && nk <= 0x7fffffff, DG_EINVAL, "packed_plan: more than 2^31 - 1 rows");
@@ -549,7 +549,7 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
 }
 
 extern "C" size_t dg_attention_tree_workspace_size(int B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
-  if (B <= 0 || N <= 0 || N > 64 || H <= 0 || Hkv <= 0 || H % Hkv || Tcap < N || D <= 0) return 0;
+  if (B <= 0 || N <= 0 || N > 64 || H <= 0 || Hkv <= 0 || H % Hkv || Tcap < N || Tcap > kMostPositions || D <= 0) return 0;
   return tree_workspace(B, N, H, Hkv, Tcap, D, dtype);
 }
 
@@ -563,6 +563,7 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "attention_tree: head_dim %d outside [1, %d]", D, kMaxHeadDim);
   DG_REQUIRE(N >= 1 && N <= 64, DG_EINVAL, "attention_tree: %d tokens a row, 1 to 64", N);
   DG_REQUIRE(Tcap >= N, DG_EINVAL, "attention_tree: the cache holds %d positions, %d tokens", Tcap, N);
+  DG_REQUIRE(Tcap <= kMostPositions, DG_EINVAL, "attention_tree: a cache of more than 2^30 positions");
   DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "attention_tree: %d query heads on %d key heads", H, Hkv);
   DG_REQUIRE(H / Hkv <= 0x7fffff, DG_EINVAL, "attention_tree: %d heads a group", H / Hkv);
   DG_REQUIRE(scale > 0.f && std::isfinite(scale), DG_EINVAL, "attention_tree: the scale must be positive");

@@ -44,6 +44,8 @@ struct SeqArgs {
 };
 
 constexpr int kTileRows = 128;  // most rows of a packed tile
+// most rows, and keys, of a sequence: positions a stage further on stay within 32 bits
+constexpr int64_t kMostPositions = (int64_t)1 << 30;
 constexpr unsigned kAtOnce = 1536;  // workgroups that start with the launch, about
 
 // A workgroup's piece: the rows row0 .. row0 + rows - 1 of a sequence of `nrows` rows,

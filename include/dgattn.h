@@ -592,7 +592,7 @@ DG_API int dg_draw_argmax(int64_t M, int V, int dtype, const void* probs, int64_
  * over such a batch.  A tile that does not lie inside Nq and Nk rows is skipped, never
  * followed.
  * fp32 / bf16 / fp16 / fp64, every head_dim up to 1024, rows with unit stride over d; the
- * scale is positive.
+ * scale is positive.  A sequence has at most 2^30 keys and (query, head of the group) rows.
  */
 typedef struct dg_packed_tile {
   int32_t q0, lq, k0, lk; /* the sequence's rows of q and of k */
@@ -620,7 +620,7 @@ DG_API int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D, in
  * of masks[b * mask_b + n] (int64 on the device; mask_b 0: one tree for all rows) is set;
  * masks NULL: token n sees tokens 0 .. n.  A token that sees nothing gets zeros.  What
  * positions hidden from a token hold, NaN and infinities included, does not reach it.
- * 1 <= N <= 64, Tcap >= N.  Long rows are split over workgroups whose partial results meet
+ * 1 <= N <= 64, N <= Tcap <= 2^30.  Long rows are split over workgroups whose partial results meet
  * in the caller's workspace (dg_attention_tree_workspace_size bytes, 16-byte aligned; its
  * contents need no initialisation, and calls that may overlap need one each).
  * Types, head_dim and scale as dg_attention_packed.

@@ -54,6 +54,9 @@ def test_plan_refusals():
     assert plan([1], [1], group=0) == -1
     assert plan([2**31], [1]) == -1
     assert plan([2**30, 2**30], [1, 1]) == -1 and b"2^31" in _native.lib().dg_last_error()
+    assert plan([2**30 + 1], [1]) == -1 and plan([2**29], [1], group=4) == -1
+    assert plan([1], [2**30]) == 0
+    assert plan([1], [2**30 + 1]) == -1 and b"2^30" in _native.lib().dg_last_error()
     assert plan([1000], [1000], cap=1, tiles=FAKE) == -1 and b"room" in _native.lib().dg_last_error()
 
 
@@ -128,7 +131,7 @@ def test_packed_refusals(kw, rc):
 @pytest.mark.parametrize("kw,rc", [(dict(B=-1), -1), (dict(dtype=9), -2), (dict(D=0), -2), (dict(D=1025), -2),
                                    (dict(N=0), -1), (dict(N=65, Tcap=100), -1), (dict(Tcap=1), -1), (dict(H=3, Hkv=2), -1),
                                    (dict(scale=-1.0), -1), (dict(length=-1), -1), (dict(length=7), -1), (dict(p=NUL), -1),
-                                   (dict(B=0), 0), (dict(H=0), 0),
+                                   (dict(B=0), 0), (dict(H=0), 0), (dict(Tcap=2**30 + 1), -1), (dict(Tcap=2**30), -4),
                                    (dict(Tcap=5000), -4), (dict(Tcap=5000, ws=FAKE, ws_bytes=16), -4)])
 def test_tree_entry_refusals(kw, rc):
     assert _tree(**kw) == rc
@@ -140,6 +143,7 @@ def test_tree_workspace_size():
     assert size(1, 1, 4, 4, 100000, 16, 0) > 0
     assert size(1, 65, 4, 4, 100000, 16, 0) == 0 and size(0, 1, 4, 4, 100000, 16, 0) == 0
     assert size(1, 1, 4, 3, 100000, 16, 0) == 0
+    assert size(1, 1, 4, 4, 2**30, 16, 0) > 0 and size(1, 1, 4, 4, 2**30 + 1, 16, 0) == 0
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(M=-1), -1), (dict(V=0), -1), (dict(dtype=9), -2), (dict(top=-1), -1),
