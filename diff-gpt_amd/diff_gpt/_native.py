@@ -829,6 +829,10 @@ def attention_packed_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, y: torc
     yt, yh, yd = y.stride()
     if not (qd == kd == vd == yd == 1) and D > 1:
         raise ValueError("attention_packed: the last (head_dim) dimension must be contiguous")
+    if torch._C._cuda_getCurrentRawStream(device) != layout.stream and not torch.cuda.is_current_stream_capturing():
+        # the table's memory must not be given away before this stream has read it (a graph
+        # replays as long as its caller keeps the layout)
+        layout.tiles.record_stream(torch.cuda.current_stream(device))
     _launch("attention_packed", device, lib().dg_attention_packed, Nq, Nk, H, Hkv, D, _DTYPE_CODE[q.dtype],
             q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, y.data_ptr(), yt, yh,
             _check_scale("attention_packed", scale), layout.tiles.data_ptr(), layout.counts)

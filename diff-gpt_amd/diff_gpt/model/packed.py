@@ -21,7 +21,7 @@ class PackedLayout:
     queries the first keys are cached ones, with fewer the first queries see nothing.
     group: query heads per key head of the tensors the layout is for."""
 
-    __slots__ = ("q_lengths", "k_lengths", "group", "total_q", "total_k", "tiles", "counts")
+    __slots__ = ("q_lengths", "k_lengths", "group", "total_q", "total_k", "tiles", "counts", "stream")
 
     def __init__(self, q_lengths: Sequence[int], k_lengths: Sequence[int] | None = None, group: int = 1,
                  device: torch.device | str = "cuda") -> None:
@@ -38,6 +38,7 @@ class PackedLayout:
         self.total_q, self.total_k = sum(self.q_lengths), sum(self.k_lengths)
         tiles, self.counts = _native.packed_plan(self.q_lengths, self.k_lengths, self.group)
         self.tiles = tiles.to(device)
+        self.stream = torch._C._cuda_getCurrentRawStream(self.tiles.get_device())  # whose memory the table is
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: PackedLayout,

@@ -195,6 +195,25 @@ def test_packed_agrees_with_the_framework_attention(dev):
     assert float((y.view_as(ref) - ref).abs().max()) <= 2e-5 * float(ref.abs().max())
 
 
+def test_packed_layout_outlives_another_streams_call(dev):
+    """A layout dropped while a call on a stream of its own still waits: its memory is not
+    handed on before that call has read it."""
+    q, k, v = _packed_case(dev, [700, 300], [700, 300], 2, 2, 64, torch.bfloat16)
+    want = attention_packed(q, k, v, PackedLayout([700, 300]))
+    torch.cuda.synchronize()
+    lay = PackedLayout([700, 300])
+    shape, at = lay.tiles.shape, lay.tiles.data_ptr()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(40_000_000)
+        y = attention_packed(q, k, v, lay)
+    del lay
+    other = [torch.zeros(shape, dtype=torch.int32, device=dev) for _ in range(4)]
+    assert at not in [t.data_ptr() for t in other]
+    side.synchronize()
+    assert torch.equal(y, want)
+
+
 def test_packed_refusals(dev):
     q, k, v = _packed_case(dev, [8], [8], 4, 2, 64, torch.bfloat16)
     lay = PackedLayout([8], group=2)
@@ -402,6 +421,31 @@ def test_tree_past_32_bit_offsets(dev):
     y2 = attention_packed(q.view(4, 4, D), flat[:, 7:8], flat[:, 33:34],
                           PackedLayout([2, 2], [150000, 150000], group=4))
     assert torch.equal(y, y2)
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Split trees and packed batches on two streams, each call with a workspace of its own
+    and both with one layout: the bits of calls one after the other."""
+    lens = torch.tensor([3000, 17, 2100], dtype=torch.int32, device=dev)
+    trees = [_tree_case(dev, 3, 12, 8, 2, 3100, 64, torch.bfloat16, seed=s) for s in range(2)]
+    masks = [tree_masks(some_tree(12, seed=s)) for s in range(2)]
+    lay = PackedLayout([500, 30, 200], group=3)
+    packed = [_packed_case(dev, [500, 30, 200], [500, 30, 200], 6, 2, 64, torch.bfloat16, seed=s) for s in range(2)]
+
+    def run(s):
+        return attention_tree(*trees[s], lens, masks[s]), attention_packed(*packed[s], lay)
+
+    want = [run(s) for s in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                got[s].append(run(s))
+    torch.cuda.synchronize()
+    for s in range(2):
+        for a, b in got[s]:
+            assert torch.equal(a, want[s][0]) and torch.equal(b, want[s][1])
 
 
 def test_tree_refusals(dev):
