@@ -3,18 +3,24 @@
 // of split rows, and the kernel that takes any shape and type.  head_dim 16, 32, 64 and
 // 128 in 16-bit types and fp32 run on the matrix cores (dg_attn_seq_mfma.hip).
 //
-// The kernel here: a wavefront takes one (query, head) row at a time.  Its 64 lanes are
-// 64 / LPK groups of LPK lanes; a group takes every (64 / LPK)-th key of the range, lane d
-// of it the elements d, d + LPK, ... of the key and of the value (consecutive lanes read
-// consecutive elements at any alignment).  Every group keeps a running maximum, sum and
-// output of its own, in fp32 (fp64 for fp64 data); the groups meet once, at the end.  A
-// hidden key is skipped outright, so nothing it holds can reach a row.  Bound by the
-// vector ALU's cross-lane sums: log2(LPK) exchanges for every key and row.
+// The kernel here (seq_tile_kernel): 32 rows of a key head by 32 keys at a time, 16 rows
+// for head_dim over 256 and 8 where a piece has no more (a decode step): 8, 16 or 32 lanes
+// a row, in fp32 (fp64 for fp64 data).  Rows lie in LDS for the whole loop; keys and then
+// values pass through it in chunks of 64 dims, read element by element (rows may start
+// anywhere) into registers while the chunk before is computed.  For the scores a row's
+// lanes have a key each, for the outputs dims each; the probabilities go from one to the
+// other through LDS.  A hidden key's score is taken out by selection and its values are
+// skipped, so nothing it holds can reach a row.  Bound by LDS reads (five of 16 bytes for
+// 16 products a lane).  16 x 512 tokens, 8 heads: head_dim 80 bf16 385 us, 96 fp32 358 (18
+// TFLOP/s), 256 bf16 1000, 64 fp64 366; a step over 32 caches of 1900, 8 heads: 80 bf16
+// 118 us, 256 bf16 216, 64 fp64 124 (4.0 TB/s).  One row a wave at a time with a running
+// softmax in each lane group took 14.9 ms, 17.4, 31.3, 13.1 and 1.2 ms, 6.1, 2.2.
 #include "dg_seq.h"
 
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <type_traits>
 #include <vector>
 
 namespace dg {
@@ -57,88 +63,203 @@ __device__ __forceinline__ void join_softmax(A& m, A& l, A m2, A l2, A& f1, A& f
   m = mn;
 }
 
-template <typename T, int LPK, int CPL, bool TREE>
-__global__ __launch_bounds__(256) void seq_vec_kernel(const SeqArgs a) {
+// N consecutive values in LDS, aligned to their size or to 16 bytes.
+template <int N, typename A>
+__device__ __forceinline__ void lds_load(const A* p, A (&x)[N]) {
+  constexpr int V = N * sizeof(A) > 16 ? 16 / sizeof(A) : N;
+  typedef A vec __attribute__((ext_vector_type(V)));
+#pragma unroll
+  for (int e = 0; e < N; e += V) {
+    const vec v = *reinterpret_cast<const vec*>(p + e);
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[e + k] = v[k];
+  }
+}
+
+// NCH: chunks of 64 dims there may be; LPR: lanes of a row.
+template <typename T, int NCH, int LPR, bool TREE>
+__global__ __launch_bounds__(256) void seq_tile_kernel(const SeqArgs a) {
   using S = SeqAcc<T>;
   using A = typename S::type;
-  constexpr int KPW = 64 / LPK;
+  constexpr int ROWS = 256 / LPR, KT = 32, KPL = KT / LPR;
+  constexpr int VW = LPR == 32 ? 2 : 4, NV = 64 / LPR / VW;  // of a chunk, a lane has dims VW (ln + LPR h) + e
+  constexpr int PAD = 16 / (int)sizeof(A);  // rows 4 banks apart
+  constexpr int QS = NCH * 64 + PAD, CS = 64 + PAD, PS = KT + PAD;
+  __shared__ __attribute__((aligned(16))) A qs[ROWS * QS], kvs[KT * CS], ps[ROWS * PS];
   SeqPiece p;
-  if (!seq_piece<TREE>(a, p)) return;
-  const int lane = threadIdx.x & 63, kl = lane / LPK, dl = lane % LPK;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (!seq_piece<TREE>(a, p)) return;  // whole workgroups
+  const int tid = threadIdx.x, row = tid / LPR, ln = tid % LPR;
+  const bool live = (tid & ~63) / LPR < p.rows;  // the wave has a row
+  const int last = p.row0 + p.rows - 1;          // rows past it repeat it and are never stored
+  const int r = min(p.row0 + row, last), i = r / a.G;
+  const A us = S::unit_scale(a);
+  for (int e = tid; e < ROWS * NCH * 64; e += 256) {
+    const int er = e / (NCH * 64), d = e % (NCH * 64), rr = min(p.row0 + er, last), ri = rr / a.G;
+    const T* qp = static_cast<const T*>(a.q) + p.b * a.qb + (p.q0 + ri) * a.qt + (int64_t)(p.kvh * a.G + rr - ri * a.G) * a.qh;
+    qs[er * QS + d] = d < a.D ? S::load(qp[d]) : (A)0;
+  }
   const T* kp = static_cast<const T*>(a.k) + p.b * a.kb + p.k0 * a.kt + (int64_t)p.kvh * a.kh;
   const T* vp = static_cast<const T*>(a.v) + p.b * a.vb + p.k0 * a.vt + (int64_t)p.kvh * a.vh;
-  const A us = S::unit_scale(a);
-  for (int r = p.row0 + wv; r < p.row0 + p.rows; r += 4) {
-    const int i = r / a.G, h = p.kvh * a.G + r % a.G;
-    const T* qp = static_cast<const T*>(a.q) + p.b * a.qb + (p.q0 + i) * a.qt + (int64_t)h * a.qh;
-    A q[CPL], o[CPL];
+  // Keys t0 .. of one chunk of dims: into registers, a step ahead of their use, and from
+  // there into LDS.  Past the piece's keys the last one stands, hidden from every row; past
+  // the head zeros.
+  const int sd = tid & 63, sk = tid >> 6;
+  T w[KT / 4];
+  auto fetch = [&](const T* x, int64_t step, int t0, int c) __attribute__((always_inline)) {
+    const T* xd = x + min(64 * c + sd, a.D - 1);
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      q[c] = dl + LPK * c < a.D ? S::load(qp[dl + LPK * c]) : (A)0;
-      o[c] = (A)0;
-    }
-    uint64_t mask = 0;
-    int end = p.kend;
-    if constexpr (TREE) mask = tree_mask(a, p.b, i);
-    else end = i + p.off + 1;
-    A m = neg_inf<A>(), l = (A)0;
-    for (int t0 = p.kbeg; t0 < end; t0 += KPW) {
-      const int t = t0 + kl;
-      bool seen = t < end;
-      if (TREE && t >= p.own) seen = seen && ((mask >> ((t - p.own) & 63)) & 1);
-      const int64_t tt = min(t, end - 1);  // lanes past the end re-read the last key
-      A d = (A)0;
+    for (int n = 0; n < KT / 4; ++n) w[n] = xd[min(t0 + sk + 4 * n, p.kend - 1) * step];
+  };
+  auto put = [&](int c) __attribute__((always_inline)) {
+    const bool in = 64 * c + sd < a.D;
 #pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (dl + LPK * c < a.D) d += q[c] * S::load(kp[tt * a.kt + dl + LPK * c]);
+    for (int n = 0; n < KT / 4; ++n) kvs[(sk + 4 * n) * CS + sd] = in ? S::load(w[n]) : (A)0;
+  };
+  const int nch = (a.D + 63) / 64;
+  uint64_t mask = 0;
+  int end = p.kend, first_open = p.own;
+  if constexpr (TREE) {
+    mask = tree_mask(a, p.b, i);
+  } else {
+    end = i + p.off + 1;
+    first_open = p.row0 / a.G + p.off + 1;
+  }
+  A o[NCH][NV][VW], m = neg_inf<A>(), l = (A)0;
 #pragma unroll
-      for (int x = 1; x < LPK; x <<= 1) d += __shfl_xor(d, x, 64);
-      d = d * us;
-      if (!seen) continue;
-      const A mn = d > m || d != d ? d : m;  // a NaN score makes the row NaN
-      const A f = m == neg_inf<A>() ? (A)0 : S::exp(m - mn);
-      const A w = mn == neg_inf<A>() ? (A)0 : S::exp(d - mn);
-      m = mn;
-      l = l * f + w;
+  for (int c = 0; c < NCH; ++c)
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        if (dl + LPK * c < a.D) o[c] = o[c] * f + w * S::load(vp[tt * a.vt + dl + LPK * c]);
+    for (int h = 0; h < NV; ++h)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) o[c][h][e] = (A)0;
+
+  if (p.kbeg < p.kend) fetch(kp, a.kt, p.kbeg, 0);
+  for (int t0 = p.kbeg; t0 < p.kend; t0 += KT) {
+    A s[KPL];
+#pragma unroll
+    for (int j = 0; j < KPL; ++j) s[j] = (A)0;
+#pragma unroll 1
+    for (int c = 0; c < nch; ++c) {
+      __syncthreads();
+      put(c);
+      __syncthreads();
+      if (c + 1 < nch) fetch(kp, a.kt, t0, c + 1);
+      else fetch(vp, a.vt, t0, 0);
+      if (live) {
+#pragma unroll 4
+        for (int d = 0; d < 64; d += 4) {
+          A q4[4];
+          lds_load(qs + row * QS + 64 * c + d, q4);
+#pragma unroll
+          for (int j = 0; j < KPL; ++j) {
+            A k4[4];
+            lds_load(kvs + (ln + LPR * j) * CS + d, k4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j] += q4[e] * k4[e];
+          }
+        }
       }
     }
+    bool seen[KPL];
+    A top = neg_inf<A>();
 #pragma unroll
-    for (int x = LPK; x < 64; x <<= 1) {
-      const A m2 = __shfl_xor(m, x, 64), l2 = __shfl_xor(l, x, 64);
-      A f1, f2;
-      join_softmax<S, A>(m, l, m2, l2, f1, f2);
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        const A o2 = __shfl_xor(o[c], x, 64);
-        // a group without a key has no output: 0 * NaN stays out
-        o[c] = (f1 == (A)0 ? (A)0 : o[c] * f1) + (f2 == (A)0 ? (A)0 : o2 * f2);
-      }
+    for (int j = 0; j < KPL; ++j) {
+      const int t = t0 + ln + LPR * j;
+      seen[j] = t < end;
+      if constexpr (TREE) seen[j] = seen[j] && (t < p.own || ((mask >> ((t - p.own) & 63)) & 1));
+      s[j] = seen[j] ? s[j] * us : neg_inf<A>();
+      top = s[j] > top ? s[j] : top;
     }
-    if (kl != 0) continue;
-    if (TREE && a.nsplit > 1) {
-      const int64_t part = ((p.b * a.Hkv + p.kvh) * (int64_t)(a.N * a.G) + r) * a.nsplit + p.split;
-      A* wo = static_cast<A*>(a.ws_o) + part * a.D;
 #pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (dl + LPK * c < a.D) wo[dl + LPK * c] = o[c];
-      if (dl == 0) {
-        A* ml = static_cast<A*>(a.ws_ml) + 2 * part;
-        ml[0] = m;
-        ml[1] = l;
-      }
-    } else {
-      // no key at all: zeros; keys whose scores are all -inf: 0 / 0, as a softmax gives
-      const bool none = TREE ? p.own == 0 && mask == 0 : end <= 0;
-      T* yp = static_cast<T*>(a.y) + p.b * a.yb + (p.q0 + i) * a.yt + (int64_t)h * a.yh;
+    for (int x = 1; x < LPR; x <<= 1) {
+      const A other = __shfl_xor(top, x, 64);
+      top = other > top ? other : top;
+    }
+    const A mn = top > m ? top : m;
+    const A f = m == neg_inf<A>() ? (A)1 : S::exp(m - mn);  // nothing to rescale yet
+    const A base = mn == neg_inf<A>() ? (A)0 : mn;
+    m = mn;
+    l *= f;
 #pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (dl + LPK * c < a.D) yp[dl + LPK * c] = S::store(none ? (A)0 : o[c] / l);
+    for (int j = 0; j < KPL; ++j) {
+      const A w = S::exp(s[j] - base);  // NaN for a NaN score, and the row with it
+      if (seen[j]) l += w;
+      ps[row * PS + ln + LPR * j] = seen[j] ? w : (A)-1;  // the row's own lanes read it, after the barriers below
+    }
+    if (f != (A)1) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c)
+#pragma unroll
+        for (int h = 0; h < NV; ++h)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) o[c][h][e] *= f;
+    }
+    const bool open = t0 + KT <= first_open;  // every row sees every key of the tile
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if (c >= nch) break;
+      __syncthreads();
+      put(c);
+      __syncthreads();
+      if (c + 1 < nch) fetch(vp, a.vt, t0, c + 1);
+      else fetch(kp, a.kt, t0 + KT, 0);
+      if (!live) continue;
+      auto add = [&](auto every) __attribute__((always_inline)) {
+#pragma unroll 2
+        for (int t = 0; t < KT; t += 4) {
+          A w4[4];
+          lds_load(ps + row * PS + t, w4);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int h = 0; h < NV; ++h) {
+              A v[VW];
+              lds_load(kvs + (t + u) * CS + VW * (ln + LPR * h), v);
+#pragma unroll
+              for (int e = 0; e < VW; ++e) {
+                const A x = o[c][h][e] + w4[u] * v[e];
+                o[c][h][e] = every.value || !(w4[u] < (A)0) ? x : o[c][h][e];  // a hidden key adds nothing
+              }
+            }
+        }
+      };
+      if (open) add(std::true_type{});
+      else add(std::false_type{});
     }
   }
+#pragma unroll
+  for (int x = 1; x < LPR; x <<= 1) l += __shfl_xor(l, x, 64);
+  if (row >= p.rows) return;
+  if (TREE && a.nsplit > 1) {
+    const int64_t part = ((p.b * a.Hkv + p.kvh) * (int64_t)(a.N * a.G) + r) * a.nsplit + p.split;
+    A* wo = static_cast<A*>(a.ws_o) + part * a.D;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int h = 0; h < NV; ++h)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          const int d = 64 * c + VW * (ln + LPR * h) + e;
+          if (d < a.D) wo[d] = o[c][h][e];
+        }
+    if (ln == 0) {
+      A* ml = static_cast<A*>(a.ws_ml) + 2 * part;
+      ml[0] = m;
+      ml[1] = l;
+    }
+    return;
+  }
+  // no key at all: zeros; keys whose scores are all -inf: 0 / 0, as a softmax gives
+  const bool none = TREE ? p.own == 0 && mask == 0 : end <= 0;
+  T* yp = static_cast<T*>(a.y) + p.b * a.yb + (p.q0 + i) * a.yt + (int64_t)(p.kvh * a.G + r - i * a.G) * a.yh;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c)
+#pragma unroll
+    for (int h = 0; h < NV; ++h)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        const int d = 64 * c + VW * (ln + LPR * h) + e;
+        if (d < a.D) yp[d] = S::store(none ? (A)0 : o[c][h][e] / l);
+      }
 }
 
 // The splits of a row joined: WPR wavefronts a row, each over every WPR-th split, lanes
@@ -315,35 +436,41 @@ void launch_join4(const SeqArgs& a, dim3 grid, int64_t rows, hipStream_t s) {
 }
 
 template <typename T, bool TREE>
-int launch_vec(const SeqArgs& a, dim3 grid, hipStream_t s) {
-#define DG_SEQ_VEC(LPK, CPL) hipLaunchKernelGGL((seq_vec_kernel<T, LPK, CPL, TREE>), grid, dim3(256), 0, s, a)
-  if (a.D <= 8) DG_SEQ_VEC(8, 1);
-  else if (a.D <= 16) DG_SEQ_VEC(16, 1);
-  else if (a.D <= 32) DG_SEQ_VEC(32, 1);
-  else if (a.D <= 64) DG_SEQ_VEC(64, 1);
-  else if (a.D <= 128) DG_SEQ_VEC(64, 2);
-  else if (a.D <= 256) DG_SEQ_VEC(64, 4);
-  else if (a.D <= 512) DG_SEQ_VEC(64, 8);
-  else DG_SEQ_VEC(64, 16);
-#undef DG_SEQ_VEC
-  return check_launch("seq_vec_kernel");
+int launch_tile(const SeqArgs& a, dim3 grid, hipStream_t s) {
+#define DG_SEQ_TILE(NCH, LPR) hipLaunchKernelGGL((seq_tile_kernel<T, NCH, LPR, TREE>), grid, dim3(256), 0, s, a)
+  if (a.rows_per_wg == 32) {
+    if (a.D <= 64) DG_SEQ_TILE(1, 8);
+    else if (a.D <= 128) DG_SEQ_TILE(2, 8);
+    else DG_SEQ_TILE(4, 8);
+  } else if (a.rows_per_wg == 16) {
+    DG_SEQ_TILE(16, 16);
+  } else {
+    if (a.D <= 128) DG_SEQ_TILE(2, 32);
+    else if (a.D <= 256) DG_SEQ_TILE(4, 32);
+    else DG_SEQ_TILE(16, 32);
+  }
+#undef DG_SEQ_TILE
+  return check_launch("seq_tile_kernel");
 }
 
 template <bool TREE>
-int launch_vec_any(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
-  if (dtype == DG_F64) return launch_vec<double, TREE>(a, grid, s);
-  if (dtype == DG_F32) return launch_vec<float, TREE>(a, grid, s);
-  if (dtype == DG_BF16) return launch_vec<bf16_t, TREE>(a, grid, s);
-  return launch_vec<f16_t, TREE>(a, grid, s);
+int launch_tile_any(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
+  if (dtype == DG_F64) return launch_tile<double, TREE>(a, grid, s);
+  if (dtype == DG_F32) return launch_tile<float, TREE>(a, grid, s);
+  if (dtype == DG_BF16) return launch_tile<bf16_t, TREE>(a, grid, s);
+  return launch_tile<f16_t, TREE>(a, grid, s);
 }
 
-constexpr int kVecRows = 32;    // rows of a workgroup of the vector kernel over a tree
+// rows of a workgroup of seq_tile_kernel, for so many rows of a key head
+int tile_rows(int rows, int D) { return rows <= 8 ? 8 : D <= 256 ? 32 : 16; }
 
 // Splits of a row: enough workgroups to fill the CUs as far as their LDS and registers let
 // them share one (256 of 128 KB, as many more as smaller ones fit), and at least so many
 // stages each that joining the splits, a launch of its own of some 6 us, costs no more than
 // it saves: 8, one where fp32 products make a stage long (16 rows of the batch, 31 tokens
-// behind up to 600 keys, 4 heads of 64: 20 us with 4, 15 with 1).  us at 256 / 512 / 1024
+// behind up to 600 keys, 4 heads of 64: 20 us with 4, 15 with 1).  seq_tile_kernel's run up
+// to seven a CU and take longer: 2048 of two stages (a step over 32 caches of 1900, 8 heads
+// of 64, fp64: 468 us unsplit, 227 so).  us at 256 / 512 / 1024
 // workgroups, bf16:
 //   rows of 32, head_dim 128 (64 rows, 4 key heads, lengths to 4096)    52.1 / 58.6 / 68.3
 //               head_dim  64 (64 rows, 8 key heads, lengths to 1024)    17.2 / 17.0 / 25.3
@@ -352,11 +479,11 @@ constexpr int kVecRows = 32;    // rows of a workgroup of the vector kernel over
 //               head_dim  64 (2 rows, 2 key heads, lengths to 131000)   77.1 / 62.3 / 61.2
 constexpr int kMaxSplits = 512;
 
-int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int rows_per_wg, int D, int dtype) {
-  const int stage = rows_per_wg == 32 ? 128 : 64;  // keys; the vector kernel has no stages
+int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int rows_per_wg, int D, int dtype, bool mfma) {
+  const int stage = rows_per_wg <= 32 ? 128 : 64;  // keys, a multiple of every kernel's own
   const int64_t row_bytes = D * dtype_bytes(dtype);
-  const int64_t fill = rows_per_wg == 32 ? (row_bytes >= 256 ? 256 : 512) : rows_per_wg == 64 ? 512 : D == 128 ? 768 : 1024;
-  const int64_t least = dtype == DG_F32 && D >= 64 ? 1 : 8;
+  const int64_t fill = !mfma ? 2048 : rows_per_wg <= 32 ? (row_bytes >= 256 ? 256 : 512) : rows_per_wg == 64 ? 512 : D == 128 ? 768 : 1024;
+  const int64_t least = !mfma ? 2 : dtype == DG_F32 && D >= 64 ? 1 : 8;
   const int64_t wg = B * Hkv * nrb;
   const int64_t want = (fill + wg - 1) / wg;
   int64_t chunk = std::max<int64_t>((keys + want - 1) / want, (keys + kMaxSplits - 1) / kMaxSplits);
@@ -370,12 +497,12 @@ struct TreeShape {
   size_t o_bytes, ws_bytes;
 };
 
-TreeShape tree_shape(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype, int rows_per_wg) {
+TreeShape tree_shape(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype, int rows_per_wg, bool mfma) {
   TreeShape t{};
   const int R = N * (H / Hkv);
   t.rows_per_wg = rows_per_wg;
   t.nrb = (R + rows_per_wg - 1) / rows_per_wg;
-  t.chunk = tree_chunk(B, Hkv, t.nrb, Tcap, rows_per_wg, D, dtype);
+  t.chunk = tree_chunk(B, Hkv, t.nrb, Tcap, rows_per_wg, D, dtype, mfma);
   t.nsplit = (int)(((int64_t)Tcap + t.chunk - 1) / t.chunk);
   const size_t acc = dtype == DG_F64 ? 8 : 4;
   const size_t parts = (size_t)B * Hkv * R * t.nsplit;
@@ -391,9 +518,9 @@ bool known_dtype(int dtype) { return dtype == DG_F32 || dtype == DG_BF16 || dtyp
 // A bound on the workspace whichever kernel a call takes (the row blocks of each give
 // other splits).
 size_t tree_workspace(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
-  size_t most = 0;
+  size_t most = tree_shape(B, N, H, Hkv, Tcap, D, dtype, tile_rows(N * (H / Hkv), D), false).ws_bytes;
   for (int rows : {32, 64, 128})
-    most = std::max(most, tree_shape(B, N, H, Hkv, Tcap, D, dtype, rows).ws_bytes);
+    most = std::max(most, tree_shape(B, N, H, Hkv, Tcap, D, dtype, rows, true).ws_bytes);
   return most;
 }
 
@@ -539,13 +666,14 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   a.tiles = tiles;
   a.nq = Nq; a.nk = Nk;
   a.nsplit = 1;
-  a.rows_per_wg = kTileRows;
-  a.nrb = 1;
   const int64_t blocks = counts[0] * Hkv;
   DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (seq_mfma_applicable(a, dtype, false)) return launch_seq_mfma_packed(a, dtype, counts, s);
-  return launch_vec_any<false>(a, dtype, dim3((unsigned)blocks), s);
+  a.rows_per_wg = tile_rows((int)counts[2], D);
+  a.nrb = (int)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg);
+  DG_REQUIRE(blocks * a.nrb <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 workgroups");
+  return launch_tile_any<false>(a, dtype, dim3((unsigned)(blocks * a.nrb)), s);
 }
 
 extern "C" size_t dg_attention_tree_workspace_size(int B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
@@ -584,7 +712,7 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   a.len = len; a.lens = lens;
   a.masks = masks; a.mask_b = mask_b;
   const bool mfma = seq_mfma_applicable(a, dtype, true);
-  const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, mfma ? seq_mfma_tree_rows(B, N * a.G, Hkv, Tcap, D, dtype) : kVecRows);
+  const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, mfma ? seq_mfma_tree_rows(B, N * a.G, Hkv, Tcap, D, dtype) : tile_rows(N * a.G, D), mfma);
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
   if (t.nsplit > 1) {
     DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,
@@ -597,7 +725,7 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rc = mfma ? launch_seq_mfma_tree(a, dtype, (unsigned)blocks, s)
-                      : launch_vec_any<true>(a, dtype, dim3((unsigned)blocks), s);
+                      : launch_tile_any<true>(a, dtype, dim3((unsigned)blocks), s);
   if (rc != DG_OK || t.nsplit == 1) return rc;
   const int64_t rows = (int64_t)B * H * N;
   // a row's waves read its splits in turn: four of them where there are many and rows few

@@ -423,6 +423,41 @@ def test_tree_past_32_bit_offsets(dev):
     assert torch.equal(y, y2)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
+@pytest.mark.parametrize("D", [1, 7, 63, 65, 130, 255, 257, 511, 1023, 1024])
+@pytest.mark.parametrize("N,G", [(1, 1), (2, 4), (3, 3), (40, 1)])
+def test_tree_of_any_shape(dev, dtype, D, N, G):
+    """8, 16 and 32 rows a workgroup of the kernel for any head_dim, with splits and without."""
+    for Tcap, lens in ((90, [0, 31, 50]), (1500, [1460, 700, 3])):
+        q, k, v = _tree_case(dev, 3, N, 2 * G, 2, Tcap, D, TDT[dtype], seed=D)
+        parents = some_tree(N, seed=N)
+        y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+        assert _native.last_kernel() in ("seq_tile_kernel", "seq_join_kernel")
+        _check_tree(q, k, v, y, lens, parents, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f64"])
+@pytest.mark.parametrize("D", [5, 65, 129, 300, 1023])
+@pytest.mark.parametrize("q_lens,k_lens", [([1, 3, 0, 2], [70, 3, 9, 1]), ([40, 100, 7], [40, 133, 3])])
+def test_packed_of_any_shape(dev, dtype, D, q_lens, k_lens):
+    """And with values that are not finite, hidden from some rows of a tile: those keep their bits."""
+    q, k, v = (x.clone() for x in _packed_case(dev, q_lens, k_lens, 4, 2, D, TDT[dtype], seed=D))
+    lay = PackedLayout(q_lens, k_lens, group=2)
+    clean = attention_packed(q, k, v, lay)
+    assert _native.last_kernel() == "seq_tile_kernel"
+    _check_packed(q, k, v, clean, q_lens, k_lens, dtype)
+    hidden = torch.ones(q.size(0), dtype=torch.bool, device=dev)
+    a = b = 0
+    for n, t in zip(q_lens, k_lens):
+        k[b + t - 1], v[b + t - 1] = NAN, INF  # the last key, that the last query alone sees
+        if n > 0:
+            hidden[a + n - 1] = False
+        a, b = a + n, b + t
+    y = attention_packed(q, k, v, lay)
+    assert torch.equal(y[hidden], clean[hidden])
+    assert bool(y[~hidden].isnan().all())
+
+
 def test_calls_on_two_streams_at_once(dev):
     """Split trees and packed batches on two streams, each call with a workspace of its own
     and both with one layout: the bits of calls one after the other."""
