@@ -1,7 +1,7 @@
 // Attention over packed sequences (dg_attention_packed) and over a few tokens per cached
 // row (dg_attention_tree): the entry points, the host-side plan of packed tiles, the join
-// of split rows, and the kernel that takes any shape and type.  head_dim 16, 32, 64 and
-// 128 in 16-bit types and fp32 run on the matrix cores (dg_attn_seq_mfma.hip).
+// of split rows, and the kernel that takes any shape and type.  Rows of whole 16-byte pieces
+// up to 128 dims in 16-bit types and fp32 run on the matrix cores (dg_attn_seq_mfma.hip).
 //
 // The kernel here (seq_tile_kernel): 32 rows of a key head by 32 keys at a time, 16 rows
 // for head_dim over 256 and 8 where a piece has no more (a decode step): 8, 16 or 32 lanes
@@ -422,16 +422,17 @@ __global__ __launch_bounds__(256) void seq_join4_kernel(const SeqArgs a, const i
   float y[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = none ? 0.f : bad ? __builtin_nanf("") : o[e] / l;
-  store_vec<T, 4>(yp + d4, y);
+  if (d4 < a.D) store_vec<T, 4>(yp + d4, y);
 }
 
 namespace {
 
 template <typename T, int WPR>
 void launch_join4(const SeqArgs& a, dim3 grid, int64_t rows, hipStream_t s) {
-  if (a.D == 16) hipLaunchKernelGGL((seq_join4_kernel<T, 16, WPR>), grid, dim3(256), 0, s, a, rows);
-  else if (a.D == 32) hipLaunchKernelGGL((seq_join4_kernel<T, 32, WPR>), grid, dim3(256), 0, s, a, rows);
-  else if (a.D == 64) hipLaunchKernelGGL((seq_join4_kernel<T, 64, WPR>), grid, dim3(256), 0, s, a, rows);
+  const int D = seq_mfma_dim(a.D);
+  if (D == 16) hipLaunchKernelGGL((seq_join4_kernel<T, 16, WPR>), grid, dim3(256), 0, s, a, rows);
+  else if (D == 32) hipLaunchKernelGGL((seq_join4_kernel<T, 32, WPR>), grid, dim3(256), 0, s, a, rows);
+  else if (D == 64) hipLaunchKernelGGL((seq_join4_kernel<T, 64, WPR>), grid, dim3(256), 0, s, a, rows);
   else hipLaunchKernelGGL((seq_join4_kernel<T, 128, WPR>), grid, dim3(256), 0, s, a, rows);
 }
 
@@ -481,6 +482,7 @@ constexpr int kMaxSplits = 512;
 
 int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int rows_per_wg, int D, int dtype, bool mfma) {
   const int stage = rows_per_wg <= 32 ? 128 : 64;  // keys, a multiple of every kernel's own
+  if (mfma) D = seq_mfma_dim(D);
   const int64_t row_bytes = D * dtype_bytes(dtype);
   const int64_t fill = !mfma ? 2048 : rows_per_wg <= 32 ? (row_bytes >= 256 ? 256 : 512) : rows_per_wg == 64 ? 512 : D == 128 ? 768 : 1024;
   const int64_t least = !mfma ? 2 : dtype == DG_F32 && D >= 64 ? 1 : 8;
@@ -507,7 +509,7 @@ TreeShape tree_shape(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtyp
   const size_t acc = dtype == DG_F64 ? 8 : 4;
   const size_t parts = (size_t)B * Hkv * R * t.nsplit;
   if (t.nsplit > 1) {
-    t.o_bytes = (parts * D * acc + 15) & ~(size_t)15;
+    t.o_bytes = (parts * (mfma ? seq_mfma_dim(D) : D) * acc + 15) & ~(size_t)15;
     t.ws_bytes = t.o_bytes + parts * 2 * acc;
   }
   return t;
@@ -520,7 +522,7 @@ bool known_dtype(int dtype) { return dtype == DG_F32 || dtype == DG_BF16 || dtyp
 size_t tree_workspace(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
   size_t most = tree_shape(B, N, H, Hkv, Tcap, D, dtype, tile_rows(N * (H / Hkv), D), false).ws_bytes;
   for (int rows : {32, 64, 128})
-    most = std::max(most, tree_shape(B, N, H, Hkv, Tcap, D, dtype, rows, true).ws_bytes);
+    if (D <= 128) most = std::max(most, tree_shape(B, N, H, Hkv, Tcap, D, dtype, rows, true).ws_bytes);
   return most;
 }
 
@@ -711,7 +713,12 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   a.B = B; a.N = N; a.Tcap = Tcap;
   a.len = len; a.lens = lens;
   a.masks = masks; a.mask_b = mask_b;
-  const bool mfma = seq_mfma_applicable(a, dtype, true);
+  // 32-row tiles of fp32 products are mostly empty over 8 rows, and long at head_dim over 64:
+  // a step over 32 caches of 1900, 8 heads of 128, 155 us there and 127 in seq_tile_kernel,
+  // 64 of up to 4000, 16 heads on 4, 285 and 221; 4 of 140, 8 heads, 18.8 and 20.6, one of
+  // 20000, 4 heads, 41 and 59.
+  const bool few = dtype == DG_F32 && D > 64 && N * a.G <= 8 && (int64_t)B * Hkv >= 64;
+  const bool mfma = !few && seq_mfma_applicable(a, dtype, true);
   const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, mfma ? seq_mfma_tree_rows(B, N * a.G, Hkv, Tcap, D, dtype) : tile_rows(N * a.G, D), mfma);
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
   if (t.nsplit > 1) {

@@ -1,6 +1,8 @@
-// Packed attention and token trees over a cache on the matrix cores: head_dim 16, 32, 64
-// and 128 in bf16, fp16 and fp32 (dg_attn_seq.hip has the entry points and the kernel for
-// every other shape).
+// Packed attention and token trees over a cache on the matrix cores: bf16, fp16 and fp32 at
+// head_dim up to 128, rows of whole 16-byte pieces (dg_attn_seq.hip has the entry points and
+// the kernel for every other shape).  D here is 16, 32, 64 or 128: a head of fewer dims is
+// computed as one of the next of these, its missing pieces zeros (16 x 512 tokens, 8 heads of
+// 80: bf16 29 us, fp32 140; in seq_tile_kernel 385 and 340).
 //
 // A workgroup is WAVES wavefronts over one key head of one sequence: RT tiles of 32
 // (query, head of the group) rows by KS = WAVES / RT groups of keys.  With few rows (RT 1:
@@ -166,20 +168,23 @@ void seq_mfma_kernel(const SeqArgs a) {
   for (int n = 0; n < (C::NDMA + RT - 1) / RT; ++n) {
     const int r = (n * RT + rt) * C::RPD + lane / PPR;
     const int piece = (lane % PPR) ^ seq_swz<PPR, ES>(r);
-    ko[n] = r * (int)a.kt * ES + 16 * piece;
-    vo[n] = r * (int)a.vt * ES + 16 * piece;
+    // pieces past the head: out of range of any resource, which makes them zeros
+    const bool in = 16 * piece < a.D * ES;
+    ko[n] = in ? r * (int)a.kt * ES + 16 * piece : (int)0x80000000u;
+    vo[n] = in ? r * (int)a.vt * ES + 16 * piece : (int)0x80000000u;
   }
   // Where the piece's keys span less than 2^31 bytes, one resource serves all stages, the
   // stage's start in the scalar offset.
   const int64_t kstep_b = a.kt * ES, vstep_b = a.vt * ES;  // bytes from key to key
   const int nkeys = max(0, pc.kend - pc.kbeg);
-  const bool near = nkeys * max(kstep_b, vstep_b) + D * ES < ((int64_t)1 << 31);
+  const int row_b = a.D * ES;
+  const bool near = nkeys * max(kstep_b, vstep_b) + row_b < ((int64_t)1 << 31);
   const T* const kp0 = kp + (int64_t)pc.kbeg * a.kt;
   const T* const vp0 = vp + (int64_t)pc.kbeg * a.vt;
   const __amdgpu_buffer_rsrc_t krs0 = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<T*>(kp0), 0, near && nkeys > 0 ? (int)((nkeys - 1) * kstep_b + D * ES) : 0, kBufferWord3);
+      const_cast<T*>(kp0), 0, near && nkeys > 0 ? (int)((nkeys - 1) * kstep_b + row_b) : 0, kBufferWord3);
   const __amdgpu_buffer_rsrc_t vrs0 = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<T*>(vp0), 0, near && nkeys > 0 ? (int)((nkeys - 1) * vstep_b + D * ES) : 0, kBufferWord3);
+      const_cast<T*>(vp0), 0, near && nkeys > 0 ? (int)((nkeys - 1) * vstep_b + row_b) : 0, kBufferWord3);
   auto copy_from = [&](T* st, __amdgpu_buffer_rsrc_t krs, __amdgpu_buffer_rsrc_t vrs, int ks0, int vs0)
       __attribute__((always_inline)) {
     T* const ks = st + kg * 2 * TILE;
@@ -197,8 +202,8 @@ void seq_mfma_kernel(const SeqArgs a) {
       copy_from(st, krs0, vrs0, rel * (int)kstep_b, rel * (int)vstep_b);
     } else {  // far, or a group's stage behind the last key: zeros
       const int left = min(BN, nkeys - rel);
-      const int kn = left <= 0 ? 0 : (int)((left - 1) * kstep_b) + D * ES;
-      const int vn = left <= 0 ? 0 : (int)((left - 1) * vstep_b) + D * ES;
+      const int kn = left <= 0 ? 0 : (int)((left - 1) * kstep_b) + row_b;
+      const int vn = left <= 0 ? 0 : (int)((left - 1) * vstep_b) + row_b;
       copy_from(st, __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp0 + rel * a.kt), 0, kn, kBufferWord3),
                 __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp0 + rel * a.vt), 0, vn, kBufferWord3), 0, 0);
     }
@@ -215,14 +220,18 @@ void seq_mfma_kernel(const SeqArgs a) {
   if constexpr (F32) {
 #pragma unroll
     for (int m = 0; m < C::QC / 4; ++m) {
-      const f32x4_t x = reinterpret_cast<const f32x4_t*>(qp + C::QC * hh)[m];
+      const int d = C::QC * hh + 4 * m;
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(qp + min(d, a.D - 4));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) qf[4 * m + e] = x[e];
+      for (int e = 0; e < 4; ++e) qf[4 * m + e] = d < a.D ? x[e] : 0.f;
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < C::NC; ++c)
-      qf[c] = __builtin_bit_cast(vec8, *reinterpret_cast<const u32x4_t*>(qp + 16 * c + 8 * hh));
+    for (int c = 0; c < C::NC; ++c) {
+      const int d = 16 * c + 8 * hh;
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qp + min(d, a.D - 8));
+      qf[c] = __builtin_bit_cast(vec8, d < a.D ? x : u32x4_t{0u, 0u, 0u, 0u});
+    }
   }
 
   const int kstep = KS * BN;
@@ -556,9 +565,10 @@ void seq_mfma_kernel(const SeqArgs a) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) w[NB * e + nb] = none ? 0.f : o[nb][4 * g + e] * inv;
 #pragma unroll
-      for (int x = 0; x < NB; ++x)
-        *reinterpret_cast<f32x4_t*>(yp + NB * (8 * g + 4 * hh) + 4 * x) =
-            f32x4_t{w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]};
+      for (int x = 0; x < NB; ++x) {
+        const int d = NB * (8 * g + 4 * hh) + 4 * x;
+        if (d < a.D) *reinterpret_cast<f32x4_t*>(yp + d) = f32x4_t{w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]};
+      }
     }
   } else {
     // through LDS, so that a store writes whole rows; the wave's own rows, no barrier
@@ -582,7 +592,7 @@ void seq_mfma_kernel(const SeqArgs a) {
       const int r = p * RPS + lane / PPR;
       const u32x4_t w = *reinterpret_cast<const u32x4_t*>(stg + r * D + 8 * (piece ^ (r & (PPR - 1))));
       const int rr = wrow + r;
-      if (rr < rend) {
+      if (rr < rend && 8 * piece < a.D) {
         const int i = rr / a.G, h = pc.kvh * a.G + (rr - i * a.G);
         T* yp = static_cast<T*>(a.y) + pc.b * a.yb + (pc.q0 + i) * a.yt + (int64_t)h * a.yh;
         *reinterpret_cast<u32x4_t*>(yp + 8 * piece) = w;
@@ -608,7 +618,7 @@ int launch_seq_d(const SeqArgs& a, dim3 grid, hipStream_t s) {
   constexpr bool kF32 = sizeof(T) == 4;
 #define DG_SEQ_D(DIM)                                  \
   if constexpr (!TREE || tree_has_shape(DIM, RT, kF32)) \
-    if (a.D == DIM) return launch_seq<T, DIM, RT, TREE>(a, grid, s)
+    if (seq_mfma_dim(a.D) == DIM) return launch_seq<T, DIM, RT, TREE>(a, grid, s)
   DG_SEQ_D(16);
   DG_SEQ_D(32);
   DG_SEQ_D(64);
@@ -626,10 +636,10 @@ int launch_seq_t(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
 
 }  // namespace
 
-// head_dim 16, 32, 64 and 128 in 16-bit types and fp32, rows aligned to the 16-byte loads
-// and stores, and a stage's rows (up to 64) within 2^31 bytes of each other.
+// 16-bit types and fp32, rows of whole 16-byte pieces, up to 128 dims, aligned to them, and
+// a stage's rows (up to 64) within 2^31 bytes of each other.
 bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree) {
-  if (dtype == DG_F64 || (a.D != 16 && a.D != 32 && a.D != 64 && a.D != 128)) return false;
+  if (dtype == DG_F64 || a.D > 128 || a.D * dtype_bytes(dtype) % 16 != 0) return false;
   const int64_t es = dtype_bytes(dtype);
   auto rows = [&](const void* p, int64_t b, int64_t t, int64_t h) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (!tree || b * es % 16 == 0) && t * es % 16 == 0 && h * es % 16 == 0;
@@ -654,7 +664,7 @@ bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree) {
 //     head_dim 128 180 / 136 / 163
 int seq_mfma_tree_rows(int64_t B, int rows, int Hkv, int keys, int D, int dtype) {
   if (rows <= 32 || D <= 32) return 32;
-  if (dtype == DG_F32) return D == 64 ? 32 : 64;
+  if (dtype == DG_F32) return D <= 64 ? 32 : 64;
   const int64_t tiles = B * Hkv * ((rows + 127) / 128);
   if (tiles * keys <= 300000) return 32;
   return rows <= 64 || tiles >= 256 ? 64 : 128;
@@ -677,7 +687,7 @@ int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream
 //   head_dim 128: 1 x 3584 in groups of 2 [448] 129 / 82 / 92, 2 x 2048 [512] 110 / 63 / 57
 int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s) {
   const int64_t tiles = counts[1] * a.Hkv;
-  const int rt = counts[2] <= 32 || tiles <= 64 ? 1 : counts[2] <= 64 || tiles <= (a.D == 128 ? 384 : 640) ? 2 : 4;
+  const int rt = counts[2] <= 32 || tiles <= 64 ? 1 : counts[2] <= 64 || tiles <= (a.D > 64 ? 384 : 640) ? 2 : 4;
   a.rows_per_wg = 32 * rt;
   a.nrb = (int)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg);
   const dim3 grid((unsigned)(counts[0] * a.Hkv * a.nrb));

@@ -1,6 +1,6 @@
 // Launch arguments shared by the kernels of packed attention and of token trees
 // over a cache (dg_attn_seq.hip: any shape; dg_attn_seq_mfma.hip: 16-bit and fp32 data
-// at head_dim 16, 32, 64 and 128).
+// at head_dim up to 128, in rows of whole 16-byte pieces).
 //
 // Both operators reduce to one piece of work: the rows of one key head, where the
 // rows are the (query, head of the group) pairs r = i * G + g of a sequence, over a
@@ -135,6 +135,9 @@ __device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n
   if (a.masks == nullptr) return n >= 63 ? ~0ull : (2ull << n) - 1;
   return (uint64_t)a.masks[b * a.mask_b + n] & all;
 }
+
+// The head_dim that the matrix-core kernels and their workspaces round D (up to 128) up to.
+constexpr int seq_mfma_dim(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // dg_attn_seq_mfma.hip: whether it takes the shape, the rows of a workgroup over so many
 // (token, head) rows, and its launches

@@ -61,7 +61,7 @@ MIXED = ([130, 5, 64, 200, 1, 128, 33, 300], [130, 40, 64, 333, 1, 100, 33, 300]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
 @pytest.mark.parametrize("Hkv,G,copies,rows", [(1, 1, 1, 32), (8, 1, 2, 64), (4, 3, 2, 64), (8, 1, 7, 128), (6, 2, 7, 128)])
 def test_packed_in_every_workgroup_shape(dev, dtype, D, Hkv, G, copies, rows):
     """One, two and four 32-row waves a tile, by how many tiles there are."""
@@ -73,7 +73,7 @@ def test_packed_in_every_workgroup_shape(dev, dtype, D, Hkv, G, copies, rows):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
 @pytest.mark.parametrize("Hkv,copies,rows", [(1, 1, 32), (8, 2, 64), (8, 7, 128)])
 def test_packed_hidden_values_in_every_workgroup_shape(dev, dtype, D, Hkv, copies, rows):
     """NaN keys and infinite and NaN values that some rows of a tile see and others do not:
@@ -124,7 +124,7 @@ def test_packed_takes_unaligned_rows(dev, dtype, D):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
 def test_packed_hidden_values_stay_hidden(dev, dtype, D):
     """NaN and infinities in the keys and values of later positions, and in rows behind
     the last sequence, reach no query that does not see them; those that do see an infinite
@@ -270,7 +270,9 @@ def test_tree_matches_float64(dev, dtype, H, Hkv, D, N, lens, Tcap):
     ("f32", 16, 2, 60, 1, 3, 70, 32), ("bf16", 32, 3, 40, 2, 2, 300, 32), ("f32", 64, 2, 50, 1, 3, 90, 32),
     ("f32", 128, 2, 50, 2, 3, 100, 64), ("f32", 128, 60, 64, 4, 1, 100, 64), ("bf16", 64, 3, 41, 2, 4, 1000, 32),
     ("f16", 128, 3, 64, 2, 1, 900, 32), ("bf16", 64, 65, 33, 4, 1, 1300, 64), ("f16", 64, 40, 64, 4, 3, 700, 32), ("f16", 64, 40, 64, 4, 3, 1000, 64),
-    ("bf16", 128, 64, 50, 4, 3, 700, 64), ("f16", 128, 128, 45, 1, 2, 2500, 128), ("bf16", 64, 250, 37, 1, 3, 1300, 128)])
+    ("bf16", 128, 64, 50, 4, 3, 700, 64), ("f16", 128, 128, 45, 1, 2, 2500, 128), ("bf16", 64, 250, 37, 1, 3, 1300, 128),
+    ("bf16", 56, 65, 33, 4, 1, 1300, 64), ("f16", 96, 128, 45, 1, 2, 2500, 128), ("f32", 100, 60, 64, 4, 1, 100, 64),
+    ("f32", 4, 3, 50, 2, 1, 100, 32)])
 def test_tree_in_every_workgroup_shape(dev, dtype, D, B, N, Hkv, G, Tcap, rows):
     """32, 64 and 128 rows a workgroup, where one takes all of a row's keys."""
     lens = [(131 * (b + 1)) % (Tcap - N + 1) for b in range(B)]
@@ -282,7 +284,7 @@ def test_tree_in_every_workgroup_shape(dev, dtype, D, B, N, Hkv, G, Tcap, rows):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
 @pytest.mark.parametrize("N,G", [(3, 1), (13, 4), (40, 3)])
 @pytest.mark.parametrize("B,Tcap", [(1, 60000), (2, 9000)])
 def test_tree_splits_meet(dev, dtype, D, N, G, B, Tcap):
@@ -421,6 +423,17 @@ def test_tree_past_32_bit_offsets(dev):
     y2 = attention_packed(q.view(4, 4, D), flat[:, 7:8], flat[:, 33:34],
                           PackedLayout([2, 2], [150000, 150000], group=4))
     assert torch.equal(y, y2)
+
+
+@pytest.mark.parametrize("D,kernel", [(64, "mfma"), (80, "tile"), (128, "tile")])
+@pytest.mark.parametrize("N,G,Tcap", [(1, 1, 100), (2, 4, 100), (1, 3, 1500)])
+def test_fp32_steps_of_many_rows(dev, D, kernel, N, G, Tcap):
+    lens = [(37 * b) % (Tcap - N + 1) for b in range(33)]
+    q, k, v = _tree_case(dev, 33, N, 2 * G, 2, Tcap, D, torch.float32, seed=D)
+    parents = some_tree(N, seed=1)
+    y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+    assert _native.last_kernel() == "seq_join_kernel" or kernel in _native.last_kernel()
+    _check_tree(q, k, v, y, lens, parents, "f32")
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
