@@ -1,7 +1,7 @@
 // Attention over packed sequences (dg_attention_packed) and over a few tokens per cached
 // row (dg_attention_tree): the entry points, the host-side plan of packed tiles, the join
 // of split rows, and the kernel that takes any shape and type.  Rows of whole 16-byte pieces
-// up to 128 dims in 16-bit types and fp32 run on the matrix cores (dg_attn_seq_mfma.hip).
+// up to 256 dims in 16-bit types, 128 in fp32, run on the matrix cores (dg_attn_seq_mfma.hip).
 //
 // The kernel here (seq_tile_kernel): 32 rows of a key head by 32 keys at a time, 16 rows
 // for head_dim over 256 and 8 where a piece has no more (a decode step): 8, 16 or 32 lanes
@@ -11,10 +11,10 @@
 // lanes have a key each, for the outputs dims each; the probabilities go from one to the
 // other through LDS.  A hidden key's score is taken out by selection and its values are
 // skipped, so nothing it holds can reach a row.  Bound by LDS reads (five of 16 bytes for
-// 16 products a lane).  16 x 512 tokens, 8 heads: head_dim 80 bf16 385 us, 96 fp32 358 (18
-// TFLOP/s), 256 bf16 1000, 64 fp64 366; a step over 32 caches of 1900, 8 heads: 80 bf16
-// 118 us, 256 bf16 216, 64 fp64 124 (4.0 TB/s).  One row a wave at a time with a running
-// softmax in each lane group took 14.9 ms, 17.4, 31.3, 13.1 and 1.2 ms, 6.1, 2.2.
+// 16 products a lane).  16 x 512 tokens, 8 heads: head_dim 65 bf16 371 us, 600
+// fp32 2.4 ms (17 TFLOP/s), 64 fp64 366; a step over 32 caches of 1900, 8 heads: 65 bf16
+// 115 us, 600 fp32 566 (4.1 TB/s), 64 fp64 124 (4.0 TB/s).  One row a wave at a time with a
+// running softmax in each lane group took 13.1 ms and 2.2 ms in fp64.
 #include "dg_seq.h"
 
 #include <algorithm>
@@ -433,7 +433,8 @@ void launch_join4(const SeqArgs& a, dim3 grid, int64_t rows, hipStream_t s) {
   if (D == 16) hipLaunchKernelGGL((seq_join4_kernel<T, 16, WPR>), grid, dim3(256), 0, s, a, rows);
   else if (D == 32) hipLaunchKernelGGL((seq_join4_kernel<T, 32, WPR>), grid, dim3(256), 0, s, a, rows);
   else if (D == 64) hipLaunchKernelGGL((seq_join4_kernel<T, 64, WPR>), grid, dim3(256), 0, s, a, rows);
-  else hipLaunchKernelGGL((seq_join4_kernel<T, 128, WPR>), grid, dim3(256), 0, s, a, rows);
+  else if (D == 128) hipLaunchKernelGGL((seq_join4_kernel<T, 128, WPR>), grid, dim3(256), 0, s, a, rows);
+  else hipLaunchKernelGGL((seq_join4_kernel<T, 256, WPR>), grid, dim3(256), 0, s, a, rows);
 }
 
 template <typename T, bool TREE>
@@ -484,7 +485,10 @@ int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int rows_per_wg, int D, in
   const int stage = rows_per_wg <= 32 ? 128 : 64;  // keys, a multiple of every kernel's own
   if (mfma) D = seq_mfma_dim(D);
   const int64_t row_bytes = D * dtype_bytes(dtype);
-  const int64_t fill = !mfma ? 2048 : rows_per_wg <= 32 ? (row_bytes >= 256 ? 256 : 512) : rows_per_wg == 64 ? 512 : D == 128 ? 768 : 1024;
+  const int64_t fill = !mfma ? 2048
+                       : rows_per_wg <= 32 ? (row_bytes >= 256 ? 256 : 512)
+                       : rows_per_wg == 64 ? (row_bytes >= 512 ? 256 : 512)
+                                           : D == 256 ? 512 : D == 128 ? 768 : 1024;
   const int64_t least = !mfma ? 2 : dtype == DG_F32 && D >= 64 ? 1 : 8;
   const int64_t wg = B * Hkv * nrb;
   const int64_t want = (fill + wg - 1) / wg;
@@ -522,7 +526,7 @@ bool known_dtype(int dtype) { return dtype == DG_F32 || dtype == DG_BF16 || dtyp
 size_t tree_workspace(int64_t B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
   size_t most = tree_shape(B, N, H, Hkv, Tcap, D, dtype, tile_rows(N * (H / Hkv), D), false).ws_bytes;
   for (int rows : {32, 64, 128})
-    if (D <= 128) most = std::max(most, tree_shape(B, N, H, Hkv, Tcap, D, dtype, rows, true).ws_bytes);
+    if (D <= 256) most = std::max(most, tree_shape(B, N, H, Hkv, Tcap, D, dtype, rows, true).ws_bytes);
   return most;
 }
 

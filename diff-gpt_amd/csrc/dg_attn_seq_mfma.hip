@@ -1,7 +1,7 @@
-// Packed attention and token trees over a cache on the matrix cores: bf16, fp16 and fp32 at
-// head_dim up to 128, rows of whole 16-byte pieces (dg_attn_seq.hip has the entry points and
-// the kernel for every other shape).  D here is 16, 32, 64 or 128: a head of fewer dims is
-// computed as one of the next of these, its missing pieces zeros (16 x 512 tokens, 8 heads of
+// Packed attention and token trees over a cache on the matrix cores: bf16 and fp16 at head_dim
+// up to 256, fp32 up to 128, rows of whole 16-byte pieces (dg_attn_seq.hip has the entry points
+// and the kernel for every other shape).  D here is 16, 32, 64, 128 or 256: a head of fewer
+// dims is computed as one of the next of these, its missing pieces zeros (16 x 512 tokens, 8 heads of
 // 80: bf16 29 us, fp32 140; in seq_tile_kernel 385 and 340).
 //
 // A workgroup is WAVES wavefronts over one key head of one sequence: RT tiles of 32
@@ -75,7 +75,7 @@ struct SeqMma<float> {
 template <typename T, int D, int RT>
 struct SeqCfg {
   static constexpr int ES = (int)sizeof(T);
-  static constexpr int WAVES = (ES == 4 && D == 128 && RT == 1) ? 2 : 4;
+  static constexpr int WAVES = (D * ES >= 512 && RT == 1) ? 2 : 4;
   static constexpr int KS = WAVES / RT;
   // 32-key blocks of a stage
   static constexpr int MB = RT == 4 ? (ES == 2 && D == 64 ? 2 : 1) : D * ES <= 64 ? 2 : 1;
@@ -93,15 +93,15 @@ struct SeqCfg {
   static_assert((((KS - 1) * RT + 1) / 2) * JOIN * 4 <= KS * 2 * TILE * ES, "joined states fit a stage");
   static_assert(ES == 4 || ((RT + 1) / 2) * 32 * D <= KS * 2 * TILE, "outputs fit a stage");
   // workgroups a CU that the registers must allow (fp32 at head_dim 64, 64 x 512 tokens: four
-  // spill, 215 us; three 177)
-  static constexpr int WGS = RT == 4 ? (ES == 4 ? (D <= 32 ? 4 : D == 64 ? 3 : 2) : D <= 64 ? 4 : 3) : (D * ES <= 128 ? 2 : 1);
+  // spill, 215 us; three 177.  bf16 at 256, 16 x 512, 8 heads: two spill, 148; one 76)
+  static constexpr int WGS = RT == 4 ? (ES == 4 ? (D <= 32 ? 4 : D == 64 ? 3 : 2) : D <= 64 ? 4 : D == 128 ? 3 : 1) : (D * ES <= 128 ? 2 : 1);
 };
 
 template <int PPR, int ES>
 __device__ __forceinline__ int seq_swz(int r) {
   if constexpr (ES == 4) return r & (PPR >= 16 ? 15 : PPR - 1);
   else if constexpr (PPR == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
-  else if constexpr (PPR == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (PPR >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
   else if constexpr (PPR == 4) return (r >> 2) & 3;
   else return 0;
 }
@@ -623,6 +623,7 @@ int launch_seq_d(const SeqArgs& a, dim3 grid, hipStream_t s) {
   DG_SEQ_D(32);
   DG_SEQ_D(64);
   DG_SEQ_D(128);
+  if constexpr (!kF32) DG_SEQ_D(256);
 #undef DG_SEQ_D
   return DG_EUNSUPPORTED;
 }
@@ -636,10 +637,10 @@ int launch_seq_t(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
 
 }  // namespace
 
-// 16-bit types and fp32, rows of whole 16-byte pieces, up to 128 dims, aligned to them, and
+// 16-bit types up to 256 dims, fp32 up to 128, rows of whole 16-byte pieces aligned to them, and
 // a stage's rows (up to 64) within 2^31 bytes of each other.
 bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree) {
-  if (dtype == DG_F64 || a.D > 128 || a.D * dtype_bytes(dtype) % 16 != 0) return false;
+  if (dtype == DG_F64 || a.D > (dtype == DG_F32 ? 128 : 256) || a.D * dtype_bytes(dtype) % 16 != 0) return false;
   const int64_t es = dtype_bytes(dtype);
   auto rows = [&](const void* p, int64_t b, int64_t t, int64_t h) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (!tree || b * es % 16 == 0) && t * es % 16 == 0 && h * es % 16 == 0;
@@ -684,6 +685,8 @@ int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream
 //   head_dim  64: 8 x 512 tokens [256] 18.7 / 14.0 / 15.2, 16 [512] 31.6 / 19.5 / 18.2,
 //     32 [1024] 52.3 / 28.7 / 23.3; 6 x 2048 [768] 69.6 / 51.5 / 50; 48 chunks of up to
 //     300 behind up to 3000 keys, groups of 4 [436] 61 / 46.5 / 61.5, 64 [550] 72 / 61 / 59
+//   head_dim 256: 2 x 512 [64] 24 / 27 / 37, 2 x 2048 in groups of 2 [256] 146 / 103 / 101,
+//     16 x 512 [512] 142 / 97 / 76
 //   head_dim 128: 1 x 3584 in groups of 2 [448] 129 / 82 / 92, 2 x 2048 [512] 110 / 63 / 57
 int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s) {
   const int64_t tiles = counts[1] * a.Hkv;

@@ -1,6 +1,6 @@
 // Launch arguments shared by the kernels of packed attention and of token trees
 // over a cache (dg_attn_seq.hip: any shape; dg_attn_seq_mfma.hip: 16-bit and fp32 data
-// at head_dim up to 128, in rows of whole 16-byte pieces).
+// at head_dim up to 256 and 128, in rows of whole 16-byte pieces).
 //
 // Both operators reduce to one piece of work: the rows of one key head, where the
 // rows are the (query, head of the group) pairs r = i * G + g of a sequence, over a
@@ -136,8 +136,8 @@ __device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n
   return (uint64_t)a.masks[b * a.mask_b + n] & all;
 }
 
-// The head_dim that the matrix-core kernels and their workspaces round D (up to 128) up to.
-constexpr int seq_mfma_dim(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+// The head_dim that the matrix-core kernels and their workspaces round D (up to 256) up to.
+constexpr int seq_mfma_dim(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 // dg_attn_seq_mfma.hip: whether it takes the shape, the rows of a workgroup over so many
 // (token, head) rows, and its launches

@@ -61,19 +61,19 @@ MIXED = ([130, 5, 64, 200, 1, 128, 33, 300], [130, 40, 64, 333, 1, 100, 33, 300]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120, 200, 256])
 @pytest.mark.parametrize("Hkv,G,copies,rows", [(1, 1, 1, 32), (8, 1, 2, 64), (4, 3, 2, 64), (8, 1, 7, 128), (6, 2, 7, 128)])
 def test_packed_in_every_workgroup_shape(dev, dtype, D, Hkv, G, copies, rows):
     """One, two and four 32-row waves a tile, by how many tiles there are."""
     q_lens, k_lens = MIXED[0] * copies, MIXED[1] * copies
     q, k, v = _packed_case(dev, q_lens, k_lens, Hkv * G, Hkv, D, TDT[dtype], seed=copies)
     y = attention_packed(q, k, v, PackedLayout(q_lens, k_lens, group=G))
-    assert _native.last_kernel() == f"seq_mfma_packed_{rows}"
+    assert _native.last_kernel() == ("seq_tile_kernel" if dtype == "f32" and D > 128 else f"seq_mfma_packed_{rows}")
     _check_packed(q, k, v, y, q_lens, k_lens, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120, 200, 256])
 @pytest.mark.parametrize("Hkv,copies,rows", [(1, 1, 32), (8, 2, 64), (8, 7, 128)])
 def test_packed_hidden_values_in_every_workgroup_shape(dev, dtype, D, Hkv, copies, rows):
     """NaN keys and infinite and NaN values that some rows of a tile see and others do not:
@@ -97,7 +97,7 @@ def test_packed_hidden_values_in_every_workgroup_shape(dev, dtype, D, Hkv, copie
         hidden[a + first : a + n] = False
         a, b = a + n, b + t
     y = attention_packed(q, kk, vv, lay)
-    assert _native.last_kernel() == f"seq_mfma_packed_{rows}"
+    assert _native.last_kernel() == ("seq_tile_kernel" if dtype == "f32" and D > 128 else f"seq_mfma_packed_{rows}")
     assert torch.equal(y[hidden], clean[hidden])
     want = what[~hidden][:, None, None].expand_as(y[~hidden])
     got = y[~hidden].float()
@@ -124,7 +124,7 @@ def test_packed_takes_unaligned_rows(dev, dtype, D):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120, 200, 256])
 def test_packed_hidden_values_stay_hidden(dev, dtype, D):
     """NaN and infinities in the keys and values of later positions, and in rows behind
     the last sequence, reach no query that does not see them; those that do see an infinite
@@ -272,7 +272,8 @@ def test_tree_matches_float64(dev, dtype, H, Hkv, D, N, lens, Tcap):
     ("f16", 128, 3, 64, 2, 1, 900, 32), ("bf16", 64, 65, 33, 4, 1, 1300, 64), ("f16", 64, 40, 64, 4, 3, 700, 32), ("f16", 64, 40, 64, 4, 3, 1000, 64),
     ("bf16", 128, 64, 50, 4, 3, 700, 64), ("f16", 128, 128, 45, 1, 2, 2500, 128), ("bf16", 64, 250, 37, 1, 3, 1300, 128),
     ("bf16", 56, 65, 33, 4, 1, 1300, 64), ("f16", 96, 128, 45, 1, 2, 2500, 128), ("f32", 100, 60, 64, 4, 1, 100, 64),
-    ("f32", 4, 3, 50, 2, 1, 100, 32)])
+    ("f32", 4, 3, 50, 2, 1, 100, 32), ("bf16", 256, 2, 9, 1, 1, 100, 32), ("f16", 136, 64, 50, 4, 3, 700, 64),
+    ("bf16", 256, 128, 45, 1, 2, 2500, 128)])
 def test_tree_in_every_workgroup_shape(dev, dtype, D, B, N, Hkv, G, Tcap, rows):
     """32, 64 and 128 rows a workgroup, where one takes all of a row's keys."""
     lens = [(131 * (b + 1)) % (Tcap - N + 1) for b in range(B)]
@@ -284,7 +285,7 @@ def test_tree_in_every_workgroup_shape(dev, dtype, D, B, N, Hkv, G, Tcap, rows):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 8, 24, 40, 80, 120, 200, 256])
 @pytest.mark.parametrize("N,G", [(3, 1), (13, 4), (40, 3)])
 @pytest.mark.parametrize("B,Tcap", [(1, 60000), (2, 9000)])
 def test_tree_splits_meet(dev, dtype, D, N, G, B, Tcap):
