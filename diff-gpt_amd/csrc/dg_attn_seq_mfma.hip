@@ -30,8 +30,8 @@
 // Bound by the softmax's vector instructions beside the matrix cores' for prompts (28 cycles
 // of a SIMD for 64 scores: fused product, exp2 at a quarter of the rate, sum, pack,
 // maximum), by HBM for few rows.  bf16: 6 sequences of up to 7168 tokens, 16 heads on 4 of
-// 128, 482 us (990 TFLOP/s; vector ALU 54 % busy, matrix cores 53 %); 64 of 100 - 2048, 8
-// heads of 64, 167 us (660 TFLOP/s; 66 %, 34 %); one token for each of 64 caches of up to
+// 128, 487 us (980 TFLOP/s; vector ALU 54 % busy, matrix cores 53 %); 64 of 100 - 2048, 8
+// heads of 64, 169 us (650 TFLOP/s; 66 %, 34 %); one token for each of 64 caches of up to
 // 4096, 16 heads on 4 of 128, 52 us (269 MB, 5.1 TB/s).
 // Not kept: the K fragments of a block in flight together, two chains for the row sums, 168
 // registers at head_dim 64, raised wave priority around the products (each within 2 %);

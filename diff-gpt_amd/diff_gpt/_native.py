@@ -262,7 +262,7 @@ _SIGNATURES = {
     "dg_attention_tree": (
         ctypes.c_int,
         [ctypes.c_int] * 7
-        + [ctypes.c_void_p, ctypes.POINTER(Stride3)] * 4  # q, k_cache, v_cache, y
+        + [ctypes.c_void_p, ctypes.c_void_p] * 4  # q, k_cache, v_cache, y, each with its dg_stride3
         + [ctypes.c_float, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
            ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
     ),
@@ -786,6 +786,8 @@ def _check_scale(what: str, scale: float) -> float:
     return scale
 
 
+_Stride3x4 = ctypes.c_int64 * 12
+
 # rows of a dg_packed_tile: eight 32-bit integers
 _TILE_WORDS = 8
 
@@ -881,9 +883,16 @@ def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     L = lib()
     ws_bytes = L.dg_attention_tree_workspace_size(B, N, H, Hkv, Tcap, D, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    st = [ctypes.byref(_bthd_strides(x)) for x in (q, k_cache, v_cache, y)]
-    _launch("attention_tree", device, L.dg_attention_tree, B, N, H, Hkv, Tcap, D, code, q.data_ptr(), st[0],
-            k_cache.data_ptr(), st[1], v_cache.data_ptr(), st[2], y.data_ptr(), st[3], scale, host_len,
+    qb, qt, qh, qd = q.stride()
+    kb, kt, kh, kd = k_cache.stride()
+    vb, vt, vh, vd = v_cache.stride()
+    yb, yt, yh, yd = y.stride()
+    if not (qd == kd == vd == yd == 1) and D > 1:
+        raise ValueError("attention_tree: the last (head_dim) dimension must be contiguous")
+    st = _Stride3x4(qb, qt, qh, kb, kt, kh, vb, vt, vh, yb, yt, yh)  # four dg_stride3
+    at = ctypes.addressof(st)
+    _launch("attention_tree", device, L.dg_attention_tree, B, N, H, Hkv, Tcap, D, code, q.data_ptr(), at,
+            k_cache.data_ptr(), at + 24, v_cache.data_ptr(), at + 48, y.data_ptr(), at + 72, scale, host_len,
             None if lens is None else lens.data_ptr(), None if masks is None else masks.data_ptr(), mask_b,
             None if ws is None else ws.data_ptr(), ws_bytes)
 

@@ -46,7 +46,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     """Causal attention of q (Nq, H, D) over k, v (Nk, Hkv, D), within each sequence of
     ``layout``; query head h reads key head h // (H / Hkv).  scale: 1 / sqrt(D) by default.
     A query that sees no key gets zeros, and so do rows behind the last sequence."""
-    y = q.new_empty(q.shape)
+    y = torch.empty_like(q, memory_format=torch.contiguous_format)
     if scale is None:
         scale = 1.0 / math.sqrt(max(1, q.size(-1)))
     _native.attention_packed_(q, k, v, y, layout, scale)

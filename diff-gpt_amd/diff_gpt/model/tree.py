@@ -52,7 +52,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     0 .. Tcap - N) and the N tokens behind them, of which token n sees those in its mask
     ((N,) or (B, N) int64, tree_masks; None: the tokens before it and itself).  Query head h
     reads key head h // (H / Hkv).  scale: 1 / sqrt(D) by default."""
-    y = q.new_empty(q.shape)
+    y = torch.empty_like(q, memory_format=torch.contiguous_format)
     if scale is None:
         scale = 1.0 / math.sqrt(max(1, q.size(-1)))
     _native.attention_tree_(q, k_cache, v_cache, y, scale, lengths, masks)
