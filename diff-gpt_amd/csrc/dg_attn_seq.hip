@@ -660,7 +660,7 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
                  counts[2] >= 0 && counts[2] <= kTileRows,
              DG_EINVAL, "attention_packed: counts (%lld, %lld, %lld) are not dg_packed_plan's", (long long)counts[0],
              (long long)counts[1], (long long)counts[2]);
-  if (Nq == 0 || H == 0 || counts[0] == 0) return DG_OK;
+  if (Nq == 0 || H == 0 || counts[1] == 0 || counts[2] == 0) return DG_OK;  // no tile
   DG_REQUIRE(q && y && tiles && (Nk == 0 || (k && v)), DG_EINVAL, "attention_packed: NULL argument");
   SeqArgs a{};
   a.q = q; a.k = k; a.v = v; a.y = y;

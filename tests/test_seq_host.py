@@ -122,7 +122,8 @@ def _tree(B=1, N=2, H=1, Hkv=1, Tcap=8, D=16, dtype=0, p=FAKE, scale=1.0, length
                                    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(p=NUL), -1),
                                    (dict(tiles=NUL), -1), (dict(counts=None), -1), (dict(counts=(-8, 0, 0)), -1),
                                    (dict(counts=(1, 1, 1)), -1), (dict(counts=(8, 9, 1)), -1),
-                                   (dict(counts=(8, 1, 129)), -1), (dict(Nq=0), 0), (dict(counts=(0, 0, 0)), 0),
+                                   (dict(counts=(8, 1, 129)), -1), (dict(Nq=0), 0), (dict(counts=(0, 0, 0)), 0), (dict(counts=(8, 0, 0)), 0),
+                                   (dict(counts=(8, 1, 0)), 0), (dict(counts=(8, 0, 5), D=7), 0),
                                    (dict(H=0), 0)])
 def test_packed_refusals(kw, rc):
     assert _packed(**kw) == rc
