@@ -7,8 +7,9 @@
 //   V <= 256, up to 16 alternatives (lp_small_kernel): 16 lanes a row, its logits in
 //     registers.  Each lane sorts its 16 as (value, inverted id) integers and the lanes'
 //     lists meet in four bitonic merges over DPP: no round per alternative.
-//   longer rows (lp_row_kernel): 64 to 1024 threads a row, its logits in registers where
-//     they fit (65536, in 16-bit types 131072), read twice otherwise.  The row's k-th
+//   longer rows (lp_row_kernel): 64 to 1024 threads a row, its logits in registers up to
+//     32768, in 16-bit types 65536; beyond, each 16 bytes' maximum in registers up to 262144
+//     and 524288, so that only those which hold candidates are read again.  The row's k-th
 //     largest logit is at least the k-th largest of 64 maxima over disjoint parts of it,
 //     which a bit-by-bit selection finds; the few logits from that bound on (about k + k^2 /
 //     128 of them for small k) go to LDS and are ranked there by counting.  Ties in number
@@ -19,7 +20,8 @@
 // Bound by the vector ALU next to HBM: a logit takes some 10 operations (two unpackings,
 // maximum, difference, exp2 at a quarter of the rate, two sums).  35328 x 256 bf16 with 8
 // alternatives 13.2 us (26 MB: 5 us of HBM; sorting is half the operations), 2048 x 49999
-// bf16 with 20 64 us (205 MB, 3.2 TB/s), 35000 x 1024 fp32 57 us (2.5 TB/s).
+// bf16 with 20 64 us (205 MB, 3.2 TB/s), 35000 x 1024 fp32 57 us (2.5 TB/s), 500 x 131072
+// fp32 53 us (262 MB, 4.9 TB/s).
 #include "dg_common.h"
 
 namespace dg {
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(256) void lp_small_kernel(const LogprobArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// 64, 256 or 1024 threads a row
+// 64 to 1024 threads a row
 // ---------------------------------------------------------------------------
 
 // The k-th largest (k from 1) of the wave's 64 values, NaN-free: bit by bit on integers
@@ -285,7 +287,7 @@ __device__ __forceinline__ float kth_largest(float v, int k) {
   }
 }
 
-// A row's logits as its threads hold them: its 16-byte vectors, the thread's j-th one
+// A row's logits as its threads hold (HELD) or read them: its 16-byte vectors, the thread's j-th one
 // vector j * NT + tid, and at most one of the logits behind them.  Where a thread has
 // none it holds -inf and an id of V or more.
 template <typename T, int NT, int NV, bool HELD>
@@ -397,16 +399,16 @@ __device__ __forceinline__ void lp_sync() {
 // Waves a SIMD that the registers must allow: two rows of 1024 threads on a CU, whose loads
 // and arithmetic then overlap, as long as a thread's logits leave room (2048 x 49999 bf16:
 // one row on a CU 95 us, one with the next one's loads in flight 87, two 68).
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool HELD>
 constexpr int lp_row_waves() {
-  return NT >= 512 && NV <= 8 ? 8 : 4;
+  return NT >= 512 && NV <= (HELD ? 8 : 32) ? 8 : 4;
 }
 
 // NT threads a row, which meet twice: when every wave's part of the softmax is known, and
 // when the candidates are collected.  Workgroups of 256 threads at least (several rows
 // where NT is 64).
 template <typename T, int NT, int NV, bool HELD>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV>())) void lp_row_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV, HELD>())) void lp_row_kernel(const LogprobArgs a) {
   constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
   constexpr int VE = 16 / (int)sizeof(T);
   __shared__ LpShared<NW, CAP> sh_all[RPB];
@@ -430,33 +432,67 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV>())) v
     for (int c = 1; c < VE; ++c) x0 = fmaxf(x0, v[c]);
     return x0;
   };
-  float vmax[HELD ? NV : 1];  // each vector's maximum
-#pragma unroll
-  for (float& x0 : vmax) x0 = kNegInf;
-  const float single_max = fmaxf(r.single, kNegInf);  // a NaN is no maximum
-  float mine = single_max;
-  r.vectors([&](const float(&v)[VE], int, int j) __attribute__((always_inline)) {
-    const float x0 = vec_max(v);
-    if constexpr (HELD) vmax[j] = x0;
-    mine = fmaxf(mine, x0);
-  });
-  r.forget_unpacked();
-  // s and t of the thread's logits about its own maximum, then of the wave's about the wave's
-  // (-inf alone: about the lowest number, which leaves s at 0)
-  const float own = fmaxf(mine, -3.402823466e38f);
-  float s = 0.f, t = 0.f;
-  if (r.extra < r.V) add_logit(r.single, own, s, t);
-  r.vectors([&](const float(&v)[VE], int, int) __attribute__((always_inline)) {
-#pragma unroll
-    for (int c = 0; c < VE; ++c) add_logit(v[c], own, s, t);
-  });
-  r.forget_unpacked();
   auto about = [](float& s1, float& t1, float m1, float m2) __attribute__((always_inline)) {
     const float d = m1 - m2;  // <= 0; where it overflows, or the factor vanishes, nothing is left
     const float f = __builtin_amdgcn_exp2f(d * kLog2e);
     t1 = f == 0.f ? 0.f : f * __builtin_fmaf(d, s1, t1);
     s1 = f * s1;
   };
+  constexpr bool ONCE = !HELD && NV > 1;
+  constexpr float kLowest = -3.402823466e38f;
+  float vmax[NV];  // each vector's maximum
+#pragma unroll
+  for (float& x0 : vmax) x0 = kNegInf;
+  const float single_max = fmaxf(r.single, kNegInf);  // a NaN is no maximum
+  float mine = single_max;
+  // s and t of the thread's logits about its own maximum, then of the wave's about the wave's
+  // (-inf alone: about the lowest number, which leaves s at 0)
+  float own = fmaxf(mine, kLowest);
+  float s = 0.f, t = 0.f;
+  if constexpr (ONCE) {
+    // kU vectors in flight, each one's logits about the maximum so far
+    constexpr int kU = 4;
+    const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
+#pragma unroll
+    for (int g = 0; g < NV / kU; ++g) {
+      if (g * kU * NT + wave0 >= r.nvec) break;
+      u32x4_t w[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) w[u] = load16(x + (int64_t)min((g * kU + u) * NT + tid, r.nvec - 1) * VE);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int j = g * kU + u;
+        T e[VE];
+        float v[VE];
+        __builtin_memcpy(e, &w[u], 16);
+#pragma unroll
+        for (int c = 0; c < VE; ++c) v[c] = j * NT + tid < r.nvec ? to_f32(e[c]) : kNegInf;
+        vmax[j] = vec_max(v);
+        const float high = fmaxf(own, vmax[j]);
+        about(s, t, own, high);
+        own = high;
+#pragma unroll
+        for (int c = 0; c < VE; ++c) add_logit(v[c], own, s, t);
+      }
+    }
+#pragma unroll
+    for (const float x0 : vmax) mine = fmaxf(mine, x0);
+    if (r.extra < r.V) add_logit(r.single, own, s, t);
+  } else {
+    r.vectors([&](const float(&v)[VE], int, int j) __attribute__((always_inline)) {
+      const float x0 = vec_max(v);
+      if constexpr (HELD) vmax[j] = x0;
+      mine = fmaxf(mine, x0);
+    });
+    r.forget_unpacked();
+    own = fmaxf(mine, kLowest);
+    if (r.extra < r.V) add_logit(r.single, own, s, t);
+    r.vectors([&](const float(&v)[VE], int, int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < VE; ++c) add_logit(v[c], own, s, t);
+    });
+    r.forget_unpacked();
+  }
   float m = wave_max(own);
   about(s, t, own, m);
   s = group_sum_dpp<64>(s);
@@ -518,14 +554,29 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV>())) v
     }
   };
   if (__builtin_amdgcn_ballot_w64(single_max >= bound) != 0) offer(r.single >= bound && r.extra < r.V, r.single, r.extra);
-  r.vectors([&](const float(&v)[VE], int id, int j) __attribute__((always_inline)) {
-    float most;
-    if constexpr (HELD) most = vmax[j];
-    else most = vec_max(v);
-    if (__builtin_amdgcn_ballot_w64(most >= bound) == 0) return;  // the lanes' vectors hold none
+  if constexpr (ONCE) {
+    // the few vectors that hold one are read again
+    uint64_t holds = 0;
 #pragma unroll
-    for (int c = 0; c < VE; ++c) offer(v[c] >= bound && id < r.V, v[c], id + c);
-  });
+    for (int j = 0; j < NV; ++j) holds |= (uint64_t)(__builtin_amdgcn_ballot_w64(vmax[j] >= bound) != 0) << j;
+    for (; holds != 0; holds &= holds - 1) {
+      const int i = __builtin_ctzll(holds) * NT + tid;
+      const u32x4_t w = r.vector(i);
+      T e[VE];
+      __builtin_memcpy(e, &w, 16);
+#pragma unroll
+      for (int c = 0; c < VE; ++c) offer(to_f32(e[c]) >= bound && i < r.nvec, to_f32(e[c]), i * VE + c);
+    }
+  } else {
+    r.vectors([&](const float(&v)[VE], int id, int j) __attribute__((always_inline)) {
+      float most;
+      if constexpr (HELD) most = vmax[j];
+      else most = vec_max(v);
+      if (__builtin_amdgcn_ballot_w64(most >= bound) == 0) return;  // the lanes' vectors hold none
+#pragma unroll
+      for (int c = 0; c < VE; ++c) offer(v[c] >= bound && id < r.V, v[c], id + c);
+    });
+  }
   lp_sync<NT>();
   const int n = sh.count;
   if (n >= top && n <= CAP) {
@@ -698,9 +749,9 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
 #undef DG_LP
     return check_launch("lp_small_kernel");
   }
-  // The least threads that hold the row, 16 to 64 logits each (128 in 16-bit types from
-  // 65537 on).  More threads a row gain little where rows are few (256 x 4000, 64 -> 1024
-  // threads: 9.7 -> 8.2 us) and lose elsewhere (512 x 2000: 8.6 -> 11.0).
+  // The least threads that hold the row, 16 to 64 logits each.  More threads a row gain
+  // little where rows are few (256 x 4000, 64 -> 1024 threads: 9.7 -> 8.2 us) and lose
+  // elsewhere (512 x 2000: 8.6 -> 11.0).
 #define DG_LP_ROW(NT, PER)                                                                                           \
   do {                                                                                                               \
     constexpr int kRows = (NT) < 256 ? 256 / (NT) : 1;                                                               \
@@ -714,12 +765,23 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
   if (a.V <= 32 * 256) DG_LP_ROW(256, 32);
   if (a.V <= 64 * 256) DG_LP_ROW(256, 64);
   if (a.V <= 64 * 512) DG_LP_ROW(512, 64);
-  if (a.V <= 64 * 1024) DG_LP_ROW(1024, 64);
   if constexpr (sizeof(T) == 2)
-    if (a.V <= 128 * 1024) DG_LP_ROW(1024, 128);
+    if (a.V <= 64 * 1024) DG_LP_ROW(1024, 64);
 #undef DG_LP_ROW
-  hipLaunchKernelGGL((lp_row_kernel<T, 1024, 1, false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
-  return check_launch("lp_long_kernel");
+  // Longer rows are read once, as far as the vectors' maxima fit, and the vectors that hold
+  // candidates again: fp32 from 32769 logits on, 16-bit types from 65537.  us held in 1024
+  // threads' registers, or read three times, / read once: 500 x 65000 fp32 38 / 33, 500 x
+  // 131072 bf16 47 / 37, fp32 112 / 53, 300 x 200000 fp32 107 / 44; 500 x 31000 fp32 21 / 23,
+  // 2048 x 49999 bf16 66 / 80.
+#define DG_LP_LONG(NV, NAME)                                                                                \
+  do {                                                                                                      \
+    hipLaunchKernelGGL((lp_row_kernel<T, 1024, (NV), false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);    \
+    return check_launch(NAME);                                                                              \
+  } while (0)
+  if (a.V / VE <= 32 * 1024) DG_LP_LONG(32, "lp_once_kernel");
+  if (a.V / VE <= 64 * 1024) DG_LP_LONG(64, "lp_once_kernel");
+  DG_LP_LONG(1, "lp_long_kernel");
+#undef DG_LP_LONG
 }
 
 }  // namespace

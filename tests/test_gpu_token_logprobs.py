@@ -1,6 +1,8 @@
 """Log probabilities of given tokens, entropy and alternatives (dg_logprobs.hip) against
 float64."""
 
+import math
+
 import pytest
 import torch
 
@@ -46,7 +48,7 @@ def _check(x, ids, r, dtype, top):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
 @pytest.mark.parametrize("M,V", [(1, 1), (3, 2), (5, 63), (7, 64), (4, 65), (33, 256), (9, 257), (130, 1024), (3, 1025),
-                                 (6, 4099), (2, 50001), (1, 131072)])
+                                 (6, 4099), (2, 50001), (1, 131072), (3, 65600), (2, 140003), (1, 262149), (1, 524291), (1, 600000)])
 @pytest.mark.parametrize("top", [0, 1, 5, 64])
 def test_matches_float64(dev, dtype, M, V, top):
     top = min(top, V)
@@ -57,7 +59,7 @@ def test_matches_float64(dev, dtype, M, V, top):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("V", [64, 256, 1000, 20000])
+@pytest.mark.parametrize("V", [64, 256, 1000, 20000, 100003, 300000])
 @pytest.mark.parametrize("order", ["ascending", "descending", "equal", "two", "few_finite"])
 def test_orders_and_ties(dev, dtype, V, order):
     """Rows sorted either way, of one value, of two, and with all but five logits -inf:
@@ -82,7 +84,7 @@ def test_orders_and_ties(dev, dtype, V, order):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("V", [256, 5000])
+@pytest.mark.parametrize("V", [256, 5000, 70000, 150001])
 def test_rows_that_are_no_distribution(dev, dtype, V):
     """NaN, +inf and -inf alone give NaN; their neighbours are untouched."""
     g = torch.Generator(device=dev).manual_seed(1)
@@ -113,6 +115,20 @@ def test_extreme_values(dev):
     h = -torch.where(logs.exp() > 0, logs.exp() * logs, 0.0).sum(-1)
     assert bool(((r.entropy.double() - h).abs() <= 1e-5).all())
     assert r.top_ids.tolist() == [[2, 1, 0], [0, 1, 2], [0, 1, 2], [0, 2, 1]]
+
+
+@pytest.mark.parametrize("V", [3000, 40000, 140000])
+def test_extreme_values_in_long_rows(dev, V):
+    """Maxima that grow from the type's lowest value to its highest over a row: earlier sums
+    vanish, differences overflow."""
+    x = (torch.linspace(-1, 1, V, dtype=torch.float64) * 3.4e38).float().to(dev)  # in fp32 the step overflows
+    rows = torch.stack([x, x.flip(0), torch.full_like(x, torch.finfo(torch.float32).min), x * 1e-37])
+    ids = torch.tensor([V - 1, 0, 7, V - 1], device=dev)
+    r = token_logprobs(rows, ids, 3)
+    assert r.logprobs[:2].tolist() == [0.0, 0.0] and r.entropy[:2].tolist() == [0.0, 0.0]
+    assert r.top_ids.tolist() == [[V - 1, V - 2, V - 3], [0, 1, 2], [0, 1, 2], [V - 1, V - 2, V - 3]]
+    assert abs(float(r.logprobs[2]) + math.log(V)) <= 1e-5 and abs(float(r.entropy[2]) - math.log(V)) <= 1e-4
+    _check(rows[3:], ids[3:], token_logprobs(rows[3:], ids[3:], 3), "f32", 3)
 
 
 def test_ids_outside_the_vocabulary(dev):
