@@ -325,7 +325,7 @@ def test_tree_masks_of_each_row_and_chains(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
-@pytest.mark.parametrize("D", [16, 64, 128, 40])
+@pytest.mark.parametrize("D", [16, 64, 128, 40, 65, 200, 300])
 @pytest.mark.parametrize("Tcap", [128, 3000])
 def test_tree_hidden_positions_stay_hidden(dev, dtype, D, Tcap):
     """NaN and infinities behind a row's tokens and in tokens that others do not see;
@@ -448,6 +448,19 @@ def test_tree_of_any_shape(dev, dtype, D, N, G):
         y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
         assert _native.last_kernel() in ("seq_tile_kernel", "seq_join_kernel")
         _check_tree(q, k, v, y, lens, parents, dtype)
+
+
+@pytest.mark.parametrize("dtype,D", [("f32", 16), ("bf16", 64), ("f16", 128), ("bf16", 65), ("f64", 16)])
+@pytest.mark.parametrize("G", [33, 130])
+def test_wide_groups(dev, dtype, D, G):
+    """A query's heads lie in several tiles, and a tile holds parts of two queries' heads."""
+    q_lens, k_lens = [1, 5, 3], [70, 5, 300]
+    q, k, v = _packed_case(dev, q_lens, k_lens, G, 1, D, TDT[dtype], seed=G)
+    _check_packed(q, k, v, attention_packed(q, k, v, PackedLayout(q_lens, k_lens, group=G)), q_lens, k_lens, dtype)
+    q, k, v = _tree_case(dev, 2, 3, G, 1, 400, D, TDT[dtype], seed=G)
+    parents = [-1, 0, 0]
+    y = attention_tree(q, k, v, torch.tensor([0, 397], dtype=torch.int32, device=dev), tree_masks(parents))
+    _check_tree(q, k, v, y, [0, 397], parents, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f64"])
