@@ -16,8 +16,13 @@
 //   O^T (D x 32 rows)      += V^T P^T   P^T is S^T's accumulator registers as they are
 //
 // 16-bit data: v_mfma_f32_32x32x16_{bf16,f16}, V^T through the transposing LDS read;
-// probabilities are rounded to the data's type once, for the second product alone (the
-// row sums add them in fp32).  fp32: v_mfma_f32_32x32x2_f32 throughout.  Lane l (half hh =
+// probabilities go into the second product as two terms of the data's type, 16 bits (bf16)
+// and 20 (fp16) of them, so that an output is rounded once, as it is stored.  One term was
+// 1.4 - 1.5 times as far from the exact result (bf16 2.3e-3 of it, now 1.6e-3), and faster:
+// us, one term / two: 6 sequences of up to 7168 tokens, 16 heads on 4 of 128, bf16 490 / 652;
+// 64 of 100 - 2048, 8 heads of 64, 192 / 237; 16 trees of 24 over up to 7168, 16 heads on 4 of
+// 128, 43 / 51; one token for each of 64 caches of up to 4096 the same.
+// fp32: v_mfma_f32_32x32x2_f32 throughout.  Lane l (half hh =
 // l / 32) holds, in register r of a 32x32 block, row 8 (r / 4) + 4 hh + r % 4 of column
 // l % 32, its row of the batch.
 //
@@ -46,12 +51,26 @@ typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 sbf16x8_t;
 typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 sf16x8_t;
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 
+// Two probabilities as pairs of T, the leading bits and the rest.  The leading ones are cut
+// off, not rounded, and the rest of one that is not 0 never vanishes (its last bit stays), so
+// both are positive and a value of +-inf times either is +-inf, never 0 * inf.
+struct ProbPairs {
+  uint32_t high, low;
+};
+
 template <typename T>
 struct SeqMma;
 template <>
 struct SeqMma<bf16_t> {
   using vec8 = sbf16x8_t;
   static constexpr uint32_t kExp = 0x7f80u;
+  __device__ static ProbPairs split(float a, float b) {
+    constexpr float kPast = 1.0f + 0x1p-23f;
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    const float la = __builtin_fmaf(a, kPast, -__uint_as_float(ua & 0xffff0000u));
+    const float lb = __builtin_fmaf(b, kPast, -__uint_as_float(ub & 0xffff0000u));
+    return {__builtin_amdgcn_perm(ub, ua, 0x07060302u), pack_pair<bf16_t>(la, lb)};
+  }
   __device__ static floatx16_t mma(vec8 a, vec8 b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -60,6 +79,17 @@ template <>
 struct SeqMma<f16_t> {
   using vec8 = sf16x8_t;
   static constexpr uint32_t kExp = 0x7c00u;
+  __device__ static ProbPairs split(float a, float b) {
+    const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    float la, lb;  // a, b less their halves of h, one instruction each
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(la) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(lb) : "v"(h), "v"(b));
+    const u16x2_t l = __builtin_bit_cast(u16x2_t, __builtin_amdgcn_cvt_pkrtz(la, lb));
+    uint32_t ones = 0x00010001u;
+    asm("" : "+s"(ones));  // the minimum of unknown numbers: one v_pk_min_u16, no comparisons
+    const u16x2_t some = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, h), __builtin_bit_cast(u16x2_t, ones));
+    return {h, __builtin_bit_cast(uint32_t, __builtin_elementwise_max(l, some))};
+  }
   __device__ static floatx16_t mma(vec8 a, vec8 b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -449,13 +479,14 @@ void seq_mfma_kernel(const SeqArgs a) {
           for (int nb = 0; nb < NB; ++nb) o[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[nb], s[mb][c], o[nb], 0, 0, 0);
         }
       } else {
-        vec8 pf[2];
+        vec8 ph[2], pl[2];
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
-          uint32_t w[4];
+          ProbPairs w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = pack_pair<T>(s[mb][8 * c2 + 2 * i], s[mb][8 * c2 + 2 * i + 1]);
-          pf[c2] = __builtin_bit_cast(vec8, u32x4_t{w[0], w[1], w[2], w[3]});
+          for (int i = 0; i < 4; ++i) w[i] = M::split(s[mb][8 * c2 + 2 * i], s[mb][8 * c2 + 2 * i + 1]);
+          ph[c2] = __builtin_bit_cast(vec8, u32x4_t{w[0].high, w[1].high, w[2].high, w[3].high});
+          pl[c2] = __builtin_bit_cast(vec8, u32x4_t{w[0].low, w[1].low, w[2].low, w[3].low});
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -463,7 +494,9 @@ void seq_mfma_kernel(const SeqArgs a) {
           for (int c2 = 0; c2 < 2; ++c2) {
             const uint2 lo = lds_read_tr16(vb + 16 * c2 * D + voff[0][nb]);
             const uint2 hi = lds_read_tr16(vb + 16 * c2 * D + voff[1][nb]);
-            o[nb] = M::mma(__builtin_bit_cast(vec8, u32x4_t{lo.x, lo.y, hi.x, hi.y}), pf[c2], o[nb]);
+            const vec8 vf = __builtin_bit_cast(vec8, u32x4_t{lo.x, lo.y, hi.x, hi.y});
+            o[nb] = M::mma(vf, ph[c2], o[nb]);
+            o[nb] = M::mma(vf, pl[c2], o[nb]);
           }
       }
     }

@@ -1,0 +1,87 @@
+"""How exact packed and tree attention are: outputs within their own rounding of the 64-bit
+ones, whatever the other rows of a tile hold."""
+
+import pytest
+import torch
+
+from diff_gpt import _native
+from diff_gpt.model.packed import PackedLayout, attention_packed
+from diff_gpt.model.tree import attention_tree, tree_masks
+from seq_cases import HALF, TDT, attend64, some_tree, tree_seen
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+# A probability's two terms, of 8 (bf16) and 11 (fp16) bits each: the first is cut off
+# (2^-7, 2^-10 of it are left), the second off by half a step of that (2^-8) or a whole
+# one (2^-10).
+TERMS = {"bf16": 2.0**-15, "f16": 2.0**-20}
+
+
+def _causal(n, t, dev):
+    return torch.arange(t, device=dev)[None] <= torch.arange(n, device=dev)[:, None] + (t - n)
+
+
+def _rounded_once(y, ref, a, dtype, keys, vmax):
+    """The output's one rounding beside fp32 arithmetic's 1e-5 of the row's largest sum of
+    p |v|, and what two terms leave of the probabilities.  fp16's second term has steps of
+    2^-24 beside a largest probability of at least 1."""
+    tol = HALF[dtype] * ref.abs() + (1e-5 + TERMS[dtype]) * a.amax(-1, keepdim=True)
+    if dtype == "f16":
+        tol = tol + keys * 2.0**-24 * vmax + 2.0**-25
+    off = (y.double() - ref).abs()
+    assert bool((off <= tol).all()), (int((off > tol).sum()), float((off - tol).max()))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 32, 64, 80, 128, 256])
+@pytest.mark.parametrize("copies", [1, 4, 24])
+def test_packed_is_rounded_once(dev, dtype, D, copies):
+    """In each of the three workgroup shapes."""
+    q_lens = [130, 5, 64, 200, 1, 128, 33, 300] * copies
+    k_lens = [130, 40, 64, 333, 1, 100, 33, 300] * copies
+    H = 4
+    g = torch.Generator(device=dev).manual_seed(D)
+    q, k, v = (torch.randn(n, H, D, generator=g, device=dev).to(TDT[dtype]) for n in (sum(q_lens), sum(k_lens), sum(k_lens)))
+    y = attention_packed(q, k, v, PackedLayout(q_lens, k_lens))
+    assert _native.last_kernel() == f"seq_mfma_packed_{32 if copies == 1 else 64 if copies == 4 else 128}"
+    a = b = 0
+    for n, t in list(zip(q_lens, k_lens))[-8:]:
+        a, b = a + n, b + t
+    a, b = q.size(0) - a, k.size(0) - b
+    for n, t in list(zip(q_lens, k_lens))[-8:]:
+        ref, mag = attend64(q[a : a + n], k[b : b + t], v[b : b + t], _causal(n, t, dev))
+        _rounded_once(y[a : a + n], ref, mag, dtype, t, float(v.abs().max()))
+        a, b = a + n, b + t
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+@pytest.mark.parametrize("N,G,Tcap", [(1, 4, 900), (31, 1, 200), (24, 4, 7000), (64, 2, 20000)])
+def test_trees_are_rounded_once(dev, dtype, D, N, G, Tcap):
+    B = 3
+    g = torch.Generator(device=dev).manual_seed(N)
+    q = torch.randn(B, N, 2 * G, D, generator=g, device=dev).to(TDT[dtype])
+    k, v = (torch.randn(B, Tcap, 2, D, generator=g, device=dev).to(TDT[dtype]) for _ in range(2))
+    lens = [0, Tcap // 3, Tcap - N]
+    parents = some_tree(N, seed=N)
+    y = attention_tree(q, k, v, torch.tensor(lens, dtype=torch.int32, device=dev), tree_masks(parents))
+    for b, n in enumerate(lens):
+        seen = torch.cat([torch.ones(N, n, dtype=torch.bool), tree_seen(parents)], dim=1).to(dev)
+        ref, mag = attend64(q[b], k[b, : n + N], v[b, : n + N], seen)
+        _rounded_once(y[b], ref, mag, dtype, n + N, float(v.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_infinite_values_of_even_weights(dev, dtype, D):
+    """Weights of exactly 1, nothing beyond their leading bits, on infinite values that every
+    row of a later tile sees."""
+    n = 300
+    q, k = (torch.zeros(n, 2, D, dtype=TDT[dtype], device=dev) for _ in range(2))
+    v = torch.ones(n, 2, D, dtype=TDT[dtype], device=dev)
+    v[5] = INF
+    y = attention_packed(q, k, v, PackedLayout([n]))
+    assert bool((y[:5] == 1).all()) and bool((y[5:] == INF).all())
+    v[5] = -INF
+    y = attention_tree(q[None, :9], k[None], v[None], 280)
+    assert bool((y == -INF).all())
