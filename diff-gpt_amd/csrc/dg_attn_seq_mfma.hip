@@ -26,9 +26,10 @@
 // l / 32) holds, in register r of a 32x32 block, row 8 (r / 4) + 4 hh + r % 4 of column
 // l % 32, its row of the batch.
 //
-// The exponent's offset is a whole number of log2 units, raised only where a row's maximum
-// outgrows it by more than kLazyLog2: rescaling by a power of two is exact, so a row's bits
-// do not depend on when its neighbours in the tile made it rescale.  Scores are masked
+// The exponent's offset is a whole number of log2 units, raised only where the row's own
+// maximum outgrows it by more than kLazyLog2 (an offset that followed the neighbours' would
+// move the grid on which the exponents are rounded): rescaling by a power of two is exact,
+// and a row's bits depend on no other row of its tile.  Scores are masked
 // only in key blocks that some row of the wave sees part of; values there that are not
 // finite are kept out of the product (clean_stage).
 //
@@ -435,8 +436,9 @@ void seq_mfma_kernel(const SeqArgs a) {
 #pragma unroll
       for (int r = mb == 0 ? 1 : 0; r < 16; ++r) mt = fmaxf(mt, s[mb][r]);
     mt = half_pair_max(mt) * a.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(mt > mo + kLazyLog2) != 0) {
-      const float mn = mt > mo ? fmaxf(__builtin_floorf(mt), mo) : mo;
+    const bool raise = mt > mo + kLazyLog2;  // the row's own affair, whatever its neighbours' scores
+    if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+      const float mn = raise ? __builtin_floorf(mt) : mo;
       // no key before: l is 0, and o what clean_stage added
       const float f = mo == kNone ? 1.f : __builtin_amdgcn_exp2f(mo - mn);
       mo = mn;

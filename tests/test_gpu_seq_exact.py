@@ -85,3 +85,40 @@ def test_infinite_values_of_even_weights(dev, dtype, D):
     v[5] = -INF
     y = attention_tree(q[None, :9], k[None], v[None], 280)
     assert bool((y == -INF).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("copies,at", [(1, 40), (1, 200), (12, 70), (12, 200), (100, 70), (100, 200)])
+def test_a_large_key_leaves_the_rows_that_do_not_see_it(dev, dtype, D, copies, at):
+    """A finite key whose scores raise the maximum of the rows that see it by hundreds: the
+    other rows of the tile keep their bits."""
+    n, H = 256, 2
+    g = torch.Generator(device=dev).manual_seed(D + at)
+    q, k, v = (torch.randn(copies * n, H, D, generator=g, device=dev).to(TDT[dtype]) for _ in range(3))
+    lay = PackedLayout([n] * copies)
+    clean = attention_packed(q, k, v, lay)
+    k[at::n] = 400 * q[at + 1 :: n].sign()
+    y = attention_packed(q, k, v, lay)
+    hidden = torch.arange(copies * n, device=dev) % n < at
+    assert torch.equal(y[hidden], clean[hidden])
+    assert not torch.equal(y[~hidden], clean[~hidden])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N,Hkv,G,Tcap", [(20, 2, 1, 200), (64, 4, 2, 1300), (48, 2, 8, 9000)])
+def test_a_large_key_of_another_branch(dev, dtype, N, Hkv, G, Tcap):
+    """The same of a token that only its own branch of the tree sees."""
+    B, D = 40, 64
+    g = torch.Generator(device=dev).manual_seed(N)
+    q = torch.randn(B, N, Hkv * G, D, generator=g, device=dev).to(TDT[dtype])
+    k, v = (torch.randn(B, Tcap, Hkv, D, generator=g, device=dev).to(TDT[dtype]) for _ in range(2))
+    lens = torch.tensor([(97 * b) % (Tcap - N) + 1 for b in range(B)], dtype=torch.int32, device=dev)
+    masks = tree_masks([-1] + [0, 1] * ((N - 1) // 2) + [0] * ((N - 1) % 2))
+    clean = attention_tree(q, k, v, lens, masks)
+    for b, n in enumerate(lens.tolist()):
+        k[b, n + 1] = 400 * q[b, 1, ::G].sign()  # token 1: seen by itself and those that hang on it
+    y = attention_tree(q, k, v, lens, masks)
+    hidden = ((masks >> 1) & 1) == 0
+    assert torch.equal(y[:, hidden], clean[:, hidden])
+    assert not torch.equal(y[:, ~hidden], clean[:, ~hidden])
