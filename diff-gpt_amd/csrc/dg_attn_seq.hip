@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void seq_tile_kernel(const SeqArgs a) {
     end = i + p.off + 1;
     first_open = p.row0 / a.G + p.off + 1;
   }
-  A o[NCH][NV][VW], m = neg_inf<A>(), l = (A)0;
+  A o[NCH][NV][VW], m = neg_inf<A>(), l = (A)0, lc = (A)0;
 #pragma unroll
   for (int c = 0; c < NCH; ++c)
 #pragma unroll
@@ -179,12 +179,15 @@ __global__ __launch_bounds__(256) void seq_tile_kernel(const SeqArgs a) {
     const A base = mn == neg_inf<A>() ? (A)0 : mn;
     m = mn;
     l *= f;
+    lc *= f;
+    A sum = (A)0;
 #pragma unroll
     for (int j = 0; j < KPL; ++j) {
       const A w = S::exp(s[j] - base);  // NaN for a NaN score, and the row with it
-      if (seen[j]) l += w;
+      if (seen[j]) sum += w;
       ps[row * PS + ln + LPR * j] = seen[j] ? w : (A)-1;  // the row's own lanes read it, after the barriers below
     }
+    add_rounded(l, lc, sum);
     if (f != (A)1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c)
@@ -226,6 +229,7 @@ __global__ __launch_bounds__(256) void seq_tile_kernel(const SeqArgs a) {
       else add(std::false_type{});
     }
   }
+  l -= lc;
 #pragma unroll
   for (int x = 1; x < LPR; x <<= 1) l += __shfl_xor(l, x, 64);
   if (row >= p.rows) return;

@@ -275,7 +275,9 @@ void seq_mfma_kernel(const SeqArgs a) {
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[nb][r] = 0.f;
-  float mo = kNone, l = 0.f;  // the exponent's offset (log2 units, whole) and this lane's sum
+  // the exponent's offset (log2 units, whole) and this lane's sum, whose last addition's
+  // rounding is lc
+  float mo = kNone, l = 0.f, lc = 0.f;
 
   // per-lane parts of the transposing reads of V (16-bit)
   const int g16 = lane >> 4, t16 = lane & 15;
@@ -443,6 +445,7 @@ void seq_mfma_kernel(const SeqArgs a) {
       const float f = mo == kNone ? 1.f : __builtin_amdgcn_exp2f(mo - mn);
       mo = mn;
       l *= f;
+      lc *= f;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -452,11 +455,13 @@ void seq_mfma_kernel(const SeqArgs a) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const T* vb = Vs + 32 * mb * D;
+      float sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[mb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][r], a.scale_log2, -moff));
-        l += s[mb][r];
+        sum += s[mb][r];
       }
+      add_rounded(l, lc, sum);
       if constexpr (F32) {
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -517,7 +522,7 @@ void seq_mfma_kernel(const SeqArgs a) {
     if (k0 + kstep < wend) compute(kv1, k0 + kstep);
     stage_ready();
   }
-  l = half_pair_sum(l);
+  l = half_pair_sum(l - lc);
 
   // ---- the key groups' states joined ---------------------------------------------------
   if constexpr (KS > 1) {

@@ -1,6 +1,8 @@
 """How exact packed and tree attention are: outputs within their own rounding of the 64-bit
 ones, whatever the other rows of a tile hold."""
 
+import math
+
 import pytest
 import torch
 
@@ -122,3 +124,34 @@ def test_a_large_key_of_another_branch(dev, dtype, N, Hkv, G, Tcap):
     hidden = ((masks >> 1) & 1) == 0
     assert torch.equal(y[:, hidden], clean[:, hidden])
     assert not torch.equal(y[:, ~hidden], clean[:, ~hidden])
+
+
+@pytest.mark.parametrize("D", [16, 64, 128, 40, 65, 256])
+@pytest.mark.parametrize("far", [25.05, 24.4, 17.3])
+@pytest.mark.parametrize("tree", [True, False])
+def test_faint_keys_count_in_a_long_rows_sum(dev, D, far, tree):
+    """One key 2^far times as likely as each of 100000 others, in fp32: the others' weights,
+    each below the last bit of the row's sum or a little above it, make up 100000 2^-far
+    of the one's.  The one's value is held to fp32 attention's 1e-5; the others' is a sum of
+    100000 equal terms in fp32, each of whose additions may be off by half a step of the sum
+    the same way: 100000 2^-24 of it."""
+    n = 100000
+    q = torch.zeros(1, 4, 1, D, device=dev)
+    q[..., 0] = 1.0
+    k = torch.zeros(1, n + 4, 1, D, device=dev)
+    k[:, :, :, 0] = -far * math.log(2) * D**0.5
+    k[:, 77] = 0.0
+    v = torch.zeros(1, n + 4, 1, D, device=dev)
+    v[:, 77, :, 0] = 1.0
+    v[..., 1] = 1.0
+    v[:, 77, :, 1] = 0.0
+    if tree:
+        y = attention_tree(q, k, v, n, tree_masks([-1] * 4))[0, :, 0]
+    else:
+        y = attention_packed(q[0], k[0], v[0], PackedLayout([4], [n + 4]))[:, 0]
+    for i in range(4):
+        others = (n - 1 + (1 if tree else i + 1)) * math.exp(float(k[0, 0, 0, 0].double()) * D**-0.5)
+        want = torch.tensor([1 / (1 + others), others / (1 + others)], dtype=torch.float64, device=dev)
+        off = (y[i, :2].double() - want).abs().tolist()
+        assert off[0] <= 1e-5 and off[1] <= 1e-5 + n * 2.0**-24 * float(want[1]), (y[i, :2].tolist(), want.tolist())
+        assert not bool(y[i, 2:].any())
