@@ -65,6 +65,7 @@ template <>
 struct SeqMma<bf16_t> {
   using vec8 = sbf16x8_t;
   static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr float kLift = 0.f;
   __device__ static ProbPairs split(float a, float b) {
     constexpr float kPast = 1.0f + 0x1p-23f;
     const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
@@ -80,6 +81,9 @@ template <>
 struct SeqMma<f16_t> {
   using vec8 = sf16x8_t;
   static constexpr uint32_t kExp = 0x7c00u;
+  // fp16's steps end at 2^-24, and a long row's faint keys count: weights are 2^7 times what
+  // they are in the other types, from 2^7 (a row's largest) to 2^15 at most (kLazyLog2)
+  static constexpr float kLift = 7.f;
   __device__ static ProbPairs split(float a, float b) {
     const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     float la, lb;  // a, b less their halves of h, one instruction each
@@ -99,6 +103,7 @@ template <>
 struct SeqMma<float> {
   using vec8 = float;  // unused
   static constexpr uint32_t kExp = 0x7f800000u;
+  static constexpr float kLift = 0.f;
 };
 
 // Workgroup shapes.  Two stages of K and V for every key group: up to 128 KB of LDS (one
@@ -451,7 +456,8 @@ void seq_mfma_kernel(const SeqArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[nb][r] *= f;
     }
-    const float moff = mo == kNone ? 0.f : mo;  // no key yet: every score here is -inf
+    // sums and outputs of all a row's parts are lifted alike
+    const float moff = mo == kNone ? 0.f : mo - M::kLift;  // no key yet: every score here is -inf
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const T* vb = Vs + 32 * mb * D;

@@ -155,3 +155,36 @@ def test_faint_keys_count_in_a_long_rows_sum(dev, D, far, tree):
         off = (y[i, :2].double() - want).abs().tolist()
         assert off[0] <= 1e-5 and off[1] <= 1e-5 + n * 2.0**-24 * float(want[1]), (y[i, :2].tolist(), want.tolist())
         assert not bool(y[i, 2:].any())
+
+
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+@pytest.mark.parametrize("far", [25.05, 24.4, 17.3])
+@pytest.mark.parametrize("tree", [True, False])
+def test_faint_keys_of_a_long_row_keep_their_weight(dev, D, far, tree):
+    """One key 2^far times as likely as each of 100000 others, in fp16: the others' weight
+    is 100000 2^-far of its, all of one value.  A weight is off by at most one step of
+    fp16's second term, 2^-24 beside a largest one of 2^7: 100000 2^-31 in all, 5e-5; the
+    others' value is a sum of 100000 terms in fp32, as above."""
+    n = 100000
+    q = torch.zeros(1, 4, 1, D, dtype=torch.float16, device=dev)
+    q[..., 0] = 16.0
+    k = torch.zeros(1, n + 4, 1, D, dtype=torch.float16, device=dev)
+    # scores -k far log(2): k's own fp16 rounding moves far alike in the answer
+    k[:, :, :, 0] = -far * math.log(2) * D**0.5 / 16.0
+    k[:, 77] = 0.0
+    v = torch.zeros(1, n + 4, 1, D, dtype=torch.float16, device=dev)
+    v[:, 77, :, 0] = 1.0
+    v[..., 1] = 1.0
+    v[:, 77, :, 1] = 0.0
+    if tree:
+        y = attention_tree(q, k, v, n, tree_masks([-1] * 4))[0, :, 0]
+    else:
+        y = attention_packed(q[0], k[0], v[0], PackedLayout([4], [n + 4]))[:, 0]
+    s = float(k[0, 0, 0, 0].double()) * 16.0 * D**-0.5
+    for i in range(4):
+        others = (n - 1 + (1 if tree else i + 1)) * math.exp(s)
+        want = torch.tensor([1 / (1 + others), others / (1 + others)], dtype=torch.float64, device=dev)
+        tol = 2.0**-11 * want + 5e-5
+        tol[1] += n * 2.0**-24 * want[1]
+        assert bool(((y[i, :2].double() - want).abs() <= tol).all()), (y[i, :2].tolist(), want.tolist())
+        assert not bool(y[i, 2:].any())
