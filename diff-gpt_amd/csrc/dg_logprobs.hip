@@ -11,10 +11,14 @@
 //     32768, in 16-bit types 65536; beyond, each 16 bytes' maximum in registers up to 262144
 //     and 524288, so that only those which hold candidates are read again.  The row's k-th
 //     largest logit is at least the k-th largest of 64 maxima over disjoint parts of it,
-//     which a bit-by-bit selection finds; the few logits from that bound on (about k + k^2 /
-//     128 of them for small k) go to LDS and are ranked there by counting.  Ties in number
-//     beyond the buffer are taken in id order from the row; what neither takes (NaN among
-//     the first k, thousands of logits above the bound) goes one alternative after the other.
+//     which a bit-by-bit selection finds; the few logits from that bound on (about 64 (1/64 +
+//     1/63 + ...), k terms: k + k^2 / 128 for small k, 300 for 64) go to LDS and are ranked
+//     there by counting.  Where they overflow the buffer (256 logits for a row of one wave,
+//     which half the rows do at 64 alternatives), the k-th largest of those it holds is the
+//     next bound, and the row is looked through again (4096 x 4096 fp32 with 64 alternatives
+//     66 us; one alternative after the other 2012).  Ties in number beyond the buffer are taken in id order from the row; what
+//     neither takes (NaN among the first k, long staircases of ties) goes one alternative
+//     after the other.
 //   fp64: a wavefront a row, one pass per alternative.
 //
 // Bound by the vector ALU next to HBM: a logit takes some 10 operations (two unpackings,
@@ -254,15 +258,31 @@ __global__ __launch_bounds__(256) void lp_small_kernel(const LogprobArgs a) {
 // 64 to 1024 threads a row
 // ---------------------------------------------------------------------------
 
-// The k-th largest (k from 1) of the wave's 64 values, NaN-free: bit by bit on integers
-// that sort as the values do.
+// Integers that sort as the values of T do, 16-bit ones in the upper half, and back.
+template <typename T>
+__device__ __forceinline__ uint32_t sort_bits(float v) {
+  uint32_t u;
+  if constexpr (sizeof(T) == 4) u = __float_as_uint(v);
+  else u = (uint32_t)from_f32<T>(v).bits << 16;  // v is a value of T
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+template <typename T>
+__device__ __forceinline__ float from_sort_bits(uint32_t u) {
+  const uint32_t bits = (u & 0x80000000u) ? u & 0x7fffffffu : ~u;
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(bits);
+  } else {
+    T r;
+    r.bits = (uint16_t)(bits >> 16);
+    return to_f32(r);
+  }
+}
+
+// The k-th largest (k from 1) of the wave's 64 values, NaN-free: bit by bit.
 template <typename T>
 __device__ __forceinline__ float kth_largest(float v, int k) {
   constexpr int BITS = 8 * (int)sizeof(T);
-  uint32_t u;
-  if constexpr (BITS == 32) u = __float_as_uint(v);
-  else u = (uint32_t)from_f32<T>(v).bits << 16;  // v is a value of T
-  u = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  const uint32_t u = sort_bits<T>(v);
   uint64_t alive = ~0ull;
   uint32_t kth = 0;
 #pragma unroll
@@ -277,14 +297,24 @@ __device__ __forceinline__ float kth_largest(float v, int k) {
       alive &= ~ones;
     }
   }
-  const uint32_t bits = (kth & 0x80000000u) ? kth & 0x7fffffffu : ~kth;
-  if constexpr (BITS == 32) {
-    return __uint_as_float(bits);
-  } else {
-    T r;
-    r.bits = (uint16_t)(bits >> 16);
-    return to_f32(r);
+  return from_sort_bits<T>(kth);
+}
+
+// The k-th largest of n values in LDS, NaN-free, the same way: the largest number that k
+// of them reach.
+template <typename T>
+__device__ __forceinline__ float kth_largest_of(const float* v, int n, int k, int lane) {
+  uint32_t kth = 0;
+#pragma unroll 1
+  for (int b = 31; b >= 32 - 8 * (int)sizeof(T); --b) {
+    const uint32_t trial = kth | (1u << b);
+    int reach = 0;
+#pragma unroll 4
+    for (int c = 0; c < n; c += 64)
+      reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(c + lane < n && sort_bits<T>(v[min(c + lane, n - 1)]) >= trial));
+    if (reach >= k) kth = trial;
   }
+  return from_sort_bits<T>(kth);
 }
 
 // A row's logits as its threads hold (HELD) or read them: its 16-byte vectors, the thread's j-th one
@@ -410,6 +440,7 @@ constexpr int lp_row_waves() {
 template <typename T, int NT, int NV, bool HELD>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV, HELD>())) void lp_row_kernel(const LogprobArgs a) {
   constexpr int NW = NT / 64, RPB = NT < 256 ? 256 / NT : 1, CAP = NT == 64 ? 256 : 1024;
+  constexpr int kRounds = 8;  // times a bound is raised at most: each leaves some top / CAP of too many
   constexpr int VE = 16 / (int)sizeof(T);
   __shared__ LpShared<NW, CAP> sh_all[RPB];
   LpShared<NW, CAP>& sh = sh_all[RPB == 1 ? 0 : threadIdx.x / NT];
@@ -526,7 +557,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV, HELD>
 
   int64_t* ids = a.top_ids + row * top;
   float* lps = static_cast<float*>(a.top_logprob) + row * top;
-  const float bound = kth_largest<T>(part, top);
+  float bound = kth_largest<T>(part, top);
   // a logit that passes, into LDS as far as there is room; the wave's lanes together
   auto offer = [&](bool in, float v, int id) __attribute__((always_inline)) {
     const uint64_t b = __builtin_amdgcn_ballot_w64(in);
@@ -542,6 +573,29 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV, HELD>
     }
   };
   auto rank = [&](int n) __attribute__((always_inline)) {
+    if constexpr (NW == 1) {
+      // one wave compares many with each other for long (n^2 / 64 times): the first `top` of
+      // them, and their ties, move to the front
+      if (n > 128) {
+        const float last = kth_largest_of<T>(sh.cand_v, n, top, lane);
+        int kept = 0;
+        for (int c = 0; c < n; c += 64) {
+          const float v = sh.cand_v[min(c + lane, n - 1)];
+          const int id = sh.cand_i[min(c + lane, n - 1)];
+          const bool in = c + lane < n && v >= last;
+          const uint64_t b = __builtin_amdgcn_ballot_w64(in);
+          lp_sync<NT>();  // everyone has read its own
+          if (in) {
+            const int at = kept + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+            sh.cand_v[at] = v;
+            sh.cand_i[at] = id;
+          }
+          kept += __builtin_popcountll(b);
+        }
+        lp_sync<NT>();
+        n = kept;
+      }
+    }
     for (int c = tid; c < n; c += NT) {
       const float v = sh.cand_v[c];
       const int id = sh.cand_i[c];
@@ -578,26 +632,41 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, (lp_row_waves<T, NT, NV, HELD>
     });
   }
   lp_sync<NT>();
-  const int n = sh.count;
+  int n = sh.count;
   if (n >= top && n <= CAP) {
     rank(n);
     return;
   }
-  // Rare from here on, and read from memory again.  Too many: those above the bound, and
-  // of those equal to it the first in id order.
-  lp_sync<NT>();  // everyone has read the count
-  if (tid == 0) sh.count = 0;
-  lp_sync<NT>();
-  for (int v0 = tid - lane; v0 < r.V; v0 += NT) {
-    const float v = to_f32(x[min(v0 + lane, r.V - 1)]);
-    offer(v > bound && v0 + lane < r.V, v, v0 + lane);
+  // From here on the row is read from memory again.  Too many: those at hand give a higher
+  // bound; where they are ties with the one before, those above it are taken, and of those
+  // equal to it the first in id order.
+  const bool enough = n >= top;
+  for (int round = 0;; ++round) {
+    const float higher = enough && round < kRounds ? kth_largest_of<T>(sh.cand_v, CAP, top, lane) : bound;
+    const bool ties = !(higher > bound);
+    bound = higher;
+    auto passes = [&](float v) __attribute__((always_inline)) { return ties ? v > bound : v >= bound; };
+    lp_sync<NT>();  // everyone has read the count and the candidates
+    if (tid == 0) sh.count = 0;
+    lp_sync<NT>();
+    if (__builtin_amdgcn_ballot_w64(passes(single_max)) != 0) offer(passes(r.single) && r.extra < r.V, r.single, r.extra);
+#pragma unroll 1
+    for (int i = tid; (i & ~63) < r.nvec; i += NT) {
+      const u32x4_t w = r.vector(i);
+      T e[VE];
+      __builtin_memcpy(e, &w, 16);
+#pragma unroll
+      for (int c = 0; c < VE; ++c) offer(passes(to_f32(e[c])) && i < r.nvec, to_f32(e[c]), i * VE + c);
+    }
+    lp_sync<NT>();
+    n = sh.count;
+    if (ties || n <= CAP) break;
   }
-  lp_sync<NT>();
-  const int above = sh.count;
-  if (n >= top && above <= CAP) {
-    rank(above);
+  if (enough && n <= CAP) {
+    rank(n);
+    // after ties fewer than the first may have come; otherwise this finds none to add
     if (wv == 0) {
-      int at = above;
+      int at = n;
       for (int v0 = 0; v0 < r.V && at < top; v0 += 64) {
         const bool in = v0 + lane < r.V && to_f32(x[min(v0 + lane, r.V - 1)]) == bound;
         const uint64_t b = __builtin_amdgcn_ballot_w64(in);
