@@ -327,6 +327,8 @@ class DiffGPT:
     def anomaly_scores_batch(self, dfs: "list[pd.DataFrame]") -> "list[pd.DataFrame]":
         """anomaly_scores for several frames at once, of any lengths: their series are scored
         as packed sequences in one forward per 65536 tokens (GPT.score)."""
+        if not callable(getattr(self.model, "score", None)):
+            raise TypeError(f"anomaly_scores_batch needs a model with score, as GPT has: {type(self.model).__name__}")
         assert len(dfs) > 0, "dfs must be a non-empty list of frames"
         encoded, orders = [], []
         for df in dfs:

@@ -248,8 +248,12 @@ class Engine:
     def score_continuations(self, tokens: list[int], continuations: list[list[int]]) -> list[list[float]]:
         """Log probability of every token of each candidate continuation of one prompt
         (row c: one float per token of continuations[c], given the prompt and the tokens
-        before it).  The prompt is prefilled once; the continuations, whose common beginnings
-        are run once, go behind its cache as trees of up to 64 tokens."""
+        before it).  The prompt is prefilled once; the continuations, of at most 65 tokens
+        each, go behind its cache as trees of up to 64 tokens, which take them in the given
+        order: beginnings that neighbours in that order share are run once.  The model must
+        have GPT's forward_tree."""
+        if not callable(getattr(self.model, "forward_tree", None)):
+            raise TypeError(f"score_continuations needs a model with forward_tree, as GPT has: {type(self.model).__name__}")
         self._check_tokens(tokens)
         assert isinstance(continuations, list) and len(continuations) > 0, (
             "continuations must be a non-empty list of token lists"

@@ -1,0 +1,43 @@
+"""Refusals and bookkeeping of the scoring paths through the model, without a GPU."""
+
+import numpy as np
+import pandas as pd
+import pytest
+import torch
+
+from diff_gpt.diff_gpt import DiffGPT
+from diff_gpt.model.engine import Engine
+from diff_gpt.model.gpt import BaseGPT
+
+
+class _Other(BaseGPT):
+    """A model that has neither GPT's score nor its forward_tree."""
+
+    def __init__(self):
+        super().__init__(block_size=16, vocab_size=64, n_embd=8, n_head=2, n_layer=1)
+        self.forwards = 0
+
+    def forward(self, idx, targets=None, kv_cache=None):
+        self.forwards += 1
+        return torch.zeros(*idx.shape, self.vocab_size), None
+
+    def generate(self, idx, max_new_tokens, sampler, seed=None):
+        raise NotImplementedError
+
+    @property
+    def device_type(self):
+        return "cpu"
+
+
+@pytest.mark.parametrize("continuations", [[[1]], [[1, 2], [1, 3]]])
+def test_continuations_of_a_model_without_trees(continuations):
+    model = _Other()
+    with pytest.raises(TypeError, match="forward_tree"):
+        Engine(model).score_continuations([1, 2, 3], continuations)
+    assert model.forwards == 0
+
+
+def test_frames_of_a_model_without_score():
+    dgpt = DiffGPT(model=_Other(), order_of_derivative=1, domain_of_definition=np.array([1.0]), use_decimal=False)
+    with pytest.raises(TypeError, match="score"):
+        dgpt.anomaly_scores_batch([pd.DataFrame({"x": np.arange(8.0)})])
