@@ -344,9 +344,11 @@ class DiffGPT:
         was_training = self.model.training
         self.model.eval()
         some = [i for i, e in enumerate(encoded) if e.size > 0]
-        scored = self.model.score([encoded[i].reshape(-1).astype(np.int64).tolist() for i in some])
-        if was_training:
-            self.model.train()
+        try:
+            scored = self.model.score([encoded[i].reshape(-1).astype(np.int64).tolist() for i in some])
+        finally:
+            if was_training:
+                self.model.train()
         out = []
         for df, e, order in zip(dfs, encoded, orders):
             out.append(np.full(df.shape, np.nan, dtype=np.float64))

@@ -41,3 +41,18 @@ def test_frames_of_a_model_without_score():
     dgpt = DiffGPT(model=_Other(), order_of_derivative=1, domain_of_definition=np.array([1.0]), use_decimal=False)
     with pytest.raises(TypeError, match="score"):
         dgpt.anomaly_scores_batch([pd.DataFrame({"x": np.arange(8.0)})])
+
+
+class _Refuses(_Other):
+    def score(self, sequences):
+        assert not self.training
+        raise MemoryError("no room for the logits")
+
+
+@pytest.mark.parametrize("training", [True, False])
+def test_a_failed_batch_leaves_the_models_mode(training):
+    model = _Refuses().train(training)
+    dgpt = DiffGPT(model=model, order_of_derivative=1, domain_of_definition=np.array([1.0]), use_decimal=False)
+    with pytest.raises(MemoryError):
+        dgpt.anomaly_scores_batch([pd.DataFrame({"x": np.arange(8.0)})])
+    assert model.training is training
