@@ -371,7 +371,7 @@ class GPT(BaseGPT):
         assert B == kv_cache.kv_shape[2], f"{B} rows, a cache of {kv_cache.kv_shape[2]}"
         rows = TreeRows(parents, kv_cache, idx.device)
         logits, _ = self.forward(idx, kv_cache=kv_cache, _rows=rows)
-        kv_cache.tree = list(parents)
+        kv_cache.tree, kv_cache.tree_start = list(parents), rows.start
         return logits
 
     @torch.inference_mode()

@@ -56,6 +56,7 @@ class KVCache:
         "_normed",
         "_exposed",
         "tree",
+        "tree_start",
     )
 
     def __init__(
@@ -89,8 +90,9 @@ class KVCache:
         # True once the cache tensor was handed to or taken from a caller
         self._exposed = False
         # the parents of the tree whose tokens lie behind pos (GPT.forward_tree), until
-        # the next append
+        # the next append, and the position it was run at
         self.tree: list[int] | None = None
+        self.tree_start = 0
 
     @property
     def keys_normed(self) -> bool:
@@ -318,6 +320,7 @@ class KVCache:
         ``path``, from a child of the cached row downwards (one list for all rows, or one
         of the same length for each row), become the next cached positions."""
         assert self.tree is not None, "no tree lies behind the cached positions"
+        assert self.pos == self.tree_start, f"the tree lies behind position {self.tree_start}, the cache is at {self.pos}"
         rows = self.kv_shape[2]
         per_row = len(path) > 0 and isinstance(path[0], (list, tuple))
         paths = [list(p) for p in path] if per_row else [list(path)]

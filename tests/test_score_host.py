@@ -8,6 +8,7 @@ import torch
 from diff_gpt.diff_gpt import DiffGPT
 from diff_gpt.model.engine import Engine
 from diff_gpt.model.gpt import BaseGPT
+from diff_gpt.model.kv_cache import KVCache
 
 
 class _Other(BaseGPT):
@@ -56,3 +57,18 @@ def test_a_failed_batch_leaves_the_models_mode(training):
     with pytest.raises(MemoryError):
         dgpt.anomaly_scores_batch([pd.DataFrame({"x": np.arange(8.0)})])
     assert model.training is training
+
+
+def test_keep_where_the_tree_does_not_lie():
+    """A cache whose position was set back (or on) after the tree ran: its next places hold
+    something else."""
+    cache = KVCache(batch_size=1, num_heads=1, seq_len=16, head_dim=4, num_layers=1)
+    cache.pos = cache.tree_start = 5
+    cache.tree = [-1, 0, 1]
+    for pos in (3, 6):
+        cache.pos = pos
+        with pytest.raises(AssertionError, match="behind position 5"):
+            cache.keep([0, 1])
+    cache.pos = 5
+    cache.keep([0, 1])
+    assert cache.pos == 7 and cache.tree is None
