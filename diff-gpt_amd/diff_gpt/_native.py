@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import os
 from pathlib import Path
 from typing import NamedTuple
@@ -868,7 +869,7 @@ def attention_tree_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             raise ValueError("attention_tree: lengths must be a contiguous (B,) int32 tensor on q's device")
         lens = lengths
     else:
-        host_len = int(lengths)
+        host_len = operator.index(lengths)
         if not 0 <= host_len <= Tcap - N:
             raise ValueError(f"attention_tree: {host_len} cached positions and {N} tokens in a cache of {Tcap}")
     mask_b = 0

@@ -6,6 +6,7 @@ signature and generation API as the reference.  Inference only: the HIP
 kernels have no backward, so a forward that would need autograd raises.
 """
 
+import operator
 from abc import ABC, abstractmethod
 from typing import Sequence
 
@@ -326,7 +327,7 @@ class GPT(BaseGPT):
         the TokenLogprobs of tokens 1 .. n - 1 given those before, (n - 1,) tensors, with the
         ``top`` most likely ids at each place.  A sequence has 1 to 2 * block_size tokens."""
         assert max_tokens >= 1, "max_tokens must be positive"
-        seqs = [[int(t) for t in s] for s in sequences]
+        seqs = [list(map(operator.index, s)) for s in sequences]  # whole numbers only
         for s in seqs:
             assert len(s) > 0, "a sequence must have at least one token"
             assert len(s) <= self.freqs_cis.shape[0], (

@@ -6,6 +6,7 @@ are.  GPT.score runs series of different lengths through the layers this way (Pa
 """
 
 import math
+import operator
 from typing import Sequence
 
 import torch
@@ -26,15 +27,15 @@ class PackedLayout:
     def __init__(self, q_lengths: Sequence[int], k_lengths: Sequence[int] | None = None, group: int = 1,
                  device: torch.device | str = "cuda") -> None:
         _native.require_device_type("PackedLayout", device)
-        self.q_lengths = [int(n) for n in q_lengths]
-        self.k_lengths = self.q_lengths if k_lengths is None else [int(n) for n in k_lengths]
+        self.q_lengths = list(map(operator.index, q_lengths))
+        self.k_lengths = self.q_lengths if k_lengths is None else list(map(operator.index, k_lengths))
         if len(self.k_lengths) != len(self.q_lengths):
             raise ValueError(f"{len(self.q_lengths)} query lengths, {len(self.k_lengths)} key lengths")
         if any(n < 0 for n in self.q_lengths) or any(n < 0 for n in self.k_lengths):
             raise ValueError("a sequence's length must not be negative")
         if group < 1:
             raise ValueError(f"group must be at least 1, got {group}")
-        self.group = int(group)
+        self.group = operator.index(group)
         self.total_q, self.total_k = sum(self.q_lengths), sum(self.k_lengths)
         tiles, self.counts = _native.packed_plan(self.q_lengths, self.k_lengths, self.group)
         self.tiles = tiles.to(device)

@@ -7,6 +7,7 @@ GPT.forward_tree runs candidate continuations through the layers this way (TreeR
 """
 
 import math
+import operator
 from typing import Sequence
 
 import torch
@@ -19,7 +20,7 @@ MAX_TREE = 64
 
 
 def _check_parents(parents: Sequence[int]) -> list[int]:
-    parents = [int(p) for p in parents]
+    parents = list(map(operator.index, parents))
     if not 1 <= len(parents) <= MAX_TREE:
         raise ValueError(f"a tree has 1 to {MAX_TREE} tokens, got {len(parents)}")
     for n, p in enumerate(parents):

@@ -7,8 +7,10 @@ import torch
 
 from diff_gpt.diff_gpt import DiffGPT
 from diff_gpt.model.engine import Engine
-from diff_gpt.model.gpt import BaseGPT
+from diff_gpt.model.gpt import GPT, BaseGPT
 from diff_gpt.model.kv_cache import KVCache
+from diff_gpt.model.packed import PackedLayout
+from diff_gpt.model.tree import tree_depths, tree_masks
 
 
 class _Other(BaseGPT):
@@ -72,3 +74,22 @@ def test_keep_where_the_tree_does_not_lie():
     cache.pos = 5
     cache.keep([0, 1])
     assert cache.pos == 7 and cache.tree is None
+
+
+def test_numbers_that_are_not_whole_are_refused():
+    """Never cut to whole ones: a token of 1.7 is not token 1."""
+    model = GPT(vocab_size=64, n_embd=8, block_size=8, n_head=2, n_layer=1)
+    with pytest.raises(TypeError):
+        model.score([[1, 1.7]])
+    with pytest.raises(TypeError):
+        PackedLayout([3, 2.5])
+    with pytest.raises(TypeError):
+        PackedLayout([3], [3.5])
+    with pytest.raises(TypeError):
+        PackedLayout([3], group=1.5)
+    for parents in ([-1, 0.5], [-0.5]):
+        with pytest.raises(TypeError):
+            tree_masks(parents, device="cpu")
+        with pytest.raises(TypeError):
+            tree_depths(parents)
+    assert tree_depths(np.array([-1, 0, 0])) == tree_depths(torch.tensor([-1, 0, 0])) == [0, 1, 1]
