@@ -181,6 +181,7 @@ class GPT(BaseGPT):
         ids = None if argmax_out is None else argmax_out.view(B * T)
         if _native.lm_head_(xn.view(B * T, C), self.lm_head.weight, cap, logits.view(B * T, V), ids):
             return logits
+        del logits  # not beside the product's own
         logits = self.lm_head(xn)
         if cap > 0:
             _native.ops().softcap_(logits, cap)  # cap * tanh(logits / cap)
@@ -320,12 +321,17 @@ class GPT(BaseGPT):
         self,
         sequences: Sequence[Sequence[int]],
         top: int = 0,
-        max_tokens: int = 65536,
+        max_tokens: int | None = None,
     ) -> list[TokenLogprobs]:
         """Log probabilities of token sequences of different lengths, in packed batches of at
-        most max_tokens tokens (a longer sequence goes alone): for each sequence of n tokens
+        most max_tokens tokens (a longer sequence goes alone; None: 65536, fewer where their
+        logits, all held at once, would pass 2 GiB): for each sequence of n tokens
         the TokenLogprobs of tokens 1 .. n - 1 given those before, (n - 1,) tensors, with the
-        ``top`` most likely ids at each place.  A sequence has 1 to 2 * block_size tokens."""
+        ``top`` most likely ids at each place.  They are views of the batch's results, which
+        live as long as any of them.  A sequence has 1 to 2 * block_size tokens."""
+        if max_tokens is None:
+            w = self.lm_head.weight
+            max_tokens = max(1, min(65536, (2 << 30) // (w.size(0) * w.element_size())))
         assert max_tokens >= 1, "max_tokens must be positive"
         seqs = [list(map(operator.index, s)) for s in sequences]  # whole numbers only
         for s in seqs:
