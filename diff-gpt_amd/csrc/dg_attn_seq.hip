@@ -676,14 +676,15 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   a.tiles = tiles;
   a.nq = Nq; a.nk = Nk;
   a.nsplit = 1;
-  const int64_t blocks = counts[0] * Hkv;
-  DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 workgroups");
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (seq_mfma_applicable(a, dtype, false)) return launch_seq_mfma_packed(a, dtype, counts, s);
-  a.rows_per_wg = tile_rows((int)counts[2], D);
+  const bool mfma = seq_mfma_applicable(a, dtype, false);
+  a.rows_per_wg = mfma ? seq_mfma_packed_rows(counts, Hkv, D) : tile_rows((int)counts[2], D);
   a.nrb = (int)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg);
-  DG_REQUIRE(blocks * a.nrb <= 0x7fffffff, DG_EINVAL, "attention_packed: more than 2^31 - 1 workgroups");
-  return launch_tile_any<false>(a, dtype, dim3((unsigned)(blocks * a.nrb)), s);
+  const int64_t blocks = counts[0] * Hkv;
+  DG_REQUIRE(blocks <= kMostWorkgroups256 && blocks * a.nrb <= kMostWorkgroups256, DG_EINVAL,
+             "attention_packed: more than 2^24 - 1 workgroups (tiles times key heads)");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(blocks * a.nrb));
+  return mfma ? launch_seq_mfma_packed(a, dtype, grid, s) : launch_tile_any<false>(a, dtype, grid, s);
 }
 
 extern "C" size_t dg_attention_tree_workspace_size(int B, int N, int H, int Hkv, int Tcap, int D, int dtype) {
@@ -736,17 +737,17 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
     a.ws_o = workspace;
     a.ws_ml = static_cast<char*>(workspace) + t.o_bytes;
   }
+  // a row's waves read its splits in turn: four of them where there are many and rows few
+  const int64_t rows = (int64_t)B * H * N;
+  const bool many = t.nsplit >= 16 && rows <= 4096;
+  const int64_t groups = t.nsplit == 1 ? 0 : many ? rows : (rows + 3) / 4;
   const int64_t blocks = ((int64_t)B * Hkv * t.nsplit + 7) / 8 * 8 * t.nrb;
-  DG_REQUIRE(blocks <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
+  DG_REQUIRE(blocks <= kMostWorkgroups256 && groups <= kMostWorkgroups256, DG_EINVAL,
+             "attention_tree: more than 2^24 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rc = mfma ? launch_seq_mfma_tree(a, dtype, (unsigned)blocks, s)
                       : launch_tile_any<true>(a, dtype, dim3((unsigned)blocks), s);
   if (rc != DG_OK || t.nsplit == 1) return rc;
-  const int64_t rows = (int64_t)B * H * N;
-  // a row's waves read its splits in turn: four of them where there are many and rows few
-  const bool many = t.nsplit >= 16 && rows <= 4096;
-  const int64_t groups = many ? rows : (rows + 3) / 4;
-  DG_REQUIRE(groups <= 0x7fffffff, DG_EINVAL, "attention_tree: more than 2^31 - 1 workgroups");
   const dim3 grid((unsigned)groups);
 #define DG_JOIN(T)                                                                         \
   do {                                                                                     \

@@ -734,14 +734,15 @@ int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream
 //   head_dim 256: 2 x 512 [64] 24 / 27 / 37, 2 x 2048 in groups of 2 [256] 146 / 103 / 101,
 //     16 x 512 [512] 142 / 97 / 76
 //   head_dim 128: 1 x 3584 in groups of 2 [448] 129 / 82 / 92, 2 x 2048 [512] 110 / 63 / 57
-int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s) {
-  const int64_t tiles = counts[1] * a.Hkv;
-  const int rt = counts[2] <= 32 || tiles <= 64 ? 1 : counts[2] <= 64 || tiles <= (a.D > 64 ? 384 : 640) ? 2 : 4;
-  a.rows_per_wg = 32 * rt;
-  a.nrb = (int)((counts[2] + a.rows_per_wg - 1) / a.rows_per_wg);
-  const dim3 grid((unsigned)(counts[0] * a.Hkv * a.nrb));
-  if (rt == 1) return launch_seq_t<1, false>(a, dtype, grid, s);
-  if (rt == 2) return launch_seq_t<2, false>(a, dtype, grid, s);
+int seq_mfma_packed_rows(const int64_t counts[3], int Hkv, int D) {
+  const int64_t tiles = counts[1] * Hkv;
+  if (counts[2] <= 32 || tiles <= 64) return 32;
+  return counts[2] <= 64 || tiles <= (D > 64 ? 384 : 640) ? 64 : 128;
+}
+
+int launch_seq_mfma_packed(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s) {
+  if (a.rows_per_wg == 32) return launch_seq_t<1, false>(a, dtype, grid, s);
+  if (a.rows_per_wg == 64) return launch_seq_t<2, false>(a, dtype, grid, s);
   return launch_seq_t<4, false>(a, dtype, grid, s);
 }
 

@@ -579,6 +579,9 @@ namespace dg {
 void set_error(const char* fmt, ...);
 int check_launch(const char* what);
 
+// Workgroups of 256 threads a launch may have: 2^32 - 1 threads in all.
+constexpr int64_t kMostWorkgroups256 = 0xffffffffll / 256;
+
 // Lane slices of a row of D elements of es bytes (the RoPE and vector
 // attention kernels): the row padded to DPAD = the next power of two spreads
 // over LPK = DPAD / EPL <= 64 lanes, EPL elements each.  Vector slices are

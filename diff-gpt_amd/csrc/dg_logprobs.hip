@@ -16,9 +16,9 @@
 //     there by counting.  Where they overflow the buffer (256 logits for a row of one wave,
 //     which half the rows do at 64 alternatives), the k-th largest of those it holds is the
 //     next bound, and the row is looked through again (4096 x 4096 fp32 with 64 alternatives
-//     66 us; one alternative after the other 2012).  Ties in number beyond the buffer are taken in id order from the row; what
-//     neither takes (NaN among the first k, long staircases of ties) goes one alternative
-//     after the other.
+//     66 us; one alternative after the other 2012).  Ties in number beyond the buffer are
+//     taken in id order from the row; what neither takes (NaN among the first k, long
+//     staircases of ties) goes one alternative after the other.
 //   fp64: a wavefront a row, one pass per alternative.
 //
 // Bound by the vector ALU next to HBM: a logit takes some 10 operations (two unpackings,
@@ -801,11 +801,16 @@ __global__ __launch_bounds__(256) void lp_f64_kernel(const LogprobArgs a) {
 
 namespace {
 
+// A launch has 2^32 - 1 threads at most.
+bool rows_fit(int64_t M, int rows, int threads) { return (M + rows - 1) / rows <= 0xffffffffll / threads; }
+#define DG_LP_MANY "token_logprobs: %lld rows are more than one launch takes"
+
 template <typename T>
 int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
   constexpr int VE = 16 / (int)sizeof(T);
   const bool vec = a.V % VE == 0;
   if (a.V <= 256 && a.top <= 16) {
+    DG_REQUIRE(rows_fit(a.M, 16, 256), DG_EINVAL, DG_LP_MANY, (long long)a.M);
     const dim3 grid((unsigned)((a.M + 15) / 16));
 #define DG_LP(KP)                                                                                    \
   do {                                                                                               \
@@ -824,6 +829,7 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
 #define DG_LP_ROW(NT, PER)                                                                                           \
   do {                                                                                                               \
     constexpr int kRows = (NT) < 256 ? 256 / (NT) : 1;                                                               \
+    DG_REQUIRE(rows_fit(a.M, kRows, (NT) < 256 ? 256 : (NT)), DG_EINVAL, DG_LP_MANY, (long long)a.M);                \
     hipLaunchKernelGGL((lp_row_kernel<T, (NT), (PER) / VE, true>), dim3((unsigned)((a.M + kRows - 1) / kRows)),      \
                        dim3((NT) < 256 ? 256 : (NT)), 0, s, a);                                                      \
     return check_launch("lp_row_kernel_" #NT);                                                                       \
@@ -842,6 +848,7 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
   // threads' registers, or read three times, / read once: 500 x 65000 fp32 38 / 33, 500 x
   // 131072 bf16 47 / 37, fp32 112 / 53, 300 x 200000 fp32 107 / 44; 500 x 31000 fp32 21 / 23,
   // 2048 x 49999 bf16 66 / 80.
+  DG_REQUIRE(rows_fit(a.M, 1, 1024), DG_EINVAL, DG_LP_MANY, (long long)a.M);
 #define DG_LP_LONG(NV, NAME)                                                                                \
   do {                                                                                                      \
     hipLaunchKernelGGL((lp_row_kernel<T, 1024, (NV), false>), dim3((unsigned)a.M), dim3(1024), 0, s, a);    \
@@ -871,6 +878,7 @@ extern "C" int dg_token_logprobs(int64_t M, int64_t V, int dtype, const void* x,
   const LogprobArgs a{x, x_ld, M, V, ids, logprob, entropy, top, top_logprob, top_ids};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == DG_F64) {
+    DG_REQUIRE(rows_fit(M, 4, 256), DG_EINVAL, DG_LP_MANY, (long long)M);
     hipLaunchKernelGGL(lp_f64_kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, a);
     return check_launch("lp_f64_kernel");
   }

@@ -151,11 +151,12 @@ __device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n
 // The head_dim that the matrix-core kernels and their workspaces round D (up to 256) up to.
 constexpr int seq_mfma_dim(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-// dg_attn_seq_mfma.hip: whether it takes the shape, the rows of a workgroup over so many
-// (token, head) rows, and its launches
+// dg_attn_seq_mfma.hip: whether it takes the shape, the rows of a tree's workgroup over so
+// many (token, head) rows and of a packed tile's, and its launches
 bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree);
 int seq_mfma_tree_rows(int64_t B, int rows, int Hkv, int keys, int D, int dtype);
-int launch_seq_mfma_packed(SeqArgs a, int dtype, const int64_t counts[3], hipStream_t s);
+int seq_mfma_packed_rows(const int64_t counts[3], int Hkv, int D);
+int launch_seq_mfma_packed(const SeqArgs& a, int dtype, dim3 grid, hipStream_t s);
 int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s);
 
 }  // namespace dg

@@ -593,6 +593,8 @@ DG_API int dg_draw_argmax(int64_t M, int V, int dtype, const void* probs, int64_
  * followed.
  * fp32 / bf16 / fp16 / fp64, every head_dim up to 1024, rows with unit stride over d; the
  * scale is positive.  A sequence has at most 2^30 keys and (query, head of the group) rows.
+ * The table's entries times Hkv, or 2, 4 or 8 times that where tiles are split over
+ * workgroups, stay below 2^24 (the launch has 2^32 - 1 threads at most); more is refused.
  */
 typedef struct dg_packed_tile {
   int32_t q0, lq, k0, lk; /* the sequence's rows of q and of k */
@@ -623,7 +625,8 @@ DG_API int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D, in
  * 1 <= N <= 64, N <= Tcap <= 2^30.  Long rows are split over workgroups whose partial results meet
  * in the caller's workspace (dg_attention_tree_workspace_size bytes, 16-byte aligned; its
  * contents need no initialisation, and calls that may overlap need one each).
- * Types, head_dim and scale as dg_attention_packed.
+ * Types, head_dim and scale as dg_attention_packed; fewer than 2^24 workgroups (rows of the
+ * batch times key heads times splits) in all.
  */
 DG_API size_t dg_attention_tree_workspace_size(int B, int N, int H, int Hkv, int Tcap, int D, int dtype);
 
@@ -646,7 +649,8 @@ DG_API int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, int 
  *     order, equal ones by ascending id (contiguous rows of `top`)
  * computed and stored in fp32 (fp64 for fp64 logits).  A row that holds a NaN or +inf, or
  * -inf alone, gives NaN log probabilities and entropy, as log_softmax does; its ids are
- * those of its largest logits, NaN ones last.  0 <= top <= min(V, 64).
+ * those of its largest logits, NaN ones last.  0 <= top <= min(V, 64).  M rows that are more
+ * than one launch takes (2^24 of up to 16 rows each, fewer of long ones) are refused.
  */
 DG_API int dg_token_logprobs(int64_t M, int64_t V, int dtype, const void* x, int64_t x_ld, const int64_t* ids,
                              void* logprob, void* entropy, int top, void* top_logprob, int64_t* top_ids,

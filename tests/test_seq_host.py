@@ -154,3 +154,27 @@ def test_logprobs_refusals(kw, rc):
     a = dict(M=2, V=100, dtype=0, p=FAKE, top=0) | kw
     p = a["p"]
     assert _native.lib().dg_token_logprobs(a["M"], a["V"], a["dtype"], p, a["V"], p, p, p, a["top"], p, p, NUL) == rc
+
+
+@pytest.mark.parametrize("counts,Hkv,D,rc", [((8 * (2**21 - 1), 8 * (2**21 - 1), 128), 8, 64, -1), ((2**24, 2**24, 1), 1, 64, -1),
+                                             ((2**23, 2**23, 40), 1, 7, -1), ((2**31 - 8, 5, 1), 2**20, 64, -1)])
+def test_packed_launches_past_the_grid(counts, Hkv, D, rc):
+    """More workgroups than a launch of 2^32 - 1 threads has: refused before anything runs."""
+    assert _packed(H=Hkv, Hkv=Hkv, D=D, counts=counts) == rc
+    assert b"workgroups" in _native.lib().dg_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(B=2**20, H=16, Hkv=16), dict(B=2**23, N=64, H=1, Tcap=64, length=0, D=7),
+                                dict(B=2**24, H=4, Hkv=4, dtype=3), dict(B=2**22, N=32, H=4, Hkv=1, Tcap=64)])
+def test_tree_launches_past_the_grid(kw):
+    """Rows times key heads times row blocks of 32: 2^24 and more."""
+    assert _tree(**kw) == -1
+    assert b"workgroups" in _native.lib().dg_last_error()
+
+
+@pytest.mark.parametrize("M,V,top,dtype", [(2**28 + 1, 2, 0, 1), (2**31 - 1, 256, 16, 0), (2**26, 64, 17, 0), (2**26, 1024, 0, 2),
+                                           (2**24, 5000, 1, 1), (2**23, 20000, 0, 0), (2**22, 40000, 0, 1), (2**22, 300000, 0, 0),
+                                           (2**26, 64, 0, 3)])
+def test_logprobs_launches_past_the_grid(M, V, top, dtype):
+    assert _native.lib().dg_token_logprobs(M, V, dtype, FAKE, V, FAKE, FAKE, FAKE, top, FAKE, FAKE, NUL) == -1
+    assert b"launch" in _native.lib().dg_last_error()
