@@ -327,7 +327,7 @@ class DiffGPT:
     def anomaly_scores_batch(self, dfs: "list[pd.DataFrame]") -> "list[pd.DataFrame]":
         """anomaly_scores for several frames at once, of any lengths: their series are scored
         as packed sequences, in few forwards (GPT.score), with log probabilities in fp32
-        whatever the model's type (anomaly_scores takes them in the logits' type)."""
+        (fp64 for an fp64 model) whatever the logits' type, which anomaly_scores takes them in."""
         if not callable(getattr(self.model, "score", None)):
             raise TypeError(f"anomaly_scores_batch needs a model with score, as GPT has: {type(self.model).__name__}")
         assert len(dfs) > 0, "dfs must be a non-empty list of frames"

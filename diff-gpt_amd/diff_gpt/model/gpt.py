@@ -371,7 +371,9 @@ class GPT(BaseGPT):
         """Logits (B, N, V) of a tree of N <= 64 tokens idx (B, N) behind every row of the
         cache: token n follows token parents[n], an earlier one, or for -1 the cached row.
         The tokens' keys and values lie behind the cached positions until the next append;
-        kv_cache.pos stays, and KVCache.keep goes on with one path of the tree."""
+        kv_cache.pos stays, and KVCache.keep goes on with one path of the tree.  A prompt that
+        the rows share (KVCache.prefill) is copied into each row's pages first, and stays
+        there."""
         B, N = idx.shape
         assert kv_cache.pos_dev is None, "a captured decode step takes one token per row"
         assert N == len(parents), f"{N} tokens, {len(parents)} parents"
