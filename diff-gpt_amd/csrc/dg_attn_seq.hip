@@ -25,6 +25,8 @@
 
 namespace dg {
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
 // arithmetic of a row: fp32 in log2 units, fp64 in natural ones (no fp64 exp2 needed)
 template <typename T>
 struct SeqAcc {
@@ -658,7 +660,7 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   DG_REQUIRE(known_dtype(dtype), DG_EUNSUPPORTED, "attention_packed: dtype %d unsupported", dtype);
   DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "attention_packed: head_dim %d outside [1, %d]", D, kMaxHeadDim);
   DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "attention_packed: %d query heads on %d key heads", H, Hkv);
-  DG_REQUIRE(scale > 0.f && std::isfinite(scale), DG_EINVAL, "attention_packed: the scale must be positive");
+  DG_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), DG_EINVAL, "attention_packed: the scale must be positive and below 2^127");
   DG_REQUIRE(counts != nullptr, DG_EINVAL, "attention_packed: NULL argument");
   DG_REQUIRE(counts[0] >= 0 && counts[0] <= 0x7fffffff && counts[0] % 8 == 0 && counts[1] >= 0 && counts[1] <= counts[0] &&
                  counts[2] >= 0 && counts[2] <= kTileRows,
@@ -672,7 +674,7 @@ extern "C" int dg_attention_packed(int64_t Nq, int64_t Nk, int H, int Hkv, int D
   a.vt = v_t; a.vh = v_h; a.yt = y_t; a.yh = y_h;
   a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
   a.scale = scale;
-  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.scale_log2 = scale * kLog2e;
   a.tiles = tiles;
   a.nq = Nq; a.nk = Nk;
   a.nsplit = 1;
@@ -705,7 +707,7 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   DG_REQUIRE(Tcap <= kMostPositions, DG_EINVAL, "attention_tree: a cache of more than 2^30 positions");
   DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "attention_tree: %d query heads on %d key heads", H, Hkv);
   DG_REQUIRE(H / Hkv <= 0x7fffff, DG_EINVAL, "attention_tree: %d heads a group", H / Hkv);
-  DG_REQUIRE(scale > 0.f && std::isfinite(scale), DG_EINVAL, "attention_tree: the scale must be positive");
+  DG_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), DG_EINVAL, "attention_tree: the scale must be positive and below 2^127");
   DG_REQUIRE(lens != nullptr || (len >= 0 && len <= Tcap - N), DG_EINVAL,
              "attention_tree: %d cached positions and %d tokens in a cache of %d", len, N, Tcap);
   if (B == 0 || H == 0) return DG_OK;
@@ -718,7 +720,7 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   a.yb = y_st->b; a.yt = y_st->t; a.yh = y_st->h;
   a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
   a.scale = scale;
-  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.scale_log2 = scale * kLog2e;
   a.B = B; a.N = N; a.Tcap = Tcap;
   a.len = len; a.lens = lens;
   a.masks = masks; a.mask_b = mask_b;

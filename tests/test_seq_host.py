@@ -178,3 +178,9 @@ def test_tree_launches_past_the_grid(kw):
 def test_logprobs_launches_past_the_grid(M, V, top, dtype):
     assert _native.lib().dg_token_logprobs(M, V, dtype, FAKE, V, FAKE, FAKE, FAKE, top, FAKE, FAKE, NUL) == -1
     assert b"launch" in _native.lib().dg_last_error()
+
+
+def test_scales_that_overflow_in_log2_units():
+    """Accepted, a scale of 3e38 was infinite times log2(e), and a score of 0 NaN."""
+    assert _packed(scale=3e38) == -1 and b"scale" in _native.lib().dg_last_error()
+    assert _tree(scale=2.4e38) == -1 and b"scale" in _native.lib().dg_last_error()
