@@ -732,6 +732,9 @@ extern "C" int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, 
   const bool mfma = !few && seq_mfma_applicable(a, dtype, true);
   const TreeShape t = tree_shape(B, N, H, Hkv, Tcap, D, dtype, mfma ? seq_mfma_tree_rows(B, N * a.G, Hkv, Tcap, D, dtype) : tile_rows(N * a.G, D), mfma);
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
+  // seq_mfma_tree_rows takes 128 for fewer than 256 tiles over more than 300000 / 255 keys, of
+  // which a split has at most a half: that kernel knows no other way
+  DG_REQUIRE(!mfma || t.rows_per_wg < 128 || t.nsplit > 1, DG_EUNSUPPORTED, "attention_tree: 128 rows unsplit");
   if (t.nsplit > 1) {
     DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,
                "attention_tree: a workspace of %zu bytes, %zu needed", workspace_bytes, t.ws_bytes);

@@ -569,7 +569,7 @@ void seq_mfma_kernel(const SeqArgs a) {
 
   // ---- the result ----------------------------------------------------------------------
   const bool stored = wrow + r32 < rend;
-  if (TREE && a.nsplit > 1) {
+  if (TREE && (RT == 4 || a.nsplit > 1)) {  // 128 rows of a tree are always split
     const int64_t part = ((pc.b * a.Hkv + pc.kvh) * (int64_t)(a.N * a.G) + row) * a.nsplit + pc.split;
     if (stored) {
       float* wo = static_cast<float*>(a.ws_o) + part * D;

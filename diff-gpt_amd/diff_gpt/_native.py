@@ -79,6 +79,7 @@ _SIGNATURES = {
     "dg_abi_version": (ctypes.c_int, []),
     "dg_last_error": (ctypes.c_char_p, []),
     "dg_last_kernel": (ctypes.c_char_p, []),
+    "dg_kernel_before": (ctypes.c_char_p, []),
     "dg_rope_qknorm_append": (
         ctypes.c_int,
         [ctypes.c_int] * 5
@@ -274,7 +275,7 @@ _SIGNATURES = {
     ),
 }
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # head_dim the kernels take: every even size up to 1024 (a row padded to the
 # next power of two spreads over at most 64 lanes of 16 elements)
@@ -319,6 +320,11 @@ def _check(rc: int, what: str) -> None:
 def last_kernel() -> str:
     """The kernel that this thread's last launch through the library ran."""
     return lib().dg_last_kernel().decode()
+
+
+def kernel_before() -> str:
+    """The kernel that its launch before the last ran."""
+    return lib().dg_kernel_before().decode()
 
 
 def _dtype_code(t: torch.Tensor) -> int:

@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define DG_ABI_VERSION 4
+#define DG_ABI_VERSION 5
 
 #if defined(__GNUC__)
 #define DG_API __attribute__((visibility("default")))
@@ -55,7 +55,7 @@ extern "C" {
  * in fp64, any other scale acts as its fp32 value.  ABI version 3 added
  * DG_F64 and made dg_swiglu's alpha / limit and dg_softcap's cap double;
  * version 4 added dg_packed_plan, dg_attention_packed, dg_attention_tree and
- * dg_token_logprobs, which take fp64 as well. */
+ * dg_token_logprobs, which take fp64 as well; version 5 dg_kernel_before. */
 enum dg_dtype { DG_F32 = 0, DG_BF16 = 1, DG_F16 = 2, DG_F64 = 3 };
 
 enum dg_status {
@@ -91,6 +91,9 @@ DG_API const char* dg_last_error(void);
 /* Name of the kernel that this thread's last successful launch ran ("" before
  * the first): which side of a dispatch rule a call took. */
 DG_API const char* dg_last_kernel(void);
+
+/* The same of the launch before that: what a call's joining launch joined. */
+DG_API const char* dg_kernel_before(void);
 
 /*
  * Fused RoPE + QK-norm + KV append.  Replaces mha.py:44-56: apply_rotary_emb on
