@@ -11,9 +11,9 @@
 // lanes have a key each, for the outputs dims each; the probabilities go from one to the
 // other through LDS.  A hidden key's score is taken out by selection and its values are
 // skipped, so nothing it holds can reach a row.  Bound by LDS reads (five of 16 bytes for
-// 16 products a lane).  16 x 512 tokens, 8 heads: head_dim 65 bf16 371 us, 600
-// fp32 2.4 ms (17 TFLOP/s), 64 fp64 366; a step over 32 caches of 1900, 8 heads: 65 bf16
-// 115 us, 600 fp32 566 (4.1 TB/s), 64 fp64 124 (4.0 TB/s).  One row a wave at a time with a
+// 16 products a lane).  16 x 512 tokens, 8 heads: head_dim 65 bf16 362 us, 600
+// fp32 1.86 ms (22 TFLOP/s), 64 fp64 384; a step over 32 caches of 1900, 8 heads: 65 bf16
+// 115 us, 600 fp32 540 (4.3 TB/s), 64 fp64 128 (3.9 TB/s).  One row a wave at a time with a
 // running softmax in each lane group took 13.1 ms and 2.2 ms in fp64.
 #include "dg_seq.h"
 
@@ -201,7 +201,14 @@ __global__ __launch_bounds__(256) void seq_tile_kernel(const SeqArgs a) {
     const bool open = t0 + KT <= first_open;  // every row sees every key of the tile
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      if (c >= nch) break;
+      // A loop that ends early is not unrolled, and o indexed at run time: in scratch memory
+      // for 16 rows (16 x 512 tokens, 8 heads of 600, fp32: 2.38 ms so, 1.86 unrolled).  A
+      // step's 8 rows have fewer outputs a lane, and unrolled they leave room for two
+      // workgroups a CU in place of three (32 caches of 1900, 8 heads of 600: 540 us so, 659).
+      if (c >= nch) {
+        if constexpr (LPR == 32) break;
+        else continue;
+      }
       __syncthreads();
       put(c);
       __syncthreads();
