@@ -487,11 +487,11 @@ int tile_rows(int rows, int D) { return rows <= 8 ? 8 : D <= 256 ? 32 : 16; }
 // to seven a CU and take longer: 2048 of two stages (a step over 32 caches of 1900, 8 heads
 // of 64, fp64: 468 us unsplit, 227 so).  us at 256 / 512 / 1024
 // workgroups, bf16:
-//   rows of 32, head_dim 128 (64 rows, 4 key heads, lengths to 4096)    52.1 / 58.6 / 68.3
-//               head_dim  64 (64 rows, 8 key heads, lengths to 1024)    17.2 / 17.0 / 25.3
-//           64, head_dim  64 (16 rows, 8 key heads, lengths to 4096)    31.7 / 26.2 / 28.1
-//          128, head_dim 128 (16 rows, 4 key heads, lengths to 7168)    57.3 / 45.2 / 41.1
-//               head_dim  64 (2 rows, 2 key heads, lengths to 131000)   77.1 / 62.3 / 61.2
+//   rows of 32, head_dim 128 (64 rows, 4 key heads, lengths to 4096)    56.2 / 63.6 / 75.2
+//               head_dim  64 (64 rows, 8 key heads, lengths to 1024)    18.0 / 17.9 / 27.7
+//           64, head_dim  64 (16 rows, 8 key heads, lengths to 4096)    36.3 / 31.1 / 34.1
+//          128, head_dim 128 (16 rows, 4 key heads, lengths to 7168)    75.7 / 57.8 / 51.7
+//               head_dim  64 (2 rows, 2 key heads, lengths to 131000)   96.1 / 84.2 / 85.3
 constexpr int kMaxSplits = 512;
 
 int tree_chunk(int64_t B, int Hkv, int nrb, int keys, int rows_per_wg, int D, int dtype, bool mfma) {
@@ -560,9 +560,9 @@ namespace {
 // CU's share, one workgroup in 32 of its XCD's, then has long and short ones, and the
 // launch ends on short ones.  Lists are filled up with empty tiles.
 // Batches of few tiles, which run at once, are one window.  us over windows of 1024 / 2048
-// / 4096 / 16384 keys, bf16: 64 x 1024 tokens, 8 heads of 64, 111 / 114 / 117 / 117;
-// 512 of 17 - 276, 4 heads of 32, 29.5 / 29.9 / 32.5 / 34.4; fp32, 16 x 1000 (128 tiles),
-// 278 / 267 / 266 / 207.
+// / 4096 / 16384 keys, bf16: 512 of 17 - 276, 4 heads of 32, 32.4 / 33.7 / 35.7 / 33.9 (64 x
+// 1024 tokens, 8 heads of 64, within 2 %); fp32, 16 x 1000 (128 tiles) in windows of 1024 /
+// 2048 / 4096 keys and in one, 278 / 267 / 266 / 207.
 constexpr int64_t kWindowKeys = 2048, kOneWindowTiles = 256;
 
 std::vector<dg_packed_tile> plan_tiles(int64_t S, const int64_t* lq, const int64_t* lk, int group) {

@@ -2,7 +2,7 @@
 // up to 256, fp32 up to 128, rows of whole 16-byte pieces (dg_attn_seq.hip has the entry points
 // and the kernel for every other shape).  D here is 16, 32, 64, 128 or 256: a head of fewer
 // dims is computed as one of the next of these, its missing pieces zeros (16 x 512 tokens, 8 heads of
-// 80: bf16 29 us, fp32 140; in seq_tile_kernel 385 and 340).
+// 80: bf16 32 us, fp32 139; in seq_tile_kernel 385 and 340).
 //
 // A workgroup is WAVES wavefronts over one key head of one sequence: RT tiles of 32
 // (query, head of the group) rows by KS = WAVES / RT groups of keys.  With few rows (RT 1:
@@ -33,12 +33,12 @@
 // only in key blocks that some row of the wave sees part of; values there that are not
 // finite are kept out of the product (clean_stage).
 //
-// Bound by the softmax's vector instructions beside the matrix cores' for prompts (28 cycles
-// of a SIMD for 64 scores: fused product, exp2 at a quarter of the rate, sum, pack,
-// maximum), by HBM for few rows.  bf16: 6 sequences of up to 7168 tokens, 16 heads on 4 of
-// 128, 487 us (980 TFLOP/s; vector ALU 54 % busy, matrix cores 53 %); 64 of 100 - 2048, 8
-// heads of 64, 169 us (650 TFLOP/s; 66 %, 34 %); one token for each of 64 caches of up to
-// 4096, 16 heads on 4 of 128, 52 us (269 MB, 5.1 TB/s).
+// Bound by the softmax's vector instructions beside the matrix cores' for prompts (38 cycles
+// of a SIMD for 64 scores: fused product, exp2 at a quarter of the rate, sum, maximum, and
+// three instructions for the two terms of a probability), by HBM for few rows.  bf16: 6 sequences of up to 7168
+// tokens, 16 heads on 4 of 128, 660 us (720 TFLOP/s; vector ALU 56 % busy, matrix cores
+// 58 %); 64 of 100 - 2048, 8 heads of 64, 221 us (500 TFLOP/s; 70 %, 39 %); one token for
+// each of 64 caches of up to 4096, 16 heads on 4 of 128, 53 us (269 MB, 5.1 TB/s).
 // Not kept: the K fragments of a block in flight together, two chains for the row sums, 168
 // registers at head_dim 64, raised wave priority around the products (each within 2 %);
 // outputs checked for values that are not finite at the end and the piece done again (5 %
@@ -129,7 +129,8 @@ struct SeqCfg {
   static_assert((((KS - 1) * RT + 1) / 2) * JOIN * 4 <= KS * 2 * TILE * ES, "joined states fit a stage");
   static_assert(ES == 4 || ((RT + 1) / 2) * 32 * D <= KS * 2 * TILE, "outputs fit a stage");
   // workgroups a CU that the registers must allow (fp32 at head_dim 64, 64 x 512 tokens: four
-  // spill, 215 us; three 177.  bf16 at 256, 16 x 512, 8 heads: two spill, 148; one 76)
+  // spill, 215 us; three 180.  bf16 at 256, 16 x 512, 8 heads, one term of each probability: two
+  // spill, 148; one 76)
   static constexpr int WGS = RT == 4 ? (ES == 4 ? (D <= 32 ? 4 : D == 64 ? 3 : 2) : D <= 64 ? 4 : D == 128 ? 3 : 1) : (D * ES <= 128 ? 2 : 1);
 };
 
@@ -700,15 +701,16 @@ bool seq_mfma_applicable(const SeqArgs& a, int dtype, bool tree) {
 // Rows of a tree's workgroup.  32 (the waves split the keys) spread a row's keys over the
 // most waves; 64 and 128 read them fewer times.  us with 32 / 64 / 128 rows, "rows of the
 // batch x (token, head) rows", lengths up to, key heads:
-//   head_dim <= 32, every one tried:  bf16 16 x 60, 600, 4: 11 / 18 / 18; fp32 32 x 60,
+//   head_dim <= 32, every one tried:  bf16 16 x 60, 600, 4: 8.7 / 13.8 / 18.1; fp32 32 x 60,
 //     2000, 4: 29.9 / 30.6 / 30.8; 64 x 64, 4000, 8: 113 / 147 / 147
 //   fp32 head_dim 64: 3 x 152, 140, 1: 11.8 / 14.2 / 18; 64 x 256, 3000, 4: 288 / 294 / 417
 //     head_dim 128: 32 x 48, 2000, 4: 148 / 105 / 105; 2 x 256, 20000, 2: 188 / 118 / 137
-//   16-bit, few keys in all: head_dim 64 16 x 60, 600, 4: 9.5 / 15.3 / 15.5, head_dim 128
-//     4 x 152, 1500, 4: 18 / 19 / 24, 32 x 96, 2000, 4: 35 / 38 / 40; many: head_dim 64
-//     4 x 128, 70000, 8: 177 / 155 / 131, head_dim 128 16 x 96, 7168, 4: 57 / 46 / 43
-//   64 rows fill the chip, no splits: 64 x 256, 4000, 4: head_dim 64 86 / 74 / 102,
-//     head_dim 128 180 / 136 / 163
+//   16-bit, few keys in all: head_dim 64 16 x 60, 600, 4: 10.8 / 16.2 / 19.2, head_dim 128
+//     4 x 152, 1500, 4: 20.9 / 19.9 / 27.9, 32 x 96, 2000, 4: 42.4 / 41.4 / 41.5; many:
+//     head_dim 64 4 x 128, 70000, 8: 140 / 143 / 125, head_dim 128 16 x 96, 7168, 4: 79.7 /
+//     53.5 / 54.3
+//   64 rows fill the chip, no splits: 64 x 256, 4000, 4: head_dim 64 108 / 104 / 128,
+//     head_dim 128 240 / 175 / 207
 int seq_mfma_tree_rows(int64_t B, int rows, int Hkv, int keys, int D, int dtype) {
   if (rows <= 32 || D <= 32) return 32;
   if (dtype == DG_F32) return D <= 64 ? 32 : 64;
@@ -728,12 +730,13 @@ int launch_seq_mfma_tree(const SeqArgs& a, int dtype, unsigned blocks, hipStream
 // four of 32 that split them in four: the more where tiles are few, since a workgroup
 // walks its keys one stage after the other, and never fewer than fill the rows.  us with
 // 32 / 64 / 128 rows, tiles times key heads in brackets, bf16:
-//   head_dim  64: 8 x 512 tokens [256] 18.7 / 14.0 / 15.2, 16 [512] 31.6 / 19.5 / 18.2,
-//     32 [1024] 52.3 / 28.7 / 23.3; 6 x 2048 [768] 69.6 / 51.5 / 50; 48 chunks of up to
-//     300 behind up to 3000 keys, groups of 4 [436] 61 / 46.5 / 61.5, 64 [550] 72 / 61 / 59
-//   head_dim 256: 2 x 512 [64] 24 / 27 / 37, 2 x 2048 in groups of 2 [256] 146 / 103 / 101,
-//     16 x 512 [512] 142 / 97 / 76
-//   head_dim 128: 1 x 3584 in groups of 2 [448] 129 / 82 / 92, 2 x 2048 [512] 110 / 63 / 57
+//   head_dim  64: 8 x 512 tokens [256] 21.1 / 16.7 / 18.0, 16 [512] 35.7 / 22.1 / 22.2,
+//     32 [1024] 59.6 / 34.3 / 28.1; 6 x 2048 [768] 88.6 / 71.2 / 70.8; 48 chunks of up to
+//     300 behind up to 3000 keys, groups of 4 [436] 60.8 / 51.3 / 68.4, 64 [550] 86.5 /
+//     81.8 / 83.0
+//   head_dim 256: 2 x 512 [64] 26.6 / 29.9 / 42.7, 2 x 2048 in groups of 2 [256] 167 / 121 /
+//     129, 16 x 512 [512] 157 / 104 / 85.5
+//   head_dim 128: 1 x 3584 in groups of 2 [448] 156 / 105 / 123, 2 x 2048 [512] 129 / 81 / 79
 int seq_mfma_packed_rows(const int64_t counts[3], int Hkv, int D) {
   const int64_t tiles = counts[1] * Hkv;
   if (counts[2] <= 32 || tiles <= 64) return 32;

@@ -91,8 +91,8 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
     // keys.  Where all run at once every other 32 of them, one for each CU, are taken in
     // reverse, so that no CU gets each time the most of 32 falling numbers of keys.
     // 48 chunks of up to 300 queries behind up to 3000 keys, fp16, head_dim 64 in groups
-    // of 4: parts apart 56 us, together 44, and reversed 43; 71 shorter ones at head_dim 128
-    // 25 / 27 / 22.  (Reversed with four times as many workgroups: 481 -> 496.)
+    // of 4: 59.9 us, reversed 56.4; 71 of 150 behind 1500, bf16, head_dim 128 51.2, 49.7.
+    // (Reversed with four times as many workgroups: 689 -> 712.)
     unsigned u = blockIdx.x >> 3;
     if (gridDim.x <= kAtOnce && (u & 32u) != 0 && (u | 31u) < gridDim.x >> 3) u ^= 31u;
     const unsigned part = u % (unsigned)a.nrb;
