@@ -45,7 +45,8 @@ class PackedLayout:
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: PackedLayout,
                      scale: float | None = None) -> torch.Tensor:
     """Causal attention of q (Nq, H, D) over k, v (Nk, Hkv, D), within each sequence of
-    ``layout``; query head h reads key head h // (H / Hkv).  scale: 1 / sqrt(D) by default.
+    ``layout``; query head h reads key head h // (H / Hkv).  scale: 1 / sqrt(D) by default,
+    any other acts as its fp32 value, for fp64 tensors too.
     A query that sees no key gets zeros, and so do rows behind the last sequence."""
     y = torch.empty_like(q, memory_format=torch.contiguous_format)
     if scale is None:

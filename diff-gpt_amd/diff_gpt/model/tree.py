@@ -52,7 +52,8 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ``lengths[b]`` cached positions (one int for all rows, or a (B,) int32 tensor, taken as
     0 .. Tcap - N) and the N tokens behind them, of which token n sees those in its mask
     ((N,) or (B, N) int64, tree_masks; None: the tokens before it and itself).  Query head h
-    reads key head h // (H / Hkv).  scale: 1 / sqrt(D) by default."""
+    reads key head h // (H / Hkv).  scale: 1 / sqrt(D) by default, any other acts as its fp32
+    value, for fp64 tensors too."""
     y = torch.empty_like(q, memory_format=torch.contiguous_format)
     if scale is None:
         scale = 1.0 / math.sqrt(max(1, q.size(-1)))

@@ -595,7 +595,9 @@ DG_API int dg_draw_argmax(int64_t M, int V, int dtype, const void* probs, int64_
  * over such a batch.  A tile that does not lie inside Nq and Nk rows is skipped, never
  * followed.
  * fp32 / bf16 / fp16 / fp64, every head_dim up to 1024, rows with unit stride over d; the
- * scale is positive and below 2^127.  A sequence has at most 2^30 keys and (query, head of the group) rows.
+ * scale is positive and below 2^127.  Outputs are summed in fp32 (fp64 for fp64) before they
+ * are divided by the row's sum of weights, a key's weight being 2^9 at most (fp16 2^16): the
+ * largest |v| times that and the number of keys has to stay within its range.  A sequence has at most 2^30 keys and (query, head of the group) rows.
  * The table's entries times Hkv, or 2, 4 or 8 times that where tiles are split over
  * workgroups, stay below 2^24 (the launch has 2^32 - 1 threads at most); more is refused.
  */
