@@ -1,0 +1,278 @@
+// Attention over a cache in pages (dg_paged_attention): the entry point, the split of long
+// rows, the forms of any shape and type of the attention (seq_tile_kernel's, dg_seq_tile.h) and
+// of the positions' weights (paged_weights_any_kernel), and the joins.  Rows of whole 16-byte
+// pieces up to 256 dims in 16-bit types, 128 in fp32, run on the matrix cores
+// (dg_attn_paged_mfma.hip).
+#include "dg_paged.h"
+#include "dg_seq_tile.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace dg {
+
+// w[t] += sum over the rows r of one key head of exp(s_rt - lse_r), 64 positions a workgroup
+// by 32 rows at a time: a thread has one position and every fourth row, keys and rows pass
+// through LDS in chunks of 64 dims.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_weights_any_kernel(const SeqArgs a, const PagedWeights w) {
+  using S = SeqAcc<T>;
+  using A = typename S::type;
+  constexpr int KT = 64, RT = 32, RPT = RT / 4, CS = 65;
+  __shared__ A ks[KT * CS], qs[RT * 64], part[4 * KT];
+  const int blk = (int)(blockIdx.x % (unsigned)w.blocks);
+  const int64_t u = blockIdx.x / (unsigned)w.blocks;
+  const int64_t b = u / a.Hkv;
+  const int kvh = (int)(u - b * a.Hkv);
+  const PagedRow pr = paged_row(a, b, __builtin_amdgcn_readfirstlane(a.lens[b]));
+  const int total = pr.own + pr.count, nrows = pr.count * a.G;
+  const int kb = blk * KT;
+  if (kb >= total || nrows == 0) return;  // whole workgroups
+  const int tid = threadIdx.x, key = tid & 63, sub = tid >> 6;
+  const int t = kb + key;
+  const int from = t >= total ? nrows : (int)max((int64_t)(t - pr.own) * a.G, (int64_t)0);
+  const int first = max(kb - pr.own, 0) * a.G / RT * RT;
+  const T* const qb = static_cast<const T*>(a.q) + b * a.qb + (int64_t)kvh * a.G * a.qh;
+  const T* const kh = static_cast<const T*>(a.k) + (int64_t)kvh * a.kh;
+  const A* const lse = static_cast<const A*>(a.lse) + (b * a.Hkv + kvh) * (int64_t)(a.N * a.G);
+  const A us = S::unit_scale(a);
+  A acc = (A)0, rest = (A)0;
+  for (int row0 = first; row0 < nrows; row0 += RT) {
+    A s[RPT];
+#pragma unroll
+    for (int j = 0; j < RPT; ++j) s[j] = (A)0;
+    for (int d0 = 0; d0 < a.D; d0 += 64) {
+      __syncthreads();
+      for (int e = tid; e < KT * 64; e += 256) {
+        const int kt = kb + e / 64, d = d0 + e % 64;
+        A x = (A)0;
+        if (kt < total && d < a.D) {
+          const int id = a.table[b * a.table_ld + (kt >> a.page_log2)];
+          if (id >= 0 && id < a.pages) x = S::load(kh[id * a.kb + (kt & ((1 << a.page_log2) - 1)) * a.kt + d]);
+        }
+        ks[e / 64 * CS + e % 64] = x;
+      }
+      for (int e = tid; e < RT * 64; e += 256) {
+        const int row = row0 + e / 64, d = d0 + e % 64, qi = row / a.G;
+        qs[e] = row < nrows && d < a.D ? S::load(qb[qi * a.qt + (int64_t)(row - qi * a.G) * a.qh + d]) : (A)0;
+      }
+      __syncthreads();
+      for (int d = 0; d < 64; ++d) {
+        const A k = ks[key * CS + d];
+#pragma unroll
+        for (int j = 0; j < RPT; ++j) s[j] += k * qs[(sub + 4 * j) * 64 + d];
+      }
+    }
+    A sum = (A)0;
+#pragma unroll
+    for (int j = 0; j < RPT; ++j) {
+      const int row = row0 + sub + 4 * j;
+      if (row >= from && row < nrows) sum += S::exp(s[j] * us - lse[row]);
+    }
+    add_rounded(acc, rest, sum);
+  }
+  part[sub * KT + key] = acc - rest;
+  __syncthreads();
+  if (sub == 0 && t < total) {
+    float* const o = w.out + b * w.wb + (int64_t)kvh * w.wh + t;
+    *o = (float)((A)*o + ((part[key] + part[KT + key]) + (part[2 * KT + key] + part[3 * KT + key])));
+  }
+}
+
+namespace {
+
+template <typename T>
+int launch_tile(const SeqArgs& a, dim3 grid, hipStream_t s) {
+#define DG_PAGED_TILE(NCH, LPR) hipLaunchKernelGGL((seq_tile_kernel<T, NCH, LPR, kPaged>), grid, dim3(256), 0, s, a)
+  if (a.rows_per_wg == 32) {
+    if (a.D <= 64) DG_PAGED_TILE(1, 8);
+    else if (a.D <= 128) DG_PAGED_TILE(2, 8);
+    else DG_PAGED_TILE(4, 8);
+  } else if (a.rows_per_wg == 16) {
+    DG_PAGED_TILE(16, 16);
+  } else {
+    if (a.D <= 128) DG_PAGED_TILE(2, 32);
+    else if (a.D <= 256) DG_PAGED_TILE(4, 32);
+    else DG_PAGED_TILE(16, 32);
+  }
+#undef DG_PAGED_TILE
+  return check_launch("seq_tile_paged");
+}
+
+template <typename T, int WPR>
+void launch_join4(const SeqArgs& a, dim3 grid, int64_t rows, hipStream_t s) {
+  const int D = seq_mfma_dim(a.D);
+  if (D == 16) hipLaunchKernelGGL((seq_join4_kernel<T, 16, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
+  else if (D == 32) hipLaunchKernelGGL((seq_join4_kernel<T, 32, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
+  else if (D == 64) hipLaunchKernelGGL((seq_join4_kernel<T, 64, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
+  else if (D == 128) hipLaunchKernelGGL((seq_join4_kernel<T, 128, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
+  else hipLaunchKernelGGL((seq_join4_kernel<T, 256, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
+}
+
+template <typename T>
+int launch_join(const SeqArgs& a, bool mfma, bool many, dim3 grid, int64_t rows, hipStream_t s) {
+  if constexpr (sizeof(T) < 8) {
+    if (mfma) {
+      if (many) launch_join4<T, 4>(a, grid, rows, s);
+      else launch_join4<T, 1>(a, grid, rows, s);
+      return check_launch("seq_join4_paged");
+    }
+  }
+  if (many) hipLaunchKernelGGL((seq_join_kernel<T, 4, kPaged>), grid, dim3(256), 0, s, a, rows);
+  else hipLaunchKernelGGL((seq_join_kernel<T, 1, kPaged>), grid, dim3(256), 0, s, a, rows);
+  return check_launch("seq_join_paged");
+}
+
+// Rows of a workgroup: few (token, head) rows as a tree's, many as a packed batch's.
+int mfma_rows(int64_t B, int64_t rows, int Hkv, int keys, int D, int dtype) {
+  if (rows <= 128) return seq_mfma_tree_rows(B, (int)rows, Hkv, keys, D, dtype);
+  const int64_t counts[3] = {0, B * ((rows + 127) / 128), 128};
+  return seq_mfma_packed_rows(counts, Hkv, D);
+}
+
+// Row blocks, splits and workspace of a call.
+struct PagedShape {
+  int rows_per_wg, nrb, nsplit, chunk;
+  size_t o_bytes, lse_at, ws_bytes;
+};
+
+constexpr int kMaxSplits = 512;
+
+// Splits: enough workgroups to fill the CUs, and no fewer keys each than `least` stages, as
+// for a tree (dg_attn_seq.hip has the times): a row's own length decides how many it uses.
+PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64_t longest, int weights, int rows_per_wg,
+                       bool mfma) {
+  PagedShape t{};
+  const int64_t R = (int64_t)N * (H / Hkv);
+  t.rows_per_wg = rows_per_wg;
+  t.nrb = (int)((R + rows_per_wg - 1) / rows_per_wg);
+  const int Dm = mfma ? seq_mfma_dim(D) : D;
+  const int64_t row_bytes = Dm * dtype_bytes(dtype);
+  const int64_t fill = !mfma ? 2048
+                       : rows_per_wg <= 32 ? (row_bytes >= 256 ? 256 : 512)
+                       : rows_per_wg == 64 ? (row_bytes >= 512 ? 256 : 512)
+                                           : Dm == 256 ? 512 : Dm == 128 ? 768 : 1024;
+  const int64_t least = !mfma ? 256 : dtype == DG_F32 && Dm >= 64 ? 128 : 1024;
+  const int64_t wg = std::max<int64_t>(1, B * Hkv * t.nrb);
+  int64_t want = (fill + wg - 1) / wg;
+  want = std::min<int64_t>({want, (longest + least - 1) / least, kMaxSplits});
+  t.nsplit = (int)std::max<int64_t>(want, 1);
+  t.chunk = (int)least;
+  const size_t acc = dtype == DG_F64 ? 8 : 4;
+  const size_t parts = (size_t)(B * Hkv * R) * t.nsplit;
+  if (t.nsplit > 1) {
+    t.o_bytes = (parts * Dm * acc + 15) & ~(size_t)15;
+    t.ws_bytes = t.o_bytes + ((parts * 2 * acc + 15) & ~(size_t)15);
+  }
+  t.lse_at = t.ws_bytes;
+  if (weights) t.ws_bytes += (size_t)(B * Hkv * R) * acc;
+  return t;
+}
+
+int tile_rows(int64_t rows, int D) { return rows <= 8 ? 8 : D <= 256 ? 32 : 16; }
+
+bool known_dtype(int dtype) { return dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64; }
+
+}  // namespace
+
+int check_paged_rows(const char* what, const dg_paged_rows* r, bool need_v, int* log2) {
+  DG_REQUIRE(r != nullptr && r->k && (r->v || !need_v) && r->table && r->lens, DG_EINVAL, "%s: NULL argument", what);
+  DG_REQUIRE(r->pages >= 1 && r->pages <= 0x7fffffff, DG_EINVAL, "%s: %lld pages", what, (long long)r->pages);
+  DG_REQUIRE(r->page >= 1 && r->page <= kMostPositions && (r->page & (r->page - 1)) == 0, DG_EINVAL,
+             "%s: a page of %lld positions, not a power of two", what, (long long)r->page);
+  DG_REQUIRE(r->width >= 1 && r->width <= kMostPositions / r->page, DG_EINVAL,
+             "%s: a table of %lld pages of %lld positions, 1 to 2^30 positions", what, (long long)r->width, (long long)r->page);
+  *log2 = 0;
+  while (((int64_t)1 << *log2) < r->page) ++*log2;
+  return DG_OK;
+}
+
+}  // namespace dg
+
+using namespace dg;
+
+extern "C" size_t dg_paged_attention_workspace_size(int B, int N, int H, int Hkv, int D, int dtype, int64_t longest,
+                                                    int weights) {
+  if (B <= 0 || N <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || !known_dtype(dtype)) return 0;
+  const int64_t R = (int64_t)N * (H / Hkv);
+  if (R > kMostPositions) return 0;
+  const int64_t keys = std::min<int64_t>(std::max<int64_t>(longest, 1), kMostPositions);
+  size_t most = paged_shape(B, N, H, Hkv, D, dtype, keys, weights, tile_rows(R, D), false).ws_bytes;
+  if (D <= 256)
+    most = std::max(most, paged_shape(B, N, H, Hkv, D, dtype, keys, weights, mfma_rows(B, R, Hkv, (int)keys, D, dtype), true).ws_bytes);
+  return most;
+}
+
+extern "C" int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
+                                  const void* q, const dg_stride3* q_st, void* y, const dg_stride3* y_st, float scale,
+                                  int64_t longest, float* weights, int64_t w_b, int64_t w_h, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  DG_REQUIRE(B >= 0 && N >= 0 && H >= 0, DG_EINVAL, "paged_attention: negative size");
+  DG_REQUIRE(known_dtype(dtype), DG_EUNSUPPORTED, "paged_attention: dtype %d unsupported", dtype);
+  DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_attention: head_dim %d outside [1, %d]", D, kMaxHeadDim);
+  DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "paged_attention: %d query heads on %d key heads", H, Hkv);
+  DG_REQUIRE((int64_t)N * (H / Hkv) <= kMostPositions, DG_EINVAL, "paged_attention: a row of more than 2^30 (token, head) rows");
+  DG_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), DG_EINVAL, "paged_attention: the scale must be positive and below 2^127");
+  if (B == 0 || N == 0 || H == 0) return DG_OK;
+  SeqArgs a{};
+  if (const int rc = check_paged_rows("paged_attention", rows, true, &a.page_log2)) return rc;
+  DG_REQUIRE(q && y && q_st && y_st, DG_EINVAL, "paged_attention: NULL argument");
+  const int64_t cap = rows->width * rows->page;
+  DG_REQUIRE(longest >= 1 && longest <= cap, DG_EINVAL, "paged_attention: longest %lld, the table covers %lld positions",
+             (long long)longest, (long long)cap);
+  a.q = q; a.k = rows->k; a.v = rows->v; a.y = y;
+  a.qb = q_st->b; a.qt = q_st->t; a.qh = q_st->h;
+  a.kb = rows->k_st.b; a.kt = rows->k_st.t; a.kh = rows->k_st.h;
+  a.vb = rows->v_st.b; a.vt = rows->v_st.t; a.vh = rows->v_st.h;
+  a.yb = y_st->b; a.yt = y_st->t; a.yh = y_st->h;
+  a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
+  a.scale = scale;
+  a.scale_log2 = scale * kLog2e;
+  a.B = B; a.N = N; a.Tcap = (int)cap;
+  a.lens = rows->lens; a.counts = rows->counts;
+  a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;
+  const int64_t R = (int64_t)N * a.G;
+  const bool mfma = seq_mfma_applicable(a, dtype, true);
+  const PagedShape t = paged_shape(B, N, H, Hkv, D, dtype, longest, weights != nullptr,
+                                   mfma ? mfma_rows(B, R, Hkv, (int)longest, D, dtype) : tile_rows(R, D), mfma);
+  a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
+  if (t.ws_bytes > 0) {
+    DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,
+               "paged_attention: a workspace of %zu bytes, %zu needed", workspace_bytes, t.ws_bytes);
+    DG_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, DG_EINVAL, "paged_attention: workspace not 16-byte aligned");
+    a.ws_o = workspace;
+    a.ws_ml = static_cast<char*>(workspace) + t.o_bytes;
+    if (weights != nullptr) a.lse = static_cast<char*>(workspace) + t.lse_at;
+  }
+  const int64_t nrows = (int64_t)B * Hkv * R;
+  const bool many = t.nsplit >= 16 && nrows <= 4096;
+  const int64_t groups = t.nsplit == 1 ? 0 : many ? nrows : (nrows + 3) / 4;
+  const int64_t blocks = ((int64_t)B * Hkv * t.nsplit + 7) / 8 * 8 * t.nrb;
+  PagedWeights w{weights, w_b, w_h, 0};
+  const int wkeys = mfma ? kWeightKeys : 64;
+  w.blocks = (int)((cap + wkeys - 1) / wkeys);
+  const int64_t wblocks = weights == nullptr ? 0 : mfma ? ((int64_t)B * Hkv + 7) / 8 * 8 * w.blocks : (int64_t)B * Hkv * w.blocks;
+  DG_REQUIRE(blocks <= kMostWorkgroups256 && groups <= kMostWorkgroups256 && wblocks <= kMostWorkgroups256, DG_EINVAL,
+             "paged_attention: more than 2^24 - 1 workgroups");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)blocks), jgrid((unsigned)groups), wgrid((unsigned)wblocks);
+  int rc;
+  if (mfma) rc = launch_seq_mfma_paged(a, dtype, (unsigned)blocks, s);
+  else if (dtype == DG_F64) rc = launch_tile<double>(a, grid, s);
+  else if (dtype == DG_F32) rc = launch_tile<float>(a, grid, s);
+  else if (dtype == DG_BF16) rc = launch_tile<bf16_t>(a, grid, s);
+  else rc = launch_tile<f16_t>(a, grid, s);
+  if (rc == DG_OK && t.nsplit > 1) {
+    if (dtype == DG_F64) rc = launch_join<double>(a, mfma, many, jgrid, nrows, s);
+    else if (dtype == DG_F32) rc = launch_join<float>(a, mfma, many, jgrid, nrows, s);
+    else if (dtype == DG_BF16) rc = launch_join<bf16_t>(a, mfma, many, jgrid, nrows, s);
+    else rc = launch_join<f16_t>(a, mfma, many, jgrid, nrows, s);
+  }
+  if (rc != DG_OK || weights == nullptr) return rc;
+  if (mfma) return launch_paged_weights_mfma(a, w, dtype, (unsigned)wblocks, s);
+  if (dtype == DG_F64) hipLaunchKernelGGL(paged_weights_any_kernel<double>, wgrid, dim3(256), 0, s, a, w);
+  else if (dtype == DG_F32) hipLaunchKernelGGL(paged_weights_any_kernel<float>, wgrid, dim3(256), 0, s, a, w);
+  else if (dtype == DG_BF16) hipLaunchKernelGGL(paged_weights_any_kernel<bf16_t>, wgrid, dim3(256), 0, s, a, w);
+  else hipLaunchKernelGGL(paged_weights_any_kernel<f16_t>, wgrid, dim3(256), 0, s, a, w);
+  return check_launch("paged_weights_any_kernel");
+}

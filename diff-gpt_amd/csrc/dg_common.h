@@ -544,6 +544,12 @@ __device__ __forceinline__ void lds_copy16_buf(__amdgpu_buffer_rsrc_t rs, int vo
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
 }
 
+// The same from an address of each lane's own, anywhere in memory.
+__device__ __forceinline__ void lds_copy16(const void* p, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
 // The 16 accumulators of a 32 x 32 MFMA block: lane l, register r holds row
 // 8*(r/4) + 4*(l/32) + r%4 of column l%32.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16_t;

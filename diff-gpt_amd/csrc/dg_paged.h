@@ -1,0 +1,26 @@
+// Shared by the entry points over a cache in pages (dg_paged.hip, dg_attn_paged.hip,
+// dg_attn_paged_mfma.hip).
+#pragma once
+
+#include "dg_seq.h"
+
+namespace dg {
+
+// What every entry point asks of a dg_paged_rows; *log2 receives that of its page.
+int check_paged_rows(const char* what, const dg_paged_rows* r, bool need_v, int* log2);
+
+// dg_attn_paged_mfma.hip: attention of workgroups of 32, 64 or 128 (token, head) rows, and the
+// positions' weights, for shapes that seq_mfma_applicable takes.
+int launch_seq_mfma_paged(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s);
+
+// The weights' arguments: a.q, a.k, the table and lengths as for the attention, a.lse its
+// result; a.nrb is unused.
+struct PagedWeights {
+  float* out;
+  int64_t wb, wh;
+  int blocks;  // key blocks of a (b, key head)
+};
+constexpr int kWeightKeys = 128;  // positions of a workgroup
+int launch_paged_weights_mfma(const SeqArgs& a, const PagedWeights& w, int dtype, unsigned blocks, hipStream_t s);
+
+}  // namespace dg

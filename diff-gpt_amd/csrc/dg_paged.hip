@@ -1,0 +1,480 @@
+// A cache in pages: new keys and values into the rows' pages, rotated and normalised
+// (dg_paged_append), and rows cut to their newest positions and those of the largest weights
+// (dg_paged_evict).
+//
+// paged_append_kernel.  y = r / sqrt(mean(r^2) + eps), r the pairs of a head turned by their
+// position's angle: both in fp32 (fp64) registers, one rounding as y is stored.  (The cache of
+// one length, dg_rope.hip, rounds r to the data's type first, as the reference does; once is
+// nearer to the exact value, bf16 1.7e-3 of it, and no dearer.)  LPR lanes share a head, 16 bytes
+// each; they take HPT heads of a token, whose loads are in flight together and whose angles
+// are read once.  Bound by HBM where tokens are many, by the launch where they are few.
+//
+// paged_select_kernel.  The m-th largest weight of a row by its bits: three passes of 11, 11
+// and 10 over an order-preserving integer, counted in LDS, then one that ranks what is above
+// it and the first of those that equal it.  One workgroup a (row, key head), each wave with a
+// stretch of the positions, so that ranks come from ballots and one exchange.
+// paged_move_kernel then copies the kept positions, 16 bytes a thread.
+#include "dg_paged.h"
+
+#include <float.h>
+
+#include <algorithm>
+
+namespace dg {
+
+struct AppendArgs {
+  const void* src[3];  // q, k, v
+  int64_t sb[3], st[3], sh[3];
+  void* dst[3];  // q_out, the pages' k and v
+  int64_t db[3], dt[3], dh[3];
+  const void* freqs;
+  int64_t freqs_ld, freqs_rows;
+  const int32_t* table;
+  int64_t table_ld, pages;
+  const int32_t* lens;
+  const int32_t* counts;
+  const int32_t* positions;
+  int64_t items;
+  int N, H, Hkv, D, cap, page_log2, groups, qknorm;
+};
+
+// N values of T from p: by 16-byte loads (VEC, p aligned to them), or one by one those below `n`.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_some(const T* p, T (&x)[N], int n) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int c = 0; c < N * (int)sizeof(T) / 16; ++c) {
+      const u32x4_t w = reinterpret_cast<const u32x4_t*>(p)[c];
+      __builtin_memcpy(reinterpret_cast<char*>(x) + 16 * c, &w, 16);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      x[e] = T{};
+      if (e < n) x[e] = p[e];
+    }
+  }
+}
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void store_some(T* p, const T (&x)[N], int n) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int c = 0; c < N * (int)sizeof(T) / 16; ++c) {
+      u32x4_t w;
+      __builtin_memcpy(&w, reinterpret_cast<const char*>(x) + 16 * c, 16);
+      reinterpret_cast<u32x4_t*>(p)[c] = w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < n) p[e] = x[e];
+  }
+}
+
+template <typename T>
+struct AppendAcc {
+  using type = float;
+  __device__ static float load(T x) { return to_f32(x); }
+  __device__ static T store(float x) { return from_f32<T>(x); }
+};
+template <>
+struct AppendAcc<double> {
+  using type = double;
+  __device__ static double load(double x) { return x; }
+  __device__ static double load(float x) { return x; }
+  __device__ static double store(double x) { return x; }
+};
+
+// EPL consecutive dims a lane and piece, LPR lanes a head, NCK pieces, HPT heads of a token.
+template <typename T, typename FT, int EPL, int LPR, int NCK, int HPT, bool VEC>
+__global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
+  using S = AppendAcc<T>;
+  using A = typename S::type;
+  const int sub = threadIdx.x % LPR;
+  const uint32_t item = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;  // below 2^31
+  if (item >= a.items) return;  // whole lane groups; no barriers follow
+  const uint32_t token = item / (uint32_t)a.groups;
+  const int h0 = (int)(item - token * (uint32_t)a.groups) * HPT;
+  const int64_t b = token / (uint32_t)a.N;
+  const int n = (int)(token - (uint32_t)b * (uint32_t)a.N);
+  const int heads = a.H + 2 * a.Hkv;
+
+  // the token's heads, which no length decides where to read
+  T x[HPT][NCK][EPL];
+#pragma unroll
+  for (int j = 0; j < HPT; ++j) {
+    const int h = min(h0 + j, heads - 1);
+    const int w = h < a.H ? 0 : h < a.H + a.Hkv ? 1 : 2;
+    const int hw = w == 0 ? h : w == 1 ? h - a.H : h - a.H - a.Hkv;
+    const T* p = static_cast<const T*>(a.src[w]) + b * a.sb[w] + n * a.st[w] + hw * a.sh[w];
+#pragma unroll
+    for (int c = 0; c < NCK; ++c) {
+      const int d = EPL * (sub + LPR * c);
+      if (d < a.D) {
+        load_some<T, EPL, VEC>(p + d, x[j][c], a.D - d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x[j][c][e] = T{};
+      }
+    }
+  }
+  const int len = a.lens[b];
+  const int own = min(max(len, 0), a.cap);
+  const int count = min(max(a.counts != nullptr ? a.counts[b] : a.N, 0), min(a.N, a.cap - own));
+  const bool there = n < count;
+  const int slot = own + n;
+  const int64_t pos = (int64_t)(a.positions != nullptr ? a.positions[b] : own) + n;
+  const bool known = pos >= 0 && pos < a.freqs_rows;
+  int id = -1;
+  if (there) id = a.table[b * a.table_ld + (slot >> a.page_log2)];
+  const bool held = id >= 0 && id < a.pages;
+  const int in_page = slot & ((1 << a.page_log2) - 1);
+  FT cs[NCK][EPL];
+#pragma unroll
+  for (int c = 0; c < NCK; ++c) {
+    const int d = EPL * (sub + LPR * c);
+    if (d < a.D) {
+      load_some<FT, EPL, VEC>(static_cast<const FT*>(a.freqs) + (known ? pos : 0) * a.freqs_ld + d, cs[c], a.D - d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) cs[c][e] = FT{};
+    }
+  }
+
+#pragma unroll
+  for (int j = 0; j < HPT; ++j) {
+    const int h = h0 + j;
+    if (h >= heads) break;  // the same in all of the group's lanes
+    const int w = h < a.H ? 0 : h < a.H + a.Hkv ? 1 : 2;
+    const int hw = w == 0 ? h : w == 1 ? h - a.H : h - a.H - a.Hkv;
+    if (w < 2) {
+      A y[NCK][EPL], ss = (A)0;
+#pragma unroll
+      for (int c = 0; c < NCK; ++c)
+#pragma unroll
+        for (int e = 0; e < EPL; e += 2) {
+          const A re = S::load(x[j][c][e]), im = S::load(x[j][c][e + 1]);
+          const A co = AppendAcc<FT>::load(cs[c][e]), si = AppendAcc<FT>::load(cs[c][e + 1]);
+          y[c][e] = re * co - im * si;
+          y[c][e + 1] = re * si + im * co;
+          ss += y[c][e] * y[c][e] + y[c][e + 1] * y[c][e + 1];
+        }
+      A f = (A)1;
+      if (a.qknorm) {
+#pragma unroll
+        for (int off = 1; off < LPR; off <<= 1) ss += __shfl_xor(ss, off, 64);
+        f = (A)1 / sqrt(ss / (A)a.D + (A)FLT_EPSILON);
+      }
+      if (!known) f = (A)__builtin_nanf("");
+#pragma unroll
+      for (int c = 0; c < NCK; ++c)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x[j][c][e] = there ? S::store(y[c][e] * f) : T{};
+    }
+    if (w > 0 && !held) continue;
+    T* o = static_cast<T*>(a.dst[w]) + hw * a.dh[w];
+    o += w == 0 ? b * a.db[w] + n * a.dt[w] : id * a.db[w] + in_page * a.dt[w];
+#pragma unroll
+    for (int c = 0; c < NCK; ++c) {
+      const int d = EPL * (sub + LPR * c);
+      if (d < a.D) store_some<T, EPL, VEC>(o + d, x[j][c], a.D - d);
+    }
+  }
+}
+
+struct EvictArgs {
+  const float* weights;
+  int64_t wb, wh;
+  const int32_t* table;
+  int64_t table_ld, pages;
+  const int32_t* to;
+  int64_t to_ld, to_cap;
+  const int32_t* lens;
+  int32_t* new_lens;
+  float* new_weights;
+  int32_t* kept;
+  const char* k;
+  const char* v;
+  int64_t kb, kt, kh, vb, vt, vh;  // bytes
+  int Hkv, cap, keep, recent, page_log2, pieces;
+  int64_t items;
+};
+
+// Larger for larger weights: the order of the bits, zeros of both signs alike, NaN above all.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kSelectBins = 2048;
+
+__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const EvictArgs a) {
+  __shared__ uint32_t hist[kSelectBins];
+  __shared__ uint32_t found[2];
+  __shared__ int above[kSelectWaves], equal[kSelectWaves];
+  const int64_t bh = blockIdx.x;
+  const int64_t b = bh / a.Hkv;
+  const int h = (int)(bh - b * a.Hkv);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int len = min(max(a.lens[b], 0), a.cap);
+  int32_t* const kept = a.kept + bh * a.keep;
+  if (h == 0 && tid == 0) a.new_lens[b] = min(len, a.keep);
+  if (len <= a.keep) {
+    for (int j = tid; j < a.keep; j += kSelectThreads) kept[j] = j < len ? j : -1;
+    return;  // whole workgroups, before any barrier
+  }
+  const int old = len - a.recent;
+  const int m = a.keep - a.recent;  // below old
+  for (int j = tid; j < a.recent; j += kSelectThreads) kept[m + j] = old + j;
+  if (m == 0) return;
+  const float* const w = a.weights + b * a.wb + (int64_t)h * a.wh;
+
+  // a wave's stretch of the positions, in whole 64
+  const int per = ((old + 63) / 64 + kSelectWaves - 1) / kSelectWaves * 64;
+  const int t0 = min(wv * per, old), t1 = min(t0 + per, old);
+
+  uint32_t prefix = 0, need = (uint32_t)m;
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t bins = pass == 2 ? 1024 : 2048;
+    for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
+    __syncthreads();
+    for (int t = t0; t < t1; t += 64) {
+      bool in = t + lane < t1;
+      const uint32_t key = in ? weight_key(w[t + lane]) : 0u;
+      if (pass > 0) in = in && (pass == 1 ? key >> 21 : key >> 10) == (pass == 1 ? prefix >> 21 : prefix >> 10);
+      const uint32_t bin = (key >> shift) & (bins - 1);
+      // many positions may share one value (zero): the lanes of the first one's are counted at once
+      const uint64_t live = __builtin_amdgcn_ballot_w64(in);
+      if (live == 0) continue;
+      const int lead = __builtin_ctzll(live);
+      const uint32_t common = __shfl(bin, lead, 64);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == common);
+      if (lane == lead) atomicAdd(&hist[common], (uint32_t)__builtin_popcountll(same));
+      if (in && bin != common) atomicAdd(&hist[bin], 1u);
+    }
+    __syncthreads();
+    if (wv == 0) {
+      // the bin that holds the need-th largest: lane l has bins 32 l .. from the top down
+      uint32_t mine = 0;
+      for (int i = 0; i < kSelectBins / 64; ++i) mine += hist[kSelectBins - 1 - (32 * lane + i)];
+      uint32_t upto = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t x = __shfl_up(upto, off, 64);
+        if (lane >= off) upto += x;
+      }
+      if (upto >= need && upto - mine < need) {
+        uint32_t c = upto - mine;
+        int i = kSelectBins - 1 - 32 * lane;
+        while (c + hist[i] < need) c += hist[i--];
+        found[0] = (uint32_t)i;
+        found[1] = c;
+      }
+    }
+    __syncthreads();
+    prefix |= found[0] << shift;
+    need -= found[1];
+    __syncthreads();  // found is read before the next pass writes it
+  }
+
+  // positions above the m-th largest weight, and the first `need` that equal it
+  int na = 0, ne = 0;
+  for (int t = t0; t < t1; t += 64) {
+    const bool in = t + lane < t1;
+    const uint32_t key = in ? weight_key(w[t + lane]) : 0u;
+    na += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && key > prefix));
+    ne += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && key == prefix));
+  }
+  if (lane == 0) {
+    above[wv] = na;
+    equal[wv] = ne;
+  }
+  __syncthreads();
+  int at = 0, eq = 0;
+  for (int i = 0; i < wv; ++i) {
+    at += above[i];
+    eq += equal[i];
+  }
+  at += min(eq, (int)need);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int t = t0; t < t1; t += 64) {
+    const bool in = t + lane < t1;
+    const uint32_t key = in ? weight_key(w[t + lane]) : 0u;
+    const uint64_t es = __builtin_amdgcn_ballot_w64(in && key == prefix);
+    const bool take = in && (key > prefix || (key == prefix && eq + __builtin_popcountll(es & below) < (int)need));
+    const uint64_t ts = __builtin_amdgcn_ballot_w64(take);
+    if (take) kept[at + __builtin_popcountll(ts & below)] = t + lane;
+    at += __builtin_popcountll(ts);
+    eq += __builtin_popcountll(es);
+  }
+}
+
+// One piece of U of one kept position of a key head a thread; the first piece's thread has
+// its weight, and those of the places behind the kept ones.
+template <typename U>
+__global__ __launch_bounds__(256) void paged_move_kernel(const EvictArgs a) {
+  const uint32_t item = blockIdx.x * 256u + threadIdx.x;  // below 2^32
+  if (item >= a.items) return;
+  const uint32_t at = item / (uint32_t)a.pieces;  // (b, h, j)
+  const int piece = (int)(item - at * (uint32_t)a.pieces);
+  const int64_t bh = at / (uint32_t)a.to_cap;
+  const int j = (int)(at - (uint32_t)bh * (uint32_t)a.to_cap);
+  const int64_t b = (uint32_t)bh / (uint32_t)a.Hkv;
+  const int h = (int)(bh - b * a.Hkv);
+  const int t = j < a.keep ? a.kept[bh * a.keep + j] : -1;
+  if (piece == 0) a.new_weights[at] = t < 0 ? 0.f : a.weights[b * a.wb + (int64_t)h * a.wh + t];
+  if (t < 0) return;
+  const int64_t src = a.table[b * a.table_ld + (t >> a.page_log2)];
+  const int64_t dst = a.to[b * a.to_ld + (j >> a.page_log2)];
+  if (dst < 0 || dst >= a.pages) return;
+  const int mask = (1 << a.page_log2) - 1;
+  U xk{}, xv{};
+  if (src >= 0 && src < a.pages) {
+    xk = *reinterpret_cast<const U*>(a.k + src * a.kb + (t & mask) * a.kt + h * a.kh + piece * (int)sizeof(U));
+    xv = *reinterpret_cast<const U*>(a.v + src * a.vb + (t & mask) * a.vt + h * a.vh + piece * (int)sizeof(U));
+  }
+  *reinterpret_cast<U*>(const_cast<char*>(a.k) + dst * a.kb + (j & mask) * a.kt + h * a.kh + piece * (int)sizeof(U)) = xk;
+  *reinterpret_cast<U*>(const_cast<char*>(a.v) + dst * a.vb + (j & mask) * a.vt + h * a.vh + piece * (int)sizeof(U)) = xv;
+}
+
+namespace {
+
+template <typename T, typename FT, int EPL, int LPR, int NCK, int HPT, bool VEC>
+int launch_append(AppendArgs& a, int64_t tokens, hipStream_t s) {
+  a.groups = (a.H + 2 * a.Hkv + HPT - 1) / HPT;
+  a.items = tokens * a.groups;
+  constexpr int PER = 256 / LPR;
+  const int64_t blocks = (a.items + PER - 1) / PER;
+  DG_REQUIRE(blocks <= kMostWorkgroups256, DG_EINVAL, "paged_append: more than 2^24 - 1 workgroups");
+  hipLaunchKernelGGL((paged_append_kernel<T, FT, EPL, LPR, NCK, HPT, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  return check_launch(VEC ? "paged_append_kernel" : "paged_append_any_kernel");
+}
+
+template <typename T, typename FT>
+int append_pick(AppendArgs& a, bool vec, int64_t tokens, hipStream_t s) {
+  constexpr int EPL = 16 / (int)sizeof(T);
+  // one head a lane group where tokens are few, four where their loads are to be in flight together
+  const bool few = tokens * (a.H + 2 * a.Hkv) <= 4096;
+  if (!vec) {
+    if (a.D <= 128) return launch_append<T, FT, 2, 64, 1, 1, false>(a, tokens, s);
+    return launch_append<T, FT, 2, 64, 8, 1, false>(a, tokens, s);
+  }
+  const int lanes = a.D / EPL;
+#define DG_APPEND(LPR)                                                                 \
+  if (lanes <= LPR)                                                                    \
+  return few ? launch_append<T, FT, EPL, LPR, 1, 1, true>(a, tokens, s)                \
+             : launch_append<T, FT, EPL, LPR, 1, 4, true>(a, tokens, s)
+  DG_APPEND(2);
+  DG_APPEND(4);
+  DG_APPEND(8);
+  DG_APPEND(16);
+  DG_APPEND(32);
+  DG_APPEND(64);
+#undef DG_APPEND
+  return launch_append<T, FT, EPL, 64, kMaxHeadDim / EPL / 64, 1, true>(a, tokens, s);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace dg
+
+using namespace dg;
+
+extern "C" int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
+                               const void* q, const dg_stride3* q_st, void* q_out, const dg_stride3* qo_st,
+                               const void* k, const dg_stride3* k_st, const void* v, const dg_stride3* v_st,
+                               const void* freqs, int64_t freqs_ld, int64_t freqs_rows, int freqs_dtype,
+                               const int32_t* positions, int flags, void* stream) {
+  DG_REQUIRE(B >= 0 && N >= 0 && H >= 0 && Hkv >= 0, DG_EINVAL, "paged_append: negative size");
+  DG_REQUIRE(D >= 2 && D % 2 == 0 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_append: head_dim %d, even ones from 2 to %d", D, kMaxHeadDim);
+  DG_REQUIRE(dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64, DG_EUNSUPPORTED,
+             "paged_append: dtype %d unsupported", dtype);
+  DG_REQUIRE(freqs_dtype == DG_F32 || freqs_dtype == dtype, DG_EUNSUPPORTED,
+             "paged_append: freqs dtype must be fp32 or equal to the data dtype");
+  DG_REQUIRE(H <= 0xffff && Hkv <= 0xffff, DG_EINVAL, "paged_append: more than 65535 heads");
+  if (B == 0 || N == 0 || H + Hkv == 0) return DG_OK;
+  AppendArgs a{};
+  if (const int rc = check_paged_rows("paged_append", rows, true, &a.page_log2)) return rc;
+  DG_REQUIRE(H == 0 || (q && q_out && q_st && qo_st), DG_EINVAL, "paged_append: NULL argument");
+  DG_REQUIRE(Hkv == 0 || (k && v && k_st && v_st), DG_EINVAL, "paged_append: NULL argument");
+  DG_REQUIRE(freqs && freqs_rows >= 1 && freqs_ld >= 0, DG_EINVAL, "paged_append: freqs table required");
+  static const dg_stride3 none = {0, 0, 0};
+  const void* src[3] = {q, k, v};
+  const dg_stride3* sst[3] = {H ? q_st : &none, Hkv ? k_st : &none, Hkv ? v_st : &none};
+  void* dst[3] = {q_out, rows->k, rows->v};
+  const dg_stride3* dst_st[3] = {H ? qo_st : &none, &rows->k_st, &rows->v_st};
+  const int64_t es = dtype_bytes(dtype), fes = dtype_bytes(freqs_dtype);
+  bool vec = D * es % 16 == 0 && aligned16(freqs) && freqs_ld * fes % 16 == 0;
+  for (int w = 0; w < 3; ++w) {
+    a.src[w] = src[w];
+    a.sb[w] = sst[w]->b; a.st[w] = sst[w]->t; a.sh[w] = sst[w]->h;
+    a.dst[w] = dst[w];
+    a.db[w] = dst_st[w]->b; a.dt[w] = dst_st[w]->t; a.dh[w] = dst_st[w]->h;
+    vec = vec && aligned16(src[w]) && aligned16(dst[w]);
+    for (int64_t x : {a.sb[w], a.st[w], a.sh[w], a.db[w], a.dt[w], a.dh[w]}) vec = vec && x * es % 16 == 0;
+  }
+  a.freqs = freqs; a.freqs_ld = freqs_ld; a.freqs_rows = freqs_rows;
+  a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;
+  a.lens = rows->lens; a.counts = rows->counts; a.positions = positions;
+  a.N = N; a.H = H; a.Hkv = Hkv; a.D = D;
+  a.cap = (int)(rows->width * rows->page);
+  a.qknorm = (flags & DG_QKNORM) ? 1 : 0;
+  const int64_t tokens = (int64_t)B * N;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == DG_F64)
+    return freqs_dtype == DG_F32 ? append_pick<double, float>(a, vec, tokens, s) : append_pick<double, double>(a, vec, tokens, s);
+  if (dtype == DG_F32) return append_pick<float, float>(a, vec, tokens, s);
+  if (dtype == DG_BF16)
+    return freqs_dtype == DG_F32 ? append_pick<bf16_t, float>(a, vec, tokens, s) : append_pick<bf16_t, bf16_t>(a, vec, tokens, s);
+  return freqs_dtype == DG_F32 ? append_pick<f16_t, float>(a, vec, tokens, s) : append_pick<f16_t, f16_t>(a, vec, tokens, s);
+}
+
+extern "C" int dg_paged_evict(int B, int Hkv, int D, int dtype, const dg_paged_rows* rows, const float* weights,
+                              int64_t w_b, int64_t w_h, int keep, int recent, const int32_t* to, int64_t to_ld,
+                              int64_t to_width, int32_t* new_lens, float* new_weights, int32_t* kept, void* stream) {
+  DG_REQUIRE(B >= 0 && Hkv >= 1, DG_EINVAL, "paged_evict: bad size");
+  DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_evict: head_dim %d outside [1, %d]", D, kMaxHeadDim);
+  DG_REQUIRE(dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64, DG_EUNSUPPORTED,
+             "paged_evict: dtype %d unsupported", dtype);
+  DG_REQUIRE(keep >= 1 && recent >= 0 && recent <= keep, DG_EINVAL, "paged_evict: keep %d positions, %d of them the last", keep, recent);
+  if (B == 0) return DG_OK;
+  EvictArgs a{};
+  if (const int rc = check_paged_rows("paged_evict", rows, true, &a.page_log2)) return rc;
+  DG_REQUIRE(weights && to && new_lens && new_weights && kept, DG_EINVAL, "paged_evict: NULL argument");
+  DG_REQUIRE(to_width >= 1 && to_width <= kMostPositions / rows->page && keep <= to_width * rows->page, DG_EINVAL,
+             "paged_evict: %d positions into %lld pages of %lld", keep, (long long)to_width, (long long)rows->page);
+  const int64_t es = dtype_bytes(dtype);
+  a.weights = weights; a.wb = w_b; a.wh = w_h;
+  a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;
+  a.to = to; a.to_ld = to_ld; a.to_cap = to_width * rows->page;
+  a.lens = rows->lens;
+  a.new_lens = new_lens; a.new_weights = new_weights; a.kept = kept;
+  a.k = static_cast<const char*>(rows->k); a.v = static_cast<const char*>(rows->v);
+  a.kb = rows->k_st.b * es; a.kt = rows->k_st.t * es; a.kh = rows->k_st.h * es;
+  a.vb = rows->v_st.b * es; a.vt = rows->v_st.t * es; a.vh = rows->v_st.h * es;
+  a.Hkv = Hkv; a.cap = (int)(rows->width * rows->page); a.keep = keep; a.recent = recent;
+  // the widest accesses that rows, heads and pages allow
+  int64_t unit = 16;
+  for (int64_t x : {(int64_t)reinterpret_cast<uintptr_t>(a.k), (int64_t)reinterpret_cast<uintptr_t>(a.v), a.kb, a.kt, a.kh, a.vb,
+                    a.vt, a.vh, D * es})
+    while (x % unit != 0) unit >>= 1;
+  DG_REQUIRE(unit >= es, DG_EINVAL, "paged_evict: pages not aligned to their element size");
+  a.pieces = (int)(D * es / unit);
+  a.items = (int64_t)B * Hkv * a.to_cap * a.pieces;
+  const int64_t blocks = (a.items + 255) / 256;
+  DG_REQUIRE(blocks <= kMostWorkgroups256 && (int64_t)B * Hkv <= 0xffffffffll / kSelectThreads, DG_EINVAL,
+             "paged_evict: more than 2^32 - 1 threads");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)(B * Hkv)), dim3(kSelectThreads), 0, s, a);
+  if (const int rc = check_launch("paged_select_kernel")) return rc;
+  const dim3 grid((unsigned)blocks);
+  if (unit == 16) hipLaunchKernelGGL(paged_move_kernel<u32x4_t>, grid, dim3(256), 0, s, a);
+  else if (unit == 8) hipLaunchKernelGGL(paged_move_kernel<u32x2_t>, grid, dim3(256), 0, s, a);
+  else if (unit == 4) hipLaunchKernelGGL(paged_move_kernel<uint32_t>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(paged_move_kernel<uint16_t>, grid, dim3(256), 0, s, a);
+  return check_launch("paged_move_kernel");
+}

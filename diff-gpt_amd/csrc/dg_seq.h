@@ -12,6 +12,11 @@
 
 namespace dg {
 
+// packed: whole sequences one after the other; tree: up to 64 tokens a row over its cache,
+// each with a mask; paged: any number of tokens a row, each seeing what lies before it, over
+// a cache in pages
+enum SeqMode { kPacked, kTree, kPaged };
+
 struct SeqArgs {
   const void* q;
   const void* k;
@@ -41,6 +46,16 @@ struct SeqArgs {
   // (b * Hkv + key head) * N * G + r
   void* ws_o;
   void* ws_ml;
+  // paged: position t of row b lies in page table[b * table_ld + (t >> page_log2)] of `pages`,
+  // kb / vb elements apart; `lens` cached positions and `counts` (null: N) tokens behind them.
+  // Tcap positions a table row covers; `chunk` is the fewest keys of a split.
+  const int32_t* table;
+  int64_t table_ld, pages;
+  int page_log2;
+  const int32_t* counts;
+  // log2 (fp64: natural logarithm) of the sum of a row's exponentials, +inf for rows that see
+  // nothing, where not null
+  void* lse;
 };
 
 constexpr int kTileRows = 128;  // most rows of a packed tile
@@ -50,23 +65,50 @@ constexpr unsigned kAtOnce = 1536;  // workgroups that start with the launch, ab
 
 // A workgroup's piece: the rows row0 .. row0 + rows - 1 of a sequence of `nrows` rows,
 // over keys [kbeg, kend).  Query i sees key t iff t < own, or t < own + 64 and bit
-// t - own of its mask; packed: iff t <= i + off.
+// t - own of its mask; packed and paged: iff t <= i + off.
 struct SeqPiece {
   int row0, rows;  // of the sequence's (query, head) rows
   int kbeg, kend;
-  int off;         // packed: Lk - Lq
-  int own;         // tree: the cached positions
-  int64_t b;       // tree: the row of the batch; packed: 0
+  int off;         // packed: Lk - Lq; paged: own
+  int own;         // tree, paged: the cached positions
+  int count;       // paged: the row's tokens; those behind see nothing
+  int64_t b;       // tree, paged: the row of the batch; packed: 0
   int64_t q0, k0;  // packed: the sequence's first rows in q and k
   int kvh, split;
 };
 
+// The cached positions and new tokens of a paged row, whatever its lengths say within what
+// its table covers.
+struct PagedRow {
+  int own, count;
+};
+__device__ __forceinline__ PagedRow paged_row(const SeqArgs& a, int64_t b, int len) {
+  PagedRow r;
+  r.own = min(max(len, 0), a.Tcap);
+  const int count = a.counts != nullptr ? __builtin_amdgcn_readfirstlane(a.counts[b]) : a.N;
+  r.count = min(max(count, 0), min(a.N, a.Tcap - r.own));
+  return r;
+}
+// Keys of each of its splits: as even as whole stages (of 128 keys at most) allow, so that
+// rows of every length are split as far as the launch has splits, and never fewer than
+// a.chunk.
+__device__ __forceinline__ int paged_chunk(const SeqArgs& a, const PagedRow& r) {
+  const int even = (r.own + r.count + a.nsplit - 1) / a.nsplit;
+  return max(a.chunk, (even + 127) & ~127);
+}
+// The keys that the row block with (query, head) row `row` sees; 0 where it has no token.
+__device__ __forceinline__ int paged_end(const SeqArgs& a, const PagedRow& r, int row) {
+  const int row0 = row / a.rows_per_wg * a.rows_per_wg;
+  if (row0 / a.G >= r.count) return 0;
+  return r.own + min(r.count, (min(row0 + a.rows_per_wg, a.N * a.G) - 1) / a.G + 1);
+}
+
 // The piece of this workgroup; false where there is nothing to do.  Nothing a table or
 // a length in device memory says takes an access outside q, k, v and y: tiles that do
 // not lie inside them are left out, lengths beyond the cache are taken as its end.
-template <bool TREE>
+template <SeqMode MODE>
 __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
-  if constexpr (TREE) {
+  if constexpr (MODE != kPacked) {
     // workgroup x runs on XCD x mod 8: the row blocks of a split, which read the same
     // keys, follow each other there
     const unsigned t = blockIdx.x >> 3;
@@ -78,13 +120,24 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
     p.b = u / a.Hkv;
     if (p.b >= a.B) return false;  // the grid is rounded up
     const int len = a.lens != nullptr ? __builtin_amdgcn_readfirstlane(a.lens[p.b]) : a.len;
-    p.own = min(max(len, 0), a.Tcap - a.N);
     p.row0 = rb * a.rows_per_wg;
     p.rows = min(a.rows_per_wg, a.N * a.G - p.row0);
-    p.kbeg = p.split * a.chunk;
-    p.kend = min(p.own + a.N, p.kbeg + a.chunk);
     p.off = 0;
     p.q0 = p.k0 = 0;
+    if constexpr (MODE == kPaged) {
+      const PagedRow r = paged_row(a, p.b, len);
+      p.own = p.off = r.own;
+      p.count = r.count;
+      const int chunk = paged_chunk(a, r);
+      const int end = paged_end(a, r, p.row0);
+      p.kbeg = p.split * chunk;  // below 2^31: fewer than a split more than the keys
+      p.kend = min(end, p.kbeg + chunk);
+      // the first split of unsplit rows that see nothing has their zeros to write
+      return p.kbeg < p.kend || a.nsplit == 1;
+    }
+    p.own = min(max(len, 0), a.Tcap - a.N);
+    p.kbeg = p.split * a.chunk;
+    p.kend = min(p.own + a.N, p.kbeg + a.chunk);
     return p.kbeg < p.kend;
   } else {
     // Position u of the XCD's workgroups: a tile's parts follow each other, they share its

@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define DG_ABI_VERSION 5
+#define DG_ABI_VERSION 6
 
 #if defined(__GNUC__)
 #define DG_API __attribute__((visibility("default")))
@@ -55,7 +55,8 @@ extern "C" {
  * in fp64, any other scale acts as its fp32 value.  ABI version 3 added
  * DG_F64 and made dg_swiglu's alpha / limit and dg_softcap's cap double;
  * version 4 added dg_packed_plan, dg_attention_packed, dg_attention_tree and
- * dg_token_logprobs, which take fp64 as well; version 5 dg_kernel_before. */
+ * dg_token_logprobs, which take fp64 as well; version 5 dg_kernel_before; version 6 the dg_paged_*
+ * entry points and dg_verify_drafts. */
 enum dg_dtype { DG_F32 = 0, DG_BF16 = 1, DG_F16 = 2, DG_F64 = 3 };
 
 enum dg_status {
@@ -660,6 +661,108 @@ DG_API int dg_attention_tree(int B, int N, int H, int Hkv, int Tcap, int D, int 
 DG_API int dg_token_logprobs(int64_t M, int64_t V, int dtype, const void* x, int64_t x_ld, const int64_t* ids,
                              void* logprob, void* entropy, int top, void* top_logprob, int64_t* top_ids,
                              void* stream);
+
+/*
+ * A cache in pages: rows of different lengths over pages of one pool, for one layer.  No
+ * counterpart in the reference, whose cache has one length for all rows.  k and v are
+ * (pages, page, Hkv, D) views (strides b: page, t: position in the page, h: head; unit stride
+ * over d); `page` is a power of two.  Position t of row b lies in page
+ * table[b * table_ld + t / page], t % page, for t < width * page (at most 2^30).  Row b holds
+ * lens[b] cached positions, and a call's tokens 0 .. counts[b] - 1 (NULL: all N) are the
+ * positions behind them.  Lengths are read on the device and taken as 0 .. width * page,
+ * counts as 0 .. N and as what the table still covers: tokens further on count as not there.
+ * A page id that the pool does not have is never followed: its positions read as zeros and
+ * are not written.
+ */
+typedef struct dg_paged_rows {
+  void* k;
+  void* v;
+  dg_stride3 k_st, v_st;
+  int64_t pages, page;
+  const int32_t* table;
+  int64_t table_ld, width;
+  const int32_t* lens;
+  const int32_t* counts;
+} dg_paged_rows;
+
+/*
+ * The rotation by position and the norm of every head of B x N tokens, and their keys and
+ * values into the pages.  With r the rotation of the D / 2 neighbouring pairs of a head by the
+ * (cos, sin) pairs freqs[position * freqs_ld ..] and, with DG_QKNORM, a division by
+ * sqrt(mean(r^2) + FLT_EPSILON):
+ *   q_out[b,n,h,:] = norm(r(q[b,n,h,:])),  the pages' k = norm(r(k[b,n,h,:])),  v = v[b,n,h,:]
+ * in fp32 (fp64 for fp64), rounded once.  Token n of row b has position positions[b] + n
+ * (NULL: lens[b] + n); outside [0, freqs_rows) its q and k become NaN.  Tokens that are not
+ * there have zeros in q_out and write nothing.  q, q_out (B,N,H,D), k, v (B,N,Hkv,D) views;
+ * freqs fp32 or of the data's type.  Every even D up to 1024; fp32 / bf16 / fp16 / fp64.
+ */
+DG_API int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
+                           const void* q, const dg_stride3* q_st, void* q_out, const dg_stride3* qo_st,
+                           const void* k, const dg_stride3* k_st, const void* v, const dg_stride3* v_st,
+                           const void* freqs, int64_t freqs_ld, int64_t freqs_rows, int freqs_dtype,
+                           const int32_t* positions, int flags, void* stream);
+
+/*
+ * Attention of each row's N newest tokens, which the pages already hold, over its positions:
+ * token n sees positions 0 .. lens[b] + n.  q, y (B,N,H,D) views; query head h reads key head
+ * h / (H / Hkv).  Tokens that are not there get zeros.  What a token does not see, NaN and
+ * infinities included, does not reach it.
+ * weights (fp32; NULL: not wanted): weights[b * w_b + h * w_h + t] += the probabilities that
+ * the row's tokens and the heads of key head h's group gave position t, summed without
+ * atomics, in an order of its own; what lies behind a row's positions is left as it is.
+ * Long rows are split over workgroups; partial results, and with weights the rows' softmax
+ * sums, meet in the caller's workspace (16-byte aligned, no initialisation, one each for calls
+ * that may overlap).  `longest`, at most width * page, is a hint of the positions that the
+ * longest row will hold, and decides how rows are split, no more than that.
+ * Types, head_dim and scale as dg_attention_packed.
+ */
+DG_API size_t dg_paged_attention_workspace_size(int B, int N, int H, int Hkv, int D, int dtype, int64_t longest,
+                                                int weights);
+
+DG_API int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
+                              const void* q, const dg_stride3* q_st, void* y, const dg_stride3* y_st, float scale,
+                              int64_t longest, float* weights, int64_t w_b, int64_t w_h,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rows cut to `keep` positions a key head: of the first lens[b] positions the `recent` last
+ * ones and of the others those of the largest weights (fp32, weights[b * w_b + h * w_h + t];
+ * equal ones: the earlier, NaN: above all), in their order, into positions 0 .. of the pages
+ * that `to` names ((B, to_width), row stride to_ld; keep <= to_width * page).  A row of at
+ * most `keep` positions moves as it is.  Written: new_lens[b] = min(lens[b], keep);
+ * kept[b][h][j], (B, Hkv, keep) contiguous, the position that j came from, -1 behind the last;
+ * new_weights, (B, Hkv, to_width * page) contiguous, the kept positions' weights and zeros
+ * behind them.  The pages that `to` names must not be any that the rows hold, nor named twice.
+ * 0 <= recent <= keep, keep >= 1; rows->counts is not looked at.  Every D up to 1024.
+ */
+DG_API int dg_paged_evict(int B, int Hkv, int D, int dtype, const dg_paged_rows* rows, const float* weights,
+                          int64_t w_b, int64_t w_h, int keep, int recent, const int32_t* to, int64_t to_ld,
+                          int64_t to_width, int32_t* new_lens, float* new_weights, int32_t* kept, void* stream);
+
+/*
+ * Drafted tokens against the target model's probabilities.  Row b has counts[b] (NULL: N;
+ * taken as 0 .. N) drafts tokens[b * N + i]; with p_i = softmax(target[b,i,:] * inv_temperature)
+ * and q_i = softmax(draft[b,i,:] * inv_temperature) (draft NULL: all of q_i is on the draft),
+ * draft i stands iff all before it do and uniforms[b * N + i] * q_i(x) < p_i(x).  With a drafts
+ * standing, the token after them is the first maximum over v of r(v) / noise[b * noise_ld + v]
+ * (noise > 0, Exp(1) variates: a draw from r), where r = max(p_a - q_a, 0), or p_a without the
+ * draft where draft is NULL, for a < counts[b] (p_a where nothing is left), and p_a for
+ * a = counts[b].  inv_temperature 0: temperature 0, draft i stands iff it is the first maximum
+ * of row i and the token after them is row a's; draft, uniforms and noise are not looked at.
+ *   accepted[b] = a;  out_tokens[b * (N + 1) + j]: the standing drafts, the token, -1 behind;
+ *   out_logprobs alike: log p_j of it (inv_temperature 0: of softmax(target)), 0 behind.
+ * target (B,N+1,V), draft (B,N,V) logits, unit stride over V; fp32 / bf16 / fp16 / fp64 all
+ * computed in fp32 with sums in fp64.  A draft outside [0, V) does not stand; nor does one of
+ * a row with NaN, +inf or -inf alone, and the token after it is then not specified but within
+ * [0, V).  0 <= N <= 64; inv_temperature 0 or from 2^-100 to 2^100.
+ */
+DG_API size_t dg_verify_drafts_workspace_size(int B, int N, int64_t V, int dtype);
+
+DG_API int dg_verify_drafts(int B, int N, int64_t V, int dtype, const void* target, int64_t t_b, int64_t t_n,
+                            const void* draft, int64_t d_b, int64_t d_n, const int64_t* tokens,
+                            const float* uniforms, const float* noise, int64_t noise_ld, const int32_t* counts,
+                            float inv_temperature, int64_t* accepted, int64_t* out_tokens, float* out_logprobs,
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
