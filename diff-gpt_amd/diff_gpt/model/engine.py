@@ -14,6 +14,9 @@ cache shared by its ``num_samples`` rows, one captured decode step for all
 rows -- with a schedule that may differ per prompt or per row.
 ``score_continuations`` gives the log probabilities of candidate continuations
 of a prompt, run as trees of tokens behind its cache.
+``generate_paged`` decodes prompts of different lengths together over a paged
+cache, with a smaller model that drafts tokens for it, and with a bound on the
+positions that a row keeps.
 """
 
 import gc
@@ -23,10 +26,13 @@ from typing import Generator, Sequence
 import numpy as np
 import torch
 
+from diff_gpt import _native
 from diff_gpt.model.gpt import GPT, BaseGPT, plain_gpt
 from diff_gpt.model.kv_cache import KVCache
+from diff_gpt.model.paged import PagedKVCache
 from diff_gpt.model.token_logprobs import token_logprobs
 from diff_gpt.model.tree import MAX_TREE
+from diff_gpt.sampler.drafts import verify_drafts
 from diff_gpt.sampler.sampler import Sampler
 from diff_gpt.sampler.temperature import draw_one
 
@@ -290,7 +296,86 @@ class Engine:
                 lp = lp[len(continuations[c]) :]
         return scores
 
+    @torch.inference_mode()
+    def generate_paged(
+        self,
+        prompts: list[list[int]],
+        max_tokens: int,
+        temperature: float = 1.0,
+        seed: int = 42,
+        draft: BaseGPT | None = None,
+        num_drafts: int = 4,
+        keep: int | None = None,
+        recent: int | None = None,
+        page_size: int = 64,
+    ) -> tuple[list[list[int]], list[list[float]]]:
+        """max_tokens tokens (fewer where 2 * block_size positions end) behind each of several
+        prompts of any lengths, decoded together over a PagedKVCache: returns (results,
+        logprobs), each prompt followed by its tokens, and the model's log probability of each
+        of these at the temperature (at 0, greedy decoding, at temperature 1).
+
+        draft: a model of the same vocabulary that proposes num_drafts tokens a row at a time,
+        which this one runs all at once and keeps as far as verify_drafts lets them stand: the
+        tokens are distributed as without it, in fewer passes.  keep: when a row comes to hold a
+        page more than so many positions, it is cut to them, the ``recent`` last ones (None: half)
+        and those that attention gave the largest weights; rejected drafts' weights count too."""
+        self._check_ragged(prompts)
+        for m in (self.model, draft):
+            if m is not None and not callable(getattr(m, "forward_paged", None)):
+                raise TypeError(f"generate_paged needs models with forward_paged, as GPT has: {type(m).__name__}")
+        model = self.model
+        assert all(0 <= t < model.vocab_size for p in prompts for t in p), "a token lies outside the vocabulary"
+        assert temperature >= 0, "the temperature must not be negative"
+        if draft is not None:
+            assert draft.vocab_size == model.vocab_size, "the draft model must have the model's vocabulary"
+            assert 1 <= num_drafts <= _native.MAX_DRAFTS, f"num_drafts must be 1 .. {_native.MAX_DRAFTS}, got {num_drafts}"
+        if keep is not None:
+            recent = keep // 2 if recent is None else recent
+            assert keep >= 1 and 0 <= recent <= keep, f"keep {keep} positions, {recent} of them the last ones"
+        device = torch.device(model.device_type)
+        rng = torch.Generator(device=device)
+        rng.manual_seed(seed)
+        left = [self._budget(len(p), max_tokens) for p in prompts]
+        if draft is not None:
+            left = [min(n, max(0, draft.block_size * 2 - len(p))) for n, p in zip(left, prompts)]
+        B, results, logprobs = len(prompts), [list(p) for p in prompts], [[] for _ in prompts]
+        if max(left) == 0:
+            return results, logprobs
+        ahead = num_drafts if draft is not None else 0
+        # every row's last token is pending: run with the drafts behind it
+        own = _PagedDecoder(model, prompts, left, ahead, page_size, keep, recent, device)
+        side = None if draft is None else _PagedDecoder(draft, prompts, left, ahead, page_size, None, None, device)
+        while max(left) > 0:
+            n = [min(ahead, max(0, k - 1)) for k in left]
+            N = max(n)
+            drafts = drafted = None
+            if N:
+                drafts, drafted = side.propose(results, n, N, temperature, rng)
+            logits = own.run([r[own.done[b] :] if left[b] else [] for b, r in enumerate(results)], drafts, n)
+            tokens = torch.zeros((B, N), dtype=torch.long, device=device) if drafts is None else drafts
+            u = e = None
+            if temperature > 0:
+                u = torch.rand((B, N), generator=rng, device=device)
+                e = torch.empty((B, logits.size(-1)), device=device).exponential_(1, generator=rng)
+            r = verify_drafts(logits, tokens, u, e, draft=drafted, counts=own.cache.ints(n), temperature=temperature)
+            new, lps, stand = r.tokens.tolist(), r.logprobs.tolist(), r.accepted.tolist()
+            for b in range(B):
+                if left[b]:
+                    results[b] += new[b][: stand[b] + 1]
+                    logprobs[b] += lps[b][: stand[b] + 1]
+                    left[b] -= stand[b] + 1
+            for d in (own, side):
+                if d is not None:
+                    d.settle(results)
+        return results, logprobs
+
     # -- shared machinery -------------------------------------------------------
+
+    @classmethod
+    def _check_ragged(cls, prompts) -> None:
+        assert isinstance(prompts, list) and len(prompts) > 0, "prompts must be a non-empty list of token lists"
+        for p in prompts:
+            cls._check_tokens(p)
 
     @staticmethod
     def _check_tokens(tokens) -> None:
@@ -504,6 +589,84 @@ class Engine:
                     self._kept = (key, cache, decode)
                 else:
                     decode.close()
+
+
+class _PagedDecoder:
+    """One model's side of generate_paged: its cache, and how many of each row's tokens the
+    cache holds (``done``; the last token is never among them)."""
+
+    __slots__ = ("model", "cache", "done", "keep", "recent", "device")
+
+    # prompts go through the layers so many tokens a row at a time
+    CHUNK = 256
+
+    def __init__(self, model: BaseGPT, prompts: list[list[int]], left: list[int], ahead: int, page_size: int,
+                 keep: int | None, recent: int | None, device: torch.device) -> None:
+        self.model, self.keep, self.recent, self.device = model, keep, recent, device
+        self.done = [0] * len(prompts)
+        chunk = self.CHUNK
+        most = [len(p) + n + ahead for p, n in zip(prompts, left)]
+        if keep is not None:  # what a row holds before it is cut: a page and a chunk, or a round's drafts, more
+            most = [min(m, keep + page_size + max(chunk, ahead + 1)) for m in most]
+        pages = sum(-(-m // page_size) for m in most)
+        if keep is not None:
+            pages += -(-keep // page_size)  # the pages that a row is cut into
+        w = next(model.parameters())
+        self.cache = PagedKVCache(len(prompts), model.n_head, model.n_embd // model.n_head, model.n_layer, pages, page_size,
+                                  max(most), w.dtype, device, weights=keep is not None)
+        ends = [len(p) - 1 if n else 0 for p, n in zip(prompts, left)]  # rows with nothing to come stay empty
+        while self.done != ends:
+            parts = [p[at : min(at + chunk, end)] for p, at, end in zip(prompts, self.done, ends)]
+            self._forward(parts)
+            self.done = [at + len(part) for at, part in zip(self.done, parts)]
+            self._cut()
+
+    def _forward(self, parts: list[list[int]], more: torch.Tensor | None = None, counts: list[int] | None = None) -> torch.Tensor:
+        """Logits of the rows' next tokens: parts[b], and behind them counts[b] of more's."""
+        N = max(len(p) for p in parts)
+        ids = self.cache.ints([p + [0] * (N - len(p)) for p in parts]).long()
+        if more is not None:
+            ids = torch.cat([ids, more], dim=1)
+        n = [len(p) + (0 if counts is None else counts[b]) for b, p in enumerate(parts)]
+        return self.model.forward_paged(ids, self.cache, n)
+
+    def run(self, pending: list[list[int]], drafts: torch.Tensor | None, n: list[int]) -> torch.Tensor:
+        """Logits (B, N + 1, V) behind each row's one pending token and its drafts; rows
+        that have ended have none."""
+        counts = [c if p else 0 for p, c in zip(pending, n)]
+        return self._forward(pending, drafts, counts)
+
+    def propose(self, results: list[list[int]], n: list[int], N: int, temperature: float,
+                rng: torch.Generator) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """n[b] drafts of each row behind its tokens, drawn one after the other: (B, N) ids,
+        and the (B, N, V) logits they were drawn from (None at temperature 0)."""
+        parts = [r[at:] if c else [] for r, at, c in zip(results, self.done, n)]
+        logits = self._forward(parts)
+        last = self.cache.ints([max(0, len(p) - 1) for p in parts]).long()
+        row = logits[torch.arange(len(parts), device=self.device), last]
+        ids, rows = [], []
+        for i in range(N):
+            if temperature == 0:
+                step = torch.argmax(row, dim=-1, keepdim=True)
+            else:
+                step = draw_one(torch.softmax(row.float() / temperature, dim=-1), rng)
+            ids.append(step)
+            rows.append(row)
+            if i + 1 < N:
+                row = self.model.forward_paged(step, self.cache, [int(c > i + 1) for c in n])[:, 0]
+        return torch.cat(ids, dim=1), None if temperature == 0 else torch.stack(rows, dim=1)
+
+    def settle(self, results: list[list[int]]) -> None:
+        """After a round: of what the cache holds, the tokens that became results stay, all but
+        the last, which is pending."""
+        now = [min(p, len(r) - 1) for p, r in zip(self.cache.next_pos, results)]
+        self.cache.truncate([a - (p - t) for a, p, t in zip(self.cache.lens, self.cache.next_pos, now)])
+        self.done = now
+        self._cut()
+
+    def _cut(self) -> None:
+        if self.keep is not None and max(self.cache.lens) >= self.keep + self.cache.page_size:
+            self.cache.evict(self.keep, self.recent)
 
 
 def _tries(continuations: list[list[int]]):

@@ -18,6 +18,7 @@ from diff_gpt import _native
 from diff_gpt.model.block import Block, plain_block
 from diff_gpt.model.kv_cache import KVCache
 from diff_gpt.model.packed import PackedRows
+from diff_gpt.model.paged import PagedKVCache, PagedRows
 from diff_gpt.model.rms_norm import rms_norm
 from diff_gpt.model.rope import precompute_freqs_cis
 from diff_gpt.model.token_logprobs import TokenLogprobs, token_logprobs
@@ -243,7 +244,7 @@ class GPT(BaseGPT):
         _argmax_out: torch.Tensor | None = None,
         _last_only: bool = False,
         _advance: bool = False,
-        _rows: PackedRows | TreeRows | None = None,
+        _rows: PackedRows | TreeRows | PagedRows | None = None,
     ) -> tuple[torch.Tensor, torch.Tensor | None]:
         """gpt.py:140-200.  _argmax_out (B, T) int64, when given, receives the
         first maximum of every logits row (greedy sampling without a separate
@@ -251,8 +252,8 @@ class GPT(BaseGPT):
         position only (a prefill whose caller reads no others; _argmax_out is
         then (B, 1)): every layer still attends and caches every position, but
         the last layer's work after its attention and the head run for that
-        position alone.  _rows: the rows are packed sequences or a tree's tokens,
-        which know their positions and attention themselves."""
+        position alone.  _rows: the rows are packed sequences, a tree's tokens
+        or chunks over a paged cache, which know their positions and attention themselves."""
         B, T = idx.shape
         assert not (_last_only and targets is not None), "_last_only returns the last position's logits alone"
         start = 0 if kv_cache is None else kv_cache.get_pos()
@@ -381,6 +382,27 @@ class GPT(BaseGPT):
         rows = TreeRows(parents, kv_cache, idx.device)
         logits, _ = self.forward(idx, kv_cache=kv_cache, _rows=rows)
         kv_cache.tree, kv_cache.tree_start = list(parents), rows.start
+        return logits
+
+    @torch.inference_mode()
+    def forward_paged(self, idx: torch.Tensor, cache: PagedKVCache, counts: Sequence[int] | None = None) -> torch.Tensor:
+        """Logits (B, N, V) of the next N tokens idx of every row of a paged cache, each row's at
+        the positions behind what it has cached.  counts: how many of the N tokens row b has,
+        0 .. N (None: all); the others may be any token, and their logits mean nothing.  The
+        cache advances by the counts; its truncate takes tokens back."""
+        B, N = idx.shape
+        rows = len(cache.lens)
+        assert B == rows, f"{B} rows, a cache of {rows}"
+        counts = [N] * B if counts is None else list(map(operator.index, counts))
+        assert len(counts) == B and all(0 <= n <= N for n in counts), f"counts must be {B} numbers from 0 to {N}"
+        end = max(p + n for p, n in zip(cache.next_pos, counts))
+        assert end <= self.freqs_cis.shape[0], (
+            f"position {end} is past 2 * block_size ({self.freqs_cis.shape[0]})"
+        )
+        cache.reserve(counts)
+        chunk = PagedRows(cache, counts)
+        logits, _ = self.forward(idx, _rows=chunk)
+        cache.advance(counts, chunk.counts)
         return logits
 
     @torch.inference_mode()

@@ -43,6 +43,7 @@ from diff_gpt.model.kv_cache import KVCache
 
 if TYPE_CHECKING:
     from diff_gpt.model.packed import PackedRows
+    from diff_gpt.model.paged import PagedRows
     from diff_gpt.model.tree import TreeRows
 
 # A prefill whose attention output y has at least this many bytes applies the
@@ -173,13 +174,13 @@ class MultiHeadAttention(nn.Module):
         return qkvg[..., 3 * self.n_head * self.head_dim :]
 
     def _attend(self, qkvg: torch.Tensor, freqs_cis: torch.Tensor, kv_cache: KVCache | None,
-                gated: bool = False, rows: PackedRows | TreeRows | None = None) -> torch.Tensor:
+                gated: bool = False, rows: PackedRows | TreeRows | PagedRows | None = None) -> torch.Tensor:
         """mha.py:44-83 on the projections qkvg (B, T, 3*inner + C), whose
         column slices are q, k, v and the gate logits: RoPE, QK-norm, the
         cache append and the attention; returns y (B, T, inner) before the
         gate, or with gated (a prefill: _gates_in_prefill) after it (mha.py:84).
         rows, when given, says which rows attend to which (packed sequences, a
-        tree over the cache) and takes the part between; ungated."""
+        tree over the cache, chunks over a paged one) and takes the part between; ungated."""
         B, T, _ = qkvg.size()
         H, D = self.n_head, self.head_dim
         ops = _native.ops()
