@@ -143,8 +143,14 @@ namespace {
 
 template <typename T, int D, int RT>
 int launch_paged(const SeqArgs& a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, kPaged>), grid, dim3(64 * SeqCfg<T, D, RT>::WAVES), 0, s, a);
-  return check_launch(RT == 1 ? "seq_mfma_paged_32" : RT == 2 ? "seq_mfma_paged_64" : "seq_mfma_paged_128");
+  const dim3 block(64 * SeqCfg<T, D, RT>::WAVES);
+  const int64_t es = (int64_t)sizeof(T), page = (int64_t)1 << a.page_log2, far = (int64_t)1 << 31;
+  if (page >= paged_granule(D, (int)es) && a.kb == a.vb && a.kt == a.vt && a.kb >= 0 && a.kb * es < far && page * a.kt * es < far) {
+    hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, kPaged>), grid, block, 0, s, a);
+    return check_launch(RT == 1 ? "seq_mfma_paged_32" : RT == 2 ? "seq_mfma_paged_64" : "seq_mfma_paged_128");
+  }
+  hipLaunchKernelGGL((seq_mfma_kernel<T, D, RT, kPagedAny>), grid, block, 0, s, a);
+  return check_launch(RT == 1 ? "seq_mfma_paged_any_32" : RT == 2 ? "seq_mfma_paged_any_64" : "seq_mfma_paged_any_128");
 }
 
 template <typename T, int RT>

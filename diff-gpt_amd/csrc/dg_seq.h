@@ -14,8 +14,9 @@ namespace dg {
 
 // packed: whole sequences one after the other; tree: up to 64 tokens a row over its cache,
 // each with a mask; paged: any number of tokens a row, each seeing what lies before it, over
-// a cache in pages
-enum SeqMode { kPacked, kTree, kPaged };
+// a cache in pages (kPagedAny: of any size and strides, where kPaged asks for pages of
+// paged_granule positions at least and the same strides, within 2^31 bytes, for keys and values)
+enum SeqMode { kPacked, kTree, kPaged, kPagedAny };
 
 struct SeqArgs {
   const void* q;
@@ -124,7 +125,7 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
     p.rows = min(a.rows_per_wg, a.N * a.G - p.row0);
     p.off = 0;
     p.q0 = p.k0 = 0;
-    if constexpr (MODE == kPaged) {
+    if constexpr (MODE >= kPaged) {
       const PagedRow r = paged_row(a, p.b, len);
       p.own = p.off = r.own;
       p.count = r.count;
@@ -200,6 +201,10 @@ __device__ __forceinline__ uint64_t tree_mask(const SeqArgs& a, int64_t b, int n
   if (a.masks == nullptr) return n >= 63 ? ~0ull : (2ull << n) - 1;
   return (uint64_t)a.masks[b * a.mask_b + n] & all;
 }
+
+// Positions that the matrix-core kernels copy from one page at a time: eight, or the rows that a
+// wave's 64 pieces of 16 bytes cover.
+constexpr int paged_granule(int D, int es) { return 1024 / (D * es) > 8 ? 1024 / (D * es) : 8; }
 
 // The head_dim that the matrix-core kernels and their workspaces round D (up to 256) up to.
 constexpr int seq_mfma_dim(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }

@@ -164,7 +164,7 @@ void seq_mfma_kernel(const SeqArgs a) {
   using M = SeqMma<T>;
   using vec8 = typename M::vec8;
   constexpr int ES = C::ES, KS = C::KS, MB = C::MB, BN = C::BN, PPR = C::PPR, NB = C::NB, TILE = C::TILE;
-  constexpr bool F32 = ES == 4, TREE = MODE == kTree, PAGED = MODE == kPaged;
+  constexpr bool F32 = ES == 4, TREE = MODE == kTree, PAGED = MODE >= kPaged;
   constexpr float kNone = kNegInf;
 
   __shared__ __attribute__((aligned(16))) T kv0[KS * 2 * TILE];
@@ -240,16 +240,52 @@ void seq_mfma_kernel(const SeqArgs a) {
     }
   };
   // Paged: lane j holds the page of key j of the stage to be copied next, loaded a stage ahead
-  // (-1: a key past the piece, or a page that the pool does not have).  Pages may end inside
-  // a copy, and the pool lies anywhere in 64 bits, so every lane has an address of its own;
-  // what is not there is read from kZeros16.
+  // and not looked at before (a comparison beside the load would wait for it, and with it for
+  // the stage's copies).
   int ids = -1;
   auto fetch_ids = [&](int k0) __attribute__((always_inline)) {
-    const int t = k0 + lane;
-    int id = -1;
-    if (t < pc.kend) id = a.table[pc.b * a.table_ld + (t >> a.page_log2)];
-    ids = (int64_t)id < a.pages ? id : -1;
+    ids = a.table[pc.b * a.table_ld + (min(k0 + lane, pc.kend - 1) >> a.page_log2)];
   };
+  // kPaged: rows of GR keys, which a page holds whole, have one resource, that of nothing for a
+  // page the pool lacks.  Rows past the piece's last key are copied too: hidden from all.
+  constexpr int GR = paged_granule(D, ES), NC1 = (C::NDMA + RT - 1) / RT;
+  uint32_t page_b = 0, key_b = 0, npages = 0;
+  const char *kbase = nullptr, *vbase = nullptr;
+  if constexpr (MODE == kPaged) {
+    page_b = (uint32_t)(a.kb * ES);
+    key_b = (uint32_t)(a.kt * ES);
+    npages = (uint32_t)a.pages;
+    kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (int64_t)pc.kvh * a.kh);
+    vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + (int64_t)pc.kvh * a.vh);
+#pragma unroll
+    for (int n = 0; n < NC1; ++n) {
+      const int r = (n * RT + rt) * C::RPD + lane / PPR;
+      const int piece = (lane % PPR) ^ seq_swz<PPR, ES>(r);
+      const int in_gr = RT == 1 ? r % GR : lane / PPR;
+      ko[n] = 16 * piece < a.D * ES ? in_gr * (int)key_b + 16 * piece : (int)0x80000000u;
+    }
+  }
+  auto copy_whole = [&](T* st, int k0) __attribute__((always_inline)) {
+    T* const ks = st + kg * 2 * TILE;
+    const int gr_b = (GR - 1) * (int)key_b + a.D * ES;
+    __amdgpu_buffer_rsrc_t rk, rv;
+#pragma unroll
+    for (int n = 0; n < NC1; ++n) {
+      const int i = n * RT + rt;
+      if (C::NDMA % RT != 0 && i >= C::NDMA) break;  // wave-uniform
+      if (RT > 1 || n * C::RPD % GR == 0) {
+        const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(ids, i * C::RPD);
+        const uint32_t slot = (uint32_t)(k0 + i * C::RPD) & ((1u << a.page_log2) - 1);
+        const uint64_t off = (uint64_t)min(id, npages - 1) * page_b + slot * key_b;
+        const int bytes = id < npages ? gr_b : 0;
+        rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kbase + off), 0, bytes, kBufferWord3);
+        rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vbase + off), 0, bytes, kBufferWord3);
+      }
+      lds_copy16_buf(rk, ko[n], 0, ks + i * C::RPD * D);
+      lds_copy16_buf(rv, ko[n], 0, ks + TILE + i * C::RPD * D);
+    }
+  };
+  // kPagedAny: every lane has an address, that of kZeros16 for what is not there.
   auto copy_pages = [&](T* st, int k0) __attribute__((always_inline)) {
     T* const ks = st + kg * 2 * TILE;
     const T* const kh = static_cast<const T*>(a.k) + (int64_t)pc.kvh * a.kh;
@@ -262,7 +298,7 @@ void seq_mfma_kernel(const SeqArgs a) {
       const int e = ((lane % PPR) ^ seq_swz<PPR, ES>(r)) * (16 / ES);
       const int id = __shfl(ids, r, 64);
       const int slot = (k0 + r) & ((1 << a.page_log2) - 1);
-      const bool in = id >= 0 && e < a.D;
+      const bool in = id >= 0 && id < a.pages && k0 + r < pc.kend && e < a.D;
       const void* const kz = in ? static_cast<const void*>(kh + id * a.kb + slot * a.kt + e) : &kZeros16;
       const void* const vz = in ? static_cast<const void*>(vh + id * a.vb + slot * a.vt + e) : &kZeros16;
       lds_copy16(kz, ks + i * C::RPD * D);
@@ -271,7 +307,8 @@ void seq_mfma_kernel(const SeqArgs a) {
   };
   auto copy_stage = [&](T* st, int k0) __attribute__((always_inline)) {
     if constexpr (PAGED) {
-      copy_pages(st, k0);
+      if constexpr (MODE == kPaged) copy_whole(st, k0);
+      else copy_pages(st, k0);
       fetch_ids(k0 + KS * BN);
       return;
     }
@@ -315,7 +352,9 @@ void seq_mfma_kernel(const SeqArgs a) {
   const int kstep = KS * BN;
   const int kfirst = pc.kbeg + kg * BN;  // this group's first stage
   const int nstage = (pc.kend - pc.kbeg + kstep - 1) / kstep;
-  if constexpr (PAGED) fetch_ids(kfirst);
+  if constexpr (PAGED) {
+    if (nstage > 0) fetch_ids(kfirst);  // pc.kend is 1 at least
+  }
   if (nstage > 0) copy_stage(kv0, kfirst);
 
   floatx16_t o[NB];

@@ -82,7 +82,7 @@ template <typename T, int NCH, int LPR, SeqMode MODE>
 __global__ __launch_bounds__(256) void seq_tile_kernel(const SeqArgs a) {
   using S = SeqAcc<T>;
   using A = typename S::type;
-  constexpr bool TREE = MODE == kTree, PAGED = MODE == kPaged;
+  constexpr bool TREE = MODE == kTree, PAGED = MODE >= kPaged;
   constexpr int ROWS = 256 / LPR, KT = 32, KPL = KT / LPR;
   constexpr int VW = LPR == 32 ? 2 : 4, NV = 64 / LPR / VW;  // of a chunk, a lane has dims VW (ln + LPR h) + e
   constexpr int PAD = 16 / (int)sizeof(A);  // rows 4 banks apart
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256) void seq_tile_kernel(const SeqArgs a) {
 template <SeqMode MODE>
 __device__ __forceinline__ void seq_join_row(const SeqArgs& a, int64_t b, int len, int i, int r, int& own, int& used,
                                              bool& none) {
-  if constexpr (MODE == kPaged) {
+  if constexpr (MODE >= kPaged) {
     const PagedRow p = paged_row(a, b, len);
     const int chunk = paged_chunk(a, p);
     own = p.own;
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void seq_join_kernel(const SeqArgs a, const in
       for (int w = 0; w < WPR - 1; ++w)
         if (lane + 64 * c < a.D) o[c] += part[w * kMaxHeadDim + lane + 64 * c];
   }
-  if constexpr (MODE == kPaged) {
+  if constexpr (MODE >= kPaged) {
     if (a.lse != nullptr && lane == 0)
       static_cast<A*>(a.lse)[row] = none ? (A)__builtin_huge_valf() : bad ? (A)__builtin_nanf("") : m + S::log(l);
   }
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256) void seq_join4_kernel(const SeqArgs a, const i
     for (int w = 0; w < WPR - 1; ++w) o += *reinterpret_cast<const f32x4_t*>(part + w * D + d4);
   }
   if (ls4 != 0) return;
-  if constexpr (MODE == kPaged) {
+  if constexpr (MODE >= kPaged) {
     constexpr float kLift = __is_same(T, f16_t) ? 7.f : 0.f;  // of the parts' sums (SeqMma)
     if (a.lse != nullptr && d4 == 0)
       static_cast<float*>(a.lse)[row] =
