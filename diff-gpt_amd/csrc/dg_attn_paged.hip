@@ -79,6 +79,29 @@ __global__ __launch_bounds__(256) void paged_weights_any_kernel(const SeqArgs a,
   }
 }
 
+// order[0 ..] = the rows of the batch by how many positions their tokens see, the most first:
+// where more workgroups than run at once take their turns, the launch then ends on short
+// ones.  Ranks by counting, at most kOrdered rows.  us as they come / so, with this launch:
+// 16 rows of 256 - 512 tokens behind 1000 - 7168, 16 heads on 4 of 128, 472 / 383.
+constexpr int kOrdered = 1024;
+
+__global__ __launch_bounds__(kOrdered) void paged_order_kernel(const SeqArgs a, int32_t* order) {
+  __shared__ int keys[kOrdered];
+  const int b = threadIdx.x;
+  int key = -1;
+  if (b < a.B) {
+    const int own = min(max(a.lens[b], 0), a.Tcap);
+    const int count = min(max(a.counts != nullptr ? a.counts[b] : a.N, 0), min(a.N, a.Tcap - own));
+    key = count > 0 ? own + count : 0;
+  }
+  keys[b] = key;
+  __syncthreads();
+  if (b >= a.B) return;
+  int rank = 0;
+  for (int j = 0; j < a.B; ++j) rank += keys[j] > key || (keys[j] == key && j < b);
+  order[rank] = b;
+}
+
 namespace {
 
 template <typename T>
@@ -123,22 +146,34 @@ int launch_join(const SeqArgs& a, bool mfma, bool many, dim3 grid, int64_t rows,
   return check_launch("seq_join_paged");
 }
 
-// Rows of a workgroup: few (token, head) rows as a tree's, many as a packed batch's.
+// Rows of a workgroup.  Few (token, head) rows as a tree's.  Many: 32 where all such workgroups
+// run at once, unless heads of 128 dims have many keys in all to read; 128 where there are so
+// many tiles that 64 would read the keys too often (a packed batch's rule, half as many
+// tiles again, since rows rarely have all of their tokens).  us with 32 / 64 / 128 rows and the
+// splits of each that are best, rows x tokens behind up to so many keys, heads on key heads:
+//   8 x 200, 4000, 8 / 8 of 64 36.3 / 43.5 / 44.0; 12 x 40, 2000, 8 / 2 of 64 16.8 / 22 / 30;
+//   1 x 300, 30000, 8 / 2 of 64 54 / 73 / 87; 48 x 300, 3000, 8 / 2 of 64 131 / 107 / 139;
+//   1 x 512, 7000, 16 / 4 of 128 78 / 64 / 70; 30 x 200, 600, 16 / 4 of 128 134 / 55 / 43;
+//   16 x 512, 7168, 16 / 4 of 128 499 / 293 / 276
 int mfma_rows(int64_t B, int64_t rows, int Hkv, int keys, int D, int dtype) {
   if (rows <= 128) return seq_mfma_tree_rows(B, (int)rows, Hkv, keys, D, dtype);
-  const int64_t counts[3] = {0, B * ((rows + 127) / 128), 128};
-  return seq_mfma_packed_rows(counts, Hkv, D);
+  const bool wide = seq_mfma_dim(D) * dtype_bytes(dtype) > 128;
+  const int64_t tiles = B * Hkv * ((rows + 127) / 128);
+  if (B * Hkv * ((rows + 31) / 32) <= (wide ? 256 : 512) && !(wide && tiles * keys > 300000)) return 32;
+  return tiles <= (D > 64 ? 576 : 960) ? 64 : 128;
 }
 
 // Row blocks, splits and workspace of a call.
 struct PagedShape {
-  int rows_per_wg, nrb, nsplit, chunk;
-  size_t o_bytes, lse_at, ws_bytes;
+  int rows_per_wg, nrb, nsplit, chunk, rb_groups, rb_each;
+  int64_t blocks;
+  bool ordered;
+  size_t o_bytes, lse_at, order_at, ws_bytes;
 };
 
 constexpr int kMaxSplits = 512;
 
-// Splits: enough workgroups to fill the CUs, and no fewer keys each than `least` stages, as
+// Splits: enough workgroups to fill the CUs, and no fewer than `least` keys each, as
 // for a tree (dg_attn_seq.hip has the times): a row's own length decides how many it uses.
 PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64_t longest, int weights, int rows_per_wg,
                        bool mfma) {
@@ -154,10 +189,17 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
                                            : Dm == 256 ? 512 : Dm == 128 ? 768 : 1024;
   const int64_t least = !mfma ? 256 : dtype == DG_F32 && Dm >= 64 ? 128 : 1024;
   const int64_t wg = std::max<int64_t>(1, B * Hkv * t.nrb);
-  int64_t want = (fill + wg - 1) / wg;
-  want = std::min<int64_t>({want, (longest + least - 1) / least, kMaxSplits});
+  // many rows' partial results cost more to write and join than a launch half full
+  int64_t want = R <= 128 ? (fill + wg - 1) / wg : fill / wg;
+  want = std::min<int64_t>({want, longest / least, kMaxSplits});
   t.nsplit = (int)std::max<int64_t>(want, 1);
   t.chunk = (int)least;
+  // every XCD has work: the row blocks of few (b, key head, split) go to several, in groups
+  const int64_t units = B * Hkv * t.nsplit;
+  t.rb_groups = (int)std::max<int64_t>(1, std::min<int64_t>(t.nrb, (64 + units - 1) / units));
+  t.rb_each = (t.nrb + t.rb_groups - 1) / t.rb_groups;
+  t.blocks = (units * t.rb_groups + 7) / 8 * 8 * t.rb_each;
+  t.ordered = B > 1 && B <= kOrdered && longest >= 1024 && t.blocks > fill;
   const size_t acc = dtype == DG_F64 ? 8 : 4;
   const size_t parts = (size_t)(B * Hkv * R) * t.nsplit;
   if (t.nsplit > 1) {
@@ -165,7 +207,9 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
     t.ws_bytes = t.o_bytes + ((parts * 2 * acc + 15) & ~(size_t)15);
   }
   t.lse_at = t.ws_bytes;
-  if (weights) t.ws_bytes += (size_t)(B * Hkv * R) * acc;
+  if (weights) t.ws_bytes += ((size_t)(B * Hkv * R) * acc + 15) & ~(size_t)15;
+  t.order_at = t.ws_bytes;
+  if (t.ordered) t.ws_bytes += (size_t)B * sizeof(int32_t);
   return t;
 }
 
@@ -236,6 +280,7 @@ extern "C" int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype
   const PagedShape t = paged_shape(B, N, H, Hkv, D, dtype, longest, weights != nullptr,
                                    mfma ? mfma_rows(B, R, Hkv, (int)longest, D, dtype) : tile_rows(R, D), mfma);
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
+  a.rb_groups = t.rb_groups; a.rb_each = t.rb_each;
   if (t.ws_bytes > 0) {
     DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,
                "paged_attention: a workspace of %zu bytes, %zu needed", workspace_bytes, t.ws_bytes);
@@ -243,11 +288,12 @@ extern "C" int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype
     a.ws_o = workspace;
     a.ws_ml = static_cast<char*>(workspace) + t.o_bytes;
     if (weights != nullptr) a.lse = static_cast<char*>(workspace) + t.lse_at;
+    if (t.ordered) a.order = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + t.order_at);
   }
   const int64_t nrows = (int64_t)B * Hkv * R;
   const bool many = t.nsplit >= 16 && nrows <= 4096;
   const int64_t groups = t.nsplit == 1 ? 0 : many ? nrows : (nrows + 3) / 4;
-  const int64_t blocks = ((int64_t)B * Hkv * t.nsplit + 7) / 8 * 8 * t.nrb;
+  const int64_t blocks = t.blocks;
   PagedWeights w{weights, w_b, w_h, 0};
   const int wkeys = mfma ? kWeightKeys : 64;
   w.blocks = (int)((cap + wkeys - 1) / wkeys);
@@ -257,6 +303,10 @@ extern "C" int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)blocks), jgrid((unsigned)groups), wgrid((unsigned)wblocks);
   int rc;
+  if (t.ordered) {
+    hipLaunchKernelGGL(paged_order_kernel, dim3(1), dim3(kOrdered), 0, s, a, const_cast<int32_t*>(a.order));
+    if ((rc = check_launch("paged_order_kernel")) != DG_OK) return rc;
+  }
   if (mfma) rc = launch_seq_mfma_paged(a, dtype, (unsigned)blocks, s);
   else if (dtype == DG_F64) rc = launch_tile<double>(a, grid, s);
   else if (dtype == DG_F32) rc = launch_tile<float>(a, grid, s);

@@ -54,6 +54,8 @@ struct SeqArgs {
   int64_t table_ld, pages;
   int page_log2;
   const int32_t* counts;
+  const int32_t* order;  // the rows of the batch, longest first (null: as they are)
+  int rb_groups, rb_each;  // row blocks of a (b, key head, split) that share an XCD, and how many such groups
   // log2 (fp64: natural logarithm) of the sum of a row's exponentials, +inf for rows that see
   // nothing, where not null
   void* lse;
@@ -109,7 +111,33 @@ __device__ __forceinline__ int paged_end(const SeqArgs& a, const PagedRow& r, in
 // not lie inside them are left out, lengths beyond the cache are taken as its end.
 template <SeqMode MODE>
 __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
-  if constexpr (MODE != kPacked) {
+  if constexpr (MODE >= kPaged) {
+    // workgroup x runs on XCD x mod 8: groups of row blocks, which read the same keys, follow
+    // each other there, the last rows first, which see the most
+    const unsigned t = blockIdx.x >> 3;
+    const unsigned each = t % (unsigned)a.rb_each;
+    unsigned u = t / (unsigned)a.rb_each * 8 + (blockIdx.x & 7u);
+    const int rb = a.nrb - 1 - (int)(u % (unsigned)a.rb_groups * (unsigned)a.rb_each + each);
+    u /= (unsigned)a.rb_groups;
+    p.split = (int)(u % (unsigned)a.nsplit);
+    u /= (unsigned)a.nsplit;
+    p.kvh = (int)(u % (unsigned)a.Hkv);
+    u /= (unsigned)a.Hkv;
+    if (rb < 0 || u >= (unsigned)a.B) return false;  // the grid is rounded up
+    p.b = a.order != nullptr ? __builtin_amdgcn_readfirstlane(a.order[u]) : (int)u;
+    p.row0 = rb * a.rows_per_wg;
+    p.rows = min(a.rows_per_wg, a.N * a.G - p.row0);
+    p.q0 = p.k0 = 0;
+    const PagedRow r = paged_row(a, p.b, __builtin_amdgcn_readfirstlane(a.lens[p.b]));
+    p.own = p.off = r.own;
+    p.count = r.count;
+    const int chunk = paged_chunk(a, r);
+    const int end = paged_end(a, r, p.row0);
+    p.kbeg = p.split * chunk;  // below 2^31: fewer than a split more than the keys
+    p.kend = min(end, p.kbeg + chunk);
+    // the first split of unsplit rows that see nothing has their zeros to write
+    return p.kbeg < p.kend || a.nsplit == 1;
+  } else if constexpr (MODE == kTree) {
     // workgroup x runs on XCD x mod 8: the row blocks of a split, which read the same
     // keys, follow each other there
     const unsigned t = blockIdx.x >> 3;
@@ -125,17 +153,6 @@ __device__ __forceinline__ bool seq_piece(const SeqArgs& a, SeqPiece& p) {
     p.rows = min(a.rows_per_wg, a.N * a.G - p.row0);
     p.off = 0;
     p.q0 = p.k0 = 0;
-    if constexpr (MODE >= kPaged) {
-      const PagedRow r = paged_row(a, p.b, len);
-      p.own = p.off = r.own;
-      p.count = r.count;
-      const int chunk = paged_chunk(a, r);
-      const int end = paged_end(a, r, p.row0);
-      p.kbeg = p.split * chunk;  // below 2^31: fewer than a split more than the keys
-      p.kend = min(end, p.kbeg + chunk);
-      // the first split of unsplit rows that see nothing has their zeros to write
-      return p.kbeg < p.kend || a.nsplit == 1;
-    }
     p.own = min(max(len, 0), a.Tcap - a.N);
     p.kbeg = p.split * a.chunk;
     p.kend = min(p.own + a.N, p.kbeg + a.chunk);

@@ -78,8 +78,8 @@ def test_workspace_covers_every_kernel():
     assert size(0, 1, 1, 1, 16, 0, 100, 0) == 0 and size(1, 1, 3, 2, 16, 0, 100, 0) == 0
     assert size(64, 1, 16, 4, 128, 1, 256, 0) == 0  # no kernel splits so few positions
     one = size(1, 1, 4, 4, 64, 1, 100000, 0)
-    assert one > 0 and size(1, 1, 4, 4, 64, 1, 100000, 1) == one + 4 * 4
-    assert size(1, 1, 4, 4, 64, 3, 100, 1) == 4 * 8
+    assert one > 0 and size(1, 1, 4, 4, 64, 1, 100000, 1) == one + 16
+    assert size(1, 1, 4, 4, 64, 3, 100, 1) == 32
     assert size(1, 1 << 30, 4, 2, 64, 3, 100, 1) == 0
 
 
