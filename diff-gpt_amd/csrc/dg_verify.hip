@@ -47,11 +47,15 @@ struct VerifyArgs {
   struct VerifyRace* races;  // (B)
 };
 
-// Maximum and sum of exp(scale (x - max)) over (a part of) a row, and its first maximum's id.
+// Sum of exp(scale (x - top)) over (a part of) a row and the logit of its draft.  top is some
+// logit of the row that no other is far above (kAhead), and at temperature 0 its maximum, at
+// the id `at`.
 struct VerifyStat {
   double sum;
   float top;
   int at;
+  float drafted;
+  int pad;
 };
 struct VerifyRace {
   unsigned long long best;  // the ratio's bits above the complement of its id
@@ -73,6 +77,7 @@ __device__ __forceinline__ float scaled_exp(const VerifyArgs& a, float d) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, a.scale_hi, d * a.scale_lo));
 }
 
+// s and what follows it in the row, o; the draft's logit stays s's.
 __device__ __forceinline__ void join_stat(const VerifyArgs& a, VerifyStat& s, const VerifyStat& o) {
   const bool up = o.top > s.top || (o.top == s.top && o.at < s.at);
   const float top = o.top > s.top ? o.top : s.top;
@@ -84,51 +89,94 @@ __device__ __forceinline__ void join_stat(const VerifyArgs& a, VerifyStat& s, co
   s.at = up ? o.at : s.at;
 }
 
-// This thread's part of a row's statistics: vectors of 16 bytes from an aligned address at or
-// before the row, every `step`-th from `first` on.  A vector holds some of the row, so what
-// it reads beside lies in the same 16 bytes.
-template <typename T>
-__device__ __forceinline__ VerifyStat row_stat(const VerifyArgs& a, const T* x, int first, int end, int step) {
+// 16 bytes of a row from any element on, in one load (rows of an odd vocabulary start
+// anywhere), so that which thread has a logit, and a row's bits, depend on its id alone.
+typedef u32x4_t __attribute__((aligned(2))) u32x4_any_t;
+
+template <typename T, int N>
+__device__ __forceinline__ void load_any(const T* p, float (&z)[N]) {
   constexpr int VE = 16 / (int)sizeof(T);
-  const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const T* const base = x - off;
-  VerifyStat s{0.0, kNegInf, 0x7fffffff};
-  float part = 0.f;
-  bool odd = false;  // a NaN
-  for (int j = first; j < end; j += step) {
-    const u32x4_t raw = *reinterpret_cast<const u32x4_t*>(base + (int64_t)j * VE);
-    T e[VE];
-    __builtin_memcpy(e, &raw, 16);
-    const int v0 = j * VE - off;
-    float z[VE], top = kNegInf;
+#pragma unroll
+  for (int c = 0; c < N / VE; ++c) {
+    const u32x4_t w = reinterpret_cast<const u32x4_any_t*>(p)[c];
+    if constexpr (sizeof(T) == 8) {
+      T e[VE];
+      __builtin_memcpy(e, &w, 16);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) z[c * VE + i] = logit<T>(e[i]);
+    } else {
+      RowRegs<T, VE> r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[i] = w[i];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) z[c * VE + i] = elem<T, VE>(r, i);
+    }
+  }
+}
+
+// log2 of how far an exponential may lie above that of `top` before it is raised (each raise
+// costs all lanes of a wave some 40 instructions, a comparison one)
+constexpr float kAhead = 16.f;
+
+// N further logits from id v0 on (-inf for what is not there) into a thread's statistics.  A
+// NaN makes the sum one.
+template <int N, bool GREEDY>
+__device__ __forceinline__ void add_logits(const VerifyArgs& a, const float (&z)[N], int v0, float& top, int& at, float& part) {
+  float m = z[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, z[i]);
+  if (GREEDY ? m > top : top == kNegInf ? m > top : (m - top) * a.scale_hi > kAhead) {
+    if constexpr (GREEDY) {
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i)
+        if (z[i] == m) at = v0 + i;
+    }
+    if (top != kNegInf) part *= scaled_exp(a, top - m);
+    top = m;
+  }
+  if (top == kNegInf) return;  // nothing yet
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum += scaled_exp(a, z[i] - top);
+  part += sum;
+}
+
+// Thread `tid` of `step`'s part of the statistics of a row's vectors first .. end - 1, and of
+// what follows the last whole one where end is past it.  Four vectors are in flight.
+template <typename T, bool GREEDY>
+__device__ __forceinline__ VerifyStat row_stat(const VerifyArgs& a, const T* x, int first, int end, int tid, int step) {
+  constexpr int VE = 16 / (int)sizeof(T), U = 4;
+  const int whole = min(end, a.V / VE);
+  float top = kNegInf, part = 0.f;
+  int at = 0x7fffffff, j = first + tid;
+  for (; j + (U - 1) * step < whole; j += U * step) {
+    float z[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_any<T, VE>(x + (int64_t)(j + u * step) * VE, z[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) add_logits<VE, GREEDY>(a, z[u], (j + u * step) * VE, top, at, part);
+  }
+  for (; j < whole; j += step) {
+    float z[VE];
+    load_any<T, VE>(x + (int64_t)j * VE, z);
+    add_logits<VE, GREEDY>(a, z, j * VE, top, at, part);
+  }
+  if (j < end) {  // the row's last, incomplete vector
+    float z[VE];
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      z[i] = v0 + i >= 0 && v0 + i < a.V ? logit<T>(e[i]) : kNegInf;
-      odd = odd || z[i] != z[i];
-      top = fmaxf(top, z[i]);
+      z[i] = kNegInf;
+      if (j * VE + i < a.V) z[i] = logit<T>(x[j * VE + i]);
     }
-    if (top > s.top) {
-#pragma unroll
-      for (int i = VE - 1; i >= 0; --i)
-        if (z[i] == top) s.at = v0 + i;
-      if (s.top != kNegInf) part *= scaled_exp(a, s.top - top);
-      s.top = top;
-    }
-    if (s.top == kNegInf) continue;  // nothing yet
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) sum += scaled_exp(a, z[i] - s.top);
-    part += sum;
+    add_logits<VE, GREEDY>(a, z, j * VE, top, at, part);
   }
-  s.sum = odd ? (double)__builtin_nanf("") : (double)part;
-  return s;
+  return VerifyStat{(double)part, top, at, 0.f, 0};
 }
 
 template <typename T>
-__device__ __forceinline__ int row_vectors(const VerifyArgs& a, const T* x) {
+__device__ __forceinline__ int row_vectors(const VerifyArgs& a) {
   constexpr int VE = 16 / (int)sizeof(T);
-  const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  return (int)(((int64_t)a.V + off + VE - 1) / VE);
+  return (a.V + VE - 1) / VE;
 }
 
 // The lanes' statistics joined, for all of them: one factor a lane, then sums in fp64.
@@ -162,9 +210,17 @@ __device__ __forceinline__ bool row_used(const VerifyArgs& a, int r, int count) 
   return r <= a.N ? r <= count : r - a.N - 1 < count;
 }
 
+// The logit of row r's draft, -inf for one outside the vocabulary.
 template <typename T>
-__device__ __forceinline__ double prob_at(const VerifyArgs& a, const T* x, const VerifyStat& s, int v) {
-  return exp((double)(logit<T>(x[v]) - s.top) * a.scale) / s.sum;
+__device__ __forceinline__ float drafted_logit(const VerifyArgs& a, int64_t b, int r, const T* x) {
+  const int i = r <= a.N ? r : r - a.N - 1;
+  if (i >= a.N) return 0.f;
+  const int64_t t = a.tokens[b * a.N + i];
+  return t >= 0 && t < a.V ? logit<T>(x[t]) : kNegInf;
+}
+
+__device__ __forceinline__ double drafted_prob(const VerifyArgs& a, const VerifyStat& s) {
+  return (double)scaled_exp(a, s.drafted - s.top) / s.sum;
 }
 
 // How many of row b's drafts stand: every wave finds it, lane i for draft i.
@@ -176,45 +232,59 @@ __device__ __forceinline__ int standing(const VerifyArgs& a, int64_t b, int coun
     if constexpr (GREEDY) {
       falls = x != stats[lane].at;
     } else {
-      bool ok = x >= 0 && x < a.V;
-      if (ok) {
-        const double p = prob_at(a, row_at<T>(a, b, lane), stats[lane], (int)x);
-        double q = 1.0;
-        if (a.draft != nullptr) q = prob_at(a, row_at<T>(a, b, a.N + 1 + lane), stats[a.N + 1 + lane], (int)x);
-        ok = (double)a.uniforms[b * a.N + lane] * q < p;
-      }
-      falls = !ok;
+      const double p = drafted_prob(a, stats[lane]);
+      const double q = a.draft != nullptr ? drafted_prob(a, stats[a.N + 1 + lane]) : 1.0;
+      falls = !((double)a.uniforms[b * a.N + lane] * q < p);  // so does a draft outside the vocabulary
     }
   }
   const uint64_t f = __builtin_amdgcn_ballot_w64(falls);
   return f == 0 ? count : __builtin_ctzll(f);
 }
 
-// A thread's best of row `at`'s race over ids v0 .. v1 - 1, every `step`-th: the ratio's bits
-// above the complement of its id, 0 where no ratio is positive.  In a row of drafts left over,
-// `any` says whether the difference p - q was positive anywhere.
+// Thread `tid` of `step`'s best of row `at`'s race over vectors first .. end - 1 (of the
+// vocabulary): the ratio's bits above the complement of its id, 0 where no ratio is positive.
+// rest: the row's draft did not stand.
 template <typename T>
 __device__ __forceinline__ unsigned long long race(const VerifyArgs& a, int64_t b, int at, bool rest, const VerifyStat& sp,
-                                                   const VerifyStat& sq, int v0, int v1, int step) {
+                                                   const VerifyStat& sq, int first, int end, int tid, int step) {
 #pragma clang fp contract(off)  // p - q of equal logits is 0, not what rounding one product leaves
+  constexpr int VE = 16 / (int)sizeof(T);
   const T* const xp = row_at<T>(a, b, at);
-  const T* const xq = a.draft != nullptr && rest ? row_at<T>(a, b, a.N + 1 + at) : nullptr;
+  const bool drawn = a.draft != nullptr && rest;  // uniform over the workgroup
+  const T* const xq = drawn ? row_at<T>(a, b, a.N + 1 + at) : xp;
   const int64_t drafted = rest && a.draft == nullptr ? a.tokens[b * a.N + at] : -1;
   const float* const e = a.noise + b * a.noise_ld;
-  const float ip = (float)(1.0 / sp.sum), iq = xq != nullptr ? (float)(1.0 / sq.sum) : 0.f;
+  const float ip = (float)(1.0 / sp.sum), iq = drawn ? (float)(1.0 / sq.sum) : 0.f;
   float best = 0.f;
   int id = 0;
-#pragma unroll 4
-  for (int v = v0; v < v1; v += step) {
-    float r = scaled_exp(a, logit<T>(xp[v]) - sp.top) * ip;
-    if (xq != nullptr) r -= scaled_exp(a, logit<T>(xq[v]) - sq.top) * iq;
+  auto run = [&](float zp, float zq, float n, int v) __attribute__((always_inline)) {
+    float r = scaled_exp(a, zp - sp.top) * ip;
+    if (drawn) r -= scaled_exp(a, zq - sq.top) * iq;
     if (v == drafted) r = 0.f;
-    r /= e[v];
+    r *= __builtin_amdgcn_rcpf(n);
     if (r > best) {  // ids rise: the first of equals stays
       best = r;
       id = v;
     }
+  };
+  const int whole = min(end, a.V / VE);
+  int j = first + tid;
+#pragma unroll 2
+  for (; j < whole; j += step) {
+    float zp[VE], zq[VE], n[VE < 4 ? 4 : VE];
+    load_any<T, VE>(xp + (int64_t)j * VE, zp);
+    if (drawn) load_any<T, VE>(xq + (int64_t)j * VE, zq);
+    if constexpr (VE >= 4) {
+      load_any<float, VE>(e + (int64_t)j * VE, n);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) n[i] = e[j * VE + i];
+    }
+#pragma unroll
+    for (int i = 0; i < VE; ++i) run(zp[i], drawn ? zq[i] : 0.f, n[i], j * VE + i);
   }
+  if (j < end)
+    for (int v = j * VE; v < a.V; ++v) run(logit<T>(xp[v]), logit<T>(xq[v]), e[v], v);
   return best > 0.f ? (unsigned long long)__float_as_uint(best) << 32 | (0xffffffffu - (unsigned)id) : 0ull;
 }
 
@@ -227,17 +297,15 @@ __device__ __forceinline__ unsigned long long wave_best(unsigned long long x) {
   return x;
 }
 
-// Row b's results, by one wave: lane j writes place j (and lane 0 the last of 64 drafts).
-template <typename T, bool GREEDY>
-__device__ __forceinline__ void write_row(const VerifyArgs& a, int64_t b, int stands, int token, const VerifyStat* stats,
-                                          int lane) {
+// Row b's results but for the token behind the standing drafts, by one wave.
+__device__ __forceinline__ void write_drafts(const VerifyArgs& a, int64_t b, int stands, const VerifyStat* stats, int lane) {
   for (int j = lane; j <= a.N; j += 64) {
+    if (j == stands) continue;
     int64_t t = -1;
     float lp = 0.f;
-    if (j <= stands) {
-      t = j < stands ? a.tokens[b * a.N + j] : token;
-      const VerifyStat s = stats[j];
-      lp = (float)((double)(logit<T>(row_at<T>(a, b, j)[t]) - s.top) * a.scale - log(s.sum));
+    if (j < stands) {
+      t = a.tokens[b * a.N + j];
+      lp = (float)((double)(stats[j].drafted - stats[j].top) * a.scale - log(stats[j].sum));
     }
     a.out_tokens[b * (a.N + 1) + j] = t;
     a.out_logprobs[b * (a.N + 1) + j] = lp;
@@ -245,8 +313,16 @@ __device__ __forceinline__ void write_row(const VerifyArgs& a, int64_t b, int st
   if (lane == 0) a.accepted[b] = stands;
 }
 
+// That token, by one thread.
+template <typename T>
+__device__ __forceinline__ void write_token(const VerifyArgs& a, int64_t b, int stands, int token, const VerifyStat& s) {
+  const float x = logit<T>(row_at<T>(a, b, stands)[token]);
+  a.out_tokens[b * (a.N + 1) + stands] = token;
+  a.out_logprobs[b * (a.N + 1) + stands] = (float)((double)(x - s.top) * a.scale - log(s.sum));
+}
+
 __device__ __forceinline__ int best_id(unsigned long long best) {
-  return best == 0 ? -1 : (int)(0xffffffffu - (unsigned)best);
+  return best == 0 ? 0 : (int)(0xffffffffu - (unsigned)best);
 }
 
 // One workgroup a row of the batch.
@@ -261,26 +337,30 @@ __global__ __launch_bounds__(512) void verify_alone_kernel(const VerifyArgs a) {
   for (int r = wv; r < a.rows; r += 8) {
     if (!row_used(a, r, count)) continue;
     const T* x = row_at<T>(a, b, r);
-    const VerifyStat s = wave_stat(a, row_stat<T>(a, x, lane, row_vectors<T>(a, x), 64));
+    float drafted = 0.f;
+    if (lane == 0) drafted = drafted_logit<T>(a, b, r, x);
+    VerifyStat s = wave_stat(a, row_stat<T, GREEDY>(a, x, 0, row_vectors<T>(a), lane, 64));
+    s.drafted = drafted;
     if (lane == 0) stats[r] = s;
   }
   __syncthreads();
   const int stands = standing<T, GREEDY>(a, b, count, stats, lane);
+  if (wv == 0) write_drafts(a, b, stands, stats, lane);
   if constexpr (GREEDY) {
-    if (wv == 0) write_row<T, GREEDY>(a, b, stands, min(stats[stands].at, a.V - 1), stats, lane);
+    if (tid == 0) write_token<T>(a, b, stands, min(stats[stands].at, a.V - 1), stats[stands]);
     return;
   }
   const bool rest = stands < count;
   const VerifyStat sp = stats[stands], sq = a.draft != nullptr && rest ? stats[a.N + 1 + stands] : sp;
   for (int again = 0; again < 2; ++again) {
-    const unsigned long long mine = wave_best(race<T>(a, b, stands, rest && again == 0, sp, sq, tid, a.V, 512));
+    const unsigned long long mine = wave_best(race<T>(a, b, stands, rest && again == 0, sp, sq, 0, row_vectors<T>(a), tid, 512));
     if (lane == 0) bests[wv] = mine;
     __syncthreads();
     unsigned long long best = bests[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) best = bests[i] > best ? bests[i] : best;
     if (best != 0 || !rest || again == 1) {  // the same in all threads
-      if (wv == 0) write_row<T, GREEDY>(a, b, stands, max(best_id(best), 0), stats, lane);
+      if (tid == 0) write_token<T>(a, b, stands, best_id(best), sp);
       return;
     }
     __syncthreads();  // nothing left of the difference: the target's row itself
@@ -288,7 +368,7 @@ __global__ __launch_bounds__(512) void verify_alone_kernel(const VerifyArgs a) {
 }
 
 // Statistics of one part of one row of logits a workgroup.
-template <typename T>
+template <typename T, bool GREEDY>
 __global__ __launch_bounds__(256) void verify_stat_kernel(const VerifyArgs a) {
   __shared__ VerifyStat waves[4];
   const int part = (int)(blockIdx.x % (unsigned)a.split);
@@ -298,15 +378,18 @@ __global__ __launch_bounds__(256) void verify_stat_kernel(const VerifyArgs a) {
   if (r == 0 && part == 0 && threadIdx.x == 0) a.races[b] = VerifyRace{0ull, 0u, 0u};
   if (!row_used(a, r, drafts_of(a, b))) return;  // whole workgroups
   const T* x = row_at<T>(a, b, r);
-  const int n = row_vectors<T>(a, x);
+  float drafted = 0.f;
+  if (part == 0 && threadIdx.x == 0) drafted = drafted_logit<T>(a, b, r, x);
+  const int n = row_vectors<T>(a);
   const int per = (n + a.split - 1) / a.split;
   const int first = min(part * per, n), end = min(first + per, n);
-  const VerifyStat s = wave_stat(a, row_stat<T>(a, x, first + (int)threadIdx.x, end, 256));
+  const VerifyStat s = wave_stat(a, row_stat<T, GREEDY>(a, x, first, end, (int)threadIdx.x, 256));
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x != 0) return;
   VerifyStat all = waves[0];
   for (int i = 1; i < 4; ++i) join_stat(a, all, waves[i]);
+  all.drafted = drafted;
   a.stats[(int64_t)br * a.split + part] = all;
 }
 
@@ -315,31 +398,41 @@ template <typename T, bool GREEDY>
 __global__ __launch_bounds__(512) void verify_race_kernel(const VerifyArgs a) {
   __shared__ VerifyStat stats[2 * kMostDrafts + 1];
   __shared__ unsigned long long bests[8];
-  __shared__ int last;
+  __shared__ bool again;
   const int64_t b = blockIdx.x / (unsigned)a.parts;
   const int part = (int)(blockIdx.x - (unsigned)b * (unsigned)a.parts);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int count = drafts_of(a, b);
-  for (int r = tid; r < a.rows; r += 512) {
-    if (!row_used(a, r, count)) continue;
-    const VerifyStat* s = a.stats + (b * a.rows + r) * a.split;
-    VerifyStat all = s[0];
-    for (int i = 1; i < a.split; ++i) join_stat(a, all, s[i]);
-    stats[r] = all;
+  if (a.split == 1) {
+    for (int r = tid; r < a.rows; r += 512)
+      if (row_used(a, r, count)) stats[r] = a.stats[b * a.rows + r];
+  } else {  // a wave a row, a lane a part
+    for (int r = wv; r < a.rows; r += 8) {
+      if (!row_used(a, r, count)) continue;
+      const VerifyStat* const s = a.stats + (b * a.rows + r) * a.split;
+      VerifyStat all{0.0, kNegInf, 0x7fffffff, 0.f, 0};
+      if (lane < a.split) all = s[lane];
+      const float drafted = __shfl(all.drafted, 0, 64);
+      all = wave_stat(a, all);
+      all.drafted = drafted;
+      if (lane == 0) stats[r] = all;
+    }
   }
   __syncthreads();
   const int stands = standing<T, GREEDY>(a, b, count, stats, lane);
+  if (part == 0 && wv == 0) write_drafts(a, b, stands, stats, lane);
   if constexpr (GREEDY) {
-    if (wv == 0) write_row<T, GREEDY>(a, b, stands, min(stats[stands].at, a.V - 1), stats, lane);
+    if (tid == 0) write_token<T>(a, b, stands, min(stats[stands].at, a.V - 1), stats[stands]);
     return;
   }
   const bool rest = stands < count;
   const VerifyStat sp = stats[stands], sq = a.draft != nullptr && rest ? stats[a.N + 1 + stands] : sp;
-  const int per = (a.V + a.parts - 1) / a.parts;
-  const int v0 = min(part * per, a.V), v1 = min(v0 + per, a.V);
+  const int nv = row_vectors<T>(a);
+  const int per = (nv + a.parts - 1) / a.parts;
+  const int v0 = min(part * per, nv), v1 = min(v0 + per, nv);
   auto block_best = [&](bool less, int from, int to) {
-    const unsigned long long mine = wave_best(race<T>(a, b, stands, less, sp, sq, from + tid, to, 512));
+    const unsigned long long mine = wave_best(race<T>(a, b, stands, less, sp, sq, from, to, tid, 512));
     if (lane == 0) bests[wv] = mine;
     __syncthreads();
     unsigned long long best = bests[0];
@@ -349,20 +442,23 @@ __global__ __launch_bounds__(512) void verify_race_kernel(const VerifyArgs a) {
     return best;
   };
   unsigned long long best = block_best(rest, v0, v1);
-  if (a.parts > 1) {
-    if (tid == 0) {
+  if (tid == 0) {
+    // the parts' best, by whom it does not matter; the last to have added its own goes on
+    bool end = true;
+    if (a.parts > 1) {
       __hip_atomic_fetch_max(&a.races[b].best, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      last = __hip_atomic_fetch_add(&a.races[b].done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)a.parts - 1;
-      if (last) bests[0] = __hip_atomic_load(&a.races[b].best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      end = __hip_atomic_fetch_add(&a.races[b].done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)a.parts - 1;
+      if (end) best = __hip_atomic_load(&a.races[b].best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    __syncthreads();
-    if (!last) return;
-    best = bests[0];
-    __syncthreads();
+    const bool none = best == 0 && rest;
+    again = end && none;
+    if (end && !none) write_token<T>(a, b, stands, best_id(best), sp);
   }
+  __syncthreads();
+  if (!again) return;
   // nothing left of the difference: the target's row itself
-  if (best == 0 && rest) best = block_best(false, 0, a.V);
-  if (wv == 0) write_row<T, GREEDY>(a, b, stands, max(best_id(best), 0), stats, lane);
+  best = block_best(false, 0, nv);
+  if (tid == 0) write_token<T>(a, b, stands, best_id(best), sp);
 }
 
 namespace {
@@ -399,7 +495,9 @@ int launch_verify(const VerifyArgs& a, const VerifyShape& t, bool greedy, hipStr
     else hipLaunchKernelGGL((verify_alone_kernel<T, false>), grid, block, 0, s, a);
     return check_launch("verify_alone_kernel");
   }
-  hipLaunchKernelGGL(verify_stat_kernel<T>, dim3((unsigned)((int64_t)a.B * a.rows * a.split)), dim3(256), 0, s, a);
+  const dim3 rows((unsigned)((int64_t)a.B * a.rows * a.split));
+  if (greedy) hipLaunchKernelGGL((verify_stat_kernel<T, true>), rows, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((verify_stat_kernel<T, false>), rows, dim3(256), 0, s, a);
   if (const int rc = check_launch("verify_stat_kernel")) return rc;
   const dim3 grid((unsigned)((int64_t)a.B * a.parts));
   if (greedy) hipLaunchKernelGGL((verify_race_kernel<T, true>), grid, block, 0, s, a);
