@@ -207,12 +207,18 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kSelectBins = 2048;
+constexpr int kSelectBins = 2048;
+constexpr uint32_t kZeroKey = 0x80000000u;
 
-__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const EvictArgs a) {
+// KPT weights a thread in registers, for rows of at most THREADS * KPT positions; 0: read anew
+// in every pass.
+template <int THREADS, int KPT>
+__global__ __launch_bounds__(THREADS) void paged_select_kernel(const EvictArgs a) {
+  constexpr int WAVES = THREADS / 64, BPT = kSelectBins / THREADS;
   __shared__ uint32_t hist[kSelectBins];
-  __shared__ uint32_t found[2];
-  __shared__ int above[kSelectWaves], equal[kSelectWaves];
+  __shared__ uint32_t totals[WAVES];
+  __shared__ uint32_t found[3];
+  __shared__ int above[WAVES], equal[WAVES];
   const int64_t bh = blockIdx.x;
   const int64_t b = bh / a.Hkv;
   const int h = (int)(bh - b * a.Hkv);
@@ -222,72 +228,102 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   int32_t* const kept = a.kept + bh * a.keep;
   if (h == 0 && tid == 0) a.new_lens[b] = min(len, a.keep);
   if (len <= a.keep) {
-    for (int j = tid; j < a.keep; j += kSelectThreads) kept[j] = j < len ? j : -1;
+    for (int j = tid; j < a.keep; j += THREADS) kept[j] = j < len ? j : -1;
     return;  // whole workgroups, before any barrier
   }
   const int old = len - a.recent;
   const int m = a.keep - a.recent;  // below old
-  for (int j = tid; j < a.recent; j += kSelectThreads) kept[m + j] = old + j;
-  if (m == 0) return;
   const float* const w = a.weights + b * a.wb + (int64_t)h * a.wh;
 
   // a wave's stretch of the positions, in whole 64
-  const int per = ((old + 63) / 64 + kSelectWaves - 1) / kSelectWaves * 64;
+  const int per = ((old + 63) / 64 + WAVES - 1) / WAVES * 64;
   const int t0 = min(wv * per, old), t1 = min(t0 + per, old);
+  uint32_t keys[KPT > 0 ? KPT : 1];
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const int t = t0 + 64 * i + lane;
+      keys[i] = t < t1 ? weight_key(w[t]) : 0u;
+    }
+  }
+  for (int j = tid; j < a.recent; j += THREADS) kept[m + j] = old + j;
+  if (m == 0) return;
+  // f(position, key, whether it is one) for each 64 of the stretch
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) {
+        const int t = t0 + 64 * i;
+        if (t < t1) f(t + lane, keys[i], t + lane < t1);
+      }
+    } else {
+      for (int t = t0; t < t1; t += 64) {
+        const bool in = t + lane < t1;
+        f(t + lane, in ? weight_key(w[t + lane]) : 0u, in);
+      }
+    }
+  };
 
-  uint32_t prefix = 0, need = (uint32_t)m;
+  // the m-th largest key's leading bits (mask): all that are left share them, and `need` of
+  // those are taken
+  uint32_t prefix = 0, mask = 0, need = (uint32_t)m;
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
-    __syncthreads();
-    for (int t = t0; t < t1; t += 64) {
-      bool in = t + lane < t1;
-      const uint32_t key = in ? weight_key(w[t + lane]) : 0u;
-      if (pass > 0) in = in && (pass == 1 ? key >> 21 : key >> 10) == (pass == 1 ? prefix >> 21 : prefix >> 10);
-      const uint32_t bin = (key >> shift) & (bins - 1);
-      // many positions may share one value (zero): the lanes of the first one's are counted at once
-      const uint64_t live = __builtin_amdgcn_ballot_w64(in);
-      if (live == 0) continue;
-      const int lead = __builtin_ctzll(live);
-      const uint32_t common = __shfl(bin, lead, 64);
-      const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == common);
-      if (lane == lead) atomicAdd(&hist[common], (uint32_t)__builtin_popcountll(same));
-      if (in && bin != common) atomicAdd(&hist[bin], 1u);
-    }
-    __syncthreads();
-    if (wv == 0) {
-      // the bin that holds the need-th largest: lane l has bins 32 l .. from the top down
-      uint32_t mine = 0;
-      for (int i = 0; i < kSelectBins / 64; ++i) mine += hist[kSelectBins - 1 - (32 * lane + i)];
-      uint32_t upto = mine;
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t x = __shfl_up(upto, off, 64);
-        if (lane >= off) upto += x;
-      }
-      if (upto >= need && upto - mine < need) {
-        uint32_t c = upto - mine;
-        int i = kSelectBins - 1 - 32 * lane;
-        while (c + hist[i] < need) c += hist[i--];
-        found[0] = (uint32_t)i;
-        found[1] = c;
+    for (int i = 0; i < BPT; ++i) hist[tid + THREADS * i] = 0;
+    __syncthreads();
+    each([&](int, uint32_t key, bool in) __attribute__((always_inline)) {
+      in = in && (key & mask) == prefix;
+      const uint32_t bin = (key >> shift) & (bins - 1);
+      // many positions may share one value, zero above all: those are counted at once
+      const uint64_t zeros = __builtin_amdgcn_ballot_w64(in && key == kZeroKey);
+      if (zeros != 0 && lane == 0) atomicAdd(&hist[(kZeroKey >> shift) & (bins - 1)], (uint32_t)__builtin_popcountll(zeros));
+      if (in && key != kZeroKey) atomicAdd(&hist[bin], 1u);
+    });
+    __syncthreads();
+    // the bin that holds the need-th largest: thread i has BPT bins from the top down
+    uint32_t n[BPT], mine = 0;
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) {
+      n[i] = hist[kSelectBins - 1 - (BPT * tid + i)];
+      mine += n[i];
+    }
+    uint32_t upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t x = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += x;
+    }
+    if (lane == 63) totals[wv] = upto;
+    __syncthreads();
+    for (int i = 0; i < wv; ++i) upto += totals[i];
+    if (upto >= need && upto - mine < need) {  // one thread
+      uint32_t c = upto - mine;
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) {
+        if (c < need && c + n[i] >= need) {
+          found[0] = (uint32_t)(kSelectBins - 1 - (BPT * tid + i));
+          found[1] = c;
+          found[2] = n[i];
+        }
+        c += n[i];
       }
     }
     __syncthreads();
     prefix |= found[0] << shift;
+    mask |= (bins - 1) << shift;
     need -= found[1];
-    __syncthreads();  // found is read before the next pass writes it
+    if (found[2] == need) break;  // all of the bin are taken
+    // the next pass writes found behind a barrier that all reach after reading it here
   }
 
   // positions above the m-th largest weight, and the first `need` that equal it
   int na = 0, ne = 0;
-  for (int t = t0; t < t1; t += 64) {
-    const bool in = t + lane < t1;
-    const uint32_t key = in ? weight_key(w[t + lane]) : 0u;
-    na += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && key > prefix));
-    ne += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && key == prefix));
-  }
+  each([&](int, uint32_t key, bool in) __attribute__((always_inline)) {
+    na += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && (key & mask) > prefix));
+    ne += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && (key & mask) == prefix));
+  });
   if (lane == 0) {
     above[wv] = na;
     equal[wv] = ne;
@@ -300,16 +336,15 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   }
   at += min(eq, (int)need);
   const uint64_t below = (1ull << lane) - 1;
-  for (int t = t0; t < t1; t += 64) {
-    const bool in = t + lane < t1;
-    const uint32_t key = in ? weight_key(w[t + lane]) : 0u;
-    const uint64_t es = __builtin_amdgcn_ballot_w64(in && key == prefix);
-    const bool take = in && (key > prefix || (key == prefix && eq + __builtin_popcountll(es & below) < (int)need));
+  each([&](int t, uint32_t key, bool in) __attribute__((always_inline)) {
+    const uint64_t es = __builtin_amdgcn_ballot_w64(in && (key & mask) == prefix);
+    const bool take = in && ((key & mask) > prefix ||
+                             ((key & mask) == prefix && eq + __builtin_popcountll(es & below) < (int)need));
     const uint64_t ts = __builtin_amdgcn_ballot_w64(take);
-    if (take) kept[at + __builtin_popcountll(ts & below)] = t + lane;
+    if (take) kept[at + __builtin_popcountll(ts & below)] = t;
     at += __builtin_popcountll(ts);
     eq += __builtin_popcountll(es);
-  }
+  });
 }
 
 // One piece of U of one kept position of a key head a thread; the first piece's thread has
@@ -466,10 +501,14 @@ extern "C" int dg_paged_evict(int B, int Hkv, int D, int dtype, const dg_paged_r
   a.pieces = (int)(D * es / unit);
   a.items = (int64_t)B * Hkv * a.to_cap * a.pieces;
   const int64_t blocks = (a.items + 255) / 256;
-  DG_REQUIRE(blocks <= kMostWorkgroups256 && (int64_t)B * Hkv <= 0xffffffffll / kSelectThreads, DG_EINVAL,
+  DG_REQUIRE(blocks <= kMostWorkgroups256 && (int64_t)B * Hkv <= 0xffffffffll / 1024, DG_EINVAL,
              "paged_evict: more than 2^32 - 1 threads");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)(B * Hkv)), dim3(kSelectThreads), 0, s, a);
+  const dim3 heads((unsigned)(B * Hkv));
+  if (a.cap <= 2048) hipLaunchKernelGGL((paged_select_kernel<256, 8>), heads, dim3(256), 0, s, a);
+  else if (a.cap <= 16384) hipLaunchKernelGGL((paged_select_kernel<1024, 16>), heads, dim3(1024), 0, s, a);
+  else if (a.cap <= 65536) hipLaunchKernelGGL((paged_select_kernel<1024, 64>), heads, dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((paged_select_kernel<1024, 0>), heads, dim3(1024), 0, s, a);
   if (const int rc = check_launch("paged_select_kernel")) return rc;
   const dim3 grid((unsigned)blocks);
   if (unit == 16) hipLaunchKernelGGL(paged_move_kernel<u32x4_t>, grid, dim3(256), 0, s, a);
