@@ -56,6 +56,10 @@ struct SeqArgs {
   const int32_t* counts;
   const int32_t* order;  // the rows of the batch, longest first (null: as they are)
   int rb_groups, rb_each;  // row blocks of a (b, key head, split) that share an XCD, and how many such groups
+  // the scores of R rows, unscaled, -inf for hidden ones: (B, Hkv, R, scores_ld), where not null
+  // (workgroups of 32 rows on the matrix cores)
+  float* scores;
+  int64_t scores_ld;
   // log2 (fp64: natural logarithm) of the sum of a row's exponentials, +inf for rows that see
   // nothing, where not null
   void* lse;

@@ -519,6 +519,17 @@ void seq_mfma_kernel(const SeqArgs a) {
         }
       }
     }
+    if constexpr (PAGED && RT == 1) {
+      if (a.scores != nullptr && pc.row0 + r32 < rend) {
+        float* const so = a.scores + ((pc.b * a.Hkv + pc.kvh) * (int64_t)(a.N * a.G) + row) * a.scores_ld + k0 + 4 * hh;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4_t*>(so + 32 * mb + 8 * g) =
+                f32x4_t{s[mb][4 * g], s[mb][4 * g + 1], s[mb][4 * g + 2], s[mb][4 * g + 3]};
+      }
+    }
     float mt = s[0][0];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)

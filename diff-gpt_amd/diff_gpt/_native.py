@@ -279,7 +279,7 @@ _SIGNATURES = {
         + [ctypes.c_void_p, ctypes.c_void_p] * 4  # q, q_out, k, v, each with its dg_stride3
         + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p],
     ),
-    "dg_paged_attention_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 6 + [ctypes.c_int64, ctypes.c_int]),
+    "dg_paged_attention_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 6 + [ctypes.c_int64] * 2 + [ctypes.c_int]),
     "dg_paged_attention": (
         ctypes.c_int,
         [ctypes.c_int] * 6 + [ctypes.c_void_p]  # the rows
@@ -1099,7 +1099,7 @@ def paged_attention_(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         raise ValueError(f"{what}: the last (head_dim) dimension must be contiguous")
     code = _DTYPE_CODE[q.dtype]
     L = lib()
-    ws_bytes = L.dg_paged_attention_workspace_size(B, N, H, Hkv, D, code, longest, w is not None)
+    ws_bytes = L.dg_paged_attention_workspace_size(B, N, H, Hkv, D, code, longest, cap, w is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     st = _Stride3x2(qb, qt, qh, yb, yt, yh)
     s = ctypes.addressof(st)

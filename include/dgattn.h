@@ -711,13 +711,13 @@ DG_API int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, const
  * the row's tokens and the heads of key head h's group gave position t, summed without
  * atomics, in an order of its own; what lies behind a row's positions is left as it is.
  * Long rows are split over workgroups; partial results, and with weights the rows' softmax
- * sums, meet in the caller's workspace (16-byte aligned, no initialisation, one each for calls
- * that may overlap).  `longest`, at most width * page, is a hint of the positions that the
+ * sums and few rows' scores, meet in the caller's workspace (16-byte aligned, no
+ * initialisation, one each for calls that may overlap; `positions` is width * page).  `longest`, at most width * page, is a hint of the positions that the
  * longest row will hold, and decides how rows are split, no more than that.
  * Types, head_dim and scale as dg_attention_packed.
  */
 DG_API size_t dg_paged_attention_workspace_size(int B, int N, int H, int Hkv, int D, int dtype, int64_t longest,
-                                                int weights);
+                                                int64_t positions, int weights);
 
 DG_API int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
                               const void* q, const dg_stride3* q_st, void* y, const dg_stride3* y_st, float scale,

@@ -65,7 +65,7 @@ def _attend(B=1, N=1, H=2, Hkv=1, D=16, dtype=0, rows=None, q=FAKE, scale=1.0, l
     (dict(N=1 << 30, H=2), EINVAL, b"2^30"), (dict(q=NUL), EINVAL, b"NULL"), (dict(rows=_rows(v=0)), EINVAL, b"NULL"),
     (dict(longest=0), EINVAL, b"longest"), (dict(longest=49), EINVAL, b"longest"), (dict(rows=_rows(page=3)), EINVAL, b"power"),
     (dict(weights=FAKE), EWORKSPACE, b"workspace"), (dict(weights=FAKE, ws=FAKE, ws_bytes=7), EWORKSPACE, b"workspace"),
-    (dict(weights=FAKE, ws=ctypes.c_void_p(0x1004), ws_bytes=64), EINVAL, b"aligned"),
+    (dict(weights=FAKE, ws=ctypes.c_void_p(0x1004), ws_bytes=1 << 20), EINVAL, b"aligned"),
     (dict(rows=_rows(page=1 << 20, width=1 << 10), longest=1 << 30), EWORKSPACE, b"workspace"),
     (dict(B=1 << 24, Hkv=1), EINVAL, b"workgroups"),
 ])
@@ -75,12 +75,13 @@ def test_attention_refusals(kw, code, word):
 
 def test_workspace_covers_every_kernel():
     size = _native.lib().dg_paged_attention_workspace_size
-    assert size(0, 1, 1, 1, 16, 0, 100, 0) == 0 and size(1, 1, 3, 2, 16, 0, 100, 0) == 0
-    assert size(64, 1, 16, 4, 128, 1, 256, 0) == 0  # no kernel splits so few positions
-    one = size(1, 1, 4, 4, 64, 1, 100000, 0)
-    assert one > 0 and size(1, 1, 4, 4, 64, 1, 100000, 1) == one + 16
-    assert size(1, 1, 4, 4, 64, 3, 100, 1) == 32
-    assert size(1, 1 << 30, 4, 2, 64, 3, 100, 1) == 0
+    assert size(0, 1, 1, 1, 16, 0, 100, 100, 0) == 0 and size(1, 1, 3, 2, 16, 0, 100, 100, 0) == 0
+    assert size(64, 1, 16, 4, 128, 1, 256, 256, 0) == 0  # no kernel splits so few positions
+    one = size(1, 1, 4, 4, 64, 1, 100000, 100000, 0)
+    assert one > 0 and size(1, 1, 4, 4, 64, 1, 100000, 100000, 1) == one + 16 + 4 * 4 * 100096  # sums and scores
+    assert size(1, 16, 4, 4, 64, 1, 100, 100, 1) == 4 * 4 * 16  # the sums of more than 8 rows
+    assert size(1, 1, 4, 4, 300, 3, 100, 100, 1) == 32
+    assert size(1, 1 << 30, 4, 2, 64, 3, 100, 100, 1) == 0 and size(1, 1, 1, 1, 64, 0, 100, 0, 1) == 0
 
 
 def _evict(B=1, Hkv=1, D=16, dtype=0, rows=None, weights=FAKE, keep=8, recent=2, to_width=1, to=FAKE):
