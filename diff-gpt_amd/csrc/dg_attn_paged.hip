@@ -199,6 +199,8 @@ int mfma_rows(int64_t B, int64_t rows, int Hkv, int keys, int D, int dtype) {
   return tiles <= (D > 64 ? 576 : 960) ? 64 : 128;
 }
 
+constexpr int kMaxSplits = 512;
+
 // Row blocks, splits and workspace of a call.
 struct PagedShape {
   int rows_per_wg, nrb, nsplit, chunk, rb_groups, rb_each;
@@ -208,10 +210,40 @@ struct PagedShape {
   size_t o_bytes, lse_at, scores_at, order_at, ws_bytes;
 };
 
-constexpr int kMaxSplits = 512;
+// Nanoseconds that a workgroup takes for 128 keys, about (each alone on its CU, or as many as
+// fit).
+int64_t stage_ns(int D, int dtype, int rows_per_wg) {
+  if (dtype == DG_F32) {
+    if (D == 128) return rows_per_wg == 128 ? 17000 : 8800;
+    return (D == 64 ? 2900 : D == 32 ? 2200 : 1100) * (rows_per_wg / 32);
+  }
+  return (D <= 32 ? 450 : D == 64 ? 700 : D == 128 ? 1000 : 2000) * (rows_per_wg / 32);
+}
 
-// Splits: enough workgroups to fill the CUs, and no fewer than `least` keys each, as
-// for a tree (dg_attn_seq.hip has the times): a row's own length decides how many it uses.
+// The number of splits of a row of `longest` keys that ends first: so many rounds of `fill`
+// workgroups at once of its share of the keys each, and from two splits on the join, a launch
+// of its own (8 us beside what the partial results take to write and read).  us measured, keys,
+// heads on key heads, rows a workgroup, by splits 1 / 2 / 4 / 8:
+//   1 x 512 tokens, 7000, 16 / 4 of 128, 64      123 / 78 / 64 / 73
+//   4 x 100, 8000, 8 / 8 of 128, 32             53.7 / 37 / 45 / 54
+//   8 x 200, 4000, 8 / 8 of 64, 32              36.3 / 43 / 51 / 51
+//   6 x 237, 5580, 2 / 2 of 16, 32              21.7 / 18 / 16 / 19
+//   5 x 25, 13386, fp32, 24 / 6 of 80, 64       909 / 464 / 246 / 198
+int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t fill, int D, int dtype, int rows_per_wg) {
+  const int64_t whole = longest * stage_ns(D, dtype, rows_per_wg) / 128;
+  int best = 1;
+  int64_t least = (wg + fill - 1) / fill * whole;
+  const int64_t most = std::min<int64_t>(longest / 256, kMaxSplits);
+  for (int k = 2; k <= most && wg * k <= 4 * fill; ++k) {
+    const int64_t cost = (wg * k + fill - 1) / fill * whole / k + 8000 + rows * k * D * 8 / 3000;
+    if (cost < least) {
+      least = cost;
+      best = k;
+    }
+  }
+  return best;
+}
+
 PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64_t longest, int64_t cap, int weights,
                        int rows_per_wg, bool mfma) {
   PagedShape t{};
@@ -224,13 +256,10 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
                        : rows_per_wg <= 32 ? (row_bytes >= 256 ? 256 : 512)
                        : rows_per_wg == 64 ? (row_bytes >= 512 ? 256 : 512)
                                            : Dm == 256 ? 512 : Dm == 128 ? 768 : 1024;
-  const int64_t least = !mfma ? 256 : dtype == DG_F32 && Dm >= 64 ? 128 : 1024;
   const int64_t wg = std::max<int64_t>(1, B * Hkv * t.nrb);
-  // many rows' partial results cost more to write and join than a launch half full
-  int64_t want = R <= 128 ? (fill + wg - 1) / wg : fill / wg;
-  want = std::min<int64_t>({want, longest / least, kMaxSplits});
-  t.nsplit = (int)std::max<int64_t>(want, 1);
-  t.chunk = (int)least;
+  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, fill, Dm, dtype, rows_per_wg)
+                  : (int)std::max<int64_t>(1, std::min<int64_t>({(fill + wg - 1) / wg, longest / 256, kMaxSplits}));
+  t.chunk = 256;
   // every XCD has work: the row blocks of few (b, key head, split) go to several, in groups
   const int64_t units = B * Hkv * t.nsplit;
   t.rb_groups = (int)std::max<int64_t>(1, std::min<int64_t>(t.nrb, (64 + units - 1) / units));
