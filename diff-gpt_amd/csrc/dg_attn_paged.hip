@@ -287,8 +287,6 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
 
 int tile_rows(int64_t rows, int D) { return rows <= 8 ? 8 : D <= 256 ? 32 : 16; }
 
-bool known_dtype(int dtype) { return dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64; }
-
 }  // namespace
 
 int check_paged_rows(const char* what, const dg_paged_rows* r, bool need_v, int* log2) {
@@ -307,54 +305,78 @@ int check_paged_rows(const char* what, const dg_paged_rows* r, bool need_v, int*
 
 using namespace dg;
 
-extern "C" size_t dg_paged_attention_workspace_size(int B, int N, int H, int Hkv, int D, int dtype, int64_t longest,
-                                                    int64_t positions, int weights) {
-  if (B <= 0 || N <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || !known_dtype(dtype)) return 0;
-  const int64_t R = (int64_t)N * (H / Hkv);
-  if (R > kMostPositions) return 0;
-  if (positions < 1 || positions > kMostPositions) return 0;
-  const int64_t keys = std::min<int64_t>(std::max<int64_t>(longest, 1), positions);
-  size_t most = paged_shape(B, N, H, Hkv, D, dtype, keys, positions, weights, tile_rows(R, D), false).ws_bytes;
-  if (D <= 256)
-    most = std::max(most, paged_shape(B, N, H, Hkv, D, dtype, keys, positions, weights,
-                                      mfma_rows(B, R, Hkv, (int)keys, D, dtype), true).ws_bytes);
-  return most;
-}
+namespace dg {
+namespace {
 
-extern "C" int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
-                                  const void* q, const dg_stride3* q_st, void* y, const dg_stride3* y_st, float scale,
-                                  int64_t longest, float* weights, int64_t w_b, int64_t w_h, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
-  DG_REQUIRE(B >= 0 && N >= 0 && H >= 0, DG_EINVAL, "paged_attention: negative size");
-  DG_REQUIRE(known_dtype(dtype), DG_EUNSUPPORTED, "paged_attention: dtype %d unsupported", dtype);
-  DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_attention: head_dim %d outside [1, %d]", D, kMaxHeadDim);
-  DG_REQUIRE(Hkv >= 1 && H % Hkv == 0, DG_EINVAL, "paged_attention: %d query heads on %d key heads", H, Hkv);
-  DG_REQUIRE((int64_t)N * (H / Hkv) <= kMostPositions, DG_EINVAL, "paged_attention: a row of more than 2^30 (token, head) rows");
+// A call looked over: its kernel's arguments and how it runs.
+struct PagedCall {
+  SeqArgs a;
+  PagedShape t;
+  bool mfma, empty;
+};
+
+int paged_call(const dg_paged_attention_args* args, PagedCall* c) {
+  DG_REQUIRE(args != nullptr, DG_EINVAL, "paged_attention: NULL argument");
+  DG_REQUIRE(int_size(args->B) && int_size(args->N) && int_size(args->H), DG_EINVAL,
+             "paged_attention: negative size or one past 2^31 - 1");
+  DG_REQUIRE(known_dtype(args->dtype), DG_EUNSUPPORTED, "paged_attention: dtype %lld unsupported", (long long)args->dtype);
+  DG_REQUIRE(args->D >= 1 && args->D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_attention: head_dim %lld outside [1, %d]",
+             (long long)args->D, kMaxHeadDim);
+  DG_REQUIRE(args->Hkv >= 1 && args->Hkv <= 0x7fffffff && args->H % args->Hkv == 0, DG_EINVAL,
+             "paged_attention: %lld query heads on %lld key heads", (long long)args->H, (long long)args->Hkv);
+  const int64_t R = args->N * (args->H / args->Hkv);
+  DG_REQUIRE(R <= kMostPositions, DG_EINVAL, "paged_attention: a row of more than 2^30 (token, head) rows");
+  const float scale = (float)args->scale;
   DG_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), DG_EINVAL, "paged_attention: the scale must be positive and below 2^127");
-  if (B == 0 || N == 0 || H == 0) return DG_OK;
-  SeqArgs a{};
+  *c = PagedCall{};
+  c->empty = args->B == 0 || args->N == 0 || args->H == 0;
+  if (c->empty) return DG_OK;
+  const int B = (int)args->B, N = (int)args->N, H = (int)args->H, Hkv = (int)args->Hkv, D = (int)args->D, dtype = (int)args->dtype;
+  const dg_paged_rows* rows = &args->rows;
+  SeqArgs& a = c->a;
   if (const int rc = check_paged_rows("paged_attention", rows, true, &a.page_log2)) return rc;
-  DG_REQUIRE(q && y && q_st && y_st, DG_EINVAL, "paged_attention: NULL argument");
+  DG_REQUIRE(args->q && args->y, DG_EINVAL, "paged_attention: NULL argument");
   const int64_t cap = rows->width * rows->page;
-  DG_REQUIRE(longest >= 1 && longest <= cap, DG_EINVAL, "paged_attention: longest %lld, the table covers %lld positions",
-             (long long)longest, (long long)cap);
-  a.q = q; a.k = rows->k; a.v = rows->v; a.y = y;
-  a.qb = q_st->b; a.qt = q_st->t; a.qh = q_st->h;
+  DG_REQUIRE(args->longest >= 1 && args->longest <= cap, DG_EINVAL, "paged_attention: longest %lld, the table covers %lld positions",
+             (long long)args->longest, (long long)cap);
+  a.q = args->q; a.k = rows->k; a.v = rows->v; a.y = args->y;
+  a.qb = args->q_st.b; a.qt = args->q_st.t; a.qh = args->q_st.h;
   a.kb = rows->k_st.b; a.kt = rows->k_st.t; a.kh = rows->k_st.h;
   a.vb = rows->v_st.b; a.vt = rows->v_st.t; a.vh = rows->v_st.h;
-  a.yb = y_st->b; a.yt = y_st->t; a.yh = y_st->h;
+  a.yb = args->y_st.b; a.yt = args->y_st.t; a.yh = args->y_st.h;
   a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
   a.scale = scale;
   a.scale_log2 = scale * kLog2e;
   a.B = B; a.N = N; a.Tcap = (int)cap;
   a.lens = rows->lens; a.counts = rows->counts;
   a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;
-  const int64_t R = (int64_t)N * a.G;
-  const bool mfma = seq_mfma_applicable(a, dtype, true);
-  const PagedShape t = paged_shape(B, N, H, Hkv, D, dtype, longest, cap, weights != nullptr,
-                                   mfma ? mfma_rows(B, R, Hkv, (int)longest, D, dtype) : tile_rows(R, D), mfma);
+  c->mfma = seq_mfma_applicable(a, dtype, true);
+  c->t = paged_shape(B, N, H, Hkv, D, dtype, args->longest, cap, args->weights != nullptr,
+                     c->mfma ? mfma_rows(B, R, Hkv, (int)args->longest, D, dtype) : tile_rows(R, D), c->mfma);
+  const PagedShape& t = c->t;
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
   a.rb_groups = t.rb_groups; a.rb_each = t.rb_each;
+  return DG_OK;
+}
+
+}  // namespace
+}  // namespace dg
+
+extern "C" size_t dg_paged_attention_workspace_size(const dg_paged_attention_args* args) {
+  PagedCall c;
+  return paged_call(args, &c) == DG_OK ? c.t.ws_bytes : 0;
+}
+
+extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  PagedCall c;
+  if (const int rc = paged_call(args, &c)) return rc;
+  if (c.empty) return DG_OK;
+  SeqArgs& a = c.a;
+  const PagedShape& t = c.t;
+  const bool mfma = c.mfma;
+  const int B = a.B, Hkv = a.Hkv, dtype = (int)args->dtype;
+  const int64_t R = (int64_t)a.N * a.G, cap = a.Tcap;
+  float* const weights = args->weights;
   if (t.ws_bytes > 0) {
     DG_REQUIRE(workspace != nullptr && workspace_bytes >= t.ws_bytes, DG_EWORKSPACE,
                "paged_attention: a workspace of %zu bytes, %zu needed", workspace_bytes, t.ws_bytes);
@@ -372,7 +394,7 @@ extern "C" int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype
   const bool many = t.nsplit >= 16 && nrows <= 4096;
   const int64_t groups = t.nsplit == 1 ? 0 : many ? nrows : (nrows + 3) / 4;
   const int64_t blocks = t.blocks;
-  PagedWeights w{weights, w_b, w_h, 0};
+  PagedWeights w{weights, args->w_b, args->w_h, 0};
   const bool scored = t.scores_ld > 0;
   const int wkeys = scored ? 1024 : mfma ? kWeightKeys : 64;
   w.blocks = (int)((cap + wkeys - 1) / wkeys);

@@ -6,6 +6,9 @@
 
 namespace dg {
 
+inline bool int_size(int64_t n) { return n >= 0 && n <= 0x7fffffff; }
+inline bool known_dtype(int64_t dtype) { return dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64; }
+
 // What every entry point asks of a dg_paged_rows; *log2 receives that of its page.
 int check_paged_rows(const char* what, const dg_paged_rows* r, bool need_v, int* log2);
 

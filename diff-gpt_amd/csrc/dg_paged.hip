@@ -454,30 +454,32 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 using namespace dg;
 
-extern "C" int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
-                               const void* q, const dg_stride3* q_st, void* q_out, const dg_stride3* qo_st,
-                               const void* k, const dg_stride3* k_st, const void* v, const dg_stride3* v_st,
-                               const void* freqs, int64_t freqs_ld, int64_t freqs_rows, int freqs_dtype,
-                               const int32_t* positions, int flags, void* stream) {
-  DG_REQUIRE(B >= 0 && N >= 0 && H >= 0 && Hkv >= 0, DG_EINVAL, "paged_append: negative size");
-  DG_REQUIRE(D >= 2 && D % 2 == 0 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_append: head_dim %d, even ones from 2 to %d", D, kMaxHeadDim);
-  DG_REQUIRE(dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64, DG_EUNSUPPORTED,
-             "paged_append: dtype %d unsupported", dtype);
+extern "C" int dg_paged_append(const dg_paged_append_args* args, void* stream) {
+  DG_REQUIRE(args != nullptr, DG_EINVAL, "paged_append: NULL argument");
+  DG_REQUIRE(int_size(args->B) && int_size(args->N) && args->H >= 0 && args->Hkv >= 0, DG_EINVAL,
+             "paged_append: negative size or one past 2^31 - 1");
+  DG_REQUIRE(args->H <= 0xffff && args->Hkv <= 0xffff, DG_EINVAL, "paged_append: more than 65535 heads");
+  DG_REQUIRE(args->D >= 2 && args->D % 2 == 0 && args->D <= kMaxHeadDim, DG_EUNSUPPORTED,
+             "paged_append: head_dim %lld, even ones from 2 to %d", (long long)args->D, kMaxHeadDim);
+  DG_REQUIRE(known_dtype(args->dtype), DG_EUNSUPPORTED, "paged_append: dtype %lld unsupported", (long long)args->dtype);
+  const int B = (int)args->B, N = (int)args->N, H = (int)args->H, Hkv = (int)args->Hkv, D = (int)args->D, dtype = (int)args->dtype;
+  const int64_t freqs_dtype = args->freqs_dtype, freqs_ld = args->freqs_ld, freqs_rows = args->freqs_rows;
+  const void *q = args->q, *k = args->k, *v = args->v, *freqs = args->freqs;
+  const dg_paged_rows* rows = &args->rows;
   DG_REQUIRE(freqs_dtype == DG_F32 || freqs_dtype == dtype, DG_EUNSUPPORTED,
              "paged_append: freqs dtype must be fp32 or equal to the data dtype");
-  DG_REQUIRE(H <= 0xffff && Hkv <= 0xffff, DG_EINVAL, "paged_append: more than 65535 heads");
   if (B == 0 || N == 0 || H + Hkv == 0) return DG_OK;
   AppendArgs a{};
   if (const int rc = check_paged_rows("paged_append", rows, true, &a.page_log2)) return rc;
-  DG_REQUIRE(H == 0 || (q && q_out && q_st && qo_st), DG_EINVAL, "paged_append: NULL argument");
-  DG_REQUIRE(Hkv == 0 || (k && v && k_st && v_st), DG_EINVAL, "paged_append: NULL argument");
+  DG_REQUIRE(H == 0 || (q && args->q_out), DG_EINVAL, "paged_append: NULL argument");
+  DG_REQUIRE(Hkv == 0 || (k && v), DG_EINVAL, "paged_append: NULL argument");
   DG_REQUIRE(freqs && freqs_rows >= 1 && freqs_ld >= 0, DG_EINVAL, "paged_append: freqs table required");
   static const dg_stride3 none = {0, 0, 0};
   const void* src[3] = {q, k, v};
-  const dg_stride3* sst[3] = {H ? q_st : &none, Hkv ? k_st : &none, Hkv ? v_st : &none};
-  void* dst[3] = {q_out, rows->k, rows->v};
-  const dg_stride3* dst_st[3] = {H ? qo_st : &none, &rows->k_st, &rows->v_st};
-  const int64_t es = dtype_bytes(dtype), fes = dtype_bytes(freqs_dtype);
+  const dg_stride3* sst[3] = {H ? &args->q_st : &none, Hkv ? &args->k_st : &none, Hkv ? &args->v_st : &none};
+  void* dst[3] = {args->q_out, rows->k, rows->v};
+  const dg_stride3* dst_st[3] = {H ? &args->qo_st : &none, &rows->k_st, &rows->v_st};
+  const int64_t es = dtype_bytes(dtype), fes = dtype_bytes((int)freqs_dtype);
   bool vec = D * es % 16 == 0 && aligned16(freqs) && freqs_ld * fes % 16 == 0;
   for (int w = 0; w < 3; ++w) {
     a.src[w] = src[w];
@@ -489,10 +491,10 @@ extern "C" int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, c
   }
   a.freqs = freqs; a.freqs_ld = freqs_ld; a.freqs_rows = freqs_rows;
   a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;
-  a.lens = rows->lens; a.counts = rows->counts; a.positions = positions;
+  a.lens = rows->lens; a.counts = rows->counts; a.positions = args->positions;
   a.N = N; a.H = H; a.Hkv = Hkv; a.D = D;
   a.cap = (int)(rows->width * rows->page);
-  a.qknorm = (flags & DG_QKNORM) ? 1 : 0;
+  a.qknorm = (args->flags & DG_QKNORM) ? 1 : 0;
   const int64_t tokens = (int64_t)B * N;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == DG_F64)
@@ -503,26 +505,32 @@ extern "C" int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, c
   return freqs_dtype == DG_F32 ? append_pick<f16_t, float>(a, vec, tokens, s) : append_pick<f16_t, f16_t>(a, vec, tokens, s);
 }
 
-extern "C" int dg_paged_evict(int B, int Hkv, int D, int dtype, const dg_paged_rows* rows, const float* weights,
-                              int64_t w_b, int64_t w_h, int keep, int recent, const int32_t* to, int64_t to_ld,
-                              int64_t to_width, int32_t* new_lens, float* new_weights, int32_t* kept, void* stream) {
-  DG_REQUIRE(B >= 0 && Hkv >= 1, DG_EINVAL, "paged_evict: bad size");
-  DG_REQUIRE(D >= 1 && D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_evict: head_dim %d outside [1, %d]", D, kMaxHeadDim);
-  DG_REQUIRE(dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64, DG_EUNSUPPORTED,
-             "paged_evict: dtype %d unsupported", dtype);
-  DG_REQUIRE(keep >= 1 && recent >= 0 && recent <= keep, DG_EINVAL, "paged_evict: keep %d positions, %d of them the last", keep, recent);
+extern "C" int dg_paged_evict(const dg_paged_evict_args* args, void* stream) {
+  DG_REQUIRE(args != nullptr, DG_EINVAL, "paged_evict: NULL argument");
+  DG_REQUIRE(int_size(args->B) && int_size(args->Hkv) && args->Hkv >= 1, DG_EINVAL, "paged_evict: bad size");
+  DG_REQUIRE(args->D >= 1 && args->D <= kMaxHeadDim, DG_EUNSUPPORTED, "paged_evict: head_dim %lld outside [1, %d]",
+             (long long)args->D, kMaxHeadDim);
+  DG_REQUIRE(known_dtype(args->dtype), DG_EUNSUPPORTED, "paged_evict: dtype %lld unsupported", (long long)args->dtype);
+  DG_REQUIRE(args->keep >= 1 && args->keep <= kMostPositions && args->recent >= 0 && args->recent <= args->keep, DG_EINVAL,
+             "paged_evict: keep %lld positions, %lld of them the last", (long long)args->keep, (long long)args->recent);
+  const int B = (int)args->B, Hkv = (int)args->Hkv, D = (int)args->D, dtype = (int)args->dtype;
+  const int keep = (int)args->keep, recent = (int)args->recent;
+  const int64_t to_ld = args->to_ld, to_width = args->to_width;
+  const dg_paged_rows* rows = &args->rows;
+  const float* weights = args->weights;
+  const int32_t* to = args->to;
   if (B == 0) return DG_OK;
   EvictArgs a{};
   if (const int rc = check_paged_rows("paged_evict", rows, true, &a.page_log2)) return rc;
-  DG_REQUIRE(weights && to && new_lens && new_weights && kept, DG_EINVAL, "paged_evict: NULL argument");
+  DG_REQUIRE(weights && to && args->new_lens && args->new_weights && args->kept, DG_EINVAL, "paged_evict: NULL argument");
   DG_REQUIRE(to_width >= 1 && to_width <= kMostPositions / rows->page && keep <= to_width * rows->page, DG_EINVAL,
              "paged_evict: %d positions into %lld pages of %lld", keep, (long long)to_width, (long long)rows->page);
   const int64_t es = dtype_bytes(dtype);
-  a.weights = weights; a.wb = w_b; a.wh = w_h;
+  a.weights = weights; a.wb = args->w_b; a.wh = args->w_h;
   a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;
   a.to = to; a.to_ld = to_ld; a.to_cap = to_width * rows->page;
   a.lens = rows->lens;
-  a.new_lens = new_lens; a.new_weights = new_weights; a.kept = kept;
+  a.new_lens = args->new_lens; a.new_weights = args->new_weights; a.kept = args->kept;
   a.k = static_cast<const char*>(rows->k); a.v = static_cast<const char*>(rows->v);
   a.kb = rows->k_st.b * es; a.kt = rows->k_st.t * es; a.kh = rows->k_st.h * es;
   a.vb = rows->v_st.b * es; a.vt = rows->v_st.t * es; a.vh = rows->v_st.h * es;

@@ -510,41 +510,45 @@ int launch_verify(const VerifyArgs& a, const VerifyShape& t, bool greedy, hipStr
 
 using namespace dg;
 
-extern "C" size_t dg_verify_drafts_workspace_size(int B, int N, int64_t V, int dtype) {
-  if (B <= 0 || N < 0 || N > kMostDrafts || V <= 0 || V > 0x3fffffff) return 0;
-  return verify_shape(B, N, V).ws_bytes;
+extern "C" size_t dg_verify_drafts_workspace_size(const dg_verify_drafts_args* args) {
+  if (args == nullptr || args->B <= 0 || args->B > 0x7fffffff || args->N < 0 || args->N > kMostDrafts || args->V <= 0 ||
+      args->V > 0x3fffffff)
+    return 0;
+  return verify_shape(args->B, (int)args->N, args->V).ws_bytes;
 }
 
-extern "C" int dg_verify_drafts(int B, int N, int64_t V, int dtype, const void* target, int64_t t_b, int64_t t_n,
-                                const void* draft, int64_t d_b, int64_t d_n, const int64_t* tokens,
-                                const float* uniforms, const float* noise, int64_t noise_ld, const int32_t* counts,
-                                float inv_temperature, int64_t* accepted, int64_t* out_tokens, float* out_logprobs,
-                                void* workspace, size_t workspace_bytes, void* stream) {
-  DG_REQUIRE(B >= 0, DG_EINVAL, "verify_drafts: negative size");
-  DG_REQUIRE(N >= 0 && N <= kMostDrafts, DG_EINVAL, "verify_drafts: %d drafts a row, 0 to %d", N, kMostDrafts);
+extern "C" int dg_verify_drafts(const dg_verify_drafts_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  DG_REQUIRE(args != nullptr, DG_EINVAL, "verify_drafts: NULL argument");
+  DG_REQUIRE(args->B >= 0 && args->B <= 0x7fffffff, DG_EINVAL, "verify_drafts: negative size or one past 2^31 - 1");
+  DG_REQUIRE(args->N >= 0 && args->N <= kMostDrafts, DG_EINVAL, "verify_drafts: %lld drafts a row, 0 to %d", (long long)args->N,
+             kMostDrafts);
+  const int B = (int)args->B, N = (int)args->N;
+  const int64_t V = args->V, dtype = args->dtype;
+  const double inv_temperature = args->inv_temperature;
+  const void *target = args->target, *draft = args->draft;
   DG_REQUIRE(V >= 1 && V <= 0x3fffffff, DG_EINVAL, "verify_drafts: a vocabulary of %lld, 1 to 2^30 - 1", (long long)V);
   DG_REQUIRE(dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16 || dtype == DG_F64, DG_EUNSUPPORTED,
-             "verify_drafts: dtype %d unsupported", dtype);
-  DG_REQUIRE(inv_temperature == 0.f || (inv_temperature >= 0x1p-100f && inv_temperature <= 0x1p100f), DG_EINVAL,
+             "verify_drafts: dtype %lld unsupported", (long long)dtype);
+  DG_REQUIRE(inv_temperature == 0.0 || (inv_temperature >= 0x1p-100 && inv_temperature <= 0x1p100), DG_EINVAL,
              "verify_drafts: the inverse temperature must be 0 or between 2^-100 and 2^100");
   if (B == 0) return DG_OK;
-  const bool greedy = inv_temperature == 0.f;
-  DG_REQUIRE(target && accepted && out_tokens && out_logprobs && (N == 0 || tokens), DG_EINVAL, "verify_drafts: NULL argument");
-  DG_REQUIRE(greedy || (noise && (N == 0 || uniforms)), DG_EINVAL, "verify_drafts: random numbers missing");
-  const int64_t es = dtype_bytes(dtype);
+  const bool greedy = inv_temperature == 0.0;
+  DG_REQUIRE(target && args->accepted && args->out_tokens && args->out_logprobs && (N == 0 || args->tokens), DG_EINVAL, "verify_drafts: NULL argument");
+  DG_REQUIRE(greedy || (args->noise && (N == 0 || args->uniforms)), DG_EINVAL, "verify_drafts: random numbers missing");
+  const int64_t es = dtype_bytes((int)dtype);
   DG_REQUIRE(reinterpret_cast<uintptr_t>(target) % es == 0 && reinterpret_cast<uintptr_t>(draft) % es == 0, DG_EINVAL,
              "verify_drafts: logits not aligned to their element size");
   VerifyArgs a{};
-  a.target = target; a.tb = t_b; a.tn = t_n;
-  a.draft = greedy ? nullptr : draft; a.db = d_b; a.dn = d_n;
-  a.tokens = tokens; a.uniforms = uniforms; a.noise = noise; a.noise_ld = noise_ld; a.counts = counts;
-  a.scale = greedy ? 1.0 : (double)inv_temperature;
+  a.target = target; a.tb = args->t_b; a.tn = args->t_n;
+  a.draft = greedy ? nullptr : draft; a.db = args->d_b; a.dn = args->d_n;
+  a.tokens = args->tokens; a.uniforms = args->uniforms; a.noise = args->noise; a.noise_ld = args->noise_ld; a.counts = args->counts;
+  a.scale = greedy ? 1.0 : inv_temperature;
   const double l2 = a.scale * 1.4426950408889634074;
   // the leading term rounded down, so that the rest is positive and -inf times it still -inf
   a.scale_hi = (float)l2;
   if ((double)a.scale_hi >= l2) a.scale_hi = std::nextafter(a.scale_hi, 0.f);
   a.scale_lo = (float)(l2 - (double)a.scale_hi);
-  a.accepted = accepted; a.out_tokens = out_tokens; a.out_logprobs = out_logprobs;
+  a.accepted = args->accepted; a.out_tokens = args->out_tokens; a.out_logprobs = args->out_logprobs;
   a.B = B; a.N = N; a.V = (int)V;
   const VerifyShape t = verify_shape(B, N, V);
   a.rows = a.draft != nullptr ? 2 * N + 1 : N + 1;

@@ -17,6 +17,7 @@ import ctypes
 import math
 import operator
 import os
+import struct
 from pathlib import Path
 from typing import NamedTuple
 
@@ -273,35 +274,13 @@ _SIGNATURES = {
         [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
     ),
-    "dg_paged_append": (
-        ctypes.c_int,
-        [ctypes.c_int] * 6 + [ctypes.c_void_p]  # the rows
-        + [ctypes.c_void_p, ctypes.c_void_p] * 4  # q, q_out, k, v, each with its dg_stride3
-        + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p],
-    ),
-    "dg_paged_attention_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 6 + [ctypes.c_int64] * 2 + [ctypes.c_int]),
-    "dg_paged_attention": (
-        ctypes.c_int,
-        [ctypes.c_int] * 6 + [ctypes.c_void_p]  # the rows
-        + [ctypes.c_void_p, ctypes.c_void_p] * 2  # q, y, each with its dg_stride3
-        + [ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
-           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
-    ),
-    "dg_paged_evict": (
-        ctypes.c_int,
-        [ctypes.c_int] * 4
-        + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
-           ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
-           ctypes.c_void_p],
-    ),
-    "dg_verify_drafts_workspace_size": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int]),
-    "dg_verify_drafts": (
-        ctypes.c_int,
-        [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int]
-        + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64] * 2  # target, draft
-        + [ctypes.c_void_p] * 3 + [ctypes.c_int64, ctypes.c_void_p, ctypes.c_float]
-        + [ctypes.c_void_p] * 3 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
-    ),
+    # each takes its arguments packed (_PAGED_APPEND ..), and where it needs one a workspace
+    "dg_paged_append": (ctypes.c_int, [ctypes.c_void_p] * 2),
+    "dg_paged_attention_workspace_size": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "dg_paged_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "dg_paged_evict": (ctypes.c_int, [ctypes.c_void_p] * 2),
+    "dg_verify_drafts_workspace_size": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "dg_verify_drafts": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
 }
 
 ABI_VERSION = 6
@@ -984,9 +963,12 @@ def _token_logprobs(logits, ids, top, logprobs, entropy, top_logprobs, top_ids) 
             None if top_ids is None else top_logprobs.data_ptr(), None if top_ids is None else top_ids.data_ptr())
 
 
-# a dg_paged_rows, and dg_stride3 after dg_stride3
-_PagedRows = ctypes.c_int64 * 15
-_Stride3x2 = ctypes.c_int64 * 6
+# The argument structs of the entry points over a cache in pages: 8-byte integers and pointers,
+# and one double.  sizes, the dg_paged_rows, tensors with their strides, the rest.
+_PAGED_APPEND = struct.Struct("43q").pack
+_PAGED_ATTENTION = struct.Struct("29q d 4q").pack
+_PAGED_EVICT = struct.Struct("30q").pack
+_VERIFY_DRAFTS = struct.Struct("15q d 3q").pack
 
 
 def _int32_rows(what: str, name: str, t: torch.Tensor, B: int, device: int) -> int:
@@ -996,31 +978,33 @@ def _int32_rows(what: str, name: str, t: torch.Tensor, B: int, device: int) -> i
     return t.data_ptr()
 
 
-def _paged_rows(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-                counts: torch.Tensor | None, B: int, device: int) -> tuple[ctypes.Array, int]:
-    """The dg_paged_rows of (P, S, Hkv, D) pages, a (B, M) int32 table of page ids and (B,)
-    int32 lengths and counts, looked over, and how many positions the table covers."""
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+def _paged_rows(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, shape: tuple, table: torch.Tensor,
+                lengths: torch.Tensor, counts: torch.Tensor | None, B: int, device: int) -> tuple[tuple, int]:
+    """The members of the dg_paged_rows of (P, S, Hkv, D) pages of that shape, a (B, M) int32
+    table of page ids and (B,) int32 lengths and counts, looked over, and how many positions the
+    table covers."""
+    P, S, _, D = shape
+    if v_pages.shape != shape:
         raise ValueError(f"{what}: the pages must be (P, S, Hkv, D)")
-    P, S, _, D = k_pages.shape
     if P < 1 or S < 1 or S & (S - 1):
         raise ValueError(f"{what}: {P} pages of {S} positions: some, of a power of two")
     kb, kt, kh, kd = k_pages.stride()
     vb, vt, vh, vd = v_pages.stride()
     if not kd == vd == 1 and D > 1:
         raise ValueError(f"{what}: the last (head_dim) dimension must be contiguous")
-    if table.dim() != 2 or table.size(0) != B or table.dtype != torch.int32 or table.get_device() != device:
+    if table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != device:
         raise ValueError(f"{what}: the table must be a ({B}, pages a row) int32 tensor on the pages' device")
-    M = table.size(1)
+    rows, M = table.shape
+    if rows != B:
+        raise ValueError(f"{what}: the table must be a ({B}, pages a row) int32 tensor on the pages' device")
     if not 1 <= M * S <= MAX_POSITIONS:
         raise ValueError(f"{what}: a table of {M} pages of {S} positions a row, 1 to 2^30 positions")
     ld, unit = table.stride()
     if M > 1 and unit != 1:
         raise ValueError(f"{what}: a table's row must be contiguous")
-    lens = _int32_rows(what, "lengths", lengths, B, device)
-    n = 0 if counts is None else _int32_rows(what, "counts", counts, B, device)
-    return _PagedRows(k_pages.data_ptr(), v_pages.data_ptr(), kb, kt, kh, vb, vt, vh, P, S, table.data_ptr(), ld, M,
-                      lens, n), M * S
+    return (k_pages.data_ptr(), v_pages.data_ptr(), kb, kt, kh, vb, vt, vh, P, S, table.data_ptr(), ld, M,
+            _int32_rows(what, "lengths", lengths, B, device),
+            0 if counts is None else _int32_rows(what, "counts", counts, B, device)), M * S
 
 
 def paged_append_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, freqs: torch.Tensor, q_out: torch.Tensor,
@@ -1029,33 +1013,40 @@ def paged_append_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, freqs: torc
     """dg_paged_append: q, q_out (B,N,H,D), k, v (B,N,Hkv,D), freqs (positions, D/2, 2)."""
     what = "append_paged"
     device = _check_tensors(what, q, k, v, q_out, k_pages, v_pages)
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q_out.shape != q.shape:
-        raise ValueError(f"{what}: q must be (B, N, H, D) and k, v (B, N, Hkv, D)")
-    B, N, H, D = q.shape
-    Hkv = k.size(2)
-    if k.shape != (B, N, Hkv, D) or k_pages.dim() != 4 or k_pages.shape[2:] != (Hkv, D):
-        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and pages {tuple(k_pages.shape)} do not fit")
+    shape, kv, pages = q.shape, k.shape, k_pages.shape
+    if len(shape) != 4 or len(kv) != 4 or v.shape != kv or q_out.shape != shape or len(pages) != 4:
+        raise ValueError(f"{what}: q must be (B, N, H, D), k, v (B, N, Hkv, D) and the pages (P, S, Hkv, D)")
+    B, N, H, D = shape
+    Hkv = kv[2]
+    if kv != (B, N, Hkv, D) or pages[2] != Hkv or pages[3] != D:
+        raise ValueError(f"{what}: q {tuple(shape)}, k {tuple(kv)} and pages {tuple(pages)} do not fit")
     if not head_dim_supported(D):
         raise ValueError(f"{what}: head_dim {D}, even ones from 2 to {MAX_HEAD_DIM}")
     if Hkv < 1:
         raise ValueError(f"{what}: no key heads")
     if freqs.dim() != 3 or freqs.shape[1:] != (D // 2, 2) or freqs.size(0) < 1:
         raise ValueError(f"{what}: freqs must be (positions, {D // 2}, 2), got {tuple(freqs.shape)}")
-    if freqs.stride(2) != 1 or (D > 2 and freqs.stride(1) != 2):
+    ld, pair, unit = freqs.stride()
+    if unit != 1 or (D > 2 and pair != 2) or ld < 0:
         freqs = freqs.contiguous()
-    if freqs.dtype not in (torch.float32, q.dtype):
-        raise TypeError(f"{what}: freqs must be fp32 or {q.dtype}, got {freqs.dtype}")
+        ld = D
+    f_dtype, dtype = freqs.dtype, q.dtype
+    if f_dtype != dtype and f_dtype != torch.float32:
+        raise TypeError(f"{what}: freqs must be fp32 or {dtype}, got {f_dtype}")
     if freqs.get_device() != device:
         raise ValueError(f"{what}: freqs must be on the pages' device")
-    if not q.stride(3) == k.stride(3) == v.stride(3) == q_out.stride(3) == 1:
+    qb, qt, qh, qd = q.stride()
+    ob, ot, oh, od = q_out.stride()
+    kb, kt, kh, kd = k.stride()
+    vb, vt, vh, vd = v.stride()
+    if not qd == od == kd == vd == 1:
         raise ValueError(f"{what}: the last (head_dim) dimension must be contiguous")
-    rows, _ = _paged_rows(what, k_pages, v_pages, table, lengths, counts, B, device)
-    at = None if positions is None else _int32_rows(what, "positions", positions, B, device)
-    st = _Stride3x4(*q.stride()[:3], *q_out.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-    s = ctypes.addressof(st)
-    _launch(what, device, lib().dg_paged_append, B, N, H, Hkv, D, _DTYPE_CODE[q.dtype], rows, q.data_ptr(), s,
-            q_out.data_ptr(), s + 24, k.data_ptr(), s + 48, v.data_ptr(), s + 72, freqs.data_ptr(), freqs.stride(0),
-            freqs.size(0), _DTYPE_CODE[freqs.dtype], at, DG_QKNORM if qknorm else 0)
+    rows, _ = _paged_rows(what, k_pages, v_pages, pages, table, lengths, counts, B, device)
+    args = _PAGED_APPEND(B, N, H, Hkv, D, _DTYPE_CODE[dtype], *rows, q.data_ptr(), qb, qt, qh, q_out.data_ptr(), ob, ot, oh,
+                         k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, freqs.data_ptr(), ld, freqs.size(0),
+                         _DTYPE_CODE[f_dtype], 0 if positions is None else _int32_rows(what, "positions", positions, B, device),
+                         DG_QKNORM if qknorm else 0)
+    _launch(what, device, lib().dg_paged_append, args)
 
 
 def _weights_strides(what: str, weights: torch.Tensor, B: int, Hkv: int, cap: int, device: int) -> tuple[int, int]:
@@ -1074,53 +1065,52 @@ def paged_attention_(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     """dg_paged_attention: q, y (B,N,H,D) over pages (P,S,Hkv,D); weights (B,Hkv,positions) fp32."""
     what = "attention_paged"
     device = _check_tensors(what, q, k_pages, v_pages, y)
-    if q.dim() != 4 or k_pages.dim() != 4 or y.shape != q.shape:
+    shape, pages = q.shape, k_pages.shape
+    if len(shape) != 4 or len(pages) != 4 or y.shape != shape:
         raise ValueError(f"{what}: q, y must be (B, N, H, D) and the pages (P, S, Hkv, D)")
-    B, N, H, D = q.shape
-    Hkv = k_pages.size(2)
-    if k_pages.size(3) != D:
-        raise ValueError(f"{what}: head_dim {D}, pages of {k_pages.size(3)}")
+    B, N, H, D = shape
+    Hkv = pages[2]
+    if pages[3] != D:
+        raise ValueError(f"{what}: head_dim {D}, pages of {pages[3]}")
     if not 1 <= D <= MAX_HEAD_DIM:
         raise ValueError(f"{what}: head_dim {D} outside 1 .. {MAX_HEAD_DIM}")
     if Hkv < 1 or H % Hkv:
         raise ValueError(f"{what}: {H} query heads on {Hkv} key heads")
-    rows, cap = _paged_rows(what, k_pages, v_pages, table, lengths, counts, B, device)
-    w, wb, wh = None, 0, 0
+    rows, cap = _paged_rows(what, k_pages, v_pages, pages, table, lengths, counts, B, device)
+    w, wb, wh = 0, 0, 0
     if weights is not None:
         wb, wh = _weights_strides(what, weights, B, Hkv, cap, device)
         if (B > 1 and abs(wb) < cap) or (Hkv > 1 and abs(wh) < cap):
             raise ValueError(f"{what}: the rows' weights overlap")
         w = weights.data_ptr()
     longest = cap if longest is None else max(1, min(operator.index(longest), cap))
-    scale = _check_scale(what, scale)
     qb, qt, qh, qd = q.stride()
     yb, yt, yh, yd = y.stride()
     if not qd == yd == 1 and D > 1:
         raise ValueError(f"{what}: the last (head_dim) dimension must be contiguous")
-    code = _DTYPE_CODE[q.dtype]
     L = lib()
-    ws_bytes = L.dg_paged_attention_workspace_size(B, N, H, Hkv, D, code, longest, cap, w is not None)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    st = _Stride3x2(qb, qt, qh, yb, yt, yh)
-    s = ctypes.addressof(st)
-    _launch(what, device, L.dg_paged_attention, B, N, H, Hkv, D, code, rows, q.data_ptr(), s, y.data_ptr(), s + 24,
-            scale, longest, w, wb, wh, None if ws is None else ws.data_ptr(), ws_bytes)
+    args = _PAGED_ATTENTION(B, N, H, Hkv, D, _DTYPE_CODE[q.dtype], *rows, q.data_ptr(), qb, qt, qh, y.data_ptr(), yb, yt, yh,
+                            _check_scale(what, scale), longest, w, wb, wh)
+    ws_bytes = L.dg_paged_attention_workspace_size(args)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    _launch(what, device, L.dg_paged_attention, args, None if ws is None else ws.data_ptr(), ws_bytes)
 
 
-def paged_evict_(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-                 weights: torch.Tensor, keep: int, recent: int, to: torch.Tensor, new_lengths: torch.Tensor,
-                 new_weights: torch.Tensor, kept: torch.Tensor) -> None:
-    """dg_paged_evict into the pages that the (B, pages) int32 table ``to`` names, with
-    new_lengths (B,) and kept (B,Hkv,keep) int32 and new_weights (B,Hkv,positions of to) fp32."""
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                weights: torch.Tensor, keep: int, recent: int, to: torch.Tensor) -> tuple[torch.Tensor, ...]:
+    """dg_paged_evict into the pages that the (B, pages) int32 table ``to`` names: new tensors
+    of the lengths (B,) int32, the weights (B,Hkv,positions of to) fp32 and the kept positions
+    (B,Hkv,keep) int32."""
     what = "evict_paged"
     device = _check_tensors(what, k_pages, v_pages)
-    if k_pages.dim() != 4 or table.dim() != 2:
+    pages = k_pages.shape
+    if len(pages) != 4 or table.dim() != 2:
         raise ValueError(f"{what}: the pages must be (P, S, Hkv, D) and the table (B, pages a row)")
-    _, S, Hkv, D = k_pages.shape
+    _, S, Hkv, D = pages
     B = table.size(0)
     if not 1 <= D <= MAX_HEAD_DIM or Hkv < 1:
         raise ValueError(f"{what}: {Hkv} heads of {D}, head dims 1 .. {MAX_HEAD_DIM}")
-    rows, cap = _paged_rows(what, k_pages, v_pages, table, lengths, None, B, device)
+    rows, cap = _paged_rows(what, k_pages, v_pages, pages, table, lengths, None, B, device)
     wb, wh = _weights_strides(what, weights, B, Hkv, cap, device)
     keep, recent = operator.index(keep), operator.index(recent)
     if not 1 <= keep <= MAX_POSITIONS or not 0 <= recent <= keep:
@@ -1128,65 +1118,69 @@ def paged_evict_(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     if to.dim() != 2 or to.size(0) != B or to.dtype != torch.int32 or to.get_device() != device or (
             to.size(1) > 1 and to.stride(1) != 1):
         raise ValueError(f"{what}: to must be a ({B}, pages) int32 tensor on the pages' device")
-    room = to.size(1) * S
+    M = to.size(1)
+    room = M * S
     if not keep <= room <= MAX_POSITIONS:
-        raise ValueError(f"{what}: {keep} positions into {to.size(1)} pages of {S}")
-    for name, t, shape, dtype in (("new_lengths", new_lengths, (B,), torch.int32), ("kept", kept, (B, Hkv, keep), torch.int32),
-                                  ("new_weights", new_weights, (B, Hkv, room), torch.float32)):
-        if t.shape != shape or t.dtype != dtype or t.get_device() != device or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be a contiguous {shape} {dtype} tensor on the pages' device")
-    _launch(what, device, lib().dg_paged_evict, B, Hkv, D, _DTYPE_CODE[k_pages.dtype], rows, weights.data_ptr(), wb, wh,
-            keep, recent, to.data_ptr(), to.stride(0), to.size(1), new_lengths.data_ptr(), new_weights.data_ptr(),
-            kept.data_ptr())
+        raise ValueError(f"{what}: {keep} positions into {M} pages of {S}")
+    new_lengths, new_weights = lengths.new_empty(B), weights.new_empty((B, Hkv, room))
+    kept = lengths.new_empty((B, Hkv, keep))
+    args = _PAGED_EVICT(B, Hkv, D, _DTYPE_CODE[k_pages.dtype], *rows, weights.data_ptr(), wb, wh, keep, recent, to.data_ptr(),
+                        to.stride(0), M, new_lengths.data_ptr(), new_weights.data_ptr(), kept.data_ptr())
+    _launch(what, device, lib().dg_paged_evict, args)
+    return new_lengths, new_weights, kept
 
 
-def verify_drafts_(target: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | None, noise: torch.Tensor | None,
-                   draft: torch.Tensor | None, counts: torch.Tensor | None, temperature: float, accepted: torch.Tensor,
-                   out_tokens: torch.Tensor, out_logprobs: torch.Tensor) -> None:
+def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | None, noise: torch.Tensor | None,
+                  draft: torch.Tensor | None, counts: torch.Tensor | None, temperature: float) -> tuple[torch.Tensor, ...]:
     """dg_verify_drafts: target (B,N+1,V), draft (B,N,V), tokens (B,N) int64, uniforms (B,N) and
-    noise (B,V) fp32 into accepted (B,) int64, out_tokens (B,N+1) int64, out_logprobs (B,N+1) fp32."""
+    noise (B,V) fp32; new tensors of the accepted (B,) int64, the tokens (B,N+1) int64 and their
+    log probabilities (B,N+1) fp32."""
     what = "verify_drafts"
     device = _check_tensors(what, target) if draft is None else _check_tensors(what, target, draft)
-    if target.dim() != 3 or target.size(1) < 1 or target.size(2) < 1:
-        raise ValueError(f"{what}: target must be (B, N + 1, V), got {tuple(target.shape)}")
-    B, N, V = target.size(0), target.size(1) - 1, target.size(2)
+    shape = target.shape
+    if len(shape) != 3 or shape[1] < 1 or shape[2] < 1:
+        raise ValueError(f"{what}: target must be (B, N + 1, V), got {tuple(shape)}")
+    B, N, V = shape[0], shape[1] - 1, shape[2]
     if N > MAX_DRAFTS:
         raise ValueError(f"{what}: {N} drafts a row, 0 to {MAX_DRAFTS}")
     temperature = float(temperature)
     if temperature != 0 and not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"{what}: the temperature must be 0 or between 1e-30 and 1e30, got {temperature}")
     t_b, t_n, unit = target.stride()
-    d_b = d_n = 0
+    d = d_b = d_n = 0
     if draft is not None:
         if draft.shape != (B, N, V):
             raise ValueError(f"{what}: draft must be {(B, N, V)}, got {tuple(draft.shape)}")
         d_b, d_n, d_unit = draft.stride()
         unit = unit if d_unit == 1 else d_unit
+        d = draft.data_ptr()
     if unit != 1 and V > 1:
         raise ValueError(f"{what}: the last (vocabulary) dimension must be contiguous")
     if temperature > 0 and (noise is None or (uniforms is None and N > 0)):
         raise ValueError(f"{what}: uniforms and noise are needed at a temperature above 0")
-    for name, t, shape, dtype in (("tokens", tokens, (B, N), torch.int64), ("uniforms", uniforms, (B, N), torch.float32),
-                                  ("accepted", accepted, (B,), torch.int64), ("out_tokens", out_tokens, (B, N + 1), torch.int64),
-                                  ("out_logprobs", out_logprobs, (B, N + 1), torch.float32)):
-        if t is not None and (t.dtype != dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be a contiguous {shape} {dtype} tensor on the logits' device")
-    ld = 0
+    if tokens.dtype != torch.int64 or tokens.shape != (B, N) or tokens.get_device() != device or not tokens.is_contiguous():
+        raise ValueError(f"{what}: tokens must be a contiguous {(B, N)} int64 tensor on the logits' device")
+    if uniforms is not None and (uniforms.dtype != torch.float32 or uniforms.shape != (B, N) or
+                                 uniforms.get_device() != device or not uniforms.is_contiguous()):
+        raise ValueError(f"{what}: uniforms must be a contiguous {(B, N)} fp32 tensor on the logits' device")
+    e = ld = 0
     if noise is not None:
         if noise.shape != (B, V) or noise.dtype != torch.float32 or noise.get_device() != device or (
                 V > 1 and noise.stride(1) != 1):
             raise ValueError(f"{what}: noise must be a {(B, V)} fp32 tensor on the logits' device, its rows contiguous")
-        ld = noise.stride(0)
-    n = None if counts is None else _int32_rows(what, "counts", counts, B, device)
+        e, ld = noise.data_ptr(), noise.stride(0)
+    new = tokens.new_empty
+    accepted, out_tokens, out_logprobs = new(B), new((B, N + 1)), new((B, N + 1), dtype=torch.float32)
     L = lib()
-    code = _DTYPE_CODE[target.dtype]
-    ws_bytes = L.dg_verify_drafts_workspace_size(B, N, V, code)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=target.device) if ws_bytes else None
-    _launch(what, device, L.dg_verify_drafts, B, N, V, code, target.data_ptr(), t_b, t_n,
-            None if draft is None else draft.data_ptr(), d_b, d_n, tokens.data_ptr(),
-            None if uniforms is None else uniforms.data_ptr(), None if noise is None else noise.data_ptr(), ld, n,
-            0.0 if temperature == 0 else 1.0 / temperature, accepted.data_ptr(), out_tokens.data_ptr(),
-            out_logprobs.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes)
+    args = _VERIFY_DRAFTS(B, N, V, _DTYPE_CODE[target.dtype], target.data_ptr(), t_b, t_n, d, d_b, d_n, tokens.data_ptr(),
+                          0 if uniforms is None else uniforms.data_ptr(), e, ld,
+                          0 if counts is None else _int32_rows(what, "counts", counts, B, device),
+                          0.0 if temperature == 0 else 1.0 / temperature, accepted.data_ptr(), out_tokens.data_ptr(),
+                          out_logprobs.data_ptr())
+    ws_bytes = L.dg_verify_drafts_workspace_size(args)
+    ws = target.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    _launch(what, device, L.dg_verify_drafts, args, None if ws is None else ws.data_ptr(), ws_bytes)
+    return accepted, out_tokens, out_logprobs
 
 
 def copy4d_(src: torch.Tensor, dst: torch.Tensor) -> None:

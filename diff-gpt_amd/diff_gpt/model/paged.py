@@ -61,12 +61,7 @@ def evict_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tenso
     their order into the pages that ``to`` (B, pages) int32 names, none of which any row may
     hold.  A row of no more positions moves as it is.  Keys stay turned by the positions they
     had."""
-    B, Hkv, S = table.size(0), k_pages.size(2), k_pages.size(1)
-    new = weights.new_empty
-    r = Evicted(new(B, dtype=torch.int32), new((B, Hkv, to.size(1) * S), dtype=torch.float32),
-                new((B, Hkv, max(0, keep)), dtype=torch.int32))
-    _native.paged_evict_(k_pages, v_pages, table, lengths, weights, keep, recent, to, r.lengths, r.weights, r.kept)
-    return r
+    return Evicted(*_native.paged_evict(k_pages, v_pages, table, lengths, weights, keep, recent, to))
 
 
 class PagedKVCache:

@@ -34,8 +34,4 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     stand): uniforms (B, N) in [0, 1) and noise (B, V) from Exp(1), fp32.  At temperature 0
     draft x stands iff it is the first maximum of its logits, nothing is drawn, and log
     probabilities are those at temperature 1.  A draft outside the vocabulary does not stand."""
-    B, N = target.size(0), target.size(1) - 1
-    new = target.new_empty
-    r = Verified(new(B, dtype=torch.int64), new((B, N + 1), dtype=torch.int64), new((B, N + 1), dtype=torch.float32))
-    _native.verify_drafts_(target, tokens, uniforms, noise, draft, counts, temperature, *r)
-    return r
+    return Verified(*_native.verify_drafts(target, tokens, uniforms, noise, draft, counts, temperature))

@@ -673,6 +673,10 @@ DG_API int dg_token_logprobs(int64_t M, int64_t V, int dtype, const void* x, int
  * counts as 0 .. N and as what the table still covers: tokens further on count as not there.
  * A page id that the pool does not have is never followed: its positions read as zeros and
  * are not written.
+ *
+ * These entry points take their arguments in a struct of 8-byte members (a call with 25 of
+ * them, through a binding that converts each, costs the host as much as the launch); sizes
+ * are looked over as everywhere.
  */
 typedef struct dg_paged_rows {
   void* k;
@@ -696,11 +700,24 @@ typedef struct dg_paged_rows {
  * there have zeros in q_out and write nothing.  q, q_out (B,N,H,D), k, v (B,N,Hkv,D) views;
  * freqs fp32 or of the data's type.  Every even D up to 1024; fp32 / bf16 / fp16 / fp64.
  */
-DG_API int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
-                           const void* q, const dg_stride3* q_st, void* q_out, const dg_stride3* qo_st,
-                           const void* k, const dg_stride3* k_st, const void* v, const dg_stride3* v_st,
-                           const void* freqs, int64_t freqs_ld, int64_t freqs_rows, int freqs_dtype,
-                           const int32_t* positions, int flags, void* stream);
+typedef struct dg_paged_append_args {
+  int64_t B, N, H, Hkv, D, dtype;
+  dg_paged_rows rows;
+  const void* q;
+  dg_stride3 q_st;
+  void* q_out;
+  dg_stride3 qo_st;
+  const void* k;
+  dg_stride3 k_st;
+  const void* v;
+  dg_stride3 v_st;
+  const void* freqs;
+  int64_t freqs_ld, freqs_rows, freqs_dtype;
+  const int32_t* positions;
+  int64_t flags;
+} dg_paged_append_args;
+
+DG_API int dg_paged_append(const dg_paged_append_args* args, void* stream);
 
 /*
  * Attention of each row's N newest tokens, which the pages already hold, over its positions:
@@ -712,17 +729,27 @@ DG_API int dg_paged_append(int B, int N, int H, int Hkv, int D, int dtype, const
  * atomics, in an order of its own; what lies behind a row's positions is left as it is.
  * Long rows are split over workgroups; partial results, and with weights the rows' softmax
  * sums and few rows' scores, meet in the caller's workspace (16-byte aligned, no
- * initialisation, one each for calls that may overlap; `positions` is width * page).  `longest`, at most width * page, is a hint of the positions that the
+ * initialisation, one each for calls that may overlap; its size is that of these arguments).  `longest`, at most width * page, is a hint of the positions that the
  * longest row will hold, and decides how rows are split, no more than that.
  * Types, head_dim and scale as dg_attention_packed.
  */
-DG_API size_t dg_paged_attention_workspace_size(int B, int N, int H, int Hkv, int D, int dtype, int64_t longest,
-                                                int64_t positions, int weights);
+typedef struct dg_paged_attention_args {
+  int64_t B, N, H, Hkv, D, dtype;
+  dg_paged_rows rows;
+  const void* q;
+  dg_stride3 q_st;
+  void* y;
+  dg_stride3 y_st;
+  double scale;
+  int64_t longest;
+  float* weights;
+  int64_t w_b, w_h;
+} dg_paged_attention_args;
 
-DG_API int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype, const dg_paged_rows* rows,
-                              const void* q, const dg_stride3* q_st, void* y, const dg_stride3* y_st, float scale,
-                              int64_t longest, float* weights, int64_t w_b, int64_t w_h,
-                              void* workspace, size_t workspace_bytes, void* stream);
+DG_API size_t dg_paged_attention_workspace_size(const dg_paged_attention_args* args);
+
+DG_API int dg_paged_attention(const dg_paged_attention_args* args, void* workspace, size_t workspace_bytes,
+                              void* stream);
 
 /*
  * Rows cut to `keep` positions a key head: of the first lens[b] positions the `recent` last
@@ -735,9 +762,19 @@ DG_API int dg_paged_attention(int B, int N, int H, int Hkv, int D, int dtype, co
  * behind them.  The pages that `to` names must not be any that the rows hold, nor named twice.
  * 0 <= recent <= keep, keep >= 1; rows->counts is not looked at.  Every D up to 1024.
  */
-DG_API int dg_paged_evict(int B, int Hkv, int D, int dtype, const dg_paged_rows* rows, const float* weights,
-                          int64_t w_b, int64_t w_h, int keep, int recent, const int32_t* to, int64_t to_ld,
-                          int64_t to_width, int32_t* new_lens, float* new_weights, int32_t* kept, void* stream);
+typedef struct dg_paged_evict_args {
+  int64_t B, Hkv, D, dtype;
+  dg_paged_rows rows;
+  const float* weights;
+  int64_t w_b, w_h, keep, recent;
+  const int32_t* to;
+  int64_t to_ld, to_width;
+  int32_t* new_lens;
+  float* new_weights;
+  int32_t* kept;
+} dg_paged_evict_args;
+
+DG_API int dg_paged_evict(const dg_paged_evict_args* args, void* stream);
 
 /*
  * Drafted tokens against the target model's probabilities.  Row b has counts[b] (NULL: N;
@@ -756,13 +793,26 @@ DG_API int dg_paged_evict(int B, int Hkv, int D, int dtype, const dg_paged_rows*
  * a row with NaN, +inf or -inf alone, and the token after it is then not specified but within
  * [0, V).  0 <= N <= 64; inv_temperature 0 or from 2^-100 to 2^100.
  */
-DG_API size_t dg_verify_drafts_workspace_size(int B, int N, int64_t V, int dtype);
+typedef struct dg_verify_drafts_args {
+  int64_t B, N, V, dtype;
+  const void* target;
+  int64_t t_b, t_n;
+  const void* draft;
+  int64_t d_b, d_n;
+  const int64_t* tokens;
+  const float* uniforms;
+  const float* noise;
+  int64_t noise_ld;
+  const int32_t* counts;
+  double inv_temperature;
+  int64_t* accepted;
+  int64_t* out_tokens;
+  float* out_logprobs;
+} dg_verify_drafts_args;
 
-DG_API int dg_verify_drafts(int B, int N, int64_t V, int dtype, const void* target, int64_t t_b, int64_t t_n,
-                            const void* draft, int64_t d_b, int64_t d_n, const int64_t* tokens,
-                            const float* uniforms, const float* noise, int64_t noise_ld, const int32_t* counts,
-                            float inv_temperature, int64_t* accepted, int64_t* out_tokens, float* out_logprobs,
-                            void* workspace, size_t workspace_bytes, void* stream);
+DG_API size_t dg_verify_drafts_workspace_size(const dg_verify_drafts_args* args);
+
+DG_API int dg_verify_drafts(const dg_verify_drafts_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
