@@ -28,7 +28,8 @@ TIMELINE_LIB = PKG / "lib" / "libdgattn_timeline.so"
 SOURCES = ["dg_abi.hip", "dg_rope.hip", "dg_attn_vec.hip", "dg_attn_mfma.hip", "dg_attn_mfma_f32.hip",
            "dg_attn_small.hip", "dg_attn_shared.hip", "dg_attn_wide.hip", "dg_block.hip", "dg_layer.hip",
            "dg_linear.hip", "dg_noalloc.hip", "dg_attn_seq.hip", "dg_attn_seq_mfma.hip", "dg_logprobs.hip",
-           "dg_attn_paged.hip", "dg_attn_paged_mfma.hip", "dg_paged.hip", "dg_verify.hip"]
+           "dg_attn_paged.hip", "dg_attn_paged_mfma.hip", "dg_attn_paged_vec.hip", "dg_paged.hip",
+           "dg_verify.hip"]
 HEADERS = ["dg_common.h", "dg_rope_math.h", "dg_prefill.h", "dg_rows.h", "dg_seq.h", "dg_seq_mfma.h", "dg_seq_tile.h", "dg_paged.h",
            str(REPO / "include" / "dgattn.h")]
 

@@ -201,6 +201,8 @@ int mfma_rows(int64_t B, int64_t rows, int Hkv, int keys, int D, int dtype) {
 
 constexpr int kMaxSplits = 512;
 
+enum PagedKernel { kTileKernel, kMfmaKernel, kVecKernel };
+
 // Row blocks, splits and workspace of a call.
 struct PagedShape {
   int rows_per_wg, nrb, nsplit, chunk, rb_groups, rb_each;
@@ -229,8 +231,8 @@ int64_t stage_ns(int D, int dtype, int rows_per_wg) {
 //   8 x 200, 4000, 8 / 8 of 64, 32              36.3 / 43 / 51 / 51
 //   6 x 237, 5580, 2 / 2 of 16, 32              21.7 / 18 / 16 / 19
 //   5 x 25, 13386, fp32, 24 / 6 of 80, 64       909 / 464 / 246 / 198
-int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t fill, int D, int dtype, int rows_per_wg) {
-  const int64_t whole = longest * stage_ns(D, dtype, rows_per_wg) / 128;
+int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t fill, int D, int64_t ns) {
+  const int64_t whole = longest * ns / 128;
   int best = 1;
   int64_t least = (wg + fill - 1) / fill * whole;
   const int64_t most = std::min<int64_t>(longest / 256, kMaxSplits);
@@ -245,7 +247,8 @@ int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t fill, int D, 
 }
 
 PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64_t longest, int64_t cap, int weights,
-                       int rows_per_wg, bool mfma) {
+                       int rows_per_wg, PagedKernel kernel) {
+  const bool mfma = kernel != kTileKernel, vec = kernel == kVecKernel;
   PagedShape t{};
   const int64_t R = (int64_t)N * (H / Hkv);
   t.rows_per_wg = rows_per_wg;
@@ -253,11 +256,13 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
   const int Dm = mfma ? seq_mfma_dim(D) : D;
   const int64_t row_bytes = Dm * dtype_bytes(dtype);
   const int64_t fill = !mfma ? 2048
+                       : vec ? 1024
                        : rows_per_wg <= 32 ? (row_bytes >= 256 ? 256 : 512)
                        : rows_per_wg == 64 ? (row_bytes >= 512 ? 256 : 512)
                                            : Dm == 256 ? 512 : Dm == 128 ? 768 : 1024;
   const int64_t wg = std::max<int64_t>(1, B * Hkv * t.nrb);
-  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, fill, Dm, dtype, rows_per_wg)
+  const int64_t ns = vec ? 1200 + Dm * R * 3 : mfma ? stage_ns(Dm, dtype, rows_per_wg) : 0;
+  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, fill, Dm, ns)
                   : (int)std::max<int64_t>(1, std::min<int64_t>({(fill + wg - 1) / wg, longest / 256, kMaxSplits}));
   t.chunk = 256;
   // every XCD has work: the row blocks of few (b, key head, split) go to several, in groups
@@ -312,7 +317,8 @@ namespace {
 struct PagedCall {
   SeqArgs a;
   PagedShape t;
-  bool mfma, empty;
+  PagedKernel kernel;
+  bool empty;
 };
 
 int paged_call(const dg_paged_attention_args* args, PagedCall* c) {
@@ -350,9 +356,17 @@ int paged_call(const dg_paged_attention_args* args, PagedCall* c) {
   a.B = B; a.N = N; a.Tcap = (int)cap;
   a.lens = rows->lens; a.counts = rows->counts;
   a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;
-  c->mfma = seq_mfma_applicable(a, dtype, true);
-  c->t = paged_shape(B, N, H, Hkv, D, dtype, args->longest, cap, args->weights != nullptr,
-                     c->mfma ? mfma_rows(B, R, Hkv, (int)args->longest, D, dtype) : tile_rows(R, D), c->mfma);
+  // fp32 heads of up to 256 dims are looked at as if of 64, up to 128 of which the matrix cores take
+  SeqArgs narrow = a;
+  narrow.D = std::min(D, 64);
+  const bool pieces = D <= 256 && D % 4 == 0 && seq_mfma_applicable(narrow, dtype, true);
+  c->kernel = dtype == DG_F32 && R <= kVecRows && pieces ? kVecKernel
+              : seq_mfma_applicable(a, dtype, true)      ? kMfmaKernel
+                                                         : kTileKernel;
+  const int rows_per_wg = c->kernel == kVecKernel    ? 32
+                          : c->kernel == kMfmaKernel ? mfma_rows(B, R, Hkv, (int)args->longest, D, dtype)
+                                                     : tile_rows(R, D);
+  c->t = paged_shape(B, N, H, Hkv, D, dtype, args->longest, cap, args->weights != nullptr, rows_per_wg, c->kernel);
   const PagedShape& t = c->t;
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
   a.rb_groups = t.rb_groups; a.rb_each = t.rb_each;
@@ -373,7 +387,7 @@ extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* wor
   if (c.empty) return DG_OK;
   SeqArgs& a = c.a;
   const PagedShape& t = c.t;
-  const bool mfma = c.mfma;
+  const bool mfma = c.kernel != kTileKernel, vec = c.kernel == kVecKernel;
   const int B = a.B, Hkv = a.Hkv, dtype = (int)args->dtype;
   const int64_t R = (int64_t)a.N * a.G, cap = a.Tcap;
   float* const weights = args->weights;
@@ -395,10 +409,10 @@ extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* wor
   const int64_t groups = t.nsplit == 1 ? 0 : many ? nrows : (nrows + 3) / 4;
   const int64_t blocks = t.blocks;
   PagedWeights w{weights, args->w_b, args->w_h, 0};
-  const bool scored = t.scores_ld > 0;
-  const int wkeys = scored ? 1024 : mfma ? kWeightKeys : 64;
+  const bool scored = t.scores_ld > 0, wmfma = mfma && (dtype != DG_F32 || a.D <= 128);
+  const int wkeys = scored ? 1024 : wmfma ? kWeightKeys : 64;
   w.blocks = (int)((cap + wkeys - 1) / wkeys);
-  const int64_t wblocks = weights == nullptr ? 0 : mfma && !scored ? ((int64_t)B * Hkv + 7) / 8 * 8 * w.blocks : (int64_t)B * Hkv * w.blocks;
+  const int64_t wblocks = weights == nullptr ? 0 : wmfma && !scored ? ((int64_t)B * Hkv + 7) / 8 * 8 * w.blocks : (int64_t)B * Hkv * w.blocks;
   DG_REQUIRE(blocks <= kMostWorkgroups256 && groups <= kMostWorkgroups256 && wblocks <= kMostWorkgroups256, DG_EINVAL,
              "paged_attention: more than 2^24 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -408,7 +422,8 @@ extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* wor
     hipLaunchKernelGGL(paged_order_kernel, dim3(1), dim3(kOrdered), 0, s, a, const_cast<int32_t*>(a.order));
     if ((rc = check_launch("paged_order_kernel")) != DG_OK) return rc;
   }
-  if (mfma) rc = launch_seq_mfma_paged(a, dtype, (unsigned)blocks, s);
+  if (vec) rc = launch_paged_vec(a, (unsigned)blocks, s);
+  else if (mfma) rc = launch_seq_mfma_paged(a, dtype, (unsigned)blocks, s);
   else if (dtype == DG_F64) rc = launch_tile<double>(a, grid, s);
   else if (dtype == DG_F32) rc = launch_tile<float>(a, grid, s);
   else if (dtype == DG_BF16) rc = launch_tile<bf16_t>(a, grid, s);
@@ -424,7 +439,7 @@ extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* wor
     hipLaunchKernelGGL(paged_scores_kernel, wgrid, dim3(256), 0, s, a, w);
     return check_launch("paged_scores_kernel");
   }
-  if (mfma) return launch_paged_weights_mfma(a, w, dtype, (unsigned)wblocks, s);
+  if (wmfma) return launch_paged_weights_mfma(a, w, dtype, (unsigned)wblocks, s);
   if (dtype == DG_F64) hipLaunchKernelGGL(paged_weights_any_kernel<double>, wgrid, dim3(256), 0, s, a, w);
   else if (dtype == DG_F32) hipLaunchKernelGGL(paged_weights_any_kernel<float>, wgrid, dim3(256), 0, s, a, w);
   else if (dtype == DG_BF16) hipLaunchKernelGGL(paged_weights_any_kernel<bf16_t>, wgrid, dim3(256), 0, s, a, w);

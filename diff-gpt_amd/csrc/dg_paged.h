@@ -16,6 +16,11 @@ int check_paged_rows(const char* what, const dg_paged_rows* r, bool need_v, int*
 // positions' weights, for shapes that seq_mfma_applicable takes.
 int launch_seq_mfma_paged(const SeqArgs& a, int dtype, unsigned blocks, hipStream_t s);
 
+// dg_attn_paged_vec.hip: up to kVecRows fp32 (token, head) rows of a key head of up to 256 dims,
+// in 16-byte pieces.
+constexpr int kVecRows = 8;
+int launch_paged_vec(const SeqArgs& a, unsigned blocks, hipStream_t s);
+
 // The weights' arguments: a.q, a.k, the table and lengths as for the attention, a.lse its
 // result; a.nrb is unused.
 struct PagedWeights {
