@@ -360,7 +360,7 @@ int paged_call(const dg_paged_attention_args* args, PagedCall* c) {
   SeqArgs narrow = a;
   narrow.D = std::min(D, 64);
   const bool pieces = D <= 256 && D % 4 == 0 && seq_mfma_applicable(narrow, dtype, true);
-  c->kernel = dtype == DG_F32 && R <= kVecRows && pieces ? kVecKernel
+  c->kernel = dtype == DG_F32 && R <= paged_vec_rows(D) && pieces ? kVecKernel
               : seq_mfma_applicable(a, dtype, true)      ? kMfmaKernel
                                                          : kTileKernel;
   const int rows_per_wg = c->kernel == kVecKernel    ? 32

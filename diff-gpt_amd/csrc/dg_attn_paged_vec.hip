@@ -1,7 +1,7 @@
-// Attention over a cache in pages for up to eight fp32 (token, head) rows of a key head: a
-// decode step, or a few drafted tokens.  The fp32 matrix instructions take 32 rows whatever
-// there are, and eight cycles of a CU for each key's 128 dims; here keys and values go
-// straight into registers and the products run on the vector units, bound by HBM.
+// Attention over a cache in pages for a few fp32 (token, head) rows of a key head: a decode
+// step.  The fp32 matrix instructions take 32 rows whatever there are; here keys and values
+// go straight into registers and the products run on the vector units, bound by HBM where rows
+// are few (which: paged_vec_rows).
 //
 // LPK = D / 8 lanes share a key (eight dims each, two 16-byte loads), a wave has KPS = 64 / LPK
 // keys at a time and U times as many in flight, the four waves of a workgroup take turns.
@@ -151,17 +151,10 @@ __global__ __launch_bounds__(256) void paged_vec_kernel(const SeqArgs a) {
     for (int x = LPK; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
     const float f = m[r] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[r] - top);
     // a state without a key has zeros; a NaN is taken along
-    float sum = (l[r] - lc[r]) * f;
-#pragma unroll
-    for (int x = LPK; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
     m[r] = top;
-    l[r] = sum;
+    l[r] = sum_over_groups<LPK>((l[r] - lc[r]) * f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      o[r][e] *= f;
-#pragma unroll
-      for (int x = LPK; x < 64; x <<= 1) o[r][e] += __shfl_xor(o[r][e], x, 64);
-    }
+    for (int e = 0; e < 8; ++e) o[r][e] = sum_over_groups<LPK>(o[r][e] * f);
   }
   if (wv > 0 && grp == 0) {
 #pragma unroll
@@ -227,11 +220,15 @@ namespace {
 
 template <int D>
 int launch_vec_rows(const SeqArgs& a, dim3 grid, hipStream_t s) {
+  constexpr int MOST = paged_vec_rows(D);
   const int R = a.N * a.G;
+  if (R > MOST) return DG_EUNSUPPORTED;
   if (R <= 1) hipLaunchKernelGGL((paged_vec_kernel<D, 1>), grid, dim3(256), 0, s, a);
   else if (R <= 2) hipLaunchKernelGGL((paged_vec_kernel<D, 2>), grid, dim3(256), 0, s, a);
-  else if (R <= 4) hipLaunchKernelGGL((paged_vec_kernel<D, 4>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((paged_vec_kernel<D, 8>), grid, dim3(256), 0, s, a);
+  else if constexpr (MOST >= 4) {
+    if (R <= 4) hipLaunchKernelGGL((paged_vec_kernel<D, 4>), grid, dim3(256), 0, s, a);
+    else if constexpr (MOST >= 8) hipLaunchKernelGGL((paged_vec_kernel<D, 8>), grid, dim3(256), 0, s, a);
+  }
   return check_launch("paged_vec_kernel");
 }
 
