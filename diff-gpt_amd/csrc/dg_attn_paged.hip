@@ -26,56 +26,58 @@ __global__ __launch_bounds__(256) void paged_weights_any_kernel(const SeqArgs a,
   const int kvh = (int)(u - b * a.Hkv);
   const PagedRow pr = paged_row(a, b, __builtin_amdgcn_readfirstlane(a.lens[b]));
   const int total = pr.own + pr.count, nrows = pr.count * a.G;
-  const int kb = blk * KT;
-  if (kb >= total || nrows == 0) return;  // whole workgroups
+  if (nrows == 0) return;  // whole workgroups
   const int tid = threadIdx.x, key = tid & 63, sub = tid >> 6;
-  const int t = kb + key;
-  const int from = t >= total ? nrows : (int)max((int64_t)(t - pr.own) * a.G, (int64_t)0);
-  const int first = max(kb - pr.own, 0) * a.G / RT * RT;
-  const T* const qb = static_cast<const T*>(a.q) + b * a.qb + (int64_t)kvh * a.G * a.qh;
-  const T* const kh = static_cast<const T*>(a.k) + (int64_t)kvh * a.kh;
-  const A* const lse = static_cast<const A*>(a.lse) + (b * a.Hkv + kvh) * (int64_t)(a.N * a.G);
-  const A us = S::unit_scale(a);
-  A acc = (A)0, rest = (A)0;
-  for (int row0 = first; row0 < nrows; row0 += RT) {
-    A s[RPT];
+  for (int64_t k0 = (int64_t)blk * KT; k0 < total; k0 += (int64_t)w.blocks * KT) {
+    const int kb = (int)k0, t = kb + key;
+    const int from = t >= total ? nrows : (int)max((int64_t)(t - pr.own) * a.G, (int64_t)0);
+    const int first = max(kb - pr.own, 0) * a.G / RT * RT;
+    const T* const qb = static_cast<const T*>(a.q) + b * a.qb + (int64_t)kvh * a.G * a.qh;
+    const T* const kh = static_cast<const T*>(a.k) + (int64_t)kvh * a.kh;
+    const A* const lse = static_cast<const A*>(a.lse) + (b * a.Hkv + kvh) * (int64_t)(a.N * a.G);
+    const A us = S::unit_scale(a);
+    A acc = (A)0, rest = (A)0;
+    for (int row0 = first; row0 < nrows; row0 += RT) {
+      A s[RPT];
 #pragma unroll
-    for (int j = 0; j < RPT; ++j) s[j] = (A)0;
-    for (int d0 = 0; d0 < a.D; d0 += 64) {
-      __syncthreads();
-      for (int e = tid; e < KT * 64; e += 256) {
-        const int kt = kb + e / 64, d = d0 + e % 64;
-        A x = (A)0;
-        if (kt < total && d < a.D) {
-          const int id = a.table[b * a.table_ld + (kt >> a.page_log2)];
-          if (id >= 0 && id < a.pages) x = S::load(kh[id * a.kb + (kt & ((1 << a.page_log2) - 1)) * a.kt + d]);
+      for (int j = 0; j < RPT; ++j) s[j] = (A)0;
+      for (int d0 = 0; d0 < a.D; d0 += 64) {
+        __syncthreads();
+        for (int e = tid; e < KT * 64; e += 256) {
+          const int kt = kb + e / 64, d = d0 + e % 64;
+          A x = (A)0;
+          if (kt < total && d < a.D) {
+            const int id = a.table[b * a.table_ld + (kt >> a.page_log2)];
+            if (id >= 0 && id < a.pages) x = S::load(kh[id * a.kb + (kt & ((1 << a.page_log2) - 1)) * a.kt + d]);
+          }
+          ks[e / 64 * CS + e % 64] = x;
         }
-        ks[e / 64 * CS + e % 64] = x;
-      }
-      for (int e = tid; e < RT * 64; e += 256) {
-        const int row = row0 + e / 64, d = d0 + e % 64, qi = row / a.G;
-        qs[e] = row < nrows && d < a.D ? S::load(qb[qi * a.qt + (int64_t)(row - qi * a.G) * a.qh + d]) : (A)0;
-      }
-      __syncthreads();
-      for (int d = 0; d < 64; ++d) {
-        const A k = ks[key * CS + d];
+        for (int e = tid; e < RT * 64; e += 256) {
+          const int row = row0 + e / 64, d = d0 + e % 64, qi = row / a.G;
+          qs[e] = row < nrows && d < a.D ? S::load(qb[qi * a.qt + (int64_t)(row - qi * a.G) * a.qh + d]) : (A)0;
+        }
+        __syncthreads();
+        for (int d = 0; d < 64; ++d) {
+          const A k = ks[key * CS + d];
 #pragma unroll
-        for (int j = 0; j < RPT; ++j) s[j] += k * qs[(sub + 4 * j) * 64 + d];
+          for (int j = 0; j < RPT; ++j) s[j] += k * qs[(sub + 4 * j) * 64 + d];
+        }
       }
-    }
-    A sum = (A)0;
+      A sum = (A)0;
 #pragma unroll
-    for (int j = 0; j < RPT; ++j) {
-      const int row = row0 + sub + 4 * j;
-      if (row >= from && row < nrows) sum += S::exp(s[j] * us - lse[row]);
+      for (int j = 0; j < RPT; ++j) {
+        const int row = row0 + sub + 4 * j;
+        if (row >= from && row < nrows) sum += S::exp(s[j] * us - lse[row]);
+      }
+      add_rounded(acc, rest, sum);
     }
-    add_rounded(acc, rest, sum);
-  }
-  part[sub * KT + key] = acc - rest;
-  __syncthreads();
-  if (sub == 0 && t < total) {
-    float* const o = w.out + b * w.wb + (int64_t)kvh * w.wh + t;
-    *o = (float)((A)*o + ((part[key] + part[KT + key]) + (part[2 * KT + key] + part[3 * KT + key])));
+    part[sub * KT + key] = acc - rest;
+    __syncthreads();
+    if (sub == 0 && t < total) {
+      float* const o = w.out + b * w.wb + (int64_t)kvh * w.wh + t;
+      *o = (float)((A)*o + ((part[key] + part[KT + key]) + (part[2 * KT + key] + part[3 * KT + key])));
+    }
+    __syncthreads();
   }
 }
 
@@ -111,28 +113,31 @@ __global__ __launch_bounds__(256) void paged_scores_kernel(const SeqArgs a, cons
   const int64_t b = bh / a.Hkv;
   const int kvh = (int)(bh - b * a.Hkv);
   const PagedRow pr = paged_row(a, b, __builtin_amdgcn_readfirstlane(a.lens[b]));
-  const int t = 4 * (blk * 256 + (int)threadIdx.x), total = pr.own + pr.count, nrows = pr.count * a.G;
-  if (t >= total || nrows == 0) return;
-  const int64_t row = bh * (a.N * a.G);
-  const float* const lse = static_cast<const float*>(a.lse) + row;
-  const float* const s = a.scores + row * a.scores_ld + t;
-  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  const int total = pr.own + pr.count, nrows = pr.count * a.G;
+  if (nrows == 0) return;
+  for (int64_t t64 = 4 * (blk * (int64_t)256 + threadIdx.x); t64 < total; t64 += (int64_t)1024 * w.blocks) {
+    const int t = (int)t64;
+    const int64_t row = bh * (a.N * a.G);
+    const float* const lse = static_cast<const float*>(a.lse) + row;
+    const float* const s = a.scores + row * a.scores_ld + t;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int r = 0; r < nrows; ++r) {
-    // a position that the row's tile was not run over lies behind what the row sees
-    const int seen = pr.own + r / a.G;
-    if (t > seen) continue;
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(s + r * a.scores_ld);
+    for (int r = 0; r < nrows; ++r) {
+      // a position that the row's tile was not run over lies behind what the row sees
+      const int seen = pr.own + r / a.G;
+      if (t > seen) continue;
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(s + r * a.scores_ld);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, -lse[r]));
-      sum[e] += t + e <= seen ? p : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale_log2, -lse[r]));
+        sum[e] += t + e <= seen ? p : 0.f;
+      }
     }
-  }
-  float* const o = w.out + b * w.wb + (int64_t)kvh * w.wh + t;
+    float* const o = w.out + b * w.wb + (int64_t)kvh * w.wh + t;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (t + e < total) o[e] += sum[e];
+    for (int e = 0; e < 4; ++e)
+      if (t + e < total) o[e] += sum[e];
+  }
 }
 
 namespace {
@@ -222,27 +227,32 @@ int64_t stage_ns(int D, int dtype, int rows_per_wg) {
   return (D <= 32 ? 450 : D == 64 ? 700 : D == 128 ? 1000 : 2000) * (rows_per_wg / 32);
 }
 
-// The number of splits of a row of `longest` keys that ends first: so many rounds of `fill`
-// workgroups at once of its share of the keys each, and from two splits on the join, a launch
-// of its own (8 us beside what the partial results take to write and read).  us measured, keys,
+// The number of splits of a row of `longest` keys that ends first: a round, or so many and a
+// quarter, of `fill` workgroups at once of its share of the keys each, and from two splits
+// on the join, a launch of its own (8 us beside what the partial results take to write and read).  us measured, keys,
 // heads on key heads, rows a workgroup, by splits 1 / 2 / 4 / 8:
 //   1 x 512 tokens, 7000, 16 / 4 of 128, 64      123 / 78 / 64 / 73
 //   4 x 100, 8000, 8 / 8 of 128, 32             53.7 / 37 / 45 / 54
 //   8 x 200, 4000, 8 / 8 of 64, 32              36.3 / 43 / 51 / 51
 //   6 x 237, 5580, 2 / 2 of 16, 32              21.7 / 18 / 16 / 19
 //   5 x 25, 13386, fp32, 24 / 6 of 80, 64       909 / 464 / 246 / 198
-int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t fill, int D, int64_t ns) {
+int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t fill, int D, int64_t ns, bool few) {
   const int64_t whole = longest * ns / 128;
+  auto percent = [&](int64_t n) { return n <= fill ? 100 : 100 * n / fill + 25; };
   int best = 1;
-  int64_t least = (wg + fill - 1) / fill * whole;
+  int64_t least = percent(wg) * whole / 100;
   const int64_t most = std::min<int64_t>(longest / 256, kMaxSplits);
   for (int k = 2; k <= most && wg * k <= 4 * fill; ++k) {
-    const int64_t cost = (wg * k + fill - 1) / fill * whole / k + 8000 + rows * k * D * 8 / 3000;
+    const int64_t cost = percent(wg * k) * whole / (100 * k) + 8000 + rows * k * D * 8 / 3000;
     if (cost < least) {
       least = cost;
       best = k;
     }
   }
+  // rows of the batch are rarely all as long as the longest: where they have one tile of rows a
+  // key head (few) and do not fill the chip, many keys are split all the same, the longest first (48 x 1 token behind 100 -
+  // 4096, 16 / 4 of 128: 70 us unsplit, 62.7 in two)
+  if (few && wg < fill && longest >= 2048) best = std::max(best, (int)std::min<int64_t>(2 * wg > fill ? 2 : fill / wg, most));
   return best;
 }
 
@@ -262,7 +272,7 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
                                            : Dm == 256 ? 512 : Dm == 128 ? 768 : 1024;
   const int64_t wg = std::max<int64_t>(1, B * Hkv * t.nrb);
   const int64_t ns = vec ? 1200 + Dm * R * 3 : mfma ? stage_ns(Dm, dtype, rows_per_wg) : 0;
-  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, fill, Dm, ns)
+  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, fill, Dm, ns, R <= 32)
                   : (int)std::max<int64_t>(1, std::min<int64_t>({(fill + wg - 1) / wg, longest / 256, kMaxSplits}));
   t.chunk = 256;
   // every XCD has work: the row blocks of few (b, key head, split) go to several, in groups
@@ -411,7 +421,7 @@ extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* wor
   PagedWeights w{weights, args->w_b, args->w_h, 0};
   const bool scored = t.scores_ld > 0, wmfma = mfma && (dtype != DG_F32 || a.D <= 128);
   const int wkeys = scored ? 1024 : wmfma ? kWeightKeys : 64;
-  w.blocks = (int)((cap + wkeys - 1) / wkeys);
+  w.blocks = (int)((args->longest + wkeys - 1) / wkeys);
   const int64_t wblocks = weights == nullptr ? 0 : wmfma && !scored ? ((int64_t)B * Hkv + 7) / 8 * 8 * w.blocks : (int64_t)B * Hkv * w.blocks;
   DG_REQUIRE(blocks <= kMostWorkgroups256 && groups <= kMostWorkgroups256 && wblocks <= kMostWorkgroups256, DG_EINVAL,
              "paged_attention: more than 2^24 - 1 workgroups");

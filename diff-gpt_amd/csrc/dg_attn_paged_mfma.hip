@@ -34,108 +34,111 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const SeqArgs a, con
   if (b >= a.B) return;  // the grid is rounded up
   const PagedRow pr = paged_row(a, b, __builtin_amdgcn_readfirstlane(a.lens[b]));
   const int total = pr.own + pr.count, nrows = pr.count * a.G;
-  const int kb = blk * kWeightKeys;
-  if (kb >= total || nrows == 0) return;  // whole workgroups, before any barrier
+  if (nrows == 0) return;  // whole workgroups, before any barrier
   const int lane = threadIdx.x & 63, hh = lane >> 5, r32 = lane & 31;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = kb + 32 * wv + r32;  // this lane's position
+  for (int64_t k0 = (int64_t)blk * kWeightKeys; k0 < total; k0 += (int64_t)w.blocks * kWeightKeys) {
+    const int kb = (int)k0;
+    const int t = kb + 32 * wv + r32;  // this lane's position
 
-  // rows are (token, head of the group) pairs; position t is seen from row `from` on
-  const int64_t from64 = (int64_t)(t - pr.own) * a.G;
-  const int from = t >= total ? nrows : (int)max(from64, (int64_t)0);
-  // the first tile that any position of the workgroup is seen from
-  const int first = max(kb - pr.own, 0) * a.G / 32 * 32;
+    // rows are (token, head of the group) pairs; position t is seen from row `from` on
+    const int64_t from64 = (int64_t)(t - pr.own) * a.G;
+    const int from = t >= total ? nrows : (int)max(from64, (int64_t)0);
+    // the first tile that any position of the workgroup is seen from
+    const int first = max(kb - pr.own, 0) * a.G / 32 * 32;
 
-  const T* const qb = static_cast<const T*>(a.q) + b * a.qb + (int64_t)kvh * a.G * a.qh;
-  const float* const lse = static_cast<const float*>(a.lse) + (b * a.Hkv + kvh) * (int64_t)(a.N * a.G);
-  auto copy_rows = [&](int st, int row0) __attribute__((always_inline)) {
+    const T* const qb = static_cast<const T*>(a.q) + b * a.qb + (int64_t)kvh * a.G * a.qh;
+    const float* const lse = static_cast<const float*>(a.lse) + (b * a.Hkv + kvh) * (int64_t)(a.N * a.G);
+    auto copy_rows = [&](int st, int row0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < (NDMA + 3) / 4; ++n) {
-      const int i = 4 * n + wv;
-      if (NDMA % 4 != 0 && i >= NDMA) break;  // wave-uniform
-      const int r = i * RPD + lane / PPR, row = row0 + r;
-      const int e = ((lane % PPR) ^ seq_swz<PPR, ES>(r)) * (16 / ES);
-      const int qi = row / a.G;
-      const bool in = row < nrows && e < a.D;
-      const void* p = in ? static_cast<const void*>(qb + qi * a.qt + (int64_t)(row - qi * a.G) * a.qh + e) : &kZeros16;
-      lds_copy16(p, qs[st] + i * RPD * D);
-    }
-    if (threadIdx.x < 32) {
-      const int row = row0 + (int)threadIdx.x;
-      ls[st][threadIdx.x] = row < nrows ? lse[row] : __builtin_huge_valf();
-    }
-  };
+      for (int n = 0; n < (NDMA + 3) / 4; ++n) {
+        const int i = 4 * n + wv;
+        if (NDMA % 4 != 0 && i >= NDMA) break;  // wave-uniform
+        const int r = i * RPD + lane / PPR, row = row0 + r;
+        const int e = ((lane % PPR) ^ seq_swz<PPR, ES>(r)) * (16 / ES);
+        const int qi = row / a.G;
+        const bool in = row < nrows && e < a.D;
+        const void* p = in ? static_cast<const void*>(qb + qi * a.qt + (int64_t)(row - qi * a.G) * a.qh + e) : &kZeros16;
+        lds_copy16(p, qs[st] + i * RPD * D);
+      }
+      if (threadIdx.x < 32) {
+        const int row = row0 + (int)threadIdx.x;
+        ls[st][threadIdx.x] = row < nrows ? lse[row] : __builtin_huge_valf();
+      }
+    };
 
-  copy_rows(0, first);
-  vec8 kf[F32 ? C::QC : C::NC];
-  int id = -1;
-  if (t < total) id = a.table[b * a.table_ld + (t >> a.page_log2)];
-  const bool there = id >= 0 && id < a.pages;
-  const T* const kp = static_cast<const T*>(a.k) + (there ? id : 0) * a.kb + (int64_t)kvh * a.kh +
-                      (t & ((1 << a.page_log2) - 1)) * a.kt;
-  if constexpr (F32) {
-#pragma unroll
-    for (int m = 0; m < C::QC / 4; ++m) {
-      const int d = C::QC * hh + 4 * m;
-      f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-      if (there && d < a.D) x = *reinterpret_cast<const f32x4_t*>(kp + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) kf[4 * m + e] = x[e];
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < C::NC; ++c) {
-      const int d = 16 * c + 8 * hh;
-      u32x4_t x = {0u, 0u, 0u, 0u};
-      if (there && d < a.D) x = *reinterpret_cast<const u32x4_t*>(kp + d);
-      kf[c] = __builtin_bit_cast(vec8, x);
-    }
-  }
-
-  const int kswz = seq_swz<PPR, ES>(r32);
-  float acc = 0.f, accc = 0.f;
-  int st = 0;
-  for (int row0 = first; row0 < nrows; row0 += 32, st ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();  // stage st filled; every wave is done with the other
-    if (row0 + 32 < nrows) copy_rows(st ^ 1, row0 + 32);
-    const T* const Q = qs[st];
-    floatx16_t s;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    copy_rows(0, first);
+    vec8 kf[F32 ? C::QC : C::NC];
+    int id = -1;
+    if (t < total) id = a.table[b * a.table_ld + (t >> a.page_log2)];
+    const bool there = id >= 0 && id < a.pages;
+    const T* const kp = static_cast<const T*>(a.k) + (there ? id : 0) * a.kb + (int64_t)kvh * a.kh +
+                        (t & ((1 << a.page_log2) - 1)) * a.kt;
     if constexpr (F32) {
 #pragma unroll
-      for (int p = 0; p < C::QC / 4; ++p) {
-        const f32x4_t qf = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(Q) + r32 * D + 4 * (((PPR / 2) * hh + p) ^ kswz));
+      for (int m = 0; m < C::QC / 4; ++m) {
+        const int d = C::QC * hh + 4 * m;
+        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+        if (there && d < a.D) x = *reinterpret_cast<const f32x4_t*>(kp + d);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(qf[e], kf[4 * p + e], s, 0, 0, 0);
+        for (int e = 0; e < 4; ++e) kf[4 * m + e] = x[e];
       }
     } else {
 #pragma unroll
       for (int c = 0; c < C::NC; ++c) {
-        const u32x4_t qf = *reinterpret_cast<const u32x4_t*>(Q + r32 * D + 8 * ((2 * c + hh) ^ kswz));
-        s = M::mma(__builtin_bit_cast(vec8, qf), kf[c], s);
+        const int d = 16 * c + 8 * hh;
+        u32x4_t x = {0u, 0u, 0u, 0u};
+        if (there && d < a.D) x = *reinterpret_cast<const u32x4_t*>(kp + d);
+        kf[c] = __builtin_bit_cast(vec8, x);
       }
     }
-    // lane l, register r: row 8 (r / 4) + 4 hh + r % 4 of the tile
-    const int lo = from - row0 - 4 * hh, hi = nrows - row0 - 4 * hh;
-    float sum = 0.f;
+
+    const int kswz = seq_swz<PPR, ES>(r32);
+    float acc = 0.f, accc = 0.f;
+    int st = 0;
+    for (int row0 = first; row0 < nrows; row0 += 32, st ^= 1) {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();  // stage st filled; every wave is done with the other
+      if (row0 + 32 < nrows) copy_rows(st ^ 1, row0 + 32);
+      const T* const Q = qs[st];
+      floatx16_t s;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4_t l4 = *reinterpret_cast<const f32x4_t*>(&ls[st][8 * g + 4 * hh]);
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+      if constexpr (F32) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 8 * g + e;
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], a.scale_log2, -l4[e]));
-        sum += r >= lo && r < hi ? p : 0.f;
+        for (int p = 0; p < C::QC / 4; ++p) {
+          const f32x4_t qf = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(Q) + r32 * D + 4 * (((PPR / 2) * hh + p) ^ kswz));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(qf[e], kf[4 * p + e], s, 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < C::NC; ++c) {
+          const u32x4_t qf = *reinterpret_cast<const u32x4_t*>(Q + r32 * D + 8 * ((2 * c + hh) ^ kswz));
+          s = M::mma(__builtin_bit_cast(vec8, qf), kf[c], s);
+        }
       }
+      // lane l, register r: row 8 (r / 4) + 4 hh + r % 4 of the tile
+      const int lo = from - row0 - 4 * hh, hi = nrows - row0 - 4 * hh;
+      float sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t l4 = *reinterpret_cast<const f32x4_t*>(&ls[st][8 * g + 4 * hh]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 8 * g + e;
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], a.scale_log2, -l4[e]));
+          sum += r >= lo && r < hi ? p : 0.f;
+        }
+      }
+      add_rounded(acc, accc, sum);
     }
-    add_rounded(acc, accc, sum);
-  }
-  acc = half_pair_sum(acc - accc);
-  if (hh == 0 && t < total) {
-    float* const o = w.out + b * w.wb + (int64_t)kvh * w.wh + t;
-    *o += acc;
+    acc = half_pair_sum(acc - accc);
+    if (hh == 0 && t < total) {
+      float* const o = w.out + b * w.wb + (int64_t)kvh * w.wh + t;
+      *o += acc;
+    }
+    __syncthreads();  // every wave is done with the rows before the next block's come
   }
 }
 

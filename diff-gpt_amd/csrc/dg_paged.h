@@ -30,7 +30,7 @@ int launch_paged_vec(const SeqArgs& a, unsigned blocks, hipStream_t s);
 struct PagedWeights {
   float* out;
   int64_t wb, wh;
-  int blocks;  // key blocks of a (b, key head)
+  int blocks;  // workgroups of a (b, key head), which take key blocks in turn
 };
 constexpr int kWeightKeys = 128;  // positions of a workgroup
 int launch_paged_weights_mfma(const SeqArgs& a, const PagedWeights& w, int dtype, unsigned blocks, hipStream_t s);

@@ -1080,8 +1080,11 @@ def paged_attention_(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     w, wb, wh = 0, 0, 0
     if weights is not None:
         wb, wh = _weights_strides(what, weights, B, Hkv, cap, device)
-        if (B > 1 and abs(wb) < cap) or (Hkv > 1 and abs(wh) < cap):
-            raise ValueError(f"{what}: the rows' weights overlap")
+        apart = cap  # what a stride must be past at least for no two rows to share an element
+        for stride, n in sorted(((wb, B), (wh, Hkv))):
+            if n > 1 and stride < apart:
+                raise ValueError(f"{what}: the rows' weights overlap")
+            apart = stride * n if n > 1 else apart
         w = weights.data_ptr()
     longest = cap if longest is None else max(1, min(operator.index(longest), cap))
     qb, qt, qh, qd = q.stride()

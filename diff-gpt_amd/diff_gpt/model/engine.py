@@ -339,7 +339,7 @@ class Engine:
         if draft is not None:
             left = [min(n, max(0, draft.block_size * 2 - len(p))) for n, p in zip(left, prompts)]
         B, results, logprobs = len(prompts), [list(p) for p in prompts], [[] for _ in prompts]
-        if max(left) == 0:
+        if max(left) <= 0:
             return results, logprobs
         ahead = num_drafts if draft is not None else 0
         # every row's last token is pending: run with the drafts behind it

@@ -2,7 +2,8 @@
 
 Beyond the reference, whose cache has one length for all rows.  The operators below work on
 one layer's (P, S, Hkv, D) views of the pool's pages, S a power of two, and a (B, M) int32
-table of page ids: position t of row b lies in page table[b, t // S].
+table of page ids: position t of row b lies in page table[b, t // S].  Rows may share pages that
+they only read; what is written (append_paged, the pages that evict_paged fills) is one row's.
 """
 
 import math
@@ -178,7 +179,7 @@ class PagedKVCache:
         self._sync()
         if self.weights is not None:  # later positions start from nothing
             t = torch.arange(self.weights.size(3), dtype=torch.int32, device=self.table.device)
-            self.weights.mul_((t < self.lengths[:, None])[None, :, None])
+            self.weights.masked_fill_((t >= self.lengths[:, None])[None, :, None], 0.0)
 
     def release(self, rows: list[int]) -> None:
         """The rows' pages go back to the pool; each of them is empty, at position 0."""

@@ -671,6 +671,7 @@ DG_API int dg_token_logprobs(int64_t M, int64_t V, int dtype, const void* x, int
  * lens[b] cached positions, and a call's tokens 0 .. counts[b] - 1 (NULL: all N) are the
  * positions behind them.  Lengths are read on the device and taken as 0 .. width * page,
  * counts as 0 .. N and as what the table still covers: tokens further on count as not there.
+ * Rows may share pages that are only read; the places that one call writes are each one row's.
  * A page id that the pool does not have is never followed: its positions read as zeros and
  * are not written.
  *

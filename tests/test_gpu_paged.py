@@ -439,3 +439,61 @@ def test_chunks_give_what_one_prompt_gives(dev):
         assert torch.allclose(y, outs[0][0], rtol=0, atol=1e-5)
         assert torch.allclose(w, outs[0][1], rtol=1e-5, atol=1e-5)
     assert math.isclose(float(outs[0][1].sum()), T * H, rel_tol=1e-5)
+
+
+@pytest.mark.parametrize("dtype,D,N", [("bf16", 64, 1), ("bf16", 64, 20), ("f32", 256, 2), ("f32", 128, 12), ("bf16", 65, 3)])
+def test_weights_past_the_hint(dev, dtype, D, N):
+    """Every form of the weights goes over all of a row's positions, whatever the hint says."""
+    _check(dev, dtype, [2500, 10, 700], [N, N, N], N, 2, 2, D, 16, longest=20)
+
+
+def test_rows_of_weights_must_not_overlap(dev):
+    from diff_gpt.model.paged import attention_paged
+
+    pool = Pool(dev, "f32", [5, 9], [1, 1], 2, 16, 16)
+    q = _queries(dev, "f32", 2, 1, 2, 16, 0)
+    cap = pool.table.size(1) * 16
+    flat = torch.zeros(8 * cap, device=dev)
+    for strides in ((cap, cap, 1), (cap - 1, 4 * cap, 1), (0, cap, 1), (2 * cap, 0, 1), (3 * cap, 2 * cap, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            attention_paged(q, pool.k, pool.v, pool.table, pool.lengths, weights=flat.as_strided((2, 2, cap), strides))
+    for strides in ((2 * cap, cap, 1), (cap, 2 * cap, 1)):
+        w = flat.zero_().as_strided((2, 2, cap), strides)
+        attention_paged(q, pool.k, pool.v, pool.table, pool.lengths, weights=w)
+        assert torch.allclose(w.sum(-1), torch.ones(2, 2, device=dev), atol=1e-6)
+
+
+def test_refusals_of_the_python_entry_points(dev):
+    from diff_gpt.model.paged import append_paged, attention_paged, evict_paged
+
+    pool = Pool(dev, "f32", [5, 9], [1, 1], 2, 16, 16)
+    q, k, v, t, n = _queries(dev, "f32", 2, 1, 4, 16, 0), pool.k, pool.v, pool.table, pool.lengths
+    new = torch.zeros(2, 1, 2, 16, device=dev)
+    freqs = torch.ones(20, 8, 2, device=dev)
+    w = torch.zeros(2, 2, t.size(1) * 16, device=dev)
+    to = torch.tensor([[pool.free[0]], [pool.free[1]]], dtype=torch.int32, device=dev)
+    attend = lambda **kw: attention_paged(**{**dict(q=q, k_pages=k, v_pages=v, table=t, lengths=n), **kw})  # noqa: E731
+    append = lambda **kw: append_paged(**{**dict(q=q, k=new, v=new, freqs=freqs, k_pages=k, v_pages=v, table=t, lengths=n), **kw})  # noqa: E731
+    evict = lambda **kw: evict_paged(**{**dict(k_pages=k, v_pages=v, table=t, lengths=n, weights=w, keep=4, recent=2, to=to), **kw})  # noqa: E731
+    attend(), append(), evict()
+    bad_pages = torch.zeros(3, 12, 2, 16, device=dev)
+    for call, kw in [(attend, dict(q=q[0])), (attend, dict(q=q[:, :, :3])), (attend, dict(q=q[..., :8])), (attend, dict(v_pages=v[:1])),
+                     (attend, dict(k_pages=bad_pages, v_pages=bad_pages)), (attend, dict(table=t.long())), (attend, dict(table=t[:1])),
+                     (attend, dict(table=t[:, :0])), (attend, dict(table=t.t().contiguous().t())), (attend, dict(lengths=n.long())),
+                     (attend, dict(lengths=n[:1])), (attend, dict(lengths=n.cpu())), (attend, dict(counts=n.cpu())),
+                     (attend, dict(weights=w[..., :3])), (attend, dict(weights=w.double())), (attend, dict(weights=w[:1])),
+                     (attend, dict(scale=0.0)), (attend, dict(scale=float("inf"))), (attend, dict(q=q.expand(2, 1, 4, 16)[..., ::2])),
+                     (append, dict(q=q[..., :8])), (append, dict(k=new[:, :, :1])), (append, dict(v=new[:1])),
+                     (append, dict(freqs=freqs[:, :4])), (append, dict(freqs=freqs[:0])), (append, dict(freqs=freqs.cpu())),
+                     (append, dict(positions=n.long())), (append, dict(table=t.cpu())),
+                     (append, dict(q=torch.zeros(2, 1, 4, 16, 2, device=dev)[..., 0])),
+                     (evict, dict(keep=0, recent=0)), (evict, dict(recent=5)), (evict, dict(keep=17)), (evict, dict(to=to.long())),
+                     (evict, dict(to=to[:1])), (evict, dict(weights=w[:, :1])), (evict, dict(to=to.cpu()))]:
+        with pytest.raises(ValueError):
+            call(**kw)
+    for call, kw in [(attend, dict(q=q.bfloat16())), (attend, dict(v_pages=v.half())), (append, dict(freqs=freqs.half())),
+                     (append, dict(v=new.double())), (attend, dict(q=q.int(), k_pages=k.int(), v_pages=v.int())), (evict, dict(keep=2.5))]:
+        with pytest.raises(TypeError):
+            call(**kw)
+    with pytest.raises(RuntimeError, match="inference"):
+        attend(q=q.clone().requires_grad_())

@@ -190,3 +190,21 @@ def test_captured_calls_replay(dev, V):
         _check(r, _exact(target, tokens, uniforms, noise, draft, [3] * 4, 1.0))
         eager = verify_drafts(target, tokens, uniforms, noise, draft=draft)
         assert all(torch.equal(a, b) for a, b in zip(r, eager))
+
+
+def test_refusals_of_the_python_entry_point(dev):
+    from diff_gpt.sampler.drafts import verify_drafts
+
+    target, draft, tokens, uniforms, noise = _inputs(dev, "f32", 3, 2, 40, 0)
+    ok = dict(target=target, tokens=tokens, uniforms=uniforms, noise=noise, draft=draft)
+    verify_drafts(**ok)
+    for kw in [dict(target=target[0]), dict(target=target[:, :0]), dict(target=target[:, :2]), dict(target=target[..., ::2]),
+               dict(tokens=tokens.int()), dict(tokens=tokens[:, :1]), dict(tokens=tokens.t().contiguous().t()), dict(uniforms=None),
+               dict(uniforms=uniforms.double()), dict(noise=None), dict(noise=noise[:, :30]), dict(noise=noise.half()),
+               dict(noise=noise.cpu()), dict(draft=draft[:, :1]), dict(draft=draft.cpu()), dict(counts=torch.tensor([1, 1, 1])),
+               dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-40),
+               dict(target=torch.zeros(1, 66, 4, device=dev), tokens=torch.zeros(1, 65, dtype=torch.long, device=dev), draft=None)]:
+        with pytest.raises((ValueError, RuntimeError)):
+            verify_drafts(**{**ok, **kw})
+    with pytest.raises(TypeError):
+        verify_drafts(**{**ok, "draft": draft.half()})
