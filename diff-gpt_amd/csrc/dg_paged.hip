@@ -7,7 +7,9 @@
 // one length, dg_rope.hip, rounds r to the data's type first, as the reference does; once is
 // nearer to the exact value, bf16 1.7e-3 of it, and no dearer.)  LPR lanes share a head, 16 bytes
 // each; they take HPT heads of a token, whose loads are in flight together and whose angles
-// are read once.  Bound by HBM where tokens are many, by the launch where they are few.
+// are read once.  Bound by HBM where tokens are many (24 x 700 tokens, 24 heads of 128, bf16:
+// 30.5 us, 172 MB; 40.5 with 64-bit products for every head's address, the angles unpacked for
+// each and a correctly rounded root), by the launch where they are few.
 //
 // paged_select_kernel.  The m-th largest weight of a row by its bits: three passes of 11, 11
 // and 10 over an order-preserving integer, counted in LDS, then one that ranks what is above
@@ -24,9 +26,10 @@ namespace dg {
 
 struct AppendArgs {
   const void* src[3];  // q, k, v
-  int64_t sb[3], st[3], sh[3];
+  int64_t sb[3], st[3];
   void* dst[3];  // q_out, the pages' k and v
-  int64_t db[3], dt[3], dh[3];
+  int64_t db[3], dt[3];
+  int sh[3], dh[3];  // from head to head, bytes
   const void* freqs;
   int64_t freqs_ld, freqs_rows;
   const int32_t* table;
@@ -110,11 +113,32 @@ struct AppendAcc<double> {
   }
 };
 
+// 1 / sqrt(x), x > 0
+__device__ __forceinline__ double inv_sqrt(double x) { return 1.0 / sqrt(x); }
+__device__ __forceinline__ float inv_sqrt(float x) {
+  // the hardware's, off by a step at most, and Newton's step behind it (a correctly rounded root
+  // and quotient are forty instructions of every head)
+  const float y = __builtin_amdgcn_rsqf(x);
+  return y == 0.f ? y : __builtin_fmaf(__builtin_fmaf(-x * y, y, 1.0f), 0.5f * y, y);  // 0 for infinity
+}
+
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float x) {
+  return group_sum_dpp<LPR>(x);
+}
+template <int LPR>
+__device__ __forceinline__ double lanes_sum(double x) {
+#pragma unroll
+  for (int off = 1; off < LPR; off <<= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
 // EPL consecutive dims a lane and piece, LPR lanes a head, NCK pieces, HPT heads of a token.
 template <typename T, typename FT, int EPL, int LPR, int NCK, int HPT, bool VEC>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
   using S = AppendAcc<T>;
   using A = typename S::type;
+  constexpr int W = EPL * (int)sizeof(T) / 4, FW = EPL * (int)sizeof(FT) / 4;
   const int sub = threadIdx.x % LPR;
   const uint32_t item = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;  // below 2^31
   if (item >= a.items) return;  // whole lane groups; no barriers follow
@@ -127,28 +151,36 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
 
   // The token's heads, which no length decides where to read.  Where tokens are many, those
   // that are not there are not read all the same (24 x 700 tokens, three quarters of them there,
-  // 24 heads of 128: 44.8 us read, 41.6 not).
+  // 24 heads of 128: 44.8 us read, 41.6 not, before the rest was as it is).
   bool read = true;
   if constexpr (HPT > 1) {
     if (a.counts != nullptr) read = n < a.counts[b];
   }
-  constexpr int W = EPL * (int)sizeof(T) / 4, FW = EPL * (int)sizeof(FT) / 4;
+  // head h's first element, of three tensors one after the other
+  auto at = [&](const char* q, const char* k, const char* v, const int (&step)[3], int h) __attribute__((always_inline)) {
+    const bool is_q = h < a.H, is_k = h < a.H + a.Hkv;
+    const char* base = is_q ? q : is_k ? k : v;
+    const int hw = is_q ? h : is_k ? h - a.H : h - a.H - a.Hkv;
+    const int by = is_q ? step[0] : is_k ? step[1] : step[2];
+    return base + (int64_t)hw * by;
+  };
+  const char *xq, *xk, *xv;
+  {
+    const int64_t es = (int64_t)sizeof(T);
+    xq = static_cast<const char*>(a.src[0]) + (b * a.sb[0] + n * a.st[0]) * es;
+    xk = static_cast<const char*>(a.src[1]) + (b * a.sb[1] + n * a.st[1]) * es;
+    xv = static_cast<const char*>(a.src[2]) + (b * a.sb[2] + n * a.st[2]) * es;
+  }
   uint32_t x[HPT][NCK][W];
 #pragma unroll
   for (int j = 0; j < HPT; ++j) {
-    const int h = min(h0 + a.groups * j, heads - 1);
-    const int w = h < a.H ? 0 : h < a.H + a.Hkv ? 1 : 2;
-    const int hw = w == 0 ? h : w == 1 ? h - a.H : h - a.H - a.Hkv;
-    const T* p = static_cast<const T*>(a.src[w]) + b * a.sb[w] + n * a.st[w] + hw * a.sh[w];
+    const T* p = reinterpret_cast<const T*>(at(xq, xk, xv, a.sh, min(h0 + a.groups * j, heads - 1)));
 #pragma unroll
     for (int c = 0; c < NCK; ++c) {
       const int d = EPL * (sub + LPR * c);
-      if (d < a.D && read) {
-        load_some<T, EPL, VEC>(p + d, x[j][c], a.D - d);
-      } else {
 #pragma unroll
-        for (int e = 0; e < W; ++e) x[j][c][e] = 0u;
-      }
+      for (int e = 0; e < W; ++e) x[j][c][e] = 0u;
+      if (d < a.D && read) load_some<T, EPL, VEC>(p + d, x[j][c], a.D - d);
     }
   }
   const int len = a.lens[b];
@@ -162,53 +194,56 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
   if (there) id = a.table[b * a.table_ld + (slot >> a.page_log2)];
   const bool held = id >= 0 && id < a.pages;
   const int in_page = slot & ((1 << a.page_log2) - 1);
-  uint32_t cs[NCK][FW];
+  A co[NCK][EPL / 2], si[NCK][EPL / 2];
 #pragma unroll
   for (int c = 0; c < NCK; ++c) {
     const int d = EPL * (sub + LPR * c);
-    if (d < a.D) {
-      load_some<FT, EPL, VEC>(static_cast<const FT*>(a.freqs) + (known ? pos : 0) * a.freqs_ld + d, cs[c], a.D - d);
-    } else {
+    uint32_t cs[FW];
 #pragma unroll
-      for (int e = 0; e < FW; ++e) cs[c][e] = 0u;
+    for (int e = 0; e < FW; ++e) cs[e] = 0u;
+    if (d < a.D) load_some<FT, EPL, VEC>(static_cast<const FT*>(a.freqs) + (known ? pos : 0) * a.freqs_ld + d, cs, a.D - d);
+#pragma unroll
+    for (int e = 0; e < EPL / 2; ++e) {
+      typename AppendAcc<FT>::type cx, sx;
+      AppendAcc<FT>::load(cs, e, cx, sx);
+      co[c][e] = cx;
+      si[c][e] = sx;
     }
+  }
+  const char *yq, *yk, *yv;
+  {
+    const int64_t es = (int64_t)sizeof(T), page = held ? id : 0;
+    yq = static_cast<const char*>(a.dst[0]) + (b * a.db[0] + n * a.dt[0]) * es;
+    yk = static_cast<const char*>(a.dst[1]) + (page * a.db[1] + in_page * a.dt[1]) * es;
+    yv = static_cast<const char*>(a.dst[2]) + (page * a.db[2] + in_page * a.dt[2]) * es;
   }
 
 #pragma unroll
   for (int j = 0; j < HPT; ++j) {
     const int h = h0 + a.groups * j;
     if (h >= heads) break;  // the same in all of the group's lanes
-    const int w = h < a.H ? 0 : h < a.H + a.Hkv ? 1 : 2;
-    const int hw = w == 0 ? h : w == 1 ? h - a.H : h - a.H - a.Hkv;
-    if (w < 2) {
+    if (h < a.H + a.Hkv) {
       A y[NCK][EPL], ss = (A)0;
 #pragma unroll
       for (int c = 0; c < NCK; ++c)
 #pragma unroll
         for (int e = 0; e < EPL; e += 2) {
           A re, im;
-          typename AppendAcc<FT>::type co, si;
           S::load(x[j][c], e / 2, re, im);
-          AppendAcc<FT>::load(cs[c], e / 2, co, si);
-          y[c][e] = re * co - im * si;
-          y[c][e + 1] = re * si + im * co;
+          y[c][e] = re * co[c][e / 2] - im * si[c][e / 2];
+          y[c][e + 1] = re * si[c][e / 2] + im * co[c][e / 2];
           ss += y[c][e] * y[c][e] + y[c][e + 1] * y[c][e + 1];
         }
       A f = (A)1;
-      if (a.qknorm) {
-#pragma unroll
-        for (int off = 1; off < LPR; off <<= 1) ss += __shfl_xor(ss, off, 64);
-        f = (A)1 / sqrt(ss / (A)a.D + (A)FLT_EPSILON);
-      }
+      if (a.qknorm) f = inv_sqrt(lanes_sum<LPR>(ss) * (A)(1.0 / a.D) + (A)FLT_EPSILON);
       if (!known) f = (A)__builtin_nanf("");
 #pragma unroll
       for (int c = 0; c < NCK; ++c)
 #pragma unroll
         for (int e = 0; e < EPL; e += 2) S::store(x[j][c], e / 2, there ? y[c][e] * f : (A)0, there ? y[c][e + 1] * f : (A)0);
     }
-    if (w > 0 && !held) continue;
-    T* o = static_cast<T*>(a.dst[w]) + hw * a.dh[w];
-    o += w == 0 ? b * a.db[w] + n * a.dt[w] : id * a.db[w] + in_page * a.dt[w];
+    if (h >= a.H && !held) continue;
+    T* o = reinterpret_cast<T*>(const_cast<char*>(at(yq, yk, yv, a.dh, h)));
 #pragma unroll
     for (int c = 0; c < NCK; ++c) {
       const int d = EPL * (sub + LPR * c);
@@ -483,11 +518,15 @@ extern "C" int dg_paged_append(const dg_paged_append_args* args, void* stream) {
   bool vec = D * es % 16 == 0 && aligned16(freqs) && freqs_ld * fes % 16 == 0;
   for (int w = 0; w < 3; ++w) {
     a.src[w] = src[w];
-    a.sb[w] = sst[w]->b; a.st[w] = sst[w]->t; a.sh[w] = sst[w]->h;
+    a.sb[w] = sst[w]->b; a.st[w] = sst[w]->t;
     a.dst[w] = dst[w];
-    a.db[w] = dst_st[w]->b; a.dt[w] = dst_st[w]->t; a.dh[w] = dst_st[w]->h;
+    a.db[w] = dst_st[w]->b; a.dt[w] = dst_st[w]->t;
+    const int64_t sh = sst[w]->h, dh = dst_st[w]->h, far = ((int64_t)1 << 31) / es;
+    DG_REQUIRE(sh > -far && sh < far && dh > -far && dh < far, DG_EINVAL, "paged_append: heads 2^31 bytes apart or more");
+    a.sh[w] = (int)(sh * es);
+    a.dh[w] = (int)(dh * es);
     vec = vec && aligned16(src[w]) && aligned16(dst[w]);
-    for (int64_t x : {a.sb[w], a.st[w], a.sh[w], a.db[w], a.dt[w], a.dh[w]}) vec = vec && x * es % 16 == 0;
+    for (int64_t x : {a.sb[w], a.st[w], sh, a.db[w], a.dt[w], dh}) vec = vec && x * es % 16 == 0;
   }
   a.freqs = freqs; a.freqs_ld = freqs_ld; a.freqs_rows = freqs_rows;
   a.table = rows->table; a.table_ld = rows->table_ld; a.pages = rows->pages;

@@ -265,6 +265,21 @@ def test_append(dev, dtype, H, Hkv, D, N, S, odd):
         assert torch.equal(torch.nan_to_num(now[~seen], nan=7.0), torch.nan_to_num(old[~seen], nan=7.0))
 
 
+def test_append_of_rows_whose_squares_overflow_or_vanish(dev):
+    """As the norm in fp32 has it: infinite squares leave zeros, zeros stay zeros, NaN stays NaN."""
+    from diff_gpt.model.paged import append_paged
+
+    pool = Pool(dev, "f32", [0], [5], 1, 16, 8)
+    q = torch.ones(1, 5, 1, 16, device=dev) * torch.tensor([1e20, 0.0, 1e-20, float("nan"), 3.0], device=dev)[:, None, None]
+    freqs = torch.tensor([1.0, 0.0], device=dev).expand(5, 8, 2)
+    out = append_paged(q, q, q, freqs, pool.k, pool.v, pool.table, pool.lengths)[0, :, 0]
+    assert not out[0].any() and not out[1].any() and bool(torch.isnan(out[3]).all())
+    # 1e-20 squared is lost beside eps = 2^-23
+    assert torch.allclose(out[2], q[0, 2, 0] * 2.0**11.5, rtol=1e-6)
+    assert torch.allclose(out[4], torch.ones(16, device=dev), rtol=1e-6)
+    assert torch.equal(torch.nan_to_num(pool.v[pool.pages_of[0][0], :5, 0]), torch.nan_to_num(q[0, :, 0]))
+
+
 def test_append_positions_outside_the_table_and_pages_outside_the_pool(dev):
     from diff_gpt.model.paged import append_paged
 
