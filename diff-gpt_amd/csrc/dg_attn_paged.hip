@@ -84,7 +84,9 @@ __global__ __launch_bounds__(256) void paged_weights_any_kernel(const SeqArgs a,
 // order[0 ..] = the rows of the batch by how many positions their tokens see, the most first:
 // where more workgroups than run at once take their turns, the launch then ends on short
 // ones.  Ranks by counting, at most kOrdered rows.  us as they come / so, with this launch:
-// 16 rows of 256 - 512 tokens behind 1000 - 7168, 16 heads on 4 of 128, 472 / 383.
+// 16 rows of 256 - 512 tokens behind 1000 - 7168, 16 heads on 4 of 128, 425 / 372; 48 of up to
+// 300 behind up to 3000, 8 on 2 of 64, 86 / 67; a token behind each of 48 of 100 - 4096, 16 on 4
+// of 128, 46.7 / 41.3, of 256 223 / 222; 16 alike 417 / 420.
 constexpr int kOrdered = 1024;
 
 __global__ __launch_bounds__(kOrdered) void paged_order_kernel(const SeqArgs a, int32_t* order) {
@@ -229,8 +231,8 @@ int64_t stage_ns(int D, int dtype, int rows_per_wg) {
 
 // The number of splits of a row of `longest` keys that ends first: a round, or so many and a
 // quarter, of `fill` workgroups at once of its share of the keys each, and from two splits
-// on the join, a launch of its own (8 us beside what the partial results take to write and read).  us measured, keys,
-// heads on key heads, rows a workgroup, by splits 1 / 2 / 4 / 8:
+// on the join, a launch of its own (8 us beside what the partial results take to write and
+// read).  us measured, keys, heads on key heads, rows a workgroup, by splits 1 / 2 / 4 / 8:
 //   1 x 512 tokens, 7000, 16 / 4 of 128, 64      123 / 78 / 64 / 73
 //   4 x 100, 8000, 8 / 8 of 128, 32             53.7 / 37 / 45 / 54
 //   8 x 200, 4000, 8 / 8 of 64, 32              36.3 / 43 / 51 / 51
@@ -341,6 +343,7 @@ int paged_call(const dg_paged_attention_args* args, PagedCall* c) {
   DG_REQUIRE(args->Hkv >= 1 && args->Hkv <= 0x7fffffff && args->H % args->Hkv == 0, DG_EINVAL,
              "paged_attention: %lld query heads on %lld key heads", (long long)args->H, (long long)args->Hkv);
   const int64_t R = args->N * (args->H / args->Hkv);
+  DG_REQUIRE(args->B * args->Hkv <= kMostWorkgroups256, DG_EINVAL, "paged_attention: more than 2^24 - 1 workgroups");
   DG_REQUIRE(R <= kMostPositions, DG_EINVAL, "paged_attention: a row of more than 2^30 (token, head) rows");
   const float scale = (float)args->scale;
   DG_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), DG_EINVAL, "paged_attention: the scale must be positive and below 2^127");

@@ -38,7 +38,9 @@
 // three instructions for the two terms of a probability), by HBM for few rows.  bf16: 6 sequences of up to 7168
 // tokens, 16 heads on 4 of 128, 660 us (720 TFLOP/s; vector ALU 56 % busy, matrix cores
 // 58 %); 64 of 100 - 2048, 8 heads of 64, 221 us (500 TFLOP/s; 70 %, 39 %); one token for
-// each of 64 caches of up to 4096, 16 heads on 4 of 128, 53 us (269 MB, 5.1 TB/s).
+// each of 64 caches of up to 4096, 16 heads on 4 of 128, 53 us (269 MB, 5.1 TB/s), in pages of
+// 64 positions 56; 16 chunks of 256 - 512 tokens behind 1000 - 7168, in pages of 16, 370 (640
+// TFLOP/s; 46 % and 46 %).
 // Not kept: the K fragments of a block in flight together, two chains for the row sums, 168
 // registers at head_dim 64, raised wave priority around the products (each within 2 %);
 // outputs checked for values that are not finite at the end and the piece done again (5 %
@@ -248,6 +250,8 @@ void seq_mfma_kernel(const SeqArgs a) {
   };
   // kPaged: rows of GR keys, which a page holds whole, have one resource, that of nothing for a
   // page the pool lacks.  Rows past the piece's last key are copied too: hidden from all.
+  // (us, an address for every lane / so: one token for each of 64 caches of up to 4096, 16 heads
+  // on 4 of 128, bf16, pages of 64, 68 / 56; 16 of 256 - 512 behind 1000 - 7168, pages of 16, 511 / 473.)
   constexpr int GR = paged_granule(D, ES), NC1 = (C::NDMA + RT - 1) / RT;
   uint32_t page_b = 0, key_b = 0, npages = 0;
   const char *kbase = nullptr, *vbase = nullptr;

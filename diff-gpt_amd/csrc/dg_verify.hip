@@ -11,10 +11,15 @@
 // that the decisions u q < p come out as in 64 bits but for a few in 10^7.  Then one
 // workgroup or several a row race over the logits of the one row that decides.
 //
-// Few logits (kAlone): one launch, a workgroup for each row of the batch.  Otherwise two: the
+// Few logits: one launch, a workgroup for each row of the batch.  Otherwise two: the
 // statistics of all rows, split where rows are few, and the race, whose parts meet in one
 // atomic maximum (its result depends on no order; the statistics' launch clears it) and whose
 // last part writes the row's results.
+//
+// 64 rows of 6 + 5 of 49999 bf16 logits: statistics 18 us, by HBM and vector instructions; race
+// 14 us, a chain of latencies: the rows' statistics, the logits, two atomics.  (26 each with
+// loads of single elements where rows start anywhere, the exponents' offset raised with every
+// new maximum and the parts of a row's statistics joined by one thread.)
 #include "dg_common.h"
 
 #include <algorithm>
@@ -119,7 +124,7 @@ __device__ __forceinline__ void load_any(const T* p, float (&z)[N]) {
 constexpr float kAhead = 16.f;
 
 // N further logits from id v0 on (-inf for what is not there) into a thread's statistics.  A
-// NaN makes the sum one.
+// NaN makes the sum one, beside logits of -inf alone too.
 template <int N, bool GREEDY>
 __device__ __forceinline__ void add_logits(const VerifyArgs& a, const float (&z)[N], int v0, float& top, int& at, float& part) {
   float m = z[0];
@@ -134,7 +139,12 @@ __device__ __forceinline__ void add_logits(const VerifyArgs& a, const float (&z)
     if (top != kNegInf) part *= scaled_exp(a, top - m);
     top = m;
   }
-  if (top == kNegInf) return;  // nothing yet
+  if (top == kNegInf) {  // nothing yet
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (z[i] != z[i]) part = z[i];
+    return;
+  }
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) sum += scaled_exp(a, z[i] - top);
@@ -230,7 +240,7 @@ __device__ __forceinline__ int standing(const VerifyArgs& a, int64_t b, int coun
   if (lane < count) {
     const int64_t x = a.tokens[b * a.N + lane];
     if constexpr (GREEDY) {
-      falls = x != stats[lane].at;
+      falls = x != stats[lane].at || stats[lane].sum != stats[lane].sum;
     } else {
       const double p = drafted_prob(a, stats[lane]);
       const double q = a.draft != nullptr ? drafted_prob(a, stats[a.N + 1 + lane]) : 1.0;
@@ -463,8 +473,13 @@ __global__ __launch_bounds__(512) void verify_race_kernel(const VerifyArgs a) {
 
 namespace {
 
-// Logits of a row of the batch up to which one workgroup does all of it.
-constexpr int64_t kAlone = 16384;
+// Logits that a wave of verify_alone_kernel goes through, up to which one workgroup does all of a
+// row of the batch: of few rows, and of so many that the others' launches fill the chip too.
+// us in one launch / two (8 waves, each with every eighth row of logits), rows of the batch x
+// rows of logits x V: 64 x 9 x 1000 9.0 / 9.5; 64 x 9 x 2000 10.5 / 9.9; 16 x 3 x 5400
+// 10.5 / 11.2; 16 x 3 x 11000 15.8 / 11.5; 8 x 1 x 16000 15.6 / 10.5; 256 x 9 x 2000
+// 10.2 / 12.2; 512 x 9 x 4000 18.5 / 21.3 (a second launch is 2 us of the host's as well).
+constexpr int64_t kAlone = 6144, kAloneMany = 8192, kManyRows = 256;
 
 struct VerifyShape {
   bool alone;
@@ -475,7 +490,7 @@ struct VerifyShape {
 VerifyShape verify_shape(int64_t B, int N, int64_t V) {
   VerifyShape t{};
   t.rows = 2 * N + 1;
-  t.alone = t.rows * V <= kAlone;
+  t.alone = (t.rows + 7) / 8 * V <= (B < kManyRows ? kAlone : kAloneMany);
   t.split = t.parts = 1;
   if (t.alone) return t;
   // about two workgroups a CU, of 2048 logits at least

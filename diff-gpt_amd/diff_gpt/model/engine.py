@@ -665,8 +665,10 @@ class _PagedDecoder:
         self._cut()
 
     def _cut(self) -> None:
-        if self.keep is not None and max(self.cache.lens) >= self.keep + self.cache.page_size:
-            self.cache.evict(self.keep, self.recent)
+        if self.keep is not None:  # each row by its own length, whatever the others'
+            long = [b for b, n in enumerate(self.cache.lens) if n >= self.keep + self.cache.page_size]
+            if long:
+                self.cache.evict(self.keep, self.recent, long)
 
 
 def _tries(continuations: list[list[int]]):

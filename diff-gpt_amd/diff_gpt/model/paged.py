@@ -154,6 +154,8 @@ class PagedKVCache:
     def advance(self, counts: list[int], on_device: torch.Tensor | None = None) -> None:
         """The rows' next counts[b] positions, which their pages hold by now, count as cached.
         on_device: the counts there, where the caller has them."""
+        if len(counts) != len(self.lens):
+            raise ValueError(f"PagedKVCache: {len(self.lens)} rows, counts {counts}")
         for b, n in enumerate(counts):
             if n < 0 or self.lens[b] + n > len(self._pages_of[b]) * self.page_size:
                 raise ValueError(f"PagedKVCache: row {b} cannot advance by {n}")
@@ -191,8 +193,8 @@ class PagedKVCache:
             self.next_pos[b] = 0
         self._sync()
 
-    def evict(self, keep: int, recent: int) -> list[list[torch.Tensor]]:
-        """Cut rows of more than ``keep`` positions to that many a key head, in every layer: the
+    def evict(self, keep: int, recent: int, rows: list[int] | None = None) -> list[list[torch.Tensor]]:
+        """Cut those of the rows (None: all) that have more than ``keep`` positions to that many a key head, in every layer: the
         ``recent`` last ones and those of the largest weights (evict_paged).  Positions that
         tokens stand at go on from where they were.  The kept positions of each layer are
         returned for each group of rows that was cut at once, (rows, H, keep) int32 (a group
@@ -202,7 +204,7 @@ class PagedKVCache:
         if not 1 <= keep or not 0 <= recent <= keep:
             raise ValueError(f"PagedKVCache: keep {keep} positions, {recent} of them the last ones")
         per = -(-keep // self.page_size)
-        long = [b for b, n in enumerate(self.lens) if n > keep]
+        long = [b for b, n in enumerate(self.lens) if n > keep and (rows is None or b in rows)]
         out = []
         while long:
             fit = min(len(long), len(self._free) // per)

@@ -265,6 +265,26 @@ def test_append(dev, dtype, H, Hkv, D, N, S, odd):
         assert torch.equal(torch.nan_to_num(now[~seen], nan=7.0), torch.nan_to_num(old[~seen], nan=7.0))
 
 
+@pytest.mark.parametrize("N", [1, 900])
+def test_append_of_single_heads_whose_stride_is_any(dev, N):
+    """One head is not stepped over: a stride no 32 bits hold says nothing."""
+    from diff_gpt.model.paged import append_paged
+
+    freqs = torch.randn(N, 8, 2, device=dev)
+    lengths, table = torch.zeros(5, dtype=torch.int32, device=dev), torch.arange(5 * 57, dtype=torch.int32, device=dev).view(5, 57)
+
+    def far(t):
+        s = t.stride()
+        return t.as_strided(t.shape, (s[0], s[1], 2**40, 1))
+
+    x = [torch.randn(5, N, 1, 16, device=dev) for _ in range(3)]
+    near = [torch.zeros(5 * 57, 16, 1, 16, device=dev) for _ in range(2)]
+    pages = [torch.zeros_like(t) for t in near]
+    a = append_paged(*x, freqs, *near, table, lengths)
+    b = append_paged(*map(far, x), freqs, *map(far, pages), table, lengths)
+    assert torch.equal(a, b) and torch.equal(near[0], pages[0]) and torch.equal(near[1], pages[1]) and bool(near[0].any())
+
+
 def test_append_of_rows_whose_squares_overflow_or_vanish(dev):
     """As the norm in fp32 has it: infinite squares leave zeros, zeros stay zeros, NaN stays NaN."""
     from diff_gpt.model.paged import append_paged

@@ -145,6 +145,24 @@ def test_decoding_within_a_budget(dev, draft, page_size, keep, recent, monkeypat
     assert max(n for own, n in held if own) <= keep + page_size + 256
 
 
+def test_rows_are_cut_by_their_own_length(dev, monkeypatch):
+    """A budget cuts a row that holds a page more, and leaves those beside it that do not."""
+    model = _gpt(dev)
+    cut = []
+    evict = PagedKVCache.evict
+    monkeypatch.setattr(PagedKVCache, "evict", lambda self, *a: (cut.append((list(self.lens), a)), evict(self, *a))[1])
+    Engine(model).generate_paged(_series([60, 45, 30]), 20, temperature=0, keep=40, recent=20, page_size=16)
+    assert cut and any(40 < n < 56 for lens, _ in cut for n in lens)
+    for lens, a in cut:
+        assert a == (40, 20, [b for b, n in enumerate(lens) if n >= 56])
+    cache = _cache(model, 3, weights=True)
+    model.forward_paged(_pad(_series([30, 25, 9]), dev), cache, [30, 25, 9])
+    cache.evict(20, 5, [1, 2])
+    assert cache.lens == [30, 20, 9] and cache.next_pos == [30, 25, 9]
+    with pytest.raises(ValueError, match="counts"):
+        cache.advance([1])
+
+
 def test_evicted_rows_attend_to_what_is_kept(dev):
     """In a model of one layer a position's key and value depend on its token alone, so a row cut
     to some positions is a row that those tokens alone were fed to."""

@@ -134,6 +134,29 @@ def test_hidden_tokens_and_broken_rows(dev, V, dtype):
     assert r.accepted[4:].tolist() == want[0].tolist() and r.tokens[4:].tolist() == want[1].tolist()
 
 
+@pytest.mark.parametrize("V", [100, 40000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f64"])
+@pytest.mark.parametrize("at", [0, 37, -1])
+def test_nan_among_hidden_tokens(dev, V, dtype, at):
+    """A NaN breaks its row wherever it stands, among tokens that are all hidden too, and no draft
+    of a broken row stands, at temperature 0 neither."""
+    from diff_gpt.sampler.drafts import verify_drafts
+
+    target, _, _, uniforms, noise = _inputs(dev, dtype, 2, 1, V, 4)
+    target[:, :, : V // 2] = float("-inf")
+    tokens = target[:, :1].argmax(-1)
+    lone = torch.arange(V, device=dev) != tokens[0, 0]
+    target[0, 0, lone] = float("-inf")  # the draft's token alone is left
+    for T in (1.0, 0):
+        fine = verify_drafts(target, tokens, torch.zeros_like(uniforms), noise, temperature=T)
+        assert fine.accepted.tolist() == [1, 1]
+        broken = target.clone()
+        broken[0, 0, at] = broken[1, 0, at] = float("nan")
+        r = verify_drafts(broken, tokens, torch.zeros_like(uniforms), noise, temperature=T)
+        assert r.accepted.tolist() == [0, 0]
+        assert bool(((r.tokens[:, 0] >= 0) & (r.tokens[:, 0] < V)).all())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f64"])
 @pytest.mark.parametrize("B,N,V", [(3, 4, 200), (5, 3, 33000), (2, 0, 64)])
 def test_temperature_zero(dev, dtype, B, N, V):

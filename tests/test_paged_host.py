@@ -37,6 +37,7 @@ def _append(B=1, N=1, H=1, Hkv=1, D=16, dtype=0, rows=_rows(), q=P, k=P, freqs=P
     (dict(rows=_rows(page=12)), EINVAL, b"power of two"), (dict(rows=_rows(page=0)), EINVAL, b"power of two"),
     (dict(rows=_rows(width=0)), EINVAL, b"2^30"), (dict(rows=_rows(page=1 << 20, width=1025)), EINVAL, b"2^30"),
     (dict(B=1 << 20, N=1 << 10, D=1024), EINVAL, b"workgroups"),
+    (dict(B=(1 << 31) - 1, N=(1 << 31) - 1, H=0xffff, Hkv=0xffff), EINVAL, b"workgroups"),
 ])
 def test_append_refusals(kw, code, word):
     assert _append(**kw) == code and word in _error()
@@ -75,6 +76,8 @@ def _attend(ws=None, ws_bytes=0, **kw):
     (dict(weights=P, ws=0x1004, ws_bytes=1 << 20), EINVAL, b"aligned"),
     (dict(rows=_rows(page=1 << 20, width=1 << 10), longest=1 << 30), EWORKSPACE, b"workspace"),
     (dict(B=1 << 24, Hkv=1), EINVAL, b"workgroups"),
+    (dict(B=(1 << 31) - 1, N=128, H=(1 << 31) - 1, Hkv=(1 << 31) - 1), EINVAL, b"workgroups"),
+    (dict(B=1 << 30, N=1, H=1 << 20, Hkv=1 << 20, weights=P), EINVAL, b"workgroups"),
 ])
 def test_attention_refusals(kw, code, word):
     assert _attend(**kw) == code and word in _error()
@@ -106,6 +109,7 @@ def _evict(B=1, Hkv=1, D=16, dtype=0, rows=_rows(), weights=P, keep=8, recent=2,
     (dict(weights=0), EINVAL, b"NULL"), (dict(to=0), EINVAL, b"NULL"), (dict(keep=17), EINVAL, b"into"),
     (dict(to_width=0), EINVAL, b"into"), (dict(rows=_rows(page=5)), EINVAL, b"power"),
     (dict(rows=_rows(k=0x1001)), EINVAL, b"aligned"), (dict(B=1 << 23), EINVAL, b"threads"),
+    (dict(B=(1 << 31) - 1, Hkv=(1 << 31) - 1), EINVAL, b"threads"),
 ])
 def test_evict_refusals(kw, code, word):
     assert _evict(**kw) == code and word in _error()
