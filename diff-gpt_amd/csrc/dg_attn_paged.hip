@@ -214,7 +214,7 @@ enum PagedKernel { kTileKernel, kMfmaKernel, kVecKernel };
 struct PagedShape {
   int rows_per_wg, nrb, nsplit, chunk, rb_groups, rb_each;
   int64_t blocks;
-  bool ordered;
+  bool ordered, ranked;  // the longest rows first: by paged_order_kernel, by each wave
   int64_t scores_ld;
   size_t o_bytes, lse_at, scores_at, order_at, ws_bytes;
 };
@@ -282,7 +282,9 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
   t.rb_groups = (int)std::max<int64_t>(1, std::min<int64_t>(t.nrb, (64 + units - 1) / units));
   t.rb_each = (t.nrb + t.rb_groups - 1) / t.rb_groups;
   t.blocks = (units * t.rb_groups + 7) / 8 * 8 * t.rb_each;
-  t.ordered = B > 1 && B <= kOrdered && longest >= 1024 && t.blocks > fill;
+  const bool turns = B > 1 && longest >= 1024 && t.blocks > fill;
+  t.ranked = turns && B <= kRankedRows;
+  t.ordered = turns && !t.ranked && B <= kOrdered;
   const size_t acc = dtype == DG_F64 ? 8 : 4;
   const size_t parts = (size_t)(B * Hkv * R) * t.nsplit;
   if (t.nsplit > 1) {
@@ -383,6 +385,7 @@ int paged_call(const dg_paged_attention_args* args, PagedCall* c) {
   const PagedShape& t = c->t;
   a.rows_per_wg = t.rows_per_wg; a.nrb = t.nrb; a.nsplit = t.nsplit; a.chunk = t.chunk;
   a.rb_groups = t.rb_groups; a.rb_each = t.rb_each;
+  a.ranked = t.ranked;
   return DG_OK;
 }
 
