@@ -11,6 +11,9 @@
 
 namespace dg {
 
+// Rows of a key head up to which, and bytes in all, the attention leaves its scores.
+constexpr int64_t kScoreRows = 8, kScoreBytes = 64 << 20;
+
 // w[t] += sum over the rows r of one key head of exp(s_rt - lse_r), 64 positions a workgroup
 // by 32 rows at a time: a thread has one position and every fourth row, keys and rows pass
 // through LDS in chunks of 64 dims.
@@ -109,18 +112,44 @@ __global__ __launch_bounds__(kOrdered) void paged_order_kernel(const SeqArgs a, 
 // The same from the scores that the attention left (a.scores), four positions a thread: where
 // few rows share a position, their scores are a fraction of its key.  48 rows of a step, 4 rows a
 // key head of 128 dims, up to 4096 positions: 5.1 us in place of the 19.9 of paged_weights_kernel.
-__global__ __launch_bounds__(256) void paged_scores_kernel(const SeqArgs a, const PagedWeights w) {
-  const int64_t bh = blockIdx.x / (unsigned)w.blocks;
-  const int blk = (int)(blockIdx.x - (unsigned)bh * (unsigned)w.blocks);
+// JOINED: the rows' sums are in a.lse; otherwise their splits' are joined here, as seq_join4 does.
+template <bool JOINED>
+__device__ __forceinline__ void paged_scores(const SeqArgs& a, const PagedWeights& w, const float lift, const unsigned block) {
+  __shared__ float sums[kScoreRows];
+  const int64_t bh = block / (unsigned)w.blocks;
+  const int blk = (int)(block - (unsigned)bh * (unsigned)w.blocks);
   const int64_t b = bh / a.Hkv;
   const int kvh = (int)(bh - b * a.Hkv);
   const PagedRow pr = paged_row(a, b, __builtin_amdgcn_readfirstlane(a.lens[b]));
   const int total = pr.own + pr.count, nrows = pr.count * a.G;
-  if (nrows == 0) return;
+  if (nrows == 0 || blk * 1024 >= total) return;  // whole workgroups
+  if constexpr (!JOINED) {
+    const int lane = threadIdx.x & 63, chunk = paged_chunk(a, pr);
+    for (int r = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < nrows; r += 4) {
+      const u32x2_t* const ml = static_cast<const u32x2_t*>(a.ws_ml) + (bh * (a.N * a.G) + r) * a.nsplit;
+      const int used = min(a.nsplit, (paged_end(a, pr, r) + chunk - 1) / chunk);
+      float m = kNegInf, l = 0.f;
+      bool bad = false;
+      for (int s = lane; s < used; s += 64) {
+        const float ms = __uint_as_float(ml[s][0]);
+        bad = bad || ms != ms || __uint_as_float(ml[s][1]) != __uint_as_float(ml[s][1]);
+        m = fmaxf(m, ms);
+      }
+      m = wave_max(m);
+      bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+      for (int s = lane; s < used; s += 64) {
+        const float ms = __uint_as_float(ml[s][0]);
+        l += ms == kNegInf ? 0.f : __uint_as_float(ml[s][1]) * __builtin_amdgcn_exp2f(ms - m);
+      }
+      l = group_sum_dpp<64>(l);
+      if (lane == 0) sums[r] = bad ? __builtin_nanf("") : m - lift + __builtin_amdgcn_logf(l);
+    }
+    __syncthreads();
+  }
   for (int64_t t64 = 4 * (blk * (int64_t)256 + threadIdx.x); t64 < total; t64 += (int64_t)1024 * w.blocks) {
     const int t = (int)t64;
     const int64_t row = bh * (a.N * a.G);
-    const float* const lse = static_cast<const float*>(a.lse) + row;
+    const float* const lse = JOINED ? static_cast<const float*>(a.lse) + row : sums;
     const float* const s = a.scores + row * a.scores_ld + t;
     f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -141,11 +170,20 @@ __global__ __launch_bounds__(256) void paged_scores_kernel(const SeqArgs a, cons
       if (t + e < total) o[e] += sum[e];
   }
 }
+__global__ __launch_bounds__(256) void paged_scores_kernel(const SeqArgs a, const PagedWeights w) {
+  paged_scores<true>(a, w, 0.f, blockIdx.x);
+}
+// The outputs of split rows joined by the first `joins` workgroups, the weights from their scores
+// by the others, in one launch (48 x 1 token behind 100 - 4096, 16 heads on 4 of 128, two
+// launches / one: 59.6 / 58.1 us with the attention).
+template <typename T, int D, int WPR>
+__global__ __launch_bounds__(256) void paged_join_scores_kernel(const SeqArgs a, const int64_t nrows, const unsigned joins,
+                                                                const PagedWeights w) {
+  if (blockIdx.x < joins) seq_join4<T, D, WPR, kPaged>(a, nrows, blockIdx.x);
+  else paged_scores<false>(a, w, seq_lift<T>(), blockIdx.x - joins);
+}
 
 namespace {
-
-// Rows of a key head up to which, and bytes in all, the attention leaves its scores.
-constexpr int64_t kScoreRows = 8, kScoreBytes = 64 << 20;
 
 template <typename T>
 int launch_tile(const SeqArgs& a, dim3 grid, hipStream_t s) {
@@ -165,27 +203,37 @@ int launch_tile(const SeqArgs& a, dim3 grid, hipStream_t s) {
   return check_launch("seq_tile_paged");
 }
 
+// scores: workgroups of the weights from scores (0: none)
+template <typename T, int D, int WPR>
+void launch_join4(const SeqArgs& a, unsigned joins, int64_t rows, const PagedWeights& w, unsigned scores, hipStream_t s) {
+  if (scores > 0)
+    hipLaunchKernelGGL((paged_join_scores_kernel<T, D, WPR>), dim3(joins + scores), dim3(256), 0, s, a, rows, joins, w);
+  else
+    hipLaunchKernelGGL((seq_join4_kernel<T, D, WPR, kPaged>), dim3(joins), dim3(256), 0, s, a, rows);
+}
+
 template <typename T, int WPR>
-void launch_join4(const SeqArgs& a, dim3 grid, int64_t rows, hipStream_t s) {
+void launch_join4_dim(const SeqArgs& a, unsigned joins, int64_t rows, const PagedWeights& w, unsigned scores, hipStream_t s) {
   const int D = seq_mfma_dim(a.D);
-  if (D == 16) hipLaunchKernelGGL((seq_join4_kernel<T, 16, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
-  else if (D == 32) hipLaunchKernelGGL((seq_join4_kernel<T, 32, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
-  else if (D == 64) hipLaunchKernelGGL((seq_join4_kernel<T, 64, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
-  else if (D == 128) hipLaunchKernelGGL((seq_join4_kernel<T, 128, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
-  else hipLaunchKernelGGL((seq_join4_kernel<T, 256, WPR, kPaged>), grid, dim3(256), 0, s, a, rows);
+  if (D == 16) launch_join4<T, 16, WPR>(a, joins, rows, w, scores, s);
+  else if (D == 32) launch_join4<T, 32, WPR>(a, joins, rows, w, scores, s);
+  else if (D == 64) launch_join4<T, 64, WPR>(a, joins, rows, w, scores, s);
+  else if (D == 128) launch_join4<T, 128, WPR>(a, joins, rows, w, scores, s);
+  else launch_join4<T, 256, WPR>(a, joins, rows, w, scores, s);
 }
 
 template <typename T>
-int launch_join(const SeqArgs& a, bool mfma, bool many, dim3 grid, int64_t rows, hipStream_t s) {
+int launch_join(const SeqArgs& a, bool mfma, bool many, unsigned joins, int64_t rows, const PagedWeights& w, unsigned scores,
+                hipStream_t s) {
   if constexpr (sizeof(T) < 8) {
     if (mfma) {
-      if (many) launch_join4<T, 4>(a, grid, rows, s);
-      else launch_join4<T, 1>(a, grid, rows, s);
-      return check_launch("seq_join4_paged");
+      if (many) launch_join4_dim<T, 4>(a, joins, rows, w, scores, s);
+      else launch_join4_dim<T, 1>(a, joins, rows, w, scores, s);
+      return check_launch(scores > 0 ? "paged_join_scores_kernel" : "seq_join4_paged");
     }
   }
-  if (many) hipLaunchKernelGGL((seq_join_kernel<T, 4, kPaged>), grid, dim3(256), 0, s, a, rows);
-  else hipLaunchKernelGGL((seq_join_kernel<T, 1, kPaged>), grid, dim3(256), 0, s, a, rows);
+  if (many) hipLaunchKernelGGL((seq_join_kernel<T, 4, kPaged>), dim3(joins), dim3(256), 0, s, a, rows);
+  else hipLaunchKernelGGL((seq_join_kernel<T, 1, kPaged>), dim3(joins), dim3(256), 0, s, a, rows);
   return check_launch("seq_join_paged");
 }
 
@@ -429,10 +477,10 @@ extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* wor
   const int wkeys = scored ? 1024 : wmfma ? kWeightKeys : 64;
   w.blocks = (int)((args->longest + wkeys - 1) / wkeys);
   const int64_t wblocks = weights == nullptr ? 0 : wmfma && !scored ? ((int64_t)B * Hkv + 7) / 8 * 8 * w.blocks : (int64_t)B * Hkv * w.blocks;
-  DG_REQUIRE(blocks <= kMostWorkgroups256 && groups <= kMostWorkgroups256 && wblocks <= kMostWorkgroups256, DG_EINVAL,
+  DG_REQUIRE(blocks <= kMostWorkgroups256 && groups + wblocks <= kMostWorkgroups256, DG_EINVAL,
              "paged_attention: more than 2^24 - 1 workgroups");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)blocks), jgrid((unsigned)groups), wgrid((unsigned)wblocks);
+  const dim3 grid((unsigned)blocks), wgrid((unsigned)wblocks);
   int rc;
   if (t.ordered) {
     hipLaunchKernelGGL(paged_order_kernel, dim3(1), dim3(kOrdered), 0, s, a, const_cast<int32_t*>(a.order));
@@ -445,12 +493,14 @@ extern "C" int dg_paged_attention(const dg_paged_attention_args* args, void* wor
   else if (dtype == DG_BF16) rc = launch_tile<bf16_t>(a, grid, s);
   else rc = launch_tile<f16_t>(a, grid, s);
   if (rc == DG_OK && t.nsplit > 1) {
-    if (dtype == DG_F64) rc = launch_join<double>(a, mfma, many, jgrid, nrows, s);
-    else if (dtype == DG_F32) rc = launch_join<float>(a, mfma, many, jgrid, nrows, s);
-    else if (dtype == DG_BF16) rc = launch_join<bf16_t>(a, mfma, many, jgrid, nrows, s);
-    else rc = launch_join<f16_t>(a, mfma, many, jgrid, nrows, s);
+    const unsigned joins = (unsigned)groups, scores = scored ? (unsigned)wblocks : 0;
+    if (dtype == DG_F64) rc = launch_join<double>(a, mfma, many, joins, nrows, w, scores, s);
+    else if (dtype == DG_F32) rc = launch_join<float>(a, mfma, many, joins, nrows, w, scores, s);
+    else if (dtype == DG_BF16) rc = launch_join<bf16_t>(a, mfma, many, joins, nrows, w, scores, s);
+    else rc = launch_join<f16_t>(a, mfma, many, joins, nrows, w, scores, s);
   }
   if (rc != DG_OK || weights == nullptr) return rc;
+  if (scored && t.nsplit > 1) return DG_OK;  // with the join
   if (scored) {
     hipLaunchKernelGGL(paged_scores_kernel, wgrid, dim3(256), 0, s, a, w);
     return check_launch("paged_scores_kernel");

@@ -391,17 +391,23 @@ __global__ __launch_bounds__(256) void seq_join_kernel(const SeqArgs a, const in
       yp[lane + 64 * c] = S::store(none ? (A)0 : bad ? (A)__builtin_nanf("") : o[c] / l);
 }
 
+// log2 of what the sums of a split's exponentials are too large by (SeqMma).
+template <typename T>
+constexpr float seq_lift() {
+  return __is_same(T, f16_t) ? 7.f : 0.f;
+}
+
 // The same for the head dims of the matrix-core kernel: a lane reads four elements of a
 // split at a time, so that a wave reads 64 / (D / 4) splits at once, and lengths and states
 // are in flight together (those of unused splits are read and not looked at).  WPR waves a
 // row as above.
 template <typename T, int D, int WPR, SeqMode MODE>
-__global__ __launch_bounds__(256) void seq_join4_kernel(const SeqArgs a, const int64_t nrows) {
+__device__ __forceinline__ void seq_join4(const SeqArgs& a, const int64_t nrows, const unsigned block) {
   constexpr int LPS = D / 4, SPW = 64 / LPS;  // lanes a split, splits a wave
   __shared__ float part[WPR > 1 ? (WPR - 1) * D : 1];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = WPR > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wv;
+  const int64_t row = WPR > 1 ? (int64_t)block : (int64_t)block * 4 + wv;
   if (row >= nrows) return;  // WPR > 1: whole workgroups
   const int sub = WPR > 1 ? wv : 0;
   const int R = a.N * a.G;
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(256) void seq_join4_kernel(const SeqArgs a, const i
   }
   if (ls4 != 0) return;
   if constexpr (MODE >= kPaged) {
-    constexpr float kLift = __is_same(T, f16_t) ? 7.f : 0.f;  // of the parts' sums (SeqMma)
+    constexpr float kLift = seq_lift<T>();
     if (a.lse != nullptr && d4 == 0)
       static_cast<float*>(a.lse)[row] =
           none ? __builtin_huge_valf() : bad ? __builtin_nanf("") : m - kLift + __builtin_amdgcn_logf(l);
@@ -478,6 +484,10 @@ __global__ __launch_bounds__(256) void seq_join4_kernel(const SeqArgs a, const i
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = none ? 0.f : bad ? __builtin_nanf("") : o[e] / l;
   if (d4 < a.D) store_vec<T, 4>(yp + d4, y);
+}
+template <typename T, int D, int WPR, SeqMode MODE>
+__global__ __launch_bounds__(256) void seq_join4_kernel(const SeqArgs a, const int64_t nrows) {
+  seq_join4<T, D, WPR, MODE>(a, nrows, blockIdx.x);
 }
 
 }  // namespace dg
