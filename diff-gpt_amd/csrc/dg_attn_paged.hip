@@ -286,12 +286,12 @@ int64_t stage_ns(int D, int dtype, int rows_per_wg) {
 //   8 x 200, 4000, 8 / 8 of 64, 32              36.3 / 43 / 51 / 51
 //   6 x 237, 5580, 2 / 2 of 16, 32              21.7 / 18 / 16 / 19
 //   5 x 25, 13386, fp32, 24 / 6 of 80, 64       909 / 464 / 246 / 198
-int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t fill, int D, int64_t ns, bool few) {
+int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t chunk, int64_t fill, int D, int64_t ns, bool few) {
   const int64_t whole = longest * ns / 128;
   auto percent = [&](int64_t n) { return n <= fill ? 100 : 100 * n / fill + 25; };
   int best = 1;
   int64_t least = percent(wg) * whole / 100;
-  const int64_t most = std::min<int64_t>(longest / 256, kMaxSplits);
+  const int64_t most = std::min<int64_t>(longest / chunk, kMaxSplits);
   for (int k = 2; k <= most && wg * k <= 4 * fill; ++k) {
     const int64_t cost = percent(wg * k) * whole / (100 * k) + 8000 + rows * k * D * 8 / 3000;
     if (cost < least) {
@@ -322,9 +322,12 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
                                            : Dm == 256 ? 512 : Dm == 128 ? 768 : 1024;
   const int64_t wg = std::max<int64_t>(1, B * Hkv * t.nrb);
   const int64_t ns = vec ? 1200 + Dm * R * 3 : mfma ? stage_ns(Dm, dtype, rows_per_wg) : 0;
-  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, fill, Dm, ns, R <= 32)
+  // fewest keys of a split: in fp32, where a stage of 128 takes as long as the join, that; us with
+  // 256 / 128, fp32: 7 x 5 tokens behind 1200 - 2500, 6 heads on 3 of 128, 39.6 / 32.0; 1 x 30,
+  // 8000, 4 on 4 of 128 39.8 / 30.8; 3 x 8, 700, 4 on 4 of 64 17.2 / 15.0
+  t.chunk = kernel == kMfmaKernel && dtype == DG_F32 && Dm >= 64 ? 128 : 256;
+  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, t.chunk, fill, Dm, ns, R <= 32)
                   : (int)std::max<int64_t>(1, std::min<int64_t>({(fill + wg - 1) / wg, longest / 256, kMaxSplits}));
-  t.chunk = 256;
   // every XCD has work: the row blocks of few (b, key head, split) go to several, in groups
   const int64_t units = B * Hkv * t.nsplit;
   t.rb_groups = (int)std::max<int64_t>(1, std::min<int64_t>(t.nrb, (64 + units - 1) / units));
