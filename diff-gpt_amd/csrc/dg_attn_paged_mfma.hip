@@ -9,23 +9,26 @@
 //
 // so that a lane's 16 scores belong to one position and add up where they are; the two
 // halves of a wave meet at the end.  No atomics: a position belongs to one wave.  8 x 200
-// tokens behind 500 - 4000 positions, 8 heads of 64 on 8, fp16: 12.8 us, the attention before it
-// 32.8 (vector ALU 27 % busy, matrix cores 4 %: bound by the latencies of a workgroup, its keys
-// and then seven tiles of rows in turn).
+// tokens behind 500 - 4000 positions, 8 heads of 64 on 8, fp16: 12 us, the attention before it
+// 32.8 (vector ALU 27 % busy, matrix cores 4 %: bound by the latencies of a workgroup: its keys
+// and then its stages of rows in turn).  Many rows: by the exponentials, a fused product, an
+// exp2 at a quarter of the rate and a sum each where nothing is hidden; 8 x 256 behind 1260 -
+// 4000, 16 heads on 4 of 128, 50 us, 56 with every score masked (two tiles a stage, which 64 dims
+// in 16 bits have, took 48 there, but left 4 waves a SIMD of 5: 64 x 5 tokens 33 -> 34.5).
 #include "dg_paged.h"
 #include "dg_seq_mfma.h"
 
 namespace dg {
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_weights_kernel(const SeqArgs a, const PagedWeights w) {
+__global__ __launch_bounds__(256, D * sizeof(T) <= 256 ? 5 : 3) void paged_weights_kernel(const SeqArgs a, const PagedWeights w) {
   using C = SeqCfg<T, D, 4>;
   using M = SeqMma<T>;
   using vec8 = typename M::vec8;
   constexpr bool F32 = C::ES == 4;
-  constexpr int ES = C::ES, PPR = C::PPR, RPD = C::RPD, TILE = 32 * D, NDMA = 32 / RPD;
-  __shared__ __attribute__((aligned(16))) T qs[2][TILE];
-  __shared__ __attribute__((aligned(16))) float ls[2][32];
+  constexpr int ES = C::ES, PPR = C::PPR, RPD = C::RPD, ROWS = D * ES <= 128 ? 64 : 32, NDMA = ROWS / RPD;
+  __shared__ __attribute__((aligned(16))) T qs[2][ROWS * D];
+  __shared__ __attribute__((aligned(16))) float ls[2][ROWS];
 
   // workgroup x runs on XCD x mod 8: the key blocks of a key head follow each other there and
   // share its rows
@@ -47,6 +50,9 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const SeqArgs a, con
     // rows are (token, head of the group) pairs; position t is seen from row `from` on
     const int64_t from64 = (int64_t)(t - pr.own) * a.G;
     const int from = t >= total ? nrows : (int)max(from64, (int64_t)0);
+    // the rows that all of the wave's positions are seen from
+    const int last = kb + 32 * wv + 31;
+    const int all_from = last >= total ? nrows : (int)max((int64_t)(last - pr.own) * a.G, (int64_t)0);
     // the first tile that any position of the workgroup is seen from
     const int first = max(kb - pr.own, 0) * a.G / 32 * 32;
 
@@ -57,6 +63,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const SeqArgs a, con
       for (int n = 0; n < (NDMA + 3) / 4; ++n) {
         const int i = 4 * n + wv;
         if (NDMA % 4 != 0 && i >= NDMA) break;  // wave-uniform
+        if (row0 + i * RPD / 32 * 32 >= nrows) break;  // tiles without a row are not computed
         const int r = i * RPD + lane / PPR, row = row0 + r;
         const int e = ((lane % PPR) ^ seq_swz<PPR, ES>(r)) * (16 / ES);
         const int qi = row / a.G;
@@ -64,13 +71,14 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const SeqArgs a, con
         const void* p = in ? static_cast<const void*>(qb + qi * a.qt + (int64_t)(row - qi * a.G) * a.qh + e) : &kZeros16;
         lds_copy16(p, qs[st] + i * RPD * D);
       }
-      if (threadIdx.x < 32) {
-        const int row = row0 + (int)threadIdx.x;
-        ls[st][threadIdx.x] = row < nrows ? lse[row] : __builtin_huge_valf();
-      }
+    };
+    auto row_lse = [&](int row0) __attribute__((always_inline)) {
+      const int row = row0 + (int)threadIdx.x;
+      return threadIdx.x < ROWS && row < nrows ? lse[row] : __builtin_huge_valf();
     };
 
     copy_rows(0, first);
+    const float head = row_lse(first);
     vec8 kf[F32 ? C::QC : C::NC];
     int id = -1;
     if (t < total) id = a.table[b * a.table_ld + (t >> a.page_log2)];
@@ -99,42 +107,64 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const SeqArgs a, con
     const int kswz = seq_swz<PPR, ES>(r32);
     float acc = 0.f, accc = 0.f;
     int st = 0;
-    for (int row0 = first; row0 < nrows; row0 += 32, st ^= 1) {
+    if (threadIdx.x < ROWS) ls[0][threadIdx.x] = head;
+    for (int stage0 = first; stage0 < nrows; stage0 += ROWS, st ^= 1) {
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();  // stage st filled; every wave is done with the other
-      if (row0 + 32 < nrows) copy_rows(st ^ 1, row0 + 32);
-      const T* const Q = qs[st];
-      floatx16_t s;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.f;
-      if constexpr (F32) {
-#pragma unroll
-        for (int p = 0; p < C::QC / 4; ++p) {
-          const f32x4_t qf = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(Q) + r32 * D + 4 * (((PPR / 2) * hh + p) ^ kswz));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(qf[e], kf[4 * p + e], s, 0, 0, 0);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < C::NC; ++c) {
-          const u32x4_t qf = *reinterpret_cast<const u32x4_t*>(Q + r32 * D + 8 * ((2 * c + hh) ^ kswz));
-          s = M::mma(__builtin_bit_cast(vec8, qf), kf[c], s);
-        }
+      float next = 0.f;
+      if (stage0 + ROWS < nrows) {
+        copy_rows(st ^ 1, stage0 + ROWS);
+        next = row_lse(stage0 + ROWS);
       }
-      // lane l, register r: row 8 (r / 4) + 4 hh + r % 4 of the tile
-      const int lo = from - row0 - 4 * hh, hi = nrows - row0 - 4 * hh;
-      float sum = 0.f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4_t l4 = *reinterpret_cast<const f32x4_t*>(&ls[st][8 * g + 4 * hh]);
+      for (int tile = 0; tile < ROWS / 32; ++tile) {
+        const int row0 = stage0 + 32 * tile;
+        if (row0 >= nrows) break;  // the same in all waves
+        const T* const Q = qs[st] + 32 * tile * D;
+        floatx16_t s;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 8 * g + e;
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], a.scale_log2, -l4[e]));
-          sum += r >= lo && r < hi ? p : 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        if constexpr (F32) {
+#pragma unroll
+          for (int p = 0; p < C::QC / 4; ++p) {
+            const f32x4_t qf = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(Q) + r32 * D + 4 * (((PPR / 2) * hh + p) ^ kswz));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(qf[e], kf[4 * p + e], s, 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < C::NC; ++c) {
+            const u32x4_t qf = *reinterpret_cast<const u32x4_t*>(Q + r32 * D + 8 * ((2 * c + hh) ^ kswz));
+            s = M::mma(__builtin_bit_cast(vec8, qf), kf[c], s);
+          }
         }
+        // lane l, register r: row 8 (r / 4) + 4 hh + r % 4 of the tile
+        const int lo = from - row0 - 4 * hh, hi = nrows - row0 - 4 * hh;
+        float sum = 0.f;
+        if (row0 >= all_from && row0 + 32 <= nrows) {  // nothing hidden
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4_t l4 = *reinterpret_cast<const f32x4_t*>(&ls[st][32 * tile + 8 * g + 4 * hh]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], a.scale_log2, -l4[e]));
+          }
+          add_rounded(acc, accc, sum);
+          continue;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4_t l4 = *reinterpret_cast<const f32x4_t*>(&ls[st][32 * tile + 8 * g + 4 * hh]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 8 * g + e;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], a.scale_log2, -l4[e]));
+            sum += r >= lo && r < hi ? p : 0.f;
+          }
+        }
+        add_rounded(acc, accc, sum);
       }
-      add_rounded(acc, accc, sum);
+      // written here, not where it is loaded: that would wait for the copies
+      if (threadIdx.x < ROWS) ls[st ^ 1][threadIdx.x] = next;
     }
     acc = half_pair_sum(acc - accc);
     if (hh == 0 && t < total) {
