@@ -9,7 +9,7 @@
 //
 // so that a lane's 16 scores belong to one position and add up where they are; the two
 // halves of a wave meet at the end.  No atomics: a position belongs to one wave.  8 x 200
-// tokens behind 500 - 4000 positions, 8 heads of 64 on 8, fp16: 12 us, the attention before it
+// tokens behind 500 - 4000 positions, 8 heads of 64 on 8, fp16: 11 us, the attention before it
 // 32.8 (vector ALU 27 % busy, matrix cores 4 %: bound by the latencies of a workgroup: its keys
 // and then its stages of rows in turn).  Many rows: by the exponentials, a fused product, an
 // exp2 at a quarter of the rate and a sum each where nothing is hidden; 8 x 256 behind 1260 -

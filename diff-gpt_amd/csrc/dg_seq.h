@@ -1,8 +1,8 @@
-// Launch arguments shared by the kernels of packed attention and of token trees
-// over a cache (dg_attn_seq.hip: any shape; dg_attn_seq_mfma.hip: 16-bit and fp32 data
-// at head_dim up to 256 and 128, in rows of whole 16-byte pieces).
+// Launch arguments shared by the kernels of packed attention, of token trees over a cache and
+// of attention over a cache in pages (dg_seq_tile.h: any shape; dg_seq_mfma.h: 16-bit and fp32
+// data at head_dim up to 256 and 128, in rows of whole 16-byte pieces).
 //
-// Both operators reduce to one piece of work: the rows of one key head, where the
+// These operators reduce to one piece of work: the rows of one key head, where the
 // rows are the (query, head of the group) pairs r = i * G + g of a sequence, over a
 // range of that sequence's keys.  Heads of a group so share every key they read, and
 // a few queries still fill a tile of rows.
