@@ -95,6 +95,18 @@ def test_long_rows_are_split(dev, dtype, N, D, S):
     _check(dev, dtype, lens, counts, N, 4, 2, D, S, longest=1)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B", [63, 64, 65])
+@pytest.mark.parametrize("N,H,Hkv,D", [(1, 16, 8, 128), (3, 8, 8, 64)])
+def test_rows_in_turns(dev, dtype, B, N, H, Hkv, D):
+    """More workgroups than run at once, whose longest rows come first: rows alike, rows of nothing
+    and rows without tokens among them."""
+    lens = [(331 * b) % 1300 if b % 5 else 700 for b in range(B)]
+    lens[0] = 1500
+    counts = [0 if b % 11 == 7 else max(1, N - b % 3) for b in range(B)]
+    _check(dev, dtype, lens, counts, N, H, Hkv, D, 64)
+
+
 def test_positions_outside_the_hint_and_the_table(dev):
     """Lengths are cut to what the table covers, counts to what is left of it."""
     from diff_gpt.model.paged import attention_paged
