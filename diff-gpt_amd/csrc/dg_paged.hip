@@ -44,12 +44,19 @@ struct AppendArgs {
   int N, H, Hkv, D, cap, page_log2, groups, qknorm;
 };
 
-// N values of T as raw words: by 16-byte accesses (VEC, p aligned to them), or one by one those below `n`.
+// N values of T as raw words: VEC by 16-byte accesses, 8 bytes of them by one of 8 (an fp32
+// table's angles of two fp64 dims), p aligned to them; or one by one those below `n`.
 template <typename T, int N, bool VEC>
 __device__ __forceinline__ void load_some(const T* p, uint32_t (&w)[N * sizeof(T) / 4], int n) {
-  if constexpr (VEC) {
+  constexpr int BYTES = N * (int)sizeof(T);
+  if constexpr (VEC && BYTES == 8) {
+    const u32x2_t x = *reinterpret_cast<const u32x2_t*>(p);
+    w[0] = x[0];
+    w[1] = x[1];
+  } else if constexpr (VEC) {
+    static_assert(BYTES % 16 == 0, "all of the values are loaded");
 #pragma unroll
-    for (int c = 0; c < N * (int)sizeof(T) / 16; ++c) {
+    for (int c = 0; c < BYTES / 16; ++c) {
       const u32x4_t x = reinterpret_cast<const u32x4_t*>(p)[c];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[4 * c + i] = x[i];
@@ -67,6 +74,7 @@ __device__ __forceinline__ void load_some(const T* p, uint32_t (&w)[N * sizeof(T
 template <typename T, int N, bool VEC>
 __device__ __forceinline__ void store_some(T* p, const uint32_t (&w)[N * sizeof(T) / 4], int n) {
   if constexpr (VEC) {
+    static_assert(N * sizeof(T) % 16 == 0, "all of the values are stored");
 #pragma unroll
     for (int c = 0; c < N * (int)sizeof(T) / 16; ++c)
       reinterpret_cast<u32x4_t*>(p)[c] = u32x4_t{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
