@@ -3,7 +3,7 @@
 // (dg_paged_evict).
 //
 // paged_append_kernel.  y = r / sqrt(mean(r^2) + eps), r the pairs of a head turned by their
-// position's angle: both in fp32 (fp64) registers, one rounding as y is stored.  (The cache of
+// position's angle: both in fp32 (fp64) registers, eps that type's, one rounding as y is stored.  (The cache of
 // one length, dg_rope.hip, rounds r to the data's type first, as the reference does; once is
 // nearer to the exact value, bf16 1.7e-3 of it, and no dearer.)  LPR lanes share a head, 16 bytes
 // each; they take HPT heads of a token, whose loads are in flight together and whose angles
@@ -91,6 +91,7 @@ __device__ __forceinline__ void store_some(T* p, const uint32_t (&w)[N * sizeof(
 template <typename T>
 struct AppendAcc {
   using type = float;
+  static constexpr float kEps = FLT_EPSILON;
   __device__ static void load(const uint32_t* w, int i, float& x, float& y) {
     if constexpr (sizeof(T) == 4) {
       x = __uint_as_float(w[2 * i]);
@@ -114,6 +115,7 @@ struct AppendAcc {
 template <>
 struct AppendAcc<double> {
   using type = double;
+  static constexpr double kEps = DBL_EPSILON;
   __device__ static void load(const uint32_t* w, int i, double& x, double& y) {
     __builtin_memcpy(&x, w + 4 * i, 8);
     __builtin_memcpy(&y, w + 4 * i + 2, 8);
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
           ss += y[c][e] * y[c][e] + y[c][e + 1] * y[c][e + 1];
         }
       A f = (A)1;
-      if (a.qknorm) f = inv_sqrt(lanes_sum<LPR>(ss) * (A)(1.0 / a.D) + (A)FLT_EPSILON);
+      if (a.qknorm) f = inv_sqrt(lanes_sum<LPR>(ss) * (A)(1.0 / a.D) + S::kEps);
       if (!known) f = (A)__builtin_nanf("");
 #pragma unroll
       for (int c = 0; c < NCK; ++c)

@@ -22,7 +22,8 @@ def append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, freqs: torch
     counts[b] of the N tokens ((B,) int32; None: all), the others' queries are zeros and their
     keys go nowhere, like those of tokens that the table has no room for.  Token n stands at position
     positions[b] + n of freqs (Tmax, D / 2, 2) (None: lengths[b] + n); outside of it queries and
-    keys are NaN.  Everything is rounded once, as it is stored."""
+    keys are NaN.  In fp32, fp64 for fp64 rows (an fp32 table's angles too), the norm's eps that
+    of the arithmetic's type; everything is rounded once, as it is stored."""
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _native.paged_append_(q, k, v, freqs, out, k_pages, v_pages, table, lengths, counts, positions, qknorm)
     return out

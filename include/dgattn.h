@@ -694,7 +694,7 @@ typedef struct dg_paged_rows {
  * The rotation by position and the norm of every head of B x N tokens, and their keys and
  * values into the pages.  With r the rotation of the D / 2 neighbouring pairs of a head by the
  * (cos, sin) pairs freqs[position * freqs_ld ..] and, with DG_QKNORM, a division by
- * sqrt(mean(r^2) + FLT_EPSILON):
+ * sqrt(mean(r^2) + FLT_EPSILON) (fp64: DBL_EPSILON):
  *   q_out[b,n,h,:] = norm(r(q[b,n,h,:])),  the pages' k = norm(r(k[b,n,h,:])),  v = v[b,n,h,:]
  * in fp32 (fp64 for fp64), rounded once.  Token n of row b has position positions[b] + n
  * (NULL: lens[b] + n); outside [0, freqs_rows) its q and k become NaN.  Tokens that are not
