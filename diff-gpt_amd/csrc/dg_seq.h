@@ -97,9 +97,10 @@ __device__ __forceinline__ PagedRow paged_row(const SeqArgs& a, int64_t b, int l
   r.count = min(max(count, 0), min(a.N, a.Tcap - r.own));
   return r;
 }
-// Keys of each of its splits: as even as whole stages (of 128 keys at most) allow, so that
-// rows of every length are split as far as the launch has splits, and never fewer than
-// a.chunk.
+// Keys of each of its splits: as even as whole 128s allow, so that rows of every length are split
+// as far as the launch has splits, and never fewer than a.chunk.  A stage of the matrix-core
+// kernel has up to 256 keys (32 rows of up to 64 bytes a key), in key blocks that a split has
+// whole or not at all.
 __device__ __forceinline__ int paged_chunk(const SeqArgs& a, const PagedRow& r) {
   const int even = (r.own + r.count + a.nsplit - 1) / a.nsplit;
   return max(a.chunk, (even + 127) & ~127);

@@ -442,7 +442,9 @@ void seq_mfma_kernel(const SeqArgs a) {
     T* const vs = st + kg * 2 * TILE + TILE;
 #pragma unroll 1
     for (int j = 0; j < BN; ++j) {
-      const bool sees = (visible(s0 + kg * BN + (j & ~31)) >> (j & 31)) & 1u;
+      bool sees = (visible(s0 + kg * BN + (j & ~31)) >> (j & 31)) & 1u;
+      // a paged split's last stage may go past its keys, into the next one's: not its own
+      if constexpr (PAGED) sees = sees && s0 + kg * BN + j < pc.kend;
       const int ksw = seq_swz<PPR, ES>(j);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
