@@ -309,7 +309,6 @@ __global__ __launch_bounds__(THREADS) void paged_select_kernel(const EvictArgs a
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int len = min(max(a.lens[b], 0), a.cap);
   int32_t* const kept = a.kept + bh * a.keep;
-  if (h == 0 && tid == 0) a.new_lens[b] = min(len, a.keep);
   if (len <= a.keep) {
     for (int j = tid; j < a.keep; j += THREADS) kept[j] = j < len ? j : -1;
     return;  // whole workgroups, before any barrier
@@ -442,6 +441,8 @@ __global__ __launch_bounds__(256) void paged_move_kernel(const EvictArgs a) {
   const int j = (int)(at - (uint32_t)bh * (uint32_t)a.to_cap);
   const int64_t b = (uint32_t)bh / (uint32_t)a.Hkv;
   const int h = (int)(bh - b * a.Hkv);
+  // by one thread a row, here: the selection is through with the lengths, which these may replace
+  if (j == 0 && h == 0 && piece == 0) a.new_lens[b] = min(min(max(a.lens[b], 0), a.cap), a.keep);
   const int t = j < a.keep ? a.kept[bh * a.keep + j] : -1;
   if (piece == 0) a.new_weights[at] = t < 0 ? 0.f : a.weights[b * a.wb + (int64_t)h * a.wh + t];
   if (t < 0) return;

@@ -757,7 +757,8 @@ DG_API int dg_paged_attention(const dg_paged_attention_args* args, void* workspa
  * ones and of the others those of the largest weights (fp32, weights[b * w_b + h * w_h + t];
  * equal ones: the earlier, NaN: above all), in their order, into positions 0 .. of the pages
  * that `to` names ((B, to_width), row stride to_ld; keep <= to_width * page).  A row of at
- * most `keep` positions moves as it is.  Written: new_lens[b] = min(lens[b], keep);
+ * most `keep` positions moves as it is.  Written: new_lens[b] = min(lens[b], keep), which may be
+ * rows.lens itself (nothing else that is written may overlap anything read);
  * kept[b][h][j], (B, Hkv, keep) contiguous, the position that j came from, -1 behind the last;
  * new_weights, (B, Hkv, to_width * page) contiguous, the kept positions' weights and zeros
  * behind them.  The pages that `to` names must not be any that the rows hold, nor named twice.
