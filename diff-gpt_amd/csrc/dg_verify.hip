@@ -7,8 +7,9 @@
 // probabilities in fp32 would move its borders by more than the small ones are apart).
 //
 // Rows of logits are read once for their maximum and sum, exponentials in fp32 with the scale
-// in two terms (its rounding would shift all of a row's exponents alike), sums in fp64, so
-// that the decisions u q < p come out as in 64 bits but for a few in 10^7.  Then one
+// in two terms (its rounding would shift all of a row's exponents alike), sums in fp64 but for a
+// thread's four vectors at a time, 32 exponentials at most, so that the decisions u q < p come
+// out as in 64 bits but for a few in 10^7.  Then one
 // workgroup or several a row race over the logits of the one row that decides.
 //
 // Few logits: one launch, a workgroup for each row of the batch.  Otherwise two: the
@@ -77,7 +78,7 @@ __device__ __forceinline__ float logit<double>(double x) {
   return (float)x;
 }
 
-// exp(scale d), d <= 0
+// exp(scale d), scale d at most kAhead in log2 units
 __device__ __forceinline__ float scaled_exp(const VerifyArgs& a, float d) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, a.scale_hi, d * a.scale_lo));
 }
@@ -123,10 +124,11 @@ __device__ __forceinline__ void load_any(const T* p, float (&z)[N]) {
 // costs all lanes of a wave some 40 instructions, a comparison one)
 constexpr float kAhead = 16.f;
 
-// N further logits from id v0 on (-inf for what is not there) into a thread's statistics.  A
-// NaN makes the sum one, beside logits of -inf alone too.
+// N further logits from id v0 on (-inf for what is not there) into a thread's statistics, whose
+// sum is `sum` and, of the latest, `part`.  A NaN makes the sum one, beside logits of -inf alone too.
 template <int N, bool GREEDY>
-__device__ __forceinline__ void add_logits(const VerifyArgs& a, const float (&z)[N], int v0, float& top, int& at, float& part) {
+__device__ __forceinline__ void add_logits(const VerifyArgs& a, const float (&z)[N], int v0, float& top, int& at, double& sum,
+                                           float& part) {
   float m = z[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) m = fmaxf(m, z[i]);
@@ -136,7 +138,11 @@ __device__ __forceinline__ void add_logits(const VerifyArgs& a, const float (&z)
       for (int i = N - 1; i >= 0; --i)
         if (z[i] == m) at = v0 + i;
     }
-    if (top != kNegInf) part *= scaled_exp(a, top - m);
+    if (top != kNegInf) {
+      const float f = scaled_exp(a, top - m);
+      part *= f;
+      sum *= (double)f;
+    }
     top = m;
   }
   if (top == kNegInf) {  // nothing yet
@@ -145,10 +151,10 @@ __device__ __forceinline__ void add_logits(const VerifyArgs& a, const float (&z)
       if (z[i] != z[i]) part = z[i];
     return;
   }
-  float sum = 0.f;
+  float some = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum += scaled_exp(a, z[i] - top);
-  part += sum;
+  for (int i = 0; i < N; ++i) some += scaled_exp(a, z[i] - top);
+  part += some;
 }
 
 // Thread `tid` of `step`'s part of the statistics of a row's vectors first .. end - 1, and of
@@ -158,18 +164,21 @@ __device__ __forceinline__ VerifyStat row_stat(const VerifyArgs& a, const T* x, 
   constexpr int VE = 16 / (int)sizeof(T), U = 4;
   const int whole = min(end, a.V / VE);
   float top = kNegInf, part = 0.f;
+  double sum = 0.0;
   int at = 0x7fffffff, j = first + tid;
   for (; j + (U - 1) * step < whole; j += U * step) {
     float z[U][VE];
 #pragma unroll
     for (int u = 0; u < U; ++u) load_any<T, VE>(x + (int64_t)(j + u * step) * VE, z[u]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) add_logits<VE, GREEDY>(a, z[u], (j + u * step) * VE, top, at, part);
+    for (int u = 0; u < U; ++u) add_logits<VE, GREEDY>(a, z[u], (j + u * step) * VE, top, at, sum, part);
+    sum += (double)part;
+    part = 0.f;
   }
   for (; j < whole; j += step) {
     float z[VE];
     load_any<T, VE>(x + (int64_t)j * VE, z);
-    add_logits<VE, GREEDY>(a, z, j * VE, top, at, part);
+    add_logits<VE, GREEDY>(a, z, j * VE, top, at, sum, part);
   }
   if (j < end) {  // the row's last, incomplete vector
     float z[VE];
@@ -178,9 +187,9 @@ __device__ __forceinline__ VerifyStat row_stat(const VerifyArgs& a, const T* x, 
       z[i] = kNegInf;
       if (j * VE + i < a.V) z[i] = logit<T>(x[j * VE + i]);
     }
-    add_logits<VE, GREEDY>(a, z, j * VE, top, at, part);
+    add_logits<VE, GREEDY>(a, z, j * VE, top, at, sum, part);
   }
-  return VerifyStat{(double)part, top, at, 0.f, 0};
+  return VerifyStat{sum + (double)part, top, at, 0.f, 0};
 }
 
 template <typename T>
