@@ -33,5 +33,6 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
     after them is the first maximum over V of max(p - q, 0) / noise (p / noise where all
     stand): uniforms (B, N) in [0, 1) and noise (B, V) from Exp(1), fp32.  At temperature 0
     draft x stands iff it is the first maximum of its logits, nothing is drawn, and log
-    probabilities are those at temperature 1.  A draft outside the vocabulary does not stand."""
+    probabilities are those at temperature 1.  A draft outside the vocabulary does not stand.
+    All of it is decided in fp32 with sums in fp64, for fp64 logits in fp64."""
     return Verified(*_native.verify_drafts(target, tokens, uniforms, noise, draft, counts, temperature))

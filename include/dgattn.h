@@ -790,10 +790,11 @@ DG_API int dg_paged_evict(const dg_paged_evict_args* args, void* stream);
  * of row i and the token after them is row a's; draft, uniforms and noise are not looked at.
  *   accepted[b] = a;  out_tokens[b * (N + 1) + j]: the standing drafts, the token, -1 behind;
  *   out_logprobs alike: log p_j of it (inv_temperature 0: of softmax(target)), 0 behind.
- * target (B,N+1,V), draft (B,N,V) logits, unit stride over V; fp32 / bf16 / fp16 / fp64 all
- * computed in fp32 with sums in fp64 (of 32 exponentials at most in fp32 before).  A draft outside [0, V) does not stand; nor does one of
- * a row with NaN, +inf or -inf alone, and the token after it is then not specified but within
- * [0, V).  0 <= N <= 64; inv_temperature 0 or from 2^-100 to 2^100.
+ * target (B,N+1,V), draft (B,N,V) logits, unit stride over V; fp32 / bf16 / fp16 computed in
+ * fp32 with sums in fp64 (of 32 exponentials at most in fp32 before), fp64 in fp64.  A draft
+ * outside [0, V) does not stand; nor does one of a row with NaN, +inf or -inf alone, and the
+ * token after it is then not specified but within [0, V).  0 <= N <= 64; inv_temperature 0 or
+ * from 2^-100 to 2^100.
  */
 typedef struct dg_verify_drafts_args {
   int64_t B, N, V, dtype;
