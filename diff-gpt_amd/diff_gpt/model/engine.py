@@ -314,7 +314,7 @@ class Engine:
         logprobs), each prompt followed by its tokens, and the model's log probability of each
         of these at the temperature (at 0, greedy decoding, at temperature 1).
 
-        draft: a model of the same vocabulary that proposes num_drafts tokens a row at a time,
+        draft: a model of the same vocabulary, of any type, that proposes num_drafts tokens a row at a time,
         which this one runs all at once and keeps as far as verify_drafts lets them stand: the
         tokens are distributed as without it, in fewer passes.  keep: when a row comes to hold a
         page more than so many positions, it is cut to them, the ``recent`` last ones (None: half)
@@ -357,6 +357,9 @@ class Engine:
             if temperature > 0:
                 u = torch.rand((B, N), generator=rng, device=device)
                 e = torch.empty((B, logits.size(-1)), device=device).exponential_(1, generator=rng)
+            if drafted is not None and drafted.dtype != logits.dtype:  # to a type that holds both as they are
+                both = torch.promote_types(drafted.dtype, logits.dtype)
+                logits, drafted = logits.to(both), drafted.to(both)
             r = verify_drafts(logits, tokens, u, e, draft=drafted, counts=own.cache.ints(n), temperature=temperature)
             new, lps, stand = r.tokens.tolist(), r.logprobs.tolist(), r.accepted.tolist()
             for b in range(B):
