@@ -78,7 +78,7 @@ class PagedKVCache:
     the current stream: use a cache on one stream at a time."""
 
     __slots__ = ("page_size", "kv", "table", "weights", "lens", "next_pos", "_state", "_pages_of", "_free", "_width",
-                 "_stale")
+                 "_stale", "_cut")
 
     def __init__(self, rows: int, num_heads: int, head_dim: int, num_layers: int, pages: int, page_size: int = 64,
                  max_positions: int | None = None, dtype: torch.dtype = torch.float32,
@@ -103,6 +103,9 @@ class PagedKVCache:
         self._pages_of: list[list[int]] = [[] for _ in range(rows)]
         self._free = list(range(pages - 1, -1, -1))
         self._stale = False  # whether the device's table is behind the host's
+        # how many of a row's first positions an eviction chose, each key head its own; behind them
+        # they follow one another
+        self._cut = [0] * rows
 
     def layer_pages(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor]:
         """A layer's (pages, page_size, H, D) views of the keys and values."""
@@ -166,14 +169,21 @@ class PagedKVCache:
         self._state.add_(self.ints(counts) if on_device is None else on_device)
 
     def truncate(self, lengths: list[int]) -> None:
-        """Row b goes back to its first lengths[b] cached positions."""
+        """Row b goes back to its first lengths[b] cached positions, and its next token to where it
+        then stands.  A row that was cut goes back no further than to the recent positions that
+        the eviction kept (before them each key head has kept others), or to nothing."""
         if len(lengths) != len(self.lens) or any(not 0 <= n <= a for n, a in zip(lengths, self.lens)):
             raise ValueError(f"PagedKVCache: rows of {self.lens} positions cannot go back to {lengths}")
         if list(lengths) == self.lens:
             return
+        for b, (n, a, cut) in enumerate(zip(lengths, self.lens, self._cut)):
+            if 0 < n < cut and n < a:
+                raise ValueError(f"PagedKVCache: row {b} was cut: it goes back to {cut} positions at least, or to none, not to {n}")
         for b, n in enumerate(lengths):
             self.next_pos[b] -= self.lens[b] - n
             self.lens[b] = n
+            if n == 0:
+                self.next_pos[b] = self._cut[b] = 0
             keep = -(-n // self.page_size)
             if len(self._pages_of[b]) > keep:
                 self._free += reversed(self._pages_of[b][keep:])
@@ -228,6 +238,7 @@ class PagedKVCache:
             for b, p in zip(some, to):
                 self._free += reversed(self._pages_of[b])
                 self._pages_of[b] = p
+                self._cut[b] = keep - min(recent, self.lens[b] - self._cut[b])
                 self.lens[b] = keep
             self._stale = True
             self._sync()
