@@ -67,3 +67,77 @@ def test_lengths_cut_where_they_are(dev):
     for b, n in enumerate(lens):
         n = min(n, keep)
         assert torch.equal(pool.k[to[b].long()].flatten(0, 1)[:n], moved[b].flatten(0, 1)[:n])
+
+
+def _attend(dev, dtype, B, N, H, Hkv, D, S, weights, v_wider=0):
+    """Ragged rows, without weights, so that the last kernel is the attention's, and with them."""
+    from diff_gpt import _native
+    from diff_gpt.model.paged import attention_paged
+
+    lens = [(37 * b) % 150 for b in range(B)]
+    counts = [0 if b % 13 == 5 else N - b % 3 for b in range(B)]
+    pool = Pool(dev, dtype, lens, counts, Hkv, D, S, seed=D + S)
+    q = _queries(dev, dtype, B, N, H, D, 1)
+    for b, n in enumerate(counts):
+        q[b, n:] = float("nan")
+    if v_wider:
+        wide = torch.full((*pool.v.shape[:3], D + v_wider), float("nan"), dtype=pool.v.dtype, device=dev)
+        wide[..., :D] = pool.v
+        pool.v = wide[..., :D]
+    ref, a, ref_w, most = attend_rows(torch.nan_to_num(q), pool)
+    w = torch.zeros(B, Hkv, pool.table.size(1) * S, device=dev) if weights else None
+    y = attention_paged(q, pool.k, pool.v, pool.table, pool.lengths, counts=pool.new, weights=w)
+    if not weights:
+        kernel = _native.last_kernel()
+    for b, n in enumerate(counts):
+        assert not y[b, n:].any()
+        if n:
+            close(y[b, :n], ref[b, :n], a[b, :n], dtype, lens[b] + n, 6.0)
+    if not weights:
+        return kernel
+    # a score's D products, the row's sum and the sums over tokens, in half steps of fp32
+    rel = 2 * (D + 8) * 2.0**-24 * most + 40 * 2.0**-24
+    for b, n in enumerate(counts):
+        t = lens[b] + n if n else 0
+        assert bool(((w[b, :, :t].double() - ref_w[b][:, :t]).abs() <= rel * ref_w[b][:, :t] + 2.0**-23 * ref_w[b][:, :t]).all())
+        assert not w[b, :, t:].any()
+
+
+@pytest.mark.parametrize("dtype,D,S", [("bf16", 16, 8), ("f16", 16, 16), ("bf16", 32, 8), ("f16", 24, 4), ("bf16", 64, 4),
+                                       ("f16", 128, 4), ("bf16", 80, 1), ("f32", 16, 8), ("f32", 32, 4), ("f32", 64, 2),
+                                       ("f32", 128, 4)])
+@pytest.mark.parametrize("B,rows", [(40, 64), (60, 128)])
+def test_wide_workgroups_over_pages_smaller_than_a_copy(dev, dtype, D, S, B, rows):
+    """An address for every lane, in workgroups of 64 and 128 rows."""
+    if D > 64 and rows == 64:
+        B = 24
+    assert _attend(dev, dtype, B, 130, 16, 4, D, S, False) == f"seq_mfma_paged_any_{rows}"
+    _attend(dev, dtype, B, 130, 16, 4, D, S, True)
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 16), ("bf16", 64), ("f16", 128), ("f32", 32), ("f32", 64)])
+@pytest.mark.parametrize("B,N,rows", [(3, 2, 32), (24, 130, 64), (60, 130, 128)])
+def test_keys_and_values_of_different_strides(dev, dtype, D, B, N, rows):
+    """Values as columns of a wider buffer, in whole 16-byte pieces."""
+    if D <= 64 and rows == 64:
+        B = 40
+    kernel = _attend(dev, dtype, B, N, 16, 4, D, 64, False, v_wider=16)
+    assert kernel == f"seq_mfma_paged_any_{rows}"
+    _attend(dev, dtype, B, N, 16, 4, D, 64, True, v_wider=16)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("B,N,most", [(1, 1, 20000), (30, 1, 2500), (6, 40, 1500)])
+def test_calls_repeat_themselves(dev, dtype, B, N, most):
+    """The same call has the same bits, outputs and weights, as often as it is made."""
+    from diff_gpt.model.paged import attention_paged
+
+    pool = Pool(dev, dtype, [most - (most // 40) * b for b in range(B)], [N] * B, 2, 64, 16)
+    q = _queries(dev, dtype, B, N, 8, 64, 3)
+    first = None
+    for _ in range(5):
+        w = torch.zeros(B, 2, pool.table.size(1) * 16, device=dev)
+        y = attention_paged(q, pool.k, pool.v, pool.table, pool.lengths, weights=w)
+        alone = attention_paged(q, pool.k, pool.v, pool.table, pool.lengths)
+        first = (y, w, alone) if first is None else first
+        assert torch.equal(y, first[0]) and torch.equal(w, first[1]) and torch.equal(alone, first[2])
