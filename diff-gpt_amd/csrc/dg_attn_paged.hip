@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void paged_weights_any_kernel(const SeqArgs a,
 // ones.  Ranks by counting, at most kOrdered rows.  us as they come / so, with this launch:
 // 16 rows of 256 - 512 tokens behind 1000 - 7168, 16 heads on 4 of 128, 425 / 372; 48 of up to
 // 300 behind up to 3000, 8 on 2 of 64, 86 / 67; a token behind each of 48 of 100 - 4096, 16 on 4
-// of 128, 46.7 / 41.3, of 256 223 / 222; 16 alike 417 / 420.
+// of 128, in two splits, 46.7 / 41.3, of 256 223 / 222; 16 alike 417 / 420.
 constexpr int kOrdered = 1024;
 
 __global__ __launch_bounds__(kOrdered) void paged_order_kernel(const SeqArgs a, int32_t* order) {
@@ -286,7 +286,7 @@ int64_t stage_ns(int D, int dtype, int rows_per_wg) {
 //   8 x 200, 4000, 8 / 8 of 64, 32              36.3 / 43 / 51 / 51
 //   6 x 237, 5580, 2 / 2 of 16, 32              21.7 / 18 / 16 / 19
 //   5 x 25, 13386, fp32, 24 / 6 of 80, 64       909 / 464 / 246 / 198
-int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t chunk, int64_t fill, int D, int64_t ns, bool few) {
+int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t chunk, int64_t fill, int D, int64_t ns, bool few, bool scored) {
   const int64_t whole = longest * ns / 128;
   auto percent = [&](int64_t n) { return n <= fill ? 100 : 100 * n / fill + 25; };
   int best = 1;
@@ -299,10 +299,20 @@ int best_splits(int64_t wg, int64_t rows, int64_t longest, int64_t chunk, int64_
       best = k;
     }
   }
-  // rows of the batch are rarely all as long as the longest: where they have one tile of rows a
-  // key head (few) and do not fill the chip, many keys are split all the same, the longest first (48 x 1 token behind 100 -
-  // 4096, 16 / 4 of 128: 70 us unsplit, 62.7 in two)
-  if (few && wg < fill && longest >= 2048) best = std::max(best, (int)std::min<int64_t>(2 * wg > fill ? 2 : fill / wg, most));
+  // One tile of rows a key head (few) and long rows (2048 positions on, whatever their type and dims):
+  // as many splits as run at once, which the model, whose join is a busy chip's, finds too dear where
+  // positions are cheap.  us as above / so, rows alike within two: 1 token behind 2100, 4 / 4 of 16 11.4 / 8.3, of 32
+  // 13.4 / 8.7; 8 of them 12.1 / 10.0, 13.5 / 11.0; of 64 and 128 dims, and behind 4100, the same
+  if (few && longest >= 2048 && 2 * wg <= fill) best = std::max(best, (int)std::min<int64_t>(fill / wg, most));
+  // Rows are rarely all as long as the longest, so that two splits pay before they run at once, but
+  // only where a launch behind the attention is there anyway, that of the weights from scores
+  // (scored).  us as above / in two, a token a row behind, with weights:
+  //   48 of 100 - 4096, 16 / 4 of 128 77 / 68, of 2000 - 4096 88 / 85; 40 of 100 - 2048, 12 / 4 41.7 / 37.2;
+  //   100 of 50 - 2500, 8 / 2 of 64 35.3 / 32.5; 200 of 100 - 3001, 4 / 2 57.2 / 56.4; rows alike lose,
+  //   48 of 4000, 16 / 4 of 128 100 / 106, and shorter ones, 48 of 100 - 1500 36.8 / 39.1
+  // the same without weights:
+  //   61 / 58, 68 / 73; 34.5 / 34.3; 25.5 / 25.5; 43.4 / 47.8; 78 / 91
+  if (scored && longest >= 2048 && wg < fill && 2 * wg > fill) best = std::max<int>(best, std::min<int64_t>(2, most));
   return best;
 }
 
@@ -326,7 +336,9 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
   // 256 / 128, fp32: 7 x 5 tokens behind 1200 - 2500, 6 heads on 3 of 128, 39.6 / 32.0; 1 x 30,
   // 8000, 4 on 4 of 128 39.8 / 30.8; 3 x 8, 700, 4 on 4 of 64 17.2 / 15.0
   t.chunk = kernel == kMfmaKernel && dtype == DG_F32 && Dm >= 64 ? 128 : 256;
-  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, t.chunk, fill, Dm, ns, R <= 32)
+  const int64_t ld = (cap + 255) / 256 * 256;
+  const bool scored = weights && mfma && rows_per_wg == 32 && R <= kScoreRows && B * Hkv * R * ld * 4 <= kScoreBytes;
+  t.nsplit = mfma ? best_splits(wg, B * Hkv * R, longest, t.chunk, fill, Dm, ns, R <= 32, scored)
                   : (int)std::max<int64_t>(1, std::min<int64_t>({(fill + wg - 1) / wg, longest / 256, kMaxSplits}));
   // every XCD has work: the row blocks of few (b, key head, split) go to several, in groups
   const int64_t units = B * Hkv * t.nsplit;
@@ -345,8 +357,7 @@ PagedShape paged_shape(int64_t B, int N, int H, int Hkv, int D, int dtype, int64
   t.lse_at = t.ws_bytes;
   if (weights) t.ws_bytes += ((size_t)(B * Hkv * R) * acc + 15) & ~(size_t)15;
   t.scores_at = t.ws_bytes;
-  const int64_t ld = (cap + 255) / 256 * 256;
-  if (weights && mfma && rows_per_wg == 32 && R <= kScoreRows && B * Hkv * R * ld * 4 <= kScoreBytes) {
+  if (scored) {
     t.scores_ld = ld;
     t.ws_bytes += (size_t)(B * Hkv * R * ld * 4);
   }

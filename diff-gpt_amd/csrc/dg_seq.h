@@ -108,7 +108,7 @@ __device__ __forceinline__ int paged_chunk(const SeqArgs& a, const PagedRow& r) 
 // The nth row of the batch by how many positions its tokens see, in whole 64s, the most first,
 // and its lengths: a lane has a row, whose rank every wave counts for itself (0.3 us of each
 // workgroup; a launch that ranks is 4 us of the call: 48 x 1 token behind 100 - 4096, 16 heads
-// on 4 of 128, 41.9 / 39.5, 64 of 8 on 8 115.8 / 113.9).
+// on 4 of 128, with weights, 62.6 / 59.6, 64 of 8 on 8 without 115.8 / 113.9).
 constexpr int kRankedRows = 64;
 __device__ __forceinline__ int paged_nth(const SeqArgs& a, int nth, PagedRow& r) {
   const int lane = threadIdx.x & 63, b = min(lane, a.B - 1);
