@@ -21,6 +21,7 @@
 // 14 us, a chain of latencies: the rows' statistics, the logits, two atomics.  (26 each with
 // loads of single elements where rows start anywhere, the exponents' offset raised with every
 // new maximum and the parts of a row's statistics joined by one thread.)
+// The same of fp64 logits, 282 MB, both launches 94 us (fp32 39; at temperature 0 58 and 23).
 #include "dg_common.h"
 
 #include <algorithm>
